@@ -45,6 +45,17 @@ class GemvJobC(ctypes.Structure):
 
 JP = ctypes.POINTER(GemvJobC)
 
+
+class Kv4C(ctypes.Structure):
+    """struct fitq_kv4"""
+    _fields_ = [
+        ("pool", P), ("page_table", P), ("prefix", P), ("q_start", P), ("tokens", I64), ("num_pages", I64),
+        ("batch", I32), ("kv_heads", I32), ("head_dim", I32), ("page_size", I32), ("max_pages", I32),
+    ]
+
+
+KP = ctypes.POINTER(Kv4C)
+
 SIGNATURES = {
     "fitq_version": (ctypes.c_char_p, []),
     "fitq_last_error": (ctypes.c_char_p, []),
@@ -88,6 +99,12 @@ SIGNATURES = {
     "fitq_verify_attention": (I32, [P, P, P, P, I64, I32, I32, I32, I32, I32, I32, P, SZ, P]),
     "fitq_attention_fwd": (I32, [P, P, P, P, P, I64, I64, I32, I32, I32, P]),
     "fitq_attention_bwd_workspace": (SZ, [I64, I64, I32]),
+    "fitq_kv4_append": (I32, [KP, P, I64, P, I64, P, I64, P, P, P, I32, I32, I32, P]),
+    "fitq_kv4_gather": (I32, [KP, P, P, I32, P]),
+    "fitq_kv4_attention_workspace": (SZ, [KP, I32, I64, I64]),
+    "fitq_kv4_attention": (I32, [KP, P, I64, P, I32, I32, I64, I64, P, SZ, P]),
+    "fitq_token_logprobs": (I32, [P, I32, P, I64, I64, I64, I32, P, P, P, P, P, P]),
+    "fitq_token_logprobs_bwd": (I32, [P, I32, P, I64, I64, I64, I32, P, P, P, P, P, P, P, P]),
     "fitq_attention_bwd": (I32, [P, P, P, P, P, P, P, P, P, I64, I64, I32, I32, I32, P, SZ, P]),
 }
 

@@ -11,6 +11,7 @@
 
 #include "common.cuh"
 #include "kernels.cuh"
+#include "kv4.cuh"
 
 // Device status word shared by all kernels of the library (first error wins).
 __device__ int g_fitq_status = 0;
@@ -1335,6 +1336,175 @@ int fitq_swiglu_bwd(const void* d_act, const void* gate, const void* up, void* d
   return launch_status(fitq::launch_swiglu_bwd(d_act, gate, up, d_gate, d_up, n,
                                                static_cast<cudaStream_t>(stream), sms),
                        "swiglu_bwd");
+}
+
+// Shape checks shared by the 4-bit cache calls; fills the kernels' addressing.
+static int kv4_view(const char* what, const fitq_kv4* c, int heads, fitq::Kv4Seq* out) {
+  if (!c || !c->pool || !c->page_table || !c->prefix) return fail(FITQ_ERR_ARG, "%s: NULL cache, pool, page_table or prefix", what);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(FITQ_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128 (got %d)", what, c->head_dim);
+  int shift = 0;
+  while (shift < 11 && (1 << shift) < c->page_size) ++shift;
+  if (c->page_size < 16 || c->page_size > 1024 || (1 << shift) != c->page_size)
+    return fail(FITQ_ERR_UNSUPPORTED, "%s: page_size must be a power of two in 16..1024 (got %d)", what, c->page_size);
+  if (c->batch <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535 || heads <= 0 || heads > 65535 || heads % c->kv_heads != 0 ||
+      c->max_pages <= 0 || c->num_pages <= 0 || c->num_pages >= (1ll << 31) || c->tokens < 0 ||
+      c->tokens >= (1ll << 31) || static_cast<int64_t>(c->batch) * c->kv_heads >= (1ll << 28))
+    return fail(FITQ_ERR_SHAPE, "%s: bad shape (tokens=%lld batch=%d heads=%d kv_heads=%d pages=%lld max_pages=%d)", what,
+                (long long)c->tokens, c->batch, heads, c->kv_heads, (long long)c->num_pages, c->max_pages);
+  if (static_cast<int64_t>(c->max_pages) * c->page_size >= (1ll << 31))
+    return fail(FITQ_ERR_SHAPE, "%s: max_pages * page_size must stay below 2^31", what);
+  if (!c->q_start && c->tokens % c->batch != 0)
+    return fail(FITQ_ERR_SHAPE, "%s: tokens=%lld do not divide over batch=%d (pass q_start)", what, (long long)c->tokens,
+                c->batch);
+  if (!al16(c->pool)) return fail(FITQ_ERR_ALIGN, "%s: pool not 16-byte aligned", what);
+  if ((reinterpret_cast<uintptr_t>(c->page_table) | reinterpret_cast<uintptr_t>(c->prefix) |
+       reinterpret_cast<uintptr_t>(c->q_start)) & 3u)
+    return fail(FITQ_ERR_ALIGN, "%s: page_table, prefix and q_start must be 4-byte aligned", what);
+  out->page_table = c->page_table;
+  out->prefix = c->prefix;
+  out->q_start = c->q_start;
+  out->tokens = c->tokens;
+  out->batch = c->batch;
+  out->t_new = c->q_start ? 0 : static_cast<int>(c->tokens / c->batch);
+  out->max_pages = c->max_pages;
+  out->page_shift = shift;
+  out->num_pages = c->num_pages;
+  out->kv_heads = c->kv_heads;
+  return FITQ_OK;
+}
+
+static bool kv4_dtype(int dtype) { return dtype == FITQ_DTYPE_BF16 || dtype == FITQ_DTYPE_F16; }
+
+int fitq_kv4_append(const fitq_kv4* cache, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                    const void* v, int64_t v_stride, void* q_out, const float* cos_half, const float* sin_half,
+                    int rope_len, int heads, int dtype, fitq_stream_t stream) {
+  fitq::Kv4Seq seq;
+  int rc = kv4_view("kv4_append", cache, heads, &seq);
+  if (rc) return rc;
+  if (cache->tokens == 0) return FITQ_OK;
+  if (!q || !k || !v || !q_out || !cos_half || !sin_half) return fail(FITQ_ERR_ARG, "kv4_append: NULL tensor");
+  if (!kv4_dtype(dtype)) return fail(FITQ_ERR_UNSUPPORTED, "kv4_append: dtype must be bf16 or fp16 (got %d)", dtype);
+  if (rope_len <= 0) return fail(FITQ_ERR_SHAPE, "kv4_append: empty rotary tables");
+  const int64_t row = static_cast<int64_t>(heads) * cache->head_dim;
+  const int64_t kv_row = static_cast<int64_t>(cache->kv_heads) * cache->head_dim;
+  if (q_stride < row || k_stride < kv_row || v_stride < kv_row || q_stride % 8 || k_stride % 8 || v_stride % 8)
+    return fail(FITQ_ERR_SHAPE, "kv4_append: token strides must cover a token and be multiples of 8");
+  if (q_out == q && q_stride != row) return fail(FITQ_ERR_ARG, "kv4_append: q_out is q, but q is strided");
+  if (!al16(q) || !al16(k) || !al16(v) || !al16(q_out) || !al16(cos_half) || !al16(sin_half))
+    return fail(FITQ_ERR_ALIGN, "kv4_append: 16-byte alignment");
+  const int sms = current_sms(&rc);
+  if (!sms) return rc;
+  return launch_status(fitq::launch_kv4_append(seq, q, q_stride, k, k_stride, v, v_stride, q_out, cache->pool, cos_half,
+                                               sin_half, rope_len, heads, cache->head_dim, dtype, status_ptr(),
+                                               static_cast<cudaStream_t>(stream), sms),
+                       "kv4_append");
+}
+
+int fitq_kv4_gather(const fitq_kv4* cache, void* k, void* v, int dtype, fitq_stream_t stream) {
+  fitq::Kv4Seq seq;
+  int rc = kv4_view("kv4_gather", cache, cache ? cache->kv_heads : 1, &seq);
+  if (rc) return rc;
+  if (cache->tokens == 0) return FITQ_OK;
+  if (!k || !v) return fail(FITQ_ERR_ARG, "kv4_gather: NULL tensor");
+  if (!kv4_dtype(dtype)) return fail(FITQ_ERR_UNSUPPORTED, "kv4_gather: dtype must be bf16 or fp16 (got %d)", dtype);
+  if (!al16(k) || !al16(v)) return fail(FITQ_ERR_ALIGN, "kv4_gather: 16-byte alignment");
+  const int sms = current_sms(&rc);
+  if (!sms) return rc;
+  return launch_status(fitq::launch_kv4_gather(seq, cache->pool, k, v, cache->head_dim, dtype, status_ptr(),
+                                               static_cast<cudaStream_t>(stream), sms),
+                       "kv4_gather");
+}
+
+size_t fitq_kv4_attention_workspace(const fitq_kv4* cache, int heads, int64_t max_new, int64_t max_len) {
+  if (!cache || cache->batch <= 0 || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads != 0 || max_new <= 0 ||
+      max_len <= 0)
+    return 0;
+  return fitq::kv4_attention_workspace(cache->batch, cache->kv_heads, heads / cache->kv_heads, max_new, max_len,
+                                       cache->head_dim, sms_for_sizing());
+}
+
+int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_stride, void* out, int heads, int dtype,
+                       int64_t max_new, int64_t max_len, void* workspace, size_t workspace_bytes,
+                       fitq_stream_t stream) {
+  fitq::Kv4Seq seq;
+  int rc = kv4_view("kv4_attention", cache, heads, &seq);
+  if (rc) return rc;
+  if (cache->tokens == 0) return FITQ_OK;
+  if (!q || !out || !workspace) return fail(FITQ_ERR_ARG, "kv4_attention: NULL tensor or workspace");
+  if (!kv4_dtype(dtype)) return fail(FITQ_ERR_UNSUPPORTED, "kv4_attention: dtype must be bf16 or fp16 (got %d)", dtype);
+  const int group = heads / cache->kv_heads;
+  if (max_new <= 0 || max_new > cache->tokens || max_len <= 0 || max_len >= (1ll << 31) ||
+      group * max_new > 32ll * 65535)
+    return fail(FITQ_ERR_SHAPE, "kv4_attention: bad max_new=%lld or max_len=%lld (tokens=%lld, heads / kv_heads=%d)",
+                (long long)max_new, (long long)max_len, (long long)cache->tokens, group);
+  if (!cache->q_start && max_new < seq.t_new)
+    return fail(FITQ_ERR_SHAPE, "kv4_attention: max_new=%lld, but every sequence has %d new tokens", (long long)max_new,
+                seq.t_new);
+  if (q_stride < static_cast<int64_t>(heads) * cache->head_dim || q_stride % 8)
+    return fail(FITQ_ERR_SHAPE, "kv4_attention: the token stride must cover a token and be a multiple of 8");
+  if (!al16(q) || !al16(out) || !al16(workspace)) return fail(FITQ_ERR_ALIGN, "kv4_attention: 16-byte alignment");
+  const int sms = current_sms(&rc);
+  if (!sms) return rc;
+  const size_t need = fitq::kv4_attention_workspace(cache->batch, cache->kv_heads, group, max_new, max_len,
+                                                    cache->head_dim, sms);
+  if (workspace_bytes < need)
+    return fail(FITQ_ERR_WORKSPACE, "kv4_attention: workspace %zu < %zu bytes", workspace_bytes, need);
+  return launch_status(fitq::launch_kv4_attention(seq, q, q_stride, cache->pool, out, heads, cache->head_dim, dtype,
+                                                  max_new, max_len, workspace, status_ptr(),
+                                                  static_cast<cudaStream_t>(stream), sms),
+                       "kv4_attention");
+}
+
+// Checks shared by the log-probability forward and backward.
+static int logprob_shape(const char* what, const void* logits, int dtype, const int64_t* ids, int64_t rows, int64_t vocab,
+                         int64_t stride, int top) {
+  if (!logits || !ids) return fail(FITQ_ERR_ARG, "%s: NULL tensor", what);
+  if (dtype != FITQ_DTYPE_BF16 && dtype != FITQ_DTYPE_F16 && dtype != FITQ_DTYPE_F32)
+    return fail(FITQ_ERR_UNSUPPORTED, "%s: unknown dtype %d", what, dtype);
+  if (rows >= (1ll << 24) || vocab <= 0 || vocab >= (1ll << 24) || stride < vocab)
+    return fail(FITQ_ERR_SHAPE, "%s: bad shape (rows=%lld vocab=%lld stride=%lld)", what, (long long)rows,
+                (long long)vocab, (long long)stride);
+  if (top < 0 || top > 64 || top > vocab)
+    return fail(FITQ_ERR_UNSUPPORTED, "%s: top must be in 0..64 and at most vocab (got %d)", what, top);
+  const uintptr_t size = dtype == FITQ_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % size || (reinterpret_cast<uintptr_t>(ids) & 7u))
+    return fail(FITQ_ERR_ALIGN, "%s: logits and ids must be aligned to their elements", what);
+  return FITQ_OK;
+}
+
+int fitq_token_logprobs(const void* logits, int dtype, const int64_t* ids, int64_t rows, int64_t vocab, int64_t stride,
+                        int top, float* logp, float* entropy, float* stats, float* top_logp, int64_t* top_ids,
+                        fitq_stream_t stream) {
+  if (rows == 0) return FITQ_OK;
+  if (rows < 0) return fail(FITQ_ERR_SHAPE, "token_logprobs: rows=%lld", (long long)rows);
+  int rc = logprob_shape("token_logprobs", logits, dtype, ids, rows, vocab, stride, top);
+  if (rc) return rc;
+  if (!logp || !entropy || !stats || (top > 0 && (!top_logp || !top_ids)))
+    return fail(FITQ_ERR_ARG, "token_logprobs: NULL output");
+  const int sms = current_sms(&rc);
+  if (!sms) return rc;
+  return launch_status(fitq::launch_token_logprobs(logits, dtype, ids, rows, vocab, stride, top, logp, entropy, stats,
+                                                   top_logp, top_ids, static_cast<cudaStream_t>(stream), sms),
+                       "token_logprobs");
+}
+
+int fitq_token_logprobs_bwd(const void* logits, int dtype, const int64_t* ids, int64_t rows, int64_t vocab,
+                            int64_t stride, int top, const float* stats, const float* entropy, const int64_t* top_ids,
+                            const float* g_logp, const float* g_entropy, const float* g_top, void* d,
+                            fitq_stream_t stream) {
+  if (rows == 0) return FITQ_OK;
+  if (rows < 0) return fail(FITQ_ERR_SHAPE, "token_logprobs_bwd: rows=%lld", (long long)rows);
+  int rc = logprob_shape("token_logprobs_bwd", logits, dtype, ids, rows, vocab, stride, top);
+  if (rc) return rc;
+  if (!stats || !entropy || !d || (g_top && !top_ids)) return fail(FITQ_ERR_ARG, "token_logprobs_bwd: NULL tensor");
+  if (d == logits && stride != vocab) return fail(FITQ_ERR_ARG, "token_logprobs_bwd: d must not overlap strided logits");
+  if (reinterpret_cast<uintptr_t>(d) & 15u) return fail(FITQ_ERR_ALIGN, "token_logprobs_bwd: d not 16-byte aligned");
+  if (!current_sms(&rc)) return rc;
+  return launch_status(fitq::launch_token_logprobs_bwd(logits, dtype, ids, rows, vocab, stride, top, stats, entropy,
+                                                       top_ids, g_logp, g_entropy, g_top, d,
+                                                       static_cast<cudaStream_t>(stream)),
+                       "token_logprobs_bwd");
 }
 
 }  // extern "C"

@@ -329,6 +329,34 @@ int launch_swiglu_fwd(const void* g, const void* u, void* act, int64_t n, cudaSt
 int launch_swiglu_bwd(const void* d, const void* g, const void* u, void* dg, void* du, int64_t n,
                       cudaStream_t st, int num_sms);
 
+// The 4-bit paged key/value cache (kv4.cu, kv4_attn.cu); shapes checked by the
+// caller.  Device-side lengths, pages and positions that lead outside the cache
+// are recorded in *status and skipped.
+struct Kv4Seq;
+int launch_kv4_append(const Kv4Seq& seq, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                      const void* v, int64_t v_stride, void* q_out, void* pool, const float* cs,
+                      const float* sn, int rope_len, int heads, int dim, int dtype, int* status,
+                      cudaStream_t st, int num_sms);
+int launch_kv4_gather(const Kv4Seq& seq, const void* pool, void* k, void* v, int dim, int dtype, int* status,
+                      cudaStream_t st, int num_sms);
+// max_new: most new tokens of a sequence; max_len: most positions of one, which
+// only sizes the grid.
+size_t kv4_attention_workspace(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim,
+                               int num_sms);
+int launch_kv4_attention(const Kv4Seq& seq, const void* q, int64_t q_stride, const void* pool, void* out, int heads,
+                         int dim, int dtype, int64_t max_new, int64_t max_len, void* workspace, int* status,
+                         cudaStream_t st, int num_sms);
+
+// Log probabilities of given tokens, entropy, top alternatives and their
+// gradient (logprob.cu).
+int launch_token_logprobs(const void* logits, int dtype, const int64_t* ids, int64_t rows, int64_t V, int64_t stride,
+                          int top, float* logp, float* entropy, float* stats, float* top_logp, int64_t* top_ids,
+                          cudaStream_t st, int num_sms);
+int launch_token_logprobs_bwd(const void* logits, int dtype, const int64_t* ids, int64_t rows, int64_t V,
+                              int64_t stride, int top, const float* stats, const float* entropy,
+                              const int64_t* top_ids, const float* g_logp, const float* g_entropy,
+                              const float* g_top, void* d, cudaStream_t st);
+
 // Optimizer kernels (optim.cu).
 int launch_adamw(float* p, const float* g, float* m, float* v, int64_t n, float lr, float b1,
                  float b2, float eps, float wd, int step, const float* clip, cudaStream_t st);

@@ -1,0 +1,549 @@
+// Log probabilities of given tokens with the row's entropy and top alternatives,
+// and the gradient.
+//
+// For a row z of V logits with M = max z, S = sum exp(z - M):
+//   logp = z[id] - M - log S,   H = log S - sum exp(z - M) (z - M) / S,
+// and the k largest logits in order, the lower index first where two are equal
+// (a NaN counts as the largest).  Upstream gradients a (logp), h (entropy) and
+// t_j (alternatives) give, with p_v = exp(z_v - M - log S),
+//   dz_v = [v = id] a + sum_j [v = top_j] t_j
+//          - p_v (a + sum_j t_j) - h p_v (z_v - M - log S + H).
+// M and log S are kept apart for the backward: their sum would lose the digits
+// that log S carries behind M.
+//
+// logprob_fwd_kernel: a cluster of CTAs shares a row; a thread holds its share
+// in registers (every load issued before the first use), so the row is read
+// once: one pass for the maximum, the sums and the candidates.  Alternatives: the
+// k-th largest of 128 thread-group maxima bounds the k-th largest logit of the
+// CTA's share from below; the few elements at or above it are collected and
+// ranked by (value, index), then the CTAs' lists are ranked together.  Where more
+// elements tie than the list holds, k rounds of a maximum search take over.
+// Bound: HBM (one read) for many rows, latency for few.
+//
+// logprob_bwd_kernel: one read and one write of the row; the up to k + 1 marked
+// elements are rewritten behind a CTA barrier.
+#include "kv4.cuh"
+#include "kernels.cuh"
+
+namespace fitq {
+namespace {
+
+constexpr int kLpThreads = 512;
+constexpr int kLpWarps = kLpThreads / 32;
+constexpr int kLpMaxTop = 64;
+constexpr int kLpGroups = 128;  // thread groups whose maxima bound the k-th largest
+constexpr int kLpList = 1024;   // candidates a CTA ranks
+
+__device__ __forceinline__ float exp_approx(float x) { return __expf(x); }
+
+// Floats in an order that unsigned comparison follows; equal floats get equal
+// values (-0 as 0), every NaN the largest.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key_of(float x, int64_t idx) {
+  return (static_cast<uint64_t>(order_of(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(idx));
+}
+
+template <typename T>
+struct Row {
+  static constexpr int kVec = 16 / sizeof(T);
+  const T* z;      // first element
+  int64_t lead;    // elements of the first 16-byte granule that lie before it
+  int64_t vectors; // granules that hold the row
+  int64_t V;
+  __device__ __forceinline__ Row(const T* base, int64_t v) : z(base), V(v) {
+    lead = (reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T);
+    vectors = (lead + v + kVec - 1) / kVec;
+  }
+  // index of element 0 of granule i (may be negative for i = 0)
+  __device__ __forceinline__ int64_t first(int64_t i) const { return i * kVec - lead; }
+  __device__ __forceinline__ bool inside(int64_t i) const { return first(i) >= 0 && first(i) + kVec <= V; }
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+// The elements of a granule as floats.
+template <typename T>
+__device__ __forceinline__ void unpack_vec(const uint4& u, float (&f)[16 / sizeof(T)]);
+template <>
+__device__ __forceinline__ void unpack_vec<__nv_bfloat16>(const uint4& u, float (&f)[8]) { unpack8<__nv_bfloat16>(u, f); }
+template <>
+__device__ __forceinline__ void unpack_vec<__half>(const uint4& u, float (&f)[8]) { unpack8<__half>(u, f); }
+template <>
+__device__ __forceinline__ void unpack_vec<float>(const uint4& u, float (&f)[4]) {
+  f[0] = __uint_as_float(u.x);
+  f[1] = __uint_as_float(u.y);
+  f[2] = __uint_as_float(u.z);
+  f[3] = __uint_as_float(u.w);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_vec(const float (&f)[16 / sizeof(T)]);
+template <>
+__device__ __forceinline__ uint4 pack_vec<__nv_bfloat16>(const float (&f)[8]) { return pack8<__nv_bfloat16>(f); }
+template <>
+__device__ __forceinline__ uint4 pack_vec<__half>(const float (&f)[8]) { return pack8<__half>(f); }
+template <>
+__device__ __forceinline__ uint4 pack_vec<float>(const float (&f)[4]) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+
+// Granule i of a row; elements outside the row read as -inf.
+template <typename T>
+__device__ __forceinline__ uint4 load_vec(const Row<T>& r, int64_t i) {
+  if (r.inside(i)) return *reinterpret_cast<const uint4*>(r.z + r.first(i));
+  float f[Row<T>::kVec];
+#pragma unroll
+  for (int j = 0; j < Row<T>::kVec; ++j) {
+    const int64_t e = r.first(i) + j;
+    f[j] = (e >= 0 && e < r.V) ? to_f32<T>(r.z[e]) : -INFINITY;
+  }
+  return pack_vec<T>(f);
+}
+
+struct LogprobFwdParams {
+  const void* logits;
+  const int64_t* ids;
+  int64_t V, stride;
+  int top;
+  float* logp;     // [rows]
+  float* entropy;  // [rows]
+  float* stats;    // [rows, 2]: M, log S
+  float* top_logp; // [rows, top]
+  int64_t* top_ids;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// (m, s, t) = max, sum exp(z - m), sum exp(z - m)(z - m) of two parts joined.
+__device__ __forceinline__ void join(float& m, float& s, float& t, float m2, float s2, float t2) {
+  const float mn = fmaxf(m, m2);
+  const float base = mn == -INFINITY ? 0.f : mn;
+  const float d1 = fmaxf(m - base, -1.0e30f), d2 = fmaxf(m2 - base, -1.0e30f);  // -inf parts weigh 0
+  const float k1 = exp_approx(d1), k2 = exp_approx(d2);
+  t = k1 * fmaf(d1, s, t) + k2 * fmaf(d2, s2, t2);
+  s = k1 * s + k2 * s2;
+  m = mn;
+}
+
+// kNV > 0: a thread's granules stay in registers; kNV = 0: they are read again.
+template <typename T, int kNV, bool kTop>
+__global__ void __launch_bounds__(kLpThreads) logprob_fwd_kernel(const LogprobFwdParams p) {
+  constexpr int kVec = Row<T>::kVec;
+  __shared__ float sh_m[kLpWarps], sh_s[kLpWarps], sh_t[kLpWarps];
+  __shared__ float sh_part[8][3];  // the cluster's parts, in its first CTA
+  __shared__ uint32_t sh_group[kTop ? kLpGroups : 1];
+  __shared__ uint32_t sh_bound;
+  __shared__ int sh_count;
+  __shared__ uint64_t sh_list[kTop ? kLpList : 1];
+  __shared__ uint64_t sh_best[kTop ? kLpMaxTop : 1];      // this CTA's top, in order
+  __shared__ uint64_t sh_all[kTop ? 8 * kLpMaxTop : 1];   // every CTA's, in the first CTA
+  __shared__ uint64_t sh_red[kLpWarps];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t cta = cluster_rank(), ctas = cluster_size();
+  const int64_t row = blockIdx.x / ctas;
+  cluster_arrive();  // waited for before the first store into another CTA's shared memory
+  pdl_launch_dependents();
+  pdl_wait();  // the logits come from the previous kernel
+  const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, p.V);
+  const int64_t share = (r.vectors + ctas - 1) / ctas;
+  const int64_t v_lo = share * cta, v_hi = v_lo + share < r.vectors ? v_lo + share : r.vectors;
+
+  uint4 held[kNV > 0 ? kNV : 1];
+  if (kNV > 0) {
+#pragma unroll
+    for (int i = 0; i < kNV; ++i) {
+      const int64_t v = v_lo + tid + static_cast<int64_t>(i) * kLpThreads;
+      if (v < v_hi) held[i] = load_vec(r, v);
+    }
+  }
+  // f(granule index, its elements as floats) over this thread's granules
+  auto each = [&](auto f) {
+    if (kNV > 0) {
+#pragma unroll
+      for (int i = 0; i < kNV; ++i) {
+        const int64_t v = v_lo + tid + static_cast<int64_t>(i) * kLpThreads;
+        if (v < v_hi) {
+          float x[kVec];
+          unpack_vec<T>(held[i], x);
+          f(v, x);
+        }
+      }
+    } else {
+      for (int64_t v = v_lo + tid; v < v_hi; v += kLpThreads) {
+        float x[kVec];
+        unpack_vec<T>(load_vec(r, v), x);
+        f(v, x);
+      }
+    }
+  };
+
+  // ---- maximum and sums of the thread's share
+  float m = -INFINITY, s = 0.f, t = 0.f;
+  if (kNV > 0) {
+    each([&](int64_t, const float (&x)[kVec]) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) m = fmaxf(m, x[j]);
+    });
+    const float base = m == -INFINITY ? 0.f : m;
+    each([&](int64_t, const float (&x)[kVec]) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const float d = x[j] - base, e = exp_approx(d);
+        s += e;
+        t = fmaf(e, fmaxf(d, -1.0e30f), t);  // a weight of 0 takes no -inf with it
+      }
+    });
+  } else {
+    each([&](int64_t, const float (&x)[kVec]) {
+      float mx = x[0];
+#pragma unroll
+      for (int j = 1; j < kVec; ++j) mx = fmaxf(mx, x[j]);
+      if (mx > m) {
+        join(m, s, t, mx, 0.f, 0.f);
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const float d = x[j] - base, e = exp_approx(d);
+        s += e;
+        t = fmaf(e, fmaxf(d, -1.0e30f), t);
+      }
+    });
+  }
+  const float thread_max = m;
+  {
+    float wm = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+    const float base = wm == -INFINITY ? 0.f : wm;
+    const float d = fmaxf(m - base, -1.0e30f), k = exp_approx(d);
+    t = k * fmaf(d, s, t);
+    s *= k;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if (lane == 0) {
+      sh_m[warp] = wm;
+      sh_s[warp] = s;
+      sh_t[warp] = t;
+    }
+  }
+  if (kTop) {
+    // the group of four threads' largest element; 0 stands for "no element"
+    uint32_t g = (v_lo + tid < v_hi) ? order_of(thread_max) : 0u;
+    g = max(g, __shfl_xor_sync(0xffffffffu, g, 1));
+    g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+    if ((tid & 3) == 0) sh_group[tid >> 2] = g;
+    if (tid == 0) sh_count = 0;
+    if (tid < kLpMaxTop) sh_best[tid] = 0;
+  }
+  __syncthreads();
+  cluster_wait();  // every CTA of the cluster runs
+  if (warp == 0) {
+    float cm = lane < kLpWarps ? sh_m[lane] : -INFINITY;
+    float cs = lane < kLpWarps ? sh_s[lane] : 0.f, ct = lane < kLpWarps ? sh_t[lane] : 0.f;
+#pragma unroll
+    for (int o = kLpWarps / 2; o > 0; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, cm, o), s2 = __shfl_xor_sync(0xffffffffu, cs, o),
+                  t2 = __shfl_xor_sync(0xffffffffu, ct, o);
+      join(cm, cs, ct, m2, s2, t2);
+    }
+    if (lane == 0) {
+      const uint32_t dst = map_rank(smem_u32(&sh_part[cta][0]), 0);
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(cm) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4), "f"(cs) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 8), "f"(ct) : "memory");
+    }
+  }
+  if (kTop) {
+    // ---- bound: the top-th largest group maximum (equal ones ranked by group)
+    if (tid < kLpGroups) {
+      const uint32_t g = sh_group[tid];
+      int rank = 0;
+      for (int i = 0; i < kLpGroups; ++i) {
+        const uint32_t o = sh_group[i];
+        rank += (o > g || (o == g && i < tid)) ? 1 : 0;
+      }
+      if (rank == p.top - 1) sh_bound = g;
+    }
+    __syncthreads();
+    const uint32_t bound = sh_bound;
+    each([&](int64_t v, const float (&x)[kVec]) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const int64_t e = r.first(v) + j;
+        if (order_of(x[j]) >= bound && e >= 0 && e < r.V) {
+          const int at = atomicAdd(&sh_count, 1);
+          if (at < kLpList) sh_list[at] = key_of(x[j], e);
+        }
+      }
+    });
+    __syncthreads();
+    const int count = sh_count;
+    if (count <= kLpList) {
+      // the list's order varies, the keys' ranks do not: every key is unique
+      for (int i = tid; i < count; i += kLpThreads) {
+        const uint64_t k = sh_list[i];
+        int rank = 0;
+        for (int j = 0; j < count && rank < p.top; ++j) rank += sh_list[j] > k ? 1 : 0;
+        if (rank < p.top) sh_best[rank] = k;
+      }
+      __syncthreads();
+    } else {
+      uint64_t last = ~0ull;
+      for (int n = 0; n < p.top; ++n) {
+        uint64_t best = 0;
+        each([&](int64_t v, const float (&x)[kVec]) {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) {
+            const int64_t e = r.first(v) + j;
+            if (e < 0 || e >= r.V) continue;
+            const uint64_t k = key_of(x[j], e);
+            if (k < last && k > best) best = k;
+          }
+        });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
+          if (k > best) best = k;
+        }
+        if (lane == 0) sh_red[warp] = best;
+        __syncthreads();
+        best = 0;
+        for (int w = 0; w < kLpWarps; ++w)
+          if (sh_red[w] > best) best = sh_red[w];
+        __syncthreads();
+        last = best;
+        if (tid == 0) sh_best[n] = best;
+        if (best == 0) break;  // uniform: fewer elements than asked for in this share
+      }
+      __syncthreads();
+    }
+    if (tid < p.top) {
+      const uint32_t dst = map_rank(smem_u32(&sh_all[cta * kLpMaxTop + tid]), 0);
+      asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(dst), "l"(sh_best[tid]) : "memory");
+    }
+  }
+  cluster_arrive();
+  cluster_wait();  // the parts have arrived; the other CTAs' shared memory is read by nobody
+  if (cta != 0) return;
+  float M = sh_part[0][0], S = sh_part[0][1], E = sh_part[0][2];
+  for (uint32_t c = 1; c < ctas; ++c) join(M, S, E, sh_part[c][0], sh_part[c][1], sh_part[c][2]);
+  const float log_s = logf(S);
+  if (tid == 0) {
+    const int64_t id = p.ids[row];
+    const bool valid = id >= 0 && id < p.V;
+    p.logp[row] = valid ? (to_f32<T>(r.z[id]) - M) - log_s : 0.f;
+    p.entropy[row] = log_s - E / S;
+    p.stats[2 * row] = M;
+    p.stats[2 * row + 1] = log_s;
+  }
+  if (kTop) {
+    const int n = static_cast<int>(ctas) * p.top;
+    for (int i = tid; i < n; i += kLpThreads) {
+      const uint64_t k = sh_all[(i / p.top) * kLpMaxTop + i % p.top];
+      if (k == 0) continue;  // no element
+      int rank = 0;
+      for (int j = 0; j < n && rank < p.top; ++j) rank += sh_all[(j / p.top) * kLpMaxTop + j % p.top] > k ? 1 : 0;
+      if (rank < p.top) {
+        const int64_t e = 0xffffffffu - static_cast<uint32_t>(k);
+        p.top_ids[row * p.top + rank] = e;
+        p.top_logp[row * p.top + rank] = (to_f32<T>(r.z[e]) - M) - log_s;
+      }
+    }
+  }
+}
+
+struct LogprobBwdParams {
+  const void* logits;
+  const int64_t* ids;
+  int64_t V, stride;
+  int top;
+  const float *stats, *entropy;
+  const int64_t* top_ids;
+  const float *g_logp, *g_entropy, *g_top;  // each may be null
+  void* d;  // [rows, V]
+};
+
+constexpr int kLbThreads = 256;
+constexpr int kLbVectors = 8;  // granules per thread
+
+template <typename T>
+__global__ void __launch_bounds__(kLbThreads) logprob_bwd_kernel(const LogprobBwdParams p, int parts) {
+  constexpr int kVec = Row<T>::kVec;
+  __shared__ int64_t sh_id[kLpMaxTop + 1];
+  __shared__ float sh_g[kLpMaxTop + 1];
+  const int tid = threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t row = blockIdx.x / parts;
+  const int part = static_cast<int>(blockIdx.x % parts);
+  T* drow = static_cast<T*>(p.d) + row * p.V;
+  const T* zrow = static_cast<const T*>(p.logits) + row * p.stride;
+  const Row<T> out(drow, p.V);  // granules follow the gradient's alignment
+  const bool aligned = ((reinterpret_cast<uintptr_t>(zrow) ^ reinterpret_cast<uintptr_t>(drow)) & 15u) == 0;
+  const float M = p.stats[2 * row], log_s = p.stats[2 * row + 1];
+  const float H = p.entropy[row];
+  const int64_t id = p.ids[row];
+  const int marks = (p.g_top ? p.top : 0) + 1;
+  if (tid < marks) {
+    const bool given = tid == 0;
+    sh_id[tid] = given ? id : p.top_ids[row * p.top + tid - 1];
+    sh_g[tid] = given ? ((p.g_logp && id >= 0 && id < p.V) ? p.g_logp[row] : 0.f) : p.g_top[row * p.top + tid - 1];
+  }
+  __syncthreads();
+  float a = 0.f;
+  for (int i = 0; i < marks; ++i) a += sh_g[i];
+  const float h = p.g_entropy ? p.g_entropy[row] : 0.f;
+  auto grad = [&](float z) {
+    const float lp = (z - M) - log_s;
+    const float pr = exp_approx(lp);
+    return -pr * (a + h * fmaxf(lp + H, -1.0e30f));  // a probability of 0 takes no -inf with it
+  };
+  const int64_t v0 = static_cast<int64_t>(part) * (kLbThreads * kLbVectors) + tid;
+  uint4 z[kLbVectors];
+#pragma unroll
+  for (int i = 0; i < kLbVectors; ++i) {
+    const int64_t v = v0 + i * kLbThreads;
+    if (aligned && v < out.vectors && out.inside(v)) z[i] = *reinterpret_cast<const uint4*>(zrow + out.first(v));
+  }
+#pragma unroll
+  for (int i = 0; i < kLbVectors; ++i) {
+    const int64_t v = v0 + i * kLbThreads;
+    if (v >= out.vectors) continue;
+    if (aligned && out.inside(v)) {
+      float x[kVec];
+      unpack_vec<T>(z[i], x);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) x[j] = grad(x[j]);
+      *reinterpret_cast<uint4*>(drow + out.first(v)) = pack_vec<T>(x);
+    } else {
+      for (int j = 0; j < kVec; ++j) {
+        const int64_t e = out.first(v) + j;
+        if (e >= 0 && e < p.V) drow[e] = from_f32<T>(grad(to_f32<T>(zrow[e])));
+      }
+    }
+  }
+  // ---- the marked elements of this part, every mark on the same element summed in order
+  const int64_t e_lo = static_cast<int64_t>(part) * (kLbThreads * kLbVectors) * kVec - out.lead;
+  const int64_t e_hi = e_lo + static_cast<int64_t>(kLbThreads) * kLbVectors * kVec;
+  __syncthreads();
+  if (tid < marks) {
+    const int64_t e = sh_id[tid];
+    if (e >= 0 && e < p.V && e >= e_lo && e < e_hi) {
+      float g = 0.f;
+      for (int i = 0; i < marks; ++i)
+        if (sh_id[i] == e) g += sh_g[i];
+      drow[e] = from_f32<T>(g + grad(to_f32<T>(zrow[e])));
+    }
+  }
+}
+
+template <typename T, int kNV>
+int fwd_t(const LogprobFwdParams& p, int64_t rows, int ctas, cudaStream_t st) {
+  auto* kernel = p.top > 0 ? logprob_fwd_kernel<T, kNV, true> : logprob_fwd_kernel<T, kNV, false>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
+  cfg.blockDim = dim3(kLpThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  note_launch();
+  if (e != cudaSuccess) return FITQ_ERR_CUDA;
+  return launch_result();
+}
+
+template <typename T>
+int fwd_sized(const LogprobFwdParams& p, int64_t rows, cudaStream_t st, int num_sms) {
+  const int64_t vectors = (p.V * static_cast<int64_t>(sizeof(T)) + 15) / 16 + 1;
+  // Few rows: up to eight CTAs of a row run on SMs of their own; many rows: as few
+  // CTAs as hold the row in registers.
+  int ctas = 1;
+  const int64_t want = rows * 4 < num_sms ? 2 : 8;  // granules per thread
+  while (ctas < 8 && vectors > want * kLpThreads * ctas) ctas *= 2;
+  const int64_t per = (vectors + ctas - 1) / ctas;
+  if (per <= 2 * kLpThreads) return fwd_t<T, 2>(p, rows, ctas, st);
+  if (per <= 5 * kLpThreads) return fwd_t<T, 5>(p, rows, ctas, st);
+  if (per <= 10 * kLpThreads) return fwd_t<T, 10>(p, rows, ctas, st);
+  return fwd_t<T, 0>(p, rows, ctas, st);
+}
+
+template <typename T>
+int bwd_t(const LogprobBwdParams& p, int64_t rows, cudaStream_t st) {
+  const int64_t vectors = (p.V * static_cast<int64_t>(sizeof(T)) + 15) / 16 + 1;
+  const int parts = static_cast<int>((vectors + kLbThreads * kLbVectors - 1) / (kLbThreads * kLbVectors));
+  const cudaError_t e = launch_pdl(logprob_bwd_kernel<T>, dim3(static_cast<unsigned>(rows * parts)), dim3(kLbThreads), 0,
+                                   st, p, parts);
+  note_launch();
+  if (e != cudaSuccess) return FITQ_ERR_CUDA;
+  return launch_result();
+}
+
+}  // namespace
+
+int launch_token_logprobs(const void* logits, int dtype, const int64_t* ids, int64_t rows, int64_t V, int64_t stride,
+                          int top, float* logp, float* entropy, float* stats, float* top_logp, int64_t* top_ids,
+                          cudaStream_t st, int num_sms) {
+  const LogprobFwdParams p{logits, ids, V, stride, top, logp, entropy, stats, top_logp, top_ids};
+  if (dtype == FITQ_DTYPE_F32) return fwd_sized<float>(p, rows, st, num_sms);
+  if (dtype == FITQ_DTYPE_F16) return fwd_sized<__half>(p, rows, st, num_sms);
+  return fwd_sized<__nv_bfloat16>(p, rows, st, num_sms);
+}
+
+int launch_token_logprobs_bwd(const void* logits, int dtype, const int64_t* ids, int64_t rows, int64_t V,
+                              int64_t stride, int top, const float* stats, const float* entropy,
+                              const int64_t* top_ids, const float* g_logp, const float* g_entropy,
+                              const float* g_top, void* d, cudaStream_t st) {
+  const LogprobBwdParams p{logits, ids, V, stride, top, stats, entropy, top_ids, g_logp, g_entropy, g_top, d};
+  if (dtype == FITQ_DTYPE_F32) return bwd_t<float>(p, rows, st);
+  if (dtype == FITQ_DTYPE_F16) return bwd_t<__half>(p, rows, st);
+  return bwd_t<__nv_bfloat16>(p, rows, st);
+}
+
+}  // namespace fitq

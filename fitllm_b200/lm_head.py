@@ -16,11 +16,97 @@ until the caller reads them.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Tuple
+from typing import List, NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
+
+
+_LOGIT_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16,
+                 torch.float32: _lib.DTYPE_F32}
+
+
+class TokenLogProbs(NamedTuple):
+    """logp and entropy fp32 [...], top_logp fp32 and top_ids int64 [..., top]."""
+    logp: torch.Tensor
+    entropy: torch.Tensor
+    top_logp: torch.Tensor
+    top_ids: torch.Tensor
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from row to row of [rows, V] (V where there is one row)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+class _TokenLogProbsFn(torch.autograd.Function):
+    """fitq_token_logprobs / fitq_token_logprobs_bwd over logits [rows, V]."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, top: int):
+        L = _lib.load()
+        dev = logits.device
+        rows, vocab = logits.shape
+        f32 = dict(dtype=torch.float32, device=dev)
+        logp, entropy = torch.empty(rows, **f32), torch.empty(rows, **f32)
+        stats, top_logp = torch.empty(rows, 2, **f32), torch.empty(rows, top, **f32)
+        top_ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check(L.fitq_token_logprobs(logits.data_ptr(), _LOGIT_DTYPES[logits.dtype], ids.data_ptr(), rows,
+                                             vocab, _row_stride(logits), top, logp.data_ptr(), entropy.data_ptr(),
+                                             stats.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr(),
+                                             ops._stream(dev)), "fitq_token_logprobs")
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(top_ids)
+        ctx.save_for_backward(logits, ids, stats, entropy, top_ids)
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        logits, ids, stats, entropy, top_ids = ctx.saved_tensors
+        L = _lib.load()
+        dev = logits.device
+        rows, vocab = logits.shape
+        top = top_ids.shape[1]
+        g_logp, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logp, g_entropy, g_top))
+        d = torch.empty(rows, vocab, dtype=logits.dtype, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check(L.fitq_token_logprobs_bwd(logits.data_ptr(), _LOGIT_DTYPES[logits.dtype], ids.data_ptr(),
+                                                 rows, vocab, _row_stride(logits), top, stats.data_ptr(),
+                                                 entropy.data_ptr(), top_ids.data_ptr(), _lib.ptr(g_logp),
+                                                 _lib.ptr(g_entropy), _lib.ptr(g_top if top else None),
+                                                 d.data_ptr(), ops._stream(dev)), "fitq_token_logprobs_bwd")
+        return d, None, None
+
+
+def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> TokenLogProbs:
+    """Log probabilities of given tokens, the rows' entropies and the `top` most
+    likely tokens, in one read of the logits; differentiable (logp, entropy and
+    top_logp) with one more read and one write.
+
+    logits [..., V] bf16, fp16 or fp32 (rows may be strided, as in
+    logits[..., :tokens]); ids [...] integers, an id outside [0, V) (-100 for
+    instance) has logp 0 and no gradient.  Equal logits rank by index."""
+    if logits.dim() < 1 or ids.shape != logits.shape[:-1]:
+        raise ValueError(f"token_logprobs: logits {tuple(logits.shape)} and ids {tuple(ids.shape)} do not match")
+    if logits.dtype not in _LOGIT_DTYPES or not logits.is_cuda:
+        raise ValueError("token_logprobs: logits must be a bf16, fp16 or fp32 CUDA tensor")
+    if ids.device != logits.device or ids.dtype.is_floating_point or ids.dtype == torch.bool:
+        raise ValueError("token_logprobs: ids must be integers on the logits' device")
+    vocab = logits.shape[-1]
+    if not 0 <= top <= min(64, vocab):
+        raise ValueError(f"token_logprobs: top must be in 0..64 and at most {vocab} (got {top})")
+    z = logits.reshape(-1, vocab) if logits.dim() != 2 else logits
+    if (vocab > 1 and z.stride(1) != 1) or (z.shape[0] > 1 and z.stride(0) < vocab):
+        z = z.contiguous()
+    lead = ids.shape
+    r = _TokenLogProbsFn.apply(z, ids.reshape(-1).to(torch.int64).contiguous(), int(top))
+    if len(lead) == 1:
+        return TokenLogProbs(*r)
+    return TokenLogProbs(r[0].view(lead), r[1].view(lead), r[2].view(*lead, top), r[3].view(*lead, top))
 
 
 class LMHeadLoss:

@@ -228,6 +228,136 @@ def verify_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
+_KV4_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+
+
+def _kv4_cache(what: str, pool: torch.Tensor, page_table: torch.Tensor, prefix: torch.Tensor,
+               q_start: Optional[torch.Tensor], tokens: int) -> _lib.Kv4C:
+    """The fitq_kv4 descriptor of a call (its pointers live as long as the tensors)."""
+    dev = pool.device
+    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or not pool.is_cuda:
+        raise ValueError(f"{what}: pool must be a contiguous uint8 CUDA tensor [pages, kv_heads, page_size / 16, "
+                         "18 * head_dim]")
+    if pool.shape[3] % 18:
+        raise ValueError(f"{what}: pool blocks have {pool.shape[3]} bytes, not 18 * head_dim")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+        raise ValueError(f"{what}: page_table must be contiguous int32 [batch, max_pages]")
+    batch = page_table.shape[0]
+    if prefix.dtype != torch.int32 or prefix.shape != (batch,) or not prefix.is_contiguous():
+        raise ValueError(f"{what}: prefix must be contiguous int32 [batch]")
+    if q_start is not None and (q_start.dtype != torch.int32 or q_start.shape != (batch + 1,)
+                                or not q_start.is_contiguous()):
+        raise ValueError(f"{what}: q_start must be contiguous int32 [batch + 1]")
+    for name, t in (("page_table", page_table), ("prefix", prefix), ("q_start", q_start)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: {name} is on {t.device}, the pool on {dev}")
+    return _lib.Kv4C(pool.data_ptr(), page_table.data_ptr(), prefix.data_ptr(), _lib.ptr(q_start), tokens,
+                     pool.shape[0], batch, pool.shape[1], pool.shape[3] // 18, pool.shape[2] * 16,
+                     page_table.shape[1])
+
+
+def _kv4_tokens(what: str, name: str, t: torch.Tensor, heads: Optional[int], dim: int, like: torch.Tensor,
+                dev) -> torch.Tensor:
+    """t as [tokens, heads, dim] whose heads and elements are dense (tokens may be strided)."""
+    if t.dim() != 3 or t.shape[2] != dim or t.shape[0] != like.shape[0] or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}")
+    if t.dtype not in _KV4_DTYPES or t.dtype != like.dtype:
+        raise ValueError(f"{what}: {name} must be bf16 or fp16, all of one dtype (got {t.dtype})")
+    if t.device != dev:
+        raise ValueError(f"{what}: {name} is on {t.device}, the pool on {dev}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or s1 != dim or s0 % 8 or s0 < t.shape[1] * dim or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _kv4_out(what: str, name: str, out: Optional[torch.Tensor], shape, dtype, dev) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if out.shape != torch.Size(shape) or out.dtype != dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor {tuple(shape)} on {dev}")
+    return out
+
+
+def kv4_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
+               prefix: torch.Tensor, cos_half: torch.Tensor, sin_half: torch.Tensor,
+               q_start: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotate the new tokens' q and k and append k and v to a 4-bit paged cache
+    (fitq_kv4_append).
+
+    q [tokens, heads, D], k, v [tokens, kv_heads, D] bf16 or fp16 (the token
+    stride is free); cos_half, sin_half fp32 [positions, D / 2], row = position.
+    Returns the rotated q (into q_out when given; rows of no sequence are left
+    as they are)."""
+    L = _lib.load()
+    dev = pool.device
+    c = _kv4_cache("kv4_append", pool, page_table, prefix, q_start, q.shape[0])
+    d, kvh = c.head_dim, c.kv_heads
+    q = _kv4_tokens("kv4_append", "q", q, None, d, q, dev)
+    k = _kv4_tokens("kv4_append", "k", k, kvh, d, q, dev)
+    v = _kv4_tokens("kv4_append", "v", v, kvh, d, q, dev)
+    for name, t in (("cos_half", cos_half), ("sin_half", sin_half)):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] * 2 != d or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"kv4_append: {name} must be contiguous fp32 [positions, {d // 2}] on {dev}")
+    if sin_half.shape != cos_half.shape:
+        raise ValueError("kv4_append: cos_half and sin_half differ in shape")
+    out = _kv4_out("kv4_append", "q_out", q_out, q.shape, q.dtype, dev)
+    with torch.cuda.device(dev):
+        _lib.check(L.fitq_kv4_append(c, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(),
+                                     v.stride(0), out.data_ptr(), cos_half.data_ptr(), sin_half.data_ptr(),
+                                     cos_half.shape[0], q.shape[1], _KV4_DTYPES[q.dtype], _stream(dev)),
+                   "fitq_kv4_append")
+    return out
+
+
+def kv4_gather(pool: torch.Tensor, page_table: torch.Tensor, prefix: torch.Tensor, tokens: int,
+               q_start: Optional[torch.Tensor] = None,
+               dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [tokens, kv_heads, D]: what a 4-bit paged cache holds at the positions
+    kv4_append writes for the same prefix, tokens and q_start (fitq_kv4_gather)."""
+    L = _lib.load()
+    dev = pool.device
+    c = _kv4_cache("kv4_gather", pool, page_table, prefix, q_start, int(tokens))
+    if dtype not in _KV4_DTYPES:
+        raise ValueError(f"kv4_gather: dtype must be bf16 or fp16 (got {dtype})")
+    k = torch.empty(int(tokens), c.kv_heads, c.head_dim, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    with torch.cuda.device(dev):
+        _lib.check(L.fitq_kv4_gather(c, k.data_ptr(), v.data_ptr(), _KV4_DTYPES[dtype], _stream(dev)),
+                   "fitq_kv4_gather")
+    return k, v
+
+
+def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor, prefix: torch.Tensor,
+                  max_len: Optional[int] = None, q_start: Optional[torch.Tensor] = None,
+                  max_new: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the new tokens over a 4-bit paged cache (fitq_kv4_attention).
+
+    q [tokens, heads, D] bf16 or fp16, rotated, its keys and values appended:
+    token i of a sequence sees positions <= prefix + i.  max_new: the most new
+    tokens of one sequence (needed with q_start); max_len: the most positions of
+    one sequence, a hint for the grid.  Returns [tokens, heads, D] (into out when
+    given; rows of no sequence are left as they are)."""
+    L = _lib.load()
+    dev = pool.device
+    c = _kv4_cache("kv4_attention", pool, page_table, prefix, q_start, q.shape[0])
+    q = _kv4_tokens("kv4_attention", "q", q, None, c.head_dim, q, dev)
+    if max_new is None:
+        if q_start is not None:
+            raise ValueError("kv4_attention: pass max_new with q_start")
+        max_new = max(1, q.shape[0] // c.batch)
+    if max_len is None:
+        max_len = c.max_pages * c.page_size
+    out = _kv4_out("kv4_attention", "out", out, q.shape, q.dtype, dev)
+    with torch.cuda.device(dev):
+        nbytes = L.fitq_kv4_attention_workspace(c, q.shape[1], max_new, max_len)
+        ws = _workspace(nbytes, dev)
+        _lib.check(L.fitq_kv4_attention(c, q.data_ptr(), q.stride(0), out.data_ptr(), q.shape[1],
+                                        _KV4_DTYPES[q.dtype], max_new, max_len, ws.data_ptr(), nbytes,
+                                        _stream(dev)), "fitq_kv4_attention")
+    return out
+
+
 def gemm_bf16_tn(a: torch.Tensor, b: torch.Tensor, c_add: Optional[torch.Tensor] = None) -> torch.Tensor:
     """c = a.b^T (+ c_add) on the tcgen05 tensor cores (bf16 in/out, fp32 accumulate)."""
     L = _lib.load()

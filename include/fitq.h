@@ -323,6 +323,98 @@ FITQ_API int fitq_attention_bwd(const void* q, const void* k, const void* v, con
                                 const void* d_o, const float* lse, void* dq, void* dk, void* dv,
                                 int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim,
                                 void* workspace, size_t workspace_bytes, fitq_stream_t stream);
+
+/* A key/value cache held in 4 bits, in pages, and the new tokens of a call.  No
+ * counterpart in the reference, which re-runs the whole context for every token
+ * it verifies (fitllm/inference.py:380-397).
+ *   pool:       uint8 [num_pages, kv_heads, page_size / 16, 18 * head_dim], 16-byte
+ *               aligned: one block per 16 positions of a KV head (layout below);
+ *   page_table: int32 [batch, max_pages], page of positions [i * page_size,
+ *               (i + 1) * page_size) of a sequence; entries behind a sequence's
+ *               last position are not read.  Sequences may share pages they only read;
+ *   prefix:     int32 [batch], positions a sequence has in the cache before the
+ *               call's new tokens;
+ *   q_start:    int32 [batch + 1], sequence b's new tokens are the packed tokens
+ *               [q_start[b], q_start[b + 1]); NULL: tokens / batch each.  Packed
+ *               tokens of no sequence are neither read nor written.
+ * The 64-element groups of a key or value are value = scale * code + low, code
+ * 0..15, scale and low fp16: low = fp16(min), scale = fp16((max - low) / 15),
+ * code = round((x - low) * (1 / scale)), each step rounded to fp32.  A group with
+ * a NaN, an infinity or a value outside fp16's range reads back as NaN.  Block
+ * bytes, with G = head_dim / 64 and eight elements per 4-byte word (element j in
+ * bits 4 j .. 4 j + 3):
+ *   keys   [16 positions][4 c][G g][2 w] words: elements 64 g + 16 c + 8 w + j;
+ *   values [2 h][8 e][4 q][2 o][G g] words: elements 64 g + 8 e + j of position
+ *          8 h + 2 q + o;
+ *   params [16 positions][key, value][G] pairs (scale, low).
+ * head_dim 64 or 128, page_size a power of two in 16..1024.
+ * What only the device sees is checked there: a token whose position lies outside
+ * the page table, whose page is not in 0..num_pages - 1, or whose prefix is
+ * negative records FITQ_ERR_ARG (fitq_get_device_status) and is not written; its
+ * query and what is read for it are zeros, and attention leaves such positions out. */
+typedef struct fitq_kv4 {
+  void* pool;
+  const int32_t* page_table;
+  const int32_t* prefix;
+  const int32_t* q_start;
+  int64_t tokens;
+  int64_t num_pages;
+  int batch;
+  int kv_heads;
+  int head_dim;
+  int page_size;
+  int max_pages;
+} fitq_kv4;
+
+/* Rotates the new tokens' q and k (rotate-half, fp32 half tables cos/sin
+ * [rope_len, head_dim / 2] indexed by the token's position; positions from
+ * rope_len on are refused like pages outside the pool), writes q to q_out
+ * [tokens, heads, head_dim] and codes k (from the fp32 rotation) and v into the
+ * pages.  q [tokens, heads, head_dim], k, v [tokens, kv_heads, head_dim] of
+ * dtype (FITQ_DTYPE_BF16 or _F16); *_stride: elements from token to token, a
+ * multiple of 8.  q_out may be q when q_stride == heads * head_dim. */
+FITQ_API int fitq_kv4_append(const fitq_kv4* cache, const void* q, int64_t q_stride, const void* k,
+                             int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
+                             const float* cos_half, const float* sin_half, int rope_len, int heads,
+                             int dtype, fitq_stream_t stream);
+/* The values that the new tokens' positions hold: k, v [tokens, kv_heads,
+ * head_dim] of dtype, scale * code + low in fp32 rounded once. */
+FITQ_API int fitq_kv4_gather(const fitq_kv4* cache, void* k, void* v, int dtype, fitq_stream_t stream);
+/* Attention of the new tokens over the cache, their own positions included
+ * (appended before): token i of a sequence sees positions <= prefix + i, query
+ * head h reads KV head h / (heads / kv_heads).  q, out [tokens, heads, head_dim]
+ * of dtype (q_stride as above); scale 1/sqrt(head_dim), fp32 softmax and sums.
+ * max_new: the most new tokens of one sequence (a sequence with more records
+ * FITQ_ERR_ARG, its tokens beyond are not written).  max_len: the most positions of
+ * one sequence, if known, else max_pages * page_size; it only sizes the grid.
+ * Deterministic.  A token that sees no position gives zeros. */
+FITQ_API size_t fitq_kv4_attention_workspace(const fitq_kv4* cache, int heads, int64_t max_new,
+                                             int64_t max_len);
+FITQ_API int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_stride, void* out,
+                                int heads, int dtype, int64_t max_new, int64_t max_len,
+                                void* workspace, size_t workspace_bytes, fitq_stream_t stream);
+
+/* Log probabilities of given tokens under rows of lm_head logits (the log-softmax
+ * value that the reference's loss takes the mean of, fitllm/backward.py:188-198,
+ * one per row), with the entropy of each row and its `top` most likely tokens.
+ * logits [rows, vocab] of dtype (bf16, fp16, fp32), `stride` elements from row to
+ * row; ids int64 [rows], an id outside [0, vocab) gives logp 0 and no gradient;
+ * 0 <= top <= 64, top <= vocab.  logp, entropy fp32 [rows]; stats fp32 [rows, 2]
+ * (row maximum and log of the sum behind it) for the backward; top_logp fp32,
+ * top_ids int64 [rows, top], largest logit first, the lower index where two are
+ * equal, a NaN before all.  -inf logits have probability 0; a row of nothing else
+ * gives NaN.  The backward writes d [rows, vocab] (dtype, contiguous) from the
+ * upstream gradients g_logp, g_entropy [rows], g_top [rows, top], each NULL for 0. */
+FITQ_API int fitq_token_logprobs(const void* logits, int dtype, const int64_t* ids, int64_t rows,
+                                 int64_t vocab, int64_t stride, int top, float* logp,
+                                 float* entropy, float* stats, float* top_logp, int64_t* top_ids,
+                                 fitq_stream_t stream);
+FITQ_API int fitq_token_logprobs_bwd(const void* logits, int dtype, const int64_t* ids, int64_t rows,
+                                     int64_t vocab, int64_t stride, int top, const float* stats,
+                                     const float* entropy, const int64_t* top_ids,
+                                     const float* g_logp, const float* g_entropy,
+                                     const float* g_top, void* d, fitq_stream_t stream);
+
 FITQ_API int fitq_swiglu_bwd(const void* d_act, const void* gate, const void* up, void* d_gate,
                              void* d_up, int64_t n, fitq_stream_t stream);
 
