@@ -1435,12 +1435,16 @@ int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_stride, v
   if (!kv4_dtype(dtype)) return fail(FITQ_ERR_UNSUPPORTED, "kv4_attention: dtype must be bf16 or fp16 (got %d)", dtype);
   const int group = heads / cache->kv_heads;
   if (max_new <= 0 || max_new > cache->tokens || max_len <= 0 || max_len >= (1ll << 31) ||
-      group * max_new > 32ll * 65535)
+      group * max_new > 16ll * 65535)
     return fail(FITQ_ERR_SHAPE, "kv4_attention: bad max_new=%lld or max_len=%lld (tokens=%lld, heads / kv_heads=%d)",
                 (long long)max_new, (long long)max_len, (long long)cache->tokens, group);
   if (!cache->q_start && max_new < seq.t_new)
     return fail(FITQ_ERR_SHAPE, "kv4_attention: max_new=%lld, but every sequence has %d new tokens", (long long)max_new,
                 seq.t_new);
+  // the kernels count the tiles of all (sequence, KV head) pairs in 31 bits
+  if (static_cast<int64_t>(cache->batch) * cache->kv_heads *
+          (static_cast<int64_t>(cache->max_pages) * cache->page_size / 64 + 4) >= (1ll << 31))
+    return fail(FITQ_ERR_SHAPE, "kv4_attention: batch * kv_heads * max_pages * page_size is too large");
   if (q_stride < static_cast<int64_t>(heads) * cache->head_dim || q_stride % 8)
     return fail(FITQ_ERR_SHAPE, "kv4_attention: the token stride must cover a token and be a multiple of 8");
   if (!al16(q) || !al16(out) || !al16(workspace)) return fail(FITQ_ERR_ALIGN, "kv4_attention: 16-byte alignment");

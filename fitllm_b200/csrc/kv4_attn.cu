@@ -8,11 +8,18 @@
 // token * G + head).  With s, l the scale and low of a group and c its codes,
 //   q . k = sum_g s_g (q_g . c_g) + l_g sum(q_g),
 //   o     = sum_g [sum_p (w_p s_pg) (c_pg - 8)] + sum_p w_p (l_pg + 8 s_pg),
-// so the tensor cores multiply the codes themselves and scales and lows are
-// applied in fp32 to scores and weights.  A code becomes a bf16 or fp16 operand
-// by OR-ing it into the mantissa of 128 (1024): bf16 keys keep that offset, it is
-// taken off with l (one fp32 term per score), values have it subtracted because
-// their sums run over the whole cache, where it would cancel badly.
+// so the tensor cores multiply the codes themselves; scales and lows are applied
+// in fp32 to scores and weights.  Both products run in fp16 whatever the type of
+// q.  One logic instruction puts two codes into the mantissas of two 1024s, as
+// 1024 + c (even elements of a word) or 1024 + 16 c (odd ones; q / 16 stands
+// against them), so a word of eight codes takes one shift.  For keys that is the
+// operand: the accumulator starts at minus what the offsets add up to (64
+// elements, off by some 2^-24 of 2^10 |q|: 1e-4 in a score at unit scale).
+// Values have the offset taken off by one half2 operation, because their sums run
+// over the whole cache, where it would cancel badly.  Queries are multiplied by a
+// power of two per column (their largest element goes to 2^12, which keeps the
+// eight bits of a bf16 value over 2^26 of range), the weights by one per warp, which
+// keeps w s in fp16's range and rounds it to 2^-12 where bf16 would to 2^-9.
 //
 // kv4_attn_kernel.  Both products have the cache as the 16-row operand of
 // mma.m16n8k16 (S^T = K.Q^T, O^T = V^T.P^T), the R columns as the n8 operand, so
@@ -20,27 +27,45 @@
 // layout (two 16-byte shared loads per 16 keys, two per 16 values), and P turns
 // from accumulator to operand with movmatrix.  Every warp streams its own blocks
 // (2,304 B at D = 128, one bulk copy each) through a private ring and keeps its
-// own running maximum, sum and output; the warps of a CTA meet once per segment.
+// own reference maximum, sum and output; the warps of a CTA meet once per segment.
+// The reference only moves when a score exceeds it by 2^8 in weight: a vote per
+// block instead of a reduction, the sums have the range to spare.
 //
-// Work split.  The 64-position tiles of all (sequence, KV head) pairs form one
-// list, cut into equal runs, one per CTA, whatever the sequences' lengths; a CTA
-// finds its first pair from the device-side lengths.  A pair that lies in one
-// run is written out; one cut between runs leaves partials that
+// Work split.  The tiles (one block per warp) of all (sequence, KV head) pairs
+// form one list, cut into equal runs, one per CTA, whatever the sequences'
+// lengths; a CTA finds its first pair from the device-side lengths.  A pair that
+// lies in one run is written out; one cut between runs leaves partials that
 // kv4_attn_combine_kernel joins in run order (deterministic).
 //
 // Bound: HBM, 18 D / 16 B per position and KV head.
+#include <type_traits>
+
 #include "kv4.cuh"
 #include "kernels.cuh"
 
 namespace fitq {
 namespace {
 
-constexpr int kAWarps = 4;
-constexpr int kAThreads = 32 * kAWarps;
-constexpr int kATile = kKv4Block * kAWarps;  // positions per tile: one block per warp
-constexpr int kAStages = 4;                  // blocks in flight per warp
+// Warps per CTA and CTAs per SM by column tiles.  Sixteen columns are the most a
+// warp takes: with 32 the output alone is 128 registers a thread and eight warps per
+// SM wait on their own latencies (a verify step of 8 x 5 tokens over 4,100 positions
+// took 42 us that way); more columns are further row tiles, whose reads hit L2.
+template <int NT>
+struct AttnShape {
+  static constexpr int kWarps = NT == 1 ? 8 : 4;
+  static constexpr int kCtas = NT == 1 ? 2 : 3;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kTile = kKv4Block * kWarps;  // positions per tile
+  static constexpr int kStages = NT == 1 ? 4 : 3;   // blocks in flight per warp
+};
 // Running maxima start finite, so that masked scores (-inf) never meet -inf - -inf.
 constexpr float kFloor = -3.0e38f;
+
+// The pair that a run opens and leaves to the runs behind it: `count` runs hold
+// parts of it (0: none).
+struct Kv4Cut {
+  int b, kvh, count;
+};
 
 struct Kv4AttnParams {
   const void* q;
@@ -49,7 +74,7 @@ struct Kv4AttnParams {
   const uint8_t* pool;
   float* o_part;  // [row tiles][runs + pairs][R][D]
   float* ml_part; // [row tiles][runs + pairs][R][2]
-  int* base;      // [row tiles][batch + 1] first tile of each sequence (per KV head)
+  Kv4Cut* cuts;   // [row tiles][runs]
   int heads, group;
   float scale_log2;  // log2(e) / sqrt(D)
   int* status;
@@ -64,7 +89,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 
@@ -76,49 +101,50 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
-template <typename T>
-struct Mma16;
-template <>
-struct Mma16<__nv_bfloat16> {
-  static constexpr uint32_t kMagic = 0x43004300u;   // 128 in both halves
-  static constexpr uint32_t kCentre = 0x43084308u;  // 136
-  static constexpr float kKeyOffset = 128.f;        // what a key operand adds to its code
-  static __device__ __forceinline__ uint32_t key(uint32_t c) { return c | kMagic; }
-  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
-                                     *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-};
-template <>
-struct Mma16<__half> {
-  static constexpr uint32_t kMagic = 0x64006400u;   // 1024 in both halves
-  static constexpr uint32_t kCentre = 0x64086408u;  // 1032
-  // An offset of 1024 would leave scores of fp16 queries ten bits short of fp32's
-  // 24: the key operand is centred too (one more instruction per pair).
-  static constexpr float kKeyOffset = -8.f;
-  static __device__ __forceinline__ uint32_t key(uint32_t c) { return sub(c | kMagic, kCentre); }
-  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-};
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// d = a.b + c with c apart from d (an accumulator's first product).
+__device__ __forceinline__ void mma_f16_init(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1, float c0, float c1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %10, %11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+
+// (x & mask) | 1024 in both halves, in one instruction (two constants in one
+// expression would be split in two).
+template <uint32_t kMask>
+__device__ __forceinline__ uint32_t nibbles(uint32_t x) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(kMask), "r"(0x64006400u));
+  return d;
+}
+// 1024 + c of the low nibble of each half; 1024 + 16 c of the second one.
+__device__ __forceinline__ uint32_t codes_even(uint32_t x) { return nibbles<0x000f000fu>(x); }
+__device__ __forceinline__ uint32_t codes_odd(uint32_t x) { return nibbles<0x00f000f0u>(x); }
+// c - 8 of either.
+__device__ __forceinline__ uint32_t centre_even(uint32_t u) {
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t centre_odd(uint32_t u) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(0.0625f, 0.0625f),
+                            __floats2half2_rn(-72.f, -72.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) { return Half16<__half>::pack(lo, hi); }
+
+// 2^k with k in [-126, 127].
+__device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }
 
 // Tiles of sequence b that columns [col0, col0 + R) see, and its lengths.
 struct SeqSpan {
@@ -130,7 +156,7 @@ struct SeqSpan {
   int tiles;
 };
 
-__device__ __forceinline__ SeqSpan seq_span(const Kv4Seq& s, int b, int group, int col0, int R) {
+__device__ __forceinline__ SeqSpan seq_span(const Kv4Seq& s, int b, int group, int col0, int R, int tile) {
   SeqSpan r;
   kv4_tokens(s, b, r.first, r.count);
   r.pre = s.prefix[b];
@@ -144,51 +170,82 @@ __device__ __forceinline__ SeqSpan seq_span(const Kv4Seq& s, int b, int group, i
   }
   r.len = static_cast<int>(len);
   // a sequence with columns but no positions still has a tile: its rows are zeros
-  r.tiles = r.cols == 0 ? 0 : (r.len == 0 ? 1 : (r.len + kATile - 1) / kATile);
+  r.tiles = r.cols == 0 ? 0 : (r.len == 0 ? 1 : (r.len + tile - 1) / tile);
   return r;
 }
 
-template <typename T, int D, int NT>
-constexpr int kv4_attn_smem() {
-  return kAWarps * kAStages * kv4_block_bytes(D) + kAWarps * 8 * NT * (D + 4) * 4 + kAWarps * 8 * NT * 2 * 4 +
-         kAWarps * kAStages * 8 + 64;
-}
+template <int D, int NT>
+struct AttnSmem {
+  using S = AttnShape<NT>;
+  static constexpr int kR = 8 * NT;
+  static constexpr int kLd = D + 4;  // row pitch of the merge buffer (floats)
+  static constexpr int kRing = S::kWarps * S::kStages * kv4_block_bytes(D);
+  static constexpr int kMerge = S::kWarps * kR * kLd * 4;
+  static constexpr int kMl = kRing + kMerge;                        // [warp][R][2] floats
+  // queries of two segments, each: fragments [group][word][nt][lane] uint4, then
+  // (sum, offsets) [R][D / 64] and the exponent factors [R]
+  static constexpr int kQ = kMl + S::kWarps * kR * 2 * 4;
+  static constexpr int kQsum = (D / 64) * 2 * NT * 512;
+  static constexpr int kQexp = kQsum + kR * (D / 64) * 8;
+  static constexpr int kQBytes = (kQexp + kR * 4 + 15) & ~15;
+  static constexpr int kBars = kQ + 2 * kQBytes;
+  static constexpr int kBytes = kBars + S::kWarps * S::kStages * 8;
+};
+
+// Weights times scales stay below 2^15 in fp16; a reference that moves leaves this
+// much (log2) to the weights that follow.
+constexpr float kRoom = 15.f, kSlack = 8.f;
+// A pair's first tile costs a run this many tiles more (queries, the pipeline's
+// start, the warps' meeting): runs are cut by cost.
+constexpr int kPairCost = 2;
+__device__ __forceinline__ int pair_cost(const SeqSpan& sp) { return sp.tiles ? sp.tiles + kPairCost : 0; }
 
 extern __shared__ __align__(128) uint8_t g_kv4_smem[];
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kAThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
+__global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     kv4_attn_kernel(const Kv4AttnParams p) {
-  constexpr int G = D / 64;            // groups of 64
-  constexpr int R = 8 * NT;            // columns
+  using S = AttnShape<NT>;
+  using L = AttnSmem<D, NT>;
+  constexpr int G = D / 64;   // groups of 64
+  constexpr int R = 8 * NT;   // columns
   constexpr int kBlk = kv4_block_bytes(D);
-  constexpr int kLd = D + 4;           // row pitch of the merge buffer (floats)
-  using M = Mma16<T>;
+  constexpr int kLd = L::kLd;
+  constexpr int kWarps = S::kWarps, kTile = S::kTile, kStages = S::kStages, kThreads = S::kThreads;
+  constexpr bool kQRegs = NT == 1;  // one column tile's query fragments fit in registers
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, qd = lane & 3;
   const int col0 = blockIdx.y * R;
 
-  uint8_t* ring = g_kv4_smem + warp * (kAStages * kBlk);
-  float* mrg_o = reinterpret_cast<float*>(g_kv4_smem + kAWarps * kAStages * kBlk);
-  float* mrg_ml = mrg_o + kAWarps * R * kLd;  // [warp][R][2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(mrg_ml + kAWarps * R * 2) + warp * kAStages;
-  __shared__ int sh_scan[kAWarps], sh_b, sh_base, sh_total;
+  uint8_t* ring = g_kv4_smem + warp * (kStages * kBlk);
+  float* mrg_o = reinterpret_cast<float*>(g_kv4_smem + L::kRing);
+  float* mrg_ml = reinterpret_cast<float*>(g_kv4_smem + L::kMl);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(g_kv4_smem + L::kBars) + warp * kStages;
+  // a run's segment: tiles [ta, tb) of a pair; tb = 0 behind the last one
+  struct Segment {
+    SeqSpan sp;
+    int b, kvh, ta, tb;
+  };
+  __shared__ Segment sh_seg[3];  // segment i in place i % 3
+  __shared__ uint32_t sh_walk_t, sh_walk_t0;  // thread 0's place in the list
+  __shared__ int sh_walk_b;
+  __shared__ int sh_scan[kWarps], sh_b, sh_base;
   __shared__ int sh_abort;
 
   if (tid == 0) sh_abort = 0;
   if (lane == 0) {
-    for (int i = 0; i < kAStages; ++i) mbar_init(&bars[i], 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&bars[i], 1);
     fence_mbar_init();
   }
   pdl_launch_dependents();
   pdl_wait();  // q and the cache append come from the previous kernels
 
   const Kv4Seq& s = p.seq;
-  // ---- the list of tiles: every thread sums a run of sequences, then a scan
-  const int per_thread = (s.batch + kAThreads - 1) / kAThreads;
+  // ---- the list of pairs in units of cost: every thread sums a run of sequences, then a scan
+  const int per_thread = (s.batch + kThreads - 1) / kThreads;
   const int b_lo = tid * per_thread, b_hi = b_lo + per_thread < s.batch ? b_lo + per_thread : s.batch;
   int mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += seq_span(s, b, p.group, col0, R).tiles;
+  for (int b = b_lo; b < b_hi; ++b) mine += pair_cost(seq_span(s, b, p.group, col0, R, kTile));
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -197,150 +254,230 @@ __global__ void __launch_bounds__(kAThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
   }
   if (lane == 31) sh_scan[warp] = incl;
   __syncthreads();
-  int before = incl - mine;
-  for (int w = 0; w < warp; ++w) before += sh_scan[w];
-  int all = 0;
-  for (int w = 0; w < kAWarps; ++w) all += sh_scan[w];
-  const int64_t total = static_cast<int64_t>(all) * s.kv_heads;
-  const int64_t per = (total + gridDim.x - 1) / gridDim.x;  // tiles per run
-  int* base = p.base + static_cast<int64_t>(blockIdx.y) * (s.batch + 1);
-  int64_t t_lo = per * blockIdx.x, t_hi = t_lo + per < total ? t_lo + per : total;
-  if (tid == 0) {
-    sh_b = s.batch;
-    sh_total = all;
+  int before = incl - mine, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const int v = sh_scan[w];
+    before += w < warp ? v : 0;
+    all += v;
   }
-  __syncthreads();
+  // (the host has checked that the list's length fits in 31 bits)
+  const uint32_t total = static_cast<uint32_t>(all) * s.kv_heads;
+  const uint32_t per = (total + gridDim.x - 1) / gridDim.x;  // cost of a run
+  const uint32_t t_lo = per * blockIdx.x, t_hi = t_lo + per < total ? t_lo + per : total;
+  Kv4Cut* cut = p.cuts + blockIdx.y * gridDim.x + blockIdx.x;  // the pair that this run opens and does not finish
+  if (tid == 0) cut->count = 0;
   {
     int at = before;
     for (int b = b_lo; b < b_hi; ++b) {
-      const SeqSpan sp = seq_span(s, b, p.group, col0, R);
-      if (blockIdx.x == 0) base[b] = at;
-      // sequence b covers tiles [at * KVH, (at + tiles) * KVH) of the list
-      if (t_lo < t_hi && static_cast<int64_t>(at) * s.kv_heads <= t_lo &&
-          t_lo < static_cast<int64_t>(at + sp.tiles) * s.kv_heads) {
+      const SeqSpan sp = seq_span(s, b, p.group, col0, R, kTile);
+      const int cost = pair_cost(sp);
+      // sequence b covers [at * KVH, (at + cost) * KVH) of the list
+      if (t_lo < t_hi && static_cast<uint32_t>(at) * s.kv_heads <= t_lo &&
+          t_lo < static_cast<uint32_t>(at + cost) * s.kv_heads) {
         sh_b = b;
         sh_base = at;
       }
-      at += sp.tiles;
-      // more columns than the launch covers, or positions outside the table
-      if (blockIdx.x == 0 &&
-          (sp.pre < 0 || (blockIdx.y == 0 && static_cast<int64_t>(sp.count) * p.group > static_cast<int64_t>(gridDim.y) * R) ||
-           (blockIdx.y == 0 && sp.count > 0 &&
-            static_cast<int64_t>(sp.pre) + sp.count > (static_cast<int64_t>(s.max_pages) << s.page_shift))))
+      // a negative prefix, positions outside the table, more columns than the launch covers
+      if (blockIdx.x == 0 && blockIdx.y == 0 && sp.count > 0 &&
+          (sp.pre < 0 || static_cast<int64_t>(sp.pre) + sp.count > (static_cast<int64_t>(s.max_pages) << s.page_shift) ||
+           static_cast<int64_t>(sp.count) * p.group > static_cast<int64_t>(gridDim.y) * R))
         report_device_error(p.status, FITQ_ERR_ARG);
+      at += cost;
     }
-    if (blockIdx.x == 0 && tid == 0) base[s.batch] = all;
   }
   __syncthreads();
   if (t_lo >= t_hi) return;
-  int b = sh_b;
-  int64_t seq_t0 = static_cast<int64_t>(sh_base) * s.kv_heads;  // first list tile of sequence b
+
+  // ---- the run's segments, found by thread 0 one ahead of their use
+  auto advance = [&](Segment& g) {
+    uint32_t t = sh_walk_t, t0 = sh_walk_t0;
+    int b = sh_walk_b;
+    g.tb = 0;
+    if (t < t_hi) {
+      SeqSpan sp = seq_span(s, b, p.group, col0, R, kTile);
+      while (t < t_hi && g.tb == 0) {
+        int cost = pair_cost(sp);
+        while (t >= t0 + static_cast<uint32_t>(cost) * s.kv_heads) {  // next sequence with work
+          t0 += static_cast<uint32_t>(cost) * s.kv_heads;
+          sp = seq_span(s, ++b, p.group, col0, R, kTile);
+          cost = pair_cost(sp);
+        }
+        g.kvh = static_cast<int>((t - t0) / static_cast<uint32_t>(cost));
+        const uint32_t pair_t0 = t0 + static_cast<uint32_t>(g.kvh) * cost;
+        const int xa = static_cast<int>(t - pair_t0);
+        const int xb = pair_t0 + cost < t_hi ? cost : static_cast<int>(t_hi - pair_t0);
+        t = pair_t0 + xb;
+        g.ta = xa > kPairCost ? xa - kPairCost : 0;
+        g.tb = xb > kPairCost ? xb - kPairCost : 0;
+        if (g.tb <= g.ta) g.tb = 0;  // the pair's first cost only, its tiles are the next run's
+      }
+      g.b = b;
+      g.sp = sp;
+    }
+    sh_walk_t = t;
+    sh_walk_t0 = t0;
+    sh_walk_b = b;
+  };
+  if (tid == 0) {
+    sh_walk_t = t_lo;
+    sh_walk_t0 = static_cast<uint32_t>(sh_base) * s.kv_heads;
+    sh_walk_b = sh_b;
+    advance(sh_seg[0]);
+  }
+  __syncthreads();
 
   const int64_t slot0 = static_cast<int64_t>(blockIdx.y) * (gridDim.x + static_cast<int64_t>(s.batch) * s.kv_heads);
   uint32_t issued = 0, taken = 0;  // this warp's copies so far
 
-  int64_t t = t_lo;
-  while (t < t_hi) {
-    SeqSpan sp = seq_span(s, b, p.group, col0, R);
-    while (sp.tiles == 0 || t >= seq_t0 + static_cast<int64_t>(sp.tiles) * s.kv_heads) {  // next sequence with work
-      seq_t0 += static_cast<int64_t>(sp.tiles) * s.kv_heads;
-      ++b;
-      sp = seq_span(s, b, p.group, col0, R);
+  // ---- this warp's blocks of the segment whose copies are under way: block j lies at
+  // position ta * kTile + 16 (warp + kWarps j); lane j % 32 looks its page up and
+  // issues its copy.
+  const uint8_t* src = nullptr;  // this lane's block of the set of 32 that is being issued
+  uint32_t valid = 0;            // which blocks of that set have a page
+  auto first_position = [&](const Segment& g) { return g.ta * kTile + kKv4Block * warp; };
+  auto block_count = [&](const Segment& g) {
+    const int first = first_position(g), end = g.tb * kTile < g.sp.len ? g.tb * kTile : g.sp.len;
+    return first < end ? (end - first + kTile - 1) / kTile : 0;
+  };
+  auto look_up = [&](const Segment& g, int j0) {
+    const int j = j0 + lane;
+    int pg = -1;
+    if (j < block_count(g)) {
+      const int64_t pos = first_position(g) + static_cast<int64_t>(j) * kTile;
+      pg = kv4_page(s, g.b, pos);
+      if (pg < 0)
+        report_device_error(p.status, FITQ_ERR_ARG);
+      else
+        src = p.pool + kv4_block_offset(s, pg, g.kvh, pos, D);
     }
-    const int kvh = static_cast<int>((t - seq_t0) / sp.tiles);
-    const int64_t pair_t0 = seq_t0 + static_cast<int64_t>(kvh) * sp.tiles;
-    const int ta = static_cast<int>(t - pair_t0);
-    int tb = sp.tiles;
-    if (pair_t0 + tb > t_hi) tb = static_cast<int>(t_hi - pair_t0);
-    const bool whole = ta == 0 && tb == sp.tiles;
-
-    // ---- this warp's blocks: block j at position ta * kATile + 16 (warp + 4 j)
-    const int pos_first = ta * kATile + kKv4Block * warp;
-    const int pos_end = tb * kATile < sp.len ? tb * kATile : sp.len;
-    const int blocks = pos_first < pos_end ? (pos_end - pos_first + kATile - 1) / kATile : 0;
-    int pages = -1;   // lane j: page of block 32 * (j / 32) + lane
-    auto load_pages = [&](int j0) {
-      const int j = j0 + lane;
-      pages = -1;
-      if (j < blocks) {
-        pages = kv4_page(s, b, pos_first + static_cast<int64_t>(j) * kATile);
-        if (pages < 0) report_device_error(p.status, FITQ_ERR_ARG);
-      }
-    };
-    auto issue = [&](int pg, int j) {  // whole warp; pg uniform
-      if (pg < 0) return;
-      const int st = issued % kAStages;
-      if (lane == 0) {
+    valid = __ballot_sync(0xffffffffu, pg >= 0);
+  };
+  int next = 0;  // next block to issue: at most kStages ahead of the first unread one
+  auto issue_next = [&](const Segment& g) {
+    if ((next & 31) == 0 && next > 0) look_up(g, next);
+    if ((valid >> (next & 31)) & 1u) {
+      if (lane == (next & 31)) {
+        const uint32_t st = issued % kStages;
         mbar_arrive_expect_tx(&bars[st], kBlk);
-        bulk_load(ring + st * kBlk,
-                  p.pool + kv4_block_offset(s, pg, kvh, pos_first + static_cast<int64_t>(j) * kATile, D), kBlk,
-                  &bars[st]);
+        bulk_load(ring + st * kBlk, src, kBlk, &bars[st]);
       }
       ++issued;
-    };
-    load_pages(0);
-    uint32_t valid = __ballot_sync(0xffffffffu, pages >= 0);  // blocks 32 k .. of the current page set
-    int next = 0;                                             // next block to issue
-    uint32_t next_valid = 0;  // validity of the page set that starts at next_set
-    int cur_pages = pages;
-    // blocks are consumed in order; the copies run at most kAStages ahead of block `done`
-    auto issue_next = [&](int done) {
-      while (next < blocks && next < done + kAStages) {
-        if ((next & 31) == 0 && next > 0) {
-          load_pages(next);
-          cur_pages = pages;
-          next_valid = __ballot_sync(0xffffffffu, pages >= 0);
-        }
-        const int pg = __shfl_sync(0xffffffffu, cur_pages, next & 31);
-        issue(pg, next);
-        ++next;
-      }
-    };
-    issue_next(0);
-
-    // ---- query fragments (column n = 8 nt + g), their group sums, column limits
-    uint32_t qf[NT][G][2][4];
-    float qs[NT][2][G];  // offset-corrected sums belong to the columns 2 qd, 2 qd + 1
-    int lim[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int n = 8 * nt + g;
+    }
+    ++next;
+  };
+  auto start = [&](const Segment& g) {
+    next = 0;
+    const int n = block_count(g);
+    for (int i = 0; i < kStages && i < n; ++i) issue_next(g);
+  };
+  // ---- a segment's queries into buffer `to`: columns scaled to fp16's range, in the
+  // order in which the codes leave their words (element pairs (e, e + 4) of eight),
+  // with their group sums
+  auto load_queries = [&](const Segment& g, uint8_t* to) {
+    uint4* sq = reinterpret_cast<uint4*>(to);
+    float2* sqsum = reinterpret_cast<float2*>(to + L::kQsum);
+    float* sqexp = reinterpret_cast<float*>(to + L::kQexp);
+    const SeqSpan& sp = g.sp;
+    const int kvh = g.kvh;
+    for (int i = tid; i < R * 4; i += kThreads) {
+      const int n = i >> 2, c = i & 3;  // four neighbouring lanes hold a column
       const bool has = n < sp.cols;
       const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
-      const T* src = static_cast<const T*>(p.q) + (sp.first + tok) * p.q_stride +
-                     static_cast<int64_t>(kvh * p.group + hd) * D;
-      float sum[G];
+      const T* qp = static_cast<const T*>(p.q) + (sp.first + tok) * p.q_stride +
+                    static_cast<int64_t>(kvh * p.group + hd) * D;
+      uint4 u[G][2];
+      float mx = 0.f;
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        sum[gr] = 0.f;
+      for (int gr = 0; gr < G; ++gr)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          uint4 u = make_uint4(0, 0, 0, 0);
-          if (has) u = *reinterpret_cast<const uint4*>(src + 64 * gr + 16 * qd + 8 * w);
+          u[gr][w] = make_uint4(0, 0, 0, 0);
+          if (has) u[gr][w] = *reinterpret_cast<const uint4*>(qp + 64 * gr + 16 * c + 8 * w);
           float f[8];
-          unpack8<T>(u, f);
+          unpack8<T>(u[gr][w], f);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sum[gr] += f[i];
-          // pairs (e, e + 4): the order in which the codes leave their word
-          qf[nt][gr][w][0] = __byte_perm(u.x, u.z, 0x5410);
-          qf[nt][gr][w][1] = __byte_perm(u.x, u.z, 0x7632);
-          qf[nt][gr][w][2] = __byte_perm(u.y, u.w, 0x5410);
-          qf[nt][gr][w][3] = __byte_perm(u.y, u.w, 0x7632);
+          for (int x = 0; x < 8; ++x) mx = fmaxf(mx, fabsf(f[x]));
         }
-        sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
-        sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
-        qs[nt][0][gr] = __shfl_sync(0xffffffffu, sum[gr], 8 * qd);
-        qs[nt][1][gr] = __shfl_sync(0xffffffffu, sum[gr], 8 * qd + 4);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      int e = (__float_as_int(mx) >> 23) - 127;
+      e = (mx == 0.f || e > 127) ? 12 : (e < -100 ? -100 : e);
+      const float up = pow2(12 - e);
+#pragma unroll
+      for (int gr = 0; gr < G; ++gr) {
+        float even = 0.f, odd = 0.f;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          float f[8];
+          unpack8<T>(u[gr][w], f);
+#pragma unroll
+          for (int x = 0; x < 8; x += 2) {
+            f[x] *= up;
+            f[x + 1] *= up * 0.0625f;
+            even += f[x];
+            odd += f[x + 1];
+          }
+          // lane 4 (n % 8) + c of the fragment of column tile n / 8
+          sq[((gr * 2 + w) * NT + (n >> 3)) * 32 + (n & 7) * 4 + c] =
+              make_uint4(pack_half2(f[0], f[4]), pack_half2(f[1], f[5]), pack_half2(f[2], f[6]), pack_half2(f[3], f[7]));
+        }
+        float sum = fmaf(16.f, odd, even), off = 1024.f * (even + odd);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        off += __shfl_xor_sync(0xffffffffu, off, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        off += __shfl_xor_sync(0xffffffffu, off, 2);
+        if (c == 0) sqsum[n * G + gr] = make_float2(sum, -off);
       }
+      if (c == 0) sqexp[n] = p.scale_log2 * pow2(e - 12);
+    }
+  };
+
+  look_up(sh_seg[0], 0);
+  start(sh_seg[0]);
+  load_queries(sh_seg[0], g_kv4_smem + L::kQ);
+  if (tid == 0) advance(sh_seg[1]);
+  int buf = 0;
+  for (int seg = 0, after = 1; sh_seg[seg].tb > 0; seg = after, after = after == 2 ? 0 : after + 1) {
+    const Segment& sg = sh_seg[seg];
+    const Segment& sn = sh_seg[after];
+    const int pos_first = first_position(sg), blocks = block_count(sg), len = sg.sp.len;
+    const uint8_t* sq_now = g_kv4_smem + L::kQ + buf * L::kQBytes;
+    const uint4* sq = reinterpret_cast<const uint4*>(sq_now);
+    const float2* sqsum = reinterpret_cast<const float2*>(sq_now + L::kQsum);
+    const float* sqexp = reinterpret_cast<const float*>(sq_now + L::kQexp);
+    buf ^= 1;
+    __syncthreads();  // the queries are there, the merge buffer and the last segment's place are free
+    if (tid == 0) advance(sh_seg[after == 2 ? 0 : after + 1]);
+    uint4 qf[kQRegs ? G : 1][2];
+    if (kQRegs) {
+#pragma unroll
+      for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) qf[kQRegs ? gr : 0][w] = sq[(gr * 2 + w) * 32 + lane];
+    }
+    float qs[NT][2][G], qo[NT][2][G], cn[NT][2];  // of the columns 2 qd, 2 qd + 1: sums, offsets, exponent per score
+    int lim[NT][2];                 // and the last position they see
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int l = sp.pre + (col0 + 8 * nt + 2 * qd + e) / p.group;
-        lim[nt][e] = l < sp.len ? l : sp.len - 1;
+        const int n = 8 * nt + 2 * qd + e;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+          const float2 v = sqsum[n * G + gr];
+          qs[nt][e][gr] = v.x;
+          qo[nt][e][gr] = v.y;
+        }
+        cn[nt][e] = sqexp[n];
+        const int l = sg.sp.pre + (col0 + n) / p.group;
+        lim[nt][e] = l < len ? l : len - 1;
       }
-    }
-    const int mask_from = sp.pre + col0 / p.group + 1;  // positions every column sees lie before it
+    const int mask_from = sg.sp.pre + col0 / p.group + 1;  // positions every column sees lie before it
 
-    float m_run[NT][2], l_run[NT][2], corr[NT][2][G], o[NT][G][4][4];
+    float m_run[NT][2], l_run[NT][2], corr[NT][2][G], o[NT][G][4][4];  // m_run in log2 units
+    // no scale met so far exceeds 2^cap_log2; weights stay below 2^(kRoom - cap_log2)
+    float cap = pow2(-30), room = kRoom + 30.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -358,26 +495,50 @@ __global__ void __launch_bounds__(kAThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
           for (int e = 0; e < 4; ++e) o[nt][gr][i][e] = 0.f;
     }
 
-    uint32_t cur_valid = valid;
-    for (int j = 0; j < blocks; ++j) {
-      if ((j & 31) == 0 && j > 0) cur_valid = next_valid;
-      if (!((cur_valid >> (j & 31)) & 1u)) {  // no page: the block is hidden from every column
-        issue_next(j + 1);
-        continue;
+    uint32_t set_valid = 0;
+    // block j; edge: some of its positions are hidden from some columns.  False once a wait ran out.
+    auto block = [&](int j, auto edge_tag) -> bool {
+      constexpr bool edge = decltype(edge_tag)::value;
+      if ((j & 31) == 0) set_valid = valid;  // block j has been issued, its set is the current one
+      if (!((set_valid >> (j & 31)) & 1u)) {  // no page: the block is hidden from every column
+        if (next < blocks) issue_next(sg);
+        return true;
       }
-      const int st = taken % kAStages;
-      if (!mbar_wait(&bars[st], (taken / kAStages) & 1u, &sh_abort, p.status)) break;
+      const uint32_t st = taken % kStages;
+      if (!mbar_wait(&bars[st], (taken / kStages) & 1u, &sh_abort, p.status)) return false;
       const uint8_t* blk = ring + st * kBlk;
-      const int pos0 = pos_first + j * kATile;
+      const int pos0 = pos_first + j * kTile;
+
+      // ---- parameters of positions g and g + 8: {key, value} x groups x (scale, low)
+      float ks[2][G], kl[2][G], vs[2][G], vl[2][G];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pr[2 * G];
+        const uint8_t* psrc = blk + 16 * D + (g + 8 * h) * 8 * G;
+        if (G == 2)
+          *reinterpret_cast<uint4*>(pr) = *reinterpret_cast<const uint4*>(psrc);
+        else
+          *reinterpret_cast<uint2*>(pr) = *reinterpret_cast<const uint2*>(psrc);
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+          const float2 a = Half16<__half>::unpack(pr[gr]);
+          const float2 c = Half16<__half>::unpack(pr[G + gr]);
+          ks[h][gr] = a.x;
+          kl[h][gr] = a.y;
+          vs[h][gr] = c.x;
+          vl[h][gr] = fmaf(8.f, c.x, c.y);
+        }
+      }
+      if (edge) {  // whatever lies behind the last position must not matter
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (pos0 + g + 8 * h >= len)
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) ks[h][gr] = kl[h][gr] = vs[h][gr] = vl[h][gr] = 0.f;
+      }
 
       // ---- S^T = K.Q^T, one accumulator set per group
       float acc[NT][G][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][gr][e] = 0.f;
       uint32_t kw[2][2 * G];
       if (G == 2) {
 #pragma unroll
@@ -389,86 +550,81 @@ __global__ void __launch_bounds__(kAThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
           *reinterpret_cast<uint2*>(kw[h]) = *reinterpret_cast<const uint2*>(blk + h * 256 + lane * 8);
       }
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr)
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t x = kw[0][2 * gr + w], y = kw[1][2 * gr + w];
+        for (int gr = 0; gr < G; ++gr) {
+          uint32_t x = kw[0][2 * gr + w], y = kw[1][2 * gr + w];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t a0 = M::key((x >> (8 * h)) & 0x000f000fu);
-            const uint32_t a1 = M::key((y >> (8 * h)) & 0x000f000fu);
-            const uint32_t a2 = M::key((x >> (8 * h + 4)) & 0x000f000fu);
-            const uint32_t a3 = M::key((y >> (8 * h + 4)) & 0x000f000fu);
+            const uint32_t a0 = codes_even(x), a1 = codes_even(y), a2 = codes_odd(x), a3 = codes_odd(y);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              M::mma(acc[nt][gr], a0, a1, a2, a3, qf[nt][gr][w][2 * h], qf[nt][gr][w][2 * h + 1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              uint2 bq;
+              if (kQRegs)
+                bq = h ? make_uint2(qf[kQRegs ? gr : 0][w].z, qf[kQRegs ? gr : 0][w].w)
+                       : make_uint2(qf[kQRegs ? gr : 0][w].x, qf[kQRegs ? gr : 0][w].y);
+              else
+                bq = *(reinterpret_cast<const uint2*>(&sq[((gr * 2 + w) * NT + nt) * 32 + lane]) + h);
+              if (w == 0 && h == 0)
+                mma_f16_init(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y, qo[nt][0][gr], qo[nt][1][gr]);
+              else
+                mma_f16(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y);
+            }
+            x >>= 8;
+            y >>= 8;
           }
         }
 
-      // ---- parameters of positions g and g + 8: {key, value} x groups x (scale, low)
-      float ks[2][G], kl[2][G], vs[2][G], vl[2][G];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t pr[2 * G];
-        const uint8_t* src = blk + 16 * D + (g + 8 * h) * 8 * G;
-        if (G == 2)
-          *reinterpret_cast<uint4*>(pr) = *reinterpret_cast<const uint4*>(src);
-        else
-          *reinterpret_cast<uint2*>(pr) = *reinterpret_cast<const uint2*>(src);
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          const float2 a = Half16<__half>::unpack(pr[gr]);
-          const float2 c = Half16<__half>::unpack(pr[G + gr]);
-          ks[h][gr] = a.x;
-          kl[h][gr] = fmaf(-M::kKeyOffset, a.x, a.y);
-          vs[h][gr] = c.x;
-          vl[h][gr] = fmaf(8.f, c.x, c.y);
-        }
-      }
-      float sc[NT][4];  // (position g: columns 2 qd, 2 qd + 1; position g + 8: the same)
+      // ---- scores in log2 units less the reference (position g: columns 2 qd, 2 qd + 1;
+      // position g + 8: the same)
+      float sc[NT][4], x[NT][4];
+      bool over = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int h = e >> 1;
-          float v = 0.f;
-#pragma unroll
-          for (int gr = 0; gr < G; ++gr) {
-            v = fmaf(ks[h][gr], acc[nt][gr][e], v);
-            v = fmaf(kl[h][gr], qs[nt][e & 1][gr], v);
+          float v = ks[h][0] * acc[nt][0][e];
+          v = fmaf(kl[h][0], qs[nt][e & 1][0], v);
+          if (G == 2) {
+            v = fmaf(ks[h][G - 1], acc[nt][G - 1][e], v);
+            v = fmaf(kl[h][G - 1], qs[nt][e & 1][G - 1], v);
           }
           sc[nt][e] = v;
+          x[nt][e] = fmaf(v, cn[nt][e & 1], -m_run[nt][e & 1]);
+          if (edge && pos0 + g + 8 * h > lim[nt][e & 1]) sc[nt][e] = x[nt][e] = -INFINITY;
+          over |= x[nt][e] > room;
         }
-      const bool edge = pos0 + kKv4Block > mask_from;
-      if (edge) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (pos0 + g + 8 * (e >> 1) > lim[nt][e & 1]) sc[nt][e] = -INFINITY;
-      }
-
-      // ---- running maximum per column (over the eight lanes that share qd)
-      bool grew = false;
-      float m_new[NT][2];
+        for (int gr = 0; gr < G; ++gr) over |= fabsf(vs[h][gr]) > cap;
+      if (__any_sync(0xffffffffu, over)) {
+        float vm = 0.f;  // the largest finite scale of the block
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(sc[nt][e], sc[nt][2 + e]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          m_new[nt][e] = fmaxf(m_run[nt][e], mx);
-          grew |= m_new[nt][e] > m_run[nt][e];
+          for (int gr = 0; gr < G; ++gr) vm = fmaxf(vm, fabsf(vs[h][gr]) <= 65504.f ? fabsf(vs[h][gr]) : 0.f);
+#pragma unroll
+        for (int o2 = 1; o2 < 32; o2 <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o2));
+        if (vm > cap) {
+          const int e = (__float_as_int(vm) >> 23) - 126;  // vm < 2^e
+          cap = pow2(e);
+          room = kRoom - static_cast<float>(e);
         }
-      if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float al = exp2_approx((m_run[nt][e] - m_new[nt][e]) * p.scale_log2);
-            m_run[nt][e] = m_new[nt][e];
+            float mx = fmaxf(sc[nt][e], sc[nt][2 + e]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            mx = fmaxf(fmaf(mx, cn[nt][e], kSlack - room), m_run[nt][e]);
+            const float al = exp2_approx(m_run[nt][e] - mx);
+            m_run[nt][e] = mx;
+            x[nt][e] = fmaf(sc[nt][e], cn[nt][e], -mx);
+            x[nt][2 + e] = fmaf(sc[nt][2 + e], cn[nt][e], -mx);
             l_run[nt][e] *= al;
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
@@ -489,7 +645,7 @@ __global__ void __launch_bounds__(kAThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = exp2_approx((sc[nt][e] - m_run[nt][e & 1]) * p.scale_log2);
+          w[e] = exp2_approx(x[nt][e]);
           l_run[nt][e & 1] += w[e];
         }
 #pragma unroll
@@ -499,12 +655,13 @@ __global__ void __launch_bounds__(kAThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
           for (int e = 0; e < 4; ++e) {
             const int h = e >> 1;
             ws[e] = w[e] * vs[h][gr];
-            float add = w[e] * vl[h][gr];
-            if (edge && pos0 + g + 8 * h > lim[nt][e & 1]) ws[e] = add = 0.f;  // whatever the hidden value holds
-            corr[nt][e & 1][gr] += add;
+            if (edge && pos0 + g + 8 * h > lim[nt][e & 1])
+              ws[e] = 0.f;  // whatever the hidden value holds
+            else
+              corr[nt][e & 1][gr] = fmaf(w[e], vl[h][gr], corr[nt][e & 1][gr]);
           }
-          pb[nt][gr][0] = movmatrix_t(Half16<T>::pack(ws[0], ws[1]));
-          pb[nt][gr][1] = movmatrix_t(Half16<T>::pack(ws[2], ws[3]));
+          pb[nt][gr][0] = movmatrix_t(pack_half2(ws[0], ws[1]));
+          pb[nt][gr][1] = movmatrix_t(pack_half2(ws[2], ws[3]));
         }
       }
 
@@ -521,30 +678,38 @@ __global__ void __launch_bounds__(kAThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
       }
       __syncwarp();  // every lane has read the block
       ++taken;
-      issue_next(j + 1);
+      if (next < blocks) issue_next(sg);
 #pragma unroll
       for (int gr = 0; gr < G; ++gr)
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          const uint32_t x = __byte_perm(vw[0][0][gr], vw[0][1][gr], z ? 0x7632 : 0x5410);
-          const uint32_t y = __byte_perm(vw[1][0][gr], vw[1][1][gr], z ? 0x7632 : 0x5410);
+          uint32_t x = __byte_perm(vw[0][0][gr], vw[0][1][gr], z ? 0x7632 : 0x5410);
+          uint32_t y = __byte_perm(vw[1][0][gr], vw[1][1][gr], z ? 0x7632 : 0x5410);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t a0 = M::sub(((x >> (8 * i)) & 0x000f000fu) | M::kMagic, M::kCentre);
-            const uint32_t a1 = M::sub(((x >> (8 * i + 4)) & 0x000f000fu) | M::kMagic, M::kCentre);
-            const uint32_t a2 = M::sub(((y >> (8 * i)) & 0x000f000fu) | M::kMagic, M::kCentre);
-            const uint32_t a3 = M::sub(((y >> (8 * i + 4)) & 0x000f000fu) | M::kMagic, M::kCentre);
+            const uint32_t a0 = centre_even(codes_even(x)), a1 = centre_odd(codes_odd(x)),
+                           a2 = centre_even(codes_even(y)), a3 = centre_odd(codes_odd(y));
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              M::mma(o[nt][gr][2 * z + i], a0, a1, a2, a3, pb[nt][gr][0], pb[nt][gr][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][gr][2 * z + i], a0, a1, a2, a3, pb[nt][gr][0], pb[nt][gr][1]);
+            x >>= 8;
+            y >>= 8;
           }
         }
-    }
+      return true;
+    };
+    // the blocks that every column sees to their end come first
+    int inner = (mask_from - pos_first - kKv4Block) / kTile + 1;
+    if (mask_from - pos_first < kKv4Block) inner = 0;
+    if (inner > blocks) inner = blocks;
+    bool fine = true;
+    for (int j = 0; j < inner && fine; ++j) fine = block(j, std::false_type{});
+    for (int j = inner; j < blocks && fine; ++j) fine = block(j, std::true_type{});
 
-    if (sh_abort) {  // a wait ran out: the copies still in flight land before the CTA leaves
-      int none = 0;
-      for (; taken != issued; ++taken)
-        mbar_wait_for(&bars[taken % kAStages], (taken / kAStages) & 1u, &none, p.status, kWaitLimitNs);
+    // ---- the next segment's copies and queries set out before the warps meet
+    if (sn.tb > 0 && fine) {
+      look_up(sn, 0);
+      start(sn);
+      load_queries(sn, g_kv4_smem + L::kQ + buf * L::kQBytes);
     }
 
     // ---- the warps' results meet in shared memory
@@ -563,29 +728,41 @@ __global__ void __launch_bounds__(kAThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
           const float c = corr[nt][e][gr];
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f[2 * i] = o[nt][gr][i][e] + c;
+            f[2 * i + 1] = o[nt][gr][i][2 + e] + c;
+          }
           float* dst = row + 64 * gr + 8 * g;
-          *reinterpret_cast<float4*>(dst) =
-              make_float4(o[nt][gr][0][e] + c, o[nt][gr][0][2 + e] + c, o[nt][gr][1][e] + c, o[nt][gr][1][2 + e] + c);
-          *reinterpret_cast<float4*>(dst + 4) =
-              make_float4(o[nt][gr][2][e] + c, o[nt][gr][2][2 + e] + c, o[nt][gr][3][e] + c, o[nt][gr][3][2 + e] + c);
+          *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
         }
         if (g == 0) *reinterpret_cast<float2*>(mrg_ml + (warp * R + n) * 2) = make_float2(m_run[nt][e], l_run[nt][e]);
       }
     __syncthreads();
+    const SeqSpan sp = sg.sp;
+    const int b = sg.b, kvh = sg.kvh;
+    const bool whole = sg.ta == 0 && sg.tb == sp.tiles;
+    if (tid == 0 && sg.ta == 0 && !whole) {
+      // this run opens the pair; the last of its other tiles lies `rest` of cost behind the run's end
+      const uint32_t rest = sp.tiles - sg.tb - 1;
+      *cut = Kv4Cut{b, kvh, static_cast<int>(2 + rest / per)};
+    }
     const int64_t slot = slot0 + blockIdx.x + static_cast<int64_t>(b) * s.kv_heads + kvh;
-    for (int i = tid; i < sp.cols * (D / 8); i += kAThreads) {
+    for (int i = tid; i < sp.cols * (D / 8); i += kThreads) {
       const int n = i / (D / 8), d0 = (i % (D / 8)) * 8;
       float mx = kFloor;
 #pragma unroll
-      for (int w = 0; w < kAWarps; ++w) mx = fmaxf(mx, mrg_ml[(w * R + n) * 2]);
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, mrg_ml[(w * R + n) * 2]);
       float l = 0.f, f[8];
 #pragma unroll
       for (int x = 0; x < 8; ++x) f[x] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kAWarps; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         const float2 ml = *reinterpret_cast<const float2*>(mrg_ml + (w * R + n) * 2);
         if (ml.y == 0.f) continue;  // this warp saw no position of the column
-        const float k = exp2_approx((ml.x - mx) * p.scale_log2);
+        const float k = exp2_approx(ml.x - mx);
         l += k * ml.y;
         const float* row = mrg_o + (w * R + n) * kLd + d0;
 #pragma unroll
@@ -605,86 +782,120 @@ __global__ void __launch_bounds__(kAThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
         if (d0 == 0) *reinterpret_cast<float2*>(p.ml_part + (slot * R + n) * 2) = make_float2(mx, l);
       }
     }
-    __syncthreads();  // the merge buffer is free again
-    t = pair_t0 + tb;
     if (sh_abort) break;
+  }
+  if (sh_abort) {  // a wait ran out: the copies still in flight land before the CTA leaves
+    int none = 0;
+    for (; taken != issued; ++taken)
+      mbar_wait_for(&bars[taken % kStages], (taken / kStages) & 1u, &none, p.status, kWaitLimitNs);
   }
 }
 
-// Joins the runs that a pair was cut into, in run order.  Grid (batch * KVH, row
-// tiles), D / 8 lanes per column.
+// Joins the runs that a pair was cut into, in a fixed order.  Grid (runs, columns,
+// row tiles): the CTA of the run that opens a pair joins one column of it; four
+// warps take every fourth run each.
+constexpr int kCWarps = 4;
+constexpr int kCMaxRuns = 1024;  // more runs than a launch has
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) kv4_attn_combine_kernel(const Kv4AttnParams p, int runs) {
+__global__ void __launch_bounds__(32 * kCWarps) kv4_attn_combine_kernel(const Kv4AttnParams p) {
   constexpr int R = 8 * NT;
+  constexpr int kE = D / 32;  // elements per lane
+  __shared__ float sh_o[kCWarps][D];
+  __shared__ float sh_ml[kCWarps][2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int run = blockIdx.x, n = blockIdx.y, runs = gridDim.x;
   pdl_launch_dependents();
   pdl_wait();  // the partials
+  const Kv4Cut cut = p.cuts[blockIdx.z * runs + run];
+  if (cut.count == 0) return;
   const Kv4Seq& s = p.seq;
-  const int b = blockIdx.x / s.kv_heads, kvh = blockIdx.x % s.kv_heads;
-  const int* base = p.base + static_cast<int64_t>(blockIdx.y) * (s.batch + 1);
-  const int64_t total = static_cast<int64_t>(base[s.batch]) * s.kv_heads;
-  const int tiles = base[b + 1] - base[b];
-  if (tiles == 0) return;
-  const int64_t per = (total + runs - 1) / runs;
-  const int64_t t0 = static_cast<int64_t>(base[b]) * s.kv_heads + static_cast<int64_t>(kvh) * tiles;
-  const int64_t c0 = t0 / per, c1 = (t0 + tiles - 1) / per;
-  if (c0 == c1) return;  // written by its one run
-  const int col0 = blockIdx.y * R;
-  const SeqSpan sp = seq_span(s, b, p.group, col0, R);
-  const int64_t slot0 = static_cast<int64_t>(blockIdx.y) * (runs + static_cast<int64_t>(s.batch) * s.kv_heads) +
-                        static_cast<int64_t>(b) * s.kv_heads + kvh;
-  for (int i = threadIdx.x; i < sp.cols * (D / 8); i += 128) {
-    const int n = i / (D / 8), d0 = (i % (D / 8)) * 8;
-    float mx = kFloor;
-    for (int64_t c = c0; c <= c1; ++c) mx = fmaxf(mx, p.ml_part[((slot0 + c) * R + n) * 2]);
-    float l = 0.f, f[8];
+  const int col0 = blockIdx.z * R;
+  const SeqSpan sp = seq_span(s, cut.b, p.group, col0, R, AttnShape<NT>::kTile);
+  if (n >= sp.cols) return;
+  const int64_t slot0 = static_cast<int64_t>(blockIdx.z) * (runs + static_cast<int64_t>(s.batch) * s.kv_heads) +
+                        static_cast<int64_t>(cut.b) * s.kv_heads + cut.kvh + run;
+  const float2* ml = reinterpret_cast<const float2*>(p.ml_part) + slot0 * R + n;
+  const float* row = p.o_part + (slot0 * R + n) * D + lane * kE;
+  float mx = kFloor, l = 0.f, f[kE];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = 0.f;
-    for (int64_t c = c0; c <= c1; ++c) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.ml_part + ((slot0 + c) * R + n) * 2);
-      if (ml.y == 0.f) continue;
-      const float k = exp2_approx((ml.x - mx) * p.scale_log2);
-      l += k * ml.y;
-      const float4* src = reinterpret_cast<const float4*>(p.o_part + ((slot0 + c) * R + n) * D + d0);
-      const float4 a = src[0], c4 = src[1];
-      f[0] = fmaf(k, a.x, f[0]); f[1] = fmaf(k, a.y, f[1]); f[2] = fmaf(k, a.z, f[2]); f[3] = fmaf(k, a.w, f[3]);
-      f[4] = fmaf(k, c4.x, f[4]); f[5] = fmaf(k, c4.y, f[5]); f[6] = fmaf(k, c4.z, f[6]); f[7] = fmaf(k, c4.w, f[7]);
-    }
-    const float inv = 1.f / l;
+  for (int x = 0; x < kE; ++x) f[x] = 0.f;
+#pragma unroll 4
+  for (int c = warp; c < cut.count; c += kCWarps) {
+    const float2 w = ml[static_cast<int64_t>(c) * R];
+    float v[kE];
+    if (kE == 4)
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(row + static_cast<int64_t>(c) * R * D);
+    else
+      *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(row + static_cast<int64_t>(c) * R * D);
+    if (w.y == 0.f) continue;  // that run saw no position of the column
+    const float m = fmaxf(mx, w.x), k0 = exp2_approx(mx - m), k1 = exp2_approx(w.x - m);
+    mx = m;
+    l = k0 * l + k1 * w.y;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) f[x] = l == 0.f ? 0.f : f[x] * inv;
-    const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
-    T* dst = static_cast<T*>(p.out) + ((sp.first + tok) * p.heads + kvh * p.group + hd) * D + d0;
-    *reinterpret_cast<uint4*>(dst) = pack8<T>(f);
+    for (int x = 0; x < kE; ++x) f[x] = k0 * f[x] + k1 * v[x];
   }
+#pragma unroll
+  for (int x = 0; x < kE; ++x) sh_o[warp][lane * kE + x] = f[x];
+  if (lane == 0) {
+    sh_ml[warp][0] = mx;
+    sh_ml[warp][1] = l;
+  }
+  __syncthreads();
+  if (threadIdx.x >= D / 2) return;
+  mx = kFloor;
+#pragma unroll
+  for (int w = 0; w < kCWarps; ++w) mx = fmaxf(mx, sh_ml[w][0]);
+  float a = 0.f, b2 = 0.f;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kCWarps; ++w) {
+    if (sh_ml[w][1] == 0.f) continue;
+    const float k = exp2_approx(sh_ml[w][0] - mx);
+    l += k * sh_ml[w][1];
+    a = fmaf(k, sh_o[w][2 * threadIdx.x], a);
+    b2 = fmaf(k, sh_o[w][2 * threadIdx.x + 1], b2);
+  }
+  const float inv = 1.f / l;
+  const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
+  T* dst = static_cast<T*>(p.out) + ((sp.first + tok) * p.heads + cut.kvh * p.group + hd) * D + 2 * threadIdx.x;
+  *reinterpret_cast<uint32_t*>(dst) = l == 0.f ? 0u : Half16<T>::pack(a * inv, b2 * inv);
 }
 
 // Columns of a call: tokens of a sequence x heads of a KV head, in n8 tiles.
 int col_tiles(int group, int64_t max_new) {
   const int64_t cols = static_cast<int64_t>(group) * max_new;
-  return cols <= 8 ? 1 : (cols <= 16 ? 2 : 4);
+  return cols <= 8 ? 1 : 2;
 }
 
 struct AttnPlan {
-  int nt, row_tiles, runs;
-  size_t base_off, ml_off, o_off, bytes;
+  int nt, row_tiles, cols, runs;  // cols: columns of the fullest row tile
+  size_t cuts_off, ml_off, o_off, bytes;
 };
+
+template <int NT>
+int64_t plan_runs(int64_t pairs, int64_t max_len, int row_tiles, int num_sms) {
+  const int64_t tiles = pairs * ((max_len + AttnShape<NT>::kTile - 1) / AttnShape<NT>::kTile);
+  int64_t runs = static_cast<int64_t>(num_sms) * AttnShape<NT>::kCtas;
+  if (row_tiles > 1) runs = (runs + row_tiles - 1) / row_tiles;
+  if (runs > tiles) runs = tiles;
+  if (runs > kCMaxRuns) runs = kCMaxRuns;
+  return runs < 1 ? 1 : runs;
+}
 
 AttnPlan attn_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim, int num_sms) {
   AttnPlan a;
   a.nt = col_tiles(group, max_new);
   const int R = 8 * a.nt;
   a.row_tiles = static_cast<int>((group * max_new + R - 1) / R);
-  const int ctas = a.nt == 1 ? 4 : (a.nt == 2 ? 3 : 2);
+  a.cols = static_cast<int>(group * max_new < R ? group * max_new : R);
   const int64_t pairs = static_cast<int64_t>(batch) * kv_heads;
-  const int64_t tiles = pairs * ((max_len + kATile - 1) / kATile);
-  int64_t runs = static_cast<int64_t>(num_sms) * ctas;
-  if (a.row_tiles > 1) runs = (runs + a.row_tiles - 1) / a.row_tiles;
-  if (runs > tiles) runs = tiles;
-  a.runs = static_cast<int>(runs < 1 ? 1 : runs);
+  a.runs = static_cast<int>(a.nt == 1 ? plan_runs<1>(pairs, max_len, a.row_tiles, num_sms)
+                                     : plan_runs<2>(pairs, max_len, a.row_tiles, num_sms));
   const size_t slots = static_cast<size_t>(a.row_tiles) * (a.runs + pairs);
   auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
-  a.base_off = 0;
-  a.ml_off = up(static_cast<size_t>(a.row_tiles) * (batch + 1) * sizeof(int));
+  a.cuts_off = 0;
+  a.ml_off = up(static_cast<size_t>(a.row_tiles) * a.runs * sizeof(Kv4Cut));
   a.o_off = a.ml_off + up(slots * R * 2 * sizeof(float));
   a.bytes = a.o_off + slots * R * dim * sizeof(float);
   return a;
@@ -692,13 +903,13 @@ AttnPlan attn_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t 
 
 template <typename T, int D, int NT>
 int attn_t(const Kv4AttnParams& p, const AttnPlan& a, cudaStream_t st) {
-  constexpr int smem = kv4_attn_smem<T, D, NT>();
+  constexpr int smem = AttnSmem<D, NT>::kBytes;
   if (!set_smem_limit(kv4_attn_kernel<T, D, NT>, smem)) return FITQ_ERR_CUDA;
-  cudaError_t e = launch_pdl(kv4_attn_kernel<T, D, NT>, dim3(a.runs, a.row_tiles), dim3(kAThreads), smem, st, p);
+  cudaError_t e = launch_pdl(kv4_attn_kernel<T, D, NT>, dim3(a.runs, a.row_tiles), dim3(AttnShape<NT>::kThreads), smem,
+                             st, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
-  e = launch_pdl(kv4_attn_combine_kernel<T, D, NT>, dim3(p.seq.batch * p.seq.kv_heads, a.row_tiles), dim3(128), 0, st,
-                 p, a.runs);
+  e = launch_pdl(kv4_attn_combine_kernel<T, D, NT>, dim3(a.runs, a.cols, a.row_tiles), dim3(32 * kCWarps), 0, st, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   return launch_result();
@@ -706,7 +917,7 @@ int attn_t(const Kv4AttnParams& p, const AttnPlan& a, cudaStream_t st) {
 
 template <typename T, int D>
 int attn_td(const Kv4AttnParams& p, const AttnPlan& a, cudaStream_t st) {
-  return a.nt == 1 ? attn_t<T, D, 1>(p, a, st) : (a.nt == 2 ? attn_t<T, D, 2>(p, a, st) : attn_t<T, D, 4>(p, a, st));
+  return a.nt == 1 ? attn_t<T, D, 1>(p, a, st) : attn_t<T, D, 2>(p, a, st);
 }
 
 }  // namespace
@@ -727,7 +938,7 @@ int launch_kv4_attention(const Kv4Seq& seq, const void* q, int64_t q_stride, con
   p.q_stride = q_stride;
   p.out = out;
   p.pool = static_cast<const uint8_t*>(pool);
-  p.base = reinterpret_cast<int*>(ws + a.base_off);
+  p.cuts = reinterpret_cast<Kv4Cut*>(ws + a.cuts_off);
   p.ml_part = reinterpret_cast<float*>(ws + a.ml_off);
   p.o_part = reinterpret_cast<float*>(ws + a.o_off);
   p.heads = heads;
