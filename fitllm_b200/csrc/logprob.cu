@@ -11,17 +11,22 @@
 // M and log S are kept apart for the backward: their sum would lose the digits
 // that log S carries behind M.
 //
-// logprob_fwd_kernel: a cluster of CTAs shares a row; a thread holds its share
-// in registers (every load issued before the first use), so the row is read
-// once: one pass for the maximum, the sums and the candidates.  Alternatives: the
-// k-th largest of 128 thread-group maxima bounds the k-th largest logit of the
-// CTA's share from below; the few elements at or above it are collected and
-// ranked by (value, index), then the CTAs' lists are ranked together.  Where more
-// elements tie than the list holds, k rounds of a maximum search take over.
+// logprob_fwd_kernel: up to eight CTAs (a cluster) share a row.  Sums are kept
+// relative to a thread's own running maximum and joined over warps, the CTA and
+// the cluster.  Few rows: a thread's share stays in registers, every load issued
+// before the first use.  Many rows: a CTA streams its row, eight 16-byte loads
+// in flight per thread.  Alternatives: the k-th largest of 128 thread-group maxima
+// bounds the k-th largest logit of the CTA's share from below; the few elements at
+// or above it are ranked by (value, index), then the CTAs' lists are ranked together.  Where more elements
+// tie than the list holds, k rounds of a maximum search take over.  A streamed row's
+// bound comes from its first granules, behind which a granule whose maximum reaches
+// it adds to the list on the way; only a list that overflows reads the row again.
 // Bound: HBM (one read) for many rows, latency for few.
 //
 // logprob_bwd_kernel: one read and one write of the row; the up to k + 1 marked
 // elements are rewritten behind a CTA barrier.
+#include <type_traits>
+
 #include "kv4.cuh"
 #include "kernels.cuh"
 
@@ -34,7 +39,24 @@ constexpr int kLpMaxTop = 64;
 constexpr int kLpGroups = 128;  // thread groups whose maxima bound the k-th largest
 constexpr int kLpList = 1024;   // candidates a CTA ranks
 
-__device__ __forceinline__ float exp_approx(float x) { return __expf(x); }
+constexpr float kLog2e = 1.4426950408889634f;
+// Exponents below this weigh exactly 0; the bound keeps a weight of 0 from
+// meeting an exponent of -inf.
+constexpr float kLowest = -1000.f;
+constexpr float kFarBelow = -3.402823466e38f;  // a base that stands for -inf: no finite value is smaller
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// max(d, kLowest) that keeps a NaN.
+__device__ __forceinline__ float bounded(float d) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d), "f"(kLowest));
+  return r;
+}
 
 // Floats in an order that unsigned comparison follows; equal floats get equal
 // values (-0 as 0), every NaN the largest.
@@ -43,24 +65,35 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+// The float of an order value (0 for -0).
+__device__ __forceinline__ float value_of(uint32_t o) {
+  return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
+}
 __device__ __forceinline__ uint64_t key_of(float x, int64_t idx) {
   return (static_cast<uint64_t>(order_of(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(idx));
 }
 
+// A row as 16-byte granules at 16-byte boundaries: the first and the last may hold
+// elements of other rows.
 template <typename T>
 struct Row {
   static constexpr int kVec = 16 / sizeof(T);
-  const T* z;      // first element
-  int64_t lead;    // elements of the first 16-byte granule that lie before it
-  int64_t vectors; // granules that hold the row
-  int64_t V;
-  __device__ __forceinline__ Row(const T* base, int64_t v) : z(base), V(v) {
-    lead = (reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T);
-    vectors = (lead + v + kVec - 1) / kVec;
+  const T* z;          // first element
+  const uint4* frame;  // granule 0
+  int lead;            // elements of granule 0 that lie before the row
+  int vectors;         // granules that hold the row
+  int in_lo, in_hi;    // granules [in_lo, in_hi) lie inside it
+  int V;
+  __device__ __forceinline__ Row(const T* base, int64_t v) : z(base), V(static_cast<int>(v)) {
+    lead = static_cast<int>((reinterpret_cast<uintptr_t>(base) & 15u) / sizeof(T));
+    frame = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(base) & ~static_cast<uintptr_t>(15));
+    vectors = (lead + V + kVec - 1) / kVec;
+    in_lo = lead ? 1 : 0;
+    in_hi = (lead + V) / kVec;
   }
   // index of element 0 of granule i (may be negative for i = 0)
-  __device__ __forceinline__ int64_t first(int64_t i) const { return i * kVec - lead; }
-  __device__ __forceinline__ bool inside(int64_t i) const { return first(i) >= 0 && first(i) + kVec <= V; }
+  __device__ __forceinline__ int first(int i) const { return i * kVec - lead; }
+  __device__ __forceinline__ bool inside(int i) const { return i >= in_lo && i < in_hi; }
 };
 
 template <typename T>
@@ -107,12 +140,12 @@ __device__ __forceinline__ uint4 pack_vec<float>(const float (&f)[4]) {
 
 // Granule i of a row; elements outside the row read as -inf.
 template <typename T>
-__device__ __forceinline__ uint4 load_vec(const Row<T>& r, int64_t i) {
-  if (r.inside(i)) return *reinterpret_cast<const uint4*>(r.z + r.first(i));
+__device__ __forceinline__ uint4 load_vec(const Row<T>& r, int i) {
+  if (r.inside(i)) return r.frame[i];
   float f[Row<T>::kVec];
 #pragma unroll
   for (int j = 0; j < Row<T>::kVec; ++j) {
-    const int64_t e = r.first(i) + j;
+    const int e = r.first(i) + j;
     f[j] = (e >= 0 && e < r.V) ? to_f32<T>(r.z[e]) : -INFINITY;
   }
   return pack_vec<T>(f);
@@ -150,24 +183,48 @@ __device__ __forceinline__ void cluster_arrive() {
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// (m, s, t) = max, sum exp(z - m), sum exp(z - m)(z - m) of two parts joined.
+// (m, s, t): the maximum m, sum exp(d) and sum exp(d) d over d = z - m, of two parts
+// joined.
 __device__ __forceinline__ void join(float& m, float& s, float& t, float m2, float s2, float t2) {
   const float mn = fmaxf(m, m2);
   const float base = mn == -INFINITY ? 0.f : mn;
-  const float d1 = fmaxf(m - base, -1.0e30f), d2 = fmaxf(m2 - base, -1.0e30f);  // -inf parts weigh 0
-  const float k1 = exp_approx(d1), k2 = exp_approx(d2);
+  const float d1 = fmaxf(m - base, kLowest), d2 = fmaxf(m2 - base, kLowest);
+  const float k1 = exp2_approx(d1 * kLog2e), k2 = exp2_approx(d2 * kLog2e);
   t = k1 * fmaf(d1, s, t) + k2 * fmaf(d2, s2, t2);
   s = k1 * s + k2 * s2;
   m = mn;
 }
 
-// kNV > 0: a thread's granules stay in registers; kNV = 0: they are read again.
+// Largest element of a granule; a NaN is passed over.
+template <typename T>
+__device__ __forceinline__ float vec_max(const uint4& u);
+template <>
+__device__ __forceinline__ float vec_max<float>(const uint4& u) {
+  return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+template <>
+__device__ __forceinline__ float vec_max<__nv_bfloat16>(const uint4& u) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+template <>
+__device__ __forceinline__ float vec_max<__half>(const uint4& u) {
+  const __half2* h = reinterpret_cast<const __half2*>(&u);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
+constexpr int kLpUnroll = 8;  // granules in flight per thread of a streamed row, in two halves
+
+// kNV > 0: a thread's granules stay in registers; kNV = 0: they are streamed.
 template <typename T, int kNV, bool kTop>
-__global__ void __launch_bounds__(kLpThreads) logprob_fwd_kernel(const LogprobFwdParams p) {
+__global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const LogprobFwdParams p) {
   constexpr int kVec = Row<T>::kVec;
+  constexpr int kHeld = kNV > 0 ? kNV : kLpUnroll;
   __shared__ float sh_m[kLpWarps], sh_s[kLpWarps], sh_t[kLpWarps];
   __shared__ float sh_part[8][3];  // the cluster's parts, in its first CTA
-  __shared__ uint32_t sh_group[kTop ? kLpGroups : 1];
+  __shared__ __align__(16) uint32_t sh_group[kTop ? kLpGroups : 4];
   __shared__ uint32_t sh_bound;
   __shared__ int sh_count;
   __shared__ uint64_t sh_list[kTop ? kLpList : 1];
@@ -182,78 +239,170 @@ __global__ void __launch_bounds__(kLpThreads) logprob_fwd_kernel(const LogprobFw
   pdl_launch_dependents();
   pdl_wait();  // the logits come from the previous kernel
   const Row<T> r(static_cast<const T*>(p.logits) + row * p.stride, p.V);
-  const int64_t share = (r.vectors + ctas - 1) / ctas;
-  const int64_t v_lo = share * cta, v_hi = v_lo + share < r.vectors ? v_lo + share : r.vectors;
+  const int share = (r.vectors + static_cast<int>(ctas) - 1) / static_cast<int>(ctas);
+  const int v_lo = share * static_cast<int>(cta), v_hi = min(v_lo + share, r.vectors);
 
-  uint4 held[kNV > 0 ? kNV : 1];
-  if (kNV > 0) {
+  uint4 held[kHeld];
+  constexpr int kStep = kLpThreads;  // granules between a thread's own
+  // the given token's logit, fetched early
+  int64_t id = -1;
+  float z_id = 0.f;
+  if (cta == 0 && tid == 0) {
+    id = p.ids[row];
+    if (id >= 0 && id < p.V) z_id = to_f32<T>(r.z[id]);
+  }
+  // granules [from, to) of `held` are the thread's from granule v0 on
+  auto load_held = [&](auto from, auto to, int v0) {
 #pragma unroll
-    for (int i = 0; i < kNV; ++i) {
-      const int64_t v = v_lo + tid + static_cast<int64_t>(i) * kLpThreads;
+    for (int i = from.value; i < to.value; ++i) {
+      const int v = v0 + (i - from.value) * kStep;
       if (v < v_hi) held[i] = load_vec(r, v);
     }
-  }
-  // f(granule index, its elements as floats) over this thread's granules
-  auto each = [&](auto f) {
-    if (kNV > 0) {
+  };
+  // f(granule) over them; a mask of those for which it is true
+  auto for_held = [&](auto from, auto to, int v0, auto f) -> uint32_t {
+    uint32_t mask = 0;
 #pragma unroll
-      for (int i = 0; i < kNV; ++i) {
-        const int64_t v = v_lo + tid + static_cast<int64_t>(i) * kLpThreads;
-        if (v < v_hi) {
-          float x[kVec];
-          unpack_vec<T>(held[i], x);
-          f(v, x);
-        }
-      }
-    } else {
-      for (int64_t v = v_lo + tid; v < v_hi; v += kLpThreads) {
-        float x[kVec];
-        unpack_vec<T>(load_vec(r, v), x);
-        f(v, x);
+    for (int i = from.value; i < to.value; ++i)
+      if (v0 + (i - from.value) * kStep < v_hi && f(held[i])) mask |= 1u << (i - from.value);
+    return mask;
+  };
+  constexpr std::integral_constant<int, 0> k0{};
+  constexpr std::integral_constant<int, kHeld / 2> kHalf{};
+  constexpr std::integral_constant<int, kHeld> kAll{};
+
+  // ---- the elements of a granule that are not below a bound go to the CTA's list
+  auto collect = [&](int v, float bound_f) {
+    float x[kVec];
+    unpack_vec<T>(load_vec(r, v), x);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const int e = r.first(v) + j;
+      if (!(x[j] < bound_f) && e >= 0 && e < r.V) {
+        const int at = atomicAdd(&sh_count, 1);
+        if (at < kLpList) sh_list[at] = key_of(x[j], e);
       }
     }
   };
+  // the same for the granules of a mask (few: they are read again)
+  auto collect_mask = [&](uint32_t mask, int v0, float bound_f) {
+    while (mask) {
+      const int i = __ffs(mask) - 1;
+      mask &= mask - 1;
+      collect(v0 + i * kStep, bound_f);
+    }
+  };
+  // The top-th largest of the thread groups' maxima (equal ones ranked by group), or
+  // -inf where fewer groups have elements: at least `top` elements are not smaller.
+  // Four threads rank a group.
+  auto find_bound = [&](float thread_max) -> float {
+    uint32_t g = (v_lo + tid < v_hi) ? order_of(thread_max) : 0u;  // 0: no element
+    g = max(g, __shfl_xor_sync(0xffffffffu, g, 1));
+    g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+    if ((tid & 3) == 0) sh_group[tid >> 2] = g;
+    if (tid == 0) sh_count = 0;
+    __syncthreads();
+    const uint4* all = reinterpret_cast<const uint4*>(sh_group);
+    const int own = tid >> 2;
+    int rank = 0;
+#pragma unroll
+    for (int i = 0; i < kLpGroups / 16; ++i) {
+      const int at = 4 * (4 * i + (tid & 3));
+      const uint4 o = all[4 * i + (tid & 3)];
+      rank += (o.x > g || (o.x == g && at < own)) + (o.y > g || (o.y == g && at + 1 < own)) +
+              (o.z > g || (o.z == g && at + 2 < own)) + (o.w > g || (o.w == g && at + 3 < own));
+    }
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+    if (rank == p.top - 1) sh_bound = g;
+    __syncthreads();
+    const uint32_t b = sh_bound;
+    return b <= 0x007fffffu ? -INFINITY : value_of(b);
+  };
 
   // ---- maximum and sums of the thread's share
-  float m = -INFINITY, s = 0.f, t = 0.f;
+  float m = -INFINITY, s = 0.f, t = 0.f, base = 0.f;
+  auto add = [&](const uint4& u) {
+    float x[kVec];
+    unpack_vec<T>(u, x);
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      // the difference first: it is exact near the maximum, and the type's lowest
+      // value times log2 e would overflow
+      const float d = bounded(x[j] - base), e = exp2_approx(d * kLog2e);
+      s += e;
+      t = fmaf(e, d, t);
+    }
+  };
+  float bound_f = INFINITY;  // what the alternatives are not smaller than
+  auto reaches = [&](const uint4& u) { return vec_max<T>(u) >= bound_f; };
   if (kNV > 0) {
-    each([&](int64_t, const float (&x)[kVec]) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) m = fmaxf(m, x[j]);
+    load_held(k0, kAll, v_lo + tid);
+    for_held(k0, kAll, v_lo + tid, [&](const uint4& u) {
+      m = fmaxf(m, vec_max<T>(u));
+      return false;
     });
-    const float base = m == -INFINITY ? 0.f : m;
-    each([&](int64_t, const float (&x)[kVec]) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const float d = x[j] - base, e = exp_approx(d);
-        s += e;
-        t = fmaf(e, fmaxf(d, -1.0e30f), t);  // a weight of 0 takes no -inf with it
-      }
+    base = m == -INFINITY ? 0.f : m;
+    for_held(k0, kAll, v_lo + tid, [&](const uint4& u) {
+      add(u);
+      return false;
     });
+    if (kTop) {
+      bound_f = find_bound(m);
+      collect_mask(for_held(k0, kAll, v_lo + tid, reaches), v_lo + tid, bound_f);
+    }
   } else {
-    each([&](int64_t, const float (&x)[kVec]) {
-      float mx = x[0];
-#pragma unroll
-      for (int j = 1; j < kVec; ++j) mx = fmaxf(mx, x[j]);
-      if (mx > m) {
-        join(m, s, t, mx, 0.f, 0.f);
+    // The sums' base only moves when a granule exceeds it by e^20, which they have room
+    // for: moving it for every new maximum would cost a warp most of its granules.  The
+    // first granules give a bound already; behind them a granule whose maximum reaches it
+    // adds its elements on the way.
+    auto stream = [&](const uint4& u) -> bool {
+      const float mx = vec_max<T>(u);
+      m = fmaxf(m, mx);
+      if (mx > base + 20.f) {
+        const float d = fmaxf(base - mx, kLowest), k = exp2_approx(d * kLog2e);
+        t = k * fmaf(d, s, t);
+        s *= k;
+        base = mx;
       }
-      const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const float d = x[j] - base, e = exp_approx(d);
-        s += e;
-        t = fmaf(e, fmaxf(d, -1.0e30f), t);
-      }
-    });
+      add(u);
+      return kTop && mx >= bound_f;
+    };
+    int v0 = v_lo + tid;
+    load_held(k0, kHalf, v0);
+    load_held(kHalf, kAll, v0 + kHalf.value * kStep);
+    if (v0 < v_hi) {
+      const float first = vec_max<T>(held[0]);
+      base = first == -INFINITY ? kFarBelow : first;
+    }
+    if (kTop) {
+      for_held(k0, kHalf, v0, stream);
+      for_held(kHalf, kAll, v0 + kHalf.value * kStep, stream);
+      bound_f = find_bound(m);
+      collect_mask(for_held(k0, kHalf, v0, reaches) |
+                       for_held(kHalf, kAll, v0 + kHalf.value * kStep, reaches) << kHalf.value,
+                   v0, bound_f);
+      v0 += kAll.value * kStep;
+      load_held(k0, kHalf, v0);
+      load_held(kHalf, kAll, v0 + kHalf.value * kStep);
+    }
+    for (; v0 < v_hi; v0 += kAll.value * kStep) {
+      const uint32_t a = for_held(k0, kHalf, v0, stream);
+      load_held(k0, kHalf, v0 + kAll.value * kStep);
+      const uint32_t b = for_held(kHalf, kAll, v0 + kHalf.value * kStep, stream);
+      load_held(kHalf, kAll, v0 + (kAll.value + kHalf.value) * kStep);
+      if (kTop) collect_mask(a | b << kHalf.value, v0, bound_f);
+    }
   }
+  const bool nan_here = s != s;
   const float thread_max = m;
   {
+    // from here on relative to the maximum itself
     float wm = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-    const float base = wm == -INFINITY ? 0.f : wm;
-    const float d = fmaxf(m - base, -1.0e30f), k = exp_approx(d);
+    const float wbase = wm == -INFINITY ? 0.f : wm;
+    const float d = fmaxf(base - wbase, kLowest), k = s == 0.f ? 0.f : exp2_approx(d * kLog2e);
     t = k * fmaf(d, s, t);
     s *= k;
 #pragma unroll
@@ -267,16 +416,9 @@ __global__ void __launch_bounds__(kLpThreads) logprob_fwd_kernel(const LogprobFw
       sh_t[warp] = t;
     }
   }
-  if (kTop) {
-    // the group of four threads' largest element; 0 stands for "no element"
-    uint32_t g = (v_lo + tid < v_hi) ? order_of(thread_max) : 0u;
-    g = max(g, __shfl_xor_sync(0xffffffffu, g, 1));
-    g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
-    if ((tid & 3) == 0) sh_group[tid >> 2] = g;
-    if (tid == 0) sh_count = 0;
-    if (tid < kLpMaxTop) sh_best[tid] = 0;
-  }
-  __syncthreads();
+  if (kTop && tid < kLpMaxTop) sh_best[tid] = 0;
+  // a granule's maximum passes NaNs over: a share that has one is searched again
+  const int nan_seen = kTop ? __syncthreads_or(nan_here) : (__syncthreads(), 0);
   cluster_wait();  // every CTA of the cluster runs
   if (warp == 0) {
     float cm = lane < kLpWarps ? sh_m[lane] : -INFINITY;
@@ -295,52 +437,44 @@ __global__ void __launch_bounds__(kLpThreads) logprob_fwd_kernel(const LogprobFw
     }
   }
   if (kTop) {
-    // ---- bound: the top-th largest group maximum (equal ones ranked by group)
-    if (tid < kLpGroups) {
-      const uint32_t g = sh_group[tid];
-      int rank = 0;
-      for (int i = 0; i < kLpGroups; ++i) {
-        const uint32_t o = sh_group[i];
-        rank += (o > g || (o == g && i < tid)) ? 1 : 0;
-      }
-      if (rank == p.top - 1) sh_bound = g;
+    int count = sh_count;
+    if ((kNV == 0 && count > kLpList) || nan_seen) {  // uniform: once more, with the whole share's bound
+      __syncthreads();
+      bound_f = find_bound(thread_max);
+      for (int v = v_lo + tid; v < v_hi; v += kStep) collect(v, bound_f);
+      __syncthreads();
+      count = sh_count;
     }
-    __syncthreads();
-    const uint32_t bound = sh_bound;
-    each([&](int64_t v, const float (&x)[kVec]) {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const int64_t e = r.first(v) + j;
-        if (order_of(x[j]) >= bound && e >= 0 && e < r.V) {
-          const int at = atomicAdd(&sh_count, 1);
-          if (at < kLpList) sh_list[at] = key_of(x[j], e);
-        }
-      }
-    });
-    __syncthreads();
-    const int count = sh_count;
     if (count <= kLpList) {
-      // the list's order varies, the keys' ranks do not: every key is unique
-      for (int i = tid; i < count; i += kLpThreads) {
-        const uint64_t k = sh_list[i];
+      // the list's order varies, the keys' ranks do not: every key is unique; eight
+      // threads rank a key
+      for (int i0 = 0; i0 < count; i0 += kLpThreads / 8) {
+        const int i = i0 + (tid >> 3);
+        const uint64_t k = i < count ? sh_list[i] : 0;
         int rank = 0;
-        for (int j = 0; j < count && rank < p.top; ++j) rank += sh_list[j] > k ? 1 : 0;
-        if (rank < p.top) sh_best[rank] = k;
+#pragma unroll 4
+        for (int j = tid & 7; j < count; j += 8) rank += sh_list[j] > k ? 1 : 0;
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 4);
+        if (i < count && rank < p.top && (tid & 7) == 0) sh_best[rank] = k;
       }
       __syncthreads();
     } else {
       uint64_t last = ~0ull;
       for (int n = 0; n < p.top; ++n) {
         uint64_t best = 0;
-        each([&](int64_t v, const float (&x)[kVec]) {
+        for (int v = v_lo + tid; v < v_hi; v += kStep) {
+          float x[kVec];
+          unpack_vec<T>(load_vec(r, v), x);
 #pragma unroll
           for (int j = 0; j < kVec; ++j) {
-            const int64_t e = r.first(v) + j;
+            const int e = r.first(v) + j;
             if (e < 0 || e >= r.V) continue;
             const uint64_t k = key_of(x[j], e);
             if (k < last && k > best) best = k;
           }
-        });
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
           const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
@@ -369,25 +503,42 @@ __global__ void __launch_bounds__(kLpThreads) logprob_fwd_kernel(const LogprobFw
   float M = sh_part[0][0], S = sh_part[0][1], E = sh_part[0][2];
   for (uint32_t c = 1; c < ctas; ++c) join(M, S, E, sh_part[c][0], sh_part[c][1], sh_part[c][2]);
   const float log_s = logf(S);
+  if (M == -INFINITY) S = NAN;  // nothing but -inf: no distribution
   if (tid == 0) {
-    const int64_t id = p.ids[row];
     const bool valid = id >= 0 && id < p.V;
-    p.logp[row] = valid ? (to_f32<T>(r.z[id]) - M) - log_s : 0.f;
+    p.logp[row] = valid ? (z_id - M) - log_s : 0.f;
     p.entropy[row] = log_s - E / S;
     p.stats[2 * row] = M;
     p.stats[2 * row + 1] = log_s;
   }
   if (kTop) {
-    const int n = static_cast<int>(ctas) * p.top;
-    for (int i = tid; i < n; i += kLpThreads) {
-      const uint64_t k = sh_all[(i / p.top) * kLpMaxTop + i % p.top];
+    // every list is in order: a key's rank is its place in its own list and the
+    // number of larger keys in each other one
+    for (int i = tid; i < static_cast<int>(ctas) * kLpMaxTop; i += kLpThreads) {
+      const int own = i / kLpMaxTop, place = i % kLpMaxTop;
+      if (place >= p.top) continue;
+      const uint64_t k = sh_all[i];
       if (k == 0) continue;  // no element
-      int rank = 0;
-      for (int j = 0; j < n && rank < p.top; ++j) rank += sh_all[(j / p.top) * kLpMaxTop + j % p.top] > k ? 1 : 0;
+      int rank = place;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (c >= static_cast<int>(ctas) || c == own) continue;
+        int lo = 0, hi = p.top;  // how many keys of list c are larger
+#pragma unroll
+        for (int step = 0; step < 7; ++step) {
+          if (lo >= hi) continue;
+          const int mid = (lo + hi) >> 1;
+          if (sh_all[c * kLpMaxTop + mid] > k)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        rank += lo;
+      }
       if (rank < p.top) {
-        const int64_t e = 0xffffffffu - static_cast<uint32_t>(k);
-        p.top_ids[row * p.top + rank] = e;
-        p.top_logp[row * p.top + rank] = (to_f32<T>(r.z[e]) - M) - log_s;
+        const uint32_t o = static_cast<uint32_t>(k >> 32);
+        p.top_ids[row * p.top + rank] = 0xffffffffu - static_cast<uint32_t>(k);
+        p.top_logp[row * p.top + rank] = ((o == 0xffffffffu ? NAN : value_of(o)) - M) - log_s;
       }
     }
   }
@@ -436,19 +587,19 @@ __global__ void __launch_bounds__(kLbThreads) logprob_bwd_kernel(const LogprobBw
   const float h = p.g_entropy ? p.g_entropy[row] : 0.f;
   auto grad = [&](float z) {
     const float lp = (z - M) - log_s;
-    const float pr = exp_approx(lp);
-    return -pr * (a + h * fmaxf(lp + H, -1.0e30f));  // a probability of 0 takes no -inf with it
+    const float pr = exp2_approx(lp * kLog2e);
+    return -pr * fmaf(h, fmaxf(lp + H, kLowest), a);  // a probability of 0 takes no -inf with it
   };
-  const int64_t v0 = static_cast<int64_t>(part) * (kLbThreads * kLbVectors) + tid;
+  const int v0 = part * (kLbThreads * kLbVectors) + tid;
   uint4 z[kLbVectors];
 #pragma unroll
   for (int i = 0; i < kLbVectors; ++i) {
-    const int64_t v = v0 + i * kLbThreads;
+    const int v = v0 + i * kLbThreads;
     if (aligned && v < out.vectors && out.inside(v)) z[i] = *reinterpret_cast<const uint4*>(zrow + out.first(v));
   }
 #pragma unroll
   for (int i = 0; i < kLbVectors; ++i) {
-    const int64_t v = v0 + i * kLbThreads;
+    const int v = v0 + i * kLbThreads;
     if (v >= out.vectors) continue;
     if (aligned && out.inside(v)) {
       float x[kVec];
@@ -502,15 +653,14 @@ int fwd_t(const LogprobFwdParams& p, int64_t rows, int ctas, cudaStream_t st) {
 template <typename T>
 int fwd_sized(const LogprobFwdParams& p, int64_t rows, cudaStream_t st, int num_sms) {
   const int64_t vectors = (p.V * static_cast<int64_t>(sizeof(T)) + 15) / 16 + 1;
-  // Few rows: up to eight CTAs of a row run on SMs of their own; many rows: as few
-  // CTAs as hold the row in registers.
+  // As many CTAs per row (up to eight) as find room at once, two on an SM, and work
+  // for every thread: one row of 152,064 bf16 logits takes 8 CTAs, rows from about 300
+  // on one each.
   int ctas = 1;
-  const int64_t want = rows * 4 < num_sms ? 2 : 8;  // granules per thread
-  while (ctas < 8 && vectors > want * kLpThreads * ctas) ctas *= 2;
+  while (ctas < 8 && rows * ctas * 2 <= 2ll * num_sms && vectors > kLpThreads * ctas) ctas *= 2;
   const int64_t per = (vectors + ctas - 1) / ctas;
   if (per <= 2 * kLpThreads) return fwd_t<T, 2>(p, rows, ctas, st);
   if (per <= 5 * kLpThreads) return fwd_t<T, 5>(p, rows, ctas, st);
-  if (per <= 10 * kLpThreads) return fwd_t<T, 10>(p, rows, ctas, st);
   return fwd_t<T, 0>(p, rows, ctas, st);
 }
 
