@@ -1484,7 +1484,7 @@ int fitq_token_logprobs(const void* logits, int dtype, const int64_t* ids, int64
   if (rows < 0) return fail(FITQ_ERR_SHAPE, "token_logprobs: rows=%lld", (long long)rows);
   int rc = logprob_shape("token_logprobs", logits, dtype, ids, rows, vocab, stride, top);
   if (rc) return rc;
-  if (!logp || !entropy || !stats || (top > 0 && (!top_logp || !top_ids)))
+  if (!logp || !entropy || (top > 0 && (!top_logp || !top_ids)))
     return fail(FITQ_ERR_ARG, "token_logprobs: NULL output");
   const int sms = current_sms(&rc);
   if (!sms) return rc;

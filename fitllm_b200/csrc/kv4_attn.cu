@@ -37,6 +37,10 @@
 // lies in one run is written out; one cut between runs leaves partials that
 // kv4_attn_combine_kernel joins in run order (deterministic).
 //
+// Few pairs of few positions (a single sequence's decode step) take the same kernel
+// in clusters: eight CTAs share a pair's tiles and join their parts over distributed
+// shared memory, one launch without partials in HBM and without the list.
+//
 // Bound: HBM, 18 D / 16 B per position and KV head.
 #include <type_traits>
 
@@ -202,7 +206,29 @@ __device__ __forceinline__ int pair_cost(const SeqSpan& sp) { return sp.tiles ? 
 
 extern __shared__ __align__(128) uint8_t g_kv4_smem[];
 
-template <typename T, int D, int NT>
+constexpr int kCluster = 8;  // CTAs per pair of a cluster launch
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Four floats of the same shared-memory address in another CTA of the cluster.
+__device__ __forceinline__ float4 peer_float4(const float* p, uint32_t rank) {
+  uint32_t a;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+
+template <typename T, int D, int NT, bool kClustered>
 __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     kv4_attn_kernel(const Kv4AttnParams p) {
   using S = AttnShape<NT>;
@@ -241,6 +267,16 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   pdl_wait();  // q and the cache append come from the previous kernels
 
   const Kv4Seq& s = p.seq;
+  // a negative prefix, positions outside the table, more columns than the launch covers
+  auto check_sequence = [&](const SeqSpan& sp) {
+    if (sp.count > 0 &&
+        (sp.pre < 0 || static_cast<int64_t>(sp.pre) + sp.count > (static_cast<int64_t>(s.max_pages) << s.page_shift) ||
+         static_cast<int64_t>(sp.count) * p.group > static_cast<int64_t>(gridDim.y) * R))
+      report_device_error(p.status, FITQ_ERR_ARG);
+  };
+  uint32_t total = 0, per = 0, t_lo = 0, t_hi = 0;
+  Kv4Cut* cut = p.cuts + blockIdx.y * gridDim.x + blockIdx.x;  // the pair that this run opens and does not finish
+  if (!kClustered) {
   // ---- the list of pairs in units of cost: every thread sums a run of sequences, then a scan
   const int per_thread = (s.batch + kThreads - 1) / kThreads;
   const int b_lo = tid * per_thread, b_hi = b_lo + per_thread < s.batch ? b_lo + per_thread : s.batch;
@@ -262,11 +298,11 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     all += v;
   }
   // (the host has checked that the list's length fits in 31 bits)
-  const uint32_t total = static_cast<uint32_t>(all) * s.kv_heads;
-  const uint32_t per = (total + gridDim.x - 1) / gridDim.x;  // cost of a run
-  const uint32_t t_lo = per * blockIdx.x, t_hi = t_lo + per < total ? t_lo + per : total;
-  Kv4Cut* cut = p.cuts + blockIdx.y * gridDim.x + blockIdx.x;  // the pair that this run opens and does not finish
-  if (tid == 0) cut->count = 0;
+  total = static_cast<uint32_t>(all) * s.kv_heads;
+  per = (total + gridDim.x - 1) / gridDim.x;  // cost of a run
+  t_lo = per * blockIdx.x;
+  t_hi = t_lo + per < total ? t_lo + per : total;
+  if (!kClustered && tid == 0) cut->count = 0;
   {
     int at = before;
     for (int b = b_lo; b < b_hi; ++b) {
@@ -278,16 +314,13 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
         sh_b = b;
         sh_base = at;
       }
-      // a negative prefix, positions outside the table, more columns than the launch covers
-      if (blockIdx.x == 0 && blockIdx.y == 0 && sp.count > 0 &&
-          (sp.pre < 0 || static_cast<int64_t>(sp.pre) + sp.count > (static_cast<int64_t>(s.max_pages) << s.page_shift) ||
-           static_cast<int64_t>(sp.count) * p.group > static_cast<int64_t>(gridDim.y) * R))
-        report_device_error(p.status, FITQ_ERR_ARG);
+      if (blockIdx.x == 0 && blockIdx.y == 0) check_sequence(sp);
       at += cost;
     }
   }
   __syncthreads();
   if (t_lo >= t_hi) return;
+  }
 
   // ---- the run's segments, found by thread 0 one ahead of their use
   auto advance = [&](Segment& g) {
@@ -320,12 +353,26 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     sh_walk_b = b;
   };
   if (tid == 0) {
-    sh_walk_t = t_lo;
-    sh_walk_t0 = static_cast<uint32_t>(sh_base) * s.kv_heads;
-    sh_walk_b = sh_b;
-    advance(sh_seg[0]);
+    if (kClustered) {  // the CTA's share of its cluster's pair, and nothing behind it
+      Segment& g = sh_seg[0];
+      const int pair = static_cast<int>(blockIdx.x) / kCluster, rank = static_cast<int>(blockIdx.x) % kCluster;
+      g.b = pair / s.kv_heads;
+      g.kvh = pair % s.kv_heads;
+      g.sp = seq_span(s, g.b, p.group, col0, R, kTile);
+      const int share = (g.sp.tiles + kCluster - 1) / kCluster;
+      g.ta = min(rank * share, g.sp.tiles);
+      g.tb = min(g.ta + share, g.sp.tiles);
+      sh_seg[1].tb = 0;
+      if (rank == 0 && g.kvh == 0 && blockIdx.y == 0) check_sequence(g.sp);
+    } else {
+      sh_walk_t = t_lo;
+      sh_walk_t0 = static_cast<uint32_t>(sh_base) * s.kv_heads;
+      sh_walk_b = sh_b;
+      advance(sh_seg[0]);
+    }
   }
   __syncthreads();
+  if (kClustered && sh_seg[0].sp.cols == 0) return;  // the whole cluster
 
   const int64_t slot0 = static_cast<int64_t>(blockIdx.y) * (gridDim.x + static_cast<int64_t>(s.batch) * s.kv_heads);
   uint32_t issued = 0, taken = 0;  // this warp's copies so far
@@ -436,9 +483,10 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   look_up(sh_seg[0], 0);
   start(sh_seg[0]);
   load_queries(sh_seg[0], g_kv4_smem + L::kQ);
-  if (tid == 0) advance(sh_seg[1]);
+  if (!kClustered && tid == 0) advance(sh_seg[1]);
   int buf = 0;
-  for (int seg = 0, after = 1; sh_seg[seg].tb > 0; seg = after, after = after == 2 ? 0 : after + 1) {
+  // a clustered CTA without tiles of its own still joins the others'
+  for (int seg = 0, after = 1; kClustered || sh_seg[seg].tb > 0; seg = after, after = after == 2 ? 0 : after + 1) {
     const Segment& sg = sh_seg[seg];
     const Segment& sn = sh_seg[after];
     const int pos_first = first_position(sg), blocks = block_count(sg), len = sg.sp.len;
@@ -448,7 +496,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     const float* sqexp = reinterpret_cast<const float*>(sq_now + L::kQexp);
     buf ^= 1;
     __syncthreads();  // the queries are there, the merge buffer and the last segment's place are free
-    if (tid == 0) advance(sh_seg[after == 2 ? 0 : after + 1]);
+    if (!kClustered && tid == 0) advance(sh_seg[after == 2 ? 0 : after + 1]);
     uint4 qf[kQRegs ? G : 1][2];
     if (kQRegs) {
 #pragma unroll
@@ -706,7 +754,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     for (int j = inner; j < blocks && fine; ++j) fine = block(j, std::true_type{});
 
     // ---- the next segment's copies and queries set out before the warps meet
-    if (sn.tb > 0 && fine) {
+    if (!kClustered && sn.tb > 0 && fine) {
       look_up(sn, 0);
       start(sn);
       load_queries(sn, g_kv4_smem + L::kQ + buf * L::kQBytes);
@@ -744,7 +792,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     const SeqSpan sp = sg.sp;
     const int b = sg.b, kvh = sg.kvh;
     const bool whole = sg.ta == 0 && sg.tb == sp.tiles;
-    if (tid == 0 && sg.ta == 0 && !whole) {
+    if (!kClustered && tid == 0 && sg.ta == 0 && !whole) {
       // this run opens the pair; the last of its other tiles lies `rest` of cost behind the run's end
       const uint32_t rest = sp.tiles - sg.tb - 1;
       *cut = Kv4Cut{b, kvh, static_cast<int>(2 + rest / per)};
@@ -768,7 +816,13 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
 #pragma unroll
         for (int x = 0; x < 8; ++x) f[x] = fmaf(k, row[x], f[x]);
       }
-      if (whole) {
+      if (kClustered) {  // where the ring was: its copies have all been consumed
+        float* dst = reinterpret_cast<float*>(g_kv4_smem) + n * D + d0;
+        *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        if (d0 == 0) *reinterpret_cast<float4*>(reinterpret_cast<float*>(g_kv4_smem) + R * D + n * 4) =
+            make_float4(mx, l, 0.f, 0.f);
+      } else if (whole) {
         const float inv = 1.f / l;
 #pragma unroll
         for (int x = 0; x < 8; ++x) f[x] = l == 0.f ? 0.f : f[x] * inv;
@@ -781,6 +835,44 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
         *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
         if (d0 == 0) *reinterpret_cast<float2*>(p.ml_part + (slot * R + n) * 2) = make_float2(mx, l);
       }
+    }
+    if (kClustered) {
+      cluster_barrier();
+      // every CTA writes its share of the columns' elements
+      const float* own_o = reinterpret_cast<const float*>(g_kv4_smem);
+      const int rank = static_cast<int>(cluster_rank());
+      for (int i = tid * kCluster + rank; i < sp.cols * (D / 4); i += kThreads * kCluster) {
+        const int n = i / (D / 4), d0 = (i % (D / 4)) * 4;
+        float4 ml[kCluster], v[kCluster];
+        float mx = kFloor;
+#pragma unroll
+        for (int c = 0; c < kCluster; ++c) {
+          ml[c] = peer_float4(own_o + R * D + n * 4, c);
+          v[c] = peer_float4(own_o + n * D + d0, c);
+        }
+#pragma unroll
+        for (int c = 0; c < kCluster; ++c) mx = fmaxf(mx, ml[c].x);
+        float l = 0.f;
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < kCluster; ++c) {
+          if (ml[c].y == 0.f) continue;
+          const float k = exp2_approx(ml[c].x - mx);
+          l += k * ml[c].y;
+          f.x = fmaf(k, v[c].x, f.x);
+          f.y = fmaf(k, v[c].y, f.y);
+          f.z = fmaf(k, v[c].z, f.z);
+          f.w = fmaf(k, v[c].w, f.w);
+        }
+        const float inv = 1.f / l;
+        const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
+        T* dst = static_cast<T*>(p.out) + ((sp.first + tok) * p.heads + kvh * p.group + hd) * D + d0;
+        *reinterpret_cast<uint2*>(dst) =
+            l == 0.f ? make_uint2(0u, 0u)
+                     : make_uint2(Half16<T>::pack(f.x * inv, f.y * inv), Half16<T>::pack(f.z * inv, f.w * inv));
+      }
+      cluster_barrier();  // the parts stay until every CTA has read them
+      break;
     }
     if (sh_abort) break;
   }
@@ -869,7 +961,7 @@ int col_tiles(int group, int64_t max_new) {
 }
 
 struct AttnPlan {
-  int nt, row_tiles, cols, runs;  // cols: columns of the fullest row tile
+  int nt, row_tiles, cols, runs;  // cols: columns of the fullest row tile; runs = 0: clusters
   size_t cuts_off, ml_off, o_off, bytes;
 };
 
@@ -892,6 +984,15 @@ AttnPlan attn_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t 
   const int64_t pairs = static_cast<int64_t>(batch) * kv_heads;
   a.runs = static_cast<int>(a.nt == 1 ? plan_runs<1>(pairs, max_len, a.row_tiles, num_sms)
                                      : plan_runs<2>(pairs, max_len, a.row_tiles, num_sms));
+  // Clusters: all of them on the card at once, and no CTA with more than eight tiles.
+  const int64_t slots_at_once = static_cast<int64_t>(num_sms) * (a.nt == 1 ? AttnShape<1>::kCtas : AttnShape<2>::kCtas);
+  const int tile = a.nt == 1 ? AttnShape<1>::kTile : AttnShape<2>::kTile;
+  if (pairs * kCluster * a.row_tiles <= slots_at_once && max_len <= 8ll * kCluster * tile) {
+    a.runs = 0;
+    a.cuts_off = a.ml_off = a.o_off = 0;
+    a.bytes = 16;
+    return a;
+  }
   const size_t slots = static_cast<size_t>(a.row_tiles) * (a.runs + pairs);
   auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
   a.cuts_off = 0;
@@ -904,9 +1005,30 @@ AttnPlan attn_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t 
 template <typename T, int D, int NT>
 int attn_t(const Kv4AttnParams& p, const AttnPlan& a, cudaStream_t st) {
   constexpr int smem = AttnSmem<D, NT>::kBytes;
-  if (!set_smem_limit(kv4_attn_kernel<T, D, NT>, smem)) return FITQ_ERR_CUDA;
-  cudaError_t e = launch_pdl(kv4_attn_kernel<T, D, NT>, dim3(a.runs, a.row_tiles), dim3(AttnShape<NT>::kThreads), smem,
-                             st, p);
+  if (a.runs == 0) {
+    auto* kernel = kv4_attn_kernel<T, D, NT, true>;
+    if (!set_smem_limit(kernel, smem)) return FITQ_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.seq.batch * p.seq.kv_heads * kCluster, a.row_tiles);
+    cfg.blockDim = dim3(AttnShape<NT>::kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    note_launch();
+    if (e != cudaSuccess) return FITQ_ERR_CUDA;
+    return launch_result();
+  }
+  auto* kernel = kv4_attn_kernel<T, D, NT, false>;
+  if (!set_smem_limit(kernel, smem)) return FITQ_ERR_CUDA;
+  cudaError_t e = launch_pdl(kernel, dim3(a.runs, a.row_tiles), dim3(AttnShape<NT>::kThreads), smem, st, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   e = launch_pdl(kv4_attn_combine_kernel<T, D, NT>, dim3(a.runs, a.cols, a.row_tiles), dim3(32 * kCWarps), 0, st, p);

@@ -158,7 +158,7 @@ struct LogprobFwdParams {
   int top;
   float* logp;     // [rows]
   float* entropy;  // [rows]
-  float* stats;    // [rows, 2]: M, log S
+  float* stats;    // [rows, 2]: M, log S; may be null
   float* top_logp; // [rows, top]
   int64_t* top_ids;
 };
@@ -508,8 +508,10 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const Logpro
     const bool valid = id >= 0 && id < p.V;
     p.logp[row] = valid ? (z_id - M) - log_s : 0.f;
     p.entropy[row] = log_s - E / S;
-    p.stats[2 * row] = M;
-    p.stats[2 * row + 1] = log_s;
+    if (p.stats) {
+      p.stats[2 * row] = M;
+      p.stats[2 * row + 1] = log_s;
+    }
   }
   if (kTop) {
     // every list is in order: a key's rank is its place in its own list and the

@@ -41,23 +41,30 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _logprobs_forward(logits, ids, top: int, want_stats: bool):
+    """(logp, entropy, top_logp, top_ids, stats) of logits [rows, V] (fitq_token_logprobs)."""
+    L = _lib.load()
+    dev = logits.device
+    rows, vocab = logits.shape
+    logp = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy = torch.empty_like(logp)
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=dev) if want_stats else None
+    top_logp = torch.empty(rows, top, dtype=torch.float32, device=dev)
+    top_ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
+    with ops._on(dev):
+        _lib.check(L.fitq_token_logprobs(logits.data_ptr(), _LOGIT_DTYPES[logits.dtype], ids.data_ptr(), rows,
+                                         vocab, _row_stride(logits), top, logp.data_ptr(), entropy.data_ptr(),
+                                         _lib.ptr(stats), top_logp.data_ptr(), top_ids.data_ptr(),
+                                         ops._raw_stream(dev.index)), "fitq_token_logprobs")
+    return logp, entropy, top_logp, top_ids, stats
+
+
 class _TokenLogProbsFn(torch.autograd.Function):
     """fitq_token_logprobs / fitq_token_logprobs_bwd over logits [rows, V]."""
 
     @staticmethod
     def forward(ctx, logits, ids, top: int):
-        L = _lib.load()
-        dev = logits.device
-        rows, vocab = logits.shape
-        f32 = dict(dtype=torch.float32, device=dev)
-        logp, entropy = torch.empty(rows, **f32), torch.empty(rows, **f32)
-        stats, top_logp = torch.empty(rows, 2, **f32), torch.empty(rows, top, **f32)
-        top_ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
-        with torch.cuda.device(dev):
-            _lib.check(L.fitq_token_logprobs(logits.data_ptr(), _LOGIT_DTYPES[logits.dtype], ids.data_ptr(), rows,
-                                             vocab, _row_stride(logits), top, logp.data_ptr(), entropy.data_ptr(),
-                                             stats.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr(),
-                                             ops._stream(dev)), "fitq_token_logprobs")
+        logp, entropy, top_logp, top_ids, stats = _logprobs_forward(logits, ids, top, True)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(top_ids)
         ctx.save_for_backward(logits, ids, stats, entropy, top_ids)
@@ -73,12 +80,12 @@ class _TokenLogProbsFn(torch.autograd.Function):
         top = top_ids.shape[1]
         g_logp, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logp, g_entropy, g_top))
         d = torch.empty(rows, vocab, dtype=logits.dtype, device=dev)
-        with torch.cuda.device(dev):
+        with ops._on(dev):
             _lib.check(L.fitq_token_logprobs_bwd(logits.data_ptr(), _LOGIT_DTYPES[logits.dtype], ids.data_ptr(),
                                                  rows, vocab, _row_stride(logits), top, stats.data_ptr(),
                                                  entropy.data_ptr(), top_ids.data_ptr(), _lib.ptr(g_logp),
                                                  _lib.ptr(g_entropy), _lib.ptr(g_top if top else None),
-                                                 d.data_ptr(), ops._stream(dev)), "fitq_token_logprobs_bwd")
+                                                 d.data_ptr(), ops._raw_stream(dev.index)), "fitq_token_logprobs_bwd")
         return d, None, None
 
 
@@ -103,7 +110,12 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tok
     if (vocab > 1 and z.stride(1) != 1) or (z.shape[0] > 1 and z.stride(0) < vocab):
         z = z.contiguous()
     lead = ids.shape
-    r = _TokenLogProbsFn.apply(z, ids.reshape(-1).to(torch.int64).contiguous(), int(top))
+    if len(lead) != 1 or ids.dtype != torch.int64 or not ids.is_contiguous():
+        ids = ids.reshape(-1).to(torch.int64).contiguous()
+    if z.requires_grad and torch.is_grad_enabled():
+        r = _TokenLogProbsFn.apply(z, ids, int(top))
+    else:
+        r = _logprobs_forward(z, ids, int(top), False)[:4]
     if len(lead) == 1:
         return TokenLogProbs(*r)
     return TokenLogProbs(r[0].view(lead), r[1].view(lead), r[2].view(*lead, top), r[3].view(*lead, top))

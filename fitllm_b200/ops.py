@@ -4,6 +4,7 @@ device tensors out; every call is asynchronous on the current CUDA stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import List, Optional, Tuple
 
@@ -15,6 +16,9 @@ from .nf4 import Nf4WeightCRef, QuantState
 
 def _stream(dev) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # handle of a device's current stream, without a Stream object
 
 
 def _bf16_2d(t: torch.Tensor, cols: int) -> torch.Tensor:
@@ -279,6 +283,15 @@ def _kv4_out(what: str, name: str, out: Optional[torch.Tensor], shape, dtype, de
     return out
 
 
+def _on(dev: torch.device):
+    """torch.cuda.device(dev), or nothing where dev is current already (a decode
+    step's calls are bound by the host)."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+_HERE = contextlib.nullcontext()
+
+
 def kv4_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
                prefix: torch.Tensor, cos_half: torch.Tensor, sin_half: torch.Tensor,
                q_start: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -302,10 +315,10 @@ def kv4_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool: torch.Te
     if sin_half.shape != cos_half.shape:
         raise ValueError("kv4_append: cos_half and sin_half differ in shape")
     out = _kv4_out("kv4_append", "q_out", q_out, q.shape, q.dtype, dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.check(L.fitq_kv4_append(c, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(),
                                      v.stride(0), out.data_ptr(), cos_half.data_ptr(), sin_half.data_ptr(),
-                                     cos_half.shape[0], q.shape[1], _KV4_DTYPES[q.dtype], _stream(dev)),
+                                     cos_half.shape[0], q.shape[1], _KV4_DTYPES[q.dtype], _raw_stream(dev.index)),
                    "fitq_kv4_append")
     return out
 
@@ -322,8 +335,8 @@ def kv4_gather(pool: torch.Tensor, page_table: torch.Tensor, prefix: torch.Tenso
         raise ValueError(f"kv4_gather: dtype must be bf16 or fp16 (got {dtype})")
     k = torch.empty(int(tokens), c.kv_heads, c.head_dim, dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    with torch.cuda.device(dev):
-        _lib.check(L.fitq_kv4_gather(c, k.data_ptr(), v.data_ptr(), _KV4_DTYPES[dtype], _stream(dev)),
+    with _on(dev):
+        _lib.check(L.fitq_kv4_gather(c, k.data_ptr(), v.data_ptr(), _KV4_DTYPES[dtype], _raw_stream(dev.index)),
                    "fitq_kv4_gather")
     return k, v
 
@@ -349,12 +362,12 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
     if max_len is None:
         max_len = c.max_pages * c.page_size
     out = _kv4_out("kv4_attention", "out", out, q.shape, q.dtype, dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         nbytes = L.fitq_kv4_attention_workspace(c, q.shape[1], max_new, max_len)
         ws = _workspace(nbytes, dev)
         _lib.check(L.fitq_kv4_attention(c, q.data_ptr(), q.stride(0), out.data_ptr(), q.shape[1],
                                         _KV4_DTYPES[q.dtype], max_new, max_len, ws.data_ptr(), nbytes,
-                                        _stream(dev)), "fitq_kv4_attention")
+                                        _raw_stream(dev.index)), "fitq_kv4_attention")
     return out
 
 

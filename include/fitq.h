@@ -400,7 +400,7 @@ FITQ_API int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_
  * logits [rows, vocab] of dtype (bf16, fp16, fp32), `stride` elements from row to
  * row; ids int64 [rows], an id outside [0, vocab) gives logp 0 and no gradient;
  * 0 <= top <= 64, top <= vocab.  logp, entropy fp32 [rows]; stats fp32 [rows, 2]
- * (row maximum and log of the sum behind it) for the backward; top_logp fp32,
+ * (row maximum and log of the sum behind it) for the backward, or NULL; top_logp fp32,
  * top_ids int64 [rows, top], largest logit first, the lower index where two are
  * equal, a NaN before all.  -inf logits have probability 0; a row of nothing else
  * gives NaN.  The backward writes d [rows, vocab] (dtype, contiguous) from the
