@@ -12,7 +12,10 @@
 // reach gets a non-finite scale and reads back as NaN.
 //
 // Bound: HBM (q, k, v in, q and the blocks out) for prompts, the launch for a
-// decode step.
+// decode step.  A CTA takes up to four tokens: their places (sequence, position,
+// page: a chain of dependent loads) are found once, by one thread each, while the
+// first heads are already on their way, and each team of lanes loads its next head
+// before it works on the current one.
 #include "kv4.cuh"
 #include "kernels.cuh"
 
@@ -43,68 +46,96 @@ struct Kv4AppendParams {
   Kv4Seq seq;
 };
 
-// Eight codes of x under (low, inv), packed low nibble first.
+// Eight codes of x under (low, inv), packed low nibble first.  A sum with 1.5 * 2^23
+// rounds to the nearest whole number, ties to even, and leaves it in the low bits;
+// the eight words add up to the codes plus a constant.
 __device__ __forceinline__ uint32_t code8(const float (&x)[8], float low, float inv) {
-  uint32_t w = 0;
+  constexpr uint32_t kBias = 0x4B400000u;  // the bits of 1.5 * 2^23
+  uint32_t w = 0, shifted = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    int c = __float2int_rn(__fmul_rn(__fsub_rn(x[i], low), inv));
-    c = c < 0 ? 0 : (c > 15 ? 15 : c);
-    w |= static_cast<uint32_t>(c) << (4 * i);
+    const float c = fminf(fmaxf(__fmul_rn(__fsub_rn(x[i], low), inv), 0.f), 15.f);
+    w += __float_as_uint(__fadd_rn(c, 12582912.f)) << (4 * i);
+    shifted += kBias << (4 * i);
   }
-  return w;
+  return w - shifted;
 }
 
-// One CTA per token (blockIdx.x) and share of its head slots (blockIdx.y); a
-// team of D / 16 lanes holds one head: lane i elements 8 i .. 8 i + 7 of each
-// half, so the rotation pairs meet in one lane and the group extrema take
-// log2(team) shuffles.
-template <typename T, int D>
-__global__ void __launch_bounds__(kAppThreads) kv4_append_kernel(const Kv4AppendParams p) {
-  constexpr int kTeam = D / 16;
-  constexpr int kTeams = kAppThreads / kTeam;
-  constexpr int kHalf = D / 2;
-  const int lane = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
-  pdl_launch_dependents();
-  pdl_wait();  // q, k, v come from the previous kernel
-  const int64_t n = blockIdx.x;
-  const Kv4Seq& s = p.seq;
+constexpr int kAppTokens = 4;  // tokens of a CTA, at most
+
+// Where a new token goes: its sequence's page and position; page < -1: no sequence,
+// -1: refused.
+struct TokenPlace {
+  int page, pos;
+};
+__device__ __forceinline__ TokenPlace token_place(const Kv4Seq& s, int64_t n, int limit, int* status) {
+  TokenPlace r{-2, 0};
+  if (n >= s.tokens) return r;
   const int b = kv4_sequence(s, n);
-  if (b < 0) return;  // a token of no sequence: left as it is
+  if (b < 0) return r;  // a token of no sequence: left as it is
   const int64_t first = s.q_start ? s.q_start[b] : static_cast<int64_t>(b) * s.t_new;
   const int pre = s.prefix[b];
   const int64_t pos = pre + (n - first);
-  const int pg = pre < 0 ? -1 : kv4_page(s, b, pos);
-  const bool ok = pg >= 0 && pos < p.rope_len;
-  if (!ok && threadIdx.x == 0) report_device_error(p.status, FITQ_ERR_ARG);
-  float c[8], sv[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = sv[i] = 0.f;  // a refused token's query reads as zeros
-  if (ok) {
-    const float4* cp = reinterpret_cast<const float4*>(p.cs + pos * kHalf + lane * 8);
-    const float4* sp = reinterpret_cast<const float4*>(p.sn + pos * kHalf + lane * 8);
-    const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
-    c[0] = c0.x; c[1] = c0.y; c[2] = c0.z; c[3] = c0.w; c[4] = c1.x; c[5] = c1.y; c[6] = c1.z; c[7] = c1.w;
-    sv[0] = s0.x; sv[1] = s0.y; sv[2] = s0.z; sv[3] = s0.w; sv[4] = s1.x; sv[5] = s1.y; sv[6] = s1.z; sv[7] = s1.w;
-  }
+  r.page = (pre < 0 || pos >= limit) ? -1 : kv4_page(s, b, pos);
+  r.pos = r.page < 0 ? 0 : static_cast<int>(pos);
+  if (r.page < 0) report_device_error(status, FITQ_ERR_ARG);
+  return r;
+}
+
+// A CTA's heads (q, then k, then v slots of each of its tokens) go round its teams
+// of D / 16 lanes (blockIdx.y: one of several CTAs of the same tokens).  Lane i of a
+// team holds elements 8 i .. 8 i + 7 of each half of the head, so the rotation pairs
+// meet in one lane and the group extrema take log2(team) shuffles.
+template <typename T, int D>
+__global__ void __launch_bounds__(kAppThreads, 3) kv4_append_kernel(const Kv4AppendParams p, int per_cta) {
+  constexpr int kTeam = D / 16;
+  constexpr int kTeams = kAppThreads / kTeam;
+  constexpr int kHalf = D / 2;
+  __shared__ TokenPlace sh_place[kAppTokens];
+  const int lane = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
+  pdl_launch_dependents();
+  pdl_wait();  // q, k, v come from the previous kernel
+  const Kv4Seq& s = p.seq;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * per_cta;
   const int slots = p.heads + 2 * s.kv_heads;
-  const int bp = static_cast<int>(pos & 15);
-  for (int s0 = blockIdx.y * kTeams; s0 < slots; s0 += gridDim.y * kTeams) {
-    const int slot = s0 + team;
-    const bool is_q = slot < p.heads, is_k = !is_q && slot < p.heads + s.kv_heads;
-    const bool is_kv = slot >= p.heads && slot < slots;
-    const int kh = is_k ? slot - p.heads : slot - p.heads - s.kv_heads;
+  const int items = static_cast<int>(n0 + per_cta <= s.tokens ? per_cta : s.tokens - n0) * slots;
+  const int step = kTeams * gridDim.y;
+
+  uint4 ra = make_uint4(0, 0, 0, 0), rb = ra;  // this lane's elements of the next head
+  auto fetch = [&](int item) {
+    if (item >= items) return;
+    const int tok = item / slots, slot = item - tok * slots;
+    const int64_t n = n0 + tok;
+    const T* src = slot < p.heads ? static_cast<const T*>(p.q) + n * p.q_stride + slot * D
+                   : slot < p.heads + s.kv_heads
+                       ? static_cast<const T*>(p.k) + n * p.k_stride + (slot - p.heads) * D
+                       : static_cast<const T*>(p.v) + n * p.v_stride + (slot - p.heads - s.kv_heads) * D;
+    ra = *reinterpret_cast<const uint4*>(src + lane * 8);
+    rb = *reinterpret_cast<const uint4*>(src + kHalf + lane * 8);
+  };
+  int item = blockIdx.y * kTeams + team;
+  fetch(item);
+  if (threadIdx.x < per_cta) sh_place[threadIdx.x] = token_place(s, n0 + threadIdx.x, p.rope_len, p.status);
+  __syncthreads();
+
+  for (int i0 = blockIdx.y * kTeams; i0 < items; i0 += step, item += step) {
+    const bool have = item < items;
+    const int tok = have ? item / slots : 0, slot = have ? item - tok * slots : 0;
+    const TokenPlace at = sh_place[tok];
+    const bool ok = have && at.page >= 0;
+    const bool is_q = have && slot < p.heads;
+    const bool is_kv = have && !is_q;
+    const bool is_k = is_kv && slot < p.heads + s.kv_heads;
     float a[8], bb[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = bb[i] = 0.f;
-    if (slot < slots) {
-      const T* src = is_q ? static_cast<const T*>(p.q) + n * p.q_stride + slot * D
-                          : (is_k ? static_cast<const T*>(p.k) + n * p.k_stride
-                                  : static_cast<const T*>(p.v) + n * p.v_stride) + kh * D;
-      unpack8<T>(*reinterpret_cast<const uint4*>(src + lane * 8), a);
-      unpack8<T>(*reinterpret_cast<const uint4*>(src + kHalf + lane * 8), bb);
-    }
+    unpack8<T>(ra, a);
+    unpack8<T>(rb, bb);
+    fetch(item + step);
     if (is_q || is_k) {
+      const float4* cp = reinterpret_cast<const float4*>(p.cs + static_cast<int64_t>(at.pos) * kHalf + lane * 8);
+      const float4* sp = reinterpret_cast<const float4*>(p.sn + static_cast<int64_t>(at.pos) * kHalf + lane * 8);
+      const float4 c0 = cp[0], c1 = cp[1], s0 = sp[0], s1 = sp[1];
+      const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      const float sv[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float x = a[i], y = bb[i];
@@ -112,14 +143,11 @@ __global__ void __launch_bounds__(kAppThreads) kv4_append_kernel(const Kv4Append
         bb[i] = __fadd_rn(__fmul_rn(y, c[i]), __fmul_rn(x, sv[i]));
       }
     }
-    if (is_q) {
-      if (!ok) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = bb[i] = 0.f;
-      }
-      T* dst = static_cast<T*>(p.q_out) + (n * p.heads + slot) * D;
-      *reinterpret_cast<uint4*>(dst + lane * 8) = pack8<T>(a);
-      *reinterpret_cast<uint4*>(dst + kHalf + lane * 8) = pack8<T>(bb);
+    if (is_q && at.page >= -1) {  // a refused token's query reads as zeros
+      T* dst = static_cast<T*>(p.q_out) + ((n0 + tok) * p.heads + slot) * D;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(dst + lane * 8) = ok ? pack8<T>(a) : zero;
+      *reinterpret_cast<uint4*>(dst + kHalf + lane * 8) = ok ? pack8<T>(bb) : zero;
     }
     if (__any_sync(0xffffffffu, is_kv)) {
       // extrema of the lane's pieces: D = 128 has one group per half, D = 64 one in all
@@ -156,7 +184,9 @@ __global__ void __launch_bounds__(kAppThreads) kv4_append_kernel(const Kv4Append
         const float g0 = __half2float(c0), g1 = __half2float(c1);
         const uint32_t w0 = code8(a, f0, g0 > 0.f ? __frcp_rn(g0) : 0.f);
         const uint32_t w1 = code8(bb, f1, g1 > 0.f ? __frcp_rn(g1) : 0.f);
-        uint32_t* blk = reinterpret_cast<uint32_t*>(p.pool + kv4_block_offset(s, pg, kh, pos, D));
+        const int kh = is_k ? slot - p.heads : slot - p.heads - s.kv_heads;
+        const int bp = at.pos & 15;
+        uint32_t* blk = reinterpret_cast<uint32_t*>(p.pool + kv4_block_offset(s, at.page, kh, at.pos, D));
         const __half2 p0 = __halves2half2(c0, l0), p1 = __halves2half2(c1, l1);
         const int side = is_k ? 0 : 1;
         if (D == 128) {
@@ -184,56 +214,69 @@ struct Kv4GatherParams {
 };
 
 // One thread per (token, KV head, side, 8 elements): value = scale * code + low
-// in fp32, rounded once.
+// in fp32, rounded once.  A thread's words of the CTA's tokens are all on their way
+// before the first is used.
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppThreads) kv4_gather_kernel(const Kv4GatherParams p) {
+__global__ void __launch_bounds__(kAppThreads) kv4_gather_kernel(const Kv4GatherParams p, int per_cta) {
+  __shared__ TokenPlace sh_place[kAppTokens];
   pdl_launch_dependents();
   pdl_wait();  // the pool is written by the previous kernel
   const Kv4Seq& s = p.seq;
   constexpr int kWords = D / 8;
-  const int64_t n = blockIdx.x;
-  const int b = kv4_sequence(s, n);
-  if (b < 0) return;
-  const int64_t first = s.q_start ? s.q_start[b] : static_cast<int64_t>(b) * s.t_new;
-  const int pre = s.prefix[b];
-  const int64_t pos = pre + (n - first);
-  const int pg = pre < 0 ? -1 : kv4_page(s, b, pos);
-  if (pg < 0 && threadIdx.x == 0) report_device_error(p.status, FITQ_ERR_ARG);
-  const int bp = static_cast<int>(pos & 15);
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * per_cta;
+  if (threadIdx.x < kAppTokens)
+    sh_place[threadIdx.x] = static_cast<int>(threadIdx.x) < per_cta
+                                ? token_place(s, n0 + threadIdx.x, 0x7fffffff, p.status)
+                                : TokenPlace{-2, 0};
+  __syncthreads();
   const int items = s.kv_heads * 2 * kWords;
   for (int i = blockIdx.y * kAppThreads + threadIdx.x; i < items; i += gridDim.y * kAppThreads) {
     const int e = i % kWords, side = (i / kWords) & 1, kh = i / (2 * kWords);
     const int g = e / 8, e8 = e % 8;
-    float f[8];
+    uint32_t w[kAppTokens], pr[kAppTokens];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = 0.f;
-    if (pg >= 0) {
-      const uint32_t* blk = reinterpret_cast<const uint32_t*>(p.pool + kv4_block_offset(s, pg, kh, pos, D));
-      const uint32_t w = blk[side ? kv4_value_word<D>(bp, g, e8) : kv4_key_word<D>(bp, g, e8)];
-      const uint32_t pr = blk[kv4_param_word<D>(bp, side, g)];
-      const float2 sl = Half16<__half>::unpack(pr);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        f[j] = __fadd_rn(__fmul_rn(sl.x, static_cast<float>((w >> (4 * j)) & 15u)), sl.y);
+    for (int t = 0; t < kAppTokens; ++t) {
+      const TokenPlace at = sh_place[t];
+      w[t] = pr[t] = 0;
+      if (at.page >= 0) {
+        const uint32_t* blk = reinterpret_cast<const uint32_t*>(p.pool + kv4_block_offset(s, at.page, kh, at.pos, D));
+        const int bp = at.pos & 15;
+        w[t] = blk[side ? kv4_value_word<D>(bp, g, e8) : kv4_key_word<D>(bp, g, e8)];
+        pr[t] = blk[kv4_param_word<D>(bp, side, g)];
+      }
     }
-    T* dst = static_cast<T*>(side ? p.v : p.k) + (n * s.kv_heads + kh) * D + e * 8;
-    *reinterpret_cast<uint4*>(dst) = pack8<T>(f);
+#pragma unroll
+    for (int t = 0; t < kAppTokens; ++t) {
+      if (sh_place[t].page < -1) continue;
+      const float2 sl = Half16<__half>::unpack(pr[t]);
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = __fadd_rn(__fmul_rn(sl.x, static_cast<float>((w[t] >> (4 * j)) & 15u)), sl.y);
+      T* dst = static_cast<T*>(side ? p.v : p.k) + ((n0 + t) * s.kv_heads + kh) * D + e * 8;
+      *reinterpret_cast<uint4*>(dst) = pack8<T>(f);
+    }
   }
 }
 
-// CTAs along y: a call of few tokens spreads the work of each over several CTAs
-// (a decode step of one token is one pass deep); from two tokens per SM on, one
-// CTA per token keeps its rotary row in registers over its passes.
-unsigned split_y(int64_t tokens, int passes, int num_sms) {
-  return tokens >= 2ll * num_sms ? 1u : static_cast<unsigned>(passes);
+// Tokens per CTA and CTAs along y: few tokens spread each over several CTAs (a decode
+// step is one pass deep); from eight per SM on a CTA takes four.
+struct TokenGrid {
+  int per_cta;
+  dim3 grid;
+};
+TokenGrid token_grid(int64_t tokens, int passes, int num_sms) {
+  TokenGrid g;
+  g.per_cta = tokens >= 8ll * num_sms ? kAppTokens : 1;
+  g.grid = dim3(static_cast<unsigned>((tokens + g.per_cta - 1) / g.per_cta),
+                tokens >= 2ll * num_sms ? 1u : static_cast<unsigned>(passes));
+  return g;
 }
 
 template <typename T, int D>
 int append_t(const Kv4AppendParams& p, cudaStream_t st, int num_sms) {
   constexpr int kTeams = kAppThreads / (D / 16);
-  const int passes = (p.heads + 2 * p.seq.kv_heads + kTeams - 1) / kTeams;
-  const dim3 grid(static_cast<unsigned>(p.seq.tokens), split_y(p.seq.tokens, passes, num_sms));
-  const cudaError_t e = launch_pdl(kv4_append_kernel<T, D>, grid, dim3(kAppThreads), 0, st, p);
+  const TokenGrid g = token_grid(p.seq.tokens, (p.heads + 2 * p.seq.kv_heads + kTeams - 1) / kTeams, num_sms);
+  const cudaError_t e = launch_pdl(kv4_append_kernel<T, D>, g.grid, dim3(kAppThreads), 0, st, p, g.per_cta);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   return launch_result();
@@ -241,9 +284,8 @@ int append_t(const Kv4AppendParams& p, cudaStream_t st, int num_sms) {
 
 template <typename T, int D>
 int gather_t(const Kv4GatherParams& p, cudaStream_t st, int num_sms) {
-  const int passes = (p.seq.kv_heads * 2 * (D / 8) + kAppThreads - 1) / kAppThreads;
-  const dim3 grid(static_cast<unsigned>(p.seq.tokens), split_y(p.seq.tokens, passes, num_sms));
-  const cudaError_t e = launch_pdl(kv4_gather_kernel<T, D>, grid, dim3(kAppThreads), 0, st, p);
+  const TokenGrid g = token_grid(p.seq.tokens, (p.seq.kv_heads * 2 * (D / 8) + kAppThreads - 1) / kAppThreads, num_sms);
+  const cudaError_t e = launch_pdl(kv4_gather_kernel<T, D>, g.grid, dim3(kAppThreads), 0, st, p, g.per_cta);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   return launch_result();

@@ -59,7 +59,8 @@ def _check_attention(c, o):
 
 APPEND = [
     ([0], [1], 8, 1, 128, 16, BF), ([15, 16, 17], [1, 1, 1], 40, 8, 128, 16, BF),
-    ([0, 63, 5], [70, 1, 33], 4, 4, 64, 32, FP), ([1000, 0], [5, 300], 14, 2, 128, 64, FP),
+    ([0, 63, 5], [70, 1, 33], 4, 4, 64, 32, FP), ([5, 0, 2000], [900, 511, 2], 3, 1, 128, 16, BF),
+    ([0, 31], [1201, 40], 20, 4, 64, 64, FP), ([1000, 0], [5, 300], 14, 2, 128, 64, FP),
     ([7, 3, 0, 100], [3, 0, 129, 1], 28, 4, 64, 128, BF),
 ]
 
@@ -144,6 +145,10 @@ ATTEND = [
     # drafts: one, two and four column tiles, an odd group
     ([100, 5], [2, 2], 16, 4, 128, 32, FP), ([511, 64, 3], [3, 3, 3], 40, 8, 128, 128, BF),
     ([300], [5], 40, 8, 128, 16, FP), ([77, 1024], [6, 2], 10, 2, 64, 64, BF), ([4095], [32], 4, 4, 128, 64, BF),
+    # more pairs than clusters take: runs of the list, cut pairs joined behind them
+    ([3, 200, 1400, 64, 0, 777], [1] * 6, 40, 8, 128, 64, BF), ([90, 2500, 1, 511, 300], [2, 3, 1, 0, 2], 40, 8, 128, 16, FP),
+    ([1000 + 37 * i for i in range(9)], [1] * 9, 8, 8, 64, 32, BF), ([9000], [1], 2, 2, 128, 128, BF),
+    ([20000], [5], 5, 1, 128, 64, FP),
     # several row tiles, prompts with and without a prefix, empty sequences
     ([0], [200], 8, 2, 128, 64, BF), ([130, 0, 9], [40, 0, 97], 12, 4, 64, 16, FP), ([31], [65], 7, 1, 128, 16, FP),
     ([0, 1, 700], [333, 17, 64], 40, 8, 128, 128, BF), ([0, 3], [129, 128], 16, 16, 64, 32, BF),
