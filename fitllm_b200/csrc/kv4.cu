@@ -87,7 +87,7 @@ __device__ __forceinline__ TokenPlace token_place(const Kv4Seq& s, int64_t n, in
 // team holds elements 8 i .. 8 i + 7 of each half of the head, so the rotation pairs
 // meet in one lane and the group extrema take log2(team) shuffles.
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppThreads, 3) kv4_append_kernel(const Kv4AppendParams p, int per_cta) {
+__global__ void __launch_bounds__(kAppThreads, 4) kv4_append_kernel(const Kv4AppendParams p, int per_cta) {
   constexpr int kTeam = D / 16;
   constexpr int kTeams = kAppThreads / kTeam;
   constexpr int kHalf = D / 2;
@@ -98,13 +98,12 @@ __global__ void __launch_bounds__(kAppThreads, 3) kv4_append_kernel(const Kv4App
   const Kv4Seq& s = p.seq;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * per_cta;
   const int slots = p.heads + 2 * s.kv_heads;
-  const int items = static_cast<int>(n0 + per_cta <= s.tokens ? per_cta : s.tokens - n0) * slots;
+  const int count = static_cast<int>(n0 + per_cta <= s.tokens ? per_cta : s.tokens - n0);
   const int step = kTeams * gridDim.y;
 
   uint4 ra = make_uint4(0, 0, 0, 0), rb = ra;  // this lane's elements of the next head
-  auto fetch = [&](int item) {
-    if (item >= items) return;
-    const int tok = item / slots, slot = item - tok * slots;
+  auto fetch = [&](int tok, int slot) {
+    if (tok >= count) return;
     const int64_t n = n0 + tok;
     const T* src = slot < p.heads ? static_cast<const T*>(p.q) + n * p.q_stride + slot * D
                    : slot < p.heads + s.kv_heads
@@ -113,14 +112,22 @@ __global__ void __launch_bounds__(kAppThreads, 3) kv4_append_kernel(const Kv4App
     ra = *reinterpret_cast<const uint4*>(src + lane * 8);
     rb = *reinterpret_cast<const uint4*>(src + kHalf + lane * 8);
   };
-  int item = blockIdx.y * kTeams + team;
-  fetch(item);
+  // (token, slot) of the team's current and next head, stepped without a division
+  int tok_next = 0, slot_next = blockIdx.y * kTeams + team;
+  auto wrap = [&]() {
+    while (slot_next >= slots) {
+      slot_next -= slots;
+      ++tok_next;
+    }
+  };
+  wrap();
+  fetch(tok_next, slot_next);
   if (threadIdx.x < per_cta) sh_place[threadIdx.x] = token_place(s, n0 + threadIdx.x, p.rope_len, p.status);
   __syncthreads();
 
-  for (int i0 = blockIdx.y * kTeams; i0 < items; i0 += step, item += step) {
-    const bool have = item < items;
-    const int tok = have ? item / slots : 0, slot = have ? item - tok * slots : 0;
+  while (__any_sync(0xffffffffu, tok_next < count)) {
+    const bool have = tok_next < count;
+    const int tok = have ? tok_next : 0, slot = slot_next;
     const TokenPlace at = sh_place[tok];
     const bool ok = have && at.page >= 0;
     const bool is_q = have && slot < p.heads;
@@ -129,7 +136,9 @@ __global__ void __launch_bounds__(kAppThreads, 3) kv4_append_kernel(const Kv4App
     float a[8], bb[8];
     unpack8<T>(ra, a);
     unpack8<T>(rb, bb);
-    fetch(item + step);
+    slot_next += step;
+    wrap();
+    fetch(tok_next, slot_next);
     if (is_q || is_k) {
       const float4* cp = reinterpret_cast<const float4*>(p.cs + static_cast<int64_t>(at.pos) * kHalf + lane * 8);
       const float4* sp = reinterpret_cast<const float4*>(p.sn + static_cast<int64_t>(at.pos) * kHalf + lane * 8);
