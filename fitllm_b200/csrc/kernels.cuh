@@ -347,6 +347,10 @@ int launch_kv4_attention(const Kv4Seq& seq, const void* q, int64_t q_stride, con
                          int dim, int dtype, int64_t max_new, int64_t max_len, void* workspace, int* status,
                          cudaStream_t st, int num_sms);
 
+// The same attention for calls of many rows, on tcgen05 (kv4_prompt.cu); no workspace.
+int launch_kv4_prompt(const Kv4Seq& seq, const void* q, int64_t q_stride, const void* pool, void* out, int heads,
+                      int dim, int dtype, int64_t max_new, int* status, cudaStream_t st);
+
 // Log probabilities of given tokens, entropy, top alternatives and their
 // gradient (logprob.cu).
 int launch_token_logprobs(const void* logits, int dtype, const int64_t* ids, int64_t rows, int64_t V, int64_t stride,

@@ -85,12 +85,6 @@ struct Kv4AttnParams {
   Kv4Seq seq;
 };
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -123,32 +117,6 @@ __device__ __forceinline__ void mma_f16_init(float (&d)[4], uint32_t a0, uint32_
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
-
-// (x & mask) | 1024 in both halves, in one instruction (two constants in one
-// expression would be split in two).
-template <uint32_t kMask>
-__device__ __forceinline__ uint32_t nibbles(uint32_t x) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(kMask), "r"(0x64006400u));
-  return d;
-}
-// 1024 + c of the low nibble of each half; 1024 + 16 c of the second one.
-__device__ __forceinline__ uint32_t codes_even(uint32_t x) { return nibbles<0x000f000fu>(x); }
-__device__ __forceinline__ uint32_t codes_odd(uint32_t x) { return nibbles<0x00f000f0u>(x); }
-// c - 8 of either.
-__device__ __forceinline__ uint32_t centre_even(uint32_t u) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t centre_odd(uint32_t u) {
-  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(0.0625f, 0.0625f),
-                            __floats2half2_rn(-72.f, -72.f));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) { return Half16<__half>::pack(lo, hi); }
-
-// 2^k with k in [-126, 127].
-__device__ __forceinline__ float pow2(int k) { return __int_as_float((k + 127) << 23); }
 
 // Tiles of sequence b that columns [col0, col0 + R) see, and its lengths.
 struct SeqSpan {
@@ -1042,10 +1010,14 @@ int attn_td(const Kv4AttnParams& p, const AttnPlan& a, cudaStream_t st) {
   return a.nt == 1 ? attn_t<T, D, 1>(p, a, st) : attn_t<T, D, 2>(p, a, st);
 }
 
+// From 65 rows on the tensor-memory kernel takes the call.
+bool prompt_rows(int group, int64_t max_new) { return group * max_new > 64; }
+
 }  // namespace
 
 size_t kv4_attention_workspace(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim,
                                int num_sms) {
+  if (prompt_rows(group, max_new)) return 16;
   return attn_plan(batch, kv_heads, group, max_new, max_len, dim, num_sms).bytes;
 }
 
@@ -1053,6 +1025,8 @@ int launch_kv4_attention(const Kv4Seq& seq, const void* q, int64_t q_stride, con
                          int dim, int dtype, int64_t max_new, int64_t max_len, void* workspace, int* status,
                          cudaStream_t st, int num_sms) {
   const int group = heads / seq.kv_heads;
+  if (prompt_rows(group, max_new))
+    return launch_kv4_prompt(seq, q, q_stride, pool, out, heads, dim, dtype, max_new, status, st);
   const AttnPlan a = attn_plan(seq.batch, seq.kv_heads, group, max_new, max_len, dim, num_sms);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Kv4AttnParams p;
