@@ -17,10 +17,10 @@
 // the scores' scale and the final 1 / l.  Queries are scaled per row by a power of
 // two as in kv4_attn.cu.
 //
-// The reference m of a row moves only when an exponent exceeds 2^15 (fp16's range for
-// P): a pass normally reads S_r once; the thread that has to move it reads it again
-// and rescales its row of O_r, which no MMA touches then (the products of the tile
-// before completed with S_r).
+// The reference m of a row moves only when a weight would exceed 2^15 (fp16's range for
+// P); the thread that moves it rescales its row of O_r, which no MMA touches then (the
+// products of the tile before completed with S_r).  A thread reads its scores twice
+// (the maximum, the weights), the next 32 on their way while it works on 32.
 //
 // A group of V whose scale or low is not finite must only reach the rows that see it,
 // and 0 x NaN would reach all: it enters as zeros, its first position is noted per
@@ -87,6 +87,14 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -271,50 +279,32 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
 #pragma unroll
       for (int gr = 0; gr < G; ++gr)
         if (sh_bad[buf][gr] <= lim) nan_groups |= 1u << gr;
-      auto hide = [&](int c, uint32_t (&v)[32]) {  // hidden scores of chunk c
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (pos0 + 32 * c + i > lim || !((pages >> (2 * c + (i >> 4))) & 1u)) v[i] = 0xff800000u;
-      };
-      uint32_t pk[64];
-      float sum;
-      auto pass = [&]() -> float {  // weights relative to m; returns the largest exponent
-        const uint64_t m2 = pack2(-m, -m);
-        float top = kPFloor;
-        uint64_t s2 = 0;
+      // ---- the largest score; hidden ones become -inf in tensor memory too
+      float raw = -INFINITY;
+      {
+        uint32_t v[2][32];
+        tmem_ld_32x32b_x32(t_s, v[0]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(t_s + 32 * c, v);
+          uint32_t(&x)[32] = v[c & 1];
           tmem_ld_wait();
-          if (masked) hide(c, v);
+          if (c < 3) tmem_ld_32x32b_x32(t_s + 32 * (c + 1), v[(c + 1) & 1]);
+          if (masked) {
+            const uint32_t pg = pages >> (2 * c);
+            const int left = lim - pos0 - 32 * c;  // elements 0 .. left are visible
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float x0, x1;
-            unpack2(fma2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), cn2, m2), x0, x1);
-            top = fmaxf(top, fmaxf(x0, x1));
-            const float w0 = exp2_approx(x0), w1 = exp2_approx(x1);
-            s2 = add2(s2, pack2(w0, w1));
-            pk[16 * c + i / 2] = pack_half2(w0, w1);
+            for (int i = 0; i < 32; ++i)
+              if (i > left || !(pg & (i < 16 ? 1u : 2u))) x[i] = 0xff800000u;
+            tmem_st_x32(t_s + 32 * c, x);
           }
-        }
-        float a, c;
-        unpack2(s2, a, c);
-        sum = a + c;
-        return top;
-      };
-      const float top = pass();
-      if (__any_sync(0xffffffffu, top > kPRoom)) {
-        float raw = kPFloor;  // the largest score, from the tile itself: m may be the floor
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(t_s + 32 * c, v);
-          tmem_ld_wait();
-          if (masked) hide(c, v);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) raw = fmaxf(raw, __uint_as_float(v[i]) * cn);
+          for (int i = 0; i < 32; i += 2)
+            raw = fmaxf(raw, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
         }
+        if (masked) tmem_st_done();
+      }
+      raw *= cn;
+      if (__any_sync(0xffffffffu, raw > m + kPRoom)) {
         const float m_new = fmaxf(m, raw);
         const float al = exp2_approx(m - m_new);
         m = m_new;
@@ -330,11 +320,33 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
             tmem_st_x32(t_o + 32 * c, v);
           }
         }
-        pass();
       }
-      l += sum;
-      tmem_st_x32(t_s, pk);
-      tmem_st_x32(t_s + 32, pk + 32);
+      // ---- weights, written over the scores (chunk c's lie where chunk c / 2's were)
+      {
+        const uint64_t m2 = pack2(-m, -m);
+        uint64_t s2 = 0;
+        uint32_t v[2][32];
+        tmem_ld_32x32b_x32(t_s, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t(&x)[32] = v[c & 1];
+          tmem_ld_wait();
+          if (c < 3) tmem_ld_32x32b_x32(t_s + 32 * (c + 1), v[(c + 1) & 1]);
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x0, x1;
+            unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), cn2, m2), x0, x1);
+            const float w0 = exp2_approx(x0), w1 = exp2_approx(x1);
+            s2 = add2(s2, pack2(w0, w1));
+            pk[i / 2] = pack_half2(w0, w1);
+          }
+          tmem_st_x16(t_s + 16 * c, pk);
+        }
+        float a, c;
+        unpack2(s2, a, c);
+        l += a + c;
+      }
       tmem_st_done();
       tc_fence_before();
       mbar_arrive(&b_pready[r]);
