@@ -8,8 +8,9 @@
 // operand, written over S_r.  While one row tile's exponentials are taken the other's
 // products run.
 //
-// Roles: warps 0-3 and 4-7 the softmax of row tiles 0 and 1, warps 8-11 decode the
-// cache, warp 12 issues the MMAs.  The decoders read blocks straight into registers,
+// Roles: warps 0-3 and 4-7 the softmax of row tiles 0 and 1, warps 8-15 decode the
+// cache (with four of them a tile took 5,400 cycles, their own instructions' latency),
+// warp 16 issues the MMAs.  The decoders read blocks straight into registers,
 // one tile ahead, and write K [position][D] and V^T [D][position] as fp16 in the
 // 128-byte-swizzled K-major layout, two buffers each.  A value of the cache is rounded
 // once more, to fp16's 2^-12 (bf16 would round to 2^-9); all are halved, so that a
@@ -36,8 +37,12 @@ namespace {
 
 constexpr int kPRows = 128;       // rows of a row tile (TMEM lanes)
 constexpr int kPTile = 128;       // positions of a tile
-constexpr int kPThreads = 416;
-constexpr int kPDecoders = 128;
+constexpr int kPThreads = 640;     // five warpgroups
+constexpr int kPDecoders = 256;
+// Registers per thread: 96 at launch (61,440 in all), then softmax 128, decoders 80,
+// issuer 64: 2 x 128 + 2 x 80 + 64 = 480 per lane of a warpgroup.
+constexpr int kPRegsSoftmax = 128, kPRegsDecode = 80, kPRegsIssue = 64;
+static_assert(2 * kPRegsSoftmax + 2 * kPRegsDecode + kPRegsIssue <= 5 * 96, "more registers than the launch has");
 constexpr float kPFloor = -3.0e38f;
 constexpr float kPRoom = 15.f;    // weights stay below 2^15
 
@@ -123,6 +128,9 @@ __device__ __forceinline__ uint32_t plain_odd(uint32_t x) {
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t a) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(a) : "memory");
+}
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Two fp32 operations in one instruction.
@@ -154,8 +162,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   __shared__ uint64_t b_qready, b_kfull[2], b_kfree[2], b_vfull[2], b_vfree[2], b_sfull[2], b_pready[2], b_ofull, b_done;
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_abort;
-  __shared__ int sh_bad[2][2];         // per buffer and group: first position that is not finite
-  __shared__ uint32_t sh_pages[2];     // per buffer: which of the tile's blocks have a page
+  // per buffer and block: 1 if it has a page, and from bit 8 and 16 the first position
+  // at which a value of group 0 and 1 is not finite (16: none)
+  __shared__ __align__(16) uint32_t sh_note[2][8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (smem_u32(g_prompt_smem) + 1023u) & ~1023u;
 
@@ -188,20 +197,20 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
 
   if (tid == 0) {
     sh_abort = 0;
-    mbar_init(&b_qready, 2 * kPRows);
+    mbar_init(&b_qready, 8);  // one arrival per warp
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&b_kfull[i], kPDecoders);
-      mbar_init(&b_vfull[i], kPDecoders);
+      mbar_init(&b_kfull[i], kPDecoders / 32);
+      mbar_init(&b_vfull[i], kPDecoders / 32);
       mbar_init(&b_kfree[i], 1);
       mbar_init(&b_vfree[i], 1);
       mbar_init(&b_sfull[i], 1);
-      mbar_init(&b_pready[i], kPRows);
+      mbar_init(&b_pready[i], kPRows / 32);
     }
     mbar_init(&b_ofull, 1);
     mbar_init(&b_done, 1);
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(&sh_tmem, 512);
     tmem_relinquish();
   }
@@ -216,7 +225,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, &sh_abort, p.status));
   };
 
+  auto arrive_warp = [&](uint64_t* bar) {  // behind every lane's stores and fences
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+
   if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPRegsSoftmax));
     // ------------------------------------------------------------ softmax: a row per thread
     const int r = warp >> 2;
     const int lr = tid & 127;
@@ -225,36 +240,38 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     const bool has = r * kPRows + lr < rows;
     const int tok = has ? static_cast<int>(row / p.group) : 0;
     const int hd = kvh * p.group + (has ? static_cast<int>(row % p.group) : 0);
-    // ---- the row's queries: scaled, fp16, swizzled
+    // ---- the row's queries: scaled, fp16, swizzled, elements as the keys'
     float cn;
     {
       const T* src = static_cast<const T*>(p.q) + (first + tok) * p.q_stride + static_cast<int64_t>(hd) * D;
-      uint4 u[D / 8];
+      const uint4* qv = reinterpret_cast<const uint4*>(src);
       float mx = 0.f;
+      if (has) {
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          float f[8];
+          unpack8<T>(qv[i], f);
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        u[i] = make_uint4(0, 0, 0, 0);
-        if (has) u[i] = reinterpret_cast<const uint4*>(src)[i];
-        float f[8];
-        unpack8<T>(u[i], f);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) mx = fmaxf(mx, fabsf(f[x]));
+          for (int x = 0; x < 8; ++x) mx = fmaxf(mx, fabsf(f[x]));
+        }
       }
       int e = (__float_as_int(mx) >> 23) - 127;
       e = (mx == 0.f || e > 127) ? 12 : (e < -100 ? -100 : e);
       const float up = pow2(12 - e);
       cn = p.scale_log2 * pow2(e - 11);  // keys enter halved
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < D / 8; ++i) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (has) u = qv[i];
         float f[8];
-        unpack8<T>(u[i], f);
+        unpack8<T>(u, f);
         sts128(s_q + r * L::kQ + (i >> 3) * (kPRows * 128) + lr * 128 + (((i & 7) ^ (lr & 7)) << 4),
-               pack_half2(f[0] * up, f[1] * up), pack_half2(f[2] * up, f[3] * up), pack_half2(f[4] * up, f[5] * up),
-               pack_half2(f[6] * up, f[7] * up));
+               pack_half2(f[0] * up, f[4] * up), pack_half2(f[1] * up, f[5] * up), pack_half2(f[2] * up, f[6] * up),
+               pack_half2(f[3] * up, f[7] * up));
       }
     }
     fence_async_proxy();
-    mbar_arrive(&b_qready);
+    arrive_warp(&b_qready);
     const uint32_t t_lane = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t t_s = tmem + t_lane + r * 128, t_o = tmem + t_lane + 256 + r * 128;
     int lim = pre + tok;  // last visible position
@@ -273,14 +290,26 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
       ok = wait_all(&b_vfull[buf], ph) && wait_all(&b_sfull[r], j & 1);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t pages = sh_pages[buf];
+      uint32_t pages = 0xffu;  // which blocks are there
       const int pos0 = j * kPTile;
+      const uint4 na = *reinterpret_cast<const uint4*>(&sh_note[buf][0]);
+      const uint4 nb = *reinterpret_cast<const uint4*>(&sh_note[buf][4]);
+      constexpr uint32_t kClean = 1u | (kKv4Block << 8) | (kKv4Block << 16);
+      if (((na.x ^ kClean) | (na.y ^ kClean) | (na.z ^ kClean) | (na.w ^ kClean) | (nb.x ^ kClean) | (nb.y ^ kClean) |
+           (nb.z ^ kClean) | (nb.w ^ kClean)) != 0) {
+        pages = 0;
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t note = sh_note[buf][i];
+          pages |= (note & 1u) << i;
+          for (int gr = 0; gr < G; ++gr) {
+            const int at = static_cast<int>((note >> (8 + 8 * gr)) & 0xffu);
+            if (at < kKv4Block && pos0 + i * kKv4Block + at <= lim) nan_groups |= 1u << gr;
+          }
+        }
+      }
       const bool masked = pos0 + kPTile > sure || pages != 0xffu;
-#pragma unroll
-      for (int gr = 0; gr < G; ++gr)
-        if (sh_bad[buf][gr] <= lim) nan_groups |= 1u << gr;
       // ---- the largest score; hidden ones become -inf in tensor memory too
-      float raw = -INFINITY;
+      float raw = -INFINITY, raw1 = -INFINITY, raw2 = -INFINITY, raw3 = -INFINITY;
       {
         uint32_t v[2][32];
         tmem_ld_32x32b_x32(t_s, v[0]);
@@ -298,12 +327,16 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
             tmem_st_x32(t_s + 32 * c, x);
           }
 #pragma unroll
-          for (int i = 0; i < 32; i += 2)
+          for (int i = 0; i < 32; i += 8) {
             raw = fmaxf(raw, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+            raw1 = fmaxf(raw1, fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
+            raw2 = fmaxf(raw2, fmaxf(__uint_as_float(x[i + 4]), __uint_as_float(x[i + 5])));
+            raw3 = fmaxf(raw3, fmaxf(__uint_as_float(x[i + 6]), __uint_as_float(x[i + 7])));
+          }
         }
         if (masked) tmem_st_done();
       }
-      raw *= cn;
+      raw = fmaxf(fmaxf(raw, raw1), fmaxf(raw2, raw3)) * cn;
       if (__any_sync(0xffffffffu, raw > m + kPRoom)) {
         const float m_new = fmaxf(m, raw);
         const float al = exp2_approx(m - m_new);
@@ -349,198 +382,179 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
       }
       tmem_st_done();
       tc_fence_before();
-      mbar_arrive(&b_pready[r]);
+      arrive_warp(&b_pready[r]);
     }
     if (ok) ok = wait_all(&b_ofull, 0);
     if (active && (ok || tiles == 0)) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 2.f / l;  // values entered halved
       T* dst = static_cast<T*>(p.out) + ((first + tok) * p.heads + hd) * D;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t v[32];
+#pragma unroll 1
+      for (int gr = 0; gr < G; ++gr) {
+        uint32_t v[2][32];
         if (tiles > 0) {
-          tmem_ld_32x32b_x32(t_o + 32 * c, v);
+          tmem_ld_32x32b_x32(t_o + 64 * gr, v[0]);
+          tmem_ld_32x32b_x32(t_o + 64 * gr + 32, v[1]);
           tmem_ld_wait();
         }
-        const bool bad = (nan_groups >> (c / 2)) & 1u;
+        const bool bad = (nan_groups >> gr) & 1u;
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
+        for (int e = 0; e < 8; ++e) {  // element 8 e + x of the group stands in column 8 x + e
           float f[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) f[x] = bad ? NAN : (l == 0.f ? 0.f : __uint_as_float(v[i + x]) * inv);
-          if (has) *reinterpret_cast<uint4*>(dst + 32 * c + i) = pack8<T>(f);
+          for (int x = 0; x < 8; ++x)
+            f[x] = bad ? NAN : (l == 0.f ? 0.f : __uint_as_float(v[x >> 2][8 * (x & 3) + e]) * inv);
+          if (has) *reinterpret_cast<uint4*>(dst + 64 * gr + 8 * e) = pack8<T>(f);
         }
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsDecode));
     // ------------------------------------------------------------ decoders
-    const int dt = tid - 256;
-    // keys: positions 32 i + dt / 4, sixteen-byte unit c = dt % 4 of each group; values:
-    // eight positions of half block h16, elements 8 e .. 8 e + 7 of each group
-    const int kc = dt & 3, kp = dt >> 2;
-    const int h16 = dt & 15, ve = dt >> 4;
-    uint32_t kw[4][2 * G], kpar[4][G], vw[8 * G], vpar[8][G];
-    auto look_up = [&](int j) -> int64_t {  // lane i (mod 8): block i of tile j
-      int64_t off = -1;
-      const int64_t pos = static_cast<int64_t>(j) * kPTile + (lane & 7) * kKv4Block;
-      if (j < tiles && pos < len) {
-        const int pg = kv4_page(s, b, pos);
-        if (pg >= 0)
-          off = kv4_block_offset(s, pg, kvh, pos, D);
-        else if (dt < 8)
-          report_device_error(p.status, FITQ_ERR_ARG);
-      }
-      return off;
+    // Warp dw decodes block dw of every tile.  Keys: lane (r, c) = (lane / 4, lane % 4) takes
+    // positions r and r + 8, unit c of each group; values: lane (e, q) takes positions
+    // 2 q, 2 q + 1 of each half, elements 8 e .. 8 e + 7 of each group.  Either way a warp
+    // reads 512 consecutive bytes at a time.  V^T's row of element 8 e + i of a group is
+    // 8 i + e, so that the lanes of a store lie in eight rows of different swizzle.
+    const int dw = warp - 8;
+    const int hi = lane >> 2, lo2 = lane & 3;
+    uint32_t kw[2][2 * G], kpar[2][G], vw[2][2][G], vpar[2][2][G];
+    // The page table's entry for this warp's block of tile j, and, one tile later (a use at
+    // once would wait for the load), the block; null: no page.
+    auto entry = [&](int j) -> int {
+      const int64_t pos = static_cast<int64_t>(j) * kPTile + dw * kKv4Block;
+      return j < tiles && pos < len ? s.page_table[static_cast<int64_t>(b) * s.max_pages + (pos >> s.page_shift)] : -2;
     };
-    auto load_k = [&](int64_t off) {
+    auto block = [&](int j, int pg) -> const uint8_t* {
+      const int64_t pos = static_cast<int64_t>(j) * kPTile + dw * kKv4Block;
+      const bool there = pg >= 0 && pg < s.num_pages;
+      if (!there && pg != -2 && lane == 0) report_device_error(p.status, FITQ_ERR_ARG);
+      return there ? p.pool + kv4_block_offset(s, pg, kvh, pos, D) : nullptr;
+    };
+    // A block without a page reads the pool's first one with scale and low 0.
+    auto load_k = [&](const uint8_t* blk) {
+      if (blk == nullptr) blk = p.pool;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int pos = 32 * i + kp;
-        const int64_t o = __shfl_sync(0xffffffffu, off, pos >> 4);
-#pragma unroll
-        for (int w = 0; w < 2 * G; ++w) kw[i][w] = 0;
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) kpar[i][gr] = 0;
-        if (o >= 0) {
-          const uint8_t* blk = p.pool + o;
-          const int bp = pos & 15;
-          if (G == 2) {
-            *reinterpret_cast<uint4*>(kw[i]) = *reinterpret_cast<const uint4*>(blk + (bp * 4 + kc) * 16);
-            *reinterpret_cast<uint2*>(kpar[i]) = *reinterpret_cast<const uint2*>(blk + 16 * D + bp * 16);
-          } else {
-            *reinterpret_cast<uint2*>(kw[i]) = *reinterpret_cast<const uint2*>(blk + (bp * 4 + kc) * 8);
-            kpar[i][0] = *reinterpret_cast<const uint32_t*>(blk + 16 * D + bp * 8);
-          }
+      for (int i = 0; i < 2; ++i) {
+        if (G == 2) {
+          *reinterpret_cast<uint4*>(kw[i]) = *reinterpret_cast<const uint4*>(blk + i * 512 + lane * 16);
+          *reinterpret_cast<uint2*>(kpar[i]) = *reinterpret_cast<const uint2*>(blk + 16 * D + (8 * i + hi) * 16);
+        } else {
+          *reinterpret_cast<uint2*>(kw[i]) = *reinterpret_cast<const uint2*>(blk + i * 256 + lane * 8);
+          kpar[i][0] = *reinterpret_cast<const uint32_t*>(blk + 16 * D + (8 * i + hi) * 8);
         }
       }
     };
-    auto load_v = [&](int64_t off) {
-      const int64_t o = __shfl_sync(0xffffffffu, off, h16 >> 1);
-      const int h = h16 & 1;
+    auto load_v = [&](const uint8_t* blk) {
+      if (blk == nullptr) blk = p.pool;
 #pragma unroll
-      for (int i = 0; i < 8 * G; ++i) vw[i] = 0;
+      for (int h = 0; h < 2; ++h) {
+        if (G == 2)
+          *reinterpret_cast<uint4*>(vw[h]) = *reinterpret_cast<const uint4*>(blk + 8 * D + h * 512 + lane * 16);
+        else
+          *reinterpret_cast<uint2*>(vw[h]) = *reinterpret_cast<const uint2*>(blk + 8 * D + h * 256 + lane * 8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) vpar[i][gr] = 0;
-      if (o >= 0) {
-        const uint8_t* blk = p.pool + o;
-        const uint4* src = reinterpret_cast<const uint4*>(blk + 8 * D + (h * 8 + ve) * 32 * G);
-#pragma unroll
-        for (int i = 0; i < 2 * G; ++i) *reinterpret_cast<uint4*>(vw + 4 * i) = src[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint8_t* ps = blk + 16 * D + (8 * h + i) * 8 * G + 4 * G;
+        for (int o = 0; o < 2; ++o) {
+          const uint8_t* ps = blk + 16 * D + (8 * h + 2 * lo2 + o) * 8 * G + 4 * G;
           if (G == 2)
-            *reinterpret_cast<uint2*>(vpar[i]) = *reinterpret_cast<const uint2*>(ps);
+            *reinterpret_cast<uint2*>(vpar[h][o]) = *reinterpret_cast<const uint2*>(ps);
           else
-            vpar[i][0] = *reinterpret_cast<const uint32_t*>(ps);
+            vpar[h][o][0] = *reinterpret_cast<const uint32_t*>(ps);
         }
       }
     };
     bool ok = tiles > 0;
-    int64_t off_now = look_up(0), off_next = look_up(1);
+    int pg_next = entry(1);
+    const uint8_t* blk = block(0, entry(0));
     if (ok) {
-      load_k(off_now);
-      load_v(off_now);
+      load_k(blk);
+      load_v(blk);
     }
     for (int j = 0; ok && j < tiles; ++j) {
       const int buf = j & 1;
       const uint32_t ph = (j >> 1) & 1;
-      const uint32_t pages = __ballot_sync(0xffffffffu, off_now >= 0) & 0xffu;
-      off_now = off_next;
-      off_next = look_up(j + 2);
+      const bool there = blk != nullptr;
+      blk = block(j + 1, pg_next);
+      pg_next = entry(j + 2);
       // ---- keys
       if (j >= 2) ok = wait_all(&b_kfree[buf], ph ^ 1u);
       if (!ok) break;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int pos = 32 * i + kp;
+      for (int i = 0; i < 2; ++i) {
+        const int pos = dw * kKv4Block + 8 * i + hi;  // its swizzle is hi
         const uint32_t dst = s_k + buf * L::kK + pos * 128;
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-          const uint32_t par = half_of(kpar[i][gr]);
+          const uint32_t par = there ? half_of(kpar[i][gr]) : 0u;
           const uint32_t sc = __byte_perm(par, par, 0x1010), lo = __byte_perm(par, par, 0x3232);
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const uint32_t x = kw[i][2 * gr + w], y = x >> 8;
-            // pairs (e, e + 4): put in order by halves
-            const uint32_t a = hfma2_u(plain_even(x), sc, lo), c = hfma2_u(plain_odd(x), sc, lo);
-            const uint32_t d = hfma2_u(plain_even(y), sc, lo), f = hfma2_u(plain_odd(y), sc, lo);
-            sts128(dst + gr * (kPTile * 128) + (((2 * kc + w) ^ (pos & 7)) << 4), __byte_perm(a, c, 0x5410),
-                   __byte_perm(d, f, 0x5410), __byte_perm(a, c, 0x7632), __byte_perm(d, f, 0x7632));
+            // the eight elements in the order 0 4 1 5 2 6 3 7, as the queries'
+            sts128(dst + gr * (kPTile * 128) + (((2 * lo2 + w) ^ hi) << 4), hfma2_u(plain_even(x), sc, lo),
+                   hfma2_u(plain_odd(x), sc, lo), hfma2_u(plain_even(y), sc, lo), hfma2_u(plain_odd(y), sc, lo));
           }
         }
       }
       fence_async_proxy();
-      mbar_arrive(&b_kfull[buf]);
-      if (j + 1 < tiles) load_k(off_now);
+      arrive_warp(&b_kfull[buf]);
+      if (j + 1 < tiles) load_k(blk);
       // ---- values
       if (j >= 2) ok = wait_all(&b_vfree[buf], ph ^ 1u);
       if (!ok) break;
-      int bad[G];
+      int bad[G];  // the block's first position that is not finite, 16: none
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) bad[gr] = 0x7fffffff;
-      const int vpos = j * kPTile + 8 * h16;
-      uint32_t sc[4][G], lo[4][G];  // of position pairs
+      for (int gr = 0; gr < G; ++gr) bad[gr] = kKv4Block;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int h = 0; h < 2; ++h) {
+        const int vpos = j * kPTile + dw * kKv4Block + 8 * h + 2 * lo2;
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          // an exponent of all ones in either half: not finite
-          const uint32_t e = vpar[i][gr] & 0x7c007c00u;
-          if (vpos + i >= len) {
-            vpar[i][gr] = 0;
-          } else if ((e & 0xffffu) == 0x7c00u || (e >> 16) == 0x7c00u) {
-            vpar[i][gr] = 0;
-            bad[gr] = min(bad[gr], vpos + i);
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+          for (int gr = 0; gr < G; ++gr) {
+            // an exponent of all ones in either half: not finite
+            const uint32_t e = vpar[h][o][gr] & 0x7c007c00u;
+            if (vpos + o >= len || !there) {
+              vpar[h][o][gr] = 0;
+            } else if ((e & 0xffffu) == 0x7c00u || (e >> 16) == 0x7c00u) {
+              vpar[h][o][gr] = 0;
+              bad[gr] = min(bad[gr], 8 * h + 2 * lo2 + o);
+            }
           }
-        }
-      if (warp == 8) {  // its lanes 0-15 hold every position of the tile
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) bad[gr] = __reduce_min_sync(0xffffffffu, bad[gr]);
-        if (lane == 0) {
-          sh_pages[buf] = pages;
-#pragma unroll
-          for (int gr = 0; gr < G; ++gr) sh_bad[buf][gr] = bad[gr];
-        }
       }
+      uint32_t note = there ? 1u : 0u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int gr = 0; gr < G; ++gr) note |= __reduce_min_sync(0xffffffffu, static_cast<unsigned>(bad[gr])) << (8 + 8 * gr);
+      if (G == 1) note |= kKv4Block << 16;
+      if (lane == 0) sh_note[buf][dw] = note;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int h16 = 2 * dw + h;
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-          sc[i][gr] = half_of(__byte_perm(vpar[2 * i][gr], vpar[2 * i + 1][gr], 0x5410));
-          lo[i][gr] = half_of(__byte_perm(vpar[2 * i][gr], vpar[2 * i + 1][gr], 0x7632));
-        }
+          const uint32_t sc = half_of(__byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x5410));
+          const uint32_t lo = half_of(__byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x7632));
+          // row 64 gr + 8 i + e, positions 8 h16 + 2 q, + 1
+          const uint32_t dst =
+              s_v + buf * L::kV + (h16 >> 3) * (D * 128) + (64 * gr + hi) * 128 + (((h16 & 7) ^ hi) << 4) + lo2 * 4;
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        const uint32_t dst = s_v + buf * L::kV + (h16 >> 3) * (D * 128) + (64 * gr + 8 * ve) * 128;
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {  // elements 4 z .. 4 z + 3
-          uint32_t o[4][4];            // element, position pair
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t x = __byte_perm(vw[(2 * i) * G + gr], vw[(2 * i + 1) * G + gr], z ? 0x7632 : 0x5410);
+          for (int z = 0; z < 2; ++z) {
+            const uint32_t x = __byte_perm(vw[h][0][gr], vw[h][1][gr], z ? 0x7632 : 0x5410);
             const uint32_t y = x >> 8;
-            o[0][i] = hfma2_u(plain_even(x), sc[i][gr], lo[i][gr]);
-            o[1][i] = hfma2_u(plain_odd(x), sc[i][gr], lo[i][gr]);
-            o[2][i] = hfma2_u(plain_even(y), sc[i][gr], lo[i][gr]);
-            o[3][i] = hfma2_u(plain_odd(y), sc[i][gr], lo[i][gr]);
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int d = 4 * z + x;  // row 64 gr + 8 ve + d: its swizzle is d
-            sts128(dst + d * 128 + (((h16 & 7) ^ d) << 4), o[x][0], o[x][1], o[x][2], o[x][3]);
+            sts32(dst + (4 * z) * 1024, hfma2_u(plain_even(x), sc, lo));
+            sts32(dst + (4 * z + 1) * 1024, hfma2_u(plain_odd(x), sc, lo));
+            sts32(dst + (4 * z + 2) * 1024, hfma2_u(plain_even(y), sc, lo));
+            sts32(dst + (4 * z + 3) * 1024, hfma2_u(plain_odd(y), sc, lo));
           }
         }
       }
       fence_async_proxy();
-      mbar_arrive(&b_vfull[buf]);
-      if (j + 1 < tiles) load_v(off_now);
+      arrive_warp(&b_vfull[buf]);
+      if (j + 1 < tiles) load_v(blk);
     }
   } else {
-    if (lane == 0 && tiles > 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsIssue));
+    if (warp == 16 && lane == 0 && tiles > 0) {
     // ------------------------------------------------------------ MMA issuer
     const uint32_t idesc_s = idesc_f16_f32(kPRows, kPTile), idesc_o = idesc_f16_f32(kPRows, D);
     const uint64_t dq = umma_smem_desc_sw128(s_q), dk = umma_smem_desc_sw128(s_k), dv = umma_smem_desc_sw128(s_v);
@@ -600,7 +614,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
