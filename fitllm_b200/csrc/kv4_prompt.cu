@@ -2,11 +2,13 @@
 //
 // The same product as kv4_attn.cu for calls whose rows (tokens x heads of a KV head)
 // fill tensor-core tiles: a CTA takes 256 rows of a (sequence, KV head) pair as two
-// tiles of 128 and walks the positions they see in tiles of 128.  Per tile and row
+// tiles of 128 and walks the positions they see in steps of 64.  Per step and row
 // tile r:  S_r = Q_r.K^T (tcgen05, both operands in shared memory), P_r = 2^(S_r c -
 // m) on 128 threads that own a row each, O_r += P_r.V with P_r as the tensor-memory
-// operand, written over S_r.  While one row tile's exponentials are taken the other's
-// products run.
+// operand, written over S_r.  Tensor memory holds two steps of S for each row tile:
+// while a thread takes the exponentials of one, the MMAs before and behind the other
+// run (with one step of 128 positions the two waited for each other, 5,200 cycles
+// per 128 positions).
 //
 // Roles: warps 0-3 and 4-7 the softmax of row tiles 0 and 1, warps 8-15 decode the
 // cache (with four of them a tile took 5,400 cycles, their own instructions' latency),
@@ -19,9 +21,8 @@
 // two as in kv4_attn.cu.
 //
 // The reference m of a row moves only when a weight would exceed 2^15 (fp16's range for
-// P); the thread that moves it rescales its row of O_r, which no MMA touches then (the
-// products of the tile before completed with S_r).  A thread reads its scores twice
-// (the maximum, the weights), the next 32 on their way while it works on 32.
+// P); the thread that moves it rescales its row of O_r once the step before has been
+// added to it.
 //
 // A group of V whose scale or low is not finite must only reach the rows that see it,
 // and 0 x NaN would reach all: it enters as zeros, its first position is noted per
@@ -36,7 +37,8 @@ namespace fitq {
 namespace {
 
 constexpr int kPRows = 128;       // rows of a row tile (TMEM lanes)
-constexpr int kPTile = 128;       // positions of a tile
+constexpr int kPTile = 128;       // positions of a decoded tile
+constexpr int kPStep = 64;        // positions of a step
 constexpr int kPThreads = 640;     // five warpgroups
 constexpr int kPDecoders = 256;
 // Registers per thread: 96 at launch (61,440 in all), then softmax 128, decoders 80,
@@ -71,17 +73,33 @@ struct Kv4PromptParams {
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N) {
   return (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
+// MMAs and commits of a warp that runs as one, issued by its elected lane: with the
+// loop around them uniform the operands are computed in uniform registers (from one
+// lane's branch every MMA took nine moves there, 90 cycles an MMA).
 __device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                             uint32_t accumulate) {
-  umma_bf16_ss(tmem_d, adesc, bdesc, idesc, accumulate);  // the type is the descriptor's
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
                                             uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void commit_warp(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
@@ -101,6 +119,14 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -159,7 +185,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4PromptParams p) {
   using L = PromptSmem<D>;
   constexpr int G = D / 64;
-  __shared__ uint64_t b_qready, b_kfull[2], b_kfree[2], b_vfull[2], b_vfree[2], b_sfull[2], b_pready[2], b_ofull, b_done;
+  __shared__ uint64_t b_qready, b_kfull[2], b_kfree[2], b_vfull[2], b_vfree[2], b_sfull[2][2], b_pready[2][2], b_odone[2], b_done;
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_abort;
   // per buffer and block: 1 if it has a page, and from bit 8 and 16 the first position
@@ -203,10 +229,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
       mbar_init(&b_vfull[i], kPDecoders / 32);
       mbar_init(&b_kfree[i], 1);
       mbar_init(&b_vfree[i], 1);
-      mbar_init(&b_sfull[i], 1);
-      mbar_init(&b_pready[i], kPRows / 32);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&b_sfull[i][h], 1);
+        mbar_init(&b_pready[i][h], kPRows / 32);
+      }
+      mbar_init(&b_odone[i], 1);
     }
-    mbar_init(&b_ofull, 1);
     mbar_init(&b_done, 1);
     fence_mbar_init();
   }
@@ -283,23 +311,28 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     uint32_t nan_groups = 0;
     bool ok = active && tiles > 0;
     const uint64_t cn2 = pack2(cn, cn);
-    for (int j = 0; ok && j < tiles; ++j) {
-      const int buf = j & 1;
-      const uint32_t ph = (j >> 1) & 1;
+    const int steps = (len + kPStep - 1) / kPStep;
+    for (int t = 0; ok && t < steps; ++t) {
+      const int j = t >> 1, h = t & 1, buf = j & 1;
+      const int pos0 = t * kPStep;
       // the tile's notes are there once V is decoded
-      ok = wait_all(&b_vfull[buf], ph) && wait_all(&b_sfull[r], j & 1);
+      if (h == 0) {
+        ok = wait_all(&b_vfull[buf], (j >> 1) & 1);
+        if (!ok) break;
+      }
+      ok = wait_all(&b_sfull[r][h], j & 1);
       if (!ok) break;
       tc_fence_after();
-      uint32_t pages = 0xffu;  // which blocks are there
-      const int pos0 = j * kPTile;
-      const uint4 na = *reinterpret_cast<const uint4*>(&sh_note[buf][0]);
-      const uint4 nb = *reinterpret_cast<const uint4*>(&sh_note[buf][4]);
+      uint32_t v[2][32];
+      tmem_ld_32x32b_x32(t_s + h * kPStep, v[0]);
+      tmem_ld_32x32b_x32(t_s + h * kPStep + 32, v[1]);
+      uint32_t pages = 0xfu;  // which of the step's blocks are there
+      const uint4 nt = *reinterpret_cast<const uint4*>(&sh_note[buf][4 * h]);
       constexpr uint32_t kClean = 1u | (kKv4Block << 8) | (kKv4Block << 16);
-      if (((na.x ^ kClean) | (na.y ^ kClean) | (na.z ^ kClean) | (na.w ^ kClean) | (nb.x ^ kClean) | (nb.y ^ kClean) |
-           (nb.z ^ kClean) | (nb.w ^ kClean)) != 0) {
+      if (((nt.x ^ kClean) | (nt.y ^ kClean) | (nt.z ^ kClean) | (nt.w ^ kClean)) != 0) {
         pages = 0;
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t note = sh_note[buf][i];
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t note = sh_note[buf][4 * h + i];
           pages |= (note & 1u) << i;
           for (int gr = 0; gr < G; ++gr) {
             const int at = static_cast<int>((note >> (8 + 8 * gr)) & 0xffu);
@@ -307,84 +340,72 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
           }
         }
       }
-      const bool masked = pos0 + kPTile > sure || pages != 0xffu;
-      // ---- the largest score; hidden ones become -inf in tensor memory too
-      float raw = -INFINITY, raw1 = -INFINITY, raw2 = -INFINITY, raw3 = -INFINITY;
-      {
-        uint32_t v[2][32];
-        tmem_ld_32x32b_x32(t_s, v[0]);
+      tmem_ld_wait();
+      if (pos0 + kPStep > sure || pages != 0xfu) {  // hidden positions
+        const int left = lim - pos0;                // elements 0 .. left are visible
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t(&x)[32] = v[c & 1];
-          tmem_ld_wait();
-          if (c < 3) tmem_ld_32x32b_x32(t_s + 32 * (c + 1), v[(c + 1) & 1]);
-          if (masked) {
-            const uint32_t pg = pages >> (2 * c);
-            const int left = lim - pos0 - 32 * c;  // elements 0 .. left are visible
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i > left || !(pg & (i < 16 ? 1u : 2u))) x[i] = 0xff800000u;
-            tmem_st_x32(t_s + 32 * c, x);
-          }
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            raw = fmaxf(raw, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
-            raw1 = fmaxf(raw1, fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
-            raw2 = fmaxf(raw2, fmaxf(__uint_as_float(x[i + 4]), __uint_as_float(x[i + 5])));
-            raw3 = fmaxf(raw3, fmaxf(__uint_as_float(x[i + 6]), __uint_as_float(x[i + 7])));
-          }
-        }
-        if (masked) tmem_st_done();
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i > left || !(pages & (1u << (2 * c + (i >> 4))))) v[c][i] = 0xff800000u;
       }
-      raw = fmaxf(fmaxf(raw, raw1), fmaxf(raw2, raw3)) * cn;
+      float top[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) top[x] = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            top[x] = fmaxf(top[x], fmaxf(__uint_as_float(v[c][i + 2 * x]), __uint_as_float(v[c][i + 2 * x + 1])));
+      const float raw = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cn;
       if (__any_sync(0xffffffffu, raw > m + kPRoom)) {
         const float m_new = fmaxf(m, raw);
         const float al = exp2_approx(m - m_new);
         m = m_new;
         l *= al;
-        if (j > 0) {
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(t_o + 32 * c, v);
+        if (t > 0) {
+          ok = wait_all(&b_odone[r], (t - 1) & 1);  // the step before has been added
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t x[16];
+            tmem_ld_x16(t_o + 16 * c, x);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * al);
-            tmem_st_x32(t_o + 32 * c, v);
+            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * al);
+            tmem_st_x16(t_o + 16 * c, x);
           }
         }
       }
-      // ---- weights, written over the scores (chunk c's lie where chunk c / 2's were)
-      {
-        const uint64_t m2 = pack2(-m, -m);
-        uint64_t s2 = 0;
-        uint32_t v[2][32];
-        tmem_ld_32x32b_x32(t_s, v[0]);
+      // ---- weights, written over the scores
+      const uint64_t m2 = pack2(-m, -m);
+      uint64_t s2[2] = {0, 0};
+      uint32_t pk[32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t(&x)[32] = v[c & 1];
-          tmem_ld_wait();
-          if (c < 3) tmem_ld_32x32b_x32(t_s + 32 * (c + 1), v[(c + 1) & 1]);
-          uint32_t pk[16];
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float x0, x1;
-            unpack2(fma2(pack2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), cn2, m2), x0, x1);
-            const float w0 = exp2_approx(x0), w1 = exp2_approx(x1);
-            s2 = add2(s2, pack2(w0, w1));
-            pk[i / 2] = pack_half2(w0, w1);
-          }
-          tmem_st_x16(t_s + 16 * c, pk);
+        for (int i = 0; i < 32; i += 2) {
+          float x0, x1;
+          unpack2(fma2(pack2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), cn2, m2), x0, x1);
+          const float w0 = exp2_approx(x0), w1 = exp2_approx(x1);
+          s2[(i >> 1) & 1] = add2(s2[(i >> 1) & 1], pack2(w0, w1));
+          pk[16 * c + i / 2] = pack_half2(w0, w1);
         }
-        float a, c;
-        unpack2(s2, a, c);
-        l += a + c;
-      }
+      tmem_st_x32(t_s + h * kPStep, pk);
+      float a, c2;
+      unpack2(add2(s2[0], s2[1]), a, c2);
+      l += a + c2;
       tmem_st_done();
       tc_fence_before();
-      arrive_warp(&b_pready[r]);
+      arrive_warp(&b_pready[r][h]);
     }
-    if (ok) ok = wait_all(&b_ofull, 0);
+    // the last two steps' products, one by one: a wait by parity tells a phase from its
+    // neighbour only (the one before these is done, S of the last step came behind it)
+    if (ok && steps > 1) ok = wait_all(&b_odone[r], (steps - 2) & 1);
+    if (ok) ok = wait_all(&b_odone[r], (steps - 1) & 1);
     if (active && (ok || tiles == 0)) {
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 2.f / l;  // values entered halved
@@ -554,59 +575,56 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsIssue));
-    if (warp == 16 && lane == 0 && tiles > 0) {
+    if (warp == 16 && tiles > 0) {
     // ------------------------------------------------------------ MMA issuer
-    const uint32_t idesc_s = idesc_f16_f32(kPRows, kPTile), idesc_o = idesc_f16_f32(kPRows, D);
+    const uint32_t idesc_s = idesc_f16_f32(kPRows, kPStep), idesc_o = idesc_f16_f32(kPRows, D);
     const uint64_t dq = umma_smem_desc_sw128(s_q), dk = umma_smem_desc_sw128(s_k), dv = umma_smem_desc_sw128(s_v);
-    auto issue_s = [&](int r, int buf) {
+    const int steps = (len + kPStep - 1) / kPStep, last = two ? 1 : 0;
+    auto issue_s = [&](int r, int t) {  // scores of step t into its half of S_r
+      const int h = t & 1, buf = (t >> 1) & 1;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint64_t qa = dq + ((r * L::kQ + (kk >> 2) * (kPRows * 128) + (kk & 3) * 32) >> 4);
-        const uint64_t kb = dk + ((buf * L::kK + (kk >> 2) * (kPTile * 128) + (kk & 3) * 32) >> 4);
-        umma_f16_ss(tmem + r * 128, qa, kb, idesc_s, kk > 0 ? 1u : 0u);
+        const uint64_t kb = dk + ((buf * L::kK + (kk >> 2) * (kPTile * 128) + h * (kPStep * 128) + (kk & 3) * 32) >> 4);
+        umma_f16_ss(tmem + r * 128 + h * kPStep, qa, kb, idesc_s, kk > 0 ? 1u : 0u);
       }
+      commit_warp(&b_sfull[r][h]);
+      // the tile's last scores: its keys' buffer is free
+      if (r == last && (h == 1 || t == steps - 1)) commit_warp(&b_kfree[buf]);
     };
-    auto issue_o = [&](int r, int buf, bool add) {
+    auto issue_o = [&](int r, int t) {  // step t's weights times its values
+      const int h = t & 1, buf = (t >> 1) & 1;
 #pragma unroll
-      for (int kk = 0; kk < kPTile / 16; ++kk) {
-        const uint64_t vb = dv + ((buf * L::kV + (kk >> 2) * (D * 128) + (kk & 3) * 32) >> 4);
-        umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + kk * 8, vb, idesc_o, add || kk > 0 ? 1u : 0u);
+      for (int kk = 0; kk < kPStep / 16; ++kk) {
+        const uint64_t vb = dv + ((buf * L::kV + h * (D * 128) + kk * 32) >> 4);
+        umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + h * kPStep + kk * 8, vb, idesc_o, t > 0 || kk > 0 ? 1u : 0u);
       }
+      commit_warp(&b_odone[r]);
+      if (r == last && (h == 1 || t == steps - 1)) commit_warp(&b_vfree[buf]);
     };
-    bool ok = mbar_wait(&b_qready, 0, &sh_abort, p.status) && mbar_wait(&b_kfull[0], 0, &sh_abort, p.status);
+    bool ok = wait_all(&b_qready, 0) && wait_all(&b_kfull[0], 0);
     if (ok) {
       tc_fence_after();
-      issue_s(0, 0);
-      umma_commit(&b_sfull[0]);
-      if (two) {
-        issue_s(1, 0);
-        umma_commit(&b_sfull[1]);
-      }
-      umma_commit(&b_kfree[0]);
+      for (int t = 0; t < 2 && t < steps; ++t)
+        for (int r = 0; r <= last; ++r) issue_s(r, t);
     }
-    for (int j = 0; ok && j < tiles; ++j) {
-      const int buf = j & 1, nbuf = buf ^ 1;
-      const bool more = j + 1 < tiles;
-      if (!mbar_wait(&b_vfull[buf], (j >> 1) & 1, &sh_abort, p.status)) break;
-      for (int r = 0; ok && r < (two ? 2 : 1); ++r) {
-        if (!mbar_wait(&b_pready[r], j & 1, &sh_abort, p.status) ||
-            (more && r == 0 && !mbar_wait(&b_kfull[nbuf], ((j + 1) >> 1) & 1, &sh_abort, p.status))) {
-          ok = false;
-          break;
-        }
+    for (int t = 0; ok && t < steps; ++t) {
+      const int j = t >> 1, h = t & 1;
+      const bool more = t + 2 < steps;
+      if (h == 0) {
+        ok = wait_all(&b_vfull[j & 1], (j >> 1) & 1) &&
+             (!more || wait_all(&b_kfull[(j + 1) & 1], ((j + 1) >> 1) & 1));
+      }
+      for (int r = 0; ok && r <= last; ++r) {
+        ok = wait_all(&b_pready[r][h], j & 1);
+        if (!ok) break;
         tc_fence_after();
-        issue_o(r, buf, j > 0);
-        if (r == (two ? 1 : 0)) umma_commit(&b_vfree[buf]);
-        if (more) {
-          issue_s(r, nbuf);
-          umma_commit(&b_sfull[r]);
-          if (r == (two ? 1 : 0)) umma_commit(&b_kfree[nbuf]);
-        }
+        issue_o(r, t);
+        if (more) issue_s(r, t + 2);
       }
     }
-    if (ok) umma_commit(&b_ofull);
     // every MMA has retired before tensor memory is given back
-    umma_commit(&b_done);
+    commit_warp(&b_done);
     int never = 0;
     mbar_wait(&b_done, 0, &never, p.status);
     }
