@@ -347,9 +347,12 @@ int launch_kv4_attention(const Kv4Seq& seq, const void* q, int64_t q_stride, con
                          int dim, int dtype, int64_t max_new, int64_t max_len, void* workspace, int* status,
                          cudaStream_t st, int num_sms);
 
-// The same attention for calls of many rows, on tcgen05 (kv4_prompt.cu); no workspace.
+// The same attention for calls of many rows, on tcgen05 (kv4_prompt.cu).
+size_t kv4_prompt_workspace(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim,
+                            int num_sms);
 int launch_kv4_prompt(const Kv4Seq& seq, const void* q, int64_t q_stride, const void* pool, void* out, int heads,
-                      int dim, int dtype, int64_t max_new, int* status, cudaStream_t st);
+                      int dim, int dtype, int64_t max_new, int64_t max_len, void* workspace, int* status,
+                      cudaStream_t st, int num_sms);
 
 // Log probabilities of given tokens, entropy, top alternatives and their
 // gradient (logprob.cu).

@@ -1017,7 +1017,8 @@ bool prompt_rows(int group, int64_t max_new) { return group * max_new > 64; }
 
 size_t kv4_attention_workspace(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim,
                                int num_sms) {
-  if (prompt_rows(group, max_new)) return 16;
+  if (prompt_rows(group, max_new))
+    return kv4_prompt_workspace(batch, kv_heads, group, max_new, max_len, dim, num_sms);
   return attn_plan(batch, kv_heads, group, max_new, max_len, dim, num_sms).bytes;
 }
 
@@ -1026,7 +1027,8 @@ int launch_kv4_attention(const Kv4Seq& seq, const void* q, int64_t q_stride, con
                          cudaStream_t st, int num_sms) {
   const int group = heads / seq.kv_heads;
   if (prompt_rows(group, max_new))
-    return launch_kv4_prompt(seq, q, q_stride, pool, out, heads, dim, dtype, max_new, status, st);
+    return launch_kv4_prompt(seq, q, q_stride, pool, out, heads, dim, dtype, max_new, max_len, workspace, status, st,
+                             num_sms);
   const AttnPlan a = attn_plan(seq.batch, seq.kv_heads, group, max_new, max_len, dim, num_sms);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Kv4AttnParams p;

@@ -28,6 +28,10 @@
 // and 0 x NaN would reach all: it enters as zeros, its first position is noted per
 // tile, and rows that see the position answer NaN for the group.
 //
+// Where the pairs' row tiles are fewer than the SMs, a pair's positions are cut into up
+// to kPMaxSplits parts of equal tiles, a CTA each; they leave (O, m, l) per row in the
+// workspace and kv4_prompt_combine_kernel joins them in order (deterministic).
+//
 // Bound: the exponentials (16 per cycle and SM: 2,048 cycles per 256 x 128 tile) and
 // the MMAs (4 x 128^3: 2,048 cycles) alike.
 #include "kv4.cuh"
@@ -47,6 +51,7 @@ constexpr int kPRegsSoftmax = 128, kPRegsDecode = 80, kPRegsIssue = 64;
 static_assert(2 * kPRegsSoftmax + 2 * kPRegsDecode + kPRegsIssue <= 5 * 96, "more registers than the launch has");
 constexpr float kPFloor = -3.0e38f;
 constexpr float kPRoom = 15.f;    // weights stay below 2^15
+constexpr int kPMaxSplits = 32;   // a lane of the combining warp each
 
 template <int D>
 struct PromptSmem {
@@ -63,6 +68,8 @@ struct Kv4PromptParams {
   int64_t q_stride;
   void* out;
   const uint8_t* pool;
+  float* ml_part;  // [CTAs without splits][splits][256 rows][2], splits > 1 only
+  float* o_part;   // [..][D]
   int heads, group, row_pairs;
   float scale_log2;
   int* status;
@@ -208,7 +215,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   const int pre = s.prefix[b];
   const int64_t room = static_cast<int64_t>(s.max_pages) << s.page_shift;
   const int64_t rows_all = static_cast<int64_t>(count) * p.group;
-  if (rp == 0 && kvh == 0 && tid == 0 && count > 0 &&
+  if (rp == 0 && kvh == 0 && blockIdx.y == 0 && tid == 0 && count > 0 &&
       (pre < 0 || static_cast<int64_t>(pre) + count > room ||
        rows_all > static_cast<int64_t>(p.row_pairs) * 2 * kPRows))
     report_device_error(p.status, FITQ_ERR_ARG);
@@ -218,8 +225,14 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   const bool two = rows > kPRows;
   int64_t len64 = pre < 0 ? 0 : static_cast<int64_t>(pre) + (row0 + rows - 1) / p.group + 1;
   if (len64 > room) len64 = room;
-  const int len = static_cast<int>(len64);
-  const int tiles = (len + kPTile - 1) / kPTile;
+  // This CTA's part: `tiles` tiles from position at0 on.  Positions below are relative to at0.
+  const int len_all = static_cast<int>(len64);
+  const int tiles_all = (len_all + kPTile - 1) / kPTile;
+  const int share = (tiles_all + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y);
+  const int tile0 = min(static_cast<int>(blockIdx.y) * share, tiles_all);
+  const int tiles = min(share, tiles_all - tile0);
+  const int at0 = tile0 * kPTile;
+  const int len = min(len_all - at0, tiles * kPTile);
 
   if (tid == 0) {
     sh_abort = 0;
@@ -302,11 +315,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     arrive_warp(&b_qready);
     const uint32_t t_lane = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t t_s = tmem + t_lane + r * 128, t_o = tmem + t_lane + 256 + r * 128;
-    int lim = pre + tok;  // last visible position
-    if (lim >= len) lim = len - 1;
+    const int lim = min(pre + tok, len_all - 1) - at0;  // last visible position
     // every row of the CTA sees the positions before this one
     const int64_t sure64 = static_cast<int64_t>(pre) + row0 / p.group + 1;
-    const int sure = sure64 < len ? static_cast<int>(sure64) : len;
+    const int sure = (sure64 < len_all ? static_cast<int>(sure64) : len_all) - at0;
     float m = kPFloor, l = 0.f;
     uint32_t nan_groups = 0;
     bool ok = active && tiles > 0;
@@ -408,8 +420,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     if (ok) ok = wait_all(&b_odone[r], (steps - 1) & 1);
     if (active && (ok || tiles == 0)) {
       tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 2.f / l;  // values entered halved
+      const bool whole = gridDim.y == 1;
+      const float inv = !whole ? 2.f : (l == 0.f ? 0.f : 2.f / l);  // values entered halved
       T* dst = static_cast<T*>(p.out) + ((first + tok) * p.heads + hd) * D;
+      const int64_t part = (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * (2 * kPRows) + r * kPRows + lr;
+      if (!whole && has) *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(m, l);
 #pragma unroll 1
       for (int gr = 0; gr < G; ++gr) {
         uint32_t v[2][32];
@@ -425,7 +440,14 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
 #pragma unroll
           for (int x = 0; x < 8; ++x)
             f[x] = bad ? NAN : (l == 0.f ? 0.f : __uint_as_float(v[x >> 2][8 * (x & 3) + e]) * inv);
-          if (has) *reinterpret_cast<uint4*>(dst + 64 * gr + 8 * e) = pack8<T>(f);
+          if (!has) continue;
+          if (whole) {
+            *reinterpret_cast<uint4*>(dst + 64 * gr + 8 * e) = pack8<T>(f);
+          } else {
+            float* po = p.o_part + part * D + 64 * gr + 8 * e;
+            *reinterpret_cast<float4*>(po) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4*>(po + 4) = make_float4(f[4], f[5], f[6], f[7]);
+          }
         }
       }
     }
@@ -443,11 +465,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     // The page table's entry for this warp's block of tile j, and, one tile later (a use at
     // once would wait for the load), the block; null: no page.
     auto entry = [&](int j) -> int {
-      const int64_t pos = static_cast<int64_t>(j) * kPTile + dw * kKv4Block;
-      return j < tiles && pos < len ? s.page_table[static_cast<int64_t>(b) * s.max_pages + (pos >> s.page_shift)] : -2;
+      const int pos = j * kPTile + dw * kKv4Block;
+      return j < tiles && pos < len
+                 ? s.page_table[static_cast<int64_t>(b) * s.max_pages + ((at0 + pos) >> s.page_shift)]
+                 : -2;
     };
     auto block = [&](int j, int pg) -> const uint8_t* {
-      const int64_t pos = static_cast<int64_t>(j) * kPTile + dw * kKv4Block;
+      const int64_t pos = static_cast<int64_t>(at0) + j * kPTile + dw * kKv4Block;
       const bool there = pg >= 0 && pg < s.num_pages;
       if (!there && pg != -2 && lane == 0) report_device_error(p.status, FITQ_ERR_ARG);
       return there ? p.pool + kv4_block_offset(s, pg, kvh, pos, D) : nullptr;
@@ -638,28 +662,120 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   }
 }
 
+// Joins the parts of the rows.  A CTA takes eight rows of a row pair, a warp each: lane
+// c holds the weight of part c, then every lane D / 32 elements.
 template <typename T, int D>
-int prompt_t(const Kv4PromptParams& p, cudaStream_t st) {
+__global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Kv4PromptParams p, int splits) {
+  constexpr int kE = D / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  pdl_wait();  // the partials
+  const Kv4Seq& s = p.seq;
+  const int64_t cta = blockIdx.x;
+  const int per_pair = s.batch * s.kv_heads;
+  const int rp = p.row_pairs - 1 - static_cast<int>(cta / per_pair), pair = static_cast<int>(cta % per_pair);
+  const int b = pair / s.kv_heads, kvh = pair % s.kv_heads;
+  int64_t first;
+  int count;
+  kv4_tokens(s, b, first, count);
+  const int in_cta = static_cast<int>(blockIdx.y) * 8 + warp;
+  const int64_t row = static_cast<int64_t>(rp) * 2 * kPRows + in_cta;
+  if (row >= static_cast<int64_t>(count) * p.group) return;
+  const int64_t part0 = cta * splits * (2 * kPRows) + in_cta;  // part c: + c * 256
+  float2 ml = make_float2(kPFloor, 0.f);
+  if (lane < splits) ml = *reinterpret_cast<const float2*>(p.ml_part + (part0 + lane * (2 * kPRows)) * 2);
+  float mx = ml.y == 0.f ? kPFloor : ml.x;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+  // a part that saw nothing weighs 0, whatever its rows hold
+  const float w = ml.y == 0.f ? 0.f : exp2_approx(ml.x - mx);
+  float l = ml.y == 0.f ? 0.f : w * ml.y;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  const uint32_t live = __ballot_sync(0xffffffffu, ml.y != 0.f);
+  float f[kE];
+#pragma unroll
+  for (int x = 0; x < kE; ++x) f[x] = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < splits; ++c) {
+    const float k = __shfl_sync(0xffffffffu, w, c);
+    if (!((live >> c) & 1u)) continue;
+    const float* src = p.o_part + (part0 + static_cast<int64_t>(c) * (2 * kPRows)) * D + lane * kE;
+    float v[kE];
+    if (kE == 4)
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+    else
+      *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+    for (int x = 0; x < kE; ++x) f[x] = fmaf(k, v[x], f[x]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* dst = static_cast<T*>(p.out) + ((first + row / p.group) * p.heads + kvh * p.group + row % p.group) * D + lane * kE;
+  if (kE == 4)
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(Half16<T>::pack(f[0] * inv, f[1] * inv), Half16<T>::pack(f[kE - 2] * inv, f[kE - 1] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(dst) = Half16<T>::pack(f[0] * inv, f[1] * inv);
+}
+
+struct PromptPlan {
+  int row_pairs, splits;
+  int64_t ctas;  // without the splits
+  size_t o_off, bytes;
+};
+
+PromptPlan prompt_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim, int num_sms) {
+  PromptPlan a;
+  a.row_pairs = static_cast<int>((group * max_new + 2 * kPRows - 1) / (2 * kPRows));
+  a.ctas = static_cast<int64_t>(a.row_pairs) * batch * kv_heads;
+  // as many parts as leave no SM a second CTA, of four tiles or more
+  int64_t splits = num_sms / a.ctas;
+  const int64_t most = (max_len + 4 * kPTile - 1) / (4 * kPTile);
+  if (splits > most) splits = most;
+  if (splits > kPMaxSplits) splits = kPMaxSplits;
+  a.splits = static_cast<int>(splits < 1 ? 1 : splits);
+  const size_t rows = static_cast<size_t>(a.ctas) * a.splits * 2 * kPRows;
+  a.o_off = a.splits > 1 ? (rows * 2 * sizeof(float) + 255) & ~static_cast<size_t>(255) : 0;
+  a.bytes = a.splits > 1 ? a.o_off + rows * dim * sizeof(float) : 16;
+  return a;
+}
+
+template <typename T, int D>
+int prompt_t(const Kv4PromptParams& p, const PromptPlan& a, cudaStream_t st) {
   constexpr int smem = PromptSmem<D>::kBytes;
   if (!set_smem_limit(kv4_prompt_kernel<T, D>, smem)) return FITQ_ERR_CUDA;
-  const int64_t ctas = static_cast<int64_t>(p.row_pairs) * p.seq.batch * p.seq.kv_heads;
-  const cudaError_t e =
-      launch_pdl(kv4_prompt_kernel<T, D>, dim3(static_cast<unsigned>(ctas)), dim3(kPThreads), smem, st, p);
+  cudaError_t e = launch_pdl(kv4_prompt_kernel<T, D>, dim3(static_cast<unsigned>(a.ctas), a.splits), dim3(kPThreads),
+                             smem, st, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
+  if (a.splits > 1) {
+    e = launch_pdl(kv4_prompt_combine_kernel<T, D>, dim3(static_cast<unsigned>(a.ctas), 2 * kPRows / 8), dim3(256), 0, st,
+                   p, a.splits);
+    note_launch();
+    if (e != cudaSuccess) return FITQ_ERR_CUDA;
+  }
   return launch_result();
 }
 
 }  // namespace
 
+size_t kv4_prompt_workspace(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim,
+                            int num_sms) {
+  return prompt_plan(batch, kv_heads, group, max_new, max_len, dim, num_sms).bytes;
+}
+
 int launch_kv4_prompt(const Kv4Seq& seq, const void* q, int64_t q_stride, const void* pool, void* out, int heads,
-                      int dim, int dtype, int64_t max_new, int* status, cudaStream_t st) {
+                      int dim, int dtype, int64_t max_new, int64_t max_len, void* workspace, int* status,
+                      cudaStream_t st, int num_sms) {
   const int group = heads / seq.kv_heads;
-  const int row_pairs = static_cast<int>((group * max_new + 2 * kPRows - 1) / (2 * kPRows));
-  const Kv4PromptParams p{q, q_stride, out, static_cast<const uint8_t*>(pool), heads, group, row_pairs,
+  const PromptPlan a = prompt_plan(seq.batch, seq.kv_heads, group, max_new, max_len, dim, num_sms);
+  float* ml = static_cast<float*>(workspace);
+  float* o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + a.o_off);
+  const Kv4PromptParams p{q, q_stride, out, static_cast<const uint8_t*>(pool), ml, o, heads, group, a.row_pairs,
                           1.4426950408889634f / sqrtf(static_cast<float>(dim)), status, seq};
-  if (dtype == FITQ_DTYPE_BF16) return dim == 128 ? prompt_t<__nv_bfloat16, 128>(p, st) : prompt_t<__nv_bfloat16, 64>(p, st);
-  return dim == 128 ? prompt_t<__half, 128>(p, st) : prompt_t<__half, 64>(p, st);
+  if (dtype == FITQ_DTYPE_BF16)
+    return dim == 128 ? prompt_t<__nv_bfloat16, 128>(p, a, st) : prompt_t<__nv_bfloat16, 64>(p, a, st);
+  return dim == 128 ? prompt_t<__half, 128>(p, a, st) : prompt_t<__half, 64>(p, a, st);
 }
 
 }  // namespace fitq

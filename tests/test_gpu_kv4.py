@@ -151,6 +151,8 @@ ATTEND = [
     ([20000], [5], 5, 1, 128, 64, FP),
     # several row tiles, prompts with and without a prefix, empty sequences
     ([0], [200], 8, 2, 128, 64, BF), ([130, 0, 9], [40, 0, 97], 12, 4, 64, 16, FP), ([31], [65], 7, 1, 128, 16, FP),
+    # few row tiles over many positions: their parts joined behind the kernel
+    ([3000], [40], 8, 1, 128, 64, BF), ([5000, 900, 0], [30, 17, 20], 16, 4, 64, 32, FP), ([2300], [130], 4, 2, 128, 128, FP),
     ([0, 1, 700], [333, 17, 64], 40, 8, 128, 128, BF), ([0, 3], [129, 128], 16, 16, 64, 32, BF),
 ]
 
