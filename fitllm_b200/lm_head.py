@@ -161,6 +161,12 @@ class LMHeadLoss:
         h2 = h.reshape(-1, h.shape[-1]).contiguous()
         return ops.gemm_bf16_tn(self._norm(h2), self.weight).view(*h.shape[:-1], self.vocab)
 
+    def token_logprobs(self, h: torch.Tensor, ids: torch.Tensor, top: int = 0) -> TokenLogProbs:
+        """token_logprobs of the lm_head logits of h [..., H] bf16 for ids [...],
+        differentiable with respect to h (the head is frozen): policy or preference
+        losses on log probabilities instead of the mean cross-entropy."""
+        return token_logprobs(_LogitsFn.apply(h, self), ids, top)
+
     def loss_and_grad(self, h: torch.Tensor, labels: torch.Tensor,
                       loss_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
         """One micro-batch: h [B, S, H] bf16 (last layer output), labels [B, S]
@@ -200,6 +206,27 @@ class LMHeadLoss:
             grad[i:i + 1] = g
             losses.append(loss)
         return losses, grad
+
+
+class _LogitsFn(torch.autograd.Function):
+    """LMHeadLoss.logits with the gradient with respect to h."""
+
+    @staticmethod
+    def forward(ctx, h, head: LMHeadLoss):
+        h2 = h.reshape(-1, h.shape[-1]).contiguous()
+        ctx.head = head
+        ctx.save_for_backward(h2)
+        with torch.cuda.device(h.device):
+            return ops.gemm_bf16_tn(head._norm(h2), head.weight).view(*h.shape[:-1], head.vocab)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d):
+        h2, = ctx.saved_tensors
+        head = ctx.head
+        with torch.cuda.device(d.device):
+            dx = ops.gemm_bf16_tn(d.reshape(-1, head.vocab), head.weight_t)
+            return head._norm_bwd(dx, h2).view(*d.shape[:-1], h2.shape[-1]), None
 
 
 def random_lm_head(hidden: int, vocab: int, device, seed: int = 0, std: float = 0.02,
