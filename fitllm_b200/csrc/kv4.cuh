@@ -150,6 +150,10 @@ __device__ __forceinline__ uint32_t nibbles(uint32_t x) {
 // 1024 + c of the low nibble of each half; 1024 + 16 c of the second one.
 __device__ __forceinline__ uint32_t codes_even(uint32_t x) { return nibbles<0x000f000fu>(x); }
 __device__ __forceinline__ uint32_t codes_odd(uint32_t x) { return nibbles<0x00f000f0u>(x); }
+// The codes as fp16 subnormals: 2^-24 c of the low nibble of each half, 2^-20 c of the
+// second one.
+__device__ __forceinline__ uint32_t tiny_even(uint32_t x) { return x & 0x000f000fu; }
+__device__ __forceinline__ uint32_t tiny_odd(uint32_t x) { return x & 0x00f000f0u; }
 // c - 8 of either.
 __device__ __forceinline__ uint32_t centre_even(uint32_t u) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));

@@ -108,14 +108,26 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// d = a.b + c with c apart from d (an accumulator's first product).
-__device__ __forceinline__ void mma_f16_init(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1, float c0, float c1) {
+// d = a.b with eight along k.
+__device__ __forceinline__ void mma_f16_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
   asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%10, %11, %10, %11};"
+      "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
+
+// Two 8 x 8 matrices of 16-bit elements, transposed; lanes 0-15 give the rows' addresses.
+__device__ __forceinline__ void ldmatrix2_t(uint32_t& a, uint32_t& b, const void* row) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];"
+               : "=r"(a), "=r"(b)
+               : "r"(smem_u32(row))
+               : "memory");
+}
+
+__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(as_half2(a), as_half2(b));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // Tiles of sequence b that columns [col0, col0 + R) see, and its lengths.
@@ -155,17 +167,17 @@ struct AttnSmem {
   static constexpr int kMerge = S::kWarps * kR * kLd * 4;
   static constexpr int kMl = kRing + kMerge;                        // [warp][R][2] floats
   // queries of two segments, each: fragments [group][word][nt][lane] uint4, then
-  // (sum, offsets) [R][D / 64] and the exponent factors [R]
+  // group sums [R][D / 64] (half2: value, rest) and the exponent factors [R]
   static constexpr int kQ = kMl + S::kWarps * kR * 2 * 4;
   static constexpr int kQsum = (D / 64) * 2 * NT * 512;
-  static constexpr int kQexp = kQsum + kR * (D / 64) * 8;
+  static constexpr int kQexp = kQsum + kR * (D / 64) * 4;
   static constexpr int kQBytes = (kQexp + kR * 4 + 15) & ~15;
   static constexpr int kBars = kQ + 2 * kQBytes;
   static constexpr int kBytes = kBars + S::kWarps * S::kStages * 8;
 };
 
-// Weights times scales stay below 2^15 in fp16; a reference that moves leaves this
-// much (log2) to the weights that follow.
+// Weights, and weights times scales, stay below 2^15 in fp16; a reference that moves
+// leaves this much (log2) to the weights that follow.
 constexpr float kRoom = 15.f, kSlack = 8.f;
 // A pair's first tile costs a run this many tiles more (queries, the pipeline's
 // start, the warps' meeting): runs are cut by cost.
@@ -206,6 +218,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   constexpr int kBlk = kv4_block_bytes(D);
   constexpr int kLd = L::kLd;
   constexpr int kWarps = S::kWarps, kTile = S::kTile, kStages = S::kStages, kThreads = S::kThreads;
+  constexpr int kRowV = G == 2 ? 4 : 0;  // the values' first row among a position's quantities
   constexpr bool kQRegs = NT == 1;  // one column tile's query fragments fit in registers
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, qd = lane & 3;
@@ -391,7 +404,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   // with their group sums
   auto load_queries = [&](const Segment& g, uint8_t* to) {
     uint4* sq = reinterpret_cast<uint4*>(to);
-    float2* sqsum = reinterpret_cast<float2*>(to + L::kQsum);
+    uint32_t* sqsum = reinterpret_cast<uint32_t*>(to + L::kQsum);
     float* sqexp = reinterpret_cast<float*>(to + L::kQexp);
     const SeqSpan& sp = g.sp;
     const int kvh = g.kvh;
@@ -417,8 +430,8 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       int e = (__float_as_int(mx) >> 23) - 127;
-      e = (mx == 0.f || e > 127) ? 12 : (e < -100 ? -100 : e);
-      const float up = pow2(12 - e);
+      e = (mx == 0.f || e > 127) ? 15 : (e < -100 ? -100 : e);
+      const float up = pow2(15 - e);
 #pragma unroll
       for (int gr = 0; gr < G; ++gr) {
         float even = 0.f, odd = 0.f;
@@ -437,14 +450,14 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           sq[((gr * 2 + w) * NT + (n >> 3)) * 32 + (n & 7) * 4 + c] =
               make_uint4(pack_half2(f[0], f[4]), pack_half2(f[1], f[5]), pack_half2(f[2], f[6]), pack_half2(f[3], f[7]));
         }
-        float sum = fmaf(16.f, odd, even), off = 1024.f * (even + odd);
+        float sum = fmaf(16.f, odd, even);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        off += __shfl_xor_sync(0xffffffffu, off, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        off += __shfl_xor_sync(0xffffffffu, off, 2);
-        if (c == 0) sqsum[n * G + gr] = make_float2(sum, -off);
+        sum *= pow2(-24);
+        const float hi = __half2float(__float2half_rn(sum));
+        if (c == 0) sqsum[n * G + gr] = pack_half2(hi, sum - hi);
       }
-      if (c == 0) sqexp[n] = p.scale_log2 * pow2(e - 12);
+      if (c == 0) sqexp[n] = p.scale_log2 * pow2(min(e + 9, 127));
     }
   };
 
@@ -460,7 +473,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     const int pos_first = first_position(sg), blocks = block_count(sg), len = sg.sp.len;
     const uint8_t* sq_now = g_kv4_smem + L::kQ + buf * L::kQBytes;
     const uint4* sq = reinterpret_cast<const uint4*>(sq_now);
-    const float2* sqsum = reinterpret_cast<const float2*>(sq_now + L::kQsum);
+    const uint32_t* sqsum = reinterpret_cast<const uint32_t*>(sq_now + L::kQsum);
     const float* sqexp = reinterpret_cast<const float*>(sq_now + L::kQexp);
     buf ^= 1;
     __syncthreads();  // the queries are there, the merge buffer and the last segment's place are free
@@ -472,43 +485,43 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
 #pragma unroll
         for (int w = 0; w < 2; ++w) qf[kQRegs ? gr : 0][w] = sq[(gr * 2 + w) * 32 + lane];
     }
-    float qs[NT][2][G], qo[NT][2][G], cn[NT][2];  // of the columns 2 qd, 2 qd + 1: sums, offsets, exponent per score
-    int lim[NT][2];                 // and the last position they see
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int n = 8 * nt + 2 * qd + e;
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          const float2 v = sqsum[n * G + gr];
-          qs[nt][e][gr] = v.x;
-          qo[nt][e][gr] = v.y;
-        }
-        cn[nt][e] = sqexp[n];
-        const int l = sg.sp.pre + (col0 + n) / p.group;
-        lim[nt][e] = l < len ? l : len - 1;
-      }
-    const int mask_from = sg.sp.pre + col0 / p.group + 1;  // positions every column sees lie before it
-
-    float m_run[NT][2], l_run[NT][2], corr[NT][2][G], o[NT][G][4][4];  // m_run in log2 units
-    // no scale met so far exceeds 2^cap_log2; weights stay below 2^(kRoom - cap_log2)
-    float cap = pow2(-30), room = kRoom + 30.f;
+    float cn[NT][2];  // of the columns 2 qd, 2 qd + 1: exponent per score
+    int lim[NT][2];   // and the last position they see
+    uint32_t qb[NT];  // the group sums as the operand that the keys' lows meet: (0, value or rest)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        m_run[nt][e] = kFloor;
-        l_run[nt][e] = 0.f;
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) corr[nt][e][gr] = 0.f;
+        const int n = 8 * nt + 2 * qd + e;
+        cn[nt][e] = sqexp[n];
+        const int l = sg.sp.pre + (col0 + n) / p.group;
+        lim[nt][e] = l < len ? l : len - 1;
       }
+      const uint32_t v = sqsum[(8 * nt + g) * G + (qd & (G - 1))];
+      qb[nt] = qd < G ? v << 16 : (qd < 2 * G ? v & 0xffff0000u : 0u);
+    }
+    const int mask_from = sg.sp.pre + col0 / p.group + 1;  // positions every column sees lie before it
+
+    // m_run in log2 units; o of the codes, off of the eights taken from them; sums: rows
+    // of the weights' products with the parameters (rows 0-7) and with one (rows 8-15)
+    float m_run[NT][2], o[NT][G][4][4], off[NT][G][4], sums[NT][4];
+    // no scale met so far exceeds cap; weights stay below 2^room
+    uint32_t cap = pack_half2(1.f, 1.f);
+    float room = kRoom;
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr)
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int e = 0; e < 2; ++e) m_run[nt][e] = kFloor;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][gr][i][e] = 0.f;
+      for (int e = 0; e < 4; ++e) {
+        sums[nt][e] = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+          off[nt][gr][e] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[nt][gr][i][e] = 0.f;
+        }
+      }
     }
 
     uint32_t set_valid = 0;
@@ -525,36 +538,28 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       const uint8_t* blk = ring + st * kBlk;
       const int pos0 = pos_first + j * kTile;
 
-      // ---- parameters of positions g and g + 8: {key, value} x groups x (scale, low)
-      float ks[2][G], kl[2][G], vs[2][G], vl[2][G];
+      const uint8_t* par = blk + 16 * D;  // [position][K, V][group](scale, low)
+      // ---- keys' parameters of positions g and g + 8
+      uint32_t kp[2][G];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t pr[2 * G];
-        const uint8_t* psrc = blk + 16 * D + (g + 8 * h) * 8 * G;
+        const uint8_t* at = par + (g + 8 * h) * 8 * G;
         if (G == 2)
-          *reinterpret_cast<uint4*>(pr) = *reinterpret_cast<const uint4*>(psrc);
+          *reinterpret_cast<uint2*>(kp[h]) = *reinterpret_cast<const uint2*>(at);
         else
-          *reinterpret_cast<uint2*>(pr) = *reinterpret_cast<const uint2*>(psrc);
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          const float2 a = Half16<__half>::unpack(pr[gr]);
-          const float2 c = Half16<__half>::unpack(pr[G + gr]);
-          ks[h][gr] = a.x;
-          kl[h][gr] = a.y;
-          vs[h][gr] = c.x;
-          vl[h][gr] = fmaf(8.f, c.x, c.y);
-        }
-      }
-      if (edge) {  // whatever lies behind the last position must not matter
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (pos0 + g + 8 * h >= len)
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr) ks[h][gr] = kl[h][gr] = vs[h][gr] = vl[h][gr] = 0.f;
+          kp[h][0] = *reinterpret_cast<const uint32_t*>(at);
       }
 
-      // ---- S^T = K.Q^T, one accumulator set per group
-      float acc[NT][G][4];
+      // ---- S^T = K.Q^T, one accumulator set per group and one of the lows
+      float acc[NT][G][4], accl[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma_f16_k8(accl[nt], qd & (G - 1) ? kp[0][G - 1] : kp[0][0], qd & (G - 1) ? kp[1][G - 1] : kp[1][0], qb[nt]);
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[nt][gr][e] = 0.f;
+      }
       uint32_t kw[2][2 * G];
       if (G == 2) {
 #pragma unroll
@@ -572,7 +577,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           uint32_t x = kw[0][2 * gr + w], y = kw[1][2 * gr + w];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t a0 = codes_even(x), a1 = codes_even(y), a2 = codes_odd(x), a3 = codes_odd(y);
+            const uint32_t a0 = tiny_even(x), a1 = tiny_even(y), a2 = tiny_odd(x), a3 = tiny_odd(y);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               uint2 bq;
@@ -581,18 +586,48 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
                        : make_uint2(qf[kQRegs ? gr : 0][w].x, qf[kQRegs ? gr : 0][w].y);
               else
                 bq = *(reinterpret_cast<const uint2*>(&sq[((gr * 2 + w) * NT + nt) * 32 + lane]) + h);
-              if (w == 0 && h == 0)
-                mma_f16_init(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y, qo[nt][0][gr], qo[nt][1][gr]);
-              else
-                mma_f16(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y);
+              mma_f16(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y);
             }
             x >>= 8;
             y >>= 8;
           }
         }
 
+      // ---- values' parameters of positions 2 qd, 2 qd + 1 and 8 behind them: the scales
+      // side by side, and all eight quantities of a position as rows of an operand
+      uint32_t vs[2][G], va[2];
+      if (G == 2) ldmatrix2_t(va[0], va[1], par + (lane & 15) * 16);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* at = par + (2 * qd + 8 * h) * 8 * G + 4 * G;
+        if (G == 2) {
+          const uint2 a = *reinterpret_cast<const uint2*>(at), b = *reinterpret_cast<const uint2*>(at + 8 * G);
+          vs[h][0] = __byte_perm(a.x, b.x, 0x5410);
+          vs[h][G - 1] = __byte_perm(a.y, b.y, 0x5410);
+        } else {
+          const uint32_t a = *reinterpret_cast<const uint32_t*>(at), b = *reinterpret_cast<const uint32_t*>(at + 8 * G);
+          vs[h][0] = __byte_perm(a, b, 0x5410);
+          va[h] = g & 1 ? __byte_perm(a, b, 0x7632) : vs[h][0];
+        }
+      }
+
+      if (edge) {  // whatever lies behind the last position must not matter
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int gr = 0; gr < G; ++gr) {
+            const int left = len - pos0 - 2 * qd - 8 * h;
+            vs[h][gr] &= left > 1 ? 0xffffffffu : (left > 0 ? 0xffffu : 0u);
+          }
+      }
+
       // ---- scores in log2 units less the reference (position g: columns 2 qd, 2 qd + 1;
       // position g + 8: the same)
+      float ks[2][G];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) ks[h][gr] = __low2float(as_half2(kp[h][gr]));
       float sc[NT][4], x[NT][4];
       bool over = false;
 #pragma unroll
@@ -600,32 +635,31 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int h = e >> 1;
-          float v = ks[h][0] * acc[nt][0][e];
-          v = fmaf(kl[h][0], qs[nt][e & 1][0], v);
-          if (G == 2) {
-            v = fmaf(ks[h][G - 1], acc[nt][G - 1][e], v);
-            v = fmaf(kl[h][G - 1], qs[nt][e & 1][G - 1], v);
-          }
+          float v = fmaf(ks[h][0], acc[nt][0][e], accl[nt][e]);
+          if (G == 2) v = fmaf(ks[h][G - 1], acc[nt][G - 1][e], v);
           sc[nt][e] = v;
           x[nt][e] = fmaf(v, cn[nt][e & 1], -m_run[nt][e & 1]);
           if (edge && pos0 + g + 8 * h > lim[nt][e & 1]) sc[nt][e] = x[nt][e] = -INFINITY;
           over |= x[nt][e] > room;
         }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) over |= fabsf(vs[h][gr]) > cap;
+      __half2 vmax = __hmax2(__habs2(as_half2(vs[0][0])), __habs2(as_half2(vs[1][0])));
+      if (G == 2) vmax = __hmax2(vmax, __hmax2(__habs2(as_half2(vs[0][G - 1])), __habs2(as_half2(vs[1][G - 1]))));
+      over |= __hgt(__hmax(__low2half(vmax), __high2half(vmax)), __low2half(as_half2(cap)));
       if (__any_sync(0xffffffffu, over)) {
         float vm = 0.f;  // the largest finite scale of the block
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int gr = 0; gr < G; ++gr) vm = fmaxf(vm, fabsf(vs[h][gr]) <= 65504.f ? fabsf(vs[h][gr]) : 0.f);
-#pragma unroll
-        for (int o2 = 1; o2 < 32; o2 <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o2));
-        if (vm > cap) {
-          const int e = (__float_as_int(vm) >> 23) - 126;  // vm < 2^e
-          cap = pow2(e);
+          for (int gr = 0; gr < G; ++gr) {
+            const float2 v = Half16<__half>::unpack(vs[h][gr]);
+            vm = fmaxf(vm, fabsf(v.x) <= 65504.f ? fabsf(v.x) : 0.f);
+            vm = fmaxf(vm, fabsf(v.y) <= 65504.f ? fabsf(v.y) : 0.f);
+          }
+        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
+        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
+        if (vm > __low2float(as_half2(cap))) {
+          const int e = (__float_as_int(vm) >> 23) - 126;  // vm < 2^e; 2^16 is infinite, a cap like any other
+          cap = pack_half2(pow2(e), pow2(e));
           room = kRoom - static_cast<float>(e);
         }
 #pragma unroll
@@ -641,10 +675,12 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
             m_run[nt][e] = mx;
             x[nt][e] = fmaf(sc[nt][e], cn[nt][e], -mx);
             x[nt][2 + e] = fmaf(sc[nt][2 + e], cn[nt][e], -mx);
-            l_run[nt][e] *= al;
+            sums[nt][e] *= al;
+            sums[nt][2 + e] *= al;
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-              corr[nt][e][gr] *= al;
+              off[nt][gr][e] *= al;
+              off[nt][gr][2 + e] *= al;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 o[nt][gr][i][e] *= al;
@@ -654,34 +690,68 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           }
       }
 
-      // ---- weights, their scaled copies per group as the n8 operand of O^T
+      // ---- weights as an n8 operand, their products with the scales as those of O^T
       uint32_t pb[NT][G][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w[e] = exp2_approx(x[nt][e]);
-          l_run[nt][e & 1] += w[e];
-        }
+        for (int e = 0; e < 4; ++e) w[e] = exp2_approx(x[nt][e]);
+        const uint32_t p0 = pack_half2(w[0], w[1]), p1 = pack_half2(w[2], w[3]);
+        const uint32_t w0 = movmatrix_t(p0), w1 = movmatrix_t(p1);
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-          float ws[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int h = e >> 1;
-            ws[e] = w[e] * vs[h][gr];
-            if (edge && pos0 + g + 8 * h > lim[nt][e & 1])
-              ws[e] = 0.f;  // whatever the hidden value holds
-            else
-              corr[nt][e & 1][gr] = fmaf(w[e], vl[h][gr], corr[nt][e & 1][gr]);
-          }
-          pb[nt][gr][0] = movmatrix_t(pack_half2(ws[0], ws[1]));
-          pb[nt][gr][1] = movmatrix_t(pack_half2(ws[2], ws[3]));
+          pb[nt][gr][0] = mul_half2(w0, vs[0][gr]);
+          pb[nt][gr][1] = mul_half2(w1, vs[1][gr]);
         }
+        if (!edge) {
+          mma_f16(sums[nt], va[0], 0x3c003c00u, va[1], 0x3c003c00u, w0, w1);
+        } else {  // whatever a hidden value holds must not matter: visible ones one by one
+          const int la = __shfl_sync(0xffffffffu, lim[nt][0], g >> 1), lb = __shfl_sync(0xffffffffu, lim[nt][1], g >> 1);
+          const int last = (g & 1 ? lb : la) - pos0 - 2 * qd;  // column g's, from position 2 qd
+          const uint32_t keep0 = (last >= 0 ? 0xffffu : 0u) | (last >= 1 ? 0xffff0000u : 0u),
+                         keep1 = (last >= 8 ? 0xffffu : 0u) | (last >= 9 ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int gr = 0; gr < G; ++gr) {
+            pb[nt][gr][0] &= keep0;
+            pb[nt][gr][1] &= keep1;
+          }
+          const float2 r[2] = {Half16<__half>::unpack(p0), Half16<__half>::unpack(p1)};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float l = 0.f, c[G];
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) c[gr] = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float we = e ? r[h].y : r[h].x;
+              if (pos0 + g + 8 * h > lim[nt][e]) continue;
+              l += we;
+#pragma unroll
+              for (int gr = 0; gr < G; ++gr) {
+                const float2 v = Half16<__half>::unpack(
+                    *reinterpret_cast<const uint32_t*>(par + (g + 8 * h) * 8 * G + 4 * G + 4 * gr));
+                c[gr] = fmaf(we, fmaf(8.f, v.x, v.y), c[gr]);
+              }
+            }
+#pragma unroll
+            for (int y = 4; y < 32; y <<= 1) {
+              l += __shfl_xor_sync(0xffffffffu, l, y);
+#pragma unroll
+              for (int gr = 0; gr < G; ++gr) c[gr] += __shfl_xor_sync(0xffffffffu, c[gr], y);
+            }
+            sums[nt][2 + e] += l;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+              if (g == kRowV + 2 * gr + 1) sums[nt][e] += c[gr];
+          }
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr)
+          mma_f16(off[nt][gr], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pb[nt][gr][0], pb[nt][gr][1]);
       }
 
-      // ---- O^T += (V - 8)^T.P^T: rows g, g + 8 of m-tile i are elements 2 i, 2 i + 1 of eight
+      // ---- O^T += V^T.P^T: rows g, g + 8 of m-tile i are elements 2 i, 2 i + 1 of eight
       uint32_t vw[2][2][G];  // half h, position parity, group
       if (G == 2) {
 #pragma unroll
@@ -703,8 +773,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           uint32_t y = __byte_perm(vw[1][0][gr], vw[1][1][gr], z ? 0x7632 : 0x5410);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t a0 = centre_even(codes_even(x)), a1 = centre_odd(codes_odd(x)),
-                           a2 = centre_even(codes_even(y)), a3 = centre_odd(codes_odd(y));
+            const uint32_t a0 = tiny_even(x), a1 = tiny_odd(x), a2 = tiny_even(y), a3 = tiny_odd(y);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][gr][2 * z + i], a0, a1, a2, a3, pb[nt][gr][0], pb[nt][gr][1]);
             x >>= 8;
@@ -733,28 +802,25 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) {
-          l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], x);
-#pragma unroll
-          for (int gr = 0; gr < G; ++gr) corr[nt][e][gr] += __shfl_xor_sync(0xffffffffu, corr[nt][e][gr], x);
-        }
         const int n = 8 * nt + 2 * qd + e;
         float* row = mrg_o + (warp * R + n) * kLd;
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-          const float c = corr[nt][e][gr];
+          // sum of w (low + 8 scale), and the codes less eight back at their size
+          const int from = 4 * (kRowV + 2 * gr) + qd;
+          const float c = fmaf(8.f, __shfl_sync(0xffffffffu, sums[nt][e], from),
+                               __shfl_sync(0xffffffffu, sums[nt][e], from + 4));
           float f[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            f[2 * i] = o[nt][gr][i][e] + c;
-            f[2 * i + 1] = o[nt][gr][i][2 + e] + c;
+            f[2 * i] = fmaf(o[nt][gr][i][e] - off[nt][gr][e], 16777216.f, c);
+            f[2 * i + 1] = fmaf(fmaf(o[nt][gr][i][2 + e], 0.0625f, -off[nt][gr][e]), 16777216.f, c);
           }
           float* dst = row + 64 * gr + 8 * g;
           *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
           *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
         }
-        if (g == 0) *reinterpret_cast<float2*>(mrg_ml + (warp * R + n) * 2) = make_float2(m_run[nt][e], l_run[nt][e]);
+        if (g == 0) *reinterpret_cast<float2*>(mrg_ml + (warp * R + n) * 2) = make_float2(m_run[nt][e], sums[nt][2 + e]);
       }
     __syncthreads();
     const SeqSpan sp = sg.sp;
