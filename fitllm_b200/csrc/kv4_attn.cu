@@ -99,6 +99,10 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       : "memory");
 }
 
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
   asm(
@@ -106,6 +110,16 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// d = a.b.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // d = a.b with eight along k.
@@ -172,7 +186,8 @@ struct AttnSmem {
   static constexpr int kQsum = (D / 64) * 2 * NT * 512;
   static constexpr int kQexp = kQsum + kR * (D / 64) * 4;
   static constexpr int kQBytes = (kQexp + kR * 4 + 15) & ~15;
-  static constexpr int kBars = kQ + 2 * kQBytes;
+  static constexpr int kRaw = kQ + 2 * kQBytes;  // queries of the next segment as they came [R][D]
+  static constexpr int kBars = kRaw + kR * D * 2;
   static constexpr int kBytes = kBars + S::kWarps * S::kStages * 8;
 };
 
@@ -368,103 +383,101 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     const int first = first_position(g), end = g.tb * kTile < g.sp.len ? g.tb * kTile : g.sp.len;
     return first < end ? (end - first + kTile - 1) / kTile : 0;
   };
-  auto look_up = [&](const Segment& g, int j0) {
-    const int j = j0 + lane;
-    int pg = -1;
-    if (j < block_count(g)) {
-      const int64_t pos = first_position(g) + static_cast<int64_t>(j) * kTile;
-      pg = kv4_page(s, g.b, pos);
-      if (pg < 0)
-        report_device_error(p.status, FITQ_ERR_ARG);
+  // the table's entry for block j0 + lane, and the set's blocks once it is there
+  auto entry = [&](const Segment& g, int j0) {
+    const int64_t pos = first_position(g) + static_cast<int64_t>(j0 + lane) * kTile;
+    return j0 + lane < block_count(g) ? s.page_table[static_cast<int64_t>(g.b) * s.max_pages + (pos >> s.page_shift)] : -1;
+  };
+  auto resolve = [&](const Segment& g, int j0, int pg) -> uint32_t {
+    const bool has = pg >= 0 && pg < s.num_pages;
+    if (has)
+      src = p.pool + kv4_block_offset(s, pg, g.kvh, first_position(g) + static_cast<int64_t>(j0 + lane) * kTile, D);
+    else if (j0 + lane < block_count(g))
+      report_device_error(p.status, FITQ_ERR_ARG);
+    return __ballot_sync(0xffffffffu, has);
+  };
+  auto issue = [&](uint32_t set, int j) {
+    if (!((set >> (j & 31)) & 1u)) return;
+    if (lane == (j & 31)) {
+      const uint32_t st = issued % kStages;
+      mbar_arrive_expect_tx(&bars[st], kBlk);
+      bulk_load(ring + st * kBlk, src, kBlk, &bars[st]);
+    }
+    ++issued;
+  };
+  // blocks [0, next) of this segment have been issued, and once they are all, [0, ahead) of
+  // the one behind it, whose table entries are on their way since this one began
+  int next = 0, ahead = 0, ahead_most = 0, ahead_entry = -1;
+  uint32_t ahead_valid = 0;
+  auto issue_ahead = [&](const Segment& g) {
+    if (ahead == 0) ahead_valid = resolve(g, 0, ahead_entry);
+    issue(ahead_valid, ahead);
+    ++ahead;
+  };
+
+  // ---- a segment's queries: set out for shared memory, then into buffer `to`: columns
+  // scaled to fp16's range, in the order in which the codes leave their words (element
+  // pairs (e, e + 4) of eight), with their group sums
+  uint8_t* raw = g_kv4_smem + L::kRaw;
+  auto fetch_queries = [&](const Segment& g) {
+    for (int i = tid; i < R * (D / 8); i += kThreads) {
+      const int n = i / (D / 8), d0 = (i % (D / 8)) * 8;
+      const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
+      if (n < g.sp.cols)
+        cp_async16(raw + i * 16, static_cast<const T*>(p.q) + (g.sp.first + tok) * p.q_stride +
+                                     static_cast<int64_t>(g.kvh * p.group + hd) * D + d0);
       else
-        src = p.pool + kv4_block_offset(s, pg, g.kvh, pos, D);
+        *reinterpret_cast<uint4*>(raw + i * 16) = make_uint4(0, 0, 0, 0);
     }
-    valid = __ballot_sync(0xffffffffu, pg >= 0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  int next = 0;  // next block to issue: at most kStages ahead of the first unread one
-  auto issue_next = [&](const Segment& g) {
-    if ((next & 31) == 0 && next > 0) look_up(g, next);
-    if ((valid >> (next & 31)) & 1u) {
-      if (lane == (next & 31)) {
-        const uint32_t st = issued % kStages;
-        mbar_arrive_expect_tx(&bars[st], kBlk);
-        bulk_load(ring + st * kBlk, src, kBlk, &bars[st]);
-      }
-      ++issued;
-    }
-    ++next;
-  };
-  auto start = [&](const Segment& g) {
-    next = 0;
-    const int n = block_count(g);
-    for (int i = 0; i < kStages && i < n; ++i) issue_next(g);
-  };
-  // ---- a segment's queries into buffer `to`: columns scaled to fp16's range, in the
-  // order in which the codes leave their words (element pairs (e, e + 4) of eight),
-  // with their group sums
-  auto load_queries = [&](const Segment& g, uint8_t* to) {
+  auto load_queries = [&](uint8_t* to) {
     uint4* sq = reinterpret_cast<uint4*>(to);
     uint32_t* sqsum = reinterpret_cast<uint32_t*>(to + L::kQsum);
     float* sqexp = reinterpret_cast<float*>(to + L::kQexp);
-    const SeqSpan& sp = g.sp;
-    const int kvh = g.kvh;
-    for (int i = tid; i < R * 4; i += kThreads) {
-      const int n = i >> 2, c = i & 3;  // four neighbouring lanes hold a column
-      const bool has = n < sp.cols;
-      const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
-      const T* qp = static_cast<const T*>(p.q) + (sp.first + tok) * p.q_stride +
-                    static_cast<int64_t>(kvh * p.group + hd) * D;
-      uint4 u[G][2];
-      float mx = 0.f;
+    // eight elements a thread, from the CTA's upper half on (the lower one joins the warps' parts)
+    for (int i = (tid + kThreads / 2) % kThreads; i < R * 8 * G; i += kThreads) {
+      const int n = i / (8 * G), gr = (i >> 3) % G, w = (i >> 2) & 1, c = i & 3;
+      float f[8], mx = 0.f;
+      unpack8<T>(*reinterpret_cast<const uint4*>(raw + (n * D + 64 * gr + 16 * c + 8 * w) * 2), f);
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr)
+      for (int x = 0; x < 8; ++x) mx = fmaxf(mx, fabsf(f[x]));
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          u[gr][w] = make_uint4(0, 0, 0, 0);
-          if (has) u[gr][w] = *reinterpret_cast<const uint4*>(qp + 64 * gr + 16 * c + 8 * w);
-          float f[8];
-          unpack8<T>(u[gr][w], f);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) mx = fmaxf(mx, fabsf(f[x]));
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      for (int x = 1; x < 8 * G; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
       int e = (__float_as_int(mx) >> 23) - 127;
       e = (mx == 0.f || e > 127) ? 15 : (e < -100 ? -100 : e);
       const float up = pow2(15 - e);
+      float even = 0.f, odd = 0.f;
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) {
-        float even = 0.f, odd = 0.f;
+      for (int x = 0; x < 8; x += 2) {
+        f[x] *= up;
+        f[x + 1] *= up * 0.0625f;
+        even += f[x];
+        odd += f[x + 1];
+      }
+      // lane 4 (n % 8) + c of the fragment of column tile n / 8
+      sq[((gr * 2 + w) * NT + (n >> 3)) * 32 + (n & 7) * 4 + c] =
+          make_uint4(pack_half2(f[0], f[4]), pack_half2(f[1], f[5]), pack_half2(f[2], f[6]), pack_half2(f[3], f[7]));
+      float sum = fmaf(16.f, odd, even);
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          float f[8];
-          unpack8<T>(u[gr][w], f);
-#pragma unroll
-          for (int x = 0; x < 8; x += 2) {
-            f[x] *= up;
-            f[x + 1] *= up * 0.0625f;
-            even += f[x];
-            odd += f[x + 1];
-          }
-          // lane 4 (n % 8) + c of the fragment of column tile n / 8
-          sq[((gr * 2 + w) * NT + (n >> 3)) * 32 + (n & 7) * 4 + c] =
-              make_uint4(pack_half2(f[0], f[4]), pack_half2(f[1], f[5]), pack_half2(f[2], f[6]), pack_half2(f[3], f[7]));
-        }
-        float sum = fmaf(16.f, odd, even);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      for (int x = 1; x < 8; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if ((i & 7) == 0) {
         sum *= pow2(-24);
         const float hi = __half2float(__float2half_rn(sum));
-        if (c == 0) sqsum[n * G + gr] = pack_half2(hi, sum - hi);
+        sqsum[n * G + gr] = pack_half2(hi, sum - hi);
       }
-      if (c == 0) sqexp[n] = p.scale_log2 * pow2(min(e + 9, 127));
+      if (i % (8 * G) == 0) sqexp[n] = p.scale_log2 * pow2(min(e + 9, 127));
     }
   };
+  auto queries_arrived = [&] { asm volatile("cp.async.wait_all;" ::: "memory"); };
 
-  look_up(sh_seg[0], 0);
-  start(sh_seg[0]);
-  load_queries(sh_seg[0], g_kv4_smem + L::kQ);
-  if (!kClustered && tid == 0) advance(sh_seg[1]);
+  fetch_queries(sh_seg[0]);
+  valid = resolve(sh_seg[0], 0, entry(sh_seg[0], 0));
+  for (const int n = min(kStages, block_count(sh_seg[0])); next < n; ++next) issue(valid, next);
+  if (!kClustered && tid == kThreads - 32) advance(sh_seg[1]);
+  queries_arrived();
+  __syncthreads();
+  load_queries(g_kv4_smem + L::kQ);
   int buf = 0;
   // a clustered CTA without tiles of its own still joins the others'
   for (int seg = 0, after = 1; kClustered || sh_seg[seg].tb > 0; seg = after, after = after == 2 ? 0 : after + 1) {
@@ -477,7 +490,15 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     const float* sqexp = reinterpret_cast<const float*>(sq_now + L::kQexp);
     buf ^= 1;
     __syncthreads();  // the queries are there, the merge buffer and the last segment's place are free
-    if (!kClustered && tid == 0) advance(sh_seg[after == 2 ? 0 : after + 1]);
+    if (!kClustered) {
+      if (tid == kThreads - 32) advance(sh_seg[after == 2 ? 0 : after + 1]);
+      ahead = ahead_most = 0;
+      if (sn.tb > 0) {
+        fetch_queries(sn);
+        ahead_most = min(kStages, block_count(sn));
+        ahead_entry = entry(sn, 0);
+      }
+    }
     uint4 qf[kQRegs ? G : 1][2];
     if (kQRegs) {
 #pragma unroll
@@ -525,12 +546,21 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     }
 
     uint32_t set_valid = 0;
+    auto feed = [&] {  // a place in the ring is free
+      if (next < blocks) {
+        if ((next & 31) == 0) valid = resolve(sg, next, entry(sg, next));
+        issue(valid, next);
+        ++next;
+      } else if (ahead < ahead_most) {
+        issue_ahead(sn);
+      }
+    };
     // block j; edge: some of its positions are hidden from some columns.  False once a wait ran out.
     auto block = [&](int j, auto edge_tag) -> bool {
       constexpr bool edge = decltype(edge_tag)::value;
       if ((j & 31) == 0) set_valid = valid;  // block j has been issued, its set is the current one
       if (!((set_valid >> (j & 31)) & 1u)) {  // no page: the block is hidden from every column
-        if (next < blocks) issue_next(sg);
+        feed();
         return true;
       }
       const uint32_t st = taken % kStages;
@@ -553,13 +583,8 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       // ---- S^T = K.Q^T, one accumulator set per group and one of the lows
       float acc[NT][G][4], accl[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
         mma_f16_k8(accl[nt], qd & (G - 1) ? kp[0][G - 1] : kp[0][0], qd & (G - 1) ? kp[1][G - 1] : kp[1][0], qb[nt]);
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][gr][e] = 0.f;
-      }
       uint32_t kw[2][2 * G];
       if (G == 2) {
 #pragma unroll
@@ -586,7 +611,10 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
                        : make_uint2(qf[kQRegs ? gr : 0][w].x, qf[kQRegs ? gr : 0][w].y);
               else
                 bq = *(reinterpret_cast<const uint2*>(&sq[((gr * 2 + w) * NT + nt) * 32 + lane]) + h);
-              mma_f16(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y);
+              if (w == 0 && h == 0)
+                mma_f16_first(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y);
+              else
+                mma_f16(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y);
             }
             x >>= 8;
             y >>= 8;
@@ -764,7 +792,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       }
       __syncwarp();  // every lane has read the block
       ++taken;
-      if (next < blocks) issue_next(sg);
+      feed();
 #pragma unroll
       for (int gr = 0; gr < G; ++gr)
 #pragma unroll
@@ -790,11 +818,12 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     for (int j = 0; j < inner && fine; ++j) fine = block(j, std::false_type{});
     for (int j = inner; j < blocks && fine; ++j) fine = block(j, std::true_type{});
 
-    // ---- the next segment's copies and queries set out before the warps meet
-    if (!kClustered && sn.tb > 0 && fine) {
-      look_up(sn, 0);
-      start(sn);
-      load_queries(sn, g_kv4_smem + L::kQ + buf * L::kQBytes);
+    // ---- the rest of the next segment's first copies
+    if (!kClustered) {
+      while (fine && ahead < ahead_most) issue_ahead(sn);
+      next = ahead;
+      valid = ahead_valid;
+      queries_arrived();
     }
 
     // ---- the warps' results meet in shared memory
@@ -823,6 +852,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
         if (g == 0) *reinterpret_cast<float2*>(mrg_ml + (warp * R + n) * 2) = make_float2(m_run[nt][e], sums[nt][2 + e]);
       }
     __syncthreads();
+    if (!kClustered && sn.tb > 0) load_queries(g_kv4_smem + L::kQ + buf * L::kQBytes);
     const SeqSpan sp = sg.sp;
     const int b = sg.b, kvh = sg.kvh;
     const bool whole = sg.ta == 0 && sg.tb == sp.tiles;
