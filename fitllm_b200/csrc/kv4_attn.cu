@@ -61,6 +61,7 @@ struct AttnShape {
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTile = kKv4Block * kWarps;  // positions per tile
   static constexpr int kStages = NT == 1 ? 4 : 3;   // blocks in flight per warp
+  static constexpr int kStep = NT == 1 ? 2 : 1;     // blocks taken at a time
 };
 // Running maxima start finite, so that masked scores (-inf) never meet -inf - -inf.
 constexpr float kFloor = -3.0e38f;
@@ -80,6 +81,7 @@ struct Kv4AttnParams {
   float* ml_part; // [row tiles][runs + pairs][R][2]
   Kv4Cut* cuts;   // [row tiles][runs]
   int heads, group;
+  int group_mul;  // ceil(2^16 / group): n / group for n of a few hundred
   float scale_log2;  // log2(e) / sqrt(D)
   int* status;
   Kv4Seq seq;
@@ -145,6 +147,11 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
 }
 
 // Tiles of sequence b that columns [col0, col0 + R) see, and its lengths.
+struct Columns {
+  int group, mul;
+  __device__ __forceinline__ int token(int n) const { return (n * mul) >> 16; }
+};
+
 struct SeqSpan {
   int64_t first;  // packed token of the sequence's first new token
   int count;      // new tokens
@@ -154,15 +161,15 @@ struct SeqSpan {
   int tiles;
 };
 
-__device__ __forceinline__ SeqSpan seq_span(const Kv4Seq& s, int b, int group, int col0, int R, int tile) {
+__device__ __forceinline__ SeqSpan seq_span(const Kv4Seq& s, int b, const Columns& c, int col0, int R, int tile) {
   SeqSpan r;
   kv4_tokens(s, b, r.first, r.count);
   r.pre = s.prefix[b];
-  int64_t total = static_cast<int64_t>(r.count) * group - col0;
+  int64_t total = static_cast<int64_t>(r.count) * c.group - col0;
   r.cols = total <= 0 ? 0 : (total > R ? R : static_cast<int>(total));
   int64_t len = 0;
   if (r.cols > 0 && r.pre >= 0) {
-    len = static_cast<int64_t>(r.pre) + (col0 + r.cols - 1) / group + 1;
+    len = static_cast<int64_t>(r.pre) + c.token(col0 + r.cols - 1) + 1;
     const int64_t room = static_cast<int64_t>(s.max_pages) << s.page_shift;
     if (len > room) len = room;
   }
@@ -234,10 +241,10 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   constexpr int kLd = L::kLd;
   constexpr int kWarps = S::kWarps, kTile = S::kTile, kStages = S::kStages, kThreads = S::kThreads;
   constexpr int kRowV = G == 2 ? 4 : 0;  // the values' first row among a position's quantities
-  constexpr bool kQRegs = NT == 1;  // one column tile's query fragments fit in registers
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, qd = lane & 3;
   const int col0 = blockIdx.y * R;
+  const Columns columns{p.group, p.group_mul};
 
   uint8_t* ring = g_kv4_smem + warp * (kStages * kBlk);
   float* mrg_o = reinterpret_cast<float*>(g_kv4_smem + L::kRing);
@@ -277,7 +284,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   const int per_thread = (s.batch + kThreads - 1) / kThreads;
   const int b_lo = tid * per_thread, b_hi = b_lo + per_thread < s.batch ? b_lo + per_thread : s.batch;
   int mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += pair_cost(seq_span(s, b, p.group, col0, R, kTile));
+  for (int b = b_lo; b < b_hi; ++b) mine += pair_cost(seq_span(s, b, columns, col0, R, kTile));
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -302,7 +309,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   {
     int at = before;
     for (int b = b_lo; b < b_hi; ++b) {
-      const SeqSpan sp = seq_span(s, b, p.group, col0, R, kTile);
+      const SeqSpan sp = seq_span(s, b, columns, col0, R, kTile);
       const int cost = pair_cost(sp);
       // sequence b covers [at * KVH, (at + cost) * KVH) of the list
       if (t_lo < t_hi && static_cast<uint32_t>(at) * s.kv_heads <= t_lo &&
@@ -324,12 +331,12 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     int b = sh_walk_b;
     g.tb = 0;
     if (t < t_hi) {
-      SeqSpan sp = seq_span(s, b, p.group, col0, R, kTile);
+      SeqSpan sp = seq_span(s, b, columns, col0, R, kTile);
       while (t < t_hi && g.tb == 0) {
         int cost = pair_cost(sp);
         while (t >= t0 + static_cast<uint32_t>(cost) * s.kv_heads) {  // next sequence with work
           t0 += static_cast<uint32_t>(cost) * s.kv_heads;
-          sp = seq_span(s, ++b, p.group, col0, R, kTile);
+          sp = seq_span(s, ++b, columns, col0, R, kTile);
           cost = pair_cost(sp);
         }
         g.kvh = static_cast<int>((t - t0) / static_cast<uint32_t>(cost));
@@ -354,7 +361,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       const int pair = static_cast<int>(blockIdx.x) / kCluster, rank = static_cast<int>(blockIdx.x) % kCluster;
       g.b = pair / s.kv_heads;
       g.kvh = pair % s.kv_heads;
-      g.sp = seq_span(s, g.b, p.group, col0, R, kTile);
+      g.sp = seq_span(s, g.b, columns, col0, R, kTile);
       const int share = (g.sp.tiles + kCluster - 1) / kCluster;
       g.ta = min(rank * share, g.sp.tiles);
       g.tb = min(g.ta + share, g.sp.tiles);
@@ -422,7 +429,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   auto fetch_queries = [&](const Segment& g) {
     for (int i = tid; i < R * (D / 8); i += kThreads) {
       const int n = i / (D / 8), d0 = (i % (D / 8)) * 8;
-      const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
+      const int tok = columns.token(col0 + n), hd = col0 + n - tok * p.group;
       if (n < g.sp.cols)
         cp_async16(raw + i * 16, static_cast<const T*>(p.q) + (g.sp.first + tok) * p.q_stride +
                                      static_cast<int64_t>(g.kvh * p.group + hd) * D + d0);
@@ -499,13 +506,6 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
         ahead_entry = entry(sn, 0);
       }
     }
-    uint4 qf[kQRegs ? G : 1][2];
-    if (kQRegs) {
-#pragma unroll
-      for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) qf[kQRegs ? gr : 0][w] = sq[(gr * 2 + w) * 32 + lane];
-    }
     float cn[NT][2];  // of the columns 2 qd, 2 qd + 1: exponent per score
     int lim[NT][2];   // and the last position they see
     uint32_t qb[NT];  // the group sums as the operand that the keys' lows meet: (0, value or rest)
@@ -515,17 +515,18 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       for (int e = 0; e < 2; ++e) {
         const int n = 8 * nt + 2 * qd + e;
         cn[nt][e] = sqexp[n];
-        const int l = sg.sp.pre + (col0 + n) / p.group;
+        const int l = sg.sp.pre + columns.token(col0 + n);
         lim[nt][e] = l < len ? l : len - 1;
       }
       const uint32_t v = sqsum[(8 * nt + g) * G + (qd & (G - 1))];
       qb[nt] = qd < G ? v << 16 : (qd < 2 * G ? v & 0xffff0000u : 0u);
     }
-    const int mask_from = sg.sp.pre + col0 / p.group + 1;  // positions every column sees lie before it
+    const int mask_from = sg.sp.pre + columns.token(col0) + 1;  // positions every column sees lie before it
 
-    // m_run in log2 units; o of the codes, off of the eights taken from them; sums: rows
-    // of the weights' products with the parameters (rows 0-7) and with one (rows 8-15)
-    float m_run[NT][2], o[NT][G][4][4], off[NT][G][4], sums[NT][4];
+    // m_run in log2 units; o of the codes, off of the eights taken from them (rows 0-7: group
+    // 0, 8-15: group 1); sums: the weights' products with the parameters (rows 0-7) and with
+    // one (rows 8-15)
+    float m_run[NT][2], o[NT][G][4][4], off[NT][4], sums[NT][4];
     // no scale met so far exceeds cap; weights stay below 2^room
     uint32_t cap = pack_half2(1.f, 1.f);
     float room = kRoom;
@@ -535,13 +536,11 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       for (int e = 0; e < 2; ++e) m_run[nt][e] = kFloor;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        sums[nt][e] = 0.f;
+        sums[nt][e] = off[nt][e] = 0.f;
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          off[nt][gr][e] = 0.f;
+        for (int gr = 0; gr < G; ++gr)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[nt][gr][i][e] = 0.f;
-        }
       }
     }
 
@@ -555,134 +554,136 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
         issue_ahead(sn);
       }
     };
-    // block j; edge: some of its positions are hidden from some columns.  False once a wait ran out.
-    auto block = [&](int j, auto edge_tag) -> bool {
+    // N blocks from j on; edge: some of their positions are hidden from some columns.  False
+    // once a wait ran out.
+    auto step = [&](int j, auto n_tag, auto edge_tag) -> bool {
+      constexpr int N = decltype(n_tag)::value;
       constexpr bool edge = decltype(edge_tag)::value;
-      if ((j & 31) == 0) set_valid = valid;  // block j has been issued, its set is the current one
-      if (!((set_valid >> (j & 31)) & 1u)) {  // no page: the block is hidden from every column
-        feed();
-        return true;
+      const uint8_t* blk[N];
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const uint32_t st = (taken + u) % kStages;
+        if (!mbar_wait(&bars[st], ((taken + u) / kStages) & 1u, &sh_abort, p.status)) return false;
+        blk[u] = ring + st * kBlk;
       }
-      const uint32_t st = taken % kStages;
-      if (!mbar_wait(&bars[st], (taken / kStages) & 1u, &sh_abort, p.status)) return false;
-      const uint8_t* blk = ring + st * kBlk;
-      const int pos0 = pos_first + j * kTile;
+      const int pos0 = pos_first + j * kTile;  // of the first block; an edge is one block
 
-      const uint8_t* par = blk + 16 * D;  // [position][K, V][group](scale, low)
-      // ---- keys' parameters of positions g and g + 8
-      uint32_t kp[2][G];
+      // ---- keys' parameters of positions g and g + 8, and S^T = K.Q^T: one accumulator set
+      // per group and one of the lows
+      uint32_t kp[N][2][G];
+      float acc[N][NT][G][4], accl[N][NT][4];
+      uint32_t kw[N][2][2 * G];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* at = par + (g + 8 * h) * 8 * G;
-        if (G == 2)
-          *reinterpret_cast<uint2*>(kp[h]) = *reinterpret_cast<const uint2*>(at);
-        else
-          kp[h][0] = *reinterpret_cast<const uint32_t*>(at);
-      }
-
-      // ---- S^T = K.Q^T, one accumulator set per group and one of the lows
-      float acc[NT][G][4], accl[NT][4];
+      for (int u = 0; u < N; ++u) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        mma_f16_k8(accl[nt], qd & (G - 1) ? kp[0][G - 1] : kp[0][0], qd & (G - 1) ? kp[1][G - 1] : kp[1][0], qb[nt]);
-      uint32_t kw[2][2 * G];
-      if (G == 2) {
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* at = blk[u] + 16 * D + (g + 8 * h) * 8 * G;  // [position][K, V][group](scale, low)
+          if (G == 2) {
+            *reinterpret_cast<uint2*>(kp[u][h]) = *reinterpret_cast<const uint2*>(at);
+            *reinterpret_cast<uint4*>(kw[u][h]) = *reinterpret_cast<const uint4*>(blk[u] + h * 512 + lane * 16);
+          } else {
+            kp[u][h][0] = *reinterpret_cast<const uint32_t*>(at);
+            *reinterpret_cast<uint2*>(kw[u][h]) = *reinterpret_cast<const uint2*>(blk[u] + h * 256 + lane * 8);
+          }
+        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint4*>(kw[h]) = *reinterpret_cast<const uint4*>(blk + h * 512 + lane * 16);
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint2*>(kw[h]) = *reinterpret_cast<const uint2*>(blk + h * 256 + lane * 8);
+        for (int nt = 0; nt < NT; ++nt)
+          mma_f16_k8(accl[u][nt], qd & (G - 1) ? kp[u][0][G - 1] : kp[u][0][0],
+                     qd & (G - 1) ? kp[u][1][G - 1] : kp[u][1][0], qb[nt]);
       }
 #pragma unroll
       for (int w = 0; w < 2; ++w)
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-          uint32_t x = kw[0][2 * gr + w], y = kw[1][2 * gr + w];
+          uint4 bq[NT];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t a0 = tiny_even(x), a1 = tiny_even(y), a2 = tiny_odd(x), a3 = tiny_odd(y);
+          for (int nt = 0; nt < NT; ++nt) bq[nt] = sq[((gr * 2 + w) * NT + nt) * 32 + lane];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint2 bq;
-              if (kQRegs)
-                bq = h ? make_uint2(qf[kQRegs ? gr : 0][w].z, qf[kQRegs ? gr : 0][w].w)
-                       : make_uint2(qf[kQRegs ? gr : 0][w].x, qf[kQRegs ? gr : 0][w].y);
-              else
-                bq = *(reinterpret_cast<const uint2*>(&sq[((gr * 2 + w) * NT + nt) * 32 + lane]) + h);
-              if (w == 0 && h == 0)
-                mma_f16_first(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y);
-              else
-                mma_f16(acc[nt][gr], a0, a1, a2, a3, bq.x, bq.y);
+          for (int u = 0; u < N; ++u) {
+            uint32_t x = kw[u][0][2 * gr + w], y = kw[u][1][2 * gr + w];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a0 = tiny_even(x), a1 = tiny_even(y), a2 = tiny_odd(x), a3 = tiny_odd(y);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if (w == 0 && h == 0)
+                  mma_f16_first(acc[u][nt][gr], a0, a1, a2, a3, bq[nt].x, bq[nt].y);
+                else
+                  mma_f16(acc[u][nt][gr], a0, a1, a2, a3, h ? bq[nt].z : bq[nt].x, h ? bq[nt].w : bq[nt].y);
+              }
+              x >>= 8;
+              y >>= 8;
             }
-            x >>= 8;
-            y >>= 8;
           }
         }
 
       // ---- values' parameters of positions 2 qd, 2 qd + 1 and 8 behind them: the scales
       // side by side, and all eight quantities of a position as rows of an operand
-      uint32_t vs[2][G], va[2];
-      if (G == 2) ldmatrix2_t(va[0], va[1], par + (lane & 15) * 16);
+      uint32_t vs[N][2][G], va[N][2];
+      __half2 vmax = __float2half2_rn(0.f);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* at = par + (2 * qd + 8 * h) * 8 * G + 4 * G;
-        if (G == 2) {
-          const uint2 a = *reinterpret_cast<const uint2*>(at), b = *reinterpret_cast<const uint2*>(at + 8 * G);
-          vs[h][0] = __byte_perm(a.x, b.x, 0x5410);
-          vs[h][G - 1] = __byte_perm(a.y, b.y, 0x5410);
-        } else {
-          const uint32_t a = *reinterpret_cast<const uint32_t*>(at), b = *reinterpret_cast<const uint32_t*>(at + 8 * G);
-          vs[h][0] = __byte_perm(a, b, 0x5410);
-          va[h] = g & 1 ? __byte_perm(a, b, 0x7632) : vs[h][0];
-        }
-      }
-
-      if (edge) {  // whatever lies behind the last position must not matter
+      for (int u = 0; u < N; ++u) {
+        const uint8_t* par = blk[u] + 16 * D;
+        if (G == 2) ldmatrix2_t(va[u][0], va[u][1], par + (lane & 15) * 16);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* at = par + (2 * qd + 8 * h) * 8 * G + 4 * G;
+          if (G == 2) {
+            const uint2 a = *reinterpret_cast<const uint2*>(at), b = *reinterpret_cast<const uint2*>(at + 8 * G);
+            vs[u][h][0] = __byte_perm(a.x, b.x, 0x5410);
+            vs[u][h][G - 1] = __byte_perm(a.y, b.y, 0x5410);
+          } else {
+            const uint32_t a = *reinterpret_cast<const uint32_t*>(at), b = *reinterpret_cast<const uint32_t*>(at + 8 * G);
+            vs[u][h][0] = __byte_perm(a, b, 0x5410);
+            va[u][h] = g & 1 ? __byte_perm(a, b, 0x7632) : vs[u][h][0];
+          }
 #pragma unroll
           for (int gr = 0; gr < G; ++gr) {
-            const int left = len - pos0 - 2 * qd - 8 * h;
-            vs[h][gr] &= left > 1 ? 0xffffffffu : (left > 0 ? 0xffffu : 0u);
+            if (edge) {  // whatever lies behind the last position must not matter
+              const int left = len - pos0 - 2 * qd - 8 * h;
+              vs[u][h][gr] &= left > 1 ? 0xffffffffu : (left > 0 ? 0xffffu : 0u);
+            }
+            vmax = __hmax2(vmax, __habs2(as_half2(vs[u][h][gr])));
           }
+        }
       }
 
       // ---- scores in log2 units less the reference (position g: columns 2 qd, 2 qd + 1;
       // position g + 8: the same)
-      float ks[2][G];
+      float sc[N][NT][4], x[N][NT][4];
+      bool over = __hgt(__hmax(__low2half(vmax), __high2half(vmax)), __low2half(as_half2(cap)));
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) ks[h][gr] = __low2float(as_half2(kp[h][gr]));
-      float sc[NT][4], x[NT][4];
-      bool over = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int h = e >> 1;
-          float v = fmaf(ks[h][0], acc[nt][0][e], accl[nt][e]);
-          if (G == 2) v = fmaf(ks[h][G - 1], acc[nt][G - 1][e], v);
-          sc[nt][e] = v;
-          x[nt][e] = fmaf(v, cn[nt][e & 1], -m_run[nt][e & 1]);
-          if (edge && pos0 + g + 8 * h > lim[nt][e & 1]) sc[nt][e] = x[nt][e] = -INFINITY;
-          over |= x[nt][e] > room;
-        }
-      __half2 vmax = __hmax2(__habs2(as_half2(vs[0][0])), __habs2(as_half2(vs[1][0])));
-      if (G == 2) vmax = __hmax2(vmax, __hmax2(__habs2(as_half2(vs[0][G - 1])), __habs2(as_half2(vs[1][G - 1]))));
-      over |= __hgt(__hmax(__low2half(vmax), __high2half(vmax)), __low2half(as_half2(cap)));
-      if (__any_sync(0xffffffffu, over)) {
-        float vm = 0.f;  // the largest finite scale of the block
+      for (int u = 0; u < N; ++u) {
+        float ks[2][G];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int gr = 0; gr < G; ++gr) {
-            const float2 v = Half16<__half>::unpack(vs[h][gr]);
-            vm = fmaxf(vm, fabsf(v.x) <= 65504.f ? fabsf(v.x) : 0.f);
-            vm = fmaxf(vm, fabsf(v.y) <= 65504.f ? fabsf(v.y) : 0.f);
+          for (int gr = 0; gr < G; ++gr) ks[h][gr] = __low2float(as_half2(kp[u][h][gr]));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int h = e >> 1;
+            float v = fmaf(ks[h][0], acc[u][nt][0][e], accl[u][nt][e]);
+            if (G == 2) v = fmaf(ks[h][G - 1], acc[u][nt][G - 1][e], v);
+            sc[u][nt][e] = v;
+            x[u][nt][e] = fmaf(v, cn[nt][e & 1], -m_run[nt][e & 1]);
+            if (edge && pos0 + g + 8 * h > lim[nt][e & 1]) sc[u][nt][e] = x[u][nt][e] = -INFINITY;
+            over |= x[u][nt][e] > room;
           }
+      }
+      if (__any_sync(0xffffffffu, over)) {
+        float vm = 0.f;  // the largest finite scale of the blocks
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+              const float2 v = Half16<__half>::unpack(vs[u][h][gr]);
+              vm = fmaxf(vm, fabsf(v.x) <= 65504.f ? fabsf(v.x) : 0.f);
+              vm = fmaxf(vm, fabsf(v.y) <= 65504.f ? fabsf(v.y) : 0.f);
+            }
         vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
         vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
         if (vm > __low2float(as_half2(cap))) {
@@ -694,120 +695,126 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(sc[nt][e], sc[nt][2 + e]);
+            float mx = fmaxf(sc[0][nt][e], sc[0][nt][2 + e]);
+            if (N == 2) mx = fmaxf(mx, fmaxf(sc[N - 1][nt][e], sc[N - 1][nt][2 + e]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             mx = fmaxf(fmaf(mx, cn[nt][e], kSlack - room), m_run[nt][e]);
             const float al = exp2_approx(m_run[nt][e] - mx);
             m_run[nt][e] = mx;
-            x[nt][e] = fmaf(sc[nt][e], cn[nt][e], -mx);
-            x[nt][2 + e] = fmaf(sc[nt][2 + e], cn[nt][e], -mx);
-            sums[nt][e] *= al;
-            sums[nt][2 + e] *= al;
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) {
-              off[nt][gr][e] *= al;
-              off[nt][gr][2 + e] *= al;
+            for (int u = 0; u < N; ++u) {
+              x[u][nt][e] = fmaf(sc[u][nt][e], cn[nt][e], -mx);
+              x[u][nt][2 + e] = fmaf(sc[u][nt][2 + e], cn[nt][e], -mx);
+            }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                o[nt][gr][i][e] *= al;
-                o[nt][gr][i][2 + e] *= al;
-              }
+            for (int h = 0; h < 4; h += 2) {
+              sums[nt][h + e] *= al;
+              off[nt][h + e] *= al;
+#pragma unroll
+              for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nt][gr][i][h + e] *= al;
             }
           }
       }
 
       // ---- weights as an n8 operand, their products with the scales as those of O^T
-      uint32_t pb[NT][G][2];
+      uint32_t pb[N][NT][G][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float w[4];
+      for (int u = 0; u < N; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = exp2_approx(x[nt][e]);
-        const uint32_t p0 = pack_half2(w[0], w[1]), p1 = pack_half2(w[2], w[3]);
-        const uint32_t w0 = movmatrix_t(p0), w1 = movmatrix_t(p1);
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4];
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          pb[nt][gr][0] = mul_half2(w0, vs[0][gr]);
-          pb[nt][gr][1] = mul_half2(w1, vs[1][gr]);
-        }
-        if (!edge) {
-          mma_f16(sums[nt], va[0], 0x3c003c00u, va[1], 0x3c003c00u, w0, w1);
-        } else {  // whatever a hidden value holds must not matter: visible ones one by one
-          const int la = __shfl_sync(0xffffffffu, lim[nt][0], g >> 1), lb = __shfl_sync(0xffffffffu, lim[nt][1], g >> 1);
-          const int last = (g & 1 ? lb : la) - pos0 - 2 * qd;  // column g's, from position 2 qd
-          const uint32_t keep0 = (last >= 0 ? 0xffffu : 0u) | (last >= 1 ? 0xffff0000u : 0u),
-                         keep1 = (last >= 8 ? 0xffffu : 0u) | (last >= 9 ? 0xffff0000u : 0u);
+          for (int e = 0; e < 4; ++e) w[e] = exp2_approx(x[u][nt][e]);
+          const uint32_t p0 = pack_half2(w[0], w[1]), p1 = pack_half2(w[2], w[3]);
+          const uint32_t w0 = movmatrix_t(p0), w1 = movmatrix_t(p1);
 #pragma unroll
           for (int gr = 0; gr < G; ++gr) {
-            pb[nt][gr][0] &= keep0;
-            pb[nt][gr][1] &= keep1;
+            pb[u][nt][gr][0] = mul_half2(w0, vs[u][0][gr]);
+            pb[u][nt][gr][1] = mul_half2(w1, vs[u][1][gr]);
           }
-          const float2 r[2] = {Half16<__half>::unpack(p0), Half16<__half>::unpack(p1)};
+          if (!edge) {
+            mma_f16(sums[nt], va[u][0], 0x3c003c00u, va[u][1], 0x3c003c00u, w0, w1);
+          } else {  // whatever a hidden value holds must not matter: visible ones one by one
+            const int la = __shfl_sync(0xffffffffu, lim[nt][0], g >> 1), lb = __shfl_sync(0xffffffffu, lim[nt][1], g >> 1);
+            const int last = (g & 1 ? lb : la) - pos0 - 2 * qd;  // column g's, from position 2 qd
+            const uint32_t keep0 = (last >= 0 ? 0xffffu : 0u) | (last >= 1 ? 0xffff0000u : 0u),
+                           keep1 = (last >= 8 ? 0xffffu : 0u) | (last >= 9 ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float l = 0.f, c[G];
+            for (int gr = 0; gr < G; ++gr) {
+              pb[u][nt][gr][0] &= keep0;
+              pb[u][nt][gr][1] &= keep1;
+            }
+            const float2 r[2] = {Half16<__half>::unpack(p0), Half16<__half>::unpack(p1)};
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) c[gr] = 0.f;
+            for (int e = 0; e < 2; ++e) {
+              float l = 0.f, c[G];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float we = e ? r[h].y : r[h].x;
-              if (pos0 + g + 8 * h > lim[nt][e]) continue;
-              l += we;
+              for (int gr = 0; gr < G; ++gr) c[gr] = 0.f;
 #pragma unroll
-              for (int gr = 0; gr < G; ++gr) {
-                const float2 v = Half16<__half>::unpack(
-                    *reinterpret_cast<const uint32_t*>(par + (g + 8 * h) * 8 * G + 4 * G + 4 * gr));
-                c[gr] = fmaf(we, fmaf(8.f, v.x, v.y), c[gr]);
+              for (int h = 0; h < 2; ++h) {
+                const float we = e ? r[h].y : r[h].x;
+                if (pos0 + g + 8 * h > lim[nt][e]) continue;
+                l += we;
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                  const float2 v = Half16<__half>::unpack(
+                      *reinterpret_cast<const uint32_t*>(blk[u] + 16 * D + (g + 8 * h) * 8 * G + 4 * G + 4 * gr));
+                  c[gr] = fmaf(we, fmaf(8.f, v.x, v.y), c[gr]);
+                }
               }
+#pragma unroll
+              for (int y = 4; y < 32; y <<= 1) {
+                l += __shfl_xor_sync(0xffffffffu, l, y);
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) c[gr] += __shfl_xor_sync(0xffffffffu, c[gr], y);
+              }
+              sums[nt][2 + e] += l;
+#pragma unroll
+              for (int gr = 0; gr < G; ++gr)
+                if (g == kRowV + 2 * gr + 1) sums[nt][e] += c[gr];
             }
-#pragma unroll
-            for (int y = 4; y < 32; y <<= 1) {
-              l += __shfl_xor_sync(0xffffffffu, l, y);
-#pragma unroll
-              for (int gr = 0; gr < G; ++gr) c[gr] += __shfl_xor_sync(0xffffffffu, c[gr], y);
-            }
-            sums[nt][2 + e] += l;
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr)
-              if (g == kRowV + 2 * gr + 1) sums[nt][e] += c[gr];
           }
+          mma_f16(off[nt], 0x00080008u, 0u, 0x00080008u, 0u, pb[u][nt][0][0], pb[u][nt][0][1]);
+          if (G == 2) mma_f16(off[nt], 0u, 0x00080008u, 0u, 0x00080008u, pb[u][nt][G - 1][0], pb[u][nt][G - 1][1]);
+        }
+
+      // ---- O^T += V^T.P^T: rows g, g + 8 of m-tile i are elements 2 i, 2 i + 1 of eight
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        uint32_t vw[2][2][G];  // half h, position parity, group
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (G == 2)
+            *reinterpret_cast<uint4*>(vw[h]) = *reinterpret_cast<const uint4*>(blk[u] + 8 * D + h * 512 + lane * 16);
+          else
+            *reinterpret_cast<uint2*>(vw[h]) = *reinterpret_cast<const uint2*>(blk[u] + 8 * D + h * 256 + lane * 8);
+        if (u == N - 1) {
+          __syncwarp();  // every lane has read the blocks
+          taken += N;
+#pragma unroll
+          for (int i = 0; i < N; ++i) feed();
         }
 #pragma unroll
         for (int gr = 0; gr < G; ++gr)
-          mma_f16(off[nt][gr], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pb[nt][gr][0], pb[nt][gr][1]);
-      }
-
-      // ---- O^T += V^T.P^T: rows g, g + 8 of m-tile i are elements 2 i, 2 i + 1 of eight
-      uint32_t vw[2][2][G];  // half h, position parity, group
-      if (G == 2) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint4*>(vw[h]) = *reinterpret_cast<const uint4*>(blk + 8 * D + h * 512 + lane * 16);
-      } else {
+          for (int z = 0; z < 2; ++z) {
+            uint32_t a = __byte_perm(vw[0][0][gr], vw[0][1][gr], z ? 0x7632 : 0x5410);
+            uint32_t b = __byte_perm(vw[1][0][gr], vw[1][1][gr], z ? 0x7632 : 0x5410);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<uint2*>(vw[h]) = *reinterpret_cast<const uint2*>(blk + 8 * D + h * 256 + lane * 8);
-      }
-      __syncwarp();  // every lane has read the block
-      ++taken;
-      feed();
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t a0 = tiny_even(a), a1 = tiny_odd(a), a2 = tiny_even(b), a3 = tiny_odd(b);
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          uint32_t x = __byte_perm(vw[0][0][gr], vw[0][1][gr], z ? 0x7632 : 0x5410);
-          uint32_t y = __byte_perm(vw[1][0][gr], vw[1][1][gr], z ? 0x7632 : 0x5410);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t a0 = tiny_even(x), a1 = tiny_odd(x), a2 = tiny_even(y), a3 = tiny_odd(y);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][gr][2 * z + i], a0, a1, a2, a3, pb[nt][gr][0], pb[nt][gr][1]);
-            x >>= 8;
-            y >>= 8;
+              for (int nt = 0; nt < NT; ++nt)
+                mma_f16(o[nt][gr][2 * z + i], a0, a1, a2, a3, pb[u][nt][gr][0], pb[u][nt][gr][1]);
+              a >>= 8;
+              b >>= 8;
+            }
           }
-        }
+      }
       return true;
     };
     // the blocks that every column sees to their end come first
@@ -815,8 +822,22 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     if (mask_from - pos_first < kKv4Block) inner = 0;
     if (inner > blocks) inner = blocks;
     bool fine = true;
-    for (int j = 0; j < inner && fine; ++j) fine = block(j, std::false_type{});
-    for (int j = inner; j < blocks && fine; ++j) fine = block(j, std::true_type{});
+    for (int j = 0; j < blocks && fine;) {
+      if ((j & 31) == 0) set_valid = valid;  // block j has been issued, its set is the current one
+      const uint32_t has = set_valid >> (j & 31);
+      if (S::kStep == 2 && j + 2 <= inner && (has & 3u) == 3u) {
+        fine = step(j, std::integral_constant<int, S::kStep>{}, std::false_type{});
+        j += 2;
+        continue;
+      }
+      if (!(has & 1u))  // no page: the block is hidden from every column
+        feed();
+      else if (S::kStep == 1 && j < inner)
+        fine = step(j, std::integral_constant<int, 1>{}, std::false_type{});
+      else
+        fine = step(j, std::integral_constant<int, 1>{}, std::true_type{});
+      ++j;
+    }
 
     // ---- the rest of the next segment's first copies
     if (!kClustered) {
@@ -842,8 +863,8 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           float f[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            f[2 * i] = fmaf(o[nt][gr][i][e] - off[nt][gr][e], 16777216.f, c);
-            f[2 * i + 1] = fmaf(fmaf(o[nt][gr][i][2 + e], 0.0625f, -off[nt][gr][e]), 16777216.f, c);
+            f[2 * i] = fmaf(o[nt][gr][i][e] - off[nt][2 * gr + e], 16777216.f, c);
+            f[2 * i + 1] = fmaf(fmaf(o[nt][gr][i][2 + e], 0.0625f, -off[nt][2 * gr + e]), 16777216.f, c);
           }
           float* dst = row + 64 * gr + 8 * g;
           *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
@@ -890,7 +911,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
         const float inv = 1.f / l;
 #pragma unroll
         for (int x = 0; x < 8; ++x) f[x] = l == 0.f ? 0.f : f[x] * inv;
-        const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
+        const int tok = columns.token(col0 + n), hd = col0 + n - tok * p.group;
         T* dst = static_cast<T*>(p.out) + ((sp.first + tok) * p.heads + kvh * p.group + hd) * D + d0;
         *reinterpret_cast<uint4*>(dst) = pack8<T>(f);
       } else {
@@ -929,7 +950,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           f.w = fmaf(k, v[c].w, f.w);
         }
         const float inv = 1.f / l;
-        const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
+        const int tok = columns.token(col0 + n), hd = col0 + n - tok * p.group;
         T* dst = static_cast<T*>(p.out) + ((sp.first + tok) * p.heads + kvh * p.group + hd) * D + d0;
         *reinterpret_cast<uint2*>(dst) =
             l == 0.f ? make_uint2(0u, 0u)
@@ -967,7 +988,8 @@ __global__ void __launch_bounds__(32 * kCWarps) kv4_attn_combine_kernel(const Kv
   if (cut.count == 0) return;
   const Kv4Seq& s = p.seq;
   const int col0 = blockIdx.z * R;
-  const SeqSpan sp = seq_span(s, cut.b, p.group, col0, R, AttnShape<NT>::kTile);
+  const Columns columns{p.group, p.group_mul};
+  const SeqSpan sp = seq_span(s, cut.b, columns, col0, R, AttnShape<NT>::kTile);
   if (n >= sp.cols) return;
   const int64_t slot0 = static_cast<int64_t>(blockIdx.z) * (runs + static_cast<int64_t>(s.batch) * s.kv_heads) +
                         static_cast<int64_t>(cut.b) * s.kv_heads + cut.kvh + run;
@@ -1013,7 +1035,7 @@ __global__ void __launch_bounds__(32 * kCWarps) kv4_attn_combine_kernel(const Kv
     b2 = fmaf(k, sh_o[w][2 * threadIdx.x + 1], b2);
   }
   const float inv = 1.f / l;
-  const int tok = (col0 + n) / p.group, hd = (col0 + n) % p.group;
+  const int tok = columns.token(col0 + n), hd = col0 + n - tok * p.group;
   T* dst = static_cast<T*>(p.out) + ((sp.first + tok) * p.heads + cut.kvh * p.group + hd) * D + 2 * threadIdx.x;
   *reinterpret_cast<uint32_t*>(dst) = l == 0.f ? 0u : Half16<T>::pack(a * inv, b2 * inv);
 }
@@ -1137,6 +1159,7 @@ int launch_kv4_attention(const Kv4Seq& seq, const void* q, int64_t q_stride, con
   p.o_part = reinterpret_cast<float*>(ws + a.o_off);
   p.heads = heads;
   p.group = group;
+  p.group_mul = (65536 + group - 1) / group;
   p.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(dim));
   p.status = status;
   p.seq = seq;
