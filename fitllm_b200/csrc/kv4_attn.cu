@@ -50,18 +50,16 @@
 namespace fitq {
 namespace {
 
-// Warps per CTA and CTAs per SM by column tiles.  Sixteen columns are the most a
-// warp takes: with 32 the output alone is 128 registers a thread and eight warps per
-// SM wait on their own latencies (a verify step of 8 x 5 tokens over 4,100 positions
-// took 42 us that way); more columns are further row tiles, whose reads hit L2.
+// Warps per CTA by column tiles; both shapes leave two CTAs to an SM.  Sixteen columns are
+// the most a warp takes: with 32 the output alone is 128 registers a thread; more columns
+// are further row tiles, whose reads hit L2.
 template <int NT>
 struct AttnShape {
   static constexpr int kWarps = NT == 1 ? 8 : 4;
-  static constexpr int kCtas = NT == 1 ? 2 : 3;
+  static constexpr int kCtas = 2;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTile = kKv4Block * kWarps;  // positions per tile
-  static constexpr int kStages = NT == 1 ? 4 : 3;   // blocks in flight per warp
-  static constexpr int kStep = NT == 1 ? 2 : 1;     // blocks taken at a time
+  static constexpr int kStages = 4;                 // blocks in flight per warp
 };
 // Running maxima start finite, so that masked scores (-inf) never meet -inf - -inf.
 constexpr float kFloor = -3.0e38f;
@@ -203,7 +201,7 @@ struct AttnSmem {
 constexpr float kRoom = 15.f, kSlack = 8.f;
 // A pair's first tile costs a run this many tiles more (queries, the pipeline's
 // start, the warps' meeting): runs are cut by cost.
-constexpr int kPairCost = 2;
+constexpr int kPairCost = 4;
 __device__ __forceinline__ int pair_cost(const SeqSpan& sp) { return sp.tiles ? sp.tiles + kPairCost : 0; }
 
 extern __shared__ __align__(128) uint8_t g_kv4_smem[];
@@ -825,15 +823,13 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     for (int j = 0; j < blocks && fine;) {
       if ((j & 31) == 0) set_valid = valid;  // block j has been issued, its set is the current one
       const uint32_t has = set_valid >> (j & 31);
-      if (S::kStep == 2 && j + 2 <= inner && (has & 3u) == 3u) {
-        fine = step(j, std::integral_constant<int, S::kStep>{}, std::false_type{});
+      if (j + 2 <= inner && (has & 3u) == 3u) {
+        fine = step(j, std::integral_constant<int, 2>{}, std::false_type{});
         j += 2;
         continue;
       }
       if (!(has & 1u))  // no page: the block is hidden from every column
         feed();
-      else if (S::kStep == 1 && j < inner)
-        fine = step(j, std::integral_constant<int, 1>{}, std::false_type{});
       else
         fine = step(j, std::integral_constant<int, 1>{}, std::true_type{});
       ++j;
@@ -1040,10 +1036,22 @@ __global__ void __launch_bounds__(32 * kCWarps) kv4_attn_combine_kernel(const Kv
   *reinterpret_cast<uint32_t*>(dst) = l == 0.f ? 0u : Half16<T>::pack(a * inv, b2 * inv);
 }
 
-// Columns of a call: tokens of a sequence x heads of a KV head, in n8 tiles.
-int col_tiles(int group, int64_t max_new) {
-  const int64_t cols = static_cast<int64_t>(group) * max_new;
-  return cols <= 8 ? 1 : 2;
+// Whether a call goes as clusters: all of them on the card at once, and no CTA with more
+// than eight tiles.
+template <int NT>
+bool clusters_fit(int64_t pairs, int64_t cols, int64_t max_len, int num_sms) {
+  const int64_t row_tiles = (cols + 8 * NT - 1) / (8 * NT);
+  return pairs * kCluster * row_tiles <= static_cast<int64_t>(num_sms) * AttnShape<NT>::kCtas &&
+         max_len <= 8ll * kCluster * AttnShape<NT>::kTile;
+}
+
+// Columns per warp, in n8 tiles.  Up to eight: one.  More: two, so that a block is decoded
+// once for sixteen columns, unless all row tiles of eight fit on the card as clusters, which
+// then end sooner: 5 tokens of 5 heads over 1,000 / 4,000 positions of one sequence take 8.1 /
+// 10.6 us in four row tiles, 10.0 / 13.0 us in two; of two sequences, whose four no longer
+// fit, 11.7 / 17.1 against 10.8 / 13.9 us.
+int col_tiles(int64_t pairs, int64_t cols, int64_t max_len, int num_sms) {
+  return cols <= 8 || clusters_fit<1>(pairs, cols, max_len, num_sms) ? 1 : 2;
 }
 
 struct AttnPlan {
@@ -1063,17 +1071,14 @@ int64_t plan_runs(int64_t pairs, int64_t max_len, int row_tiles, int num_sms) {
 
 AttnPlan attn_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim, int num_sms) {
   AttnPlan a;
-  a.nt = col_tiles(group, max_new);
+  const int64_t pairs = static_cast<int64_t>(batch) * kv_heads, cols = static_cast<int64_t>(group) * max_new;
+  a.nt = col_tiles(pairs, cols, max_len, num_sms);
   const int R = 8 * a.nt;
-  a.row_tiles = static_cast<int>((group * max_new + R - 1) / R);
-  a.cols = static_cast<int>(group * max_new < R ? group * max_new : R);
-  const int64_t pairs = static_cast<int64_t>(batch) * kv_heads;
+  a.row_tiles = static_cast<int>((cols + R - 1) / R);
+  a.cols = static_cast<int>(cols < R ? cols : R);
   a.runs = static_cast<int>(a.nt == 1 ? plan_runs<1>(pairs, max_len, a.row_tiles, num_sms)
                                      : plan_runs<2>(pairs, max_len, a.row_tiles, num_sms));
-  // Clusters: all of them on the card at once, and no CTA with more than eight tiles.
-  const int64_t slots_at_once = static_cast<int64_t>(num_sms) * (a.nt == 1 ? AttnShape<1>::kCtas : AttnShape<2>::kCtas);
-  const int tile = a.nt == 1 ? AttnShape<1>::kTile : AttnShape<2>::kTile;
-  if (pairs * kCluster * a.row_tiles <= slots_at_once && max_len <= 8ll * kCluster * tile) {
+  if (a.nt == 1 ? clusters_fit<1>(pairs, cols, max_len, num_sms) : clusters_fit<2>(pairs, cols, max_len, num_sms)) {
     a.runs = 0;
     a.cuts_off = a.ml_off = a.o_off = 0;
     a.bytes = 16;
