@@ -65,9 +65,10 @@ struct AttnShape {
 constexpr float kFloor = -3.0e38f;
 
 // The pair that a run opens and leaves to the runs behind it: `count` runs hold
-// parts of it (0: none).
-struct Kv4Cut {
-  int b, kvh, count;
+// parts of it (0: none), the first in `slot`.
+struct __align__(16) Kv4Cut {
+  int64_t first;  // packed token of the sequence's first new token
+  int count, cols, slot, kvh;
 };
 
 struct Kv4AttnParams {
@@ -254,9 +255,9 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     int b, kvh, ta, tb;
   };
   __shared__ Segment sh_seg[3];  // segment i in place i % 3
-  __shared__ uint32_t sh_walk_t, sh_walk_t0;  // thread 0's place in the list
+  __shared__ uint32_t sh_walk_t, sh_walk_t0;  // the place in the list behind the last segment found
   __shared__ int sh_walk_b;
-  __shared__ int sh_scan[kWarps], sh_b, sh_base;
+  __shared__ int sh_scan[kWarps];
   __shared__ int sh_abort;
 
   if (tid == 0) sh_abort = 0;
@@ -277,53 +278,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   };
   uint32_t total = 0, per = 0, t_lo = 0, t_hi = 0;
   Kv4Cut* cut = p.cuts + blockIdx.y * gridDim.x + blockIdx.x;  // the pair that this run opens and does not finish
-  if (!kClustered) {
-  // ---- the list of pairs in units of cost: every thread sums a run of sequences, then a scan
-  const int per_thread = (s.batch + kThreads - 1) / kThreads;
-  const int b_lo = tid * per_thread, b_hi = b_lo + per_thread < s.batch ? b_lo + per_thread : s.batch;
-  int mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += pair_cost(seq_span(s, b, columns, col0, R, kTile));
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) sh_scan[warp] = incl;
-  __syncthreads();
-  int before = incl - mine, all = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const int v = sh_scan[w];
-    before += w < warp ? v : 0;
-    all += v;
-  }
-  // (the host has checked that the list's length fits in 31 bits)
-  total = static_cast<uint32_t>(all) * s.kv_heads;
-  per = (total + gridDim.x - 1) / gridDim.x;  // cost of a run
-  t_lo = per * blockIdx.x;
-  t_hi = t_lo + per < total ? t_lo + per : total;
-  if (!kClustered && tid == 0) cut->count = 0;
-  {
-    int at = before;
-    for (int b = b_lo; b < b_hi; ++b) {
-      const SeqSpan sp = seq_span(s, b, columns, col0, R, kTile);
-      const int cost = pair_cost(sp);
-      // sequence b covers [at * KVH, (at + cost) * KVH) of the list
-      if (t_lo < t_hi && static_cast<uint32_t>(at) * s.kv_heads <= t_lo &&
-          t_lo < static_cast<uint32_t>(at + cost) * s.kv_heads) {
-        sh_b = b;
-        sh_base = at;
-      }
-      if (blockIdx.x == 0 && blockIdx.y == 0) check_sequence(sp);
-      at += cost;
-    }
-  }
-  __syncthreads();
-  if (t_lo >= t_hi) return;
-  }
-
-  // ---- the run's segments, found by thread 0 one ahead of their use
+  // ---- the run's segments, found one ahead of their use
   auto advance = [&](Segment& g) {
     uint32_t t = sh_walk_t, t0 = sh_walk_t0;
     int b = sh_walk_b;
@@ -353,24 +308,69 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     sh_walk_t0 = t0;
     sh_walk_b = b;
   };
-  if (tid == 0) {
-    if (kClustered) {  // the CTA's share of its cluster's pair, and nothing behind it
-      Segment& g = sh_seg[0];
-      const int pair = static_cast<int>(blockIdx.x) / kCluster, rank = static_cast<int>(blockIdx.x) % kCluster;
-      g.b = pair / s.kv_heads;
-      g.kvh = pair % s.kv_heads;
-      g.sp = seq_span(s, g.b, columns, col0, R, kTile);
-      const int share = (g.sp.tiles + kCluster - 1) / kCluster;
-      g.ta = min(rank * share, g.sp.tiles);
-      g.tb = min(g.ta + share, g.sp.tiles);
-      sh_seg[1].tb = 0;
-      if (rank == 0 && g.kvh == 0 && blockIdx.y == 0) check_sequence(g.sp);
-    } else {
-      sh_walk_t = t_lo;
-      sh_walk_t0 = static_cast<uint32_t>(sh_base) * s.kv_heads;
-      sh_walk_b = sh_b;
-      advance(sh_seg[0]);
+
+  if (!kClustered) {
+    // ---- the list of pairs in units of cost: every thread sums a run of sequences, then a scan
+    const int per_thread = (s.batch + kThreads - 1) / kThreads;
+    const int b_lo = tid * per_thread, b_hi = b_lo + per_thread < s.batch ? b_lo + per_thread : s.batch;
+    int mine = 0;
+    for (int b = b_lo; b < b_hi; ++b) mine += pair_cost(seq_span(s, b, columns, col0, R, kTile));
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
     }
+    if (lane == 31) sh_scan[warp] = incl;
+    __syncthreads();
+    int before = incl - mine, all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const int v = sh_scan[w];
+      before += w < warp ? v : 0;
+      all += v;
+    }
+    // (the host has checked that the list's length fits in 31 bits)
+    total = static_cast<uint32_t>(all) * s.kv_heads;
+    per = (total + gridDim.x - 1) / gridDim.x;  // cost of a run
+    t_lo = per * blockIdx.x;
+    t_hi = t_lo + per < total ? t_lo + per : total;
+    if (tid == 0) cut->count = 0;
+    {
+      int at = before, found = -1, found_at = 0;
+      for (int b = b_lo; b < b_hi; ++b) {
+        const SeqSpan sp = seq_span(s, b, columns, col0, R, kTile);
+        const int cost = pair_cost(sp);
+        // sequence b covers [at * KVH, (at + cost) * KVH) of the list
+        if (t_lo < t_hi && static_cast<uint32_t>(at) * s.kv_heads <= t_lo &&
+            t_lo < static_cast<uint32_t>(at + cost) * s.kv_heads) {
+          found = b;
+          found_at = at;
+        }
+        if (blockIdx.x == 0 && blockIdx.y == 0) check_sequence(sp);
+        at += cost;
+      }
+      if (found >= 0) {
+        sh_walk_t = t_lo;
+        sh_walk_t0 = static_cast<uint32_t>(found_at) * s.kv_heads;
+        sh_walk_b = found;
+        advance(sh_seg[0]);
+      }
+    }
+    if (t_lo >= t_hi) return;
+  }
+
+  if (kClustered && tid == 0) {  // the CTA's share of its cluster's pair, and nothing behind it
+    Segment& g = sh_seg[0];
+    const int pair = static_cast<int>(blockIdx.x) / kCluster, rank = static_cast<int>(blockIdx.x) % kCluster;
+    g.b = pair / s.kv_heads;
+    g.kvh = pair % s.kv_heads;
+    g.sp = seq_span(s, g.b, columns, col0, R, kTile);
+    const int share = (g.sp.tiles + kCluster - 1) / kCluster;
+    g.ta = min(rank * share, g.sp.tiles);
+    g.tb = min(g.ta + share, g.sp.tiles);
+    sh_seg[1].tb = 0;
+    if (rank == 0 && g.kvh == 0 && blockIdx.y == 0) check_sequence(g.sp);
   }
   __syncthreads();
   if (kClustered && sh_seg[0].sp.cols == 0) return;  // the whole cluster
@@ -873,12 +873,12 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     const SeqSpan sp = sg.sp;
     const int b = sg.b, kvh = sg.kvh;
     const bool whole = sg.ta == 0 && sg.tb == sp.tiles;
+    const int64_t slot = slot0 + blockIdx.x + static_cast<int64_t>(b) * s.kv_heads + kvh;
     if (!kClustered && tid == 0 && sg.ta == 0 && !whole) {
       // this run opens the pair; the last of its other tiles lies `rest` of cost behind the run's end
       const uint32_t rest = sp.tiles - sg.tb - 1;
-      *cut = Kv4Cut{b, kvh, static_cast<int>(2 + rest / per)};
+      *cut = Kv4Cut{sp.first, static_cast<int>(2 + rest / per), sp.cols, static_cast<int>(slot), kvh};
     }
-    const int64_t slot = slot0 + blockIdx.x + static_cast<int64_t>(b) * s.kv_heads + kvh;
     for (int i = tid; i < sp.cols * (D / 8); i += kThreads) {
       const int n = i / (D / 8), d0 = (i % (D / 8)) * 8;
       float mx = kFloor;
@@ -981,14 +981,10 @@ __global__ void __launch_bounds__(32 * kCWarps) kv4_attn_combine_kernel(const Kv
   pdl_launch_dependents();
   pdl_wait();  // the partials
   const Kv4Cut cut = p.cuts[blockIdx.z * runs + run];
-  if (cut.count == 0) return;
-  const Kv4Seq& s = p.seq;
+  if (n >= cut.cols || cut.count == 0) return;
   const int col0 = blockIdx.z * R;
   const Columns columns{p.group, p.group_mul};
-  const SeqSpan sp = seq_span(s, cut.b, columns, col0, R, AttnShape<NT>::kTile);
-  if (n >= sp.cols) return;
-  const int64_t slot0 = static_cast<int64_t>(blockIdx.z) * (runs + static_cast<int64_t>(s.batch) * s.kv_heads) +
-                        static_cast<int64_t>(cut.b) * s.kv_heads + cut.kvh + run;
+  const int64_t slot0 = cut.slot;
   const float2* ml = reinterpret_cast<const float2*>(p.ml_part) + slot0 * R + n;
   const float* row = p.o_part + (slot0 * R + n) * D + lane * kE;
   float mx = kFloor, l = 0.f, f[kE];
@@ -1032,7 +1028,7 @@ __global__ void __launch_bounds__(32 * kCWarps) kv4_attn_combine_kernel(const Kv
   }
   const float inv = 1.f / l;
   const int tok = columns.token(col0 + n), hd = col0 + n - tok * p.group;
-  T* dst = static_cast<T*>(p.out) + ((sp.first + tok) * p.heads + cut.kvh * p.group + hd) * D + 2 * threadIdx.x;
+  T* dst = static_cast<T*>(p.out) + ((cut.first + tok) * p.heads + cut.kvh * p.group + hd) * D + 2 * threadIdx.x;
   *reinterpret_cast<uint32_t*>(dst) = l == 0.f ? 0u : Half16<T>::pack(a * inv, b2 * inv);
 }
 
