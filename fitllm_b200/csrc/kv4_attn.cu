@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
               const int left = len - pos0 - 2 * qd - 8 * h;
               vs[u][h][gr] &= left > 1 ? 0xffffffffu : (left > 0 ? 0xffffu : 0u);
             }
-            vmax = __hmax2(vmax, __habs2(as_half2(vs[u][h][gr])));
+            vmax = __hmax2_nan(vmax, __habs2(as_half2(vs[u][h][gr])));
           }
         }
       }
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       // ---- scores in log2 units less the reference (position g: columns 2 qd, 2 qd + 1;
       // position g + 8: the same)
       float sc[N][NT][4], x[N][NT][4];
-      bool over = __hgt(__hmax(__low2half(vmax), __high2half(vmax)), __low2half(as_half2(cap)));
+      bool over = !__hle(__hmax_nan(__low2half(vmax), __high2half(vmax)), __low2half(as_half2(cap)));
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         float ks[2][G];
@@ -671,22 +671,27 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           }
       }
       if (__any_sync(0xffffffffu, over)) {
-        float vm = 0.f;  // the largest finite scale of the blocks
+        // the largest finite scale of the blocks; the others reach their group's elements
+        // through the sums, and as zeros nothing else
+        float vm = 0.f;
 #pragma unroll
         for (int u = 0; u < N; ++u)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-              const float2 v = Half16<__half>::unpack(vs[u][h][gr]);
-              vm = fmaxf(vm, fabsf(v.x) <= 65504.f ? fabsf(v.x) : 0.f);
-              vm = fmaxf(vm, fabsf(v.y) <= 65504.f ? fabsf(v.y) : 0.f);
+              float2 v = Half16<__half>::unpack(vs[u][h][gr]);
+              v.x = fabsf(v.x) <= 65504.f ? v.x : 0.f;
+              v.y = fabsf(v.y) <= 65504.f ? v.y : 0.f;
+              vs[u][h][gr] = pack_half2(v.x, v.y);
+              vm = fmaxf(vm, fmaxf(fabsf(v.x), fabsf(v.y)));
             }
         vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
         vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
         if (vm > __low2float(as_half2(cap))) {
-          const int e = (__float_as_int(vm) >> 23) - 126;  // vm < 2^e; 2^16 is infinite, a cap like any other
-          cap = pack_half2(pow2(e), pow2(e));
+          const int e = (__float_as_int(vm) >> 23) - 126;  // vm < 2^e
+          const float most = fminf(pow2(e), 65504.f);
+          cap = pack_half2(most, most);
           room = kRoom - static_cast<float>(e);
         }
 #pragma unroll

@@ -4,10 +4,10 @@ Append and read-back are held to the stated arithmetic bit for bit (every step
 of the coding is a single fp32 rounding).  Attention is compared with 64-bit
 attention over the values the cache stands for.  Its bound per element: with u
 half a step of the type (bf16 2^-8, fp16 2^-11) the scaled weights w s enter the
-tensor cores rounded once, off by at most u of a term s |code - 8| <= 8 s, and
-the output is rounded once (u |o|); scores carry the fp32 rounding of sums of up
-to 143 s |q| over 128 elements, below 2^-10 in the exponent at these sizes, which
-moves a weighted mean of values within [-vmax, vmax] by at most 2^-10 * 2 vmax.
+tensor cores rounded, off by at most u of a term s |code - 8| <= 8 s, and the
+output is rounded once (u |o|); weights rounded to fp16 before (2^-11) and the fp32
+rounding of the scores' sums (below 2^-11 in the exponent at these sizes) move a
+weighted mean of values within [-vmax, vmax] by at most 2^-10 * 2 vmax.
 """
 import pytest
 import torch
@@ -200,6 +200,30 @@ def test_attention_gives_nan_only_where_a_nan_is_seen(cuda_dev):
     o = _attend(c)
     assert bool(o[:, :2].isfinite().all()) and bool(o[:20].isfinite().all())
     assert bool(o[20:, 2:].isnan().all())
+
+
+@pytest.mark.parametrize("prefix,counts,h,kvh,d,ps,dtype", [
+    ([40, 20], [1, 1], 8, 2, 128, 16, BF), ([30, 200, 1400, 64, 0, 777], [1] * 6, 40, 8, 128, 64, BF),
+    ([90, 2500, 60, 511, 300], [2, 3, 1, 4, 2], 40, 8, 128, 16, FP), ([300, 40], [5, 5], 10, 2, 64, 64, BF),
+    ([70, 33], [40, 3], 8, 2, 128, 32, BF)])
+@pytest.mark.parametrize("bits", [0x7c00, 0xfe00])
+def test_a_value_group_without_numbers_spoils_its_own_elements_only(cuda_dev, prefix, counts, h, kvh, d, ps, dtype,
+                                                                    bits):
+    """An infinite or NaN scale of one group: inside the cache, and at the last new token."""
+    c = _case(prefix, counts, h, kvh, d, ps, dtype, cuda_dev, seed=5)
+    want = ref.attention(c["q"], c["pool"], c["table"], c["prefix"], c["starts"], c["counts"])
+    spoilt = torch.zeros(want.shape, dtype=torch.bool, device=cuda_dev)
+    for b, pos, kv, gr in ((0, 17, 0, 0), (1, prefix[1] + counts[1] - 1, kvh - 1, d // 64 - 1)):
+        at = 16 * d + ((pos % 16) * 2 * (d // 64) + d // 64 + gr) * 4
+        block = c["pool"][int(c["table"][b, pos // ps]), kv, pos % ps // 16]
+        block[at], block[at + 1] = bits & 255, bits >> 8
+        for i in range(counts[b]):
+            if pos <= prefix[b] + i:
+                spoilt[c["starts"][b] + i, kv * (h // kvh):(kv + 1) * (h // kvh), 64 * gr:64 * gr + 64] = True
+    o = _attend(c).double()
+    assert not bool(o[spoilt].isfinite().any())
+    bound = U[dtype] * (8 * 0.3 + want.abs()) + 2.0 ** -10 * 2 * (8 * 0.3 + 1)
+    assert bool(((o - want).abs() <= bound)[~spoilt].all())
 
 
 def test_bad_pages_positions_and_prefixes_are_recorded_and_left_out(cuda_dev):
