@@ -1352,8 +1352,8 @@ static int kv4_view(const char* what, const fitq_kv4* c, int heads, fitq::Kv4Seq
       c->tokens >= (1ll << 31) || static_cast<int64_t>(c->batch) * c->kv_heads >= (1ll << 28))
     return fail(FITQ_ERR_SHAPE, "%s: bad shape (tokens=%lld batch=%d heads=%d kv_heads=%d pages=%lld max_pages=%d)", what,
                 (long long)c->tokens, c->batch, heads, c->kv_heads, (long long)c->num_pages, c->max_pages);
-  if (static_cast<int64_t>(c->max_pages) * c->page_size >= (1ll << 31))
-    return fail(FITQ_ERR_SHAPE, "%s: max_pages * page_size must stay below 2^31", what);
+  if (static_cast<int64_t>(c->max_pages) * c->page_size > (1ll << 30))
+    return fail(FITQ_ERR_SHAPE, "%s: max_pages * page_size must not exceed 2^30", what);
   if (!c->q_start && c->tokens % c->batch != 0)
     return fail(FITQ_ERR_SHAPE, "%s: tokens=%lld do not divide over batch=%d (pass q_start)", what, (long long)c->tokens,
                 c->batch);
@@ -1443,7 +1443,7 @@ int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_stride, v
                 seq.t_new);
   // the kernels count the tiles of all (sequence, KV head) pairs in 31 bits
   if (static_cast<int64_t>(cache->batch) * cache->kv_heads *
-          (static_cast<int64_t>(cache->max_pages) * cache->page_size / 64 + 4) >= (1ll << 31))
+          (static_cast<int64_t>(cache->max_pages) * cache->page_size / 64 + 8) >= (1ll << 31))
     return fail(FITQ_ERR_SHAPE, "kv4_attention: batch * kv_heads * max_pages * page_size is too large");
   if (q_stride < static_cast<int64_t>(heads) * cache->head_dim || q_stride % 8)
     return fail(FITQ_ERR_SHAPE, "kv4_attention: the token stride must cover a token and be a multiple of 8");

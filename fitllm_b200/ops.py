@@ -358,7 +358,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
     if max_new is None:
         if q_start is not None:
             raise ValueError("kv4_attention: pass max_new with q_start")
-        max_new = max(1, q.shape[0] // c.batch)
+        max_new = max(1, q.shape[0] // max(1, c.batch))
     if max_len is None:
         max_len = c.max_pages * c.page_size
     out = _kv4_out("kv4_attention", "out", out, q.shape, q.dtype, dev)

@@ -246,6 +246,8 @@ def paged_verify_pass(layers: List[DecoderLayer], h: torch.Tensor, cache: PagedK
             starts.append(starts[-1] + c)
         q_start = torch.tensor(starts, dtype=torch.int32, device=h.device)
     cache.reserve(news)
+    if max(news) == 0:
+        return h
     max_len = max(n + c for n, c in zip(cache.lengths, news))
     for i, layer in enumerate(layers):
         h = paged_layer_forward(layer, h, cache.pools[i], cache, max_len, q_start, max(news))

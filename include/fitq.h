@@ -347,7 +347,8 @@ FITQ_API int fitq_attention_bwd(const void* q, const void* k, const void* v, con
  *   values [2 h][8 e][4 q][2 o][G g] words: elements 64 g + 8 e + j of position
  *          8 h + 2 q + o;
  *   params [16 positions][key, value][G] pairs (scale, low).
- * head_dim 64 or 128, page_size a power of two in 16..1024.
+ * head_dim 64 or 128, page_size a power of two in 16..1024, max_pages * page_size
+ * at most 2^30.
  * What only the device sees is checked there: a token whose position lies outside
  * the page table, whose page is not in 0..num_pages - 1, or whose prefix is
  * negative records FITQ_ERR_ARG (fitq_get_device_status) and is not written; its

@@ -39,7 +39,7 @@ BAD_CACHES = [
     (dict(page_size=2048), UNSUPPORTED), (dict(page_size=0), UNSUPPORTED), (dict(batch=0), SHAPE),
     (dict(kv_heads=3), SHAPE), (dict(kv_heads=0), SHAPE), (dict(tokens=7), SHAPE), (dict(tokens=-4), SHAPE),
     (dict(tokens=1 << 31), SHAPE), (dict(num_pages=0), SHAPE), (dict(max_pages=0), SHAPE),
-    (dict(max_pages=1 << 25), SHAPE), (dict(pool=P + 8), ALIGN), (dict(prefix=P + 2), ALIGN),
+    (dict(max_pages=1 << 25), SHAPE), (dict(max_pages=(1 << 24) + 1), SHAPE), (dict(pool=P + 8), ALIGN), (dict(prefix=P + 2), ALIGN),
 ]
 
 

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from fitllm_b200.verify import PagedKVCache
+from fitllm_b200.verify import PagedKVCache, paged_verify_pass
 
 
 def _cache(**kw):
@@ -49,3 +49,11 @@ def test_refusals_change_nothing():
 def test_bytes_read_counts_blocks():
     # 4.5 bits an element, keys and values: 18 * 64 bytes per 16 positions of a head
     assert _cache().bytes_read(160) == 2 * 3 * 2 * 10 * 18 * 64
+
+
+def test_a_pass_without_new_tokens_is_one_without_layers():
+    c = _cache()
+    h = torch.zeros(1, 0, 128, dtype=torch.bfloat16)
+    assert paged_verify_pass([None], h, c, [0, 0, 0]) is h
+    with pytest.raises(ValueError, match="counts"):
+        paged_verify_pass([None], h, c, [0, 1, 0])
