@@ -1502,7 +1502,11 @@ int fitq_token_logprobs_bwd(const void* logits, int dtype, const int64_t* ids, i
   int rc = logprob_shape("token_logprobs_bwd", logits, dtype, ids, rows, vocab, stride, top);
   if (rc) return rc;
   if (!stats || !entropy || !d || (g_top && !top_ids)) return fail(FITQ_ERR_ARG, "token_logprobs_bwd: NULL tensor");
-  if (d == logits && stride != vocab) return fail(FITQ_ERR_ARG, "token_logprobs_bwd: d must not overlap strided logits");
+  // the marked elements' logits are read again behind the first write
+  const uintptr_t size = dtype == FITQ_DTYPE_F32 ? 4 : 2, z0 = reinterpret_cast<uintptr_t>(logits), d0 = reinterpret_cast<uintptr_t>(d);
+  if (d0 < z0 + static_cast<uintptr_t>((rows - 1) * stride + vocab) * size &&
+      z0 < d0 + static_cast<uintptr_t>(rows * vocab) * size)
+    return fail(FITQ_ERR_ARG, "token_logprobs_bwd: d must not overlap the logits");
   if (reinterpret_cast<uintptr_t>(d) & 15u) return fail(FITQ_ERR_ALIGN, "token_logprobs_bwd: d not 16-byte aligned");
   if (!current_sms(&rc)) return rc;
   return launch_status(fitq::launch_token_logprobs_bwd(logits, dtype, ids, rows, vocab, stride, top, stats, entropy,

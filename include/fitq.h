@@ -404,8 +404,8 @@ FITQ_API int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_
  * (row maximum and log of the sum behind it) for the backward, or NULL; top_logp fp32,
  * top_ids int64 [rows, top], largest logit first, the lower index where two are
  * equal, a NaN before all.  -inf logits have probability 0; a row of nothing else
- * gives NaN.  The backward writes d [rows, vocab] (dtype, contiguous) from the
- * upstream gradients g_logp, g_entropy [rows], g_top [rows, top], each NULL for 0. */
+ * gives NaN.  The backward writes d [rows, vocab] (dtype, contiguous, not over the
+ * logits) from the upstream gradients g_logp, g_entropy [rows], g_top [rows, top], each NULL for 0. */
 FITQ_API int fitq_token_logprobs(const void* logits, int dtype, const int64_t* ids, int64_t rows,
                                  int64_t vocab, int64_t stride, int top, float* logp,
                                  float* entropy, float* stats, float* top_logp, int64_t* top_ids,

@@ -98,6 +98,8 @@ def test_logprob_refusals(L):
     assert fwd(z=P + 1) == ALIGN and fwd(dtype=2, z=P + 2) == ALIGN and fwd(ids=P + 4) == ALIGN
     assert fwd(rows=0) == 0 and bwd(rows=0) == 0
     assert bwd(stats=None) == ARG and bwd(d=None) == ARG and bwd(top_ids=None) == ARG
+    assert bwd(d=P) == ARG and bwd(d=P + 4 * 100 * 2 - 16) == ARG  # over the logits
+    assert bwd(stride=104, d=P + 3 * 104 * 2) == ARG
     assert bwd(stride=128, d=P) == ARG and bwd(d=P + 4104) == ALIGN
 
 
