@@ -1374,6 +1374,12 @@ static int kv4_view(const char* what, const fitq_kv4* c, int heads, fitq::Kv4Seq
   return FITQ_OK;
 }
 
+// Whether `bytes` from a on and `tokens` rows of `row` 16-bit elements, `stride` apart, from b on meet.
+static bool kv4_meets(const void* a, int64_t bytes, const void* b, int64_t tokens, int64_t stride, int64_t row) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + static_cast<uintptr_t>((tokens - 1) * stride + row) * 2 && y < x + static_cast<uintptr_t>(bytes);
+}
+
 static bool kv4_dtype(int dtype) { return dtype == FITQ_DTYPE_BF16 || dtype == FITQ_DTYPE_F16; }
 
 int fitq_kv4_append(const fitq_kv4* cache, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
@@ -1393,6 +1399,11 @@ int fitq_kv4_append(const fitq_kv4* cache, const void* q, int64_t q_stride, cons
   if (q_out == q && q_stride != row) return fail(FITQ_ERR_ARG, "kv4_append: q_out is q, but q is strided");
   if (!al16(q) || !al16(k) || !al16(v) || !al16(q_out) || !al16(cos_half) || !al16(sin_half))
     return fail(FITQ_ERR_ALIGN, "kv4_append: 16-byte alignment");
+  const int64_t out_bytes = cache->tokens * row * 2;
+  if ((q_out != q && kv4_meets(q_out, out_bytes, q, cache->tokens, q_stride, row)) ||
+      kv4_meets(q_out, out_bytes, k, cache->tokens, k_stride, kv_row) ||
+      kv4_meets(q_out, out_bytes, v, cache->tokens, v_stride, kv_row))
+    return fail(FITQ_ERR_ARG, "kv4_append: q_out overlaps q (other than being q), k or v");
   const int sms = current_sms(&rc);
   if (!sms) return rc;
   return launch_status(fitq::launch_kv4_append(seq, q, q_stride, k, k_stride, v, v_stride, q_out, cache->pool, cos_half,
@@ -1448,6 +1459,10 @@ int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_stride, v
   if (q_stride < static_cast<int64_t>(heads) * cache->head_dim || q_stride % 8)
     return fail(FITQ_ERR_SHAPE, "kv4_attention: the token stride must cover a token and be a multiple of 8");
   if (!al16(q) || !al16(out) || !al16(workspace)) return fail(FITQ_ERR_ALIGN, "kv4_attention: 16-byte alignment");
+  const int64_t row = static_cast<int64_t>(heads) * cache->head_dim;
+  // (a query's row is read by its own pair's CTAs only, before any of them writes it)
+  if (!(out == q && q_stride == row) && kv4_meets(out, cache->tokens * row * 2, q, cache->tokens, q_stride, row))
+    return fail(FITQ_ERR_ARG, "kv4_attention: out overlaps q, other than being q of dense tokens");
   const int sms = current_sms(&rc);
   if (!sms) return rc;
   const size_t need = fitq::kv4_attention_workspace(cache->batch, cache->kv_heads, group, max_new, max_len,

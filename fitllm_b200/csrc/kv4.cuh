@@ -1,5 +1,5 @@
 // The 4-bit paged key/value cache: block layout and addressing shared by the
-// append, gather and attention kernels (kv4.cu, kv4_attn.cu).
+// append, gather and attention kernels (kv4.cu, kv4_attn.cu, kv4_prompt.cu).
 //
 // A pool holds pages of page_size positions, uint8
 // [pages, KVH, page_size / 16, 18 D]: one block per 16 positions of a KV head.
@@ -139,31 +139,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// (x & mask) | 1024 in both halves, in one instruction (two constants in one
-// expression would be split in two).
-template <uint32_t kMask>
-__device__ __forceinline__ uint32_t nibbles(uint32_t x) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(kMask), "r"(0x64006400u));
-  return d;
-}
-// 1024 + c of the low nibble of each half; 1024 + 16 c of the second one.
-__device__ __forceinline__ uint32_t codes_even(uint32_t x) { return nibbles<0x000f000fu>(x); }
-__device__ __forceinline__ uint32_t codes_odd(uint32_t x) { return nibbles<0x00f000f0u>(x); }
 // The codes as fp16 subnormals: 2^-24 c of the low nibble of each half, 2^-20 c of the
 // second one.
 __device__ __forceinline__ uint32_t tiny_even(uint32_t x) { return x & 0x000f000fu; }
 __device__ __forceinline__ uint32_t tiny_odd(uint32_t x) { return x & 0x00f000f0u; }
-// c - 8 of either.
-__device__ __forceinline__ uint32_t centre_even(uint32_t u) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1032.f, 1032.f));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t centre_odd(uint32_t u) {
-  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(0.0625f, 0.0625f),
-                            __floats2half2_rn(-72.f, -72.f));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) { return Half16<__half>::pack(lo, hi); }
 
 // 2^k with k in [-126, 127].

@@ -6,20 +6,25 @@
 //
 // A KV head's G heads and R / G tokens fold into R = 8 NT columns (column =
 // token * G + head).  With s, l the scale and low of a group and c its codes,
-//   q . k = sum_g s_g (q_g . c_g) + l_g sum(q_g),
-//   o     = sum_g [sum_p (w_p s_pg) (c_pg - 8)] + sum_p w_p (l_pg + 8 s_pg),
-// so the tensor cores multiply the codes themselves; scales and lows are applied
-// in fp32 to scores and weights.  Both products run in fp16 whatever the type of
-// q.  One logic instruction puts two codes into the mantissas of two 1024s, as
-// 1024 + c (even elements of a word) or 1024 + 16 c (odd ones; q / 16 stands
-// against them), so a word of eight codes takes one shift.  For keys that is the
-// operand: the accumulator starts at minus what the offsets add up to (64
-// elements, off by some 2^-24 of 2^10 |q|: 1e-4 in a score at unit scale).
-// Values have the offset taken off by one half2 operation, because their sums run
-// over the whole cache, where it would cancel badly.  Queries are multiplied by a
-// power of two per column (their largest element goes to 2^12, which keeps the
-// eight bits of a bf16 value over 2^26 of range), the weights by one per warp, which
-// keeps w s in fp16's range and rounds it to 2^-12 where bf16 would to 2^-9.
+//   q . k = sum_g s_g (q_g . c_g) + sum_g l_g sum(q_g),
+//   o     = sum_g [sum_p (w_p s_pg) c_pg - 8 sum_p (w_p s_pg)] + sum_p w_p (l_pg + 8 s_pg),
+// so the tensor cores multiply the codes themselves: one logic instruction leaves two
+// codes of a word as the fp16 subnormals 2^-24 c (even elements) or 2^-20 c (odd ones, q
+// / 16 against them), exact in the product, and the factors go back in once per score
+// and per output.  What else is a sum over positions or groups is an MMA of few rows as
+// well: the lows against the queries' sums (in two fp16 pieces), the weights against the
+// scales, lows and a one (the denominator: of the rounded weights, so that their rounding
+// cancels where it is common), and the eights, whose product is taken off exactly where
+// the scaled weights' own rounding would leave a constant behind.
+// Both products run in fp16 whatever the type of q.  Queries are multiplied by a power of
+// two per column (their largest element goes to 2^15, which keeps the eight bits of a
+// bf16 value over 2^29 of range).  Weights are rounded to fp16 and times the scale once
+// more, each by half a step, 2^-11, where bf16 would take 2^-8; they stay below 2^15 and
+// so does their product with a scale.  Scores, maxima, denominators and outputs are fp32.
+//
+// A scale that is no number only makes its own group's elements of the columns that see
+// it none: it reaches them through the parameters' products, and enters the scaled
+// weights as zero.
 //
 // kv4_attn_kernel.  Both products have the cache as the 16-row operand of
 // mma.m16n8k16 (S^T = K.Q^T, O^T = V^T.P^T), the R columns as the n8 operand, so
@@ -28,8 +33,12 @@
 // from accumulator to operand with movmatrix.  Every warp streams its own blocks
 // (2,304 B at D = 128, one bulk copy each) through a private ring and keeps its
 // own reference maximum, sum and output; the warps of a CTA meet once per segment.
-// The reference only moves when a score exceeds it by 2^8 in weight: a vote per
-// block instead of a reduction, the sums have the range to spare.
+// It takes two blocks at a time, so that one's products run in the other's latencies
+// (64 sequences of 100 to 8,191 positions, 40 heads on 8: 86.1 -> 83.9 us; 131,072
+// positions of one: 42.9 -> 40.3 us).  The reference only moves when a score exceeds it
+// by 2^8 in weight: a vote per two blocks instead of a reduction, the sums have the range
+// to spare.  Pages of the next segment are looked up and its queries fetched when a
+// segment begins, its first copies take the places that the last blocks leave.
 //
 // Work split.  The tiles (one block per warp) of all (sequence, KV head) pairs
 // form one list, cut into equal runs, one per CTA, whatever the sequences'
@@ -39,9 +48,14 @@
 //
 // Few pairs of few positions (a single sequence's decode step) take the same kernel
 // in clusters: eight CTAs share a pair's tiles and join their parts over distributed
-// shared memory, one launch without partials in HBM and without the list.
+// shared memory, one launch without partials in HBM and without the list (one sequence
+// of 1,024 positions: 5.9 us).
 //
-// Bound: HBM, 18 D / 16 B per position and KV head.
+// Bound: HBM, 18 D / 16 B per position and KV head, and the instructions of a block (some
+// 270 for eight columns, of 380 that an SM's schedulers have time for at 6.5 TB/s).  The
+// 64 sequences above take 75.5 us, 4.2 TB/s; 200 of them 209 us, 4.6 TB/s; inside the
+// loop it is 5.5 TB/s, the rest is the start (5 us until the first block), the two CTAs
+// of an SM ending apart and the join (4 us).
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -200,8 +214,9 @@ struct AttnSmem {
 // Weights, and weights times scales, stay below 2^15 in fp16; a reference that moves
 // leaves this much (log2) to the weights that follow.
 constexpr float kRoom = 15.f, kSlack = 8.f;
-// A pair's first tile costs a run this many tiles more (queries, the pipeline's
-// start, the warps' meeting): runs are cut by cost.
+// A pair's first tile costs a run this many tiles more (the warps' meeting, the first
+// blocks' reference): runs are cut by cost.  64 sequences of 100 to 8,191 positions take
+// 83.9, 75.5, 78.5 us with 2, 4, 8.
 constexpr int kPairCost = 4;
 __device__ __forceinline__ int pair_cost(const SeqSpan& sp) { return sp.tiles ? sp.tiles + kPairCost : 0; }
 
@@ -1134,7 +1149,10 @@ int attn_td(const Kv4AttnParams& p, const AttnPlan& a, cudaStream_t st) {
   return a.nt == 1 ? attn_t<T, D, 1>(p, a, st) : attn_t<T, D, 2>(p, a, st);
 }
 
-// From 65 rows on the tensor-memory kernel takes the call.
+// From 65 rows on the tensor-memory kernel takes the call.  45 rows of one sequence over
+// 1,000 / 8,000 positions, of eight over 1,000 / 8,000: 10.7 / 20.8 / 27.7 / 79.8 us here,
+// 18.0 / 19.8 / 19.6 / 82.4 us there; 65 rows: 14.6 / 27.0 / 32.0 / 197 and 18.7 / 21.3 /
+// 20.2 / 83.3 us.
 bool prompt_rows(int group, int64_t max_new) { return group * max_new > 64; }
 
 }  // namespace

@@ -15,7 +15,7 @@
 // warp 16 issues the MMAs.  The decoders read blocks straight into registers,
 // one tile ahead, and write K [position][D] and V^T [D][position] as fp16 in the
 // 128-byte-swizzled K-major layout, two buffers each.  A value of the cache is rounded
-// once more, to fp16's 2^-12 (bf16 would round to 2^-9); all are halved, so that a
+// once more, by half a step of fp16, 2^-11 (bf16's is 2^-8); all are halved, so that a
 // group that ends at fp16's largest value stays finite, and the factors go back in with
 // the scores' scale and the final 1 / l.  Queries are scaled per row by a power of
 // two as in kv4_attn.cu.
@@ -33,7 +33,11 @@
 // workspace and kv4_prompt_combine_kernel joins them in order (deterministic).
 //
 // Bound: the exponentials (16 per cycle and SM: 2,048 cycles per 256 x 128 tile) and
-// the MMAs (4 x 128^3: 2,048 cycles) alike.
+// the MMAs (4 x 128^3: 2,048 cycles) alike; measured, the chain of a step (wait, read S,
+// maximum, exponentials, write P) and its hand-overs, some 2,000 cycles of 64 positions
+// that two row tiles per SM cover in part.  Two sequences of up to 2,048 tokens (40 heads
+// on 8) behind up to 513: 173 us, 0.57 PFLOP/s.  Half the exponentials as a polynomial
+// on the FMA pipe made it 183 us, sixteen softmax warps (two threads a row) 200 us.
 #include "kv4.cuh"
 #include "kernels.cuh"
 
@@ -146,6 +150,17 @@ __device__ __forceinline__ uint32_t half_of(uint32_t a) {  // both halves times 
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), __floats2half2_rn(0.5f, 0.5f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+// (x & mask) | 1024 in both halves, in one instruction (two constants in one
+// expression would be split in two).
+template <uint32_t kMask>
+__device__ __forceinline__ uint32_t nibbles(uint32_t x) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(kMask), "r"(0x64006400u));
+  return d;
+}
+// 1024 + c of the low nibble of each half; 1024 + 16 c of the second one.
+__device__ __forceinline__ uint32_t codes_even(uint32_t x) { return nibbles<0x000f000fu>(x); }
+__device__ __forceinline__ uint32_t codes_odd(uint32_t x) { return nibbles<0x00f000f0u>(x); }
 // Codes 0..15 as half2 from the low / second nibble of each half.
 __device__ __forceinline__ uint32_t plain_even(uint32_t x) {
   const uint32_t u = codes_even(x);

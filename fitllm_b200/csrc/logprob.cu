@@ -17,14 +17,17 @@
 // before the first use.  Many rows: a CTA streams its row, eight 16-byte loads
 // in flight per thread.  Alternatives: the k-th largest of 128 thread-group maxima
 // bounds the k-th largest logit of the CTA's share from below; the few elements at
-// or above it are ranked by (value, index), then the CTAs' lists are ranked together.  Where more elements
-// tie than the list holds, k rounds of a maximum search take over.  A streamed row's
+// or above it are ranked by (value, index), then the CTAs' lists are ranked together.
+// Where more elements tie than the list holds, k rounds of a maximum search take over.  A streamed row's
 // bound comes from its first granules, behind which a granule whose maximum reaches
 // it adds to the list on the way; only a list that overflows reads the row again.
-// Bound: HBM (one read) for many rows, latency for few.
+// Bound: HBM (one read) for many rows, latency for few: 2,048 rows of 152,064 bf16
+// logits 139 us, 4.5 TB/s; 40 of fp32 with 5 alternatives 15 us; one of bf16 with 20
+// alternatives 8.8 us.
 //
 // logprob_bwd_kernel: one read and one write of the row; the up to k + 1 marked
-// elements are rewritten behind a CTA barrier.
+// elements are rewritten behind a CTA barrier.  Bound: HBM; 2,048 rows as above 233 us,
+// 5.3 TB/s.
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -44,12 +47,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 // meeting an exponent of -inf.
 constexpr float kLowest = -1000.f;
 constexpr float kFarBelow = -3.402823466e38f;  // a base that stands for -inf: no finite value is smaller
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // max(d, kLowest) that keeps a NaN.
 __device__ __forceinline__ float bounded(float d) {

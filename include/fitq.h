@@ -373,7 +373,8 @@ typedef struct fitq_kv4 {
  * [tokens, heads, head_dim] and codes k (from the fp32 rotation) and v into the
  * pages.  q [tokens, heads, head_dim], k, v [tokens, kv_heads, head_dim] of
  * dtype (FITQ_DTYPE_BF16 or _F16); *_stride: elements from token to token, a
- * multiple of 8.  q_out may be q when q_stride == heads * head_dim. */
+ * multiple of 8.  q_out may be q when q_stride == heads * head_dim, and overlaps none
+ * of the inputs otherwise. */
 FITQ_API int fitq_kv4_append(const fitq_kv4* cache, const void* q, int64_t q_stride, const void* k,
                              int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
                              const float* cos_half, const float* sin_half, int rope_len, int heads,
@@ -384,7 +385,7 @@ FITQ_API int fitq_kv4_gather(const fitq_kv4* cache, void* k, void* v, int dtype,
 /* Attention of the new tokens over the cache, their own positions included
  * (appended before): token i of a sequence sees positions <= prefix + i, query
  * head h reads KV head h / (heads / kv_heads).  q, out [tokens, heads, head_dim]
- * of dtype (q_stride as above); scale 1/sqrt(head_dim), fp32 softmax and sums.
+ * of dtype (q_stride as above; out may be q as above); scale 1/sqrt(head_dim), fp32 softmax and sums.
  * max_new: the most new tokens of one sequence (a sequence with more records
  * FITQ_ERR_ARG, its tokens beyond are not written).  max_len: the most positions of
  * one sequence, if known, else max_pages * page_size; it only sizes the grid.

@@ -179,6 +179,15 @@ def test_attention_is_deterministic_and_ignores_the_hint(cuda_dev, dtype):
     _check_attention(c, _attend(c))
 
 
+@pytest.mark.parametrize("prefix,counts,h,kvh", [([900], [1], 40, 8), ([900, 3, 5000] * 3, [1] * 9, 40, 8),
+                                                 ([400, 30, 900, 0] * 2, [5, 2, 1, 3] * 2, 40, 8), ([3, 500], [60, 41], 8, 2),
+                                                 ([4000], [70], 8, 2)])
+def test_attention_may_write_over_its_queries(cuda_dev, prefix, counts, h, kvh):
+    c = _case(prefix, counts, h, kvh, 128, 64, BF, cuda_dev, seed=8)
+    want = _attend(c)
+    assert torch.equal(_attend(c, out=c["q"]), want)
+
+
 @pytest.mark.parametrize("counts", [[1, 1], [40, 3]])
 def test_attention_never_reads_what_is_hidden(cuda_dev, counts):
     """Positions behind a sequence hold NaN codes' parameters and huge scales."""

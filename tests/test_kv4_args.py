@@ -61,6 +61,8 @@ def test_append_refusals(L):
     assert _append(L, c, rope=0) == SHAPE
     assert _append(L, c, qs=1000) == SHAPE and _append(L, c, qs=1028) == SHAPE and _append(L, c, ks=248) == SHAPE
     assert _append(L, c, q=P, out=P, qs=2048) == ARG
+    far = P + (1 << 20)
+    assert _append(L, c, q=P, out=P + 2048, k=far, v=far) == ARG and _append(L, c, q=far, out=P + 16, k=far) == ARG
     assert _append(L, c, q=P + 2) == ALIGN and _append(L, c, cos=P + 4) == ALIGN
     assert _append(L, _cache(tokens=0)) == 0
 
@@ -76,6 +78,7 @@ def test_attention_refusals(L):
     assert call(c, max_len=0) == SHAPE and call(c, heads=7) == SHAPE
     assert call(c, stride=1020) == SHAPE and call(c, stride=512) == SHAPE
     assert call(c, q=P + 8) == ALIGN
+    assert call(c, stride=1032) == ARG and call(c, out=P + 2048) == ARG and call(c, q=P + 2048) == ARG  # out over q
     assert call(_cache(tokens=0)) == 0
     if not torch.cuda.is_available():
         assert call(c) == NO_DEVICE
