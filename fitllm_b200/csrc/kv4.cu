@@ -4,9 +4,9 @@
 // (rotate-half, fp32 tables indexed by the token's absolute position), the
 // queries are written out in their own type, and the rotated keys (in fp32, not
 // rounded first) and the values are coded in groups of 64:
-//   low = fp16(min), scale = fp16((max - low) / 15),
+//   low = fp16(min), scale = fp16((max - low) * (1 / 15)),
 //   code = round((x - low) * (1 / scale)) in 0..15, 0 where scale is 0,
-// every difference, product and quotient rounded to fp32 on its own (no fused
+// every difference, product and reciprocal rounded to fp32 on its own (no fused
 // multiply-add: a code next to a border is then the same wherever it is
 // computed).  A group that holds a NaN, an infinity or a value fp16 cannot
 // reach gets a non-finite scale and reads back as NaN.
@@ -24,6 +24,7 @@ namespace fitq {
 namespace {
 
 constexpr int kAppThreads = 256;
+constexpr float kFifteenth = 1.f / 15.f;
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -189,8 +190,8 @@ __global__ void __launch_bounds__(kAppThreads, 4) kv4_append_kernel(const Kv4App
       if (is_kv && ok) {
         const __half l0 = __float2half_rn(lo0), l1 = __float2half_rn(lo1);
         const float f0 = __half2float(l0), f1 = __half2float(l1);
-        const __half c0 = __float2half_rn(__fdiv_rn(__fsub_rn(hi0, f0), 15.f));
-        const __half c1 = __float2half_rn(__fdiv_rn(__fsub_rn(hi1, f1), 15.f));
+        const __half c0 = __float2half_rn(__fmul_rn(__fsub_rn(hi0, f0), kFifteenth));
+        const __half c1 = __float2half_rn(__fmul_rn(__fsub_rn(hi1, f1), kFifteenth));
         const float g0 = __half2float(c0), g1 = __half2float(c1);
         const uint32_t w0 = code8(a, f0, g0 > 0.f ? __frcp_rn(g0) : 0.f);
         const uint32_t w1 = code8(bb, f1, g1 > 0.f ? __frcp_rn(g1) : 0.f);

@@ -338,7 +338,7 @@ FITQ_API int fitq_attention_bwd(const void* q, const void* k, const void* v, con
  *               [q_start[b], q_start[b + 1]); NULL: tokens / batch each.  Packed
  *               tokens of no sequence are neither read nor written.
  * The 64-element groups of a key or value are value = scale * code + low, code
- * 0..15, scale and low fp16: low = fp16(min), scale = fp16((max - low) / 15),
+ * 0..15, scale and low fp16: low = fp16(min), scale = fp16((max - low) * (1 / 15)),
  * code = round((x - low) * (1 / scale)), each step rounded to fp32.  A group with
  * a NaN, an infinity or a value outside fp16's range reads back as NaN.  Block
  * bytes, with G = head_dim / 64 and eight elements per 4-byte word (element j in

@@ -13,7 +13,7 @@ def fp32(x):
 def code_group(x):
     """(codes, scale, low) of x [..., 64] fp32, each step rounded to fp32."""
     low = x.amin(-1, keepdim=True).half()
-    scale = ((x.amax(-1, keepdim=True) - low.float()) / fp32(15.0).to(x.device)).half()
+    scale = ((x.amax(-1, keepdim=True) - low.float()) * (fp32(1.0) / fp32(15.0)).to(x.device)).half()
     inv = torch.ones_like(scale, dtype=torch.float32) / scale.float()
     code = torch.where(scale > 0, torch.round((x - low.float()) * inv), torch.zeros_like(x)).clamp(0, 15)
     return code.nan_to_num(0).to(torch.uint8), scale, low
