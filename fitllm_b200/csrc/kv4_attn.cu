@@ -18,9 +18,11 @@
 // the scaled weights' own rounding would leave a constant behind.
 // Both products run in fp16 whatever the type of q.  Queries are multiplied by a power of
 // two per column (their largest element goes to 2^15, which keeps the eight bits of a
-// bf16 value over 2^29 of range).  Weights are rounded to fp16 and times the scale once
-// more, each by half a step, 2^-11, where bf16 would take 2^-8; they stay below 2^15 and
-// so does their product with a scale.  Scores, maxima, denominators and outputs are fp32.
+// bf16 value over 2^29 of range).  Weights are rounded to fp16 by half a step, 2^-11
+// (bf16's is 2^-8), and for bf16 results, whose own rounding is eight times that, once
+// more behind their product with the scale; for fp16 results that product is taken in
+// fp32 and rounded once.  Both stay below 2^15.  Scores, maxima, denominators and outputs
+// are fp32.
 //
 // A scale that is no number only makes its own group's elements of the columns that see
 // it none: it reaches them through the parameters' products, and enters the scaled
@@ -153,6 +155,18 @@ __device__ __forceinline__ void ldmatrix2_t(uint32_t& a, uint32_t& b, const void
                : "memory");
 }
 
+// N neighbouring words (1 or 2) of shared memory.
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint8_t* at) {
+  if (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    w[0] = v.x;
+    w[N - 1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(at);
+  }
+}
+
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(as_half2(a), as_half2(b));
@@ -254,6 +268,8 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   constexpr int kBlk = kv4_block_bytes(D);
   constexpr int kLd = L::kLd;
   constexpr int kWarps = S::kWarps, kTile = S::kTile, kStages = S::kStages, kThreads = S::kThreads;
+  // fp16 results show the weights' rounding before their scaling: there they are scaled in fp32
+  constexpr bool kOnce = std::is_same<T, __half>::value;
   constexpr int kRowV = G == 2 ? 4 : 0;  // the values' first row among a position's quantities
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, qd = lane & 3;
@@ -541,8 +557,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     // one (rows 8-15)
     float m_run[NT][2], o[NT][G][4][4], off[NT][4], sums[NT][4];
     // no scale met so far exceeds cap; weights stay below 2^room
-    uint32_t cap = pack_half2(1.f, 1.f);
-    float room = kRoom;
+    float cap = 1.f, room = kRoom;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -591,13 +606,11 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint8_t* at = blk[u] + 16 * D + (g + 8 * h) * 8 * G;  // [position][K, V][group](scale, low)
-          if (G == 2) {
-            *reinterpret_cast<uint2*>(kp[u][h]) = *reinterpret_cast<const uint2*>(at);
+          load_words(kp[u][h], at);
+          if (G == 2)
             *reinterpret_cast<uint4*>(kw[u][h]) = *reinterpret_cast<const uint4*>(blk[u] + h * 512 + lane * 16);
-          } else {
-            kp[u][h][0] = *reinterpret_cast<const uint32_t*>(at);
+          else
             *reinterpret_cast<uint2*>(kw[u][h]) = *reinterpret_cast<const uint2*>(blk[u] + h * 256 + lane * 8);
-          }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -630,41 +643,48 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           }
         }
 
-      // ---- values' parameters of positions 2 qd, 2 qd + 1 and 8 behind them: the scales
-      // side by side, and all eight quantities of a position as rows of an operand
+      // ---- values' parameters: all eight quantities of a position as rows of an operand,
+      // and the scales, of positions g, g + 8 (kOnce) or side by side of 2 qd, 2 qd + 1 and 8
+      // behind them
       uint32_t vs[N][2][G], va[N][2];
-      __half2 vmax = __float2half2_rn(0.f);
+      float vf[N][2][G];
+      bool over = false;
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         const uint8_t* par = blk[u] + 16 * D;
+        __half2 vmax = __float2half2_rn(0.f);
         if (G == 2) ldmatrix2_t(va[u][0], va[u][1], par + (lane & 15) * 16);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          uint32_t a[G], b[G];
           const uint8_t* at = par + (2 * qd + 8 * h) * 8 * G + 4 * G;
-          if (G == 2) {
-            const uint2 a = *reinterpret_cast<const uint2*>(at), b = *reinterpret_cast<const uint2*>(at + 8 * G);
-            vs[u][h][0] = __byte_perm(a.x, b.x, 0x5410);
-            vs[u][h][G - 1] = __byte_perm(a.y, b.y, 0x5410);
-          } else {
-            const uint32_t a = *reinterpret_cast<const uint32_t*>(at), b = *reinterpret_cast<const uint32_t*>(at + 8 * G);
-            vs[u][h][0] = __byte_perm(a, b, 0x5410);
-            va[u][h] = g & 1 ? __byte_perm(a, b, 0x7632) : vs[u][h][0];
+          if (G == 1 || !kOnce) {
+            load_words(a, at);
+            load_words(b, at + 8 * G);
           }
+          if (G == 1) va[u][h] = __byte_perm(a[0], b[0], g & 1 ? 0x7632 : 0x5410);
+          if (kOnce) load_words(a, par + (g + 8 * h) * 8 * G + 4 * G);
 #pragma unroll
           for (int gr = 0; gr < G; ++gr) {
-            if (edge) {  // whatever lies behind the last position must not matter
+            // whatever lies behind the last position must not matter
+            if (kOnce) {
+              vf[u][h][gr] = __low2float(as_half2(a[gr]));
+              if (edge && pos0 + g + 8 * h >= len) vf[u][h][gr] = 0.f;
+              over |= !(fabsf(vf[u][h][gr]) <= cap);
+            } else {
+              vs[u][h][gr] = __byte_perm(a[gr], b[gr], 0x5410);
               const int left = len - pos0 - 2 * qd - 8 * h;
-              vs[u][h][gr] &= left > 1 ? 0xffffffffu : (left > 0 ? 0xffffu : 0u);
+              if (edge) vs[u][h][gr] &= left > 1 ? 0xffffffffu : (left > 0 ? 0xffffu : 0u);
+              vmax = __hmax2_nan(vmax, __habs2(as_half2(vs[u][h][gr])));
             }
-            vmax = __hmax2_nan(vmax, __habs2(as_half2(vs[u][h][gr])));
           }
         }
+        if (!kOnce) over |= !(__half2float(__hmax_nan(__low2half(vmax), __high2half(vmax))) <= cap);
       }
 
       // ---- scores in log2 units less the reference (position g: columns 2 qd, 2 qd + 1;
       // position g + 8: the same)
       float sc[N][NT][4], x[N][NT][4];
-      bool over = !__hle(__hmax_nan(__low2half(vmax), __high2half(vmax)), __low2half(as_half2(cap)));
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         float ks[2][G];
@@ -695,18 +715,20 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
-              float2 v = Half16<__half>::unpack(vs[u][h][gr]);
+              float2 v = kOnce ? make_float2(vf[u][h][gr], 0.f) : Half16<__half>::unpack(vs[u][h][gr]);
               v.x = fabsf(v.x) <= 65504.f ? v.x : 0.f;
               v.y = fabsf(v.y) <= 65504.f ? v.y : 0.f;
-              vs[u][h][gr] = pack_half2(v.x, v.y);
+              if (kOnce)
+                vf[u][h][gr] = v.x;
+              else
+                vs[u][h][gr] = pack_half2(v.x, v.y);
               vm = fmaxf(vm, fmaxf(fabsf(v.x), fabsf(v.y)));
             }
-        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
-        vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
-        if (vm > __low2float(as_half2(cap))) {
+#pragma unroll
+        for (int y = kOnce ? 4 : 1; y < (kOnce ? 32 : 4); y <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, y));
+        if (vm > cap) {
           const int e = (__float_as_int(vm) >> 23) - 126;  // vm < 2^e
-          const float most = fminf(pow2(e), 65504.f);
-          cap = pack_half2(most, most);
+          cap = pow2(e);
           room = kRoom - static_cast<float>(e);
         }
 #pragma unroll
@@ -751,8 +773,13 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           const uint32_t w0 = movmatrix_t(p0), w1 = movmatrix_t(p1);
 #pragma unroll
           for (int gr = 0; gr < G; ++gr) {
-            pb[u][nt][gr][0] = mul_half2(w0, vs[u][0][gr]);
-            pb[u][nt][gr][1] = mul_half2(w1, vs[u][1][gr]);
+            if (kOnce) {
+              pb[u][nt][gr][0] = movmatrix_t(pack_half2(w[0] * vf[u][0][gr], w[1] * vf[u][0][gr]));
+              pb[u][nt][gr][1] = movmatrix_t(pack_half2(w[2] * vf[u][1][gr], w[3] * vf[u][1][gr]));
+            } else {
+              pb[u][nt][gr][0] = mul_half2(w0, vs[u][0][gr]);
+              pb[u][nt][gr][1] = mul_half2(w1, vs[u][1][gr]);
+            }
           }
           if (!edge) {
             mma_f16(sums[nt], va[u][0], 0x3c003c00u, va[u][1], 0x3c003c00u, w0, w1);
