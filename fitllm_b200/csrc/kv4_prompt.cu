@@ -207,7 +207,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4PromptParams p) {
   using L = PromptSmem<D>;
   constexpr int G = D / 64;
-  __shared__ uint64_t b_qready, b_kfull[2], b_kfree[2], b_vfull[2], b_vfree[2], b_sfull[2][2], b_pready[2][2], b_odone[2], b_done;
+  __shared__ uint64_t b_qready, b_kfull[2], b_kfree[2], b_vfull[2], b_vfree[2], b_sfull[2][2], b_pready[2][2], b_odone[2][2], b_done;
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_abort;
   // per buffer and block: 1 if it has a page, and from bit 8 and 16 the first position
@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
       for (int h = 0; h < 2; ++h) {
         mbar_init(&b_sfull[i][h], 1);
         mbar_init(&b_pready[i][h], kPRows / 32);
+        mbar_init(&b_odone[i][h], 1);
       }
-      mbar_init(&b_odone[i], 1);
     }
     mbar_init(&b_done, 1);
     fence_mbar_init();
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
         m = m_new;
         l *= al;
         if (t > 0) {
-          ok = wait_all(&b_odone[r], (t - 1) & 1);  // the step before has been added
+          ok = wait_all(&b_odone[r][h ^ 1], ((t - 1) >> 1) & 1);  // the step before has been added
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
@@ -429,10 +429,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
       tc_fence_before();
       arrive_warp(&b_pready[r][h]);
     }
-    // the last two steps' products, one by one: a wait by parity tells a phase from its
-    // neighbour only (the one before these is done, S of the last step came behind it)
-    if (ok && steps > 1) ok = wait_all(&b_odone[r], (steps - 2) & 1);
-    if (ok) ok = wait_all(&b_odone[r], (steps - 1) & 1);
+    // the last step's products (and those before them).  A wait by parity tells a phase from
+    // its neighbours only: the steps take two barriers in turn, so that the last phase of
+    // each has none behind it and the one before it was done when S of this step came.
+    if (ok) ok = wait_all(&b_odone[r][(steps - 1) & 1], ((steps - 1) >> 1) & 1);
     if (active && (ok || tiles == 0)) {
       tc_fence_after();
       const bool whole = gridDim.y == 1;
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
         const uint64_t vb = dv + ((buf * L::kV + h * (D * 128) + kk * 32) >> 4);
         umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + h * kPStep + kk * 8, vb, idesc_o, t > 0 || kk > 0 ? 1u : 0u);
       }
-      commit_warp(&b_odone[r]);
+      commit_warp(&b_odone[r][h]);
       if (r == last && (h == 1 || t == steps - 1)) commit_warp(&b_vfree[buf]);
     };
     bool ok = wait_all(&b_qready, 0) && wait_all(&b_kfull[0], 0);

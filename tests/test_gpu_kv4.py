@@ -188,6 +188,24 @@ def test_attention_may_write_over_its_queries(cuda_dev, prefix, counts, h, kvh):
     assert torch.equal(_attend(c, out=c["q"]), want)
 
 
+@pytest.mark.parametrize("d,steps", [(64, 0), (64, 1), (128, 0), (128, 1)])
+def test_many_rows_end_under_every_schedule(cuda_dev, d, steps):
+    """The tensor-memory kernel's roles hand over by parity: many calls whose last tile has one
+    step of positions or two, beside another stream's work, end without a wait run out."""
+    from fitllm_b200 import ops
+    c = _case([128 * (3 + 7 * i) + 64 * steps for i in range(10)], [61] * 10, 32, 8, d, 128, BF, cuda_dev, ragged=False)
+    want = _attend(c)
+    _check_attention(c, want)
+    side, x = torch.cuda.Stream(cuda_dev), torch.randn(4096, 4096, device=cuda_dev)
+    for _ in range(40):
+        with torch.cuda.stream(side):
+            y = x.sin()
+        got = [_attend(c) for _ in range(5)]
+        assert all(torch.equal(g, want) for g in got)
+    side.synchronize()
+    assert y.isfinite().all() and ops.device_status() == 0
+
+
 @pytest.mark.parametrize("counts", [[1, 1], [40, 3]])
 def test_attention_never_reads_what_is_hidden(cuda_dev, counts):
     """Positions behind a sequence hold NaN codes' parameters and huge scales."""
