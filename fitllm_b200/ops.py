@@ -238,48 +238,52 @@ _KV4_DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 def _kv4_cache(what: str, pool: torch.Tensor, page_table: torch.Tensor, prefix: torch.Tensor,
                q_start: Optional[torch.Tensor], tokens: int) -> _lib.Kv4C:
     """The fitq_kv4 descriptor of a call (its pointers live as long as the tensors)."""
-    dev = pool.device
-    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or not pool.is_cuda:
+    dev, shape, table = pool.device, pool.shape, page_table.shape
+    if pool.dtype != torch.uint8 or len(shape) != 4 or not pool.is_contiguous() or not pool.is_cuda:
         raise ValueError(f"{what}: pool must be a contiguous uint8 CUDA tensor [pages, kv_heads, page_size / 16, "
                          "18 * head_dim]")
-    if pool.shape[3] % 18:
-        raise ValueError(f"{what}: pool blocks have {pool.shape[3]} bytes, not 18 * head_dim")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+    pages, kv_heads, per_page, block = shape
+    if block % 18:
+        raise ValueError(f"{what}: pool blocks have {block} bytes, not 18 * head_dim")
+    if page_table.dtype != torch.int32 or len(table) != 2 or not page_table.is_contiguous():
         raise ValueError(f"{what}: page_table must be contiguous int32 [batch, max_pages]")
-    batch = page_table.shape[0]
+    batch, max_pages = table
     if prefix.dtype != torch.int32 or prefix.shape != (batch,) or not prefix.is_contiguous():
         raise ValueError(f"{what}: prefix must be contiguous int32 [batch]")
-    if q_start is not None and (q_start.dtype != torch.int32 or q_start.shape != (batch + 1,)
-                                or not q_start.is_contiguous()):
-        raise ValueError(f"{what}: q_start must be contiguous int32 [batch + 1]")
-    for name, t in (("page_table", page_table), ("prefix", prefix), ("q_start", q_start)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what}: {name} is on {t.device}, the pool on {dev}")
-    return _lib.Kv4C(pool.data_ptr(), page_table.data_ptr(), prefix.data_ptr(), _lib.ptr(q_start), tokens,
-                     pool.shape[0], batch, pool.shape[1], pool.shape[3] // 18, pool.shape[2] * 16,
-                     page_table.shape[1])
+    if page_table.device != dev or prefix.device != dev:
+        raise ValueError(f"{what}: page_table is on {page_table.device}, prefix on {prefix.device}, the pool on {dev}")
+    start = None
+    if q_start is not None:
+        if q_start.dtype != torch.int32 or q_start.shape != (batch + 1,) or not q_start.is_contiguous():
+            raise ValueError(f"{what}: q_start must be contiguous int32 [batch + 1]")
+        if q_start.device != dev:
+            raise ValueError(f"{what}: q_start is on {q_start.device}, the pool on {dev}")
+        start = q_start.data_ptr()
+    return _lib.Kv4C(pool.data_ptr(), page_table.data_ptr(), prefix.data_ptr(), start, tokens, pages, batch, kv_heads,
+                     block // 18, per_page * 16, max_pages)
 
 
 def _kv4_tokens(what: str, name: str, t: torch.Tensor, heads: Optional[int], dim: int, like: torch.Tensor,
                 dev) -> torch.Tensor:
     """t as [tokens, heads, dim] whose heads and elements are dense (tokens may be strided)."""
-    if t.dim() != 3 or t.shape[2] != dim or t.shape[0] != like.shape[0] or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or shape[0] != like.shape[0] or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what}: {name} has shape {tuple(shape)}")
     if t.dtype not in _KV4_DTYPES or t.dtype != like.dtype:
         raise ValueError(f"{what}: {name} must be bf16 or fp16, all of one dtype (got {t.dtype})")
     if t.device != dev:
         raise ValueError(f"{what}: {name} is on {t.device}, the pool on {dev}")
     s0, s1, s2 = t.stride()
-    if s2 != 1 or s1 != dim or s0 % 8 or s0 < t.shape[1] * dim or t.data_ptr() % 16:
+    if s2 != 1 or s1 != dim or s0 % 8 or s0 < shape[1] * dim or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _kv4_out(what: str, name: str, out: Optional[torch.Tensor], shape, dtype, dev) -> torch.Tensor:
+def _kv4_out(what: str, name: str, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    if out.shape != torch.Size(shape) or out.dtype != dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor {tuple(shape)} on {dev}")
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {like.dtype} tensor {tuple(like.shape)} on {like.device}")
     return out
 
 
@@ -309,16 +313,17 @@ def kv4_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool: torch.Te
     q = _kv4_tokens("kv4_append", "q", q, None, d, q, dev)
     k = _kv4_tokens("kv4_append", "k", k, kvh, d, q, dev)
     v = _kv4_tokens("kv4_append", "v", v, kvh, d, q, dev)
+    rows = cos_half.shape
+    if len(rows) != 2 or rows[1] * 2 != d or sin_half.shape != rows:
+        raise ValueError(f"kv4_append: cos_half and sin_half must be of one shape [positions, {d // 2}]")
     for name, t in (("cos_half", cos_half), ("sin_half", sin_half)):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] * 2 != d or not t.is_contiguous() or t.device != dev:
-            raise ValueError(f"kv4_append: {name} must be contiguous fp32 [positions, {d // 2}] on {dev}")
-    if sin_half.shape != cos_half.shape:
-        raise ValueError("kv4_append: cos_half and sin_half differ in shape")
-    out = _kv4_out("kv4_append", "q_out", q_out, q.shape, q.dtype, dev)
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"kv4_append: {name} must be contiguous fp32 on {dev}")
+    out = _kv4_out("kv4_append", "q_out", q_out, q)
     with _on(dev):
         _lib.check(L.fitq_kv4_append(c, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(),
                                      v.stride(0), out.data_ptr(), cos_half.data_ptr(), sin_half.data_ptr(),
-                                     cos_half.shape[0], q.shape[1], _KV4_DTYPES[q.dtype], _raw_stream(dev.index)),
+                                     rows[0], q.shape[1], _KV4_DTYPES[q.dtype], _raw_stream(dev.index)),
                    "fitq_kv4_append")
     return out
 
@@ -361,10 +366,10 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
         max_new = max(1, q.shape[0] // max(1, c.batch))
     if max_len is None:
         max_len = c.max_pages * c.page_size
-    out = _kv4_out("kv4_attention", "out", out, q.shape, q.dtype, dev)
+    out = _kv4_out("kv4_attention", "out", out, q)
     with _on(dev):
         nbytes = L.fitq_kv4_attention_workspace(c, q.shape[1], max_new, max_len)
-        ws = _workspace(nbytes, dev)
+        ws = pool.new_empty(max(nbytes, 1))
         _lib.check(L.fitq_kv4_attention(c, q.data_ptr(), q.stride(0), out.data_ptr(), q.shape[1],
                                         _KV4_DTYPES[q.dtype], max_new, max_len, ws.data_ptr(), nbytes,
                                         _raw_stream(dev.index)), "fitq_kv4_attention")
