@@ -18,12 +18,13 @@
 // in flight per thread.  Alternatives: the k-th largest of 128 thread-group maxima
 // bounds the k-th largest logit of the CTA's share from below; the few elements at
 // or above it are ranked by (value, index), then the CTAs' lists are ranked together.
-// Where more elements tie than the list holds, k rounds of a maximum search take over.  A streamed row's
-// bound comes from its first granules, behind which a granule whose maximum reaches
-// it adds to the list on the way; only a list that overflows reads the row again.
+// Where more elements tie than the list holds, k rounds of a maximum search take over.
+// A streamed row's bound comes from its first granules, behind which a granule whose
+// maximum reaches it is noted and read again at the end; only a list that overflows
+// reads the whole row again.
 // Bound: HBM (one read) for many rows, latency for few: 2,048 rows of 152,064 bf16
-// logits 139 us, 4.5 TB/s; 40 of fp32 with 5 alternatives 15 us; one of bf16 with 20
-// alternatives 8.8 us.
+// logits 119 us, 5.2 TB/s; 40 of fp32 with 5 alternatives 14 us; one of bf16 with 20
+// alternatives 8.6 us.
 //
 // logprob_bwd_kernel: one read and one write of the row; the up to k + 1 marked
 // elements are rewritten behind a CTA barrier.  Bound: HBM; 2,048 rows as above 233 us,
@@ -37,7 +38,6 @@ namespace fitq {
 namespace {
 
 constexpr int kLpThreads = 512;
-constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 64;
 constexpr int kLpGroups = 128;  // thread groups whose maxima bound the k-th largest
 constexpr int kLpList = 1024;   // candidates a CTA ranks
@@ -212,18 +212,27 @@ __device__ __forceinline__ float vec_max<__half>(const uint4& u) {
   return fmaxf(__low2float(m), __high2float(m));
 }
 
-constexpr int kLpUnroll = 8;  // granules in flight per thread of a streamed row, in two halves
+constexpr int kLpUnroll = 8;  // granules in flight per thread of a streamed row
+// From four rows per SM on, without alternatives, CTAs of 256 threads, four on an SM, cover
+// each other's starts and ends better than two of 512: 2,048 / 1,200 / 600 / 400 rows of
+// 152,064 bf16 logits 119 / 80 / 50 / 37 us against 134 / 86 / 50 / 33, 5,000 rows of 32,001 81
+// against 111.  With alternatives, whose bound and ranking are work of a whole CTA, they lose
+// (2,048 rows with 20: 248 against 217 us).
+constexpr int kLpSmall = 256, kLpUnrollSmall = 6, kLpSmallRows = 4;
 
 // kNV > 0: a thread's granules stay in registers; kNV = 0: they are streamed.
-template <typename T, int kNV, bool kTop>
-__global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const LogprobFwdParams p) {
+template <typename T, int kNV, bool kTop, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprob_fwd_kernel(const LogprobFwdParams p) {
+  static_assert(!kTop || kThreads == 4 * kLpGroups, "four threads a group");
   constexpr int kVec = Row<T>::kVec;
-  constexpr int kHeld = kNV > 0 ? kNV : kLpUnroll;
+  constexpr int kLpWarps = kThreads / 32;
+  constexpr int kHeld = kNV > 0 ? kNV : (kThreads == kLpThreads ? kLpUnroll : kLpUnrollSmall);
   __shared__ float sh_m[kLpWarps], sh_s[kLpWarps], sh_t[kLpWarps];
   __shared__ float sh_part[8][3];  // the cluster's parts, in its first CTA
   __shared__ __align__(16) uint32_t sh_group[kTop ? kLpGroups : 4];
   __shared__ uint32_t sh_bound;
-  __shared__ int sh_count;
+  __shared__ int sh_count, sh_granules;
+  __shared__ int sh_granule[kTop && kNV == 0 ? kLpList : 1];  // a streamed row's granules that reach the bound
   __shared__ uint64_t sh_list[kTop ? kLpList : 1];
   __shared__ uint64_t sh_best[kTop ? kLpMaxTop : 1];      // this CTA's top, in order
   __shared__ uint64_t sh_all[kTop ? 8 * kLpMaxTop : 1];   // every CTA's, in the first CTA
@@ -240,7 +249,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const Logpro
   const int v_lo = share * static_cast<int>(cta), v_hi = min(v_lo + share, r.vectors);
 
   uint4 held[kHeld];
-  constexpr int kStep = kLpThreads;  // granules between a thread's own
+  constexpr int kStep = kThreads;  // granules between a thread's own
   // the given token's logit, fetched early
   int64_t id = -1;
   float z_id = 0.f;
@@ -248,38 +257,47 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const Logpro
     id = p.ids[row];
     if (id >= 0 && id < p.V) z_id = to_f32<T>(r.z[id]);
   }
-  // granules [from, to) of `held` are the thread's from granule v0 on
-  auto load_held = [&](auto from, auto to, int v0) {
-#pragma unroll
-    for (int i = from.value; i < to.value; ++i) {
-      const int v = v0 + (i - from.value) * kStep;
-      if (v < v_hi) held[i] = load_vec(r, v);
-    }
-  };
-  // f(granule) over them; a mask of those for which it is true
-  auto for_held = [&](auto from, auto to, int v0, auto f) -> uint32_t {
+  // f(granule) over those of `held` from..to that the thread has, `held` being its granules from
+  // v0 on; a mask of those for which it is true.  refill: each is replaced by the one kHeld
+  // behind it at once.
+  auto for_held = [&](auto from, auto to, auto refill, int v0, auto f) -> uint32_t {
     uint32_t mask = 0;
 #pragma unroll
-    for (int i = from.value; i < to.value; ++i)
-      if (v0 + (i - from.value) * kStep < v_hi && f(held[i])) mask |= 1u << (i - from.value);
+    for (int i = from.value; i < to.value; ++i) {
+      const int v = v0 + i * kStep;
+      if (v < v_hi && f(held[i])) mask |= 1u << i;
+      if (refill.value && v + kHeld * kStep < v_hi) held[i] = load_vec(r, v + kHeld * kStep);
+    }
     return mask;
   };
   constexpr std::integral_constant<int, 0> k0{};
   constexpr std::integral_constant<int, kHeld / 2> kHalf{};
   constexpr std::integral_constant<int, kHeld> kAll{};
+  constexpr std::false_type kKeep{};
+  constexpr std::true_type kRefill{};
+  {
+    const int v0 = v_lo + tid;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (v0 + i * kStep < v_hi) held[i] = load_vec(r, v0 + i * kStep);
+  }
 
   // ---- the elements of a granule that are not below a bound go to the CTA's list
   auto collect = [&](int v, float bound_f) {
     float x[kVec];
     unpack_vec<T>(load_vec(r, v), x);
+    uint32_t hits = 0;
+    const int e0 = r.first(v);
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const int e = r.first(v) + j;
-      if (!(x[j] < bound_f) && e >= 0 && e < r.V) {
-        const int at = atomicAdd(&sh_count, 1);
-        if (at < kLpList) sh_list[at] = key_of(x[j], e);
+    for (int j = 0; j < kVec; ++j)
+      if (!(x[j] < bound_f) && static_cast<uint32_t>(e0 + j) < static_cast<uint32_t>(r.V)) hits |= 1u << j;
+    int at = atomicAdd(&sh_count, __popc(hits));
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      if ((hits >> j) & 1u) {
+        if (at < kLpList) sh_list[at] = key_of(x[j], e0 + j);
+        ++at;
       }
-    }
   };
   // the same for the granules of a mask (few: they are read again)
   auto collect_mask = [&](uint32_t mask, int v0, float bound_f) {
@@ -297,7 +315,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const Logpro
     g = max(g, __shfl_xor_sync(0xffffffffu, g, 1));
     g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
     if ((tid & 3) == 0) sh_group[tid >> 2] = g;
-    if (tid == 0) sh_count = 0;
+    if (tid == 0) sh_count = sh_granules = 0;
     __syncthreads();
     const uint4* all = reinterpret_cast<const uint4*>(sh_group);
     const int own = tid >> 2;
@@ -318,79 +336,84 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const Logpro
   };
 
   // ---- maximum and sums of the thread's share
-  float m = -INFINITY, s = 0.f, t = 0.f, base = 0.f;
+  float m = -INFINITY, base = 0.f;
+  uint64_t s2 = 0, t2 = 0;  // the sums of the even and the odd elements
   auto add = [&](const uint4& u) {
     float x[kVec];
     unpack_vec<T>(u, x);
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) {
+    for (int j = 0; j < kVec; j += 2) {
       // the difference first: it is exact near the maximum, and the type's lowest
       // value times log2 e would overflow
-      const float d = bounded(x[j] - base), e = exp2_approx(d * kLog2e);
-      s += e;
-      t = fmaf(e, d, t);
+      float d0, d1, x0, x1;
+      unpack2(add2(pack2(x[j], x[j + 1]), pack2(-base, -base)), d0, d1);
+      const uint64_t d = pack2(bounded(d0), bounded(d1));
+      unpack2(mul2(d, pack2(kLog2e, kLog2e)), x0, x1);
+      const uint64_t e = pack2(exp2_approx(x0), exp2_approx(x1));
+      s2 = add2(s2, e);
+      t2 = fma2(e, d, t2);
     }
   };
   float bound_f = INFINITY;  // what the alternatives are not smaller than
   auto reaches = [&](const uint4& u) { return vec_max<T>(u) >= bound_f; };
   if (kNV > 0) {
-    load_held(k0, kAll, v_lo + tid);
-    for_held(k0, kAll, v_lo + tid, [&](const uint4& u) {
+    for_held(k0, kAll, kKeep, v_lo + tid, [&](const uint4& u) {
       m = fmaxf(m, vec_max<T>(u));
       return false;
     });
     base = m == -INFINITY ? 0.f : m;
-    for_held(k0, kAll, v_lo + tid, [&](const uint4& u) {
+    for_held(k0, kAll, kKeep, v_lo + tid, [&](const uint4& u) {
       add(u);
       return false;
     });
     if (kTop) {
       bound_f = find_bound(m);
-      collect_mask(for_held(k0, kAll, v_lo + tid, reaches), v_lo + tid, bound_f);
+      collect_mask(for_held(k0, kAll, kKeep, v_lo + tid, reaches), v_lo + tid, bound_f);
     }
   } else {
     // The sums' base only moves when a granule exceeds it by e^20, which they have room
     // for: moving it for every new maximum would cost a warp most of its granules.  The
-    // first granules give a bound already; behind them a granule whose maximum reaches it
-    // adds its elements on the way.
+    // first granules give a bound already.
     auto stream = [&](const uint4& u) -> bool {
       const float mx = vec_max<T>(u);
       m = fmaxf(m, mx);
       if (mx > base + 20.f) {
         const float d = fmaxf(base - mx, kLowest), k = exp2_approx(d * kLog2e);
-        t = k * fmaf(d, s, t);
-        s *= k;
+        t2 = mul2(pack2(k, k), fma2(pack2(d, d), s2, t2));
+        s2 = mul2(pack2(k, k), s2);
         base = mx;
       }
       add(u);
       return kTop && mx >= bound_f;
     };
     int v0 = v_lo + tid;
-    load_held(k0, kHalf, v0);
-    load_held(kHalf, kAll, v0 + kHalf.value * kStep);
     if (v0 < v_hi) {
       const float first = vec_max<T>(held[0]);
       base = first == -INFINITY ? kFarBelow : first;
     }
+    // granules that reach the bound are noted, for the CTA to take together behind the row: at
+    // once a warp would wait for each (2,048 rows of 152,064 with 20 alternatives: 249 -> 217 us)
+    auto note = [&](uint32_t mask) {
+      if (mask == 0) return;
+      for (int at = atomicAdd(&sh_granules, __popc(mask)); mask; mask &= mask - 1, ++at)
+        if (at < kLpList) sh_granule[at] = v0 + (__ffs(mask) - 1) * kStep;
+    };
     if (kTop) {
-      for_held(k0, kHalf, v0, stream);
-      for_held(kHalf, kAll, v0 + kHalf.value * kStep, stream);
+      for_held(k0, kAll, kKeep, v0, stream);
       bound_f = find_bound(m);
-      collect_mask(for_held(k0, kHalf, v0, reaches) |
-                       for_held(kHalf, kAll, v0 + kHalf.value * kStep, reaches) << kHalf.value,
-                   v0, bound_f);
-      v0 += kAll.value * kStep;
-      load_held(k0, kHalf, v0);
-      load_held(kHalf, kAll, v0 + kHalf.value * kStep);
+      note(for_held(k0, kAll, kRefill, v0, reaches));
+      v0 += kHeld * kStep;
     }
-    for (; v0 < v_hi; v0 += kAll.value * kStep) {
-      const uint32_t a = for_held(k0, kHalf, v0, stream);
-      load_held(k0, kHalf, v0 + kAll.value * kStep);
-      const uint32_t b = for_held(kHalf, kAll, v0 + kHalf.value * kStep, stream);
-      load_held(kHalf, kAll, v0 + (kAll.value + kHalf.value) * kStep);
-      if (kTop) collect_mask(a | b << kHalf.value, v0, bound_f);
+    for (; v0 < v_hi; v0 += kHeld * kStep) {
+      const uint32_t mask = for_held(k0, kAll, kRefill, v0, stream);
+      if (kTop) note(mask);
     }
   }
+  float s, t, s_odd, t_odd;
+  unpack2(s2, s, s_odd);
+  unpack2(t2, t, t_odd);
+  s += s_odd;
+  t += t_odd;
   const bool nan_here = s != s;
   const float thread_max = m;
   {
@@ -434,6 +457,12 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const Logpro
     }
   }
   if (kTop) {
+    if (kNV == 0) {
+      const int granules = sh_granules;
+      for (int i = tid; i < granules && granules <= kLpList; i += kThreads) collect(sh_granule[i], bound_f);
+      if (granules > kLpList && tid == 0) sh_count = kLpList + 1;
+      __syncthreads();
+    }
     int count = sh_count;
     if ((kNV == 0 && count > kLpList) || nan_seen) {  // uniform: once more, with the whole share's bound
       __syncthreads();
@@ -445,7 +474,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const Logpro
     if (count <= kLpList) {
       // the list's order varies, the keys' ranks do not: every key is unique; eight
       // threads rank a key
-      for (int i0 = 0; i0 < count; i0 += kLpThreads / 8) {
+      for (int i0 = 0; i0 < count; i0 += kThreads / 8) {
         const int i = i0 + (tid >> 3);
         const uint64_t k = i < count ? sh_list[i] : 0;
         int rank = 0;
@@ -513,7 +542,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprob_fwd_kernel(const Logpro
   if (kTop) {
     // every list is in order: a key's rank is its place in its own list and the
     // number of larger keys in each other one
-    for (int i = tid; i < static_cast<int>(ctas) * kLpMaxTop; i += kLpThreads) {
+    for (int i = tid; i < static_cast<int>(ctas) * kLpMaxTop; i += kThreads) {
       const int own = i / kLpMaxTop, place = i % kLpMaxTop;
       if (place >= p.top) continue;
       const uint64_t k = sh_all[i];
@@ -629,11 +658,13 @@ __global__ void __launch_bounds__(kLbThreads) logprob_bwd_kernel(const LogprobBw
 }
 
 template <typename T, int kNV>
-int fwd_t(const LogprobFwdParams& p, int64_t rows, int ctas, cudaStream_t st) {
-  auto* kernel = p.top > 0 ? logprob_fwd_kernel<T, kNV, true> : logprob_fwd_kernel<T, kNV, false>;
+int fwd_t(const LogprobFwdParams& p, int64_t rows, int ctas, cudaStream_t st, bool small = false) {
+  auto* kernel = p.top > 0 ? logprob_fwd_kernel<T, kNV, true, kLpThreads>
+                 : small   ? logprob_fwd_kernel<T, 0, false, kLpSmall>
+                           : logprob_fwd_kernel<T, kNV, false, kLpThreads>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.blockDim = dim3(p.top == 0 && small ? kLpSmall : kLpThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -660,7 +691,7 @@ int fwd_sized(const LogprobFwdParams& p, int64_t rows, cudaStream_t st, int num_
   const int64_t per = (vectors + ctas - 1) / ctas;
   if (per <= 2 * kLpThreads) return fwd_t<T, 2>(p, rows, ctas, st);
   if (per <= 5 * kLpThreads) return fwd_t<T, 5>(p, rows, ctas, st);
-  return fwd_t<T, 0>(p, rows, ctas, st);
+  return fwd_t<T, 0>(p, rows, ctas, st, ctas == 1 && rows >= kLpSmallRows * num_sms);
 }
 
 template <typename T>
