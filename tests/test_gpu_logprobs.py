@@ -54,6 +54,8 @@ CASES = [
     (7, 4099, FP, 5, None, 0), (1, 32001, F32, 64, None, 1), (300, 8191, BF, 3, 8200, 5), (4, 152064, BF, 20, None, 0),
     (600, 152064, BF, 1, None, 0), (1, 152064, F32, 20, None, 0), (3, 151665, FP, 8, 152064, 0), (2, 500009, F32, 5, None, 0),
     (2, 1000003, BF, 64, None, 0), (149, 50257, BF, 0, None, 0), (37, 20000, F32, 64, None, 0),
+    # many rows: CTAs of 256 threads
+    (600, 30001, FP, 0, None, 1), (700, 24000, BF, 0, 24008, 3), (592, 12289, F32, 0, None, 0),
 ]
 
 
@@ -113,6 +115,32 @@ def test_masked_nan_and_infinite_logits(cuda_dev):
     assert bool((z.grad[0, 1000:] == 0).all()) and bool((z.grad[4, 10:] == 0).all())
     assert int(r.top_ids[2, 0]) == 17 and int(r.top_ids[3, 0]) == 9
     assert r.top_ids[1].tolist() == [0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("dtype,vocab", [(BF, 30000), (FP, 30001), (F32, 12345)])
+@pytest.mark.parametrize("top", [20, 0])
+def test_ties_masks_and_nans_in_streamed_rows(cuda_dev, dtype, vocab, top):
+    """More rows than find room as clusters: a row's candidates overflow their list, or hold a NaN."""
+    from fitllm_b200.lm_head import token_logprobs
+    rows, kinds = 700, 7
+    z, ids = _logits(rows, vocab, dtype, cuda_dev, seed=vocab)
+    z[0::kinds] = 0.0
+    z[1::kinds] = float("-inf")
+    z[1::kinds, 7] = z[1::kinds, vocab - 1] = 1.0
+    z[2::kinds] = (torch.arange(vocab, device=cuda_dev) // 50 * -1.0).to(dtype).clamp(min=torch.finfo(dtype).min)
+    z[3::kinds] = torch.finfo(dtype).min
+    z[4::kinds, vocab // 2] = float("nan")
+    z[5::kinds, 20:] = torch.finfo(dtype).min
+    ids[1::kinds] = 7
+    r = token_logprobs(z, ids, top=top)
+    keep = torch.arange(rows, device=cuda_dev) % kinds != 4
+    lp, logp, ent, top_lp, order = _want(z[keep], ids[keep], top)
+    assert bool(((r.logp.double()[keep] - logp).abs() <= 2.0 ** -17 + 2.0 ** -23 * logp.abs()).all())
+    assert bool(((r.entropy.double()[keep] - ent).abs() <= 2.0 ** -17 * (1 + ent)).all())
+    assert bool(r.logp[~keep].isnan().all()) and bool(r.entropy[~keep].isnan().all())
+    assert torch.equal(r.top_ids[keep], order)
+    if top:
+        assert bool((r.top_ids[~keep, 0] == vocab // 2).all())
 
 
 @pytest.mark.parametrize("rows,vocab,dtype,top,stride,offset",
