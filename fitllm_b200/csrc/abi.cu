@@ -1445,8 +1445,9 @@ int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_stride, v
   if (!q || !out || !workspace) return fail(FITQ_ERR_ARG, "kv4_attention: NULL tensor or workspace");
   if (!kv4_dtype(dtype)) return fail(FITQ_ERR_UNSUPPORTED, "kv4_attention: dtype must be bf16 or fp16 (got %d)", dtype);
   const int group = heads / cache->kv_heads;
+  // (256 rows of a pair are a CTA of the grid's first dimension at most)
   if (max_new <= 0 || max_new > cache->tokens || max_len <= 0 || max_len >= (1ll << 31) ||
-      group * max_new > 16ll * 65535)
+      (group * max_new / 256 + 1) * cache->batch * cache->kv_heads >= (1ll << 31))
     return fail(FITQ_ERR_SHAPE, "kv4_attention: bad max_new=%lld or max_len=%lld (tokens=%lld, heads / kv_heads=%d)",
                 (long long)max_new, (long long)max_len, (long long)cache->tokens, group);
   if (!cache->q_start && max_new < seq.t_new)

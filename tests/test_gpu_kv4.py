@@ -326,6 +326,23 @@ def test_long_pools_and_many_sequences(cuda_dev):
     _check_attention(small, o)
 
 
+def test_a_long_prompt_of_many_heads(cuda_dev):
+    """More than 2^20 rows in one call."""
+    n, h, d, ps = 131072, 8, 64, 128
+    g = torch.Generator(device=cuda_dev).manual_seed(6)
+    table, pages = ref.page_table([n], ps, g, cuda_dev)
+    pool = ref.random_pool(pages, 1, ps, d, g, cuda_dev)
+    q = torch.randn(n, h, d, generator=g, device=cuda_dev, dtype=BF)
+    from fitllm_b200 import ops
+    o = ops.kv4_attention(q, pool, table, torch.zeros(1, dtype=torch.int32, device=cuda_dev))
+    k, v = (x[0] for x in ref.read_sequence(pool, table[0], n))
+    for i in (0, 1, 127, 128, 5000, 65535, 100001, n - 1):
+        want = torch.softmax(q[i].double() @ k[:i + 1].T / d ** 0.5, -1) @ v[:i + 1]
+        bound = U[BF] * (8 * 0.3 + want.abs()) + 2.0 ** -10 * 2 * (8 * 0.3 + 1)
+        assert bool(((o[i].double() - want).abs() <= bound).all())
+    assert ops.device_status() == 0
+
+
 def test_captured_calls_follow_lengths_on_another_stream(cuda_dev):
     from fitllm_b200 import ops
     c = _case([500, 100], [1, 1], 40, 8, 128, 64, BF, cuda_dev, ragged=False)
@@ -358,3 +375,31 @@ def test_captured_calls_follow_lengths_on_another_stream(cuda_dev):
             assert torch.equal(q, gq) and torch.equal(o, go)
         # sequence 1 has pages for 128 positions: the second round leads behind them
         assert ops.device_status() == (1 if pre[1] > 127 else 0)
+
+
+def test_two_threads_on_two_streams(cuda_dev):
+    """Calls at once share nothing but the pool they read."""
+    import threading
+    from fitllm_b200.lm_head import token_logprobs
+    a = _case([900, 3, 5000], [1, 1, 1], 40, 8, 128, 64, BF, cuda_dev, ragged=False)
+    b = _case([700, 90], [60, 41], 8, 2, 128, 64, FP, cuda_dev)
+    z = torch.randn(40, 32001, device=cuda_dev)
+    ids = torch.arange(40, device=cuda_dev)
+    jobs = [lambda: _attend(a), lambda: _attend(b), lambda: token_logprobs(z, ids, top=8).top_logp]
+    want = [f() for f in jobs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(order):
+        with torch.cuda.stream(torch.cuda.Stream(cuda_dev)):
+            for _ in range(30):
+                got = [(i, jobs[i]()) for i in order]
+                torch.cuda.current_stream().synchronize()
+                bad.extend(i for i, g in got if not torch.equal(g, want[i]))
+
+    threads = [threading.Thread(target=work, args=(o,)) for o in ([0, 1, 2], [2, 0, 1])]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

@@ -250,3 +250,12 @@ def test_forward_and_backward_in_a_captured_graph_and_on_another_stream(cuda_dev
         e = token_logprobs(leaf, ids, top=3)
         want, = torch.autograd.grad(e.logp, leaf, up)
         assert torch.equal(r.logp, e.logp) and torch.equal(r.top_ids, e.top_ids) and torch.equal(grad, want)
+
+
+def test_a_second_derivative_is_refused(cuda_dev):
+    from fitllm_b200.lm_head import token_logprobs
+    z = torch.randn(3, 50, device=cuda_dev, requires_grad=True)
+    r = token_logprobs(z, torch.tensor([1, 2, 3], device=cuda_dev))
+    (g,) = torch.autograd.grad(r.logp.sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

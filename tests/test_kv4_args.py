@@ -80,8 +80,11 @@ def test_attention_refusals(L):
     assert call(c, q=P + 8) == ALIGN
     assert call(c, stride=1032) == ARG and call(c, out=P + 2048) == ARG and call(c, q=P + 2048) == ARG  # out over q
     assert call(_cache(tokens=0)) == 0
+    wide = dict(tokens=1 << 28, batch=1, max_pages=1 << 20)
+    assert call(_cache(**wide, kv_heads=8), heads=8 * 4096, stride=8 * 4096 * 128, max_new=1 << 28) == SHAPE
     if not torch.cuda.is_available():
-        assert call(c) == NO_DEVICE
+        assert call(c, out=P + 65536) == NO_DEVICE
+        assert call(_cache(**dict(wide, tokens=131072), kv_heads=1), max_new=131072, out=P + (1 << 30)) == NO_DEVICE
     assert L.fitq_kv4_attention_workspace(c, 8, 2, 192) > 0
     assert L.fitq_kv4_attention_workspace(c, 7, 2, 192) == 0
     assert L.fitq_kv4_attention_workspace(c, 8, 0, 192) == 0
