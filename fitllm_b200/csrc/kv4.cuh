@@ -98,6 +98,13 @@ __device__ __forceinline__ int64_t kv4_block_offset(const Kv4Seq& s, int pg, int
   return ((static_cast<int64_t>(pg) * s.kv_heads + kvh) * per + in_page) * kv4_block_bytes(dim);
 }
 
+// A warp's wait: every lane goes on, or none (a wait ran out).  A lane decides by its own
+// view of the barrier, the abort flag and the clock; behind the wait stand shuffles, votes
+// and MMAs of the whole warp, which lanes that had given up would never reach.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status));
+}
+
 // 16-bit activations: bf16 or fp16.
 template <typename T>
 struct Half16;

@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         const uint32_t st = (taken + u) % kStages;
-        if (!mbar_wait(&bars[st], ((taken + u) / kStages) & 1u, &sh_abort, p.status)) return false;
+        if (!mbar_wait_warp(&bars[st], ((taken + u) / kStages) & 1u, &sh_abort, p.status)) return false;
         blk[u] = ring + st * kBlk;
       }
       const int pos0 = pos_first + j * kTile;  // of the first block; an edge is one block

@@ -257,9 +257,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   const uint32_t tmem = sh_tmem;  // S_0, S_1 (128 columns each), O_0, O_1 (D each, 128 apart)
   const uint32_t s_q = base, s_k = base + L::kOffK, s_v = base + L::kOffV;
 
-  // a warp's wait: all of its lanes go on, or none (a wait ran out)
   auto wait_all = [&](uint64_t* bar, uint32_t parity) -> bool {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, &sh_abort, p.status));
+    return mbar_wait_warp(bar, parity, &sh_abort, p.status);
   };
 
   auto arrive_warp = [&](uint64_t* bar) {  // behind every lane's stores and fences
