@@ -96,6 +96,7 @@ struct Kv4AttnParams {
   float* ml_part; // [row tiles][runs + pairs][R][2]
   Kv4Cut* cuts;   // [row tiles][runs]
   int heads, group;
+  int max_new;    // the most new tokens of a sequence that the launch covers
   int group_mul;  // ceil(2^16 / group): n / group for n of a few hundred
   float scale_log2;  // log2(e) / sqrt(D)
   int* status;
@@ -173,9 +174,10 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Tiles of sequence b that columns [col0, col0 + R) see, and its lengths.
+// Tiles of sequence b that columns [col0, col0 + R) see, and its lengths.  Tokens from
+// max_new on have no columns, whatever the device-side counts say.
 struct Columns {
-  int group, mul;
+  int group, mul, max_new;
   __device__ __forceinline__ int token(int n) const { return (n * mul) >> 16; }
 };
 
@@ -192,7 +194,7 @@ __device__ __forceinline__ SeqSpan seq_span(const Kv4Seq& s, int b, const Column
   SeqSpan r;
   kv4_tokens(s, b, r.first, r.count);
   r.pre = s.prefix[b];
-  int64_t total = static_cast<int64_t>(r.count) * c.group - col0;
+  int64_t total = static_cast<int64_t>(min(r.count, c.max_new)) * c.group - col0;
   r.cols = total <= 0 ? 0 : (total > R ? R : static_cast<int>(total));
   int64_t len = 0;
   if (r.cols > 0 && r.pre >= 0) {
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, qd = lane & 3;
   const int col0 = blockIdx.y * R;
-  const Columns columns{p.group, p.group_mul};
+  const Columns columns{p.group, p.group_mul, p.max_new};
 
   uint8_t* ring = g_kv4_smem + warp * (kStages * kBlk);
   float* mrg_o = reinterpret_cast<float*>(g_kv4_smem + L::kRing);
@@ -300,11 +302,11 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   pdl_wait();  // q and the cache append come from the previous kernels
 
   const Kv4Seq& s = p.seq;
-  // a negative prefix, positions outside the table, more columns than the launch covers
+  // a negative prefix, positions outside the table, more tokens than the launch covers
   auto check_sequence = [&](const SeqSpan& sp) {
     if (sp.count > 0 &&
         (sp.pre < 0 || static_cast<int64_t>(sp.pre) + sp.count > (static_cast<int64_t>(s.max_pages) << s.page_shift) ||
-         static_cast<int64_t>(sp.count) * p.group > static_cast<int64_t>(gridDim.y) * R))
+         sp.count > p.max_new))
       report_device_error(p.status, FITQ_ERR_ARG);
   };
   uint32_t total = 0, per = 0, t_lo = 0, t_hi = 0;
@@ -1030,7 +1032,7 @@ __global__ void __launch_bounds__(32 * kCWarps) kv4_attn_combine_kernel(const Kv
   const Kv4Cut cut = p.cuts[blockIdx.z * runs + run];
   if (n >= cut.cols || cut.count == 0) return;
   const int col0 = blockIdx.z * R;
-  const Columns columns{p.group, p.group_mul};
+  const Columns columns{p.group, p.group_mul, p.max_new};
   const int64_t slot0 = cut.slot;
   const float2* ml = reinterpret_cast<const float2*>(p.ml_part) + slot0 * R + n;
   const float* row = p.o_part + (slot0 * R + n) * D + lane * kE;
@@ -1210,6 +1212,7 @@ int launch_kv4_attention(const Kv4Seq& seq, const void* q, int64_t q_stride, con
   p.o_part = reinterpret_cast<float*>(ws + a.o_off);
   p.heads = heads;
   p.group = group;
+  p.max_new = static_cast<int>(max_new);
   p.group_mul = (65536 + group - 1) / group;
   p.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(dim));
   p.status = status;

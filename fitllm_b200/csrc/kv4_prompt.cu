@@ -75,6 +75,7 @@ struct Kv4PromptParams {
   float* ml_part;  // [CTAs without splits][splits][256 rows][2], splits > 1 only
   float* o_part;   // [..][D]
   int heads, group, row_pairs;
+  int max_new;  // the most new tokens of a sequence that the launch covers
   float scale_log2;
   int* status;
   Kv4Seq seq;
@@ -210,10 +211,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   kv4_tokens(s, b, first, count);
   const int pre = s.prefix[b];
   const int64_t room = static_cast<int64_t>(s.max_pages) << s.page_shift;
-  const int64_t rows_all = static_cast<int64_t>(count) * p.group;
+  const int64_t rows_all = static_cast<int64_t>(min(count, p.max_new)) * p.group;
   if (rp == 0 && kvh == 0 && blockIdx.y == 0 && tid == 0 && count > 0 &&
-      (pre < 0 || static_cast<int64_t>(pre) + count > room ||
-       rows_all > static_cast<int64_t>(p.row_pairs) * 2 * kPRows))
+      (pre < 0 || static_cast<int64_t>(pre) + count > room || count > p.max_new))
     report_device_error(p.status, FITQ_ERR_ARG);
   const int64_t row0 = static_cast<int64_t>(rp) * 2 * kPRows;
   if (row0 >= rows_all) return;
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Kv4Prompt
   kv4_tokens(s, b, first, count);
   const int in_cta = static_cast<int>(blockIdx.y) * 8 + warp;
   const int64_t row = static_cast<int64_t>(rp) * 2 * kPRows + in_cta;
-  if (row >= static_cast<int64_t>(count) * p.group) return;
+  if (row >= static_cast<int64_t>(min(count, p.max_new)) * p.group) return;
   const int64_t part0 = cta * splits * (2 * kPRows) + in_cta;  // part c: + c * 256
   float2 ml = make_float2(kPFloor, 0.f);
   if (lane < splits) ml = *reinterpret_cast<const float2*>(p.ml_part + (part0 + lane * (2 * kPRows)) * 2);
@@ -767,7 +767,7 @@ int launch_kv4_prompt(const Kv4Seq& seq, const void* q, int64_t q_stride, const 
   float* ml = static_cast<float*>(workspace);
   float* o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + a.o_off);
   const Kv4PromptParams p{q, q_stride, out, static_cast<const uint8_t*>(pool), ml, o, heads, group, a.row_pairs,
-                          1.4426950408889634f / sqrtf(static_cast<float>(dim)), status, seq};
+                          static_cast<int>(max_new), 1.4426950408889634f / sqrtf(static_cast<float>(dim)), status, seq};
   if (dtype == FITQ_DTYPE_BF16)
     return dim == 128 ? prompt_t<__nv_bfloat16, 128>(p, a, st) : prompt_t<__nv_bfloat16, 64>(p, a, st);
   return dim == 128 ? prompt_t<__half, 128>(p, a, st) : prompt_t<__half, 64>(p, a, st);
