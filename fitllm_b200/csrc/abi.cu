@@ -1427,10 +1427,17 @@ int fitq_kv4_gather(const fitq_kv4* cache, void* k, void* v, int dtype, fitq_str
                        "kv4_gather");
 }
 
+// Whether attention's launch covers such a call: sizes in 31 bits, and 256 rows of a pair are a CTA of
+// the grid's first dimension at most.
+static bool kv4_attention_fits(const fitq_kv4* c, int heads, int64_t max_new, int64_t max_len) {
+  return c->batch > 0 && c->kv_heads > 0 && c->kv_heads <= 65535 && heads > 0 && heads <= 65535 &&
+         heads % c->kv_heads == 0 && max_new > 0 && max_new < (1ll << 31) && max_len > 0 && max_len < (1ll << 31) &&
+         static_cast<int64_t>(c->batch) * c->kv_heads < (1ll << 28) &&
+         heads / c->kv_heads * max_new / 256 + 1 <= ((1ll << 31) - 1) / (static_cast<int64_t>(c->batch) * c->kv_heads);
+}
+
 size_t fitq_kv4_attention_workspace(const fitq_kv4* cache, int heads, int64_t max_new, int64_t max_len) {
-  if (!cache || cache->batch <= 0 || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads != 0 || max_new <= 0 ||
-      max_len <= 0)
-    return 0;
+  if (!cache || !kv4_attention_fits(cache, heads, max_new, max_len)) return 0;
   return fitq::kv4_attention_workspace(cache->batch, cache->kv_heads, heads / cache->kv_heads, max_new, max_len,
                                        cache->head_dim, sms_for_sizing());
 }
@@ -1445,9 +1452,7 @@ int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_stride, v
   if (!q || !out || !workspace) return fail(FITQ_ERR_ARG, "kv4_attention: NULL tensor or workspace");
   if (!kv4_dtype(dtype)) return fail(FITQ_ERR_UNSUPPORTED, "kv4_attention: dtype must be bf16 or fp16 (got %d)", dtype);
   const int group = heads / cache->kv_heads;
-  // (256 rows of a pair are a CTA of the grid's first dimension at most)
-  if (max_new <= 0 || max_new > cache->tokens || max_len <= 0 || max_len >= (1ll << 31) ||
-      (group * max_new / 256 + 1) * cache->batch * cache->kv_heads >= (1ll << 31))
+  if (max_new > cache->tokens || !kv4_attention_fits(cache, heads, max_new, max_len))
     return fail(FITQ_ERR_SHAPE, "kv4_attention: bad max_new=%lld or max_len=%lld (tokens=%lld, heads / kv_heads=%d)",
                 (long long)max_new, (long long)max_len, (long long)cache->tokens, group);
   if (!cache->q_start && max_new < seq.t_new)

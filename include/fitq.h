@@ -389,7 +389,8 @@ FITQ_API int fitq_kv4_gather(const fitq_kv4* cache, void* k, void* v, int dtype,
  * max_new: the most new tokens of one sequence (a sequence with more records
  * FITQ_ERR_ARG, its tokens beyond are not written).  max_len: the most positions of
  * one sequence, if known, else max_pages * page_size; it only sizes the grid.
- * Deterministic.  A token that sees no position gives zeros. */
+ * Deterministic.  A token that sees no position gives zeros.  The workspace of sizes that
+ * no call takes is 0 bytes. */
 FITQ_API size_t fitq_kv4_attention_workspace(const fitq_kv4* cache, int heads, int64_t max_new,
                                              int64_t max_len);
 FITQ_API int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_stride, void* out,
