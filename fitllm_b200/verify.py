@@ -73,7 +73,8 @@ class PagedKVCache:
     new tokens behind ``lengths`` without moving it: ``advance`` accepts them,
     so that rejected drafts are overwritten by the next pass.  capacity: the most
     positions of one sequence; num_pages: pages shared by all sequences (default:
-    enough for every sequence at capacity)."""
+    enough for every sequence at capacity); rope_theta: the layers' rotary base (a
+    pass refuses layers of another one, whose rotation is not the tables')."""
 
     def __init__(self, num_layers: int, batch: int, kv_heads: int, head_dim: int, capacity: int, device,
                  page_size: int = 64, num_pages: Optional[int] = None, rope_theta: float = 1e6):
@@ -81,7 +82,7 @@ class PagedKVCache:
             raise ValueError(f"PagedKVCache: head_dim must be 64 or 128 (got {head_dim})")
         if page_size not in (16, 32, 64, 128, 256, 512, 1024):
             raise ValueError(f"PagedKVCache: page_size must be a power of two in 16..1024 (got {page_size})")
-        self.page_size, self.capacity = page_size, capacity
+        self.page_size, self.capacity, self.rope_theta = page_size, capacity, rope_theta
         max_pages = -(-capacity // page_size)
         num_pages = batch * max_pages if num_pages is None else num_pages
         shape = (num_pages, kv_heads, page_size // 16, 18 * head_dim)
@@ -96,6 +97,12 @@ class PagedKVCache:
     @property
     def batch(self) -> int:
         return len(self.lengths)
+
+    def check_rotary(self, layer: DecoderLayer) -> None:
+        """Raises where the layer rotates with another base than the cache's tables."""
+        if layer.cfg.rope_theta != self.rope_theta:
+            raise ValueError(f"PagedKVCache: the layer's rope_theta is {layer.cfg.rope_theta:g}, the cache's "
+                             f"{self.rope_theta:g}")
 
     def reserve(self, counts: Sequence[int]) -> None:
         """Pages for counts[b] more positions of every sequence; raises, and changes
@@ -213,6 +220,7 @@ def paged_layer_forward(layer: DecoderLayer, h: torch.Tensor, pool: torch.Tensor
                         max_new: Optional[int] = None) -> torch.Tensor:
     """One layer over new tokens behind a paged cache: h [B, T, hidden] (T tokens of
     every sequence) or, with q_start int32 [batch + 1], [1, tokens, hidden] packed."""
+    cache.check_rotary(layer)
     cfg = layer.cfg
     cos, sin = cache.tables
 
@@ -245,9 +253,11 @@ def paged_verify_pass(layers: List[DecoderLayer], h: torch.Tensor, cache: PagedK
         for c in news:
             starts.append(starts[-1] + c)
         q_start = torch.tensor(starts, dtype=torch.int32, device=h.device)
-    cache.reserve(news)
     if max(news) == 0:
         return h
+    for layer in layers:
+        cache.check_rotary(layer)
+    cache.reserve(news)
     max_len = max(n + c for n, c in zip(cache.lengths, news))
     for i, layer in enumerate(layers):
         h = paged_layer_forward(layer, h, cache.pools[i], cache, max_len, q_start, max(news))
