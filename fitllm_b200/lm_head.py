@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import List, NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
@@ -96,7 +97,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tok
 
     logits [..., V] bf16, fp16 or fp32 (rows may be strided, as in
     logits[..., :tokens]); ids [...] integers, an id outside [0, V) (-100 for
-    instance) has logp 0 and no gradient.  Equal logits rank by index."""
+    instance) has logp 0 and no gradient.  Equal logits rank by index.  There is no
+    forward-mode derivative."""
     if logits.dim() < 1 or ids.shape != logits.shape[:-1]:
         raise ValueError(f"token_logprobs: logits {tuple(logits.shape)} and ids {tuple(ids.shape)} do not match")
     if logits.dtype not in _LOGIT_DTYPES or not logits.is_cuda:
@@ -112,6 +114,8 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top: int = 0) -> Tok
     lead = ids.shape
     if len(lead) != 1 or ids.dtype != torch.int64 or not ids.is_contiguous():
         ids = ids.reshape(-1).to(torch.int64).contiguous()
+    if forward_ad.unpack_dual(z).tangent is not None:  # the kernels would lose it
+        raise NotImplementedError("token_logprobs: logits with a tangent (there is no forward-mode derivative)")
     if z.requires_grad and torch.is_grad_enabled():
         r = _TokenLogProbsFn.apply(z, ids, int(top))
     else:
