@@ -18,7 +18,10 @@ def _stream(dev) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # handle of a device's current stream, without a Stream object
+def _raw_stream(index: int) -> int:
+    """Handle of a device's current stream, without a Stream object (looked up at the
+    call: torch builds without CUDA lack it)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _bf16_2d(t: torch.Tensor, cols: int) -> torch.Tensor:
