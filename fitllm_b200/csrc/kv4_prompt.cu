@@ -21,8 +21,11 @@
 // two as in kv4_attn.cu.
 //
 // The reference m of a row moves only when a weight would exceed 2^15 (fp16's range for
-// P); the thread that moves it rescales its row of O_r once the step before has been
-// added to it.
+// P), and then to 2^7 below the row's largest, so that eight more bits of growth move
+// nothing; the thread that moves it rescales its row of O_r once the step before has been
+// added to it.  Weights keep fp16's 11 bits down to 2^-21 of the largest met and some of
+// them down to 2^-32: behind a first position with 99.9% of the mass, 131,000 others
+// still count (with the reference at the largest itself all of them rounded to zero).
 //
 // A group of V whose scale or low is not finite must only reach the rows that see it,
 // and 0 x NaN would reach all: it enters as zeros, its first position is noted per
@@ -55,6 +58,7 @@ constexpr int kPRegsSoftmax = 128, kPRegsDecode = 80, kPRegsIssue = 64;
 static_assert(2 * kPRegsSoftmax + 2 * kPRegsDecode + kPRegsIssue <= 5 * 96, "more registers than the launch has");
 constexpr float kPFloor = -3.0e38f;
 constexpr float kPRoom = 15.f;    // weights stay below 2^15
+constexpr float kPSlack = 8.f;    // a reference that moves leaves this much (log2) to the weights that follow
 constexpr int kPMaxSplits = 32;   // a lane of the combining warp each
 
 template <int D>
@@ -368,7 +372,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
             top[x] = fmaxf(top[x], fmaxf(__uint_as_float(v[c][i + 2 * x]), __uint_as_float(v[c][i + 2 * x + 1])));
       const float raw = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cn;
       if (__any_sync(0xffffffffu, raw > m + kPRoom)) {
-        const float m_new = fmaxf(m, raw);
+        const float m_new = fmaxf(m, raw - (kPRoom - kPSlack));
         const float al = exp2_approx(m - m_new);
         m = m_new;
         l *= al;

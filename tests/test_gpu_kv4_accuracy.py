@@ -1,0 +1,166 @@
+"""Accuracy of attention over the 4-bit cache, held per token and head to the rounding that the
+kernels state, so that the bound shrinks with the output it is for.
+
+Errors of a row o = sum_p w_p v_p / sum_p w_p (norms over the head's D elements), with r = 2^-11 half a
+step of fp16 and each rounding's error spread evenly over its half steps (standard deviation 1/sqrt(3) of it):
+* the result is rounded once to its type: at most u |o| (u: bf16 2^-8, fp16 2^-11), and for an fp16
+  element below 2^-14, whose steps are 2^-24 however small it is, half of that: 2^-25 sqrt(D) over a row;
+* up to 64 rows: a weight is rounded to fp16, and its product with the group's scale once more; more
+  rows: the weight and the value are.  Either way two roundings of terms not larger than
+  w_p a_p, a_p^2 = sum_d v_pd^2 + (8 s_pd)^2 (codes enter the products less eight);
+* more rows: keys are rounded too, which moves a score by r q.k element by element, and so a
+  weight by kappa_p, kappa_p^2 = sum_d q_d^2 (k_pd^2 + tiny^2) / D, and the row by w_p kappa_p |v_p - o|;
+* below fp16's normal range a rounding is 2^-25 at most: of weights, and of weights times scales, whose
+  largest lies at 2^7 / max(1, s) or above; of halved keys and values and of their halved lows
+  (2^-23 of a value in all: `tiny` is that over r).
+The errors of different positions are independent: they add up in squares.  Three standard deviations
+cover a row (one rounding alone reaches sqrt(3) of its own).  fp32 sums and exponentials are far below.
+"""
+import math
+
+import pytest
+import torch
+
+from tests import kv4_ref as ref
+from tests.test_gpu_kv4 import ATTEND, BF, FP, U, _attend, _case
+
+pytestmark = pytest.mark.gpu
+R = 2.0 ** -11
+TINY = 2.0 ** -23
+
+
+def _params(pool, d):
+    """(scale, low) pairs of a pool as a view [pages, KVH, blocks, 16, key / value, D / 64, 2] fp16."""
+    return pool[..., 16 * d:].view(torch.float16).view(*pool.shape[:3], 16, 2, d // 64, 2)
+
+
+def _scales(pool, table_row, length):
+    """The values' scales float64 [KVH, length, D] behind one row of a page table."""
+    d = pool.shape[3] // 18
+    ps = pool.shape[2] * 16
+    rows = table_row[:-(-length // ps)].long()
+    s = _params(pool, d)[rows][..., 1, :, 0].double()  # [n, KVH, blocks, 16, G]
+    s = s.permute(1, 0, 2, 3, 4).reshape(pool.shape[1], -1, d // 64)[:, :length]
+    return s.repeat_interleave(64, -1)
+
+
+def _rows(q, k, v, s, pre, i0, dtype):
+    """(want, bound) of queries q [n, D] (tokens i0, i0 + 1, ... behind `pre`) over k, v [N, D]."""
+    n, d = q.shape
+    q = q.double()
+    at = torch.arange(k.shape[0], device=q.device)[None]
+    hidden = at > pre + i0 + torch.arange(n, device=q.device)[:, None]
+    p = torch.softmax((q @ k.T / math.sqrt(d)).masked_fill(hidden, float("-inf")), -1)
+    want = p @ v
+    p2, seen = p.square(), (~hidden).double()
+    a2 = (v.square() + (8 * s).square()).sum(-1)
+    kappa2 = q.square() @ (k.square() + (TINY / R) ** 2).T / d
+    away2 = (v.square().sum(-1)[None] - 2 * want @ v.T + want.square().sum(-1)[:, None]).clamp(min=0)
+    wide = 2.0 ** max(0, math.ceil(math.log2(float(s.max().clamp(min=1.0)))))
+    low = p.amax(-1) * 2.0 ** -32 * wide * (seen @ (a2 + 64.0 * d)).sqrt()
+    spread = (p2 @ (2 * a2) + (p2 * kappa2 * away2).sum(-1)).sqrt() * R
+    tiny = TINY * (d * p2.sum(-1)).sqrt()
+    step = 2.0 ** -25 * math.sqrt(d) if dtype == FP else 0.0
+    return want, U[dtype] * want.norm(dim=-1) + step + 3 / math.sqrt(3) * (spread + low + tiny)
+
+
+def _check(c, o, rows=None):
+    """Every row of o, or tokens `rows` of every sequence; returns the largest |o| and the worst ratio."""
+    h, d = c["q"].shape[1:]
+    kvh = c["pool"].shape[1]
+    worst, norms = 0.0, []
+    for b, (pre, a, n) in enumerate(zip(c["prefix"], c["starts"], c["counts"])):
+        if n == 0:
+            continue
+        k, v = ref.read_sequence(c["pool"], c["table"][b], pre + n)
+        s = _scales(c["pool"], c["table"][b], pre + n)
+        for i in range(h):
+            kv = i // (h // kvh)
+            for t in ([slice(0, n)] if rows is None else [slice(r, r + 1) for r in rows]):
+                want, bound = _rows(c["q"][a:a + n][t, i], k[kv], v[kv], s[kv], pre, t.start, c["q"].dtype)
+                err = (o[a:a + n][t, i].double() - want).norm(dim=-1)
+                worst = max(worst, float((err / bound).max()))
+                norms.append((want.norm(dim=-1) / bound).min())
+    assert worst <= 1, f"worst {worst:.2f} of the bound"
+    assert float(min(norms)) > 2, "an output of zeros would pass"
+
+
+@pytest.mark.parametrize("prefix,counts,h,kvh,d,ps,dtype", ATTEND)
+def test_rows_are_as_near_as_their_roundings(cuda_dev, prefix, counts, h, kvh, d, ps, dtype):
+    from fitllm_b200 import ops
+    c = _case(prefix, counts, h, kvh, d, ps, dtype, cuda_dev, seed=2 * h + d + prefix[0], head=1, tail=2)
+    o = _attend(c)
+    assert ops.device_status() == 0
+    _check(c, o)
+
+
+LONG = [([131071], [1], 2, 2, 128, 128, BF), ([131071], [1], 5, 1, 64, 64, FP), ([65000, 40000], [5, 5], 8, 2, 128, 64, FP),
+        ([60000], [70], 2, 1, 128, 128, BF), ([60000, 33333], [40, 40], 16, 8, 64, 64, FP)]
+
+
+@pytest.mark.parametrize("prefix,counts,h,kvh,d,ps,dtype", LONG)
+def test_long_contexts_lose_no_part(cuda_dev, prefix, counts, h, kvh, d, ps, dtype):
+    c = _case(prefix, counts, h, kvh, d, ps, dtype, cuda_dev, seed=3)
+    _check(c, _attend(c))
+
+
+def test_rows_of_a_long_prompt_of_many_heads(cuda_dev):
+    """More than 2^20 rows in one call."""
+    from fitllm_b200 import ops
+    n, h, d, ps = 131072, 8, 64, 128
+    g = torch.Generator(device=cuda_dev).manual_seed(6)
+    table, pages = ref.page_table([n], ps, g, cuda_dev)
+    pool = ref.random_pool(pages, 1, ps, d, g, cuda_dev)
+    q = torch.randn(n, h, d, generator=g, device=cuda_dev, dtype=BF)
+    o = ops.kv4_attention(q, pool, table, torch.zeros(1, dtype=torch.int32, device=cuda_dev))
+    assert ops.device_status() == 0
+    c = dict(q=q, pool=pool, table=table, prefix=[0], starts=[0], counts=[n])
+    _check(c, o, rows=(0, 1, 127, 128, 5000, 65535, 100001, n - 1))
+
+
+FORMS = [([900, 3000, 64], [1, 1, 1], 40, 8), ([3000] * 9, [1] * 9, 40, 8), ([500, 2000], [5, 3], 10, 2),
+         ([700, 40], [60, 90], 8, 4), ([200], [120], 160, 160)]
+
+
+@pytest.mark.parametrize("prefix,counts,h,kvh", FORMS)
+@pytest.mark.parametrize("d,dtype", [(128, BF), (128, FP), (64, BF), (64, FP)])
+def test_peaked_rows_of_queries_with_outlier_channels(cuda_dev, prefix, counts, h, kvh, d, dtype):
+    c = _case(prefix, counts, h, kvh, d, 64, dtype, cuda_dev, seed=d)
+    c["q"] = c["q"] * 3
+    c["q"][..., [3, d - 5]] *= 12
+    c["q"][..., 9] *= 1e-3
+    _check(c, _attend(c))
+
+
+@pytest.mark.parametrize("n", [32768, 131072])
+@pytest.mark.parametrize("batch,count", [(1, 1), (40, 1), (2, 70), (80, 70)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_what_stands_behind_a_strong_first_position(cuda_dev, n, batch, count, dtype):
+    """The first position holds 99.9% of a row's mass and a value of zero; the result is what the rest
+    adds up to.  Sequences share the pages.  One token of one sequence and of many, tiles whose
+    positions are split over CTAs and tiles whose positions are not."""
+    d, ps = 128, 128
+    g = torch.Generator(device=cuda_dev).manual_seed(n)
+    pool = ref.random_pool(n // ps, 1, ps, d, g, cuda_dev)
+    par = _params(pool, d)
+    par[..., 1, :, 1] += 1.0          # values around one
+    par[0, 0, 0, 0, 1] = 0.0          # the first position's are zeros
+    table = torch.arange(n // ps, dtype=torch.int32, device=cuda_dev).expand(batch, -1).contiguous()
+    k, v = (x[0] for x in ref.read_sequence(pool, table[0], n))
+    # q along the first key, so long that its score stands at log(999 * the others' sum)
+    dirn = k[0] / k[0].norm()
+    lo, hi = 0.0, 400.0
+    for _ in range(60):
+        mid = (lo + hi) / 2
+        s = k @ dirn * mid / math.sqrt(d)
+        lo, hi = (mid, hi) if float(s[0] - torch.logsumexp(s[1:], 0)) < math.log(999.0) else (lo, mid)
+    q = (dirn * hi + 0.01 * torch.randn(batch * count, 1, d, generator=g, device=cuda_dev)).to(dtype)
+    pre = n - count
+    c = dict(q=q, pool=pool, table=table, prefix=[pre] * batch, starts=[i * count for i in range(batch)],
+             counts=[count] * batch, pre=torch.full((batch,), pre, dtype=torch.int32, device=cuda_dev), q_start=None,
+             max_new=count, max_len=n)
+    o = _attend(c)
+    few = dict(c, prefix=c["prefix"][:2], starts=c["starts"][:2], counts=c["counts"][:2])
+    _check(few, o)
+    # the sequences differ in their queries' small part only
+    assert float((o.double().mean(-1) / o.double().mean() - 1).abs().max()) < 0.2
