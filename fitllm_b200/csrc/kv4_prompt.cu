@@ -17,8 +17,10 @@
 // 128-byte-swizzled K-major layout, two buffers each.  A value of the cache is rounded
 // once more, by half a step of fp16, 2^-11 (bf16's is 2^-8); all are halved, so that a
 // group that ends at fp16's largest value stays finite, and the factors go back in with
-// the scores' scale and the final 1 / l.  Queries are scaled per row by a power of
-// two as in kv4_attn.cu.
+// the scores' scale and the final 1 / l.  It is the codes that are halved, which is
+// exact: a halved scale would lose a bit below 2^-13, fifteen times over in a value.  What
+// remains there is the rounding of the halved low and of the sum: 2^-23 of a value at most.
+// Queries are scaled per row by a power of two as in kv4_attn.cu.
 //
 // The reference m of a row moves only when a weight would exceed 2^15 (fp16's range for
 // P), and then to 2^7 below the row's largest, so that eight more bits of growth move
@@ -155,27 +157,28 @@ __device__ __forceinline__ uint32_t half_of(uint32_t a) {  // both halves times 
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), __floats2half2_rn(0.5f, 0.5f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// (x & mask) | 1024 in both halves, in one instruction (two constants in one
+// (x & mask) | 512 in both halves, in one instruction (two constants in one
 // expression would be split in two).
 template <uint32_t kMask>
 __device__ __forceinline__ uint32_t nibbles(uint32_t x) {
   uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(kMask), "r"(0x64006400u));
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(kMask), "r"(0x60006000u));
   return d;
 }
-// 1024 + c of the low nibble of each half; 1024 + 16 c of the second one.
+// 512 + c / 2 of the low nibble of each half (fp16's steps are 1/2 there); 512 + 8 c of
+// the second one.
 __device__ __forceinline__ uint32_t codes_even(uint32_t x) { return nibbles<0x000f000fu>(x); }
 __device__ __forceinline__ uint32_t codes_odd(uint32_t x) { return nibbles<0x00f000f0u>(x); }
-// Codes 0..15 as half2 from the low / second nibble of each half.
-__device__ __forceinline__ uint32_t plain_even(uint32_t x) {
+// Half the codes, 0, 1/2 .. 15/2, as half2 from the low / second nibble of each half.
+__device__ __forceinline__ uint32_t halved_even(uint32_t x) {
   const uint32_t u = codes_even(x);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1024.f, 1024.f));
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(512.f, 512.f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t plain_odd(uint32_t x) {
+__device__ __forceinline__ uint32_t halved_odd(uint32_t x) {
   const uint32_t u = codes_odd(x);
   const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(0.0625f, 0.0625f),
-                            __floats2half2_rn(-64.f, -64.f));
+                            __floats2half2_rn(-32.f, -32.f));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -529,14 +532,14 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
         const uint32_t dst = s_k + buf * L::kK + pos * 128;
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-          const uint32_t par = there ? half_of(kpar[i][gr]) : 0u;
-          const uint32_t sc = __byte_perm(par, par, 0x1010), lo = __byte_perm(par, par, 0x3232);
+          const uint32_t par = there ? kpar[i][gr] : 0u, half = half_of(par);
+          const uint32_t sc = __byte_perm(par, par, 0x1010), lo = __byte_perm(half, half, 0x3232);
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const uint32_t x = kw[i][2 * gr + w], y = x >> 8;
             // the eight elements in the order 0 4 1 5 2 6 3 7, as the queries'
-            sts128(dst + gr * (kPTile * 128) + (((2 * lo2 + w) ^ hi) << 4), hfma2_u(plain_even(x), sc, lo),
-                   hfma2_u(plain_odd(x), sc, lo), hfma2_u(plain_even(y), sc, lo), hfma2_u(plain_odd(y), sc, lo));
+            sts128(dst + gr * (kPTile * 128) + (((2 * lo2 + w) ^ hi) << 4), hfma2_u(halved_even(x), sc, lo),
+                   hfma2_u(halved_odd(x), sc, lo), hfma2_u(halved_even(y), sc, lo), hfma2_u(halved_odd(y), sc, lo));
           }
         }
       }
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
         const int h16 = 2 * dw + h;
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
-          const uint32_t sc = half_of(__byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x5410));
+          const uint32_t sc = __byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x5410);
           const uint32_t lo = half_of(__byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x7632));
           // row 64 gr + 8 i + e, positions 8 h16 + 2 q, + 1
           const uint32_t dst =
@@ -585,10 +588,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
           for (int z = 0; z < 2; ++z) {
             const uint32_t x = __byte_perm(vw[h][0][gr], vw[h][1][gr], z ? 0x7632 : 0x5410);
             const uint32_t y = x >> 8;
-            sts32(dst + (4 * z) * 1024, hfma2_u(plain_even(x), sc, lo));
-            sts32(dst + (4 * z + 1) * 1024, hfma2_u(plain_odd(x), sc, lo));
-            sts32(dst + (4 * z + 2) * 1024, hfma2_u(plain_even(y), sc, lo));
-            sts32(dst + (4 * z + 3) * 1024, hfma2_u(plain_odd(y), sc, lo));
+            sts32(dst + (4 * z) * 1024, hfma2_u(halved_even(x), sc, lo));
+            sts32(dst + (4 * z + 1) * 1024, hfma2_u(halved_odd(x), sc, lo));
+            sts32(dst + (4 * z + 2) * 1024, hfma2_u(halved_even(y), sc, lo));
+            sts32(dst + (4 * z + 3) * 1024, hfma2_u(halved_odd(y), sc, lo));
           }
         }
       }

@@ -132,6 +132,23 @@ def test_peaked_rows_of_queries_with_outlier_channels(cuda_dev, prefix, counts, 
     _check(c, _attend(c))
 
 
+@pytest.mark.parametrize("prefix,counts,h,kvh", FORMS)
+@pytest.mark.parametrize("d,dtype", [(128, BF), (128, FP), (64, BF), (64, FP)])
+@pytest.mark.parametrize("factor", [4000.0, 30.0, 2.0 ** -9, 2.0 ** -14])
+def test_values_of_every_size(cuda_dev, prefix, counts, h, kvh, d, dtype, factor):
+    """Value scales from 0.3 x 4,000 (fp16's end) down to 2^-17 (a few steps of fp16's subnormals); every
+    third position keeps a tenth of it, and one sequence meets its largest only late."""
+    c = _case(prefix, counts, h, kvh, d, 64, dtype, cuda_dev, seed=d + 1)
+    par = _params(c["pool"], d)
+    v = par[..., 1, :, :].float() * factor
+    v[:, :, :, ::3] *= 0.1
+    par[..., 1, :, :] = v.half()
+    if factor > 1:  # the pages of the first half of sequence 0 hold small ones
+        early = c["table"][0, :(c["prefix"][0] // 64 + 1) // 2].long()
+        par[early, ..., 1, :, :] = (v[early] / factor).half()
+    _check(c, _attend(c))
+
+
 @pytest.mark.parametrize("n", [32768, 131072])
 @pytest.mark.parametrize("batch,count", [(1, 1), (40, 1), (2, 70), (80, 70)])
 @pytest.mark.parametrize("dtype", [BF, FP])
