@@ -230,6 +230,7 @@ struct AttnSmem {
 // Weights, and weights times scales, stay below 2^15 in fp16; a reference that moves
 // leaves this much (log2) to the weights that follow.
 constexpr float kRoom = 15.f, kSlack = 8.f;
+constexpr float kGaveUp = -1.f;  // the cap of a lane whose wait ran out
 // A pair's first tile costs a run this many tiles more (the warps' meeting, the first
 // blocks' reference): runs are cut by cost.  64 sequences of 100 to 8,191 positions take
 // 83.9, 75.5, 78.5 us with 2, 4, 8.
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     // 0, 8-15: group 1); sums: the weights' products with the parameters (rows 0-7) and with
     // one (rows 8-15)
     float m_run[NT][2], o[NT][G][4][4], off[NT][4], sums[NT][4];
-    // no scale met so far exceeds cap; weights stay below 2^room
+    // no scale met so far exceeds cap (kGaveUp: below every scale); weights stay below 2^room
     float cap = 1.f, room = kRoom;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -590,11 +591,21 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       constexpr int N = decltype(n_tag)::value;
       constexpr bool edge = decltype(edge_tag)::value;
       const uint8_t* blk[N];
+      // A wait that runs out is one lane's finding.  The others need it up to the vote below,
+      // which its cap takes to the rare branch; what it reads until then is the ring's, and
+      // thrown away.  (A vote of its own behind each wait: 77.8 -> 79.6 us for 64 sequences;
+      // a loop of waits per block instead of one try for both first: 78.8.)
+      bool here = true;
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         const uint32_t st = (taken + u) % kStages;
-        if (!mbar_wait_warp(&bars[st], ((taken + u) / kStages) & 1u, &sh_abort, p.status)) return false;
+        here &= mbar_try_wait(&bars[st], ((taken + u) / kStages) & 1u);
         blk[u] = ring + st * kBlk;
+      }
+      if (!here) {
+#pragma unroll 1
+        for (int u = 0; u < N; ++u)
+          if (!mbar_wait(&bars[(taken + u) % kStages], ((taken + u) / kStages) & 1u, &sh_abort, p.status)) cap = kGaveUp;
       }
       const int pos0 = pos_first + j * kTile;  // of the first block; an edge is one block
 
@@ -708,6 +719,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           }
       }
       if (__any_sync(0xffffffffu, over)) {
+        if (__any_sync(0xffffffffu, cap == kGaveUp)) return false;  // the warp as one
         // the largest finite scale of the blocks; the others reach their group's elements
         // through the sums, and as zeros nothing else
         float vm = 0.f;
