@@ -71,7 +71,9 @@ class PagedKVCache:
     The host keeps the sequences' lengths and hands pages out (``reserve``); the
     device sees them as ``page_table`` and ``prefix``.  ``verify_pass`` writes the
     new tokens behind ``lengths`` without moving it: ``advance`` accepts them,
-    so that rejected drafts are overwritten by the next pass.  capacity: the most
+    so that rejected drafts are overwritten by the next pass.  Positions are accepted
+    as far as they were reserved, by a pass or, for passes that are captured and
+    replayed, by ``reserve`` beforehand.  capacity: the most
     positions of one sequence; num_pages: pages shared by all sequences (default:
     enough for every sequence at capacity); rope_theta: the layers' rotary base (a
     pass refuses layers of another one, whose rotation is not the tables')."""
@@ -91,6 +93,7 @@ class PagedKVCache:
         self.prefix = torch.zeros(batch, dtype=torch.int32, device=device)
         self.tables = rotary_tables(max_pages * page_size, head_dim, rope_theta, device)
         self.lengths = [0] * batch
+        self._reserved = [0] * batch  # positions of each sequence that advance may accept
         self._pages: List[List[int]] = [[] for _ in range(batch)]
         self._free = list(range(num_pages - 1, -1, -1))
 
@@ -118,6 +121,7 @@ class PagedKVCache:
         if sum(need) > len(self._free):
             raise RuntimeError(f"reserve: {sum(need)} pages needed, {len(self._free)} free")
         for b, n in enumerate(need):
+            self._reserved[b] = max(self._reserved[b], self.lengths[b] + int(counts[b]))
             if n:
                 fresh = [self._free.pop() for _ in range(n)]
                 at = len(self._pages[b])
@@ -125,11 +129,12 @@ class PagedKVCache:
                 self.page_table[b, at:at + n] = torch.tensor(fresh, dtype=torch.int32)
 
     def advance(self, counts: Sequence[int]) -> None:
-        """The first counts[b] positions written behind sequence b's length stay."""
+        """The first counts[b] positions written behind sequence b's length stay; raises, and
+        changes nothing, where they were not reserved."""
         if len(counts) != self.batch:
             raise ValueError(f"advance: {len(counts)} counts for {self.batch} sequences")
         for b, c in enumerate(counts):
-            if c < 0 or self.lengths[b] + c > len(self._pages[b]) * self.page_size:
+            if c < 0 or self.lengths[b] + c > self._reserved[b]:
                 raise ValueError(f"advance: sequence {b} has no {c} positions behind {self.lengths[b]}")
         self.lengths = [n + int(c) for n, c in zip(self.lengths, counts)]
         self.prefix.copy_(torch.tensor(self.lengths, dtype=torch.int32))
@@ -139,7 +144,7 @@ class PagedKVCache:
         self._free += reversed(self._pages[b])
         self._pages[b] = []
         self.page_table[b].fill_(-1)
-        self.lengths[b] = 0
+        self.lengths[b] = self._reserved[b] = 0
         self.prefix[b] = 0
 
     def read(self, layer: int, b: int) -> Tuple[torch.Tensor, torch.Tensor]:
