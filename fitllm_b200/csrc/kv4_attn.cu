@@ -24,6 +24,14 @@
 // fp32 and rounded once.  Both stay below 2^15.  Scores, maxima, denominators and outputs
 // are fp32.
 //
+// An MMA's sum rounds towards zero at the accumulator's size, and sums of codes and lows grow
+// with the positions where the output, their small difference, shrinks.  So every 32 blocks
+// (fp16 results of more than 2^15 positions: 8) a warp adds what it has, the difference taken,
+// to its part in shared memory, rounded to nearest, and starts anew.  Relative errors of 5 heads
+// over 131,072 positions, 640 sequences: bf16 1.1e-2 -> 1.7e-3, fp16 1.3e-2 -> 3.0e-4; over a
+// million, 16 sequences: 1.0e-2 -> 1.7e-3 and 1.1e-2 -> 3.8e-4.  It costs 1.4 us of 78 (64
+// sequences), in registers rather than in its own work.
+//
 // A scale that is no number only makes its own group's elements of the columns that see
 // it none: it reaches them through the parameters' products, and enters the scaled
 // weights as zero.
@@ -273,6 +281,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
   constexpr int kWarps = S::kWarps, kTile = S::kTile, kStages = S::kStages, kThreads = S::kThreads;
   // fp16 results show the weights' rounding before their scaling: there they are scaled in fp32
   constexpr bool kOnce = std::is_same<T, __half>::value;
+  constexpr int kLong = 1 << 15;  // positions from which fp16 sums are joined four times as often
   constexpr int kRowV = G == 2 ? 4 : 0;  // the values' first row among a position's quantities
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, qd = lane & 3;
@@ -561,19 +570,23 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     float m_run[NT][2], o[NT][G][4][4], off[NT][4], sums[NT][4];
     // no scale met so far exceeds cap (kGaveUp: below every scale); weights stay below 2^room
     float cap = 1.f, room = kRoom;
+    auto clear = [&] {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sums[nt][e] = off[nt][e] = 0.f;
+#pragma unroll
+          for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[nt][gr][i][e] = 0.f;
+        }
+    };
+    clear();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) m_run[nt][e] = kFloor;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sums[nt][e] = off[nt][e] = 0.f;
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[nt][gr][i][e] = 0.f;
-      }
-    }
 
     uint32_t set_valid = 0;
     auto feed = [&] {  // a place in the ring is free
@@ -876,24 +889,71 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       }
       return true;
     };
+    // ---- what the registers hold joins the warp's part in shared memory: the sums of codes less
+    // eight, back at their size, and of w (low + 8 scale)
+    auto flush = [&](bool first) {
+      __syncwarp();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int n = 8 * nt + 2 * qd + e;
+          float* ml = mrg_ml + (warp * R + n) * 2;
+          float2 was = make_float2(0.f, 0.f);
+          if (!first) {
+            was = *reinterpret_cast<const float2*>(ml);
+            was.x = exp2_approx(was.x - m_run[nt][e]);
+          }
+          float* row = mrg_o + (warp * R + n) * kLd;
+#pragma unroll
+          for (int gr = 0; gr < G; ++gr) {
+            const int from = 4 * (kRowV + 2 * gr) + qd;
+            const float c = fmaf(8.f, __shfl_sync(0xffffffffu, sums[nt][e], from),
+                                 __shfl_sync(0xffffffffu, sums[nt][e], from + 4));
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f[2 * i] = fmaf(o[nt][gr][i][e] - off[nt][2 * gr + e], 16777216.f, c);
+              f[2 * i + 1] = fmaf(fmaf(o[nt][gr][i][2 + e], 0.0625f, -off[nt][2 * gr + e]), 16777216.f, c);
+            }
+            float* dst = row + 64 * gr + 8 * g;
+            if (!first) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] = fmaf(was.x, dst[i], f[i]);
+            }
+            *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
+          }
+          __syncwarp();
+          if (g == 0) *reinterpret_cast<float2*>(ml) = make_float2(m_run[nt][e], fmaf(was.x, was.y, sums[nt][2 + e]));
+        }
+    };
     // the blocks that every column sees to their end come first
     int inner = (mask_from - pos_first - kKv4Block) / kTile + 1;
     if (mask_from - pos_first < kKv4Block) inner = 0;
     if (inner > blocks) inner = blocks;
     bool fine = true;
+    const int window = kOnce && len > kLong ? 8 : 32;
     for (int j = 0; j < blocks && fine;) {
       if ((j & 31) == 0) set_valid = valid;  // block j has been issued, its set is the current one
-      const uint32_t has = set_valid >> (j & 31);
-      if (j + 2 <= inner && (has & 3u) == 3u) {
-        fine = step(j, std::integral_constant<int, 2>{}, std::false_type{});
-        j += 2;
-        continue;
+      const int stop = min((j | (window - 1)) + 1, blocks);  // (a pair may end one behind it)
+      while (j < stop && fine) {
+        const uint32_t has = set_valid >> (j & 31);
+        if (j + 2 <= inner && (has & 3u) == 3u) {
+          fine = step(j, std::integral_constant<int, 2>{}, std::false_type{});
+          j += 2;
+          continue;
+        }
+        if (!(has & 1u))  // no page: the block is hidden from every column
+          feed();
+        else
+          fine = step(j, std::integral_constant<int, 1>{}, std::true_type{});
+        ++j;
       }
-      if (!(has & 1u))  // no page: the block is hidden from every column
-        feed();
-      else
-        fine = step(j, std::integral_constant<int, 1>{}, std::true_type{});
-      ++j;
+      if (!kClustered && j < blocks) {
+        flush(stop == window);
+        clear();
+      }
     }
 
     // ---- the rest of the next segment's first copies
@@ -905,30 +965,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
     }
 
     // ---- the warps' results meet in shared memory
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int n = 8 * nt + 2 * qd + e;
-        float* row = mrg_o + (warp * R + n) * kLd;
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          // sum of w (low + 8 scale), and the codes less eight back at their size
-          const int from = 4 * (kRowV + 2 * gr) + qd;
-          const float c = fmaf(8.f, __shfl_sync(0xffffffffu, sums[nt][e], from),
-                               __shfl_sync(0xffffffffu, sums[nt][e], from + 4));
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f[2 * i] = fmaf(o[nt][gr][i][e] - off[nt][2 * gr + e], 16777216.f, c);
-            f[2 * i + 1] = fmaf(fmaf(o[nt][gr][i][2 + e], 0.0625f, -off[nt][2 * gr + e]), 16777216.f, c);
-          }
-          float* dst = row + 64 * gr + 8 * g;
-          *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
-          *reinterpret_cast<float4*>(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
-        }
-        if (g == 0) *reinterpret_cast<float2*>(mrg_ml + (warp * R + n) * 2) = make_float2(m_run[nt][e], sums[nt][2 + e]);
-      }
+    flush(blocks <= window);
     __syncthreads();
     if (!kClustered && sn.tb > 0) load_queries(g_kv4_smem + L::kQ + buf * L::kQBytes);
     const SeqSpan sp = sg.sp;

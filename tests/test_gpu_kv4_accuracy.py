@@ -181,3 +181,58 @@ def test_what_stands_behind_a_strong_first_position(cuda_dev, n, batch, count, d
     _check(few, o)
     # the sequences differ in their queries' small part only
     assert float((o.double().mean(-1) / o.double().mean() - 1).abs().max()) < 0.2
+
+
+# ---- long sums, over all heads together: the outputs' own rounding and one of the weights.
+# A rounding to nearest is off by u / m of a value with mantissa m in [1, 2) at most, evenly: its variance
+# is u^2 / 3 E[1 / m^2] of the value's square, 3 / (8 ln 2) u^2 / 3 = 0.18 u^2 where mantissas spread as
+# logarithms do.  The results' own is taken from the results.  Sums in the tensor cores round towards zero at
+# the accumulator's size, at most 2^-23 of it each:
+# * up to 64 rows: of 16 positions each and at most 32 blocks of codes less eight (fp16 results of more than
+#   2^15 positions: 8) before they are joined in fp32, that is 2^-23 * 32 * 8 s w_p per position on average over
+#   the blocks; the halves that cancel (codes against eights, scales against lows) bring 2 of that;
+# * more rows: 2^14 / 16 (bf16: 2^16 / 16) of them before parts are joined, of the output itself.
+# A quarter more for the statistics of a few hundred values.
+
+def _long(dev, n, d, dtype, h, new, batch, mean):
+    g = torch.Generator(device=dev).manual_seed(n + d + batch)
+    pool = ref.random_pool(n // 128, 1, 128, d, g, dev)
+    _params(pool, d)[..., 1, :, 1] += mean
+    q = torch.randn(new, h, d, generator=g, device=dev).to(dtype)
+    table = torch.randperm(n // 128, generator=g, device=dev).int().expand(batch, -1).contiguous()
+    return dict(q=q.repeat(batch, 1, 1), pool=pool, table=table, q_start=None, max_new=new, max_len=n,
+                pre=torch.full((batch,), n - new, dtype=torch.int32, device=dev))
+
+
+def _long_bound(c, o, n, new, few):
+    """(error, bound) of the last sequence's first eight tokens, norms over all of their heads."""
+    h, d = c["q"].shape[1:]
+    dtype = c["q"].dtype
+    k, v = (x[0] for x in ref.read_sequence(c["pool"], c["table"][-1], n))
+    s = _scales(c["pool"], c["table"][-1], n)[0]
+    rows = c["table"][-1].long()
+    low = _params(c["pool"], d)[rows][..., 1, :, 1].double().permute(1, 0, 2, 3, 4).reshape(n, -1).repeat_interleave(64, -1)
+    mid = low + 8 * s
+    terms = ((v - mid).square() + mid.square()).sum(-1) if few else (v.square() if dtype == FP else 3 * v.square()).sum(-1)
+    err2 = want2 = out2 = weights2 = sums2 = 0.0
+    for i in range(min(new, 8)):
+        seen = n - new + i + 1
+        p = torch.softmax(c["q"][i].double() @ k[:seen].T / math.sqrt(d), -1)
+        want = p @ v[:seen]
+        err2 += float((o[i - new].double() - want).square().sum())
+        want2 += float(want.square().sum())
+        out2 += float((want.to(dtype).double() - want).square().sum())
+        weights2 += float((p.square() @ terms[:seen]).sum()) * 0.18 * R ** 2
+        window = 8 if dtype == FP and n > 1 << 15 else 32
+        sums = 2 * window * 8 * (p @ s[:seen]) if few else want * ((1 << 14 if dtype == FP else 1 << 16) / 16)
+        sums2 += float(sums.square().sum()) * 2.0 ** -46
+    return math.sqrt(err2), 1.25 * math.sqrt(out2 + weights2) + math.sqrt(sums2), math.sqrt(want2)
+
+
+@pytest.mark.parametrize("n,batch,new", [(65536, 1, 1), (131072, 64, 3), (131072, 640, 1), (1 << 20, 1, 4), (1 << 20, 16, 3)])
+@pytest.mark.parametrize("d,dtype", [(128, BF), (128, FP), (64, BF), (64, FP)])
+def test_few_rows_keep_their_digits_over_long_contexts(cuda_dev, n, batch, new, d, dtype):
+    c = _long(cuda_dev, n, d, dtype, 5, new, batch, 0.0)
+    err, bound, norm = _long_bound(c, _attend(c), n, new, True)
+    assert err <= bound, f"{err / norm:.2e} of the output, the bound {bound / norm:.2e}"
+    assert bound < norm / 20
