@@ -20,7 +20,11 @@
 // the scores' scale and the final 1 / l.  It is the codes that are halved, which is
 // exact: a halved scale would lose a bit below 2^-13, fifteen times over in a value.  What
 // remains there is the rounding of the halved low and of the sum: 2^-23 of a value at most.
-// Queries are scaled per row by a power of two as in kv4_attn.cu.
+// fp16 results would show it, once of the keys and once of the values (relative error
+// 4.2e-4 where the result's rounding and the weights' alone give 2.9e-4): there a value is
+// the sum of two fp16 numbers, computed in fp32, tiles are 64 positions of two rows (columns
+// of V^T) each, half of the decoders decode keys and half values, and both products take twice
+// the MMAs: 176 -> 272 us for the two sequences below.  Queries are scaled per row by a power of two as in kv4_attn.cu.
 //
 // The reference m of a row moves only when a weight would exceed 2^15 (fp16's range for
 // P), and then to 2^7 below the row's largest, so that eight more bits of growth move
@@ -43,6 +47,8 @@
 // that two row tiles per SM cover in part.  Two sequences of up to 2,048 tokens (40 heads
 // on 8) behind up to 513: 173 us, 0.57 PFLOP/s.  Half the exponentials as a polynomial
 // on the FMA pipe made it 183 us, sixteen softmax warps (two threads a row) 200 us.
+#include <type_traits>
+
 #include "kv4.cuh"
 #include "kernels.cuh"
 
@@ -50,10 +56,9 @@ namespace fitq {
 namespace {
 
 constexpr int kPRows = 128;       // rows of a row tile (TMEM lanes)
-constexpr int kPTile = 128;       // positions of a decoded tile
+constexpr int kPTile = 128;       // rows of a decoded tile
 constexpr int kPStep = 64;        // positions of a step
 constexpr int kPThreads = 640;     // five warpgroups
-constexpr int kPDecoders = 256;
 // Registers per thread: 96 at launch (61,440 in all), then softmax 128, decoders 80,
 // issuer 64: 2 x 128 + 2 x 80 + 64 = 480 per lane of a warpgroup.
 constexpr int kPRegsSoftmax = 128, kPRegsDecode = 80, kPRegsIssue = 64;
@@ -190,12 +195,31 @@ __device__ __forceinline__ void sts32(uint32_t addr, uint32_t a) {
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 
+// v / 2 = hi + lo, both fp16, of two values: from their codes' halves, scales and halved lows.
+struct Pair2 {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Pair2 value_pair(uint32_t codes, float s0, float s1, float l0, float l1) {
+  const float2 c = Half16<__half>::unpack(codes);
+  const float a = fmaf(c.x, s0, l0), b = fmaf(c.y, s1, l1);
+  Pair2 r;
+  r.hi = pack_half2(a, b);
+  const float2 h = Half16<__half>::unpack(r.hi);
+  r.lo = pack_half2(a - h.x, b - h.y);
+  return r;
+}
+
 extern __shared__ uint8_t g_prompt_smem[];
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4PromptParams p) {
   using L = PromptSmem<D>;
   constexpr int G = D / 64;
+  // two fp16 numbers a value, hi in the tile's first half and lo in its second
+  constexpr bool kTwo = std::is_same<T, __half>::value;
+  constexpr int kTile = kTwo ? kPTile / 2 : kPTile;  // positions of a decoded tile
+  constexpr int kSteps = kTile / kPStep;             // steps of one
+  constexpr int kBlocks = kTile / kKv4Block;         // blocks of one, a warp each
   __shared__ uint64_t b_qready, b_kfull[2], b_kfree[2], b_vfull[2], b_vfree[2], b_sfull[2][2], b_pready[2][2], b_odone[2][2], b_done;
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_abort;
@@ -230,19 +254,19 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   if (len64 > room) len64 = room;
   // This CTA's part: `tiles` tiles from position at0 on.  Positions below are relative to at0.
   const int len_all = static_cast<int>(len64);
-  const int tiles_all = (len_all + kPTile - 1) / kPTile;
+  const int tiles_all = (len_all + kTile - 1) / kTile;
   const int share = (tiles_all + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y);
   const int tile0 = min(static_cast<int>(blockIdx.y) * share, tiles_all);
   const int tiles = min(share, tiles_all - tile0);
-  const int at0 = tile0 * kPTile;
-  const int len = min(len_all - at0, tiles * kPTile);
+  const int at0 = tile0 * kTile;
+  const int len = min(len_all - at0, tiles * kTile);
 
   if (tid == 0) {
     sh_abort = 0;
     mbar_init(&b_qready, 8);  // one arrival per warp
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&b_kfull[i], kPDecoders / 32);
-      mbar_init(&b_vfull[i], kPDecoders / 32);
+      mbar_init(&b_kfull[i], kBlocks);
+      mbar_init(&b_vfull[i], kBlocks);
       mbar_init(&b_kfree[i], 1);
       mbar_init(&b_vfree[i], 1);
       for (int h = 0; h < 2; ++h) {
@@ -327,26 +351,26 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     const uint64_t cn2 = pack2(cn, cn);
     const int steps = (len + kPStep - 1) / kPStep;
     for (int t = 0; ok && t < steps; ++t) {
-      const int j = t >> 1, h = t & 1, buf = j & 1;
+      const int j = t / kSteps, sub = t % kSteps, buf = j & 1, h = t & 1;
       const int pos0 = t * kPStep;
       // the tile's notes are there once V is decoded
-      if (h == 0) {
+      if (sub == 0) {
         ok = wait_all(&b_vfull[buf], (j >> 1) & 1);
         if (!ok) break;
       }
-      ok = wait_all(&b_sfull[r][h], j & 1);
+      ok = wait_all(&b_sfull[r][h], (t >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
       uint32_t v[2][32];
       tmem_ld_32x32b_x32(t_s + h * kPStep, v[0]);
       tmem_ld_32x32b_x32(t_s + h * kPStep + 32, v[1]);
       uint32_t pages = 0xfu;  // which of the step's blocks are there
-      const uint4 nt = *reinterpret_cast<const uint4*>(&sh_note[buf][4 * h]);
+      const uint4 nt = *reinterpret_cast<const uint4*>(&sh_note[buf][4 * sub]);
       constexpr uint32_t kClean = 1u | (kKv4Block << 8) | (kKv4Block << 16);
       if (((nt.x ^ kClean) | (nt.y ^ kClean) | (nt.z ^ kClean) | (nt.w ^ kClean)) != 0) {
         pages = 0;
         for (int i = 0; i < 4; ++i) {
-          const uint32_t note = sh_note[buf][4 * h + i];
+          const uint32_t note = sh_note[buf][4 * sub + i];
           pages |= (note & 1u) << i;
           for (int gr = 0; gr < G; ++gr) {
             const int at = static_cast<int>((note >> (8 + 8 * gr)) & 0xffu);
@@ -456,149 +480,178 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   } else if (warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsDecode));
     // ------------------------------------------------------------ decoders
-    // Warp dw decodes block dw of every tile.  Keys: lane (r, c) = (lane / 4, lane % 4) takes
-    // positions r and r + 8, unit c of each group; values: lane (e, q) takes positions
-    // 2 q, 2 q + 1 of each half, elements 8 e .. 8 e + 7 of each group.  Either way a warp
-    // reads 512 consecutive bytes at a time.  V^T's row of element 8 e + i of a group is
+    // Warp dw decodes block dw of every tile (kTwo: its keys or its values).  Keys: lane
+    // (r, c) = (lane / 4, lane % 4) takes positions r and r + 8, unit c of each group; values:
+    // lane (e, q) takes positions 2 q, 2 q + 1 of each half, elements 8 e .. 8 e + 7 of each
+    // group.  Either way a warp reads 512 consecutive bytes at a time.  V^T's row of element 8 e + i of a group is
     // 8 i + e, so that the lanes of a store lie in eight rows of different swizzle.
-    const int dw = warp - 8;
+    const int dw = (warp - 8) % kBlocks;
     const int hi = lane >> 2, lo2 = lane & 3;
-    uint32_t kw[2][2 * G], kpar[2][G], vw[2][2][G], vpar[2][2][G];
-    // The page table's entry for this warp's block of tile j, and, one tile later (a use at
-    // once would wait for the load), the block; null: no page.
-    auto entry = [&](int j) -> int {
-      const int pos = j * kPTile + dw * kKv4Block;
-      return j < tiles && pos < len
-                 ? s.page_table[static_cast<int64_t>(b) * s.max_pages + ((at0 + pos) >> s.page_shift)]
-                 : -2;
-    };
-    auto block = [&](int j, int pg) -> const uint8_t* {
-      const int64_t pos = static_cast<int64_t>(at0) + j * kPTile + dw * kKv4Block;
-      const bool there = pg >= 0 && pg < s.num_pages;
-      if (!there && pg != -2 && lane == 0) report_device_error(p.status, FITQ_ERR_ARG);
-      return there ? p.pool + kv4_block_offset(s, pg, kvh, pos, D) : nullptr;
-    };
-    // A block without a page reads the pool's first one with scale and low 0.
-    auto load_k = [&](const uint8_t* blk) {
-      if (blk == nullptr) blk = p.pool;
+    auto decode = [&](auto keys_tag, auto values_tag) {
+      constexpr bool does_k = decltype(keys_tag)::value, does_v = decltype(values_tag)::value;
+      uint32_t kw[2][2 * G], kpar[2][G], vw[2][2][G], vpar[2][2][G];
+      // The page table's entry for this warp's block of tile j, and, one tile later (a use at
+      // once would wait for the load), the block; null: no page.
+      auto entry = [&](int j) -> int {
+        const int pos = j * kTile + dw * kKv4Block;
+        return j < tiles && pos < len
+                   ? s.page_table[static_cast<int64_t>(b) * s.max_pages + ((at0 + pos) >> s.page_shift)]
+                   : -2;
+      };
+      auto block = [&](int j, int pg) -> const uint8_t* {
+        const int64_t pos = static_cast<int64_t>(at0) + j * kTile + dw * kKv4Block;
+        const bool there = pg >= 0 && pg < s.num_pages;
+        if (!there && pg != -2 && lane == 0) report_device_error(p.status, FITQ_ERR_ARG);
+        return there ? p.pool + kv4_block_offset(s, pg, kvh, pos, D) : nullptr;
+      };
+      // A block without a page reads the pool's first one with scale and low 0.
+      auto load_k = [&](const uint8_t* blk) {
+        if (blk == nullptr) blk = p.pool;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (G == 2) {
-          *reinterpret_cast<uint4*>(kw[i]) = *reinterpret_cast<const uint4*>(blk + i * 512 + lane * 16);
-          *reinterpret_cast<uint2*>(kpar[i]) = *reinterpret_cast<const uint2*>(blk + 16 * D + (8 * i + hi) * 16);
-        } else {
-          *reinterpret_cast<uint2*>(kw[i]) = *reinterpret_cast<const uint2*>(blk + i * 256 + lane * 8);
-          kpar[i][0] = *reinterpret_cast<const uint32_t*>(blk + 16 * D + (8 * i + hi) * 8);
-        }
-      }
-    };
-    auto load_v = [&](const uint8_t* blk) {
-      if (blk == nullptr) blk = p.pool;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (G == 2)
-          *reinterpret_cast<uint4*>(vw[h]) = *reinterpret_cast<const uint4*>(blk + 8 * D + h * 512 + lane * 16);
-        else
-          *reinterpret_cast<uint2*>(vw[h]) = *reinterpret_cast<const uint2*>(blk + 8 * D + h * 256 + lane * 8);
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          const uint8_t* ps = blk + 16 * D + (8 * h + 2 * lo2 + o) * 8 * G + 4 * G;
-          if (G == 2)
-            *reinterpret_cast<uint2*>(vpar[h][o]) = *reinterpret_cast<const uint2*>(ps);
-          else
-            vpar[h][o][0] = *reinterpret_cast<const uint32_t*>(ps);
-        }
-      }
-    };
-    bool ok = tiles > 0;
-    int pg_next = entry(1);
-    const uint8_t* blk = block(0, entry(0));
-    if (ok) {
-      load_k(blk);
-      load_v(blk);
-    }
-    for (int j = 0; ok && j < tiles; ++j) {
-      const int buf = j & 1;
-      const uint32_t ph = (j >> 1) & 1;
-      const bool there = blk != nullptr;
-      blk = block(j + 1, pg_next);
-      pg_next = entry(j + 2);
-      // ---- keys
-      if (j >= 2) ok = wait_all(&b_kfree[buf], ph ^ 1u);
-      if (!ok) break;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int pos = dw * kKv4Block + 8 * i + hi;  // its swizzle is hi
-        const uint32_t dst = s_k + buf * L::kK + pos * 128;
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          const uint32_t par = there ? kpar[i][gr] : 0u, half = half_of(par);
-          const uint32_t sc = __byte_perm(par, par, 0x1010), lo = __byte_perm(half, half, 0x3232);
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t x = kw[i][2 * gr + w], y = x >> 8;
-            // the eight elements in the order 0 4 1 5 2 6 3 7, as the queries'
-            sts128(dst + gr * (kPTile * 128) + (((2 * lo2 + w) ^ hi) << 4), hfma2_u(halved_even(x), sc, lo),
-                   hfma2_u(halved_odd(x), sc, lo), hfma2_u(halved_even(y), sc, lo), hfma2_u(halved_odd(y), sc, lo));
+        for (int i = 0; i < 2; ++i) {
+          if (G == 2) {
+            *reinterpret_cast<uint4*>(kw[i]) = *reinterpret_cast<const uint4*>(blk + i * 512 + lane * 16);
+            *reinterpret_cast<uint2*>(kpar[i]) = *reinterpret_cast<const uint2*>(blk + 16 * D + (8 * i + hi) * 16);
+          } else {
+            *reinterpret_cast<uint2*>(kw[i]) = *reinterpret_cast<const uint2*>(blk + i * 256 + lane * 8);
+            kpar[i][0] = *reinterpret_cast<const uint32_t*>(blk + 16 * D + (8 * i + hi) * 8);
           }
         }
-      }
-      fence_async_proxy();
-      arrive_warp(&b_kfull[buf]);
-      if (j + 1 < tiles) load_k(blk);
-      // ---- values
-      if (j >= 2) ok = wait_all(&b_vfree[buf], ph ^ 1u);
-      if (!ok) break;
-      int bad[G];  // the block's first position that is not finite, 16: none
+      };
+      auto load_v = [&](const uint8_t* blk) {
+        if (blk == nullptr) blk = p.pool;
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) bad[gr] = kKv4Block;
+        for (int h = 0; h < 2; ++h) {
+          if (G == 2)
+            *reinterpret_cast<uint4*>(vw[h]) = *reinterpret_cast<const uint4*>(blk + 8 * D + h * 512 + lane * 16);
+          else
+            *reinterpret_cast<uint2*>(vw[h]) = *reinterpret_cast<const uint2*>(blk + 8 * D + h * 256 + lane * 8);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int vpos = j * kPTile + dw * kKv4Block + 8 * h + 2 * lo2;
+          for (int o = 0; o < 2; ++o) {
+            const uint8_t* ps = blk + 16 * D + (8 * h + 2 * lo2 + o) * 8 * G + 4 * G;
+            if (G == 2)
+              *reinterpret_cast<uint2*>(vpar[h][o]) = *reinterpret_cast<const uint2*>(ps);
+            else
+              vpar[h][o][0] = *reinterpret_cast<const uint32_t*>(ps);
+          }
+        }
+      };
+      bool ok = tiles > 0;
+      int pg_next = entry(1);
+      const uint8_t* blk = block(0, entry(0));
+      if (ok && does_k) load_k(blk);
+      if (ok && does_v) load_v(blk);
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int buf = j & 1;
+        const uint32_t ph = (j >> 1) & 1;
+        const bool there = blk != nullptr;
+        blk = block(j + 1, pg_next);
+        pg_next = entry(j + 2);
+        if (does_k) {
+          // ---- keys
+          if (j >= 2) ok = wait_all(&b_kfree[buf], ph ^ 1u);
+          if (!ok) break;
 #pragma unroll
-        for (int o = 0; o < 2; ++o)
+          for (int i = 0; i < 2; ++i) {
+            const int pos = dw * kKv4Block + 8 * i + hi;  // its swizzle is hi
+            const uint32_t dst = s_k + buf * L::kK + pos * 128;
 #pragma unroll
-          for (int gr = 0; gr < G; ++gr) {
-            // an exponent of all ones in either half: not finite
-            const uint32_t e = vpar[h][o][gr] & 0x7c007c00u;
-            if (vpos + o >= len || !there) {
-              vpar[h][o][gr] = 0;
-            } else if ((e & 0xffffu) == 0x7c00u || (e >> 16) == 0x7c00u) {
-              vpar[h][o][gr] = 0;
-              bad[gr] = min(bad[gr], 8 * h + 2 * lo2 + o);
+            for (int gr = 0; gr < G; ++gr) {
+              const uint32_t par = there ? kpar[i][gr] : 0u, half = half_of(par);
+              const uint32_t sc = __byte_perm(par, par, 0x1010), lo = __byte_perm(half, half, 0x3232);
+              const float2 sl = Half16<__half>::unpack(par);
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                const uint32_t x = kw[i][2 * gr + w], y = x >> 8;
+                // the eight elements in the order 0 4 1 5 2 6 3 7, as the queries'
+                const uint32_t c[4] = {halved_even(x), halved_odd(x), halved_even(y), halved_odd(y)};
+                const uint32_t at = dst + gr * (kPTile * 128) + (((2 * lo2 + w) ^ hi) << 4);
+                if (kTwo) {
+                  Pair2 v[4];
+#pragma unroll
+                  for (int u = 0; u < 4; ++u) v[u] = value_pair(c[u], sl.x, sl.x, 0.5f * sl.y, 0.5f * sl.y);
+                  sts128(at, v[0].hi, v[1].hi, v[2].hi, v[3].hi);
+                  sts128(at + kTile * 128, v[0].lo, v[1].lo, v[2].lo, v[3].lo);
+                } else {
+                  sts128(at, hfma2_u(c[0], sc, lo), hfma2_u(c[1], sc, lo), hfma2_u(c[2], sc, lo), hfma2_u(c[3], sc, lo));
+                }
+              }
             }
           }
-      }
-      uint32_t note = there ? 1u : 0u;
+          fence_async_proxy();
+          arrive_warp(&b_kfull[buf]);
+          if (j + 1 < tiles) load_k(blk);
+        }
+        if (!does_v) continue;
+        // ---- values
+        if (j >= 2) ok = wait_all(&b_vfree[buf], ph ^ 1u);
+        if (!ok) break;
+        int bad[G];  // the block's first position that is not finite, 16: none
 #pragma unroll
-      for (int gr = 0; gr < G; ++gr) note |= __reduce_min_sync(0xffffffffu, static_cast<unsigned>(bad[gr])) << (8 + 8 * gr);
-      if (G == 1) note |= kKv4Block << 16;
-      if (lane == 0) sh_note[buf][dw] = note;
+        for (int gr = 0; gr < G; ++gr) bad[gr] = kKv4Block;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int h16 = 2 * dw + h;
+        for (int h = 0; h < 2; ++h) {
+          const int vpos = j * kTile + dw * kKv4Block + 8 * h + 2 * lo2;
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-          const uint32_t sc = __byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x5410);
-          const uint32_t lo = half_of(__byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x7632));
-          // row 64 gr + 8 i + e, positions 8 h16 + 2 q, + 1
-          const uint32_t dst =
-              s_v + buf * L::kV + (h16 >> 3) * (D * 128) + (64 * gr + hi) * 128 + (((h16 & 7) ^ hi) << 4) + lo2 * 4;
+          for (int o = 0; o < 2; ++o)
 #pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            const uint32_t x = __byte_perm(vw[h][0][gr], vw[h][1][gr], z ? 0x7632 : 0x5410);
-            const uint32_t y = x >> 8;
-            sts32(dst + (4 * z) * 1024, hfma2_u(halved_even(x), sc, lo));
-            sts32(dst + (4 * z + 1) * 1024, hfma2_u(halved_odd(x), sc, lo));
-            sts32(dst + (4 * z + 2) * 1024, hfma2_u(halved_even(y), sc, lo));
-            sts32(dst + (4 * z + 3) * 1024, hfma2_u(halved_odd(y), sc, lo));
+            for (int gr = 0; gr < G; ++gr) {
+              // an exponent of all ones in either half: not finite
+              const uint32_t e = vpar[h][o][gr] & 0x7c007c00u;
+              if (vpos + o >= len || !there) {
+                vpar[h][o][gr] = 0;
+              } else if ((e & 0xffffu) == 0x7c00u || (e >> 16) == 0x7c00u) {
+                vpar[h][o][gr] = 0;
+                bad[gr] = min(bad[gr], 8 * h + 2 * lo2 + o);
+              }
+            }
+        }
+        uint32_t note = there ? 1u : 0u;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) note |= __reduce_min_sync(0xffffffffu, static_cast<unsigned>(bad[gr])) << (8 + 8 * gr);
+        if (G == 1) note |= kKv4Block << 16;
+        if (lane == 0) sh_note[buf][dw] = note;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int h16 = 2 * dw + h;
+#pragma unroll
+          for (int gr = 0; gr < G; ++gr) {
+            const uint32_t sc = __byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x5410);
+            const uint32_t lo = half_of(__byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x7632));
+            const float2 s2 = Half16<__half>::unpack(sc);
+            const float2 l2 = Half16<__half>::unpack(__byte_perm(vpar[h][0][gr], vpar[h][1][gr], 0x7632));
+            // row 64 gr + 8 i + e, positions 8 h16 + 2 q, + 1
+            const uint32_t dst =
+                s_v + buf * L::kV + (h16 >> 3) * (D * 128) + (64 * gr + hi) * 128 + (((h16 & 7) ^ hi) << 4) + lo2 * 4;
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t x = __byte_perm(vw[h][0][gr], vw[h][1][gr], z ? 0x7632 : 0x5410);
+              const uint32_t y = x >> 8;
+              const uint32_t c[4] = {halved_even(x), halved_odd(x), halved_even(y), halved_odd(y)};
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                if (kTwo) {
+                  const Pair2 v = value_pair(c[u], s2.x, s2.y, 0.5f * l2.x, 0.5f * l2.y);
+                  sts32(dst + (4 * z + u) * 1024, v.hi);
+                  sts32(dst + D * 128 + (4 * z + u) * 1024, v.lo);
+                } else {
+                  sts32(dst + (4 * z + u) * 1024, hfma2_u(c[u], sc, lo));
+                }
+              }
+            }
           }
         }
+        fence_async_proxy();
+        arrive_warp(&b_vfull[buf]);
+        if (j + 1 < tiles) load_v(blk);
       }
-      fence_async_proxy();
-      arrive_warp(&b_vfull[buf]);
-      if (j + 1 < tiles) load_v(blk);
-    }
+    };
+    if constexpr (!kTwo)
+      decode(std::true_type{}, std::true_type{});
+    else if (warp - 8 < kBlocks)
+      decode(std::true_type{}, std::false_type{});
+    else
+      decode(std::false_type{}, std::true_type{});
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPRegsIssue));
     if (warp == 16 && tiles > 0) {
@@ -607,46 +660,58 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     const uint64_t dq = umma_smem_desc_sw128(s_q), dk = umma_smem_desc_sw128(s_k), dv = umma_smem_desc_sw128(s_v);
     const int steps = (len + kPStep - 1) / kPStep, last = two ? 1 : 0;
     auto issue_s = [&](int r, int t) {  // scores of step t into its half of S_r
-      const int h = t & 1, buf = (t >> 1) & 1;
+      const int h = t & 1, sub = t % kSteps, buf = (t / kSteps) & 1;
+#pragma unroll 1
+      for (int part = 0; part < (kTwo ? 2 : 1); ++part)
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint64_t qa = dq + ((r * L::kQ + (kk >> 2) * (kPRows * 128) + (kk & 3) * 32) >> 4);
-        const uint64_t kb = dk + ((buf * L::kK + (kk >> 2) * (kPTile * 128) + h * (kPStep * 128) + (kk & 3) * 32) >> 4);
-        umma_f16_ss(tmem + r * 128 + h * kPStep, qa, kb, idesc_s, kk > 0 ? 1u : 0u);
-      }
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t qa = dq + ((r * L::kQ + (kk >> 2) * (kPRows * 128) + (kk & 3) * 32) >> 4);
+          const uint64_t kb =
+              dk + ((buf * L::kK + (kk >> 2) * (kPTile * 128) + (sub + part) * (kPStep * 128) + (kk & 3) * 32) >> 4);
+          umma_f16_ss(tmem + r * 128 + h * kPStep, qa, kb, idesc_s, kk > 0 || part > 0 ? 1u : 0u);
+        }
       commit_warp(&b_sfull[r][h]);
       // the tile's last scores: its keys' buffer is free
-      if (r == last && (h == 1 || t == steps - 1)) commit_warp(&b_kfree[buf]);
+      if (r == last && (sub == kSteps - 1 || t == steps - 1)) commit_warp(&b_kfree[buf]);
     };
     auto issue_o = [&](int r, int t) {  // step t's weights times its values
-      const int h = t & 1, buf = (t >> 1) & 1;
+      const int h = t & 1, sub = t % kSteps, buf = (t / kSteps) & 1;
+#pragma unroll 1
+      for (int part = 0; part < (kTwo ? 2 : 1); ++part)
 #pragma unroll
-      for (int kk = 0; kk < kPStep / 16; ++kk) {
-        const uint64_t vb = dv + ((buf * L::kV + h * (D * 128) + kk * 32) >> 4);
-        umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + h * kPStep + kk * 8, vb, idesc_o, t > 0 || kk > 0 ? 1u : 0u);
-      }
+        for (int kk = 0; kk < kPStep / 16; ++kk) {
+          const uint64_t vb = dv + ((buf * L::kV + (sub + part) * (D * 128) + kk * 32) >> 4);
+          umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + h * kPStep + kk * 8, vb, idesc_o,
+                      t > 0 || kk > 0 || part > 0 ? 1u : 0u);
+        }
       commit_warp(&b_odone[r][h]);
-      if (r == last && (h == 1 || t == steps - 1)) commit_warp(&b_vfree[buf]);
+      if (r == last && (sub == kSteps - 1 || t == steps - 1)) commit_warp(&b_vfree[buf]);
     };
-    bool ok = wait_all(&b_qready, 0) && wait_all(&b_kfull[0], 0);
-    if (ok) {
+    // keys of the tile that step t opens
+    auto keys_here = [&](int t) -> bool {
+      return t >= steps || t % kSteps != 0 || wait_all(&b_kfull[(t / kSteps) & 1], (t / kSteps >> 1) & 1);
+    };
+    bool ok = wait_all(&b_qready, 0);
+    for (int t = 0; ok && t < 2 && t < steps; ++t) {
+      ok = keys_here(t);
+      if (!ok) break;
       tc_fence_after();
-      for (int t = 0; t < 2 && t < steps; ++t)
-        for (int r = 0; r <= last; ++r) issue_s(r, t);
+      for (int r = 0; r <= last; ++r) issue_s(r, t);
     }
     for (int t = 0; ok && t < steps; ++t) {
-      const int j = t >> 1, h = t & 1;
-      const bool more = t + 2 < steps;
-      if (h == 0) {
-        ok = wait_all(&b_vfull[j & 1], (j >> 1) & 1) &&
-             (!more || wait_all(&b_kfull[(j + 1) & 1], ((j + 1) >> 1) & 1));
-      }
+      const int h = t & 1;
+      if (t % kSteps == 0)
+        ok = wait_all(&b_vfull[(t / kSteps) & 1], (t / kSteps >> 1) & 1) && (kTwo || keys_here(t + 2));
       for (int r = 0; ok && r <= last; ++r) {
-        ok = wait_all(&b_pready[r][h], j & 1);
+        ok = wait_all(&b_pready[r][h], (t >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
         issue_o(r, t);
-        if (more) issue_s(r, t + 2);
+        if (kTwo && r == 0) {
+          ok = keys_here(t + 2);
+          tc_fence_after();
+        }
+        if (ok && t + 2 < steps) issue_s(r, t + 2);
       }
     }
     // every MMA has retired before tensor memory is given back

@@ -236,3 +236,25 @@ def test_few_rows_keep_their_digits_over_long_contexts(cuda_dev, n, batch, new, 
     err, bound, norm = _long_bound(c, _attend(c), n, new, True)
     assert err <= bound, f"{err / norm:.2e} of the output, the bound {bound / norm:.2e}"
     assert bound < norm / 20
+
+
+@pytest.mark.parametrize("prefix,counts,h,kvh", [([0, 700], [333, 200], 8, 4), ([3000], [130], 2, 1), ([300] * 80, [70] * 80, 1, 1)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_fp16_rows_of_prompts_show_their_weights_rounding_only(cuda_dev, prefix, counts, h, kvh, d):
+    """Keys and values lose nothing: the result's own rounding and one of the weights are all there is (with
+    keys and values rounded to fp16 as well the error is 1.4 times that)."""
+    c = _case(prefix, counts, h, kvh, d, 64, FP, cuda_dev, seed=d)
+    o = _attend(c)
+    err2 = expect2 = 0.0
+    for b, (pre, a, n) in enumerate(zip(prefix, c["starts"], counts)):
+        k, v = ref.read_sequence(c["pool"], c["table"][b], pre + n)
+        hidden = torch.arange(pre + n, device=cuda_dev)[None] > torch.arange(pre, pre + n, device=cuda_dev)[:, None]
+        for i in range(h):
+            kv = i // (h // kvh)
+            s = c["q"][a:a + n, i].double() @ k[kv].T / math.sqrt(d)
+            p = torch.softmax(s.masked_fill(hidden, float("-inf")), -1)
+            want = p @ v[kv]
+            err2 += float((o[a:a + n, i].double() - want).square().sum())
+            expect2 += float((want.half().double() - want).square().sum())
+            expect2 += float((p.square() @ v[kv].square().sum(-1)).sum()) * 0.18 * R ** 2
+    assert err2 <= 1.15 ** 2 * expect2, f"{math.sqrt(err2 / expect2):.2f} of what two roundings give"
