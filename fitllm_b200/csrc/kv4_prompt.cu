@@ -39,7 +39,9 @@
 //
 // Where the pairs' row tiles are fewer than the SMs, a pair's positions are cut into up
 // to kPMaxSplits parts of equal tiles, a CTA each; they leave (O, m, l) per row in the
-// workspace and kv4_prompt_combine_kernel joins them in order (deterministic).
+// workspace and kv4_prompt_combine_kernel joins them in order (deterministic).  So are
+// positions beyond most_positions, for the sums' sake; where the parts of all rows would
+// take more than kPScratch, the call goes in several launches.
 //
 // Bound: the exponentials (16 per cycle and SM: 2,048 cycles per 256 x 128 tile) and
 // the MMAs (4 x 128^3: 2,048 cycles) alike; measured, the chain of a step (wait, read S,
@@ -66,7 +68,13 @@ static_assert(2 * kPRegsSoftmax + 2 * kPRegsDecode + kPRegsIssue <= 5 * 96, "mor
 constexpr float kPFloor = -3.0e38f;
 constexpr float kPRoom = 15.f;    // weights stay below 2^15
 constexpr float kPSlack = 8.f;    // a reference that moves leaves this much (log2) to the weights that follow
-constexpr int kPMaxSplits = 32;   // a lane of the combining warp each
+constexpr int kPMaxSplits = 32;   // parts that fill the card, at most
+// The most positions of a part.  An accumulation in tensor memory rounds towards zero at the
+// accumulator's size, some 2^-24 of it each time, which adds up to 5e-4 of the output over
+// 131,072 positions and 5e-3 over a million; parts are joined in fp32.
+template <typename T>
+__host__ __device__ constexpr int most_positions() { return std::is_same<T, __half>::value ? 1 << 14 : 1 << 16; }
+constexpr int64_t kPScratch = 256ll << 20;  // bytes of parts that a launch leaves, about, at most
 
 template <int D>
 struct PromptSmem {
@@ -83,10 +91,12 @@ struct Kv4PromptParams {
   int64_t q_stride;
   void* out;
   const uint8_t* pool;
-  float* ml_part;  // [CTAs without splits][splits][256 rows][2], splits > 1 only
+  float* ml_part;  // [CTAs of the launch without splits][splits][256 rows][2], splits > 1 only
   float* o_part;   // [..][D]
   int heads, group, row_pairs;
   int max_new;  // the most new tokens of a sequence that the launch covers
+  int splits;   // parts that fill the card; a longer pair takes more
+  int cta0;     // CTA (without splits) that this launch begins with
   float scale_log2;
   int* status;
   Kv4Seq seq;
@@ -234,8 +244,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   const Kv4Seq& s = p.seq;
   // the row pairs with the most positions come first
   const int per_pair = s.batch * s.kv_heads;
-  const int rp = p.row_pairs - 1 - static_cast<int>(blockIdx.x) / per_pair;
-  const int pair = static_cast<int>(blockIdx.x) % per_pair;
+  const int cta = p.cta0 + static_cast<int>(blockIdx.x);
+  const int rp = p.row_pairs - 1 - cta / per_pair, pair = cta % per_pair;
   const int b = pair / s.kv_heads, kvh = pair % s.kv_heads;
   int64_t first;
   int count;
@@ -255,11 +265,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   // This CTA's part: `tiles` tiles from position at0 on.  Positions below are relative to at0.
   const int len_all = static_cast<int>(len64);
   const int tiles_all = (len_all + kTile - 1) / kTile;
-  const int share = (tiles_all + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y);
-  const int tile0 = min(static_cast<int>(blockIdx.y) * share, tiles_all);
+  const int parts = min(max(p.splits, (len_all + most_positions<T>() - 1) / most_positions<T>()), static_cast<int>(gridDim.y));
+  const int share = (tiles_all + parts - 1) / parts;
+  const int tile0 = static_cast<int>(min(static_cast<int64_t>(blockIdx.y) * share, static_cast<int64_t>(tiles_all)));
   const int tiles = min(share, tiles_all - tile0);
   const int at0 = tile0 * kTile;
   const int len = min(len_all - at0, tiles * kTile);
+  if (gridDim.y > 1 && tiles == 0) {  // a part of nothing: weighs 0
+    if (tid < rows)
+      *reinterpret_cast<float2*>(p.ml_part + ((static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * (2 * kPRows) + tid) * 2) =
+          make_float2(kPFloor, 0.f);
+    return;
+  }
 
   if (tid == 0) {
     sh_abort = 0;
@@ -730,17 +747,17 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
 }
 
 // Joins the parts of the rows.  A CTA takes eight rows of a row pair, a warp each: lane
-// c holds the weight of part c, then every lane D / 32 elements.
-template <typename T, int D>
+// c holds the weight of part c (of 32 at a time), then every lane D / 32 elements.
+template <typename T, int D, bool kMany>
 __global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Kv4PromptParams p, int splits) {
   constexpr int kE = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   pdl_wait();  // the partials
   const Kv4Seq& s = p.seq;
-  const int64_t cta = blockIdx.x;
+  const int cta = p.cta0 + static_cast<int>(blockIdx.x);
   const int per_pair = s.batch * s.kv_heads;
-  const int rp = p.row_pairs - 1 - static_cast<int>(cta / per_pair), pair = static_cast<int>(cta % per_pair);
+  const int rp = p.row_pairs - 1 - cta / per_pair, pair = cta % per_pair;
   const int b = pair / s.kv_heads, kvh = pair % s.kv_heads;
   int64_t first;
   int count;
@@ -748,33 +765,43 @@ __global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Kv4Prompt
   const int in_cta = static_cast<int>(blockIdx.y) * 8 + warp;
   const int64_t row = static_cast<int64_t>(rp) * 2 * kPRows + in_cta;
   if (row >= static_cast<int64_t>(min(count, p.max_new)) * p.group) return;
-  const int64_t part0 = cta * splits * (2 * kPRows) + in_cta;  // part c: + c * 256
-  float2 ml = make_float2(kPFloor, 0.f);
-  if (lane < splits) ml = *reinterpret_cast<const float2*>(p.ml_part + (part0 + lane * (2 * kPRows)) * 2);
-  float mx = ml.y == 0.f ? kPFloor : ml.x;
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-  // a part that saw nothing weighs 0, whatever its rows hold
-  const float w = ml.y == 0.f ? 0.f : exp2_approx(ml.x - mx);
-  float l = ml.y == 0.f ? 0.f : w * ml.y;
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-  const uint32_t live = __ballot_sync(0xffffffffu, ml.y != 0.f);
-  float f[kE];
+  const int64_t part0 = static_cast<int64_t>(blockIdx.x) * splits * (2 * kPRows) + in_cta;  // part c: + c * 256
+  float m = kPFloor, l = 0.f, f[kE];
 #pragma unroll
   for (int x = 0; x < kE; ++x) f[x] = 0.f;
-#pragma unroll 4
-  for (int c = 0; c < splits; ++c) {
-    const float k = __shfl_sync(0xffffffffu, w, c);
-    if (!((live >> c) & 1u)) continue;
-    const float* src = p.o_part + (part0 + static_cast<int64_t>(c) * (2 * kPRows)) * D + lane * kE;
-    float v[kE];
-    if (kE == 4)
-      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-    else
-      *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+  for (int c0 = 0; c0 < (kMany ? splits : 1); c0 += 32) {
+    float2 ml = make_float2(kPFloor, 0.f);
+    if (c0 + lane < splits)
+      ml = *reinterpret_cast<const float2*>(p.ml_part + (part0 + static_cast<int64_t>(c0 + lane) * (2 * kPRows)) * 2);
+    // a part that saw nothing weighs 0, whatever its rows hold
+    const uint32_t live = __ballot_sync(0xffffffffu, ml.y != 0.f);
+    if (kMany && live == 0) continue;
+    float mx = ml.y == 0.f ? kPFloor : ml.x;
 #pragma unroll
-    for (int x = 0; x < kE; ++x) f[x] = fmaf(k, v[x], f[x]);
+    for (int x = 1; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+    mx = fmaxf(mx, m);
+    const float w = ml.y == 0.f ? 0.f : exp2_approx(ml.x - mx), was = exp2_approx(m - mx);
+    float sum = ml.y == 0.f ? 0.f : w * ml.y;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    m = mx;
+    l = fmaf(was, l, sum);
+#pragma unroll
+    for (int x = 0; x < kE; ++x) f[x] *= was;
+    const int most = kMany ? min(splits - c0, 32) : splits;
+#pragma unroll 4
+    for (int c = 0; c < most; ++c) {
+      const float k = __shfl_sync(0xffffffffu, w, c);
+      if (!((live >> c) & 1u)) continue;
+      const float* src = p.o_part + (part0 + static_cast<int64_t>(c0 + c) * (2 * kPRows)) * D + lane * kE;
+      float v[kE];
+      if (kE == 4)
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+      else
+        *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+      for (int x = 0; x < kE; ++x) f[x] = fmaf(k, v[x], f[x]);
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* dst = static_cast<T*>(p.out) + ((first + row / p.group) * p.heads + kvh * p.group + row % p.group) * D + lane * kE;
@@ -786,38 +813,52 @@ __global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Kv4Prompt
 }
 
 struct PromptPlan {
-  int row_pairs, splits;
-  int64_t ctas;  // without the splits
+  int row_pairs, fill, splits;  // parts that fill the card, and of a launch
+  int64_t ctas, per_launch;     // without the splits
   size_t o_off, bytes;
 };
 
-PromptPlan prompt_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim, int num_sms) {
+// most: the most positions of a part
+PromptPlan prompt_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim, int most,
+                       int num_sms) {
   PromptPlan a;
   a.row_pairs = static_cast<int>((group * max_new + 2 * kPRows - 1) / (2 * kPRows));
   a.ctas = static_cast<int64_t>(a.row_pairs) * batch * kv_heads;
   // as many parts as leave no SM a second CTA, of four tiles or more
-  int64_t splits = num_sms / a.ctas;
-  const int64_t most = (max_len + 4 * kPTile - 1) / (4 * kPTile);
-  if (splits > most) splits = most;
-  if (splits > kPMaxSplits) splits = kPMaxSplits;
-  a.splits = static_cast<int>(splits < 1 ? 1 : splits);
-  const size_t rows = static_cast<size_t>(a.ctas) * a.splits * 2 * kPRows;
-  a.o_off = a.splits > 1 ? (rows * 2 * sizeof(float) + 255) & ~static_cast<size_t>(255) : 0;
-  a.bytes = a.splits > 1 ? a.o_off + rows * dim * sizeof(float) : 16;
+  int64_t fill = num_sms / a.ctas;
+  const int64_t four = (max_len + 4 * kPTile - 1) / (4 * kPTile);
+  if (fill > four) fill = four;
+  if (fill > kPMaxSplits) fill = kPMaxSplits;
+  a.fill = static_cast<int>(fill < 1 ? 1 : fill);
+  const int64_t need = (max_len + most - 1) / most;
+  a.splits = static_cast<int>(need > 65535 ? 65535 : need > a.fill ? need : a.fill);
+  a.per_launch = a.ctas;
+  a.o_off = 0;
+  a.bytes = 16;
+  if (a.splits > 1) {
+    const int64_t part = 2 * kPRows * (dim + 2) * static_cast<int64_t>(sizeof(float));
+    const int64_t fits = kPScratch / (part * a.splits);
+    if (a.per_launch > fits) a.per_launch = fits < 1 ? 1 : fits;
+    const size_t rows = static_cast<size_t>(a.per_launch) * a.splits * 2 * kPRows;
+    a.o_off = (rows * 2 * sizeof(float) + 255) & ~static_cast<size_t>(255);
+    a.bytes = a.o_off + rows * dim * sizeof(float);
+  }
   return a;
 }
 
 template <typename T, int D>
-int prompt_t(const Kv4PromptParams& p, const PromptPlan& a, cudaStream_t st) {
+int prompt_t(Kv4PromptParams p, const PromptPlan& a, cudaStream_t st) {
   constexpr int smem = PromptSmem<D>::kBytes;
   if (!set_smem_limit(kv4_prompt_kernel<T, D>, smem)) return FITQ_ERR_CUDA;
-  cudaError_t e = launch_pdl(kv4_prompt_kernel<T, D>, dim3(static_cast<unsigned>(a.ctas), a.splits), dim3(kPThreads),
-                             smem, st, p);
-  note_launch();
-  if (e != cudaSuccess) return FITQ_ERR_CUDA;
-  if (a.splits > 1) {
-    e = launch_pdl(kv4_prompt_combine_kernel<T, D>, dim3(static_cast<unsigned>(a.ctas), 2 * kPRows / 8), dim3(256), 0, st,
-                   p, a.splits);
+  for (int64_t at = 0; at < a.ctas; at += a.per_launch) {
+    const unsigned ctas = static_cast<unsigned>(a.ctas - at < a.per_launch ? a.ctas - at : a.per_launch);
+    p.cta0 = static_cast<int>(at);
+    cudaError_t e = launch_pdl(kv4_prompt_kernel<T, D>, dim3(ctas, a.splits), dim3(kPThreads), smem, st, p);
+    note_launch();
+    if (e != cudaSuccess) return FITQ_ERR_CUDA;
+    if (a.splits == 1) continue;
+    auto* combine = a.splits > 32 ? kv4_prompt_combine_kernel<T, D, true> : kv4_prompt_combine_kernel<T, D, false>;
+    e = launch_pdl(combine, dim3(ctas, 2 * kPRows / 8), dim3(256), 0, st, p, a.splits);
     note_launch();
     if (e != cudaSuccess) return FITQ_ERR_CUDA;
   }
@@ -828,18 +869,22 @@ int prompt_t(const Kv4PromptParams& p, const PromptPlan& a, cudaStream_t st) {
 
 size_t kv4_prompt_workspace(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim,
                             int num_sms) {
-  return prompt_plan(batch, kv_heads, group, max_new, max_len, dim, num_sms).bytes;
+  // the query does not know the type
+  const size_t a = prompt_plan(batch, kv_heads, group, max_new, max_len, dim, most_positions<__nv_bfloat16>(), num_sms).bytes;
+  const size_t b = prompt_plan(batch, kv_heads, group, max_new, max_len, dim, most_positions<__half>(), num_sms).bytes;
+  return a > b ? a : b;
 }
 
 int launch_kv4_prompt(const Kv4Seq& seq, const void* q, int64_t q_stride, const void* pool, void* out, int heads,
                       int dim, int dtype, int64_t max_new, int64_t max_len, void* workspace, int* status,
                       cudaStream_t st, int num_sms) {
   const int group = heads / seq.kv_heads;
-  const PromptPlan a = prompt_plan(seq.batch, seq.kv_heads, group, max_new, max_len, dim, num_sms);
+  const int most = dtype == FITQ_DTYPE_BF16 ? most_positions<__nv_bfloat16>() : most_positions<__half>();
+  const PromptPlan a = prompt_plan(seq.batch, seq.kv_heads, group, max_new, max_len, dim, most, num_sms);
   float* ml = static_cast<float*>(workspace);
   float* o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + a.o_off);
   const Kv4PromptParams p{q, q_stride, out, static_cast<const uint8_t*>(pool), ml, o, heads, group, a.row_pairs,
-                          static_cast<int>(max_new), 1.4426950408889634f / sqrtf(static_cast<float>(dim)), status, seq};
+                          static_cast<int>(max_new), a.fill, 0, 1.4426950408889634f / sqrtf(static_cast<float>(dim)), status, seq};
   if (dtype == FITQ_DTYPE_BF16)
     return dim == 128 ? prompt_t<__nv_bfloat16, 128>(p, a, st) : prompt_t<__nv_bfloat16, 64>(p, a, st);
   return dim == 128 ? prompt_t<__half, 128>(p, a, st) : prompt_t<__half, 64>(p, a, st);
