@@ -386,11 +386,14 @@ FITQ_API int fitq_kv4_gather(const fitq_kv4* cache, void* k, void* v, int dtype,
  * (appended before): token i of a sequence sees positions <= prefix + i, query
  * head h reads KV head h / (heads / kv_heads).  q, out [tokens, heads, head_dim]
  * of dtype (q_stride as above; out may be q as above); scale 1/sqrt(head_dim), fp32 softmax and sums.
+ * The weights enter the second product rounded to fp16; from heads / kv_heads * max_new = 65
+ * rows on and for bf16 results keys and values are rounded to fp16 too (2^-11 of a value, 2^-23
+ * where it is below fp16's normal range).
  * max_new: the most new tokens of one sequence (a sequence with more records
  * FITQ_ERR_ARG, its tokens beyond are not written).  max_len: the most positions of
  * one sequence, if known, else max_pages * page_size; it only sizes the grid.
  * Deterministic.  A token that sees no position gives zeros.  The workspace of sizes that
- * no call takes is 0 bytes. */
+ * no call takes is 0 bytes; over 16,384 positions it grows to some 256 MB. */
 FITQ_API size_t fitq_kv4_attention_workspace(const fitq_kv4* cache, int heads, int64_t max_new,
                                              int64_t max_len);
 FITQ_API int fitq_kv4_attention(const fitq_kv4* cache, const void* q, int64_t q_stride, void* out,
