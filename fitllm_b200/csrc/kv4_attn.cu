@@ -711,6 +711,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
       // ---- scores in log2 units less the reference (position g: columns 2 qd, 2 qd + 1;
       // position g + 8: the same)
       float sc[N][NT][4], x[N][NT][4];
+      float largest = -INFINITY;
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         float ks[2][G];
@@ -728,9 +729,10 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
             sc[u][nt][e] = v;
             x[u][nt][e] = fmaf(v, cn[nt][e & 1], -m_run[nt][e & 1]);
             if (edge && pos0 + g + 8 * h > lim[nt][e & 1]) sc[u][nt][e] = x[u][nt][e] = -INFINITY;
-            over |= x[u][nt][e] > room;
+            largest = fmaxf(largest, x[u][nt][e]);
           }
       }
+      over |= largest > room;
       if (__any_sync(0xffffffffu, over)) {
         if (__any_sync(0xffffffffu, cap == kGaveUp)) return false;  // the warp as one
         // the largest finite scale of the blocks; the others reach their group's elements
