@@ -62,8 +62,8 @@
 // of 1,024 positions: 5.9 us).
 //
 // Bound: HBM, 18 D / 16 B per position and KV head, and the instructions of a block (some
-// 300 for eight columns, of 380 that an SM's schedulers have time for at 6.5 TB/s).  The
-// 64 sequences above take 75.5 us, 4.2 TB/s; 200 of them 209 us, 4.6 TB/s; inside the
+// 310 for eight columns, of 380 that an SM's schedulers have time for at 6.5 TB/s).  The
+// 64 sequences above take 78.8 us, 4.0 TB/s; 200 of them 217 us, 4.5 TB/s; inside the
 // loop it is 5.5 TB/s, the rest is the start (5 us until the first block), the two CTAs
 // of an SM ending apart and the join (4 us).
 #include <type_traits>

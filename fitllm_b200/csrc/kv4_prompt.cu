@@ -24,7 +24,7 @@
 // 4.2e-4 where the result's rounding and the weights' alone give 2.9e-4): there a value is
 // the sum of two fp16 numbers, computed in fp32, tiles are 64 positions of two rows (columns
 // of V^T) each, half of the decoders decode keys and half values, and both products take twice
-// the MMAs: 176 -> 272 us for the two sequences below.  Queries are scaled per row by a power of two as in kv4_attn.cu.
+// the MMAs: 176 -> 275 us for the two sequences below.  Queries are scaled per row by a power of two as in kv4_attn.cu.
 //
 // The reference m of a row moves only when a weight would exceed 2^15 (fp16's range for
 // P), and then to 2^7 below the row's largest, so that eight more bits of growth move
@@ -47,7 +47,7 @@
 // the MMAs (4 x 128^3: 2,048 cycles) alike; measured, the chain of a step (wait, read S,
 // maximum, exponentials, write P) and its hand-overs, some 2,000 cycles of 64 positions
 // that two row tiles per SM cover in part.  Two sequences of up to 2,048 tokens (40 heads
-// on 8) behind up to 513: 173 us, 0.57 PFLOP/s.  Half the exponentials as a polynomial
+// on 8) behind up to 513: 175.5 us, 0.56 PFLOP/s.  Half the exponentials as a polynomial
 // on the FMA pipe made it 183 us, sixteen softmax warps (two threads a row) 200 us.
 #include <type_traits>
 
