@@ -1,8 +1,9 @@
 // Log probabilities of given tokens with the row's entropy and top alternatives,
 // and the gradient.
 //
-// For a row z of V logits with M = max z, S = sum exp(z - M):
-//   logp = z[id] - M - log S,   H = log S - sum exp(z - M) (z - M) / S,
+// For a row z of V logits with M = max z, S = sum exp(z - M) = 1 + S' (S': all elements but
+// one that is M), E' = sum exp(z - M) (z - M):
+//   logp = z[id] - M - log1p(S'),   H = log1p(S') - E' / (1 + S'),
 // and the k largest logits in order, the lower index first where two are equal
 // (a NaN counts as the largest).  Upstream gradients a (logp), h (entropy) and
 // t_j (alternatives) give, with p_v = exp(z_v - M - log S),
@@ -12,8 +13,9 @@
 // that log S carries behind M.
 //
 // logprob_fwd_kernel: up to eight CTAs (a cluster) share a row.  Sums are kept
-// relative to a thread's own running maximum and joined over warps, the CTA and
-// the cluster.  Few rows: a thread's share stays in registers, every load issued
+// relative to a thread's own running maximum, which stays out of them (a likely token's 1
+// would take the digits of what the others add up to: entropies of 0.04 were off by 5e-4 of
+// themselves, now by 2e-6), and joined over warps, the CTA and the cluster.  Few rows: a thread's share stays in registers, every load issued
 // before the first use.  Many rows: a CTA streams its row, eight 16-byte loads
 // in flight per thread.  Alternatives: the k-th largest of 128 thread-group maxima
 // bounds the k-th largest logit of the CTA's share from below; the few elements at
@@ -23,7 +25,7 @@
 // maximum reaches it is noted and read again at the end; only a list that overflows
 // reads the whole row again.
 // Bound: HBM (one read) for many rows, latency for few: 2,048 rows of 152,064 bf16
-// logits 119 us, 5.2 TB/s; 40 of fp32 with 5 alternatives 14 us; one of bf16 with 20
+// logits 123 us, 5.1 TB/s; 40 of fp32 with 5 alternatives 14 us; one of bf16 with 20
 // alternatives 8.6 us.
 //
 // logprob_bwd_kernel: one read and one write of the row; the up to k + 1 marked
@@ -47,6 +49,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // meeting an exponent of -inf.
 constexpr float kLowest = -1000.f;
 constexpr float kFarBelow = -3.402823466e38f;  // a base that stands for -inf: no finite value is smaller
+// How far a streamed element may exceed the sums' base, by which what lies between loses digits
+// and for which a warp's granules wait: 4 / 6 / 8 / 20 took 125.7 / 123.3 / 122.0 / 121.8 us for
+// 2,048 rows of 152,064, 127.8 / 127.2 / 126.3 / 122.1 of logits spread by 6.
+constexpr float kMove = 6.f;
 
 // max(d, kLowest) that keeps a NaN.
 __device__ __forceinline__ float bounded(float d) {
@@ -180,16 +186,18 @@ __device__ __forceinline__ void cluster_arrive() {
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// (m, s, t): the maximum m, sum exp(d) and sum exp(d) d over d = z - m, of two parts
-// joined.
+// (m, s, t): the maximum m, and sum exp(d) and sum exp(d) d, d = z - m, over all elements
+// but one that is m; of two parts joined.
 __device__ __forceinline__ void join(float& m, float& s, float& t, float m2, float s2, float t2) {
-  const float mn = fmaxf(m, m2);
-  const float base = mn == -INFINITY ? 0.f : mn;
-  const float d1 = fmaxf(m - base, kLowest), d2 = fmaxf(m2 - base, kLowest);
-  const float k1 = exp2_approx(d1 * kLog2e), k2 = exp2_approx(d2 * kLog2e);
-  t = k1 * fmaf(d1, s, t) + k2 * fmaf(d2, s2, t2);
-  s = k1 * s + k2 * s2;
-  m = mn;
+  if (m2 > m) {
+    const float a = m, b = s, c = t;
+    m = m2, s = s2, t = t2;
+    m2 = a, s2 = b, t2 = c;
+  }
+  if (m2 == -INFINITY) return;  // no element
+  const float d = fmaxf(m2 - m, kLowest), k = exp2_approx(d * kLog2e), all = s2 + 1.f;
+  s = fmaf(k, all, s);
+  t = fmaf(k, fmaf(d, all, t2), t);
 }
 
 // Largest element of a granule; a NaN is passed over.
@@ -214,10 +222,10 @@ __device__ __forceinline__ float vec_max<__half>(const uint4& u) {
 
 constexpr int kLpUnroll = 8;  // granules in flight per thread of a streamed row
 // From four rows per SM on, without alternatives, CTAs of 256 threads, four on an SM, cover
-// each other's starts and ends better than two of 512: 2,048 / 1,200 / 600 / 400 rows of
-// 152,064 bf16 logits 119 / 80 / 50 / 37 us against 134 / 86 / 50 / 33, 5,000 rows of 32,001 81
-// against 111.  With alternatives, whose bound and ranking are work of a whole CTA, they lose
-// (2,048 rows with 20: 248 against 217 us).
+// each other's starts and ends better than two of 512: 2,048 / 1,200 / 600 rows of 152,064
+// bf16 logits 123 / 84 / 53 us against 140 / 91 / 53, 5,000 rows of 32,001 86 against 117; 400
+// rows lost (37 against 33).  With alternatives, whose bound and ranking are work of a whole
+// CTA, they lose too (2,048 rows with 20: 248 against 217 us).
 constexpr int kLpSmall = 256, kLpUnrollSmall = 6, kLpSmallRows = 4;
 
 // kNV > 0: a thread's granules stay in registers; kNV = 0: they are streamed.
@@ -353,6 +361,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprob_fwd_kernel(
       t2 = fma2(e, d, t2);
     }
   };
+  // sums without one of the elements that are the base: a 1 in the larger half
+  auto less_one = [](uint64_t x) {
+    float a, b;
+    unpack2(x, a, b);
+    return a >= b ? pack2(a - 1.f, b) : pack2(a, b - 1.f);
+  };
   float bound_f = INFINITY;  // what the alternatives are not smaller than
   auto reaches = [&](const uint4& u) { return vec_max<T>(u) >= bound_f; };
   if (kNV > 0) {
@@ -365,18 +379,29 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprob_fwd_kernel(
       add(u);
       return false;
     });
+    if (m != -INFINITY) s2 = less_one(s2);
     if (kTop) {
       bound_f = find_bound(m);
       collect_mask(for_held(k0, kAll, kKeep, v_lo + tid, reaches), v_lo + tid, bound_f);
     }
   } else {
-    // The sums' base only moves when a granule exceeds it by e^20, which they have room
-    // for: moving it for every new maximum would cost a warp most of its granules.  The
+    // The sums' base, an element that stays out of them, only moves when a granule exceeds it
+    // by kMove: moving it for every new maximum would cost a warp most of its granules.  The
     // first granules give a bound already.
+    // Behind a batch in which it moved, it is taken off the sums, and the one before it comes in:
+    // an element far above the others takes the digits of its batch's sums only.
+    float was = kFarBelow;
+    auto settle = [&] {
+      if (base == was) return;
+      const float d = fmaxf(was - base, kLowest), k = exp2_approx(d * kLog2e);
+      s2 = add2(less_one(s2), pack2(k, 0.f));
+      t2 = add2(t2, pack2(k * d, 0.f));
+      was = base;
+    };
     auto stream = [&](const uint4& u) -> bool {
       const float mx = vec_max<T>(u);
       m = fmaxf(m, mx);
-      if (mx > base + 20.f) {
+      if (mx > base + kMove) {
         const float d = fmaxf(base - mx, kLowest), k = exp2_approx(d * kLog2e);
         t2 = mul2(pack2(k, k), fma2(pack2(d, d), s2, t2));
         s2 = mul2(pack2(k, k), s2);
@@ -386,12 +411,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprob_fwd_kernel(
       return kTop && mx >= bound_f;
     };
     int v0 = v_lo + tid;
+    base = kFarBelow;
     if (v0 < v_hi) {
       const float first = vec_max<T>(held[0]);
       base = first == -INFINITY ? kFarBelow : first;
     }
+    if (base == kFarBelow) s2 = pack2(-1.f, 0.f);
     // granules that reach the bound are noted, for the CTA to take together behind the row: at
-    // once a warp would wait for each (2,048 rows of 152,064 with 20 alternatives: 249 -> 217 us)
+    // once a warp would wait for each (2,048 rows of 152,064 with 20 alternatives: 249 -> 217 us,
+    // 222 with what follows for the digits of likely tokens)
     auto note = [&](uint32_t mask) {
       if (mask == 0) return;
       for (int at = atomicAdd(&sh_granules, __popc(mask)); mask; mask &= mask - 1, ++at)
@@ -399,12 +427,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprob_fwd_kernel(
     };
     if (kTop) {
       for_held(k0, kAll, kKeep, v0, stream);
+      settle();
       bound_f = find_bound(m);
       note(for_held(k0, kAll, kRefill, v0, reaches));
       v0 += kHeld * kStep;
     }
     for (; v0 < v_hi; v0 += kHeld * kStep) {
       const uint32_t mask = for_held(k0, kAll, kRefill, v0, stream);
+      settle();
       if (kTop) note(mask);
     }
   }
@@ -415,13 +445,21 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprob_fwd_kernel(
   t += t_odd;
   const bool nan_here = s != s;
   const float thread_max = m;
+  if (kNV == 0 && m > base) {
+    // from here on relative to the maximum itself, which stays out instead of the base
+    const float d = m - base, e = exp2_approx(d * kLog2e), k = exp2_approx(-d * kLog2e);
+    s = s + 1.f - e;
+    t = k * fmaf(-d, s, fmaf(-e, d, t));
+    s *= k;
+  }
   {
-    // from here on relative to the maximum itself
     float wm = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-    const float wbase = wm == -INFINITY ? 0.f : wm;
-    const float d = fmaxf(base - wbase, kLowest), k = s == 0.f ? 0.f : exp2_approx(d * kLog2e);
+    // one lane's maximum stays out, the others' come in
+    const bool out = lane == __ffs(__ballot_sync(0xffffffffu, m == wm)) - 1 || m == -INFINITY;
+    const float d = fmaxf(m - (wm == -INFINITY ? 0.f : wm), kLowest), k = exp2_approx(d * kLog2e);
+    s += out ? 0.f : 1.f;
     t = k * fmaf(d, s, t);
     s *= k;
 #pragma unroll
@@ -527,12 +565,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) logprob_fwd_kernel(
   if (cta != 0) return;
   float M = sh_part[0][0], S = sh_part[0][1], E = sh_part[0][2];
   for (uint32_t c = 1; c < ctas; ++c) join(M, S, E, sh_part[c][0], sh_part[c][1], sh_part[c][2]);
-  const float log_s = logf(S);
-  if (M == -INFINITY) S = NAN;  // nothing but -inf: no distribution
+  // S: of all elements but one that is M.  Nothing but -inf, or an infinity: no distribution
+  const float log_s = fabsf(M) <= 3.402823466e38f ? log1pf(S) : NAN;
   if (tid == 0) {
     const bool valid = id >= 0 && id < p.V;
     p.logp[row] = valid ? (z_id - M) - log_s : 0.f;
-    p.entropy[row] = log_s - E / S;
+    p.entropy[row] = log_s - E / (1.f + S);
     if (p.stats) {
       p.stats[2 * row] = M;
       p.stats[2 * row + 1] = log_s;
