@@ -24,7 +24,7 @@
 // 4.2e-4 where the result's rounding and the weights' alone give 2.9e-4): there a value is
 // the sum of two fp16 numbers, computed in fp32, tiles are 64 positions of two rows (columns
 // of V^T) each, half of the decoders decode keys and half values, and both products take twice
-// the MMAs: 176 -> 275 us for the two sequences below.  Queries are scaled per row by a power of two as in kv4_attn.cu.
+// the MMAs: 176 -> 279 us for the two sequences below.  Queries are scaled per row by a power of two as in kv4_attn.cu.
 //
 // The reference m of a row moves only when a weight would exceed 2^15 (fp16's range for
 // P), and then to 2^7 below the row's largest, so that eight more bits of growth move
@@ -39,9 +39,9 @@
 //
 // Where the pairs' row tiles are fewer than the SMs, a pair's positions are cut into up
 // to kPMaxSplits parts of equal tiles, a CTA each; they leave (O, m, l) per row in the
-// workspace and kv4_prompt_combine_kernel joins them in order (deterministic).  So are
-// positions beyond most_positions, for the sums' sake; where the parts of all rows would
-// take more than kPScratch, the call goes in several launches.
+// workspace and kv4_prompt_combine_kernel joins them in order (deterministic).  After
+// window_steps O_r joins the rows' sums in the workspace and begins anew.  Where the parts or
+// sums of all rows would take more than kPScratch, the call goes in several launches.
 //
 // Bound: the exponentials (16 per cycle and SM: 2,048 cycles per 256 x 128 tile) and
 // the MMAs (4 x 128^3: 2,048 cycles) alike; measured, the chain of a step (wait, read S,
@@ -68,13 +68,13 @@ static_assert(2 * kPRegsSoftmax + 2 * kPRegsDecode + kPRegsIssue <= 5 * 96, "mor
 constexpr float kPFloor = -3.0e38f;
 constexpr float kPRoom = 15.f;    // weights stay below 2^15
 constexpr float kPSlack = 8.f;    // a reference that moves leaves this much (log2) to the weights that follow
-constexpr int kPMaxSplits = 32;   // parts that fill the card, at most
-// The most positions of a part.  An accumulation in tensor memory rounds towards zero at the
-// accumulator's size, some 2^-24 of it each time, which adds up to 5e-4 of the output over
-// 131,072 positions and 5e-3 over a million; parts are joined in fp32.
+constexpr int kPMaxSplits = 32;   // a lane of the combining warp each
+// Steps after which O_r joins its rows' sums in the workspace.  An accumulation in tensor
+// memory rounds towards zero at the accumulator's size, some 2^-24 of it each time, which adds
+// up to 5e-4 of the output over 131,072 positions and 5e-3 over a million.
 template <typename T>
-__host__ __device__ constexpr int most_positions() { return std::is_same<T, __half>::value ? 1 << 14 : 1 << 16; }
-constexpr int64_t kPScratch = 256ll << 20;  // bytes of parts that a launch leaves, about, at most
+constexpr int window_steps() { return std::is_same<T, __half>::value ? 1 << 8 : 1 << 10; }
+constexpr int64_t kPScratch = 256ll << 20;  // bytes of such sums and of parts that a launch needs, about, at most
 
 template <int D>
 struct PromptSmem {
@@ -92,10 +92,9 @@ struct Kv4PromptParams {
   void* out;
   const uint8_t* pool;
   float* ml_part;  // [CTAs of the launch without splits][splits][256 rows][2], splits > 1 only
-  float* o_part;   // [..][D]
+  float* o_part;   // [..][D], splits > 1 or where a call may have more than window_steps
   int heads, group, row_pairs;
   int max_new;  // the most new tokens of a sequence that the launch covers
-  int splits;   // parts that fill the card; a longer pair takes more
   int cta0;     // CTA (without splits) that this launch begins with
   float scale_log2;
   int* status;
@@ -221,7 +220,8 @@ __device__ __forceinline__ Pair2 value_pair(uint32_t codes, float s0, float s1, 
 
 extern __shared__ uint8_t g_prompt_smem[];
 
-template <typename T, int D>
+// kLong: a row may see more than window_steps.
+template <typename T, int D, bool kLong>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4PromptParams p) {
   using L = PromptSmem<D>;
   constexpr int G = D / 64;
@@ -230,6 +230,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   constexpr int kTile = kTwo ? kPTile / 2 : kPTile;  // positions of a decoded tile
   constexpr int kSteps = kTile / kPStep;             // steps of one
   constexpr int kBlocks = kTile / kKv4Block;         // blocks of one, a warp each
+  constexpr int kWindow = window_steps<T>();
   __shared__ uint64_t b_qready, b_kfull[2], b_kfree[2], b_vfull[2], b_vfree[2], b_sfull[2][2], b_pready[2][2], b_odone[2][2], b_done;
   __shared__ uint32_t sh_tmem;
   __shared__ int sh_abort;
@@ -265,18 +266,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
   // This CTA's part: `tiles` tiles from position at0 on.  Positions below are relative to at0.
   const int len_all = static_cast<int>(len64);
   const int tiles_all = (len_all + kTile - 1) / kTile;
-  const int parts = min(max(p.splits, (len_all + most_positions<T>() - 1) / most_positions<T>()), static_cast<int>(gridDim.y));
-  const int share = (tiles_all + parts - 1) / parts;
-  const int tile0 = static_cast<int>(min(static_cast<int64_t>(blockIdx.y) * share, static_cast<int64_t>(tiles_all)));
+  const int share = (tiles_all + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y);
+  const int tile0 = min(static_cast<int>(blockIdx.y) * share, tiles_all);
   const int tiles = min(share, tiles_all - tile0);
   const int at0 = tile0 * kTile;
   const int len = min(len_all - at0, tiles * kTile);
-  if (gridDim.y > 1 && tiles == 0) {  // a part of nothing: weighs 0
-    if (tid < rows)
-      *reinterpret_cast<float2*>(p.ml_part + ((static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * (2 * kPRows) + tid) * 2) =
-          make_float2(kPFloor, 0.f);
-    return;
-  }
 
   if (tid == 0) {
     sh_abort = 0;
@@ -362,101 +356,132 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
     // every row of the CTA sees the positions before this one
     const int64_t sure64 = static_cast<int64_t>(pre) + row0 / p.group + 1;
     const int sure = (sure64 < len_all ? static_cast<int>(sure64) : len_all) - at0;
-    float m = kPFloor, l = 0.f;
+    float m = kPFloor, l = 0.f, m_kept = kPFloor;
+    const int64_t part = (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * (2 * kPRows) + r * kPRows + lr;
     uint32_t nan_groups = 0;
     bool ok = active && tiles > 0;
     const uint64_t cn2 = pack2(cn, cn);
     const int steps = (len + kPStep - 1) / kPStep;
-    for (int t = 0; ok && t < steps; ++t) {
-      const int j = t / kSteps, sub = t % kSteps, buf = j & 1, h = t & 1;
-      const int pos0 = t * kPStep;
-      // the tile's notes are there once V is decoded
-      if (sub == 0) {
-        ok = wait_all(&b_vfull[buf], (j >> 1) & 1);
+    for (int t0 = 0; ok && t0 < steps;) {
+      if (kLong && t0 > 0) {  // O_r joins the row's sums, whose columns are its own, and begins anew
+        ok = wait_all(&b_odone[r][(t0 - 1) & 1], ((t0 - 1) >> 1) & 1);
         if (!ok) break;
+        tc_fence_after();
+        const float k = exp2_approx(m_kept - m);
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t x[16];
+          tmem_ld_x16(t_o + 16 * c, x);
+          tmem_ld_wait();
+          if (has) {
+            float4* sum = reinterpret_cast<float4*>(p.o_part + part * D + 16 * c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float4 v = t0 > kWindow ? sum[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+              v.x = fmaf(k, v.x, __uint_as_float(x[4 * i]));
+              v.y = fmaf(k, v.y, __uint_as_float(x[4 * i + 1]));
+              v.z = fmaf(k, v.z, __uint_as_float(x[4 * i + 2]));
+              v.w = fmaf(k, v.w, __uint_as_float(x[4 * i + 3]));
+              sum[i] = v;
+            }
+          }
+          __syncwarp();
+        }
+        m_kept = m;
       }
-      ok = wait_all(&b_sfull[r][h], (t >> 1) & 1);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t v[2][32];
-      tmem_ld_32x32b_x32(t_s + h * kPStep, v[0]);
-      tmem_ld_32x32b_x32(t_s + h * kPStep + 32, v[1]);
-      uint32_t pages = 0xfu;  // which of the step's blocks are there
-      const uint4 nt = *reinterpret_cast<const uint4*>(&sh_note[buf][4 * sub]);
-      constexpr uint32_t kClean = 1u | (kKv4Block << 8) | (kKv4Block << 16);
-      if (((nt.x ^ kClean) | (nt.y ^ kClean) | (nt.z ^ kClean) | (nt.w ^ kClean)) != 0) {
-        pages = 0;
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t note = sh_note[buf][4 * sub + i];
-          pages |= (note & 1u) << i;
-          for (int gr = 0; gr < G; ++gr) {
-            const int at = static_cast<int>((note >> (8 + 8 * gr)) & 0xffu);
-            if (at < kKv4Block && pos0 + i * kKv4Block + at <= lim) nan_groups |= 1u << gr;
+      const int t1 = kLong && steps - t0 > kWindow ? t0 + kWindow : steps;
+      for (int t = t0; ok && t < t1; ++t) {
+        const int j = t / kSteps, sub = t % kSteps, buf = j & 1, h = t & 1;
+        const int pos0 = t * kPStep;
+        // the tile's notes are there once V is decoded
+        if (sub == 0) {
+          ok = wait_all(&b_vfull[buf], (j >> 1) & 1);
+          if (!ok) break;
+        }
+        ok = wait_all(&b_sfull[r][h], (t >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t v[2][32];
+        tmem_ld_32x32b_x32(t_s + h * kPStep, v[0]);
+        tmem_ld_32x32b_x32(t_s + h * kPStep + 32, v[1]);
+        uint32_t pages = 0xfu;  // which of the step's blocks are there
+        const uint4 nt = *reinterpret_cast<const uint4*>(&sh_note[buf][4 * sub]);
+        constexpr uint32_t kClean = 1u | (kKv4Block << 8) | (kKv4Block << 16);
+        if (((nt.x ^ kClean) | (nt.y ^ kClean) | (nt.z ^ kClean) | (nt.w ^ kClean)) != 0) {
+          pages = 0;
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t note = sh_note[buf][4 * sub + i];
+            pages |= (note & 1u) << i;
+            for (int gr = 0; gr < G; ++gr) {
+              const int at = static_cast<int>((note >> (8 + 8 * gr)) & 0xffu);
+              if (at < kKv4Block && pos0 + i * kKv4Block + at <= lim) nan_groups |= 1u << gr;
+            }
           }
         }
-      }
-      tmem_ld_wait();
-      if (pos0 + kPStep > sure || pages != 0xfu) {  // hidden positions
-        const int left = lim - pos0;                // elements 0 .. left are visible
+        tmem_ld_wait();
+        if (pos0 + kPStep > sure || pages != 0xfu) {  // hidden positions
+          const int left = lim - pos0;                // elements 0 .. left are visible
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * c + i > left || !(pages & (1u << (2 * c + (i >> 4))))) v[c][i] = 0xff800000u;
+        }
+        float top[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) top[x] = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * c + i > left || !(pages & (1u << (2 * c + (i >> 4))))) v[c][i] = 0xff800000u;
-      }
-      float top[4];
+          for (int i = 0; i < 32; i += 8)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) top[x] = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; i += 8)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            top[x] = fmaxf(top[x], fmaxf(__uint_as_float(v[c][i + 2 * x]), __uint_as_float(v[c][i + 2 * x + 1])));
-      const float raw = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cn;
-      if (__any_sync(0xffffffffu, raw > m + kPRoom)) {
-        const float m_new = fmaxf(m, raw - (kPRoom - kPSlack));
-        const float al = exp2_approx(m - m_new);
-        m = m_new;
-        l *= al;
-        if (t > 0) {
-          ok = wait_all(&b_odone[r][h ^ 1], ((t - 1) >> 1) & 1);  // the step before has been added
-          if (!ok) break;
-          tc_fence_after();
+            for (int x = 0; x < 4; ++x)
+              top[x] = fmaxf(top[x], fmaxf(__uint_as_float(v[c][i + 2 * x]), __uint_as_float(v[c][i + 2 * x + 1])));
+        const float raw = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cn;
+        if (__any_sync(0xffffffffu, raw > m + kPRoom)) {
+          const float m_new = fmaxf(m, raw - (kPRoom - kPSlack));
+          const float al = exp2_approx(m - m_new);
+          m = m_new;
+          l *= al;
+          if (t > t0) {
+            ok = wait_all(&b_odone[r][h ^ 1], ((t - 1) >> 1) & 1);  // the step before has been added
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 16; ++c) {
-            uint32_t x[16];
-            tmem_ld_x16(t_o + 16 * c, x);
-            tmem_ld_wait();
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t x[16];
+              tmem_ld_x16(t_o + 16 * c, x);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * al);
-            tmem_st_x16(t_o + 16 * c, x);
+              for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * al);
+              tmem_st_x16(t_o + 16 * c, x);
+            }
           }
         }
+        // ---- weights, written over the scores
+        const uint64_t m2 = pack2(-m, -m);
+        uint64_t s2[2] = {0, 0};
+        uint32_t pk[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x0, x1;
+            unpack2(fma2(pack2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), cn2, m2), x0, x1);
+            const float w0 = exp2_approx(x0), w1 = exp2_approx(x1);
+            s2[(i >> 1) & 1] = add2(s2[(i >> 1) & 1], pack2(w0, w1));
+            pk[16 * c + i / 2] = pack_half2(w0, w1);
+          }
+        tmem_st_x32(t_s + h * kPStep, pk);
+        float a, c2;
+        unpack2(add2(s2[0], s2[1]), a, c2);
+        l += a + c2;
+        tmem_st_done();
+        tc_fence_before();
+        arrive_warp(&b_pready[r][h]);
       }
-      // ---- weights, written over the scores
-      const uint64_t m2 = pack2(-m, -m);
-      uint64_t s2[2] = {0, 0};
-      uint32_t pk[32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float x0, x1;
-          unpack2(fma2(pack2(__uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1])), cn2, m2), x0, x1);
-          const float w0 = exp2_approx(x0), w1 = exp2_approx(x1);
-          s2[(i >> 1) & 1] = add2(s2[(i >> 1) & 1], pack2(w0, w1));
-          pk[16 * c + i / 2] = pack_half2(w0, w1);
-        }
-      tmem_st_x32(t_s + h * kPStep, pk);
-      float a, c2;
-      unpack2(add2(s2[0], s2[1]), a, c2);
-      l += a + c2;
-      tmem_st_done();
-      tc_fence_before();
-      arrive_warp(&b_pready[r][h]);
-    }
+      t0 = t1;
+      }
     // the last step's products (and those before them).  A wait by parity tells a phase from
     // its neighbours only: the steps take two barriers in turn, so that the last phase of
     // each has none behind it and the one before it was done when S of this step came.
@@ -466,7 +491,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
       const bool whole = gridDim.y == 1;
       const float inv = !whole ? 2.f : (l == 0.f ? 0.f : 2.f / l);  // values entered halved
       T* dst = static_cast<T*>(p.out) + ((first + tok) * p.heads + hd) * D;
-      const int64_t part = (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * (2 * kPRows) + r * kPRows + lr;
+      const float kept = exp2_approx(m_kept - m);
       if (!whole && has) *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(m, l);
 #pragma unroll 1
       for (int gr = 0; gr < G; ++gr) {
@@ -475,6 +500,18 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
           tmem_ld_32x32b_x32(t_o + 64 * gr, v[0]);
           tmem_ld_32x32b_x32(t_o + 64 * gr + 32, v[1]);
           tmem_ld_wait();
+          if (kLong && steps > kWindow && has) {  // what joined the sums before
+            const float4* sum = reinterpret_cast<const float4*>(p.o_part + part * D + 64 * gr);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float4 x = sum[i];
+              uint32_t* to = &v[i >> 3][4 * (i & 7)];
+              to[0] = __float_as_uint(fmaf(kept, x.x, __uint_as_float(to[0])));
+              to[1] = __float_as_uint(fmaf(kept, x.y, __uint_as_float(to[1])));
+              to[2] = __float_as_uint(fmaf(kept, x.z, __uint_as_float(to[2])));
+              to[3] = __float_as_uint(fmaf(kept, x.w, __uint_as_float(to[3])));
+            }
+          }
         }
         const bool bad = (nan_groups >> gr) & 1u;
 #pragma unroll
@@ -699,7 +736,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
         for (int kk = 0; kk < kPStep / 16; ++kk) {
           const uint64_t vb = dv + ((buf * L::kV + (sub + part) * (D * 128) + kk * 32) >> 4);
           umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + h * kPStep + kk * 8, vb, idesc_o,
-                      t > 0 || kk > 0 || part > 0 ? 1u : 0u);
+                      (kLong ? t % kWindow : t) != 0 || kk > 0 || part > 0 ? 1u : 0u);
         }
       commit_warp(&b_odone[r][h]);
       if (r == last && (sub == kSteps - 1 || t == steps - 1)) commit_warp(&b_vfree[buf]);
@@ -747,8 +784,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prompt_kernel(const Kv4Promp
 }
 
 // Joins the parts of the rows.  A CTA takes eight rows of a row pair, a warp each: lane
-// c holds the weight of part c (of 32 at a time), then every lane D / 32 elements.
-template <typename T, int D, bool kMany>
+// c holds the weight of part c, then every lane D / 32 elements.
+template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Kv4PromptParams p, int splits) {
   constexpr int kE = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -766,42 +803,32 @@ __global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Kv4Prompt
   const int64_t row = static_cast<int64_t>(rp) * 2 * kPRows + in_cta;
   if (row >= static_cast<int64_t>(min(count, p.max_new)) * p.group) return;
   const int64_t part0 = static_cast<int64_t>(blockIdx.x) * splits * (2 * kPRows) + in_cta;  // part c: + c * 256
-  float m = kPFloor, l = 0.f, f[kE];
+  float2 ml = make_float2(kPFloor, 0.f);
+  if (lane < splits) ml = *reinterpret_cast<const float2*>(p.ml_part + (part0 + lane * (2 * kPRows)) * 2);
+  float mx = ml.y == 0.f ? kPFloor : ml.x;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+  // a part that saw nothing weighs 0, whatever its rows hold
+  const float w = ml.y == 0.f ? 0.f : exp2_approx(ml.x - mx);
+  float l = ml.y == 0.f ? 0.f : w * ml.y;
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  const uint32_t live = __ballot_sync(0xffffffffu, ml.y != 0.f);
+  float f[kE];
 #pragma unroll
   for (int x = 0; x < kE; ++x) f[x] = 0.f;
-  for (int c0 = 0; c0 < (kMany ? splits : 1); c0 += 32) {
-    float2 ml = make_float2(kPFloor, 0.f);
-    if (c0 + lane < splits)
-      ml = *reinterpret_cast<const float2*>(p.ml_part + (part0 + static_cast<int64_t>(c0 + lane) * (2 * kPRows)) * 2);
-    // a part that saw nothing weighs 0, whatever its rows hold
-    const uint32_t live = __ballot_sync(0xffffffffu, ml.y != 0.f);
-    if (kMany && live == 0) continue;
-    float mx = ml.y == 0.f ? kPFloor : ml.x;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    mx = fmaxf(mx, m);
-    const float w = ml.y == 0.f ? 0.f : exp2_approx(ml.x - mx), was = exp2_approx(m - mx);
-    float sum = ml.y == 0.f ? 0.f : w * ml.y;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    m = mx;
-    l = fmaf(was, l, sum);
-#pragma unroll
-    for (int x = 0; x < kE; ++x) f[x] *= was;
-    const int most = kMany ? min(splits - c0, 32) : splits;
 #pragma unroll 4
-    for (int c = 0; c < most; ++c) {
-      const float k = __shfl_sync(0xffffffffu, w, c);
-      if (!((live >> c) & 1u)) continue;
-      const float* src = p.o_part + (part0 + static_cast<int64_t>(c0 + c) * (2 * kPRows)) * D + lane * kE;
-      float v[kE];
-      if (kE == 4)
-        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-      else
-        *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+  for (int c = 0; c < splits; ++c) {
+    const float k = __shfl_sync(0xffffffffu, w, c);
+    if (!((live >> c) & 1u)) continue;
+    const float* src = p.o_part + (part0 + static_cast<int64_t>(c) * (2 * kPRows)) * D + lane * kE;
+    float v[kE];
+    if (kE == 4)
+      *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+    else
+      *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
 #pragma unroll
-      for (int x = 0; x < kE; ++x) f[x] = fmaf(k, v[x], f[x]);
-    }
+    for (int x = 0; x < kE; ++x) f[x] = fmaf(k, v[x], f[x]);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   T* dst = static_cast<T*>(p.out) + ((first + row / p.group) * p.heads + kvh * p.group + row % p.group) * D + lane * kE;
@@ -813,32 +840,31 @@ __global__ void __launch_bounds__(256) kv4_prompt_combine_kernel(const Kv4Prompt
 }
 
 struct PromptPlan {
-  int row_pairs, fill, splits;  // parts that fill the card, and of a launch
-  int64_t ctas, per_launch;     // without the splits
+  int row_pairs, splits;
+  bool long_sums;
+  int64_t ctas, per_launch;  // without the splits
   size_t o_off, bytes;
 };
 
-// most: the most positions of a part
-PromptPlan prompt_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim, int most,
+// steps: window_steps of the type
+PromptPlan prompt_plan(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim, int steps,
                        int num_sms) {
   PromptPlan a;
   a.row_pairs = static_cast<int>((group * max_new + 2 * kPRows - 1) / (2 * kPRows));
   a.ctas = static_cast<int64_t>(a.row_pairs) * batch * kv_heads;
   // as many parts as leave no SM a second CTA, of four tiles or more
-  int64_t fill = num_sms / a.ctas;
-  const int64_t four = (max_len + 4 * kPTile - 1) / (4 * kPTile);
-  if (fill > four) fill = four;
-  if (fill > kPMaxSplits) fill = kPMaxSplits;
-  a.fill = static_cast<int>(fill < 1 ? 1 : fill);
-  const int64_t need = (max_len + most - 1) / most;
-  a.splits = static_cast<int>(need > 65535 ? 65535 : need > a.fill ? need : a.fill);
+  int64_t splits = num_sms / a.ctas;
+  const int64_t most = (max_len + 4 * kPTile - 1) / (4 * kPTile);
+  if (splits > most) splits = most;
+  if (splits > kPMaxSplits) splits = kPMaxSplits;
+  a.splits = static_cast<int>(splits < 1 ? 1 : splits);
+  a.long_sums = max_len > static_cast<int64_t>(steps) * kPStep;
   a.per_launch = a.ctas;
   a.o_off = 0;
   a.bytes = 16;
-  if (a.splits > 1) {
-    const int64_t part = 2 * kPRows * (dim + 2) * static_cast<int64_t>(sizeof(float));
-    const int64_t fits = kPScratch / (part * a.splits);
-    if (a.per_launch > fits) a.per_launch = fits < 1 ? 1 : fits;
+  if (a.splits > 1 || a.long_sums) {
+    const int64_t fits = kPScratch / (2 * kPRows * (dim + 2) * static_cast<int64_t>(sizeof(float)) * a.splits);
+    if (a.per_launch > fits) a.per_launch = fits;
     const size_t rows = static_cast<size_t>(a.per_launch) * a.splits * 2 * kPRows;
     a.o_off = (rows * 2 * sizeof(float) + 255) & ~static_cast<size_t>(255);
     a.bytes = a.o_off + rows * dim * sizeof(float);
@@ -849,16 +875,17 @@ PromptPlan prompt_plan(int batch, int kv_heads, int group, int64_t max_new, int6
 template <typename T, int D>
 int prompt_t(Kv4PromptParams p, const PromptPlan& a, cudaStream_t st) {
   constexpr int smem = PromptSmem<D>::kBytes;
-  if (!set_smem_limit(kv4_prompt_kernel<T, D>, smem)) return FITQ_ERR_CUDA;
+  // joining sums costs every step registers: 0.6% in bf16, 4% in fp16
+  auto* kernel = a.long_sums ? kv4_prompt_kernel<T, D, true> : kv4_prompt_kernel<T, D, false>;
+  if (!set_smem_limit(kernel, smem)) return FITQ_ERR_CUDA;
   for (int64_t at = 0; at < a.ctas; at += a.per_launch) {
     const unsigned ctas = static_cast<unsigned>(a.ctas - at < a.per_launch ? a.ctas - at : a.per_launch);
     p.cta0 = static_cast<int>(at);
-    cudaError_t e = launch_pdl(kv4_prompt_kernel<T, D>, dim3(ctas, a.splits), dim3(kPThreads), smem, st, p);
+    cudaError_t e = launch_pdl(kernel, dim3(ctas, a.splits), dim3(kPThreads), smem, st, p);
     note_launch();
     if (e != cudaSuccess) return FITQ_ERR_CUDA;
     if (a.splits == 1) continue;
-    auto* combine = a.splits > 32 ? kv4_prompt_combine_kernel<T, D, true> : kv4_prompt_combine_kernel<T, D, false>;
-    e = launch_pdl(combine, dim3(ctas, 2 * kPRows / 8), dim3(256), 0, st, p, a.splits);
+    e = launch_pdl(kv4_prompt_combine_kernel<T, D>, dim3(ctas, 2 * kPRows / 8), dim3(256), 0, st, p, a.splits);
     note_launch();
     if (e != cudaSuccess) return FITQ_ERR_CUDA;
   }
@@ -870,8 +897,8 @@ int prompt_t(Kv4PromptParams p, const PromptPlan& a, cudaStream_t st) {
 size_t kv4_prompt_workspace(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim,
                             int num_sms) {
   // the query does not know the type
-  const size_t a = prompt_plan(batch, kv_heads, group, max_new, max_len, dim, most_positions<__nv_bfloat16>(), num_sms).bytes;
-  const size_t b = prompt_plan(batch, kv_heads, group, max_new, max_len, dim, most_positions<__half>(), num_sms).bytes;
+  const size_t a = prompt_plan(batch, kv_heads, group, max_new, max_len, dim, window_steps<__nv_bfloat16>(), num_sms).bytes;
+  const size_t b = prompt_plan(batch, kv_heads, group, max_new, max_len, dim, window_steps<__half>(), num_sms).bytes;
   return a > b ? a : b;
 }
 
@@ -879,12 +906,12 @@ int launch_kv4_prompt(const Kv4Seq& seq, const void* q, int64_t q_stride, const 
                       int dim, int dtype, int64_t max_new, int64_t max_len, void* workspace, int* status,
                       cudaStream_t st, int num_sms) {
   const int group = heads / seq.kv_heads;
-  const int most = dtype == FITQ_DTYPE_BF16 ? most_positions<__nv_bfloat16>() : most_positions<__half>();
-  const PromptPlan a = prompt_plan(seq.batch, seq.kv_heads, group, max_new, max_len, dim, most, num_sms);
+  const int steps = dtype == FITQ_DTYPE_BF16 ? window_steps<__nv_bfloat16>() : window_steps<__half>();
+  const PromptPlan a = prompt_plan(seq.batch, seq.kv_heads, group, max_new, max_len, dim, steps, num_sms);
   float* ml = static_cast<float*>(workspace);
   float* o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + a.o_off);
   const Kv4PromptParams p{q, q_stride, out, static_cast<const uint8_t*>(pool), ml, o, heads, group, a.row_pairs,
-                          static_cast<int>(max_new), a.fill, 0, 1.4426950408889634f / sqrtf(static_cast<float>(dim)), status, seq};
+                          static_cast<int>(max_new), 0, 1.4426950408889634f / sqrtf(static_cast<float>(dim)), status, seq};
   if (dtype == FITQ_DTYPE_BF16)
     return dim == 128 ? prompt_t<__nv_bfloat16, 128>(p, a, st) : prompt_t<__nv_bfloat16, 64>(p, a, st);
   return dim == 128 ? prompt_t<__half, 128>(p, a, st) : prompt_t<__half, 64>(p, a, st);
