@@ -339,8 +339,8 @@ int launch_kv4_append(const Kv4Seq& seq, const void* q, int64_t q_stride, const 
                       cudaStream_t st, int num_sms);
 int launch_kv4_gather(const Kv4Seq& seq, const void* pool, void* k, void* v, int dim, int dtype, int* status,
                       cudaStream_t st, int num_sms);
-// max_new: most new tokens of a sequence; max_len: most positions of one, which
-// only sizes the grid.
+// max_new: most new tokens of a sequence; max_len: most positions of one, which sizes the
+// grid and the workspace.
 size_t kv4_attention_workspace(int batch, int kv_heads, int group, int64_t max_new, int64_t max_len, int dim,
                                int num_sms);
 int launch_kv4_attention(const Kv4Seq& seq, const void* q, int64_t q_stride, const void* pool, void* out, int heads,

@@ -952,7 +952,7 @@ __global__ void __launch_bounds__(AttnShape<NT>::kThreads, AttnShape<NT>::kCtas)
           fine = step(j, std::integral_constant<int, 1>{}, std::true_type{});
         ++j;
       }
-      if (!kClustered && j < blocks) {
+      if (j < blocks) {
         flush(stop == window);
         clear();
       }

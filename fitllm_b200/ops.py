@@ -357,7 +357,7 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
     q [tokens, heads, D] bf16 or fp16, rotated, its keys and values appended:
     token i of a sequence sees positions <= prefix + i.  max_new: the most new
     tokens of one sequence (needed with q_start); max_len: the most positions of
-    one sequence, a hint for the grid.  Returns [tokens, heads, D] (into out when
+    one sequence, a hint for the grid and the scratch.  Returns [tokens, heads, D] (into out when
     given; rows of no sequence are left as they are)."""
     L = _lib.load()
     dev = pool.device

@@ -391,7 +391,8 @@ FITQ_API int fitq_kv4_gather(const fitq_kv4* cache, void* k, void* v, int dtype,
  * where it is below fp16's normal range).
  * max_new: the most new tokens of one sequence (a sequence with more records
  * FITQ_ERR_ARG, its tokens beyond are not written).  max_len: the most positions of
- * one sequence, if known, else max_pages * page_size; it only sizes the grid.
+ * one sequence, if known, else max_pages * page_size; it sizes the grid and the workspace (where
+ * it is smaller than the truth, sums over more than 16,384 positions keep fewer digits).
  * Deterministic.  A token that sees no position gives zeros.  The workspace of sizes that
  * no call takes is 0 bytes; over 16,384 positions it grows to some 256 MB. */
 FITQ_API size_t fitq_kv4_attention_workspace(const fitq_kv4* cache, int heads, int64_t max_new,

@@ -297,3 +297,13 @@ def test_a_long_call_of_many_rows_comes_in_several_launches(cuda_dev):
         assert torch.equal(o, _attend(c, out=torch.full_like(q, 7.0)))
         c["max_len"] = 4096  # a hint that is too small: no sums apart, the same result within its roundings
         _check(few, _attend(c))
+
+
+@pytest.mark.parametrize("d,dtype", [(128, BF), (128, FP), (64, BF), (64, FP)])
+def test_few_rows_keep_their_digits_where_max_len_is_too_small(cuda_dev, d, dtype):
+    """A captured call goes on as clusters of few tiles when its sequences have grown long."""
+    n = 1 << 19
+    c = _long(cuda_dev, n, d, dtype, 5, 1, 2, 0.0)
+    c["max_len"] = 1000
+    err, bound, norm = _long_bound(c, _attend(c), n, 1, True)
+    assert err <= bound, f"{err / norm:.2e} of the output, the bound {bound / norm:.2e}"
