@@ -56,6 +56,18 @@ class Kv4C(ctypes.Structure):
 
 KP = ctypes.POINTER(Kv4C)
 
+
+class TreeC(ctypes.Structure):
+    """struct fitq_tree"""
+    _fields_ = [
+        ("parents", P), ("prefix", P), ("parents_stride", I64), ("capacity", I64), ("stride_b", I64),
+        ("stride_h", I64), ("stride_p", I64), ("batch", I32), ("tokens", I32), ("kv_heads", I32), ("head_dim", I32),
+        ("dtype", I32),
+    ]
+
+
+TP = ctypes.POINTER(TreeC)
+
 SIGNATURES = {
     "fitq_version": (ctypes.c_char_p, []),
     "fitq_last_error": (ctypes.c_char_p, []),
@@ -105,6 +117,13 @@ SIGNATURES = {
     "fitq_kv4_attention": (I32, [KP, P, I64, P, I32, I32, I64, I64, P, SZ, P]),
     "fitq_token_logprobs": (I32, [P, I32, P, I64, I64, I64, I32, P, P, P, P, P, P]),
     "fitq_token_logprobs_bwd": (I32, [P, I32, P, I64, I64, I64, I32, P, P, P, P, P, P, P, P]),
+    "fitq_tree_append": (I32, [TP, P, I64, P, I64, P, I64, P, P, P, P, P, I32, I32, P]),
+    "fitq_tree_attention_workspace": (SZ, [TP, I32]),
+    "fitq_tree_attention": (I32, [TP, P, I64, P, P, P, I32, P, SZ, P]),
+    "fitq_tree_verify": (I32, [P, I32, I64, I64, I64, I32, I64, P, P, I64, P, P, I64, I64, P, F32, P, P, P, P]),
+    "fitq_tree_keep": (I32, [TP, P, P, I32, P, P, P, P]),
+    "fitq_multi_lora_workspace": (SZ, [I64, I64, I64, I32, I32]),
+    "fitq_multi_lora": (I32, [P, I64, I64, I64, I64, P, P, I32, I32, P, P, P, I32, P, I64, P, I32, P, SZ, P]),
     "fitq_attention_bwd": (I32, [P, P, P, P, P, P, P, P, P, I64, I64, I32, I32, I32, P, SZ, P]),
 }
 

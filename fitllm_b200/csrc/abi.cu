@@ -12,6 +12,7 @@
 #include "common.cuh"
 #include "kernels.cuh"
 #include "kv4.cuh"
+#include "tree.cuh"
 
 // Device status word shared by all kernels of the library (first error wins).
 __device__ int g_fitq_status = 0;
@@ -1534,6 +1535,196 @@ int fitq_token_logprobs_bwd(const void* logits, int dtype, const int64_t* ids, i
                                                        top_ids, g_logp, g_entropy, g_top, d,
                                                        static_cast<cudaStream_t>(stream)),
                        "token_logprobs_bwd");
+}
+
+// Shape checks shared by the calls on a tree of drafted tokens; fills the kernels' addressing.
+static int tree_view(const char* what, const fitq_tree* t, int heads, fitq::TreeView* out) {
+  if (!t || !t->parents || !t->prefix) return fail(FITQ_ERR_ARG, "%s: NULL tree, parents or prefix", what);
+  if (t->head_dim != 64 && t->head_dim != 128)
+    return fail(FITQ_ERR_UNSUPPORTED, "%s: head_dim must be 64 or 128 (got %d)", what, t->head_dim);
+  if (t->dtype != FITQ_DTYPE_BF16 && t->dtype != FITQ_DTYPE_F16)
+    return fail(FITQ_ERR_UNSUPPORTED, "%s: dtype must be bf16 or fp16 (got %d)", what, t->dtype);
+  if (t->tokens < 1 || t->tokens > fitq::kTreeTokens)
+    return fail(FITQ_ERR_UNSUPPORTED, "%s: a tree has 1..%d tokens (got %d)", what, fitq::kTreeTokens, t->tokens);
+  if (t->batch < 1 || t->batch > 65535 || t->kv_heads < 1 || heads < 1 || heads > 65535 || heads % t->kv_heads != 0 ||
+      t->capacity < 1 || t->capacity > (1ll << 30))
+    return fail(FITQ_ERR_SHAPE, "%s: bad shape (batch=%d heads=%d kv_heads=%d capacity=%lld)", what, t->batch, heads,
+                t->kv_heads, (long long)t->capacity);
+  if (t->parents_stride != 0 && t->parents_stride < t->tokens)
+    return fail(FITQ_ERR_SHAPE, "%s: parents_stride=%lld", what, (long long)t->parents_stride);
+  if (t->stride_b < 0 || t->stride_h < 0 || t->stride_p < t->head_dim ||
+      ((t->stride_b | t->stride_h | t->stride_p) & 7) || t->stride_b >= (1ll << 38) || t->stride_h >= (1ll << 38) ||
+      t->stride_p >= (1ll << 38))
+    return fail(FITQ_ERR_SHAPE, "%s: cache strides must be multiples of 8 that cover a head (got %lld, %lld, %lld)", what,
+                (long long)t->stride_b, (long long)t->stride_h, (long long)t->stride_p);
+  if ((reinterpret_cast<uintptr_t>(t->parents) | reinterpret_cast<uintptr_t>(t->prefix)) & 3u)
+    return fail(FITQ_ERR_ALIGN, "%s: parents and prefix must be 4-byte aligned", what);
+  *out = fitq::TreeView{t->parents, t->parents_stride, t->prefix, t->batch, t->tokens, t->kv_heads,
+                        t->capacity, t->stride_b, t->stride_h, t->stride_p};
+  return FITQ_OK;
+}
+
+int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                     const void* v, int64_t v_stride, void* q_out, void* k_cache, void* v_cache,
+                     const float* cos_half, const float* sin_half, int rope_len, int heads, fitq_stream_t stream) {
+  fitq::TreeView t;
+  int rc = tree_view("tree_append", tree, heads, &t);
+  if (rc) return rc;
+  if (!q || !k || !v || !q_out || !k_cache || !v_cache || !cos_half || !sin_half)
+    return fail(FITQ_ERR_ARG, "tree_append: NULL tensor");
+  if (rope_len < 1) return fail(FITQ_ERR_SHAPE, "tree_append: empty rotary tables");
+  const int64_t row = static_cast<int64_t>(heads) * tree->head_dim, kv_row = static_cast<int64_t>(t.kv_heads) * tree->head_dim;
+  if (q_stride < row || k_stride < kv_row || v_stride < kv_row || ((q_stride | k_stride | v_stride) & 7))
+    return fail(FITQ_ERR_SHAPE, "tree_append: token strides must cover a token and be multiples of 8");
+  if (!al16(q) || !al16(k) || !al16(v) || !al16(q_out) || !al16(k_cache) || !al16(v_cache) || !al16(cos_half) ||
+      !al16(sin_half))
+    return fail(FITQ_ERR_ALIGN, "tree_append: 16-byte alignment");
+  const int64_t n = static_cast<int64_t>(t.batch) * t.tokens;
+  if (q_out == q && q_stride != row) return fail(FITQ_ERR_ARG, "tree_append: q_out is q, but q is strided");
+  if ((q_out != q && kv4_meets(q_out, n * row * 2, q, n, q_stride, row)) ||
+      kv4_meets(q_out, n * row * 2, k, n, k_stride, kv_row) || kv4_meets(q_out, n * row * 2, v, n, v_stride, kv_row))
+    return fail(FITQ_ERR_ARG, "tree_append: q_out overlaps q (other than being q), k or v");
+  if (!current_sms(&rc)) return rc;
+  return launch_status(fitq::launch_tree_append(t, q, q_stride, k, k_stride, v, v_stride, q_out, k_cache, v_cache,
+                                                cos_half, sin_half, rope_len, heads, tree->head_dim, tree->dtype,
+                                                status_ptr(), static_cast<cudaStream_t>(stream)),
+                       "tree_append");
+}
+
+// Whether the attention's tiles can be counted in 31 bits.
+static bool tree_attention_fits(const fitq::TreeView& t, int heads) {
+  const int64_t row_tiles = (static_cast<int64_t>(heads / t.kv_heads) * t.tokens + 255) / 256;
+  return row_tiles * t.batch * t.kv_heads * ((t.capacity + 127) / 128 + 1) < (1ll << 31);
+}
+
+size_t fitq_tree_attention_workspace(const fitq_tree* tree, int heads) {
+  fitq::TreeView t;
+  if (tree_view("tree_attention", tree, heads, &t) != FITQ_OK || !tree_attention_fits(t, heads)) return 0;
+  return fitq::tree_attention_workspace(t, heads, tree->head_dim, sms_for_sizing());
+}
+
+int fitq_tree_attention(const fitq_tree* tree, const void* q, int64_t q_stride, const void* k_cache,
+                        const void* v_cache, void* out, int heads, void* workspace, size_t workspace_bytes,
+                        fitq_stream_t stream) {
+  fitq::TreeView t;
+  int rc = tree_view("tree_attention", tree, heads, &t);
+  if (rc) return rc;
+  if (!q || !k_cache || !v_cache || !out || !workspace) return fail(FITQ_ERR_ARG, "tree_attention: NULL tensor or workspace");
+  if (!tree_attention_fits(t, heads))
+    return fail(FITQ_ERR_SHAPE, "tree_attention: batch * kv_heads * capacity is too large");
+  const int64_t row = static_cast<int64_t>(heads) * tree->head_dim, n = static_cast<int64_t>(t.batch) * t.tokens;
+  if (q_stride < row || (q_stride & 7))
+    return fail(FITQ_ERR_SHAPE, "tree_attention: the token stride must cover a token and be a multiple of 8");
+  if (!al16(q) || !al16(k_cache) || !al16(v_cache) || !al16(out) || !al16(workspace))
+    return fail(FITQ_ERR_ALIGN, "tree_attention: 16-byte alignment");
+  if (!(out == q && q_stride == row) && kv4_meets(out, n * row * 2, q, n, q_stride, row))
+    return fail(FITQ_ERR_ARG, "tree_attention: out overlaps q, other than being q of dense tokens");
+  const int sms = current_sms(&rc);
+  if (!sms) return rc;
+  const size_t need = fitq::tree_attention_workspace(t, heads, tree->head_dim, sms);
+  if (workspace_bytes < need)
+    return fail(FITQ_ERR_WORKSPACE, "tree_attention: workspace %zu < %zu bytes", workspace_bytes, need);
+  return launch_status(fitq::launch_tree_attention(t, q, q_stride, k_cache, v_cache, out, heads, tree->head_dim,
+                                                   tree->dtype, workspace, status_ptr(),
+                                                   static_cast<cudaStream_t>(stream), sms),
+                       "tree_attention");
+}
+
+int fitq_tree_verify(const void* logits, int dtype, int64_t stride_b, int64_t stride_t, int64_t batch, int tokens,
+                     int64_t vocab, const int64_t* ids, const int32_t* parents, int64_t parents_stride,
+                     const float* uniforms, const float* probs, int64_t probs_stride_b, int64_t probs_stride_t,
+                     const float* temperatures, float temperature, int32_t* path, int64_t* accepted,
+                     int64_t* next_token, fitq_stream_t stream) {
+  if (!logits || !ids || !parents || !uniforms || !path || !accepted || !next_token)
+    return fail(FITQ_ERR_ARG, "tree_verify: NULL tensor");
+  if (dtype != FITQ_DTYPE_BF16 && dtype != FITQ_DTYPE_F16 && dtype != FITQ_DTYPE_F32)
+    return fail(FITQ_ERR_UNSUPPORTED, "tree_verify: unknown dtype %d", dtype);
+  if (tokens < 1 || tokens > fitq::kTreeTokens)
+    return fail(FITQ_ERR_UNSUPPORTED, "tree_verify: a tree has 1..%d tokens (got %d)", fitq::kTreeTokens, tokens);
+  if (batch < 1 || batch >= (1ll << 24) || vocab < 1 || vocab >= (1ll << 24) || stride_t < vocab || stride_b < 0 ||
+      (parents_stride != 0 && parents_stride < tokens) || (probs && (probs_stride_t < vocab || probs_stride_b < 0)))
+    return fail(FITQ_ERR_SHAPE, "tree_verify: bad shape (batch=%lld vocab=%lld strides %lld, %lld)", (long long)batch,
+                (long long)vocab, (long long)stride_b, (long long)stride_t);
+  if (!temperatures && !(temperature >= 0.f && temperature <= 3.4e38f))
+    return fail(FITQ_ERR_ARG, "tree_verify: temperature must not be negative (got %g)", static_cast<double>(temperature));
+  const uintptr_t size = dtype == FITQ_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % size ||
+      ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(accepted) | reinterpret_cast<uintptr_t>(next_token)) & 7u) ||
+      ((reinterpret_cast<uintptr_t>(parents) | reinterpret_cast<uintptr_t>(uniforms) | reinterpret_cast<uintptr_t>(probs) |
+        reinterpret_cast<uintptr_t>(temperatures) | reinterpret_cast<uintptr_t>(path)) & 3u))
+    return fail(FITQ_ERR_ALIGN, "tree_verify: tensors must be aligned to their elements");
+  int rc;
+  const int sms = current_sms(&rc);
+  if (!sms) return rc;
+  return launch_status(fitq::launch_tree_verify(logits, dtype, stride_b, stride_t, batch, tokens, vocab, ids, parents,
+                                                parents_stride, uniforms, probs, probs_stride_b, probs_stride_t,
+                                                temperatures, temperature, path, accepted, next_token, status_ptr(),
+                                                static_cast<cudaStream_t>(stream), sms),
+                       "tree_verify");
+}
+
+int fitq_tree_keep(const fitq_tree* tree, void* const* k_caches, void* const* v_caches, int layers,
+                   const int32_t* path, const int64_t* accepted, int32_t* lengths, fitq_stream_t stream) {
+  fitq::TreeView t;
+  int rc = tree_view("tree_keep", tree, tree ? tree->kv_heads : 1, &t);
+  if (rc) return rc;
+  if (!k_caches || !v_caches || !path || !accepted || !lengths) return fail(FITQ_ERR_ARG, "tree_keep: NULL tensor");
+  if (layers < 1 || layers > (1 << 20)) return fail(FITQ_ERR_SHAPE, "tree_keep: layers=%d", layers);
+  for (int i = 0; i < layers; ++i) {
+    if (!k_caches[i] || !v_caches[i]) return fail(FITQ_ERR_ARG, "tree_keep: NULL cache of layer %d", i);
+    if (!al16(k_caches[i]) || !al16(v_caches[i])) return fail(FITQ_ERR_ALIGN, "tree_keep: 16-byte alignment");
+  }
+  if ((reinterpret_cast<uintptr_t>(accepted) & 7u) ||
+      ((reinterpret_cast<uintptr_t>(path) | reinterpret_cast<uintptr_t>(lengths)) & 3u))
+    return fail(FITQ_ERR_ALIGN, "tree_keep: tensors must be aligned to their elements");
+  if (!current_sms(&rc)) return rc;
+  return launch_status(fitq::launch_tree_keep(t, k_caches, v_caches, layers, tree->head_dim, path, accepted, lengths,
+                                              status_ptr(), static_cast<cudaStream_t>(stream)),
+                       "tree_keep");
+}
+
+static bool multi_lora_fits(int64_t tokens, int64_t k, int64_t n, int rank, int batch) {
+  return tokens >= 0 && tokens < (1ll << 28) && k >= 8 && k < (1ll << 24) && k % 8 == 0 && n >= 8 && n < (1ll << 24) &&
+         n % 8 == 0 && (rank == 16 || rank == 32 || rank == 48 || rank == 64) && batch >= 1;
+}
+
+size_t fitq_multi_lora_workspace(int64_t tokens, int64_t k, int64_t n, int rank, int batch) {
+  if (!multi_lora_fits(tokens, k, n, rank, batch)) return 0;
+  return fitq::multi_lora_workspace(tokens, k, n, rank, batch, sms_for_sizing());
+}
+
+int fitq_multi_lora(const void* x, int64_t x_stride, int64_t tokens, int64_t k, int64_t n, const void* a,
+                    const void* b, int rank, int adapters, const float* scale, const int32_t* adapter,
+                    const int32_t* q_start, int batch, const void* y_add, int64_t y_add_stride, void* y, int dtype,
+                    void* workspace, size_t workspace_bytes, fitq_stream_t stream) {
+  if (rank != 16 && rank != 32 && rank != 48 && rank != 64)
+    return fail(FITQ_ERR_UNSUPPORTED, "multi_lora: rank must be 16, 32, 48 or 64 (got %d)", rank);
+  if (dtype != FITQ_DTYPE_BF16 && dtype != FITQ_DTYPE_F16)
+    return fail(FITQ_ERR_UNSUPPORTED, "multi_lora: dtype must be bf16 or fp16 (got %d)", dtype);
+  if (!multi_lora_fits(tokens, k, n, rank, batch) || adapters < 1 || adapters >= (1 << 24) ||
+      x_stride < k || x_stride % 8 || y_add_stride < n || y_add_stride % 8 || (!q_start && tokens % batch))
+    return fail(FITQ_ERR_SHAPE, "multi_lora: bad shape (tokens=%lld k=%lld n=%lld adapters=%d batch=%d strides %lld, %lld)",
+                (long long)tokens, (long long)k, (long long)n, adapters, batch, (long long)x_stride, (long long)y_add_stride);
+  if (tokens == 0) return FITQ_OK;
+  if (!x || !a || !b || !scale || !adapter || !y_add || !y || !workspace)
+    return fail(FITQ_ERR_ARG, "multi_lora: NULL tensor or workspace");
+  if (!al16(x) || !al16(a) || !al16(b) || !al16(y_add) || !al16(y) || !al16(workspace))
+    return fail(FITQ_ERR_ALIGN, "multi_lora: 16-byte alignment");
+  if ((reinterpret_cast<uintptr_t>(scale) | reinterpret_cast<uintptr_t>(adapter) | reinterpret_cast<uintptr_t>(q_start)) & 3u)
+    return fail(FITQ_ERR_ALIGN, "multi_lora: scale, adapter and q_start must be 4-byte aligned");
+  if (!(y == y_add && y_add_stride == n) && kv4_meets(y, tokens * n * 2, y_add, tokens, y_add_stride, n))
+    return fail(FITQ_ERR_ARG, "multi_lora: y overlaps y_add, other than being y_add of dense rows");
+  if (kv4_meets(y, tokens * n * 2, x, tokens, x_stride, k)) return fail(FITQ_ERR_ARG, "multi_lora: y overlaps x");
+  int rc;
+  const int sms = current_sms(&rc);
+  if (!sms) return rc;
+  const size_t need = fitq::multi_lora_workspace(tokens, k, n, rank, batch, sms);
+  if (workspace_bytes < need)
+    return fail(FITQ_ERR_WORKSPACE, "multi_lora: workspace %zu < %zu bytes", workspace_bytes, need);
+  return launch_status(fitq::launch_multi_lora(x, x_stride, tokens, k, n, a, b, rank, adapters, scale, adapter, q_start,
+                                               batch, y_add, y_add_stride, y, dtype, workspace, status_ptr(),
+                                               static_cast<cudaStream_t>(stream), sms),
+                       "multi_lora");
 }
 
 }  // extern "C"

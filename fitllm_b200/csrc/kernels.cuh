@@ -364,6 +364,32 @@ int launch_token_logprobs_bwd(const void* logits, int dtype, const int64_t* ids,
                               const int64_t* top_ids, const float* g_logp, const float* g_entropy,
                               const float* g_top, void* d, cudaStream_t st);
 
+// Trees of drafted tokens: append, keep (tree.cu), attention (tree_attn.cu), verification
+// (tree_verify.cu).  Shapes checked by the caller; what only the device sees is recorded
+// in *status and skipped.
+struct TreeView;
+int launch_tree_append(const TreeView& tree, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                       const void* v, int64_t v_stride, void* q_out, void* k_cache, void* v_cache, const float* cs,
+                       const float* sn, int rope_len, int heads, int dim, int dtype, int* status, cudaStream_t st);
+int launch_tree_keep(const TreeView& tree, void* const* k_caches, void* const* v_caches, int layers, int dim,
+                     const int32_t* path, const int64_t* accepted, int32_t* lengths, int* status, cudaStream_t st);
+size_t tree_attention_workspace(const TreeView& tree, int heads, int dim, int num_sms);
+int launch_tree_attention(const TreeView& tree, const void* q, int64_t q_stride, const void* k_cache,
+                          const void* v_cache, void* out, int heads, int dim, int dtype, void* workspace, int* status,
+                          cudaStream_t st, int num_sms);
+int launch_tree_verify(const void* logits, int dtype, int64_t stride_b, int64_t stride_t, int64_t batch, int tokens,
+                       int64_t vocab, const int64_t* ids, const int32_t* parents, int64_t parents_stride,
+                       const float* uniforms, const float* probs, int64_t probs_stride_b, int64_t probs_stride_t,
+                       const float* temperatures, float temperature, int32_t* path, int64_t* accepted,
+                       int64_t* next_token, int* status, cudaStream_t st, int num_sms);
+
+// Low-rank adapters of many requests beside a shared projection (multi_lora.cu).
+size_t multi_lora_workspace(int64_t tokens, int64_t k, int64_t n, int rank, int batch, int num_sms);
+int launch_multi_lora(const void* x, int64_t x_stride, int64_t tokens, int64_t k, int64_t n, const void* a,
+                      const void* b, int rank, int adapters, const float* scale, const int32_t* adapter,
+                      const int32_t* q_start, int batch, const void* y_add, int64_t y_add_stride, void* y, int dtype,
+                      void* workspace, int* status, cudaStream_t st, int num_sms);
+
 // Optimizer kernels (optim.cu).
 int launch_adamw(float* p, const float* g, float* m, float* v, int64_t n, float lr, float b1,
                  float b2, float eps, float wd, int step, const float* clip, cudaStream_t st);

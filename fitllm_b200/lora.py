@@ -11,15 +11,19 @@ one fused QLoRA call on the sm_100a kernels (the adapter is handed over as the
 transposed views A^T [r, in] and B^T [out, r]).  A dense ``nn.Linear`` base
 (the reference's unquantised test models) keeps the reference's plain torch
 arithmetic, since there is no NF4 weight to stream.
+
+``MultiLoRAManager`` serves many trained adapters on one model: each sequence of a
+batch takes its own (``MultiLoRALinear``, ops.multi_lora).
 """
 from __future__ import annotations
 
 import logging
-from typing import Dict, Iterator, List, Tuple
+from typing import Dict, Iterator, List, Optional, Tuple
 
 import torch
 import torch.nn as nn
 
+from . import ops
 from .qlora import Linear4bit, _QLoRAFunction
 
 logger = logging.getLogger(__name__)
@@ -111,3 +115,142 @@ class LoRAManager:
     @property
     def num_lora_layers(self) -> int:
         return len(self._lora_layers)
+
+
+class AdapterRoute:
+    """Which adapter slot each sequence of the running batch uses: ``adapter`` int32 [batch]
+    (-1: none) and ``q_start`` int32 [batch + 1] of packed tokens, or None where every
+    sequence has as many.  Shared by the layers of a MultiLoRAManager."""
+
+    def __init__(self) -> None:
+        self.adapter: Optional[torch.Tensor] = None
+        self.q_start: Optional[torch.Tensor] = None
+
+
+class MultiLoRALinear(nn.Module):
+    """An NF4 Linear4bit with ``slots`` adapters of rank up to ``rank``, one per sequence:
+    forward(x) = base(x) + scaling[l] (x.A_l^T).B_l^T, l = the sequence's slot in ``route``.
+    The adapters are held in bf16 as the kernels read them, A [slots, rank, in] and B [slots,
+    out, rank].  For serving: there is no gradient."""
+
+    def __init__(self, base_layer: Linear4bit, slots: int, rank: int, route: AdapterRoute) -> None:
+        super().__init__()
+        if rank not in (16, 32, 48, 64):
+            raise ValueError(f"rank {rank} unsupported (kernels take 16, 32, 48 or 64; smaller adapters are padded)")
+        if slots < 1:
+            raise ValueError(f"MultiLoRALinear: slots={slots}")
+        if base_layer.in_features % 8 or base_layer.out_features % 8:
+            raise ValueError("MultiLoRALinear: in_features and out_features must be multiples of 8")
+        self.base_layer, self.slots, self.rank, self.route = base_layer, slots, rank, route
+        dev = base_layer.weight.device
+        self.register_buffer("lora_A", torch.zeros(slots, rank, base_layer.in_features, dtype=torch.bfloat16, device=dev))
+        self.register_buffer("lora_B", torch.zeros(slots, base_layer.out_features, rank, dtype=torch.bfloat16, device=dev))
+        self.register_buffer("scaling", torch.zeros(slots, dtype=torch.float32, device=dev))
+
+    @property
+    def in_features(self) -> int:
+        return self.base_layer.in_features
+
+    @property
+    def out_features(self) -> int:
+        return self.base_layer.out_features
+
+    @torch.no_grad()
+    def load(self, slot: int, lora_a: torch.Tensor, lora_b: torch.Tensor, scaling: float) -> None:
+        """Adapter A [r, in], B [out, r] (PEFT layout, r <= rank) into a slot."""
+        r = lora_a.shape[0]
+        if not 0 <= slot < self.slots:
+            raise IndexError(f"slot {slot} of {self.slots}")
+        if r > self.rank or lora_a.shape != (r, self.in_features) or lora_b.shape != (self.out_features, r):
+            raise ValueError(f"adapter {tuple(lora_a.shape)}, {tuple(lora_b.shape)} does not fit [<= {self.rank}, "
+                             f"{self.in_features}], [{self.out_features}, .]")
+        self.unload(slot)
+        self.lora_A[slot, :r].copy_(lora_a)
+        self.lora_B[slot, :, :r].copy_(lora_b)
+        self.scaling[slot] = float(scaling)
+
+    @torch.no_grad()
+    def unload(self, slot: int) -> None:
+        self.lora_A[slot].zero_()
+        self.lora_B[slot].zero_()
+        self.scaling[slot] = 0.0
+
+    @torch.no_grad()
+    def add_adapters(self, x2: torch.Tensor, y2: torch.Tensor) -> torch.Tensor:
+        """y2 [tokens, out] (bf16, written over) plus the adapters of x2 [tokens, in]."""
+        route = self.route
+        if route.adapter is None:
+            return y2
+        return ops.multi_lora(x2, self.lora_A, self.lora_B, self.scaling, route.adapter, y2, q_start=route.q_start, out=y2)
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        y = self.base_layer(x, residual=residual)
+        y2 = self.add_adapters(ops._bf16_2d(x, self.in_features), ops._bf16_2d(y, self.out_features))
+        return y2.view(y.shape).to(y.dtype)
+
+    def extra_repr(self) -> str:
+        return f"slots={self.slots}, rank={self.rank}"
+
+
+class MultiLoRAManager:
+    """Adapters of many requests on one model: ``apply`` wraps the target Linear4bit modules,
+    ``load`` puts a trained adapter (PEFT names, as QLoRAManager saves them) into a slot, ``route``
+    says which sequence of the next passes uses which slot."""
+
+    def __init__(self, slots: int, rank: int = 16,
+                 targets: Tuple[str, ...] = ("q_proj", "k_proj", "v_proj", "o_proj")) -> None:
+        self.slots, self.rank, self.targets = slots, rank, tuple(targets)
+        self.routing = AdapterRoute()
+        self.layers: Dict[str, MultiLoRALinear] = {}
+
+    def apply(self, model: nn.Module) -> nn.Module:
+        """Wraps every Linear4bit whose name is, or ends with, a target."""
+        for mod_name, mod in list(model.named_modules()):
+            for child_name, child in list(mod.named_children()):
+                full = f"{mod_name}.{child_name}" if mod_name else child_name
+                if isinstance(child, Linear4bit) and any(full == t or full.endswith("." + t) for t in self.targets):
+                    layer = MultiLoRALinear(child, self.slots, self.rank, self.routing)
+                    setattr(mod, child_name, layer)
+                    self.layers[full] = layer
+        return model
+
+    def load(self, slot: int, state: Dict[str, torch.Tensor], alpha: float) -> int:
+        """A state dict with ``...<module>.lora_A(.default).weight`` and ``lora_B`` keys into a
+        slot, scaled by alpha / r; returns how many projections it covers, and raises, changing
+        nothing, where a pair is incomplete or none matches.  Projections it does not name have none."""
+        pairs: Dict[str, Dict[str, torch.Tensor]] = {}
+        for key, t in state.items():
+            for part in ("lora_A", "lora_B"):
+                if f".{part}." in key:
+                    pairs.setdefault(key.split(f".{part}.")[0], {})[part] = t
+        found = {}
+        for name, layer in self.layers.items():
+            hits = [m for m in pairs if m == name or m.endswith("." + name)]
+            if len(hits) > 1 or (hits and len(pairs[hits[0]]) != 2):
+                raise ValueError(f"adapter state: {name} has no single pair of lora_A and lora_B")
+            if hits:
+                a, b = pairs[hits[0]]["lora_A"], pairs[hits[0]]["lora_B"]
+                r = a.shape[0]
+                if r > layer.rank or a.shape != (r, layer.in_features) or b.shape != (layer.out_features, r):
+                    raise ValueError(f"adapter state: {name} has shapes {tuple(a.shape)}, {tuple(b.shape)}")
+                found[name] = (a, b)
+        if not found:
+            raise ValueError("adapter state: no key names a wrapped projection")
+        for name, layer in self.layers.items():
+            if name in found:
+                a, b = found[name]
+                layer.load(slot, a, b, alpha / a.shape[0])
+            else:
+                layer.unload(slot)
+        return len(found)
+
+    def unload(self, slot: int) -> None:
+        for layer in self.layers.values():
+            layer.unload(slot)
+
+    def route(self, adapter: Optional[torch.Tensor], q_start: Optional[torch.Tensor] = None) -> None:
+        """adapter int32 [batch] slots on the model's device (-1: none), or None: no adapters."""
+        if adapter is not None and (adapter.dtype != torch.int32 or adapter.dim() != 1):
+            raise ValueError("route: adapter must be int32 [batch]")
+        self.routing.adapter, self.routing.q_start = adapter, q_start

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-from typing import List, Optional, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -376,6 +376,234 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
         _lib.check(L.fitq_kv4_attention(c, q.data_ptr(), q.stride(0), out.data_ptr(), q.shape[1],
                                         _KV4_DTYPES[q.dtype], max_new, max_len, ws.data_ptr(), nbytes,
                                         _raw_stream(dev.index)), "fitq_kv4_attention")
+    return out
+
+
+def _serving_only(what: str, *tensors) -> None:
+    """Refuses tensors whose gradient the call would lose."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError(f"{what}: an input requires a gradient, which this call does not have "
+                                  "(use torch.no_grad())")
+
+
+def _tree_parents(what: str, parents: torch.Tensor, batch: int, t: int, dev) -> int:
+    """Entries from sequence to sequence of parents int32 [batch, t], or 0 of [t]."""
+    shape = tuple(parents.shape)
+    if parents.dtype != torch.int32 or shape not in ((batch, t), (t,)) or (t > 1 and parents.stride(-1) != 1):
+        raise ValueError(f"{what}: parents must be int32 [{batch}, {t}] or [{t}] with dense rows (got {parents.dtype} "
+                         f"{shape})")
+    if parents.device != dev:
+        raise ValueError(f"{what}: parents is on {parents.device}, not on {dev}")
+    if len(shape) == 1 or batch == 1:
+        return 0
+    if 0 < parents.stride(0) < t:
+        raise ValueError(f"{what}: rows of parents overlap")
+    return parents.stride(0)
+
+
+def _tree_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix: torch.Tensor, parents: torch.Tensor,
+                t: int) -> _lib.TreeC:
+    """The fitq_tree descriptor of a call (its pointers live as long as the tensors)."""
+    dev, shape = k_cache.device, k_cache.shape
+    if k_cache.dtype not in _KV4_DTYPES or len(shape) != 4 or not k_cache.is_cuda:
+        raise ValueError(f"{what}: caches must be bf16 or fp16 CUDA tensors [batch, kv_heads, capacity, head_dim]")
+    if v_cache.shape != shape or v_cache.dtype != k_cache.dtype or v_cache.device != dev:
+        raise ValueError(f"{what}: k_cache and v_cache differ in shape, dtype or device")
+    batch, kv_heads, cap, d = shape
+    strides = k_cache.stride()
+    if v_cache.stride() != strides:
+        raise ValueError(f"{what}: k_cache and v_cache differ in strides")
+    sb, sh, sp = (s if n > 1 else 0 for s, n in zip(strides[:3], shape))
+    sp = sp if cap > 1 else d
+    if strides[3] != 1 or sp < d or (sb | sh | sp) % 8 or (sb == 0 and batch > 1) or (sh == 0 and kv_heads > 1) \
+            or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise ValueError(f"{what}: caches need dense heads, strides in multiples of 8 elements and 16-byte alignment "
+                         f"(got strides {strides})")
+    if prefix.dtype != torch.int32 or prefix.shape != (batch,) or not prefix.is_contiguous() or prefix.device != dev:
+        raise ValueError(f"{what}: prefix must be contiguous int32 [{batch}] on {dev}")
+    ps = _tree_parents(what, parents, batch, t, dev)
+    return _lib.TreeC(parents.data_ptr(), prefix.data_ptr(), ps, cap, sb, sh, sp, batch, t, kv_heads, d,
+                      _KV4_DTYPES[k_cache.dtype])
+
+
+def _tree_tokens(what: str, name: str, x: torch.Tensor, heads: Optional[int], cache: torch.Tensor,
+                 t: int) -> torch.Tensor:
+    """x [batch, t, heads, head_dim] whose tokens follow one another at one stride, heads dense."""
+    shape, d = x.shape, cache.shape[3]
+    if len(shape) != 4 or shape[0] != cache.shape[0] or shape[1] != t or shape[3] != d or shape[2] == 0 \
+            or (heads is not None and shape[2] != heads):
+        raise ValueError(f"{what}: {name} has shape {tuple(shape)}")
+    if x.dtype != cache.dtype or x.device != cache.device:
+        raise ValueError(f"{what}: {name} must be {cache.dtype} on {cache.device} like the caches (got {x.dtype} on "
+                         f"{x.device})")
+    s0, s1, s2, s3 = x.stride()
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x
+    if t == 1:
+        s1 = s0
+    if s3 != 1 or s2 != d or s1 % 8 or s1 < shape[2] * d or (shape[0] > 1 and s0 != t * s1) or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _token_stride(x: torch.Tensor) -> int:
+    """Elements from token to token of what _tree_tokens gives."""
+    b, t, h, d = x.shape
+    return x.stride(1) if t > 1 else x.stride(0) if b > 1 else h * d
+
+
+def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                prefix: torch.Tensor, parents: torch.Tensor, cos_half: torch.Tensor, sin_half: torch.Tensor,
+                q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotate a tree's q and k and write its k and v to the cache (fitq_tree_append).
+
+    q [B, T, heads, D], k, v [B, T, kv_heads, D] and the caches [B, kv_heads, capacity, D]
+    of one dtype (bf16 or fp16; tokens and caches may be strided); prefix int32 [B]: cached
+    positions; parents int32 [B, T] or [T]: a token's parent, -1 for one right behind the
+    cached positions, -2 for no token.  Token i goes to slot prefix + i and is rotated at
+    position prefix + depth with row prefix + depth of cos_half, sin_half fp32 [positions,
+    D / 2].  Returns the rotated q [B, T, heads, D] (into q_out when given; absent tokens: zeros)."""
+    L = _lib.load()
+    _serving_only("tree_append", q, k, v, k_cache, v_cache)
+    t = q.shape[1] if q.dim() == 4 else 0
+    c = _tree_cache("tree_append", k_cache, v_cache, prefix, parents, t)
+    dev = k_cache.device
+    q = _tree_tokens("tree_append", "q", q, None, k_cache, t)
+    k = _tree_tokens("tree_append", "k", k, c.kv_heads, k_cache, t)
+    v = _tree_tokens("tree_append", "v", v, c.kv_heads, k_cache, t)
+    rows = cos_half.shape
+    if len(rows) != 2 or rows[1] * 2 != c.head_dim or sin_half.shape != rows:
+        raise ValueError(f"tree_append: cos_half and sin_half must be of one shape [positions, {c.head_dim // 2}]")
+    for name, x in (("cos_half", cos_half), ("sin_half", sin_half)):
+        if x.dtype != torch.float32 or not x.is_contiguous() or x.device != dev or x.data_ptr() % 16:
+            raise ValueError(f"tree_append: {name} must be contiguous, 16-byte aligned fp32 on {dev}")
+    out = _kv4_out("tree_append", "q_out", q_out, q)
+    with _on(dev):
+        _lib.check(L.fitq_tree_append(c, q.data_ptr(), _token_stride(q), k.data_ptr(), _token_stride(k), v.data_ptr(),
+                                      _token_stride(v), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                      cos_half.data_ptr(), sin_half.data_ptr(), rows[0], q.shape[2],
+                                      _raw_stream(dev.index)), "fitq_tree_append")
+    return out
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix: torch.Tensor,
+                   parents: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a tree of drafted tokens over a cache (fitq_tree_attention).
+
+    q [B, T, heads, D], rotated, the tree's keys and values in the cache's slots
+    [prefix, prefix + T) (tree_append; arguments as there): token i sees the cached
+    positions, its ancestors and itself.  Returns [B, T, heads, D] (into out when given;
+    absent tokens: zeros)."""
+    L = _lib.load()
+    _serving_only("tree_attention", q, k_cache, v_cache)
+    t = q.shape[1] if q.dim() == 4 else 0
+    c = _tree_cache("tree_attention", k_cache, v_cache, prefix, parents, t)
+    dev = k_cache.device
+    q = _tree_tokens("tree_attention", "q", q, None, k_cache, t)
+    out = _kv4_out("tree_attention", "out", out, q)
+    with _on(dev):
+        nbytes = L.fitq_tree_attention_workspace(c, q.shape[2])
+        ws = _workspace(nbytes, dev)
+        _lib.check(L.fitq_tree_attention(c, q.data_ptr(), _token_stride(q), k_cache.data_ptr(), v_cache.data_ptr(),
+                                         out.data_ptr(), q.shape[2], ws.data_ptr(), nbytes, _raw_stream(dev.index)),
+                   "fitq_tree_attention")
+    return out
+
+
+def tree_keep(k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor], prefix: torch.Tensor,
+              path: torch.Tensor, accepted: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The accepted path of a tree stays in the caches of all layers (fitq_tree_keep): slot
+    prefix + path[b, i] moves to prefix + i for i <= accepted[b].  path int32 [B, T], accepted
+    int64 [B] as verify.verify_tree gives them.  Returns prefix + accepted + 1 as int32 [B] (into
+    lengths when given, which may be prefix)."""
+    L = _lib.load()
+    if not k_caches or len(k_caches) != len(v_caches):
+        raise ValueError(f"tree_keep: {len(k_caches)} key and {len(v_caches)} value caches")
+    first = k_caches[0]
+    if path.dim() != 2 or path.dtype != torch.int32 or not path.is_contiguous() or path.device != first.device \
+            or path.shape[0] != first.shape[0]:
+        raise ValueError("tree_keep: path must be contiguous int32 [batch, T] on the caches' device")
+    batch, t = path.shape
+    if accepted.dtype != torch.int64 or accepted.shape != (batch,) or not accepted.is_contiguous() \
+            or accepted.device != first.device:
+        raise ValueError(f"tree_keep: accepted must be contiguous int64 [{batch}] on the caches' device")
+    c = _tree_cache("tree_keep", first, v_caches[0], prefix, path, t)
+    for x in (*k_caches, *v_caches):
+        if x.shape != first.shape or x.stride() != first.stride() or x.dtype != first.dtype or x.device != first.device:
+            raise ValueError("tree_keep: the layers' caches must be of one shape, stride, dtype and device")
+    if lengths is None:
+        lengths = torch.empty_like(prefix)
+    elif lengths.dtype != torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous() \
+            or lengths.device != first.device:
+        raise ValueError(f"tree_keep: lengths must be contiguous int32 [{batch}] on the caches' device")
+    n = len(k_caches)
+    array = ctypes.c_void_p * n
+    with _on(first.device):
+        _lib.check(L.fitq_tree_keep(c, array(*[x.data_ptr() for x in k_caches]), array(*[x.data_ptr() for x in v_caches]),
+                                    n, path.data_ptr(), accepted.data_ptr(), lengths.data_ptr(),
+                                    _raw_stream(first.device.index)), "fitq_tree_keep")
+    return lengths
+
+
+def _lora_rows(x: torch.Tensor, cols: int) -> torch.Tensor:
+    """x [tokens, cols] with dense, aligned rows (the row stride is free)."""
+    if x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < cols)) or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scale: torch.Tensor, adapter: torch.Tensor,
+               y: torch.Tensor, q_start: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Adapters of many requests beside a shared projection (fitq_multi_lora):
+    y[n] + scale[l] (x[n].A_l^T).B_l^T with l = adapter[sequence of token n].
+
+    x [tokens, K], y [tokens, N] (the shared projection of x; rows may be strided), lora_a
+    [adapters, R, K], lora_b [adapters, N, R], all bf16 or all fp16, R 16, 32, 48 or 64;
+    scale fp32 [adapters]; adapter int32 [batch], -1 for none; q_start int32 [batch + 1]
+    (sequence b has the tokens [q_start[b], q_start[b + 1])), or None for tokens / batch
+    each.  Returns [tokens, N] (into out when given, which may be y; rows of no sequence
+    are left as they are there)."""
+    L = _lib.load()
+    _serving_only("multi_lora", x, lora_a, lora_b, scale, y)
+    if x.dim() != 2 or y.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
+        raise ValueError("multi_lora: x and y are [tokens, .], lora_a and lora_b [adapters, ., .]")
+    tokens, k = x.shape
+    n, (n_ad, r) = y.shape[1], lora_a.shape[:2]
+    dev = x.device
+    if lora_a.shape != (n_ad, r, k) or lora_b.shape != (n_ad, n, r) or y.shape[0] != tokens:
+        raise ValueError(f"multi_lora: x {tuple(x.shape)}, y {tuple(y.shape)}, lora_a {tuple(lora_a.shape)} and lora_b "
+                         f"{tuple(lora_b.shape)} do not match")
+    if x.dtype not in _KV4_DTYPES or not x.is_cuda:
+        raise ValueError("multi_lora: x must be a bf16 or fp16 CUDA tensor")
+    for name, t in (("y", y), ("lora_a", lora_a), ("lora_b", lora_b)):
+        if t.dtype != x.dtype or t.device != dev:
+            raise ValueError(f"multi_lora: {name} must be {x.dtype} on {dev} (got {t.dtype} on {t.device})")
+    if not (lora_a.is_contiguous() and lora_b.is_contiguous()):
+        raise ValueError("multi_lora: lora_a and lora_b must be contiguous")
+    if scale.dtype != torch.float32 or scale.shape != (n_ad,) or not scale.is_contiguous() or scale.device != dev:
+        raise ValueError(f"multi_lora: scale must be contiguous fp32 [{n_ad}] on {dev}")
+    if adapter.dtype != torch.int32 or adapter.dim() != 1 or not adapter.is_contiguous() or adapter.device != dev:
+        raise ValueError(f"multi_lora: adapter must be contiguous int32 [batch] on {dev}")
+    batch, start = adapter.shape[0], None
+    if q_start is not None:
+        if q_start.dtype != torch.int32 or q_start.shape != (batch + 1,) or not q_start.is_contiguous() \
+                or q_start.device != dev:
+            raise ValueError(f"multi_lora: q_start must be contiguous int32 [{batch + 1}] on {dev}")
+        start = q_start.data_ptr()
+    if out is None:
+        out = torch.empty(tokens, n, dtype=x.dtype, device=dev)
+    elif out.shape != (tokens, n) or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"multi_lora: out must be a contiguous {x.dtype} tensor {(tokens, n)} on {dev}")
+    x, y = _lora_rows(x, k), _lora_rows(y, n)
+    with _on(dev):
+        nbytes = L.fitq_multi_lora_workspace(tokens, k, n, r, batch)
+        ws = _workspace(nbytes, dev)
+        _lib.check(L.fitq_multi_lora(x.data_ptr(), x.stride(0) if tokens > 1 else k, tokens, k, n, lora_a.data_ptr(),
+                                     lora_b.data_ptr(), r, n_ad, scale.data_ptr(), adapter.data_ptr(), start, batch,
+                                     y.data_ptr(), y.stride(0) if tokens > 1 else n, out.data_ptr(),
+                                     _KV4_DTYPES[x.dtype], ws.data_ptr(), nbytes, _raw_stream(dev.index)),
+                   "fitq_multi_lora")
     return out
 
 

@@ -25,6 +25,11 @@ one the rotation, the coding and the append are one launch (fitq_kv4_append)
 and attention reads the codes (fitq_kv4_attention) for single tokens, drafts and
 prompts alike.  ``score_drafts`` turns the pass's hidden states into the drafts'
 log probabilities, the model's alternatives and the number of drafts it accepts.
+
+``TreeKVCache`` is the step for trees of drafted tokens: a bf16 or fp16 cache whose lengths
+live on the device.  ``tree_pass`` runs the layers over a tree per sequence (ops.tree_append,
+ops.tree_attention), ``verify_tree`` accepts drafts against the model's probabilities by
+given random numbers, and ``TreeKVCache.keep`` leaves the accepted path in the cache.
 """
 from __future__ import annotations
 
@@ -33,11 +38,11 @@ from typing import List, NamedTuple, Optional, Sequence, Tuple
 import torch
 import torch.nn.functional as F
 
-from . import ops
+from . import _lib, ops
 from .layer import DecoderLayer, rotary_tables
 from .layer_ops import rope_kv_append, swiglu
-from .lm_head import LMHeadLoss, token_logprobs
-from .qlora import QLoRALinear4bit, grouped_forward, swiglu_forward
+from .lm_head import _LOGIT_DTYPES, LMHeadLoss, token_logprobs
+from .qlora import Linear4bit, grouped_forward, swiglu_forward
 
 
 class KVCache:
@@ -185,8 +190,7 @@ def _layer_forward(layer: DecoderLayer, h: torch.Tensor, attend) -> torch.Tensor
     h1 = attn.o_proj(attend(q_raw, k_raw, v_raw), residual=h)
     mlp = layer.mlp
     x2 = layer.post_attention_layernorm(h1)
-    if grouped and not isinstance(mlp.gate_proj, QLoRALinear4bit) and not isinstance(mlp.up_proj,
-                                                                                       QLoRALinear4bit):
+    if grouped and isinstance(mlp.gate_proj, Linear4bit) and isinstance(mlp.up_proj, Linear4bit):
         act = swiglu_forward(mlp.gate_proj, mlp.up_proj, x2)  # gate/up/SwiGLU, one GEMM + one finish
     else:
         gate, up = grouped_forward([mlp.gate_proj, mlp.up_proj], x2) if grouped else (
@@ -313,3 +317,126 @@ def score_drafts(head: LMHeadLoss, h: torch.Tensor, drafts: torch.Tensor, top: i
     accepted = (first[:, :-1] == ids[:, :-1]).long().cumprod(dim=1).sum(dim=1)
     return DraftScores(r.logp[:, :-1], r.entropy, r.top_logp, r.top_ids, accepted,
                        first.gather(1, accepted[:, None])[:, 0])
+
+
+class TreeVerdict(NamedTuple):
+    """path int32 [B, T] (token 0 and the accepted drafts in order, then -1), accepted int64 [B]
+    (how many drafts; -1 for a sequence without a token) and next_token int64 [B]."""
+    path: torch.Tensor
+    accepted: torch.Tensor
+    next_token: torch.Tensor
+
+
+@torch.no_grad()
+def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, uniforms: torch.Tensor,
+                draft_probs: Optional[torch.Tensor] = None, temperature=1.0) -> TreeVerdict:
+    """Drafted tokens against the model's probabilities, from given random numbers
+    (fitq_tree_verify): accepted and next tokens are a sample of softmax(logits /
+    temperature), whatever was drafted.
+
+    logits [B, T, V] bf16, fp16 or fp32 (rows may be strided), row i behind token i; tokens
+    [B, T] integers; parents int32 [B, T] or [T] as in ops.tree_append (a chain: chain_parents);
+    token 0, with parent -1, is the last one that is certain.  uniforms fp32 [B, T] in [0, 1).
+    draft_probs [B, T - 1 or more, V]: row i the distribution that token i's children were
+    drawn from; None where they are a model's choice.  temperature: a number, or fp32 [B]; 0
+    takes the largest logit."""
+    L = _lib.load()
+    if logits.dim() != 3 or logits.dtype not in _LOGIT_DTYPES or not logits.is_cuda:
+        raise ValueError("verify_tree: logits must be a bf16, fp16 or fp32 CUDA tensor [batch, T, vocab]")
+    b, t, vocab = logits.shape
+    dev = logits.device
+    if tokens.shape != (b, t) or tokens.dtype.is_floating_point or tokens.dtype == torch.bool or tokens.device != dev:
+        raise ValueError(f"verify_tree: tokens must be integers [{b}, {t}] on {dev}")
+    if uniforms.shape != (b, t) or uniforms.dtype != torch.float32 or uniforms.device != dev:
+        raise ValueError(f"verify_tree: uniforms must be fp32 [{b}, {t}] on {dev}")
+    ps = ops._tree_parents("verify_tree", parents, b, t, dev)
+    if (vocab > 1 and logits.stride(2) != 1) or (t > 1 and logits.stride(1) < vocab):
+        logits = logits.contiguous()
+    tokens, uniforms = tokens.to(torch.int64).contiguous(), uniforms.contiguous()
+    q, qb, qt = None, 0, vocab
+    if draft_probs is not None:
+        shape = draft_probs.shape
+        if len(shape) != 3 or shape[0] != b or shape[1] < t - 1 or shape[2] != vocab or draft_probs.device != dev \
+                or not draft_probs.dtype.is_floating_point:
+            raise ValueError(f"verify_tree: draft_probs must be [{b}, {t - 1}, {vocab}] on {dev}")
+        q = draft_probs.float()
+        if (vocab > 1 and q.stride(2) != 1) or (shape[1] > 1 and q.stride(1) < vocab):
+            q = q.contiguous()
+        qb, qt = (q.stride(0) if b > 1 else 0), (q.stride(1) if shape[1] > 1 else vocab)
+    temps, temp = None, 0.0
+    if isinstance(temperature, torch.Tensor):
+        if temperature.shape != (b,) or temperature.dtype != torch.float32 or temperature.device != dev:
+            raise ValueError(f"verify_tree: temperature must be a number or fp32 [{b}] on {dev}")
+        temps = temperature.contiguous()
+    else:
+        temp = float(temperature)
+    r = TreeVerdict(torch.empty(b, t, dtype=torch.int32, device=dev), torch.empty(b, dtype=torch.int64, device=dev),
+                    torch.empty(b, dtype=torch.int64, device=dev))
+    with ops._on(dev):
+        _lib.check(L.fitq_tree_verify(logits.data_ptr(), _LOGIT_DTYPES[logits.dtype], logits.stride(0) if b > 1 else 0,
+                                      logits.stride(1) if t > 1 else vocab, b, t, vocab, tokens.data_ptr(),
+                                      parents.data_ptr(), ps, uniforms.data_ptr(), _lib.ptr(q), qb, qt, _lib.ptr(temps),
+                                      temp, r.path.data_ptr(), r.accepted.data_ptr(), r.next_token.data_ptr(),
+                                      ops._raw_stream(dev.index)), "fitq_tree_verify")
+    return r
+
+
+def chain_parents(t: int, device) -> torch.Tensor:
+    """The tree of T tokens in a row: int32 [t], each the child of the one before."""
+    return torch.arange(-1, t - 1, dtype=torch.int32, device=device)
+
+
+class TreeKVCache(KVCache):
+    """A KVCache whose sequences have lengths of their own, on the device (``prefix`` int32
+    [B]), for passes over trees of drafted tokens: ``tree_pass`` writes a tree's tokens behind
+    the lengths without moving them, ``keep`` accepts a path (no copy to the host: a step of
+    both can be captured and replayed).  rope_theta: the layers' rotary base (a pass refuses
+    layers of another one)."""
+
+    def __init__(self, num_layers: int, batch: int, kv_heads: int, head_dim: int, capacity: int, device,
+                 dtype=torch.bfloat16, rope_theta: float = 1e6):
+        if head_dim not in (64, 128):
+            raise ValueError(f"TreeKVCache: head_dim must be 64 or 128 (got {head_dim})")
+        super().__init__(num_layers, batch, kv_heads, head_dim, capacity, device, dtype)
+        self.rope_theta = rope_theta
+        self.prefix = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.tables = rotary_tables(capacity, head_dim, rope_theta, device)
+
+    @property
+    def batch(self) -> int:
+        return self.prefix.shape[0]
+
+    def keep(self, verdict: TreeVerdict) -> None:
+        """The verdict's path stays behind each sequence's length, in all layers."""
+        ops.tree_keep(self.k, self.v, self.prefix, verdict.path, verdict.accepted, lengths=self.prefix)
+
+    def release(self, b: int) -> None:
+        """Sequence b is done: its length is 0."""
+        self.prefix[b] = 0
+
+
+@torch.no_grad()
+def tree_pass(layers: List[DecoderLayer], h: torch.Tensor, cache: TreeKVCache, parents: torch.Tensor) -> torch.Tensor:
+    """All layers over the trees h [B, T, hidden] behind the cache's lengths; returns the final
+    hidden states.  parents int32 [B, T] or [T]; layers whose projections carry adapters of many
+    requests (lora.MultiLoRAManager) take each sequence's own."""
+    b, t, _ = h.shape
+    if b != cache.batch or len(layers) != len(cache.k):
+        raise ValueError(f"tree_pass: {b} sequences and {len(layers)} layers, the cache has {cache.batch} and {len(cache.k)}")
+    for layer in layers:
+        if layer.cfg.rope_theta != cache.rope_theta:
+            raise ValueError(f"tree_pass: the layer's rope_theta is {layer.cfg.rope_theta:g}, the cache's "
+                             f"{cache.rope_theta:g}")
+    cos, sin = cache.tables
+    for layer, k_cache, v_cache in zip(layers, cache.k, cache.v):
+        cfg = layer.cfg
+
+        def attend(q_raw, k_raw, v_raw):
+            q, k, v = (x.view(b, t, n, cfg.head_dim) for x, n in ((q_raw, cfg.heads), (k_raw, cfg.kv_heads),
+                                                                  (v_raw, cfg.kv_heads)))
+            q = ops.tree_append(q, k, v, k_cache, v_cache, cache.prefix, parents, cos, sin)
+            o = ops.tree_attention(q, k_cache, v_cache, cache.prefix, parents)
+            return o.view(b, t, cfg.heads * cfg.head_dim)
+
+        h = _layer_forward(layer, h, attend)
+    return h

@@ -422,6 +422,105 @@ FITQ_API int fitq_token_logprobs_bwd(const void* logits, int dtype, const int64_
                                      const float* g_logp, const float* g_entropy,
                                      const float* g_top, void* d, fitq_stream_t stream);
 
+/* A tree of drafted tokens behind a 16-bit key/value cache whose sequences have lengths of
+ * their own.  No counterpart in the reference, whose drafts are a chain and re-run the whole
+ * context (fitllm/inference.py:380-397).
+ *   parents:  int32 [batch, tokens] (or [tokens], parents_stride 0: one tree for all): the
+ *             index of a token's parent, below the token's own; -1 for a token right behind
+ *             the cached positions; -2 where there is no token;
+ *   prefix:   int32 [batch], cached positions of each sequence;
+ *   caches:   [batch, kv_heads, capacity, head_dim] of dtype (FITQ_DTYPE_BF16 or _F16) with
+ *             the given strides (elements, multiples of 8; head_dim elements are dense), one
+ *             set for keys and values, 16-byte aligned.
+ * 1 <= tokens <= 64, head_dim 64 or 128, capacity at most 2^30.  Token i stands in slot
+ * prefix + i and sees the cached positions, its ancestors and itself.
+ * What only the device sees is checked there: another parent, a negative prefix, a token
+ * whose slot lies behind the capacity record FITQ_ERR_ARG (fitq_get_device_status); such a
+ * token, and one with an ancestor that is absent, counts as absent. */
+typedef struct fitq_tree {
+  const int32_t* parents;
+  const int32_t* prefix;
+  int64_t parents_stride;
+  int64_t capacity;
+  int64_t stride_b, stride_h, stride_p;
+  int batch;
+  int tokens;
+  int kv_heads;
+  int head_dim;
+  int dtype;
+} fitq_tree;
+
+/* Rotates the tree's q and k at position prefix + depth (rotate-half, fp32 half tables
+ * cos/sin [rope_len, head_dim / 2]; a token whose position lies behind them is refused like
+ * a slot behind the capacity) and writes k and v to the tokens' slots.  q, q_out
+ * [batch * tokens, heads, head_dim], k, v [batch * tokens, kv_heads, head_dim]; *_stride:
+ * elements from token to token, a multiple of 8.  Absent tokens' queries are zeros, their
+ * slots stay as they are.  q_out may be q when q_stride == heads * head_dim, and overlaps none
+ * of the inputs otherwise. */
+FITQ_API int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_stride, const void* k,
+                              int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
+                              void* k_cache, void* v_cache, const float* cos_half,
+                              const float* sin_half, int rope_len, int heads, fitq_stream_t stream);
+/* Attention of the tree's tokens over the cache, their own slots included (appended before).
+ * q (q_stride as above), out [batch * tokens, heads, head_dim]; query head h reads KV head
+ * h / (heads / kv_heads); scale 1/sqrt(head_dim), fp32 softmax and sums.  An absent token
+ * gives zeros.  Slots that no token sees are not read into any sum, whatever they hold.
+ * Deterministic.  out may be q as above.  The workspace of sizes that no call takes is 0. */
+FITQ_API size_t fitq_tree_attention_workspace(const fitq_tree* tree, int heads);
+FITQ_API int fitq_tree_attention(const fitq_tree* tree, const void* q, int64_t q_stride,
+                                 const void* k_cache, const void* v_cache, void* out, int heads,
+                                 void* workspace, size_t workspace_bytes, fitq_stream_t stream);
+/* The drafted tokens against the model's probabilities.  logits of dtype (bf16, fp16,
+ * fp32): row (b, i) the model's logits behind token i, stride_b and stride_t elements
+ * apart; ids int64 [batch, tokens], parents as above (token 0 with parent -1 is the last token
+ * that is certain); uniforms fp32 [batch, tokens] in [0, 1).  The walk starts at token 0 with
+ * p = softmax(logits / temperature) and tries the token's children in order: child c is
+ * accepted where uniforms[c] * q(id) < p(id), and the walk goes on from it; where it is
+ * refused p becomes max(p - q, 0), normalised.  probs fp32: row (b, i) the distribution q
+ * that token i's children were drawn from, for i < tokens - 1; NULL: q(id) is 1, and a
+ * refusal takes id out of p.  Behind the last child next_token is the first whose cumulated p
+ * exceeds uniforms[0].  An id outside [0, vocab) is refused.  temperature 0: p is 1 at
+ * the largest logit, the lower index where two are equal, and children are compared with it.
+ * temperatures fp32 [batch] or NULL (then `temperature`, not negative).
+ * path int32 [batch, tokens]: token 0 and the accepted ones, then -1; accepted int64 [batch]:
+ * how many drafts; next_token int64 [batch].  A row with a NaN, or without a finite largest logit,
+ * ends the walk with next_token -1; a sequence without token 0 gives accepted -1, next_token
+ * -1.  Sums are fp64; where refusals leave no weight the largest logit's token is next. */
+FITQ_API int fitq_tree_verify(const void* logits, int dtype, int64_t stride_b, int64_t stride_t,
+                              int64_t batch, int tokens, int64_t vocab, const int64_t* ids,
+                              const int32_t* parents, int64_t parents_stride, const float* uniforms,
+                              const float* probs, int64_t probs_stride_b, int64_t probs_stride_t,
+                              const float* temperatures, float temperature, int32_t* path,
+                              int64_t* accepted, int64_t* next_token, fitq_stream_t stream);
+/* The accepted path stays: slot prefix + path[i] moves to slot prefix + i for
+ * i <= accepted in every layer (k_caches, v_caches: host arrays of `layers` device pointers),
+ * lengths[b] = prefix[b] + accepted[b] + 1 (lengths may be prefix).  path, accepted as
+ * fitq_tree_verify writes them; a path that does not ascend within the tree and the capacity
+ * records FITQ_ERR_ARG and leaves its sequence as it was. */
+FITQ_API int fitq_tree_keep(const fitq_tree* tree, void* const* k_caches, void* const* v_caches,
+                            int layers, const int32_t* path, const int64_t* accepted,
+                            int32_t* lengths, fitq_stream_t stream);
+
+/* Low-rank adapters of many requests beside a shared projection (the LoRA term that
+ * PEFT's lora.Linear4bit adds for one adapter, fitllm/qlora.py:74-83):
+ *   y[n] = y_add[n] + scale[l] (x[n].A_l^T).B_l^T,  l = adapter[sequence of token n].
+ * x [tokens, k], y_add [tokens, n] of dtype (bf16 or fp16), *_stride elements from token to
+ * token; y [tokens, n], which may be y_add (y_add_stride == n); a [adapters, rank, k], b
+ * [adapters, n, rank] of dtype, scale fp32 [adapters]; rank 16, 32, 48 or 64 (smaller
+ * adapters padded with zeros); k and n multiples of 8; pointers 16-byte aligned.
+ * adapter int32 [batch], -1: none, y = y_add; an entry that names no adapter records
+ * FITQ_ERR_ARG and counts as -1.  q_start int32 [batch + 1] as in fitq_kv4, or NULL: tokens /
+ * batch each; rows of no sequence are left as they are.  fp32 sums, one rounding of y; x.A^T
+ * enters the second product as two numbers of dtype.  Deterministic.  The workspace of sizes
+ * that no call takes is 0. */
+FITQ_API size_t fitq_multi_lora_workspace(int64_t tokens, int64_t k, int64_t n, int rank, int batch);
+FITQ_API int fitq_multi_lora(const void* x, int64_t x_stride, int64_t tokens, int64_t k, int64_t n,
+                             const void* a, const void* b, int rank, int adapters,
+                             const float* scale, const int32_t* adapter, const int32_t* q_start,
+                             int batch, const void* y_add, int64_t y_add_stride, void* y, int dtype,
+                             void* workspace, size_t workspace_bytes, fitq_stream_t stream);
+
+
 FITQ_API int fitq_swiglu_bwd(const void* d_act, const void* gate, const void* up, void* d_gate,
                              void* d_up, int64_t n, fitq_stream_t stream);
 
