@@ -27,7 +27,7 @@ SOURCES = ["nf4.cu", "gemm_sm100.cu", "lora.cu", "gemv.cu", "optim.cu", "abi.cu"
            "selftest.cu", "gemm_nf4.cu", "gemm_nf4_2cta.cu", "merge.cu", "train_attn.cu", "kv4.cu",
            "kv4_attn.cu", "kv4_prompt.cu", "logprob.cu", "tree.cu", "tree_attn.cu", "tree_verify.cu",
            "multi_lora.cu"]
-HEADERS = ["common.cuh", "kernels.cuh", "pair.cuh", "nf4_decode.cuh", "kv4.cuh", "tree.cuh"]
+HEADERS = ["common.cuh", "kernels.cuh", "pair.cuh", "nf4_decode.cuh", "kv4.cuh", "tree.cuh", "umma_warp.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1594,7 +1594,7 @@ int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_stride, con
 // Whether the attention's tiles can be counted in 31 bits.
 static bool tree_attention_fits(const fitq::TreeView& t, int heads) {
   const int64_t row_tiles = (static_cast<int64_t>(heads / t.kv_heads) * t.tokens + 255) / 256;
-  return row_tiles * t.batch * t.kv_heads * ((t.capacity + 127) / 128 + 1) < (1ll << 31);
+  return row_tiles * t.batch * t.kv_heads * ((t.capacity + 63) / 64 + 1) < (1ll << 31);
 }
 
 size_t fitq_tree_attention_workspace(const fitq_tree* tree, int heads) {

@@ -336,6 +336,31 @@ bool encode_tmap_2d(CUtensorMap* m, CUtensorMapDataType dtype, const void* base,
   return r == CUDA_SUCCESS;
 }
 
+bool encode_tmap_4d(CUtensorMap* m, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[4],
+                    const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4]) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+  const cuuint64_t st[3] = {stride_bytes[0], stride_bytes[1], stride_bytes[2]};
+  const cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]}, es[4] = {1, 1, 1, 1};
+  auto encode = [&] {
+    return fn(m, dtype, 4, const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT && bind_primary_context()) r = encode();
+  if (r != CUDA_SUCCESS) {
+    char msg[256];
+    snprintf(msg, sizeof(msg), "cuTensorMapEncodeTiled = %d (base %p, dims %llu x %llu x %llu x %llu, strides %llu, %llu, %llu B)",
+             static_cast<int>(r), base, static_cast<unsigned long long>(dims[0]), static_cast<unsigned long long>(dims[1]),
+             static_cast<unsigned long long>(dims[2]), static_cast<unsigned long long>(dims[3]),
+             static_cast<unsigned long long>(stride_bytes[0]), static_cast<unsigned long long>(stride_bytes[1]),
+             static_cast<unsigned long long>(stride_bytes[2]));
+    note_launch_detail(msg);
+  }
+  return r == CUDA_SUCCESS;
+}
+
 // Tile width: 256 unless a narrower one finishes the grid in less tile time
 // (waves x width, one CTA per SM); FITQ_GEMM_BN forces one of the built widths.
 int pick_bn(int64_t m, int64_t n, int num_sms) {

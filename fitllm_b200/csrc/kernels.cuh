@@ -219,6 +219,10 @@ bool encode_tmap_2d(CUtensorMap* m, CUtensorMapDataType dtype, const void* base,
                     uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
                     CUtensorMapSwizzle swizzle, CUtensorMapL2promotion l2);
 
+// The same of 4-D tensors of 16-bit elements, innermost dimension first, 128-byte swizzle.
+bool encode_tmap_4d(CUtensorMap* m, CUtensorMapDataType dtype, const void* base, const uint64_t (&dims)[4],
+                    const uint64_t (&stride_bytes)[3], const uint32_t (&box)[4]);
+
 // NF4 skinny GEMM on tcgen05 with the decoded weights in tensor memory
 // (gemv_tc.cu), 8 < M <= 64 (FITQ_GEMV_TC=1: also M <= 8, =0: never);
 // N % 128 == 0, K % 256 == 0, packed weights and x 16-byte aligned.  Writes

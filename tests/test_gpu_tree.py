@@ -79,6 +79,11 @@ CASES = [
     (1, 9, 64, 1, 128, torch.bfloat16, [383], "tree"),       # 576 rows of one KV head
     (65, 3, 4, 2, 64, torch.bfloat16, [(37 * i) % 200 for i in range(65)], "chain"),
     (3, 4, 8, 1, 128, torch.float16, [2049, 0, 4100], "tree"),
+    (150, 1, 1, 1, 128, torch.bfloat16, [255] * 150, "chain"),   # several tiles of a pair per CTA
+    (8, 32, 40, 8, 128, torch.bfloat16, [600 + i for i in range(8)], "tree"),
+    (64, 8, 40, 8, 128, torch.bfloat16, [(97 * i) % 800 for i in range(64)], "tree"),  # several pairs per CTA
+    (64, 7, 20, 4, 64, torch.float16, [(197 * i) % 1800 for i in range(64)], "holes"),
+    (5, 64, 40, 8, 128, torch.float16, [(997 * i) % 3800 for i in range(5)], "tree"),
 ]
 
 
@@ -199,6 +204,25 @@ def test_attention_of_a_long_cache(cuda_dev):
         # factors, so that it enters once more), and tensor-core sums that round towards zero
         tol = 3 * ref.EPS[torch.bfloat16] * (w @ vv.abs())
         assert ((got[s, i, hd].double() - exact).abs() <= tol).all()
+
+
+def test_attention_of_long_runs_in_fp16(cuda_dev):
+    """More steps of a unit than its sums are kept in tensor memory for, many pairs at once."""
+    from fitllm_b200 import ops
+    b, t, h, kvh, d, n = 19, 3, 8, 8, 64, 40_000
+    g = torch.Generator(device=cuda_dev).manual_seed(2)
+    k, v = (torch.empty(b, kvh, n + 8, d, device=cuda_dev, dtype=torch.float16).normal_(generator=g) for _ in range(2))
+    q = torch.randn(b, t, h, d, device=cuda_dev, generator=g).half()
+    q[:, 1] *= 4
+    prefix = torch.full((b,), n, dtype=torch.int32, device=cuda_dev)
+    parents = [[-1, 0, 0]] * b
+    got = ops.tree_attention(q, k, v, prefix, torch.tensor(parents[0], dtype=torch.int32, device=cuda_dev))
+    for s in (0, 7, 18):
+        one = q[s:s + 1], k[s:s + 1], v[s:s + 1], prefix[s:s + 1], parents[:1]
+        exact = ref.attention(*one)
+        err, size = (got[s:s + 1].double() - exact).norm(dim=-1), exact.norm(dim=-1)
+        # the result's rounding and the weights', each at most eps, seldom near it in all 64 elements
+        assert (err <= 2 * ref.EPS[torch.float16] * size + 1e-6).all(), (err / size).max()
 
 
 @pytest.mark.parametrize("dtype,d,shape", [(torch.bfloat16, 128, "tree"), (torch.float16, 64, "holes"),
