@@ -14,8 +14,9 @@
 // tree_attn_combine_kernel joins them in order (deterministic).
 //
 // Roles: warps 0-3 and 4-7 are two softmax units, a thread per row (TMEM lane); warp 8
-// loads K and V tiles by TMA into one ring, warp 9 issues the MMAs, warp 10 cleans the
-// values behind the cached positions.  Per step S = Q.K^T goes to one of two halves of the
+// loads K and V tiles by TMA into one ring, warps 9 and 11 issue the units' MMAs (one warp
+// for both took 3,340 cycles a tile, 1,240 of waits and issues for each unit, where a unit's
+// softmax takes 1,000), warp 10 cleans the values behind the cached positions.  Per step S = Q.K^T goes to one of two halves of the
 // unit's columns of tensor memory, the unit writes P = 2^(S c - m) over it, and O += P.V
 // takes P from there and V as loaded, position by position (an MN-major operand).
 // With one row tile the units take the tiles in turn, each with sums O, m and l of its own
@@ -40,7 +41,7 @@ namespace {
 
 constexpr int kRows = 128;      // rows of a row tile (TMEM lanes)
 constexpr int kStep = 64;       // positions of a tile
-constexpr int kThreads = 352;
+constexpr int kThreads = 384;
 constexpr float kFloor = -3.0e38f;
 constexpr float kRoom = 15.f;   // weights stay below 2^15
 constexpr float kSlack = 8.f;   // a reference that moves leaves this much (log2) to the weights that follow
@@ -56,10 +57,13 @@ struct TreeSmem {
   static constexpr int kTile = D / 64 * kPanel;
   static constexpr int kQPanel = kRows * 128;
   static constexpr int kQ = D / 64 * kQPanel;           // one row tile's queries
-  static constexpr int kStages = D == 64 ? 16 : kTwo ? 9 : 11;
+  // A multiple of four: where the units take the tiles in turn a slot then stays with one unit,
+  // whose issuer has seen each of its phases complete before it waits for the next (by parity).
+  // 8 / 12 of them: 236 / 217 us for 64 sequences of 100 to 8,191.
+  static constexpr int kStages = D == 64 ? 24 : kTwo ? 8 : 12;
   static constexpr int kOffRing = (kTwo ? 2 : 1) * kQ;
-  static constexpr int kOffMl = kOffRing + kStages * kTile;
-  static constexpr int kBytes = kOffMl + 2 * 2 * kRows * 16 + 1024;  // tiles start on a 1,024-byte boundary
+  static constexpr int kBytes = kOffRing + kStages * kTile + 1024;  // tiles start on a 1,024-byte boundary
+  static_assert(kStages % 4 == 0 && kStages <= 32, "phases are kept in a word");
 };
 
 struct TreeAttnParams {
@@ -120,8 +124,8 @@ __device__ __forceinline__ LaneTree load_tree(const TreeView& t, int b, int pre,
   w.root1 = lane + 32 < t.tokens ? tree_parent(t, b, lane + 32, &bad) : -2;
   w.seen0 = 1ull << lane;
   w.seen1 = 1ull << (lane + 32);
-#pragma unroll 1
-  for (int k = 0; k < 6; ++k) {  // the walk's length doubles: 64 tokens
+  // the walk's length doubles: six rounds at most, as parents lie below their children
+  while (__any_sync(0xffffffffu, w.root0 >= 0 || w.root1 >= 0)) {
     // a token's entries through its current ancestor
     auto ask = [&](int at, uint64_t& seen, int& root) {
       const int src = at < 0 ? 0 : at;
@@ -210,7 +214,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = (smem_u32(g_tree_smem) + 1023u) & ~1023u;
   const uint32_t s_q = base, s_ring = base + L::kOffRing;
-  float4* sh_ml = reinterpret_cast<float4*>(g_tree_smem + (base - smem_u32(g_tree_smem)) + L::kOffMl);  // [2 pieces][2 units][128]
 
   pdl_launch_dependents();
   pdl_wait();
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1 && lane == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&b_full[i], 1);
-      mbar_init(&b_free[i], 1);
+      mbar_init(&b_free[i], 2);  // both units', or the one's that takes the tile
       mbar_init(&b_tail[i], 1);
     }
     mbar_init(&b_qready, 8);  // an arrival per softmax warp
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     mbar_init(&b_fixed, 1);
-    mbar_init(&b_done, 1);
+    mbar_init(&b_done, 2);
     fence_mbar_init();
   } else if (warp == 9) {
     tmem_alloc(&sh_tmem, 512);
@@ -308,7 +311,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     LaneTree tree;
     int tree_b = -1;
-    auto prepare = [&](const Cursor& c) -> Row {  // the piece's row of this thread; its queries go to shared memory
+    // The thread's row's queries (both units share a row where one row tile is enough), on their
+    // way while the piece before ends: 215 -> 201 us for 64 sequences of 100 to 8,191.  Twice as
+    // many registers of them, for two row tiles, spill and cost 6%.
+    uint4 queries[D / 16];
+    const uint4* source = nullptr;
+    auto fetch = [&](const Cursor& c) -> Row {
       Row w;
       const int kvh = c.kr / p.row_pairs, rows = rows_of(c.kr);
       const bool par = rows <= kRows;
@@ -319,29 +327,46 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tok = row / p.group;
       w.hd = kvh * p.group + row % p.group;
       w.token = static_cast<int64_t>(c.b) * tr.tokens + tok;
+      source = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + w.token * p.q_stride + static_cast<int64_t>(w.hd) * D) +
+               (par ? r * (D / 16) : 0);
+      if (!kTwo) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) queries[i] = w.has ? source[i] : make_uint4(0, 0, 0, 0);
+      }
       if (c.b != tree_b) {
         tree = load_tree(tr, c.b, c.pre, lane, warp == 0 && c.kr == 0 && c.t0 == 0, p.status);
         tree_b = c.b;
       }
       w.here = tree_token(tree, tok, w.seen) && w.has;
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + w.token * p.q_stride + static_cast<int64_t>(w.hd) * D);
+      return w;
+    };
+    auto put = [&](const Cursor& c, bool has) {  // the queries to shared memory
+      const bool par = rows_of(c.kr) <= kRows;
       const uint32_t dst = s_q + (par ? 0 : r * L::kQ) + lr * 128;
-      const int i0 = par ? r * (D / 16) : 0, i1 = par ? i0 + D / 16 : D / 8;  // both units share a row's queries
-#pragma unroll 8
-      for (int i = i0; i < i1; ++i) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (w.has) u = src[i];
-        sts128(dst + (i >> 3) * L::kQPanel + (((i & 7) ^ (lr & 7)) << 4), u.x, u.y, u.z, u.w);
+      const int i0 = par ? r * (D / 16) : 0;
+#pragma unroll 1
+      for (int part = 0; part < (kTwo && !par ? 2 : 1); ++part) {
+        if (kTwo) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) queries[i] = has ? source[part * (D / 16) + i] : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int x = i0 + part * (D / 16) + i;
+          sts128(dst + (x >> 3) * L::kQPanel + (((x & 7) ^ (lr & 7)) << 4), queries[i].x, queries[i].y, queries[i].z, queries[i].w);
+        }
       }
       fence_async_proxy();
       arrive_warp(&b_qready);
-      return w;
     };
     int u = 0;  // steps of this unit before the piece
     int piece = 0;
     bool ok = c.left > 0;
     Row w{};
-    if (ok) w = prepare(c);
+    if (ok) {
+      w = fetch(c);
+      put(c, w.has);
+    }
     const float cn = p.scale_log2;
     const uint64_t cn2 = pack2(cn, cn);
     while (ok) {
@@ -454,28 +479,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         arrive_warp(&b_pready[r][h]);
       }
+      const Cursor old = c;
+      const Row row = w;
+      if (!ok) break;
+      next_piece(p, c);
+      if (c.left > 0) w = fetch(c);
       // the last step's products (and those before them), and the cleaned values' notes
       if (ok && steps > 0) ok = wait_all(&b_odone[r][(u + steps - 1) & 1], ((u + steps - 1) >> 1) & 1);
       if (ok) ok = wait_all(&b_fixed, piece & 1);
       if (!ok) break;
       u += steps;
       const float kept = steps > kWindow && kLong ? exp2_approx(m_kept - m) : 0.f;
-      float4* ml = sh_ml + (piece & 1) * 2 * kRows;
-      ml[r * kRows + lr] = make_float4(m, l, kept, steps > kWindow && kLong ? 1.f : 0.f);
+      // m, l and the factor of the sums meet the other unit's in the unit's columns of scores
+      const uint32_t mine[4] = {__float_as_uint(m), __float_as_uint(l), __float_as_uint(kept),
+                                kLong && steps > kWindow ? 1u : 0u};
+      tmem_st_x4(t_s, mine);
+      tmem_st_done();
+      tc_fence_before();
       arrive_warp(&b_alldone);
       ok = wait_all(&b_alldone, piece & 1);
       if (!ok) break;
       tc_fence_after();
-      const uint64_t bad = sh_bad[piece & 1] & w.seen;
-      const Cursor old = c;
-      const Row row = w;
-      next_piece(p, c);
-      if (c.left > 0) w = prepare(c);  // the next piece's scores begin while this one's rows are written
+      uint32_t ml_a[4], ml_b[4];
+      tmem_ld_x4(par ? tmem + t_lane : t_s, ml_a);
+      tmem_ld_x4(tmem + t_lane + 128, ml_b);
+      tmem_ld_wait();
+      tc_fence_before();
+      const uint64_t bad = sh_bad[piece & 1] & row.seen;
+      if (c.left > 0) put(c, w.has);  // the next piece's scores begin while this one's rows are written
       // ---- the piece's rows
       if (row.live) {
-        const float4 ma = ml[(par ? 0 : r) * kRows + lr];
-        float4 mb = make_float4(kFloor, 0.f, 0.f, 0.f);
-        if (par) mb = ml[kRows + lr];
+        const float4 ma = make_float4(__uint_as_float(ml_a[0]), __uint_as_float(ml_a[1]), __uint_as_float(ml_a[2]),
+                                      ml_a[3] ? 1.f : 0.f);
+        const float4 mb = make_float4(__uint_as_float(ml_b[0]), par ? __uint_as_float(ml_b[1]) : 0.f,
+                                      __uint_as_float(ml_b[2]), ml_b[3] ? 1.f : 0.f);
         // a unit that saw nothing weighs 0, whatever its sums hold
         const bool use_a = row.here && ma.y != 0.f, use_b = row.here && mb.y != 0.f;
         const float mm = fmaxf(use_a ? ma.x : kFloor, use_b ? mb.x : kFloor);
@@ -611,60 +648,69 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issuer
+  } else if (warp != 10) {
+    // ------------------------------------------------------------ MMA issuers
+    const int r = warp == 9 ? 0 : 1;
     const uint32_t idesc_s = (1u << 4) | Mma16<T>::kType | (kStep >> 3 << 17) | (kRows >> 4 << 24);
     const uint32_t idesc_o = (1u << 4) | Mma16<T>::kType | (1u << 16) | (D >> 3 << 17) | (kRows >> 4 << 24);
     const uint64_t dq = umma_smem_desc_sw128(s_q), dk = umma_smem_desc_sw128(s_ring), dv = desc_mn(s_ring, L::kPanel);
-    int piece = 0, u[2] = {0, 0};
+    int piece = 0, u = 0;
     uint32_t lb = 0;  // loads before the piece
     bool ok = true;
     while (ok && c.left > 0) {
       const int rows = rows_of(c.kr), nt = c.t1 - c.t0;
       const bool par = rows <= kRows;
-      const int steps[2] = {steps_of(par, rows, nt, 0), steps_of(par, rows, nt, 1)};
-      const int last = rows > kRows ? 1 : 0;  // the unit behind whose MMAs a tile is free, where both take it
-      auto issue_s = [&](int r, int t) -> bool {
-        const int h = (u[r] + t) & 1, j = par ? 2 * t + r : t;
-        const uint32_t at = lb + 2 * j, slot = at % kStages;
-        if (!wait_all(&b_full[slot], (at / kStages) & 1)) return false;
-        tc_fence_after();
+      const int steps = steps_of(par, rows, nt, r);
+      auto release = [&](uint32_t slot) {
+        commit_warp(&b_free[slot]);
+        if (par) commit_warp(&b_free[slot]);
+      };
+      auto issue_s = [&](int t) {
+        const int h = (u + t) & 1, j = par ? 2 * t + r : t;
+        const uint32_t slot = (lb + 2 * j) % kStages;
         const uint64_t qa = dq + ((!kTwo || par ? 0 : r * L::kQ) >> 4), kb = dk + (slot * L::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
           umma_f16_ss(tmem + r * 128 + h * kStep, qa + (((kk >> 2) * L::kQPanel + (kk & 3) * 32) >> 4),
                       kb + (((kk >> 2) * L::kPanel + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
         commit_warp(&b_sfull[r][h]);
-        if (par || r == last) commit_warp(&b_free[slot]);
-        return true;
+        release(slot);
       };
-      auto issue_o = [&](int r, int t) -> bool {
-        const int h = (u[r] + t) & 1, j = par ? 2 * t + r : t;
-        const uint32_t at = lb + 2 * j + 1, slot = at % kStages;
-        if (!wait_all(&b_pready[r][h], ((u[r] + t) >> 1) & 1)) return false;
-        if (!wait_all(&b_full[slot], (at / kStages) & 1)) return false;
-        tc_fence_after();
+      auto issue_o = [&](int t) {
+        const int h = (u + t) & 1, j = par ? 2 * t + r : t;
+        const uint32_t slot = (lb + 2 * j + 1) % kStages;
         const uint64_t vb = dv + (slot * L::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < kStep / 16; ++kk)
           umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + h * kStep + kk * 8, vb + (kk * 2048 >> 4), idesc_o,
                       (kLong ? t % kWindow : t) != 0 || kk > 0 ? 1u : 0u);
         commit_warp(&b_odone[r][h]);
-        if (par || r == last) commit_warp(&b_free[slot]);
-        return true;
+        release(slot);
       };
       ok = wait_all(&b_qready, piece & 1);
-      for (int t = 0; ok && t < 2; ++t)
-        for (int r = 0; ok && r < 2; ++r)
-          if (t < steps[r]) ok = issue_s(r, t);
-      for (int t = 0; ok && (t < steps[0] || t < steps[1]); ++t)
-        for (int r = 0; ok && r < 2; ++r)
-          if (t < steps[r]) {
-            ok = issue_o(r, t);
-            if (ok && t + 2 < steps[r]) ok = issue_s(r, t + 2);
-          }
-      u[0] += steps[0];
-      u[1] += steps[1];
+      auto loaded = [&](int t, int values) -> bool {  // step t's keys or values
+        const uint32_t at = lb + 2 * (par ? 2 * t + r : t) + values;
+        return wait_all(&b_full[at % kStages], (at / kStages) & 1);
+      };
+      for (int t = 0; ok && t < 2 && t < steps; ++t) {
+        ok = loaded(t, 0);
+        if (!ok) break;
+        tc_fence_after();
+        issue_s(t);
+      }
+      for (int t = 0; ok && t < steps; ++t) {
+        ok = loaded(t, 1) && wait_all(&b_pready[r][(u + t) & 1], ((u + t) >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        issue_o(t);
+        if (t + 2 < steps) {
+          ok = loaded(t + 2, 0);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(t + 2);
+        }
+      }
+      u += steps;
       lb += 2 * nt;
       ++piece;
       next_piece(p, c);
@@ -713,22 +759,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 uint32_t v[4];
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
-                bool hit = false;
+                // an exponent of all ones carries into the sign's place
+                constexpr uint32_t kE2 = Mma16<T>::kExp * 0x10001u, kOne2 = (0x8000u - Mma16<T>::kExp) * 0x10001u;
+                if (((((v[0] & kE2) + kOne2) | ((v[1] & kE2) + kOne2) | ((v[2] & kE2) + kOne2) | ((v[3] & kE2) + kOne2)) & 0x80008000u) == 0)
+                  continue;
+                odd = true;
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                  if ((v[y] & Mma16<T>::kExp) == Mma16<T>::kExp) {
-                    v[y] &= 0xffff0000u;
-                    hit = true;
-                  }
-                  if ((v[y] & (Mma16<T>::kExp << 16)) == (Mma16<T>::kExp << 16)) {
-                    v[y] &= 0x0000ffffu;
-                    hit = true;
-                  }
+                  if ((v[y] & Mma16<T>::kExp) == Mma16<T>::kExp) v[y] &= 0xffff0000u;
+                  if ((v[y] & (Mma16<T>::kExp << 16)) == (Mma16<T>::kExp << 16)) v[y] &= 0x0000ffffu;
                 }
-                if (hit) {
-                  sts128(a, v[0], v[1], v[2], v[3]);
-                  odd = true;
-                }
+                sts128(a, v[0], v[1], v[2], v[3]);
               }
           }
           const uint32_t odds = __ballot_sync(0xffffffffu, odd);
