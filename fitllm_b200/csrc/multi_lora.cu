@@ -10,10 +10,12 @@
 // tokens / kSlot + batch of them without knowing any.
 //
 // multi_lora_shrink_kernel, T = x.A_l^T: a cluster of up to eight CTAs shares a slot, each a part of
-// K; a CTA's eight warps are dealt to its tokens (32 each) and the parts of K that are left over,
-// so that a single token is summed by 64 warps.  A lane reads 16 bytes of a row of x and of A at
-// a time and feeds them to two MMAs: the contraction index is permuted alike in both.  Parts
-// join in shared memory, then over the cluster, in order (deterministic); T stays in fp32.
+// K.  Up to sixteen tokens: the eight warps split the part again, and a lane reads 16 bytes of a
+// row of x and of A at a time and feeds them to two MMAs (the contraction index is permuted
+// alike in both), so that a single token is summed by 64 warps with every load in flight at
+// once.  More: sixteen tokens per warp, x and A through four stages of cp.async, 64 columns
+// each.  Parts join in shared memory, then over the cluster, in order (deterministic); T stays
+// in fp32.
 //
 // multi_lora_expand_kernel, y = y_add + s T.B_l^T: T enters as two 16-bit numbers, hi + lo (a
 // relative error of eps^2; one alone would cost the delta half its digits), scaled by a power of
@@ -29,9 +31,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kSlot = 256;       // tokens of a slot: 32 for each warp of the first kernel
-constexpr int kTile = 128;       // of one of the second: 16 for each warp
-constexpr int kCols = 512;       // columns of a CTA of the second
+constexpr int kSlot = 128;       // tokens of a slot: 16 for each warp
+constexpr int kCols = 1024;      // columns of a CTA of the second kernel
 constexpr int kMaxParts = 8;     // CTAs of a cluster
 
 struct MultiLoraParams {
@@ -127,11 +128,31 @@ __device__ __forceinline__ float4 remote_float4(const float* p, uint32_t rank) {
 
 extern __shared__ float4 g_lora_smem[];
 
-template <typename T, int R>
-__global__ void __launch_bounds__(kThreads) multi_lora_shrink_kernel(const MultiLoraParams p) {
+__device__ __forceinline__ void cp16_zfill(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+
+// Stages of the first kernel's copies: 64 columns of a slot's tokens and of A.
+template <int R>
+struct ShrinkSmem {
+  static constexpr int kStages = 4;
+  static constexpr int kX = kSlot * 128, kA = R * 128, kStage = kX + kA;
+  static constexpr int kRed = kWarps * 16 * R * 4;  // the warps' sums: 16 tokens each
+  static constexpr int kMany = kStages * kStage > kRed ? kStages * kStage : kRed;
+};
+
+// kMany: some slot may have more than sixteen tokens.
+template <typename T, int R, bool kMany>
+__global__ void __launch_bounds__(kThreads, 2) multi_lora_shrink_kernel(const MultiLoraParams p) {
   constexpr int NT = R / 8;
-  constexpr int kUnroll = R == 16 ? 4 : R == 32 ? 2 : 1;  // what the registers hold beside the sums
-  float* red = reinterpret_cast<float*>(g_lora_smem);     // [warps][32][R]
+  constexpr int kUnroll = R == 16 ? 4 : R == 32 ? 3 : 2;  // what the registers hold beside the sums
+  using L = ShrinkSmem<R>;
+  float* red = reinterpret_cast<float*>(g_lora_smem);     // [warps][16][R]
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
@@ -139,101 +160,126 @@ __global__ void __launch_bounds__(kThreads) multi_lora_shrink_kernel(const Multi
   int64_t first;
   int count, l;
   if (!slot_of<kSlot>(p, blockIdx.x / p.parts, lane, first, count, l, part == 0 && warp == 0) || l < 0) return;  // the whole cluster
-  // warps over tokens and, what is left, over K
-  const int mw = count <= 32 ? 1 : count <= 64 ? 2 : count <= 128 ? 4 : 8, kw = kWarps / mw;
-  const int wm = warp / kw, wk = warp % kw;
-  const int m0 = wm * 32;
-  const bool second = count - m0 > 16;  // the warp's other sixteen tokens
   const int k0 = part * p.part_cols, k1 = min(p.k, k0 + p.part_cols);
-  float acc[2][NT][4];
+  const T* x = static_cast<const T*>(p.x) + first * p.x_stride;
+  const T* a = static_cast<const T*>(p.a) + static_cast<int64_t>(l) * R * p.k;
+  const bool few = !kMany || count <= 16;
+  float acc[NT][4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[h][t][i] = 0.f;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  const T* x = static_cast<const T*>(p.x);
-  const T* rows[4];
-  bool has[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    has[i] = m0 + 8 * i + g < count;
-    rows[i] = x + (first + (has[i] ? m0 + 8 * i + g : 0)) * p.x_stride;
-  }
-  const T* a = static_cast<const T*>(p.a) + (static_cast<int64_t>(l) * R + g) * p.k;
-  if (m0 < count) {
-    for (int c0 = k0 + wk * 32; c0 < k1; c0 += kw * 32 * kUnroll) {
-      uint4 xv[kUnroll][4], av[kUnroll][NT];
+    for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+  if (few) {
+    // ---- every warp has all tokens and columns of its own, loaded straight into fragments
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const bool has0 = g < count, has1 = g + 8 < count;
+    const T* x0 = x + (has0 ? g : 0) * p.x_stride;
+    const T* x1 = x + (has1 ? g + 8 : 0) * p.x_stride;
+    const T* ag = a + static_cast<int64_t>(g) * p.k;
+    for (int c0 = k0 + warp * 32; c0 < k1; c0 += kWarps * 32 * kUnroll) {
+      uint4 xv[kUnroll][2], av[kUnroll][NT];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        const int col = c0 + u * kw * 32 + 8 * q;
+        const int col = c0 + u * kWarps * 32 + 8 * q;
         const bool in = col < k1;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          av[u][t] = in ? __ldg(reinterpret_cast<const uint4*>(a + static_cast<int64_t>(8 * t) * p.k + col)) : zero;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) xv[u][i] = in && has[i] ? __ldg(reinterpret_cast<const uint4*>(rows[i] + col)) : zero;
-        if (second) {
-#pragma unroll
-          for (int i = 2; i < 4; ++i) xv[u][i] = in && has[i] ? __ldg(reinterpret_cast<const uint4*>(rows[i] + col)) : zero;
-        }
+          av[u][t] = in ? __ldg(reinterpret_cast<const uint4*>(ag + static_cast<int64_t>(8 * t) * p.k + col)) : zero;
+        xv[u][0] = in && has0 ? __ldg(reinterpret_cast<const uint4*>(x0 + col)) : zero;
+        xv[u][1] = in && has1 ? __ldg(reinterpret_cast<const uint4*>(x1 + col)) : zero;
       }
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
+      for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          mma_16816<T>(acc[0][t], xv[u][0].x, xv[u][1].x, xv[u][0].y, xv[u][1].y, av[u][t].x, av[u][t].y);
-          mma_16816<T>(acc[0][t], xv[u][0].z, xv[u][1].z, xv[u][0].w, xv[u][1].w, av[u][t].z, av[u][t].w);
+          mma_16816<T>(acc[t], xv[u][0].x, xv[u][1].x, xv[u][0].y, xv[u][1].y, av[u][t].x, av[u][t].y);
+          mma_16816<T>(acc[t], xv[u][0].z, xv[u][1].z, xv[u][0].w, xv[u][1].w, av[u][t].z, av[u][t].w);
         }
-        if (second) {
+    }
+  } else if constexpr (kMany) {
+    // ---- sixteen tokens per warp, 64 columns at a time through shared memory: rows of 128 bytes,
+    // 16-byte piece c of row r at c ^ (r & 7)
+    const uint32_t base = smem_u32(g_lora_smem);
+    const int steps = (k1 - k0 + 63) / 64;
+    auto load = [&](int s) {
+      if (s < steps) {
+        const uint32_t at = base + s % L::kStages * L::kStage;
+        const int c = threadIdx.x & 7, col = k0 + s * 64 + 8 * c;
+        const uint32_t in = col < k1 ? 16u : 0u;
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            mma_16816<T>(acc[1][t], xv[u][2].x, xv[u][3].x, xv[u][2].y, xv[u][3].y, av[u][t].x, av[u][t].y);
-            mma_16816<T>(acc[1][t], xv[u][2].z, xv[u][3].z, xv[u][2].w, xv[u][3].w, av[u][t].z, av[u][t].w);
-          }
+        for (int i = 0; i < kSlot / 32; ++i) {
+          const int row = (threadIdx.x >> 3) + 32 * i;
+          const bool ok = row < count && in;
+          cp16_zfill(at + row * 128 + ((c ^ (row & 7)) << 4), ok ? x + row * p.x_stride + col : x, ok ? 16u : 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < (R + 31) / 32; ++i) {
+          const int row = (threadIdx.x >> 3) + 32 * i;
+          if (R % 32 == 0 || row < R)
+            cp16_zfill(at + L::kX + row * 128 + ((c ^ (row & 7)) << 4), in ? a + static_cast<int64_t>(row) * p.k + col : a, in);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int s = 0; s < L::kStages - 1; ++s) load(s);
+    const int mat = lane >> 3, r8 = lane & 7;
+    const int xrow = warp * 16 + (mat & 1) * 8 + r8;  // matrices: rows 0-7 | 8-15 x columns 0-7 | 8-15 of sixteen
+    const int arow = (mat >> 1) * 8 + r8;             // matrices: columns 0-7 | 8-15 x two MMAs' rows
+    for (int s = 0; s < steps; ++s) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
+      __syncthreads();  // stage s is there; every warp is done with the one that is loaded next
+      load(s + L::kStages - 1);
+      if (warp * 16 >= count) continue;
+      const uint32_t at = base + s % L::kStages * L::kStage;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        uint32_t xa[4];
+        ldsm4(at + xrow * 128 + (((2 * kk + (mat >> 1)) ^ (xrow & 7)) << 4), xa);
+#pragma unroll
+        for (int t = 0; t < NT; t += 2) {
+          uint32_t bb[4];
+          const int row = 8 * t + arow;
+          ldsm4(at + L::kX + row * 128 + (((2 * kk + (mat & 1)) ^ (row & 7)) << 4), bb);
+          mma_16816<T>(acc[t], xa[0], xa[1], xa[2], xa[3], bb[0], bb[1]);
+          mma_16816<T>(acc[t + 1], xa[0], xa[1], xa[2], xa[3], bb[2], bb[3]);
         }
       }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the stages' place becomes the sums'
   }
-  float* mine = red + warp * 32 * R;
+  float* mine = red + warp * 16 * R;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (h == 1 && !second) break;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      *reinterpret_cast<float2*>(mine + (16 * h + g) * R + 8 * t + 2 * q) = make_float2(acc[h][t][0], acc[h][t][1]);
-      *reinterpret_cast<float2*>(mine + (16 * h + g + 8) * R + 8 * t + 2 * q) = make_float2(acc[h][t][2], acc[h][t][3]);
-    }
+  for (int t = 0; t < NT; ++t) {
+    *reinterpret_cast<float2*>(mine + g * R + 8 * t + 2 * q) = make_float2(acc[t][0], acc[t][1]);
+    *reinterpret_cast<float2*>(mine + (g + 8) * R + 8 * t + 2 * q) = make_float2(acc[t][2], acc[t][3]);
   }
   __syncthreads();
-  // the parts of K of a CTA, in the warps' order, into the first warp's place
   const int cells = count * (R / 4);
   float4* red4 = reinterpret_cast<float4*>(red);
-  auto place = [&](int e) { return (e / (32 * (R / 4))) * kw * (32 * (R / 4)) + e % (32 * (R / 4)); };
-  if (kw > 1) {
+  if (few) {  // the warps' sums in order, into the first warp's place
     for (int e = threadIdx.x; e < cells; e += kThreads) {
-      float4* at = red4 + place(e);
-      float4 s = *at;
-      for (int w = 1; w < kw; ++w) {
-        const float4 v = at[w * 32 * (R / 4)];
+      float4 s = red4[e];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) {
+        const float4 v = red4[e + w * 16 * (R / 4)];
         s.x += v.x;
         s.y += v.y;
         s.z += v.z;
         s.w += v.w;
       }
-      *at = s;
+      red4[e] = s;
     }
   }
   float4* out = reinterpret_cast<float4*>(p.t + first * R);
   if (p.parts == 1) {
     __syncthreads();
-    for (int e = threadIdx.x; e < cells; e += kThreads) out[e] = red4[place(e)];
+    for (int e = threadIdx.x; e < cells; e += kThreads) out[e] = red4[e];
     return;
   }
   cluster_barrier();
   for (int e = threadIdx.x * p.parts + part; e < cells; e += kThreads * p.parts) {
-    const float* at = reinterpret_cast<const float*>(red4 + place(e));
+    const float* at = reinterpret_cast<const float*>(red4 + e);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int r = 0; r < p.parts; ++r) {
       const float4 v = remote_float4(at, r);
@@ -251,12 +297,13 @@ template <typename T, int R>
 __global__ void __launch_bounds__(kThreads) multi_lora_expand_kernel(const MultiLoraParams p) {
   constexpr int KS = R / 16;   // steps of the contraction
   constexpr int kPer = R / 4;  // its elements that a lane holds: [q kPer, (q + 1) kPer), four to a step
+  constexpr int kGroups = R == 16 ? 4 : R == 32 ? 2 : 1;  // of 32 columns, loaded at once
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   int64_t first;
   int count, l;
-  if (!slot_of<kTile>(p, blockIdx.x / p.chunks, lane, first, count, l, false)) return;
+  if (!slot_of<kSlot>(p, blockIdx.x / p.chunks, lane, first, count, l, false)) return;
   const int c_lo = blockIdx.x % p.chunks * kCols, c_hi = min(p.n, c_lo + kCols);
   const int mw = count <= 16 ? 1 : count <= 32 ? 2 : count <= 64 ? 4 : 8, nw = kWarps / mw;
   const int m0 = warp / nw * 16, wn = warp % nw;
@@ -275,6 +322,38 @@ __global__ void __launch_bounds__(kThreads) multi_lora_expand_kernel(const Multi
     }
     return;
   }
+  const T* b = static_cast<const T*>(p.b) + static_cast<int64_t>(l) * p.n * R + q * kPer;
+  // column 2 q' + e of MMA j is column 8 q' + 2 j + e of the thirty-two
+  uint2 bv[kGroups][4][KS];
+  uint4 v0[kGroups], v1[kGroups];
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int u = 0; u < kGroups; ++u) {
+      const int cu = c0 + u * nw * 32;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int col = cu + 8 * (g >> 1) + 2 * j + (g & 1);
+        const uint2* src = reinterpret_cast<const uint2*>(b + static_cast<int64_t>(col < c_hi ? col : 0) * R);
+        if constexpr (KS % 2 == 0) {
+#pragma unroll
+          for (int s = 0; s < KS; s += 2) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + s));
+            bv[u][j][s] = make_uint2(v.x, v.y);
+            bv[u][j][s + 1] = make_uint2(v.z, v.w);
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) bv[u][j][s] = __ldg(src + s);
+        }
+      }
+      const int c = cu + 8 * q;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      v0[u] = c < c_hi && has0 ? *reinterpret_cast<const uint4*>(add0 + c) : zero;
+      v1[u] = c < c_hi && has1 ? *reinterpret_cast<const uint4*>(add1 + c) : zero;
+    }
+  };
+  int c0 = c_lo + wn * 32;
+  load(c0);  // on their way while T is made ready
   // T of rows g and g + 8 as hi + lo
   uint32_t hi[KS][4], lo[KS][4];  // registers 0 and 2 row g, 1 and 3 row g + 8
   float f0 = p.scale[l], f1 = f0;
@@ -315,48 +394,30 @@ __global__ void __launch_bounds__(kThreads) multi_lora_expand_kernel(const Multi
         lo[s][2 * i + r] = Half16<T>::pack(fabsf(back.x) < INFINITY ? u - back.x : 0.f, fabsf(back.y) < INFINITY ? v - back.y : 0.f);
       }
   }
-  const T* b = static_cast<const T*>(p.b) + static_cast<int64_t>(l) * p.n * R + q * kPer;
-  for (int c0 = c_lo + wn * 32; c0 < c_hi; c0 += nw * 32) {
-    // column 2 q' + e of MMA j is column 8 q' + 2 j + e of the thirty-two
-    uint2 bv[4][KS];
+  while (c0 < c_hi) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = c0 + 8 * (g >> 1) + 2 * j + (g & 1);
-      const uint2* src = reinterpret_cast<const uint2*>(b + static_cast<int64_t>(col < p.n ? col : 0) * R);
-      if constexpr (KS % 2 == 0) {
+    for (int u = 0; u < kGroups; ++u) {
+      const int c = c0 + u * nw * 32 + 8 * q;
+      float o0[8], o1[8];
+      unpack8<T>(v0[u], o0);
+      unpack8<T>(v1[u], o1);
 #pragma unroll
-        for (int s = 0; s < KS; s += 2) {
-          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + s));
-          bv[j][s] = make_uint2(v.x, v.y);
-          bv[j][s + 1] = make_uint2(v.z, v.w);
-        }
-      } else {
+      for (int j = 0; j < 4; ++j) {
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < KS; ++s) bv[j][s] = __ldg(src + s);
+        for (int s = 0; s < KS; ++s) mma_16816<T>(d, lo[s][0], lo[s][1], lo[s][2], lo[s][3], bv[u][j][s].x, bv[u][j][s].y);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) mma_16816<T>(d, hi[s][0], hi[s][1], hi[s][2], hi[s][3], bv[u][j][s].x, bv[u][j][s].y);
+        o0[2 * j] = fmaf(f0, d[0], o0[2 * j]);
+        o0[2 * j + 1] = fmaf(f0, d[1], o0[2 * j + 1]);
+        o1[2 * j] = fmaf(f1, d[2], o1[2 * j]);
+        o1[2 * j + 1] = fmaf(f1, d[3], o1[2 * j + 1]);
       }
+      if (c < c_hi && has0) *reinterpret_cast<uint4*>(y0 + c) = pack8<T>(o0);
+      if (c < c_hi && has1) *reinterpret_cast<uint4*>(y1 + c) = pack8<T>(o1);
     }
-    const int c = c0 + 8 * q;
-    const bool in = c < c_hi;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    const uint4 v0 = in && has0 ? *reinterpret_cast<const uint4*>(add0 + c) : zero;
-    const uint4 v1 = in && has1 ? *reinterpret_cast<const uint4*>(add1 + c) : zero;
-    float o0[8], o1[8];
-    unpack8<T>(v0, o0);
-    unpack8<T>(v1, o1);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) mma_16816<T>(d, lo[s][0], lo[s][1], lo[s][2], lo[s][3], bv[j][s].x, bv[j][s].y);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) mma_16816<T>(d, hi[s][0], hi[s][1], hi[s][2], hi[s][3], bv[j][s].x, bv[j][s].y);
-      o0[2 * j] = fmaf(f0, d[0], o0[2 * j]);
-      o0[2 * j + 1] = fmaf(f0, d[1], o0[2 * j + 1]);
-      o1[2 * j] = fmaf(f1, d[2], o1[2 * j]);
-      o1[2 * j + 1] = fmaf(f1, d[3], o1[2 * j + 1]);
-    }
-    if (in && has0) *reinterpret_cast<uint4*>(y0 + c) = pack8<T>(o0);
-    if (in && has1) *reinterpret_cast<uint4*>(y1 + c) = pack8<T>(o1);
+    c0 += kGroups * nw * 32;
+    if (c0 < c_hi) load(c0);
   }
 }
 
@@ -369,13 +430,14 @@ int64_t slots_of(int64_t tokens, int batch, bool ragged, int size) {
 template <typename T, int R>
 int multi_lora_t(MultiLoraParams p, cudaStream_t st, int num_sms) {
   const int64_t slots = slots_of(p.tokens, p.batch, p.q_start != nullptr, kSlot);
-  // parts of K: as many as give every SM some eight CTAs, of 256 columns at least
+  // parts of K: as many as find room at once, two CTAs on an SM, of 256 columns at least
   int parts = 1;
-  while (parts < kMaxParts && slots * parts * 2 <= 8ll * num_sms && p.k > 256 * parts) parts *= 2;
+  while (parts < kMaxParts && slots * parts * 2 <= 2ll * num_sms && p.k > 256 * parts) parts *= 2;
   p.parts = parts;
-  p.part_cols = ((p.k + parts - 1) / parts + 31) / 32 * 32;
-  constexpr int smem = kWarps * 32 * R * 4;
-  auto* shrink = multi_lora_shrink_kernel<T, R>;
+  p.part_cols = ((p.k + parts - 1) / parts + 63) / 64 * 64;
+  const bool many = p.q_start != nullptr || p.t_new > 16;
+  const int smem = many ? ShrinkSmem<R>::kMany : ShrinkSmem<R>::kRed;
+  auto* shrink = many ? multi_lora_shrink_kernel<T, R, true> : multi_lora_shrink_kernel<T, R, false>;
   if (smem > 48 * 1024 && !set_smem_limit(shrink, smem)) return FITQ_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(slots * parts));
@@ -393,9 +455,8 @@ int multi_lora_t(MultiLoraParams p, cudaStream_t st, int num_sms) {
   cudaError_t e = cudaLaunchKernelEx(&cfg, shrink, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
-  const int64_t tiles = slots_of(p.tokens, p.batch, p.q_start != nullptr, kTile);
   p.chunks = (p.n + kCols - 1) / kCols;
-  e = launch_pdl(multi_lora_expand_kernel<T, R>, dim3(static_cast<unsigned>(tiles * p.chunks)), dim3(kThreads), 0, st, p);
+  e = launch_pdl(multi_lora_expand_kernel<T, R>, dim3(static_cast<unsigned>(slots * p.chunks)), dim3(kThreads), 0, st, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   return launch_result();
