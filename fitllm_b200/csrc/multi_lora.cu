@@ -32,7 +32,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSlot = 128;       // tokens of a slot: 16 for each warp
-constexpr int kCols = 1024;      // columns of a CTA of the second kernel
+constexpr int kCols = 256;       // columns of a CTA of the second kernel for more than sixteen tokens
+constexpr int kAhead = 4;        // of their groups of 32, those whose y_add is on its way
 constexpr int kMaxParts = 8;     // CTAs of a cluster
 
 struct MultiLoraParams {
@@ -293,21 +294,29 @@ __global__ void __launch_bounds__(kThreads, 2) multi_lora_shrink_kernel(const Mu
   cluster_barrier();  // no CTA leaves while its sums are read
 }
 
-template <typename T, int R>
-__global__ void __launch_bounds__(kThreads) multi_lora_expand_kernel(const MultiLoraParams p) {
+// Groups of 32 columns that a warp of a slot of few tokens loads at once.
+template <int R>
+constexpr int few_groups() { return R == 16 ? 4 : R == 32 ? 2 : 1; }
+
+// kMany as above; the grid has p.chunks parts of N for every slot, of kCols columns or, where
+// no slot has more than sixteen tokens, of all that eight warps load at once.
+template <typename T, int R, bool kMany>
+__global__ void __launch_bounds__(kThreads, 2) multi_lora_expand_kernel(const MultiLoraParams p) {
   constexpr int KS = R / 16;   // steps of the contraction
   constexpr int kPer = R / 4;  // its elements that a lane holds: [q kPer, (q + 1) kPer), four to a step
-  constexpr int kGroups = R == 16 ? 4 : R == 32 ? 2 : 1;  // of 32 columns, loaded at once
+  constexpr int kGroups = few_groups<R>(), kFewCols = kGroups * 32 * kWarps;
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   int64_t first;
   int count, l;
   if (!slot_of<kSlot>(p, blockIdx.x / p.chunks, lane, first, count, l, false)) return;
-  const int c_lo = blockIdx.x % p.chunks * kCols, c_hi = min(p.n, c_lo + kCols);
-  const int mw = count <= 16 ? 1 : count <= 32 ? 2 : count <= 64 ? 4 : 8, nw = kWarps / mw;
-  const int m0 = warp / nw * 16, wn = warp % nw;
-  if (m0 >= count) return;
+  const bool few = !kMany || count <= 16;
+  const int chunk = blockIdx.x % p.chunks, cols = few ? kFewCols : kCols;
+  const int64_t c_first = static_cast<int64_t>(chunk) * cols;
+  if (c_first >= p.n) return;  // the slot has fewer parts than the grid
+  const int c_lo = static_cast<int>(c_first), c_hi = min(p.n, c_lo + cols);
+  const int nw = few ? kWarps : 1, m0 = few ? 0 : warp * 16, wn = few ? warp : 0;
   const bool has0 = m0 + g < count, has1 = m0 + g + 8 < count;
   const int64_t n0 = first + m0 + g, n1 = n0 + 8;
   const T* add0 = static_cast<const T*>(p.y_add) + n0 * p.y_add_stride;
@@ -322,10 +331,32 @@ __global__ void __launch_bounds__(kThreads) multi_lora_expand_kernel(const Multi
     }
     return;
   }
-  const T* b = static_cast<const T*>(p.b) + static_cast<int64_t>(l) * p.n * R + q * kPer;
+  const T* b = static_cast<const T*>(p.b) + static_cast<int64_t>(l) * p.n * R;
+  // many tokens: the CTA's columns of B in shared memory, rows of 2 R bytes, 16-byte piece c of row r at
+  // c ^ (the bits of r in which a load's eight rows differ)
+  const uint32_t s_b = smem_u32(g_lora_smem);
+  auto b_at = [&](int row, int piece) {
+    const int mix = ((row & 1) | ((row >> 3) & 3) << 1) & (R % 64 == 0 ? 7 : R % 32 == 0 ? 3 : R == 16 ? 1 : 0);
+    return s_b + row * (2 * R) + ((piece ^ mix) << 4);
+  };
+  if (kMany && !few) {
+    for (int e = threadIdx.x; e < kCols * (R / 8); e += kThreads) {
+      const int row = e / (R / 8), piece = e % (R / 8);
+      const bool in = c_lo + row < p.n;
+      cp16_zfill(b_at(row, piece), b + static_cast<int64_t>(in ? c_lo + row : 0) * R + piece * 8, in ? 16u : 0u);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  const uint4 zero = make_uint4(0, 0, 0, 0);
   // column 2 q' + e of MMA j is column 8 q' + 2 j + e of the thirty-two
+  constexpr int kSets = kMany && kAhead > kGroups ? kAhead : kGroups;
   uint2 bv[kGroups][4][KS];
-  uint4 v0[kGroups], v1[kGroups];
+  uint4 v0[kSets], v1[kSets];
+  auto load_y = [&](int u, int cu) {
+    const int c = cu + 8 * q;
+    v0[u] = c < c_hi && has0 ? *reinterpret_cast<const uint4*>(add0 + c) : zero;
+    v1[u] = c < c_hi && has1 ? *reinterpret_cast<const uint4*>(add1 + c) : zero;
+  };
   auto load = [&](int c0) {
 #pragma unroll
     for (int u = 0; u < kGroups; ++u) {
@@ -333,7 +364,7 @@ __global__ void __launch_bounds__(kThreads) multi_lora_expand_kernel(const Multi
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int col = cu + 8 * (g >> 1) + 2 * j + (g & 1);
-        const uint2* src = reinterpret_cast<const uint2*>(b + static_cast<int64_t>(col < c_hi ? col : 0) * R);
+        const uint2* src = reinterpret_cast<const uint2*>(b + static_cast<int64_t>(col < c_hi ? col : 0) * R + q * kPer);
         if constexpr (KS % 2 == 0) {
 #pragma unroll
           for (int s = 0; s < KS; s += 2) {
@@ -346,14 +377,16 @@ __global__ void __launch_bounds__(kThreads) multi_lora_expand_kernel(const Multi
           for (int s = 0; s < KS; ++s) bv[u][j][s] = __ldg(src + s);
         }
       }
-      const int c = cu + 8 * q;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      v0[u] = c < c_hi && has0 ? *reinterpret_cast<const uint4*>(add0 + c) : zero;
-      v1[u] = c < c_hi && has1 ? *reinterpret_cast<const uint4*>(add1 + c) : zero;
+      load_y(u, cu);
     }
   };
-  int c0 = c_lo + wn * 32;
-  load(c0);  // on their way while T is made ready
+  const int c0 = c_lo + wn * 32;
+  if (few)  // on their way while T is made ready
+    load(c0);
+  else if constexpr (kMany) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) load_y(u, c0 + 32 * u);
+  }
   // T of rows g and g + 8 as hi + lo
   uint32_t hi[KS][4], lo[KS][4];  // registers 0 and 2 row g, 1 and 3 row g + 8
   float f0 = p.scale[l], f1 = f0;
@@ -394,30 +427,51 @@ __global__ void __launch_bounds__(kThreads) multi_lora_expand_kernel(const Multi
         lo[s][2 * i + r] = Half16<T>::pack(fabsf(back.x) < INFINITY ? u - back.x : 0.f, fabsf(back.y) < INFINITY ? v - back.y : 0.f);
       }
   }
-  while (c0 < c_hi) {
+  auto finish = [&](int u, int c, const uint2 (&w)[4][KS]) {  // y of the eight columns from c on
+    float o0[8], o1[8];
+    unpack8<T>(v0[u], o0);
+    unpack8<T>(v1[u], o1);
 #pragma unroll
-    for (int u = 0; u < kGroups; ++u) {
-      const int c = c0 + u * nw * 32 + 8 * q;
-      float o0[8], o1[8];
-      unpack8<T>(v0[u], o0);
-      unpack8<T>(v1[u], o1);
+    for (int j = 0; j < 4; ++j) {
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < KS; ++s) mma_16816<T>(d, lo[s][0], lo[s][1], lo[s][2], lo[s][3], w[j][s].x, w[j][s].y);
 #pragma unroll
-        for (int s = 0; s < KS; ++s) mma_16816<T>(d, lo[s][0], lo[s][1], lo[s][2], lo[s][3], bv[u][j][s].x, bv[u][j][s].y);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) mma_16816<T>(d, hi[s][0], hi[s][1], hi[s][2], hi[s][3], bv[u][j][s].x, bv[u][j][s].y);
-        o0[2 * j] = fmaf(f0, d[0], o0[2 * j]);
-        o0[2 * j + 1] = fmaf(f0, d[1], o0[2 * j + 1]);
-        o1[2 * j] = fmaf(f1, d[2], o1[2 * j]);
-        o1[2 * j + 1] = fmaf(f1, d[3], o1[2 * j + 1]);
-      }
-      if (c < c_hi && has0) *reinterpret_cast<uint4*>(y0 + c) = pack8<T>(o0);
-      if (c < c_hi && has1) *reinterpret_cast<uint4*>(y1 + c) = pack8<T>(o1);
+      for (int s = 0; s < KS; ++s) mma_16816<T>(d, hi[s][0], hi[s][1], hi[s][2], hi[s][3], w[j][s].x, w[j][s].y);
+      o0[2 * j] = fmaf(f0, d[0], o0[2 * j]);
+      o0[2 * j + 1] = fmaf(f0, d[1], o0[2 * j + 1]);
+      o1[2 * j] = fmaf(f1, d[2], o1[2 * j]);
+      o1[2 * j + 1] = fmaf(f1, d[3], o1[2 * j + 1]);
     }
-    c0 += kGroups * nw * 32;
-    if (c0 < c_hi) load(c0);
+    if (c < c_hi && has0) *reinterpret_cast<uint4*>(y0 + c) = pack8<T>(o0);
+    if (c < c_hi && has1) *reinterpret_cast<uint4*>(y1 + c) = pack8<T>(o1);
+  };
+  if (few) {
+#pragma unroll
+    for (int u = 0; u < kGroups; ++u) finish(u, c0 + u * nw * 32 + 8 * q, bv[u]);
+  } else if constexpr (kMany) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+#pragma unroll 1
+    for (int g0 = 0; g0 < kCols / 32; g0 += kAhead) {
+      if (c_lo + 32 * g0 >= c_hi) break;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        uint2 w[4][KS];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = 32 * (g0 + u) + 8 * (g >> 1) + 2 * j + (g & 1);
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const int byte = q * 2 * kPer + 8 * s;
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[j][s].x), "=r"(w[j][s].y) : "r"(b_at(row, byte >> 4) + (byte & 15)));
+          }
+        }
+        const int c = c_lo + 32 * (g0 + u);
+        finish(u, c + 8 * q, w);
+        load_y(u, c + 32 * kAhead);
+      }
+    }
   }
 }
 
@@ -430,9 +484,12 @@ int64_t slots_of(int64_t tokens, int batch, bool ragged, int size) {
 template <typename T, int R>
 int multi_lora_t(MultiLoraParams p, cudaStream_t st, int num_sms) {
   const int64_t slots = slots_of(p.tokens, p.batch, p.q_start != nullptr, kSlot);
-  // parts of K: as many as find room at once, two CTAs on an SM, of 256 columns at least
+  // parts of K: as many as find room at once, two CTAs on an SM, of 256 columns at least.  Slots
+  // are counted as a batch of any lengths has them on average (a sequence's last one half full), so
+  // that the sums do not depend on how the lengths were passed.
+  const int64_t half = p.tokens / kSlot + p.batch / 2, real = half > p.batch ? half : p.batch;
   int parts = 1;
-  while (parts < kMaxParts && slots * parts * 2 <= 2ll * num_sms && p.k > 256 * parts) parts *= 2;
+  while (parts < kMaxParts && real * parts * 2 <= 2ll * num_sms && p.k > 256 * parts) parts *= 2;
   p.parts = parts;
   p.part_cols = ((p.k + parts - 1) / parts + 63) / 64 * 64;
   const bool many = p.q_start != nullptr || p.t_new > 16;
@@ -455,8 +512,10 @@ int multi_lora_t(MultiLoraParams p, cudaStream_t st, int num_sms) {
   cudaError_t e = cudaLaunchKernelEx(&cfg, shrink, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
-  p.chunks = (p.n + kCols - 1) / kCols;
-  e = launch_pdl(multi_lora_expand_kernel<T, R>, dim3(static_cast<unsigned>(slots * p.chunks)), dim3(kThreads), 0, st, p);
+  const int cols = many ? kCols : few_groups<R>() * 32 * kWarps;
+  p.chunks = (p.n + cols - 1) / cols;
+  auto* expand = many ? multi_lora_expand_kernel<T, R, true> : multi_lora_expand_kernel<T, R, false>;
+  e = launch_pdl(expand, dim3(static_cast<unsigned>(slots * p.chunks)), dim3(kThreads), many ? kCols * R * 2 : 0, st, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   return launch_result();
