@@ -1645,8 +1645,8 @@ int fitq_tree_verify(const void* logits, int dtype, int64_t stride_b, int64_t st
       (parents_stride != 0 && parents_stride < tokens) || (probs && (probs_stride_t < vocab || probs_stride_b < 0)))
     return fail(FITQ_ERR_SHAPE, "tree_verify: bad shape (batch=%lld vocab=%lld strides %lld, %lld)", (long long)batch,
                 (long long)vocab, (long long)stride_b, (long long)stride_t);
-  if (!temperatures && !(temperature >= 0.f && temperature <= 3.4e38f))
-    return fail(FITQ_ERR_ARG, "tree_verify: temperature must not be negative (got %g)", static_cast<double>(temperature));
+  if (!temperatures && !(temperature == 0.f || (temperature >= 1e-30f && temperature <= 3.4e38f)))
+    return fail(FITQ_ERR_ARG, "tree_verify: temperature must be 0 or from 1e-30 on (got %g)", static_cast<double>(temperature));
   const uintptr_t size = dtype == FITQ_DTYPE_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(logits) % size ||
       ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(accepted) | reinterpret_cast<uintptr_t>(next_token)) & 7u) ||

@@ -10,11 +10,20 @@
 // last child the next token is the first whose cumulated p exceeds u_0.
 //
 // Everything is computed in fp64 from the logits: a border between two tokens moves by
-// some 1e-15 with the order of a sum, by 1e-8 in fp32, and a random number falls into
-// that gap once in 10^3 rows of 152,064 tokens.
+// some 1e-14 with the order of a sum and the exponentials' last digits, by 1e-8 in fp32, and a
+// random number falls into that gap once in 10^3 rows of 152,064 tokens (once in 10^6 with
+// what is left here).  An exponential is 2^(n / 1024) from a table times a polynomial of degree
+// two (its Taylor series: 7e-12 of it at |x| <= ln 2 / 2048), summed by the last product:
+// seven fp64 operations and some ten others per element, which the issue of instructions
+// bounds (with twice as many it took 36 us instead of 23 for 64 rows of 152,064).
 //
 // A cluster of up to eight CTAs walks with a sequence; every warp owns a run of the
-// vocabulary, so that the cumulated sum is found by its parts: ranks, warps, lanes.
+// vocabulary, so that the cumulated sum is found by its parts: ranks, warps, lanes.  A CTA sums
+// by its own largest logit, and one exchange over the cluster joins largest logits and
+// sums.  A refused child costs another read of the row (from L1 and L2) with its q.
+// Bound: few sequences, the chain of a row (read, largest, read, exponentials, exchange); many,
+// fp64's rate.
+#include <mutex>
 #include <type_traits>
 
 #include "kernels.cuh"
@@ -25,7 +34,10 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxCtas = 8;
+constexpr int kMaxCtas = 16;
+constexpr int kAlone = 120 * 1024;  // shared memory that leaves an SM to one CTA
+constexpr int kTable = 1024;
+constexpr int kAhead = 2;  // a lane's granules on their way
 
 struct TreeVerifyParams {
   const void* logits;
@@ -55,36 +67,92 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
-__device__ __forceinline__ uint64_t remote_u64(const void* p, uint32_t rank) {
+__device__ __forceinline__ void store_remote(const void* p, uint32_t rank, uint64_t v) {
   uint32_t a;
-  uint64_t v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
 
-// Floats in an order that unsigned comparison follows (-0 as 0), every NaN the largest.
-__device__ __forceinline__ uint32_t order_of(float x) {
-  if (x != x) return 0xffffffffu;
-  const uint32_t u = __float_as_uint(x + 0.0f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+__device__ __forceinline__ void store_remote_f32(const void* p, uint32_t rank, float v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
-__device__ __forceinline__ float value_of(uint32_t o) {
-  return __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
+
+// The larger, a NaN before all.
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float max_vec(const uint4& u) {
+  if constexpr (sizeof(T) == 4) {
+    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else {
+    auto pair = [](uint32_t x, uint32_t y) {
+      uint32_t r;
+      if constexpr (std::is_same<T, __half>::value)
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+      else
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+      return r;
+    };
+    const float2 f = Half16<T>::unpack(pair(pair(u.x, u.y), pair(u.z, u.w)));
+    return max_nan(f.x, f.y);
+  }
+}
+
+// A float as a double by integer operations (the conversion instruction takes two elements per
+// cycle and SM: 36 us for 64 rows, see below).  Zeros and subnormals read as some 2^-127, infinities
+// as 2^128, none of which a weight shows.  16-bit types leave the low word empty.
+template <bool kLow>
+__device__ __forceinline__ double widen(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return __hiloint2double((static_cast<int>(u) >> 3 & 0x8fffffff) + (896 << 20), kLow ? static_cast<int>(u << 29) : 0);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) tree_verify_kernel(const TreeVerifyParams p) {
+__device__ __forceinline__ void unpack_vec(const uint4& u, float (&f)[16 / sizeof(T)]);
+template <>
+__device__ __forceinline__ void unpack_vec<__nv_bfloat16>(const uint4& u, float (&f)[8]) { unpack8<__nv_bfloat16>(u, f); }
+template <>
+__device__ __forceinline__ void unpack_vec<__half>(const uint4& u, float (&f)[8]) { unpack8<__half>(u, f); }
+template <>
+__device__ __forceinline__ void unpack_vec<float>(const uint4& u, float (&f)[4]) {
+  f[0] = __uint_as_float(u.x);
+  f[1] = __uint_as_float(u.y);
+  f[2] = __uint_as_float(u.z);
+  f[3] = __uint_as_float(u.w);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVerifyParams p) {
+  constexpr int kVec = 16 / sizeof(T);
   __shared__ int up[kTreeTokens];
-  __shared__ uint64_t sh_warp[kWarps], sh_mine[2];
+  __shared__ double sh_table[kTable], sh_roots[64];
+  __shared__ float sh_top[kWarps], sh_tops[2][kMaxCtas];   // largest logits; double-buffered by exchange
+  __shared__ double sh_run[kWarps], sh_sums[2][kMaxCtas];
   __shared__ double sh_inv[kTreeTokens];   // 1 / sum of the weights before refusal k
   __shared__ int64_t sh_gone[kTreeTokens]; // ids refused at this token (without q)
+  __shared__ int sh_hit[kWarps], sh_have[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // 2^(j / 1024) in [1, 2) as a product of two of 32, its exponent less by j / 1024 of a binade's
+  // distance: adding n << 10 to the high word then makes it 2^(n / 1024) for every n
+  if (tid < 64) sh_roots[tid] = exp2(static_cast<double>(tid < 32 ? tid : (tid - 32) * 32) / kTable);
+  __syncthreads();
+  for (int j = tid; j < kTable; j += kThreads) {
+    const double e = sh_roots[j & 31] * sh_roots[32 + (j >> 5)];
+    sh_table[j] = __hiloint2double(__double2hiint(e) - (j << 10), __double2loint(e));
+  }
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
   const int64_t b = blockIdx.x / ranks;
   if (tid < p.T) {
@@ -96,7 +164,7 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const TreeVerifyP
   }
   __syncthreads();
   const float temp = p.temperatures ? p.temperatures[b] : p.temperature;
-  if (up[0] != -1 || !(temp >= 0.f) || temp == INFINITY) {  // no token to start from: the whole cluster
+  if (up[0] != -1 || !(temp == 0.f || temp >= 1e-30f) || temp == INFINITY) {  // no token to start from: the whole cluster
     if (tid == 0 && rank == 0) {
       if (up[0] != -2) report_device_error(p.status, FITQ_ERR_ARG);
       p.accepted[b] = -1;
@@ -104,52 +172,52 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const TreeVerifyP
     }
     return;
   }
+  cluster_arrive();  // waited for before the first store into another CTA's shared memory
   const bool greedy = temp == 0.f;
-  const double inv_t = greedy ? 0.0 : 1.0 / static_cast<double>(temp);
-  // this warp's run of the vocabulary
-  const int per = (p.V + static_cast<int>(ranks) * kWarps - 1) / (static_cast<int>(ranks) * kWarps);
-  const int lo = min(p.V, (static_cast<int>(rank) * kWarps + warp) * per), hi = min(p.V, lo + per);
+  // exponents in 1024ths per logit; where a row's largest is so far from 0 that this leaves its weight no
+  // digits, as much less as leaves all others nothing still
+  const double per_logit = greedy ? 0.0 : kTable * 1.4426950408889634074 / static_cast<double>(temp);
+  auto scale_of = [&](float by) {
+    const double far = per_logit * static_cast<double>(fabsf(by));
+    return far <= 1.4e17 ? per_logit : per_logit * (1.4e17 / far);
+  };
   int slot = 0;
-
-  // The cluster's words in the order of its warps; every thread gets all ranks' totals.
-  auto gather = [&](uint64_t mine, auto join, uint64_t (&all)[kMaxCtas]) {
-    if (lane == 0) sh_warp[warp] = mine;
-    __syncthreads();
-    if (tid == 0) {
-      uint64_t x = sh_warp[0];
-      for (int w = 1; w < kWarps; ++w) x = join(x, sh_warp[w]);
-      sh_mine[slot] = x;
-    }
-    cluster_barrier();
-    for (uint32_t r = 0; r < ranks; ++r) all[r] = remote_u64(&sh_mine[slot], r);
-    slot ^= 1;
-  };
-  auto add = [](uint64_t x, uint64_t y) {
-    return static_cast<uint64_t>(__double_as_longlong(__longlong_as_double(x) + __longlong_as_double(y)));
-  };
-  auto larger = [](uint64_t x, uint64_t y) { return x > y ? x : y; };
+  bool fresh = true;
 
   int cur = 0, taken = 0, refused = 0;
   bool usable = true;
   double total = 0.0;
-  float top = 0.f;
+  float top = 0.f;          // the row's largest logit
   int best = 0;
   const T* z = nullptr;
   const float* q = nullptr;
-  // the weight of token v at this point of the walk
-  auto weight = [&](int v) -> double {
-    double w;
-    if (greedy) {
-      w = v == best ? 1.0 : 0.0;
+  const uint4* frame = nullptr;  // the row's 16-byte granules, the first and last perhaps shared with others
+  int lead = 0, lo = 0, hi = 0;  // elements of granule 0 before the row; this warp's granules
+  double rescale = 0.0;          // what makes sh_run this CTA's part of the total
+  double its_sum = 0.0;          // lane r: rank r's part
+  float floor_x = 0.f;
+  double scale = 0.0, start = 0.0;  // of the row's largest logit
+
+  // exp((x - by) / temperature), the weight of a logit before any refusal, where x >= floor_of(by), with
+  // scale = scale_of(by), start = -scale by
+  auto weigh = [&](float x, double scale, double start) -> double {
+    const double v = fma(widen<sizeof(T) == 4>(x), scale, start);
+    const double t = v + 6755399441055744.0;  // 1.5 * 2^52: the whole part in the low bits
+    const double r = v - (t - 6755399441055744.0);
+    constexpr double kL = 0.69314718055994531 / kTable;
+    const int n = __double2loint(t);
+    const double e = sh_table[n & (kTable - 1)];
+    return __hiloint2double(__double2hiint(e) + (n << 10), __double2loint(e)) * fma(r, fma(r, kL * kL / 2.0, kL), 1.0);
+  };
+  // what lies below weighs nothing: some 2^-1020 of the largest
+  auto floor_of = [&](float by) -> float { return __double2float_ru(static_cast<double>(by) - 707.0 * static_cast<double>(temp)); };
+  // what refusals have left of weight w of token v
+  auto left = [&](double w, int v, float qv) -> double {
+    if (q) {
+      for (int k = 0; k < refused; ++k) w = fmax(fma(w, sh_inv[k], -widen<true>(qv)), 0.0);
     } else {
-      const float x = static_cast<float>(z[v]);
-      w = exp((static_cast<double>(x) - static_cast<double>(top)) * inv_t);
-      if (p.probs) {
-        for (int k = 0; k < refused; ++k) w = fmax(w * sh_inv[k] - static_cast<double>(q[v]), 0.0);
-      } else {
-        for (int k = 0; k < refused; ++k)
-          if (sh_gone[k] == v) w = 0.0;
-      }
+      for (int k = 0; k < refused; ++k)
+        if (sh_gone[k] == v) w = 0.0;
     }
     return w;
   };
@@ -157,32 +225,213 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const TreeVerifyP
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
   };
-  uint64_t all[kMaxCtas];
-  double run = 0.0;  // this warp's sum
-  auto sum_up = [&]() {
+  // calls f(element index, place in the granule, logit) for the row's elements of granule i, read as `u`
+  auto elements = [&](int i, const uint4& u, auto f) {
+    float x[kVec];
+    unpack_vec<T>(u, x);
+    const int v0 = i * kVec - lead;
+    if (v0 >= 0 && v0 + kVec <= p.V) {
+#pragma unroll
+      for (int y = 0; y < kVec; ++y) f(v0 + y, y, x[y]);
+    } else {
+#pragma unroll
+      for (int y = 0; y < kVec; ++y)
+        if (v0 + y >= 0 && v0 + y < p.V) f(v0 + y, y, x[y]);
+    }
+  };
+  // calls f(granule, its 16 bytes) for the lane's granules, kAhead of them on their way at once
+  auto granules_of = [&](auto f) {
+    for (int i0 = lo + lane; i0 < hi; i0 += 32 * kAhead) {
+      uint4 u[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) u[k] = i0 + 32 * k < hi ? __ldg(frame + i0 + 32 * k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (i0 + 32 * k < hi) f(i0 + 32 * k, u[k]);
+    }
+  };
+  // q of the elements of granule i
+  auto q_of = [&](int i, float (&f)[kVec]) {
+    const int v0 = i * kVec - lead;
+    const float* src = q + v0;
+    if (v0 >= 0 && v0 + kVec <= p.V && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
+#pragma unroll
+      for (int y = 0; y < kVec; y += 4) {
+        const float4 w = __ldg(reinterpret_cast<const float4*>(src + y));
+        f[y] = w.x;
+        f[y + 1] = w.y;
+        f[y + 2] = w.z;
+        f[y + 3] = w.w;
+      }
+    } else {
+#pragma unroll
+      for (int y = 0; y < kVec; ++y) f[y] = v0 + y >= 0 && v0 + y < p.V ? __ldg(src + y) : 0.f;
+    }
+  };
+  // the weights of granule i, side by side (one after the other, each with its refusals, they took five
+  // times as long)
+  auto weights = [&](int i, const uint4& u, double scale, double start, float low, double (&w)[kVec]) {
+    float x[kVec];
+    unpack_vec<T>(u, x);
+#pragma unroll
+    for (int y = 0; y < kVec; ++y) w[y] = weigh(x[y], scale, start);
+#pragma unroll
+    for (int y = 0; y < kVec; ++y) w[y] = x[y] >= low ? w[y] : 0.0;
+    const int v0 = i * kVec - lead;
+    if (v0 < 0 || v0 + kVec > p.V) {
+#pragma unroll
+      for (int y = 0; y < kVec; ++y)
+        if (v0 + y < 0 || v0 + y >= p.V) w[y] = 0.0;
+    }
+  };
+  auto refuse = [&](int i, double (&w)[kVec]) {
+    if (refused == 0) return;
+    if (q) {
+      float qv[kVec];
+      q_of(i, qv);
+      for (int k = 0; k < refused; ++k) {
+        const double inv = sh_inv[k];
+#pragma unroll
+        for (int y = 0; y < kVec; ++y) {
+          w[y] = fma(w[y], inv, -widen<true>(qv[y]));
+          w[y] = w[y] > 0.0 ? w[y] : 0.0;
+        }
+      }
+    } else {
+      for (int k = 0; k < refused; ++k) {
+        const int64_t at = sh_gone[k] - (i * kVec - lead);
+#pragma unroll
+        for (int y = 0; y < kVec; ++y)
+          if (at == y) w[y] = 0.0;
+      }
+    }
+  };
+  auto total_of = [](const double (&w)[kVec]) {
+    double s[kVec / 2];
+#pragma unroll
+    for (int y = 0; y < kVec / 2; ++y) s[y] = w[2 * y] + w[2 * y + 1];
+    if constexpr (kVec == 8) return (s[0] + s[1]) + (s[2] + s[3]);
+    return s[0] + s[1];
+  };
+  // sh_run's sum (and this CTA's largest logit) to all CTAs; on return sh_sums[slot ^ 1] and
+  // sh_tops[slot ^ 1] hold the ranks'
+  auto exchange = [&](bool tops, float mine) {
+    __syncthreads();
+    if (fresh) cluster_wait();  // every CTA of the cluster runs
+    fresh = false;
+    if (warp == 0) {
+      double s = lane < kWarps ? sh_run[lane] : 0.0;
+      s = warp_sum(s);
+      if (lane < static_cast<int>(ranks)) {
+        store_remote(&sh_sums[slot][rank], lane, static_cast<uint64_t>(__double_as_longlong(s)));
+        if (tops) store_remote_f32(&sh_tops[slot][rank], lane, mine);
+      }
+    }
+    cluster_barrier();
+    slot ^= 1;
+  };
+  // the largest of this CTA's logits, for all its threads
+  auto largest = [&]() -> float {
+    float m = -INFINITY;
+    granules_of([&](int i, const uint4& u) {
+      const int v0 = i * kVec - lead;
+      if (v0 >= 0 && v0 + kVec <= p.V)
+        m = max_nan(m, max_vec<T>(u));
+      else
+        elements(i, u, [&](int, int, float x) { m = max_nan(m, x); });
+    });
+    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) sh_top[warp] = m;
+    __syncthreads();
+    m = sh_top[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) m = max_nan(m, sh_top[w]);
+    return m;
+  };
+  // the row's first token with logit x, for the whole cluster
+  auto first_of = [&](float x) -> int {
+    int at = 0x7fffffff;
+    granules_of([&](int i, const uint4& u) {
+      elements(i, u, [&](int v, int, float y) {
+        if (y == x && v < at) at = v;
+      });
+    });
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) sh_run[warp] = static_cast<double>(at);
+    __syncthreads();
+    double low = sh_run[0];
+    for (int w = 1; w < kWarps; ++w) low = fmin(low, sh_run[w]);
+    __syncthreads();
+    if (lane == 0) sh_run[warp] = warp == 0 ? low : 0.0;  // the exchange adds the warps' up
+    exchange(false, 0.f);
+    low = sh_sums[slot ^ 1][0];
+    for (uint32_t r = 1; r < ranks; ++r) low = fmin(low, sh_sums[slot ^ 1][r]);
+    return static_cast<int>(low);
+  };
+  // the weight of one logit, by the row's largest
+  auto point = [&](float x) -> double { return x >= floor_x ? weigh(x, scale, start) : 0.0; };
+  auto sum_up = [&]() {  // the weights' sum after another refusal
     double s = 0.0;
-    for (int v = lo + lane; v < hi; v += 32) s += weight(v);
-    run = warp_sum(s);
-    gather(static_cast<uint64_t>(__double_as_longlong(run)), add, all);
-    total = 0.0;
-    for (uint32_t r = 0; r < ranks; ++r) total += __longlong_as_double(all[r]);
+    granules_of([&](int i, const uint4& u) {
+      double w[kVec];
+      weights(i, u, scale, start, floor_x, w);
+      refuse(i, w);
+      s += total_of(w);
+    });
+    s = warp_sum(s);
+    if (lane == 0) sh_run[warp] = s;
+    exchange(false, 0.f);
+    its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] : 0.0;
+    total = warp_sum(its_sum);
+    rescale = 1.0;
   };
   auto enter = [&]() {  // the row of token cur
     z = static_cast<const T*>(p.logits) + b * p.stride_b + cur * p.stride_t;
     q = p.probs ? p.probs + b * p.probs_stride_b + min(cur, p.T - 2) * p.probs_stride_t : nullptr;
     refused = 0;
-    uint64_t key = 0;
-    for (int v = lo + lane; v < hi; v += 32) {
-      const uint64_t k = (static_cast<uint64_t>(order_of(static_cast<float>(z[v]))) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
-      key = key > k ? key : k;
+    frame = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(z) & ~static_cast<uintptr_t>(15));
+    lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
+    const int granules = (lead + p.V + kVec - 1) / kVec, warps = static_cast<int>(ranks) * kWarps;
+    const int per = (granules + warps - 1) / warps;
+    lo = min(granules, (static_cast<int>(rank) * kWarps + warp) * per);
+    hi = min(granules, lo + per);
+    // ---- the CTA's largest logit (a NaN counts as the largest)
+    const float mine = largest();
+    // ---- its weights' sum, by that logit
+    const bool sums = !greedy && fabsf(mine) < INFINITY;
+    double s = 0.0;
+    if (sums) {
+      const double by = scale_of(mine), from = -by * static_cast<double>(mine);
+      const float low = floor_of(mine);
+      granules_of([&](int i, const uint4& u) {
+        double w[kVec];
+        weights(i, u, by, from, low, w);
+        s += total_of(w);
+      });
     }
-    for (int o = 16; o; o >>= 1) key = larger(key, __shfl_xor_sync(0xffffffffu, key, o));
-    gather(key, larger, all);
-    for (uint32_t r = 0; r < ranks; ++r) key = larger(key, all[r]);
-    top = value_of(static_cast<uint32_t>(key >> 32));
-    best = static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
-    usable = static_cast<uint32_t>(key >> 32) != 0xffffffffu && top != -INFINITY && (greedy || top != INFINITY);
-    if (usable) sum_up();
+    s = warp_sum(s);
+    if (lane == 0) sh_run[warp] = s;
+    exchange(true, mine);
+    top = -INFINITY;
+    bool odd = false;
+    for (uint32_t r = 0; r < ranks; ++r) {
+      const float its = sh_tops[slot ^ 1][r];
+      odd = odd || its != its;
+      top = fmaxf(top, its);
+    }
+    usable = !odd && top != -INFINITY && (greedy || top != INFINITY);
+    if (!usable) return;
+    if (greedy) {
+      best = first_of(top);
+      return;
+    }
+    floor_x = floor_of(top);
+    scale = scale_of(top);
+    start = -scale * static_cast<double>(top);
+    // the ranks' sums, by the row's largest logit: a lane each
+    its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] * point(sh_tops[slot ^ 1][lane]) : 0.0;
+    total = warp_sum(its_sum);
+    rescale = point(mine);
   };
 
   enter();
@@ -191,14 +440,18 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const TreeVerifyP
     if (up[i] != cur) continue;
     const int64_t x = p.tokens[b * p.T + i];
     const bool known = x >= 0 && x < p.V;
-    const double u = p.uniforms[b * p.T + i];
-    const double w = known ? weight(static_cast<int>(x)) : 0.0;
-    const bool take = known && total > 0.0 && (greedy ? w > 0.0 : u * (q ? static_cast<double>(q[x]) : 1.0) * total < w);
+    bool take = false;
+    if (greedy) {
+      take = known && x == best;
+    } else if (known && total > 0.0) {
+      const double u = p.uniforms[b * p.T + i];
+      const float qx = q ? q[x] : 1.f;
+      take = u * static_cast<double>(qx) * total < left(point(static_cast<float>(z[x])), static_cast<int>(x), qx);
+    }
     if (take) {
       cur = i;
       ++taken;
       if (tid == 0 && rank == 0) p.path[b * p.T + taken] = i;
-      __syncthreads();
       enter();
     } else if (!greedy && total > 0.0) {
       __syncthreads();  // weights read the refusals so far
@@ -211,16 +464,17 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const TreeVerifyP
       sum_up();
     }
   }
-  int64_t next = -1;
-  if (usable && (greedy || !(total > 0.0))) {
-    next = best;
-  } else if (usable) {
+  if (tid == 0 && rank == 0) p.accepted[b] = taken;
+  if (!usable || greedy || !(total > 0.0)) {
+    if (usable && !greedy) best = first_of(top);  // refusals have left no weight
+    if (tid == 0 && rank == 0) p.next_token[b] = usable ? best : -1;
+  } else {
     // the first token whose cumulated weight exceeds u_0 of the total
     const double goal = static_cast<double>(p.uniforms[b * p.T]) * total;
     double before = 0.0;
     int at = -1, last = 0;
     for (int r = 0; r < static_cast<int>(ranks); ++r) {
-      const double s = __longlong_as_double(all[r]);
+      const double s = __shfl_sync(0xffffffffu, its_sum, r);
       if (s > 0.0) last = r;
       if (at < 0 && before + s > goal) at = r;
       if (at < 0) before += s;
@@ -228,53 +482,99 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const TreeVerifyP
     const bool past = at < 0;  // a random number of one or more: the last token that has weight
     if (past) at = last;
     if (static_cast<int>(rank) == at) {
-      // sh_warp still holds the sums of this CTA's warps
       int w_at = -1, w_last = 0;
       double base = past ? 0.0 : before;
       for (int w = 0; w < kWarps; ++w) {
-        const double s = __longlong_as_double(sh_warp[w]);
+        const double s = sh_run[w] * rescale;
         if (s > 0.0) w_last = w;
         if (!past && w_at < 0 && base + s > goal) w_at = w;
         if (w_at < 0 && !past) base += s;
       }
       if (w_at < 0) w_at = w_last;
-      if (warp == w_at) {
-        int found = -1, heavy = lo;
-        for (int v0 = lo; v0 < hi && found < 0; v0 += 32) {
-          const int v = v0 + lane;
-          const double w = v < hi ? weight(v) : 0.0;
-          double c = w;
-          for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xffffffffu, c, o);
-            if (lane >= o) c += y;
-          }
-          const uint32_t have = __ballot_sync(0xffffffffu, w > 0.0);
-          const uint32_t hit = __ballot_sync(0xffffffffu, w > 0.0 && base + c > goal);
-          if (have) heavy = v0 + 31 - __clz(have);
-          if (!past && hit) found = v0 + __ffs(hit) - 1;
-          base += __shfl_sync(0xffffffffu, c, 31);
+      // that run again, 32 granules a warp, then the warp in whose granules it lies
+      const int granules = (lead + p.V + kVec - 1) / kVec, warps = static_cast<int>(ranks) * kWarps;
+      const int per = (granules + warps - 1) / warps, first = min(granules, (static_cast<int>(rank) * kWarps + w_at) * per);
+      const int end = min(granules, first + per);
+      int found = -1, heavy = -1;
+      for (int i0 = first; i0 < end && found < 0; i0 += 32 * kWarps) {
+        const int i = i0 + 32 * warp + lane;
+        double w[kVec], mine = 0.0;
+#pragma unroll
+        for (int y = 0; y < kVec; ++y) w[y] = 0.0;
+        if (i < end) {
+          weights(i, __ldg(frame + i), scale, start, floor_x, w);
+          refuse(i, w);
         }
-        if (lane == 0) p.next_token[b] = found >= 0 ? found : heavy;
+#pragma unroll
+        for (int y = 0; y < kVec; ++y) mine += w[y];
+        double c = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, c, o);
+          if (lane >= o) c += y;
+        }
+        __syncthreads();  // sh_run has been read
+        if (lane == 31) sh_run[warp] = c;
+        __syncthreads();
+        double at_warp = base;  // what lies before this warp's granules
+        for (int k = 0; k < warp; ++k) at_warp += sh_run[k];
+        for (int k = 0; k < kWarps; ++k) base += sh_run[k];
+        // within the lane's elements
+        int hit = -1, have = -1;
+        double sum = at_warp + (c - mine);
+#pragma unroll
+        for (int y = 0; y < kVec; ++y) {
+          sum += w[y];
+          if (w[y] > 0.0) {
+            have = i * kVec - lead + y;
+            if (hit < 0 && !past && sum > goal) hit = have;
+          }
+        }
+        const uint32_t hits = __ballot_sync(0xffffffffu, hit >= 0), haves = __ballot_sync(0xffffffffu, have >= 0);
+        if (lane == 0) {
+          sh_hit[warp] = -1;
+          sh_have[warp] = -1;
+        }
+        __syncwarp();
+        if (hits && lane == __ffs(hits) - 1) sh_hit[warp] = hit;
+        if (haves && lane == 31 - __clz(haves)) sh_have[warp] = have;
+        __syncthreads();
+        for (int k = 0; k < kWarps; ++k) {
+          if (found < 0) found = sh_hit[k];
+          if (sh_have[k] >= 0) heavy = sh_have[k];
+        }
       }
+      if (tid == 0) p.next_token[b] = found >= 0 ? found : heavy;
     }
-    if (tid == 0 && rank == 0) p.accepted[b] = taken;
-    cluster_barrier();  // no CTA leaves while its words are read
-    return;
   }
-  if (tid == 0 && rank == 0) {
-    p.accepted[b] = taken;
-    p.next_token[b] = next;
-  }
-  cluster_barrier();
+  cluster_barrier();  // no CTA leaves while its words are written
 }
 
 template <typename T>
 int verify_t(const TreeVerifyParams& p, int64_t batch, cudaStream_t st, int num_sms) {
+  // CTAs of a sequence: as many as find room at once, two on an SM, and have a granule for every
+  // lane; sixteen where they fill a third of the card at most (their clusters need whole GPCs).
   int ctas = 1;
-  while (ctas < kMaxCtas && batch * ctas * 2 <= 2ll * num_sms && p.V > kThreads * ctas * 2) ctas *= 2;
+  while (ctas < 8 && batch * ctas * 2 <= 2ll * num_sms && p.V > kThreads * ctas * 2) ctas *= 2;
+  auto* kernel = tree_verify_kernel<T>;
+  if (ctas == 8 && batch * 48 <= num_sms && p.V > kThreads * 16) {
+    static std::mutex mu;
+    static bool done[64] = {false};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FITQ_ERR_CUDA;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!done[dev] && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return FITQ_ERR_CUDA;
+    done[dev] = true;
+    ctas = 16;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch * ctas));
   cfg.blockDim = dim3(kThreads);
+  // few CTAs spread over the SMs instead of meeting on some of them
+  if (batch * ctas <= num_sms / 2) {
+    if (!set_smem_limit(kernel, kAlone)) return FITQ_ERR_CUDA;
+    cfg.dynamicSmemBytes = kAlone;
+  }
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -284,7 +584,7 @@ int verify_t(const TreeVerifyParams& p, int64_t batch, cudaStream_t st, int num_
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_verify_kernel<T>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   return launch_result();

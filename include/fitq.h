@@ -481,7 +481,8 @@ FITQ_API int fitq_tree_attention(const fitq_tree* tree, const void* q, int64_t q
  * refusal takes id out of p.  Behind the last child next_token is the first whose cumulated p
  * exceeds uniforms[0].  An id outside [0, vocab) is refused.  temperature 0: p is 1 at
  * the largest logit, the lower index where two are equal, and children are compared with it.
- * temperatures fp32 [batch] or NULL (then `temperature`, not negative).
+ * temperatures fp32 [batch] or NULL (then `temperature`), 0 or from 1e-30 on; a sequence with
+ * another one records FITQ_ERR_ARG and counts as one without token 0.
  * path int32 [batch, tokens]: token 0 and the accepted ones, then -1; accepted int64 [batch]:
  * how many drafts; next_token int64 [batch].  A row with a NaN, or without a finite largest logit,
  * ends the walk with next_token -1; a sequence without token 0 gives accepted -1, next_token
