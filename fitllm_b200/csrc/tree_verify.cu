@@ -32,8 +32,6 @@
 namespace fitq {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCtas = 16;
 constexpr int kAlone = 120 * 1024;  // shared memory that leaves an SM to one CTA
 constexpr int kTable = 1024;
@@ -132,8 +130,130 @@ __device__ __forceinline__ void unpack_vec<float>(const uint4& u, float (&f)[4])
   f[3] = __uint_as_float(u.w);
 }
 
+// 2^(j / 1024) in [1, 2), its high word less by j << 10: adding n << 10 for any n with n & 1023 = j
+// then makes it 2^(n / 1024).  By all threads of a CTA.
+__device__ __forceinline__ void make_table(double* table, double* roots) {
+  if (threadIdx.x < 64) roots[threadIdx.x] = exp2(static_cast<double>(threadIdx.x < 32 ? threadIdx.x : (threadIdx.x - 32) * 32) / kTable);
+  __syncthreads();
+  for (int j = threadIdx.x; j < kTable; j += blockDim.x) {
+    const double e = roots[j & 31] * roots[32 + (j >> 5)];
+    table[j] = __hiloint2double(__double2hiint(e) - (j << 10), __double2loint(e));
+  }
+}
+
+// Weights exp((x - top) / temperature) of logits.
+struct Scale {
+  double scale, start;  // exponent in 1024ths: scale x + start
+  float low;            // what lies below weighs nothing: some 2^-1020 of the largest
+  // Where the largest is so far from 0 that its weight would have no digits left, the exponents are as
+  // much smaller as leaves all other logits nothing still.
+  __device__ __forceinline__ void set(float top, float temp) {
+    const double per = kTable * 1.4426950408889634074 / static_cast<double>(temp), far = per * static_cast<double>(fabsf(top));
+    scale = far <= 1.4e17 ? per : per * (1.4e17 / far);
+    start = -scale * static_cast<double>(top);
+    low = __double2float_ru(static_cast<double>(top) - 707.0 * static_cast<double>(temp));
+  }
+  template <bool kLow>
+  __device__ __forceinline__ double weigh(const double* table, float x) const {  // for x >= low
+    const double v = fma(widen<kLow>(x), scale, start);
+    const double t = v + 6755399441055744.0;  // 1.5 * 2^52: the whole part in the low bits
+    const double r = v - (t - 6755399441055744.0);
+    constexpr double kL = 0.69314718055994531 / kTable;
+    const int n = __double2loint(t);
+    const double e = table[n & (kTable - 1)];
+    return __hiloint2double(__double2hiint(e) + (n << 10), __double2loint(e)) * fma(r, fma(r, kL * kL / 2.0, kL), 1.0);
+  }
+  __device__ __forceinline__ double point(const double* table, float x) const { return x >= low ? weigh<true>(table, x) : 0.0; }
+};
+
+// A row of logits as 16-byte granules, the first and the last perhaps shared with other rows.
 template <typename T>
+struct Row {
+  static constexpr int kVec = 16 / sizeof(T);
+  const uint4* frame;
+  int lead, V, granules;
+  __device__ __forceinline__ Row(const T* z, int v) : V(v) {
+    frame = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(z) & ~static_cast<uintptr_t>(15));
+    lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
+    granules = (lead + V + kVec - 1) / kVec;
+  }
+  __device__ __forceinline__ int first(int i) const { return i * kVec - lead; }  // index of granule i's element 0
+  __device__ __forceinline__ bool inside(int i) const { return first(i) >= 0 && first(i) + kVec <= V; }
+  // calls f(granule, its 16 bytes) for granules lo + lane, lo + lane + 32 .. below hi, kAhead on their way
+  template <typename F>
+  __device__ __forceinline__ void each(int lo, int hi, F f) const {
+    for (int i0 = lo + static_cast<int>(threadIdx.x & 31); i0 < hi; i0 += 32 * kAhead) {
+      uint4 u[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) u[k] = i0 + 32 * k < hi ? __ldg(frame + i0 + 32 * k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (i0 + 32 * k < hi) f(i0 + 32 * k, u[k]);
+    }
+  }
+  // the largest of a warp's granules, a NaN before all
+  __device__ __forceinline__ float largest(int lo, int hi) const {
+    float m = -INFINITY;
+    each(lo, hi, [&](int i, const uint4& u) {
+      if (inside(i)) {
+        m = max_nan(m, max_vec<T>(u));
+      } else {
+        float x[kVec];
+        unpack_vec<T>(u, x);
+#pragma unroll
+        for (int y = 0; y < kVec; ++y)
+          if (first(i) + y >= 0 && first(i) + y < V) m = max_nan(m, x[y]);
+      }
+    });
+    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+  }
+  // the first index of a warp's granules with logit x, or 2^31 - 1
+  __device__ __forceinline__ int first_of(int lo, int hi, float x) const {
+    int at = 0x7fffffff;
+    each(lo, hi, [&](int i, const uint4& u) {
+      float f[kVec];
+      unpack_vec<T>(u, f);
+#pragma unroll
+      for (int y = kVec - 1; y >= 0; --y) {
+        const int v = first(i) + y;
+        if (f[y] == x && v >= 0 && v < V && v < at) at = v;
+      }
+    });
+    return __reduce_min_sync(0xffffffffu, at);
+  }
+  // the weights of a granule, side by side (one after the other, each with its refusals, they took five
+  // times as long)
+  __device__ __forceinline__ void weights(const double* table, const Scale& s, int i, const uint4& u, double (&w)[kVec]) const {
+    float x[kVec];
+    unpack_vec<T>(u, x);
+#pragma unroll
+    for (int y = 0; y < kVec; ++y) w[y] = s.weigh<sizeof(T) == 4>(table, x[y]);
+#pragma unroll
+    for (int y = 0; y < kVec; ++y) w[y] = x[y] >= s.low ? w[y] : 0.0;
+    if (!inside(i)) {
+#pragma unroll
+      for (int y = 0; y < kVec; ++y)
+        if (first(i) + y < 0 || first(i) + y >= V) w[y] = 0.0;
+    }
+  }
+  static __device__ __forceinline__ double total_of(const double (&w)[kVec]) {
+    double s[kVec / 2];
+#pragma unroll
+    for (int y = 0; y < kVec / 2; ++y) s[y] = w[2 * y] + w[2 * y + 1];
+    if constexpr (kVec == 8) return (s[0] + s[1]) + (s[2] + s[3]);
+    return s[0] + s[1];
+  }
+};
+
+__device__ __forceinline__ double warp_sum(double s) {
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVerifyParams p) {
+  constexpr int kWarps = kThreads / 32;
   constexpr int kVec = 16 / sizeof(T);
   __shared__ int up[kTreeTokens];
   __shared__ double sh_table[kTable], sh_roots[64];
@@ -143,14 +263,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
   __shared__ int64_t sh_gone[kTreeTokens]; // ids refused at this token (without q)
   __shared__ int sh_hit[kWarps], sh_have[kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // 2^(j / 1024) in [1, 2) as a product of two of 32, its exponent less by j / 1024 of a binade's
-  // distance: adding n << 10 to the high word then makes it 2^(n / 1024) for every n
-  if (tid < 64) sh_roots[tid] = exp2(static_cast<double>(tid < 32 ? tid : (tid - 32) * 32) / kTable);
-  __syncthreads();
-  for (int j = tid; j < kTable; j += kThreads) {
-    const double e = sh_roots[j & 31] * sh_roots[32 + (j >> 5)];
-    sh_table[j] = __hiloint2double(__double2hiint(e) - (j << 10), __double2loint(e));
-  }
+  make_table(sh_table, sh_roots);
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t rank = cluster_rank(), ranks = cluster_size();
@@ -174,43 +287,24 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
   }
   cluster_arrive();  // waited for before the first store into another CTA's shared memory
   const bool greedy = temp == 0.f;
-  // exponents in 1024ths per logit; where a row's largest is so far from 0 that this leaves its weight no
-  // digits, as much less as leaves all others nothing still
-  const double per_logit = greedy ? 0.0 : kTable * 1.4426950408889634074 / static_cast<double>(temp);
-  auto scale_of = [&](float by) {
-    const double far = per_logit * static_cast<double>(fabsf(by));
-    return far <= 1.4e17 ? per_logit : per_logit * (1.4e17 / far);
-  };
   int slot = 0;
   bool fresh = true;
 
   int cur = 0, taken = 0, refused = 0;
   bool usable = true;
-  double total = 0.0;
+  double total = 0.0;       // of the weights as refusals have left them
+  double entered = 0.0;     // the total before any refusal
+  bool pared = false;       // refusals have been taken out of total, its_sum and sh_run one by one
   float top = 0.f;          // the row's largest logit
   int best = 0;
+  Scale by{};
   const T* z = nullptr;
   const float* q = nullptr;
-  const uint4* frame = nullptr;  // the row's 16-byte granules, the first and last perhaps shared with others
-  int lead = 0, lo = 0, hi = 0;  // elements of granule 0 before the row; this warp's granules
-  double rescale = 0.0;          // what makes sh_run this CTA's part of the total
-  double its_sum = 0.0;          // lane r: rank r's part
-  float floor_x = 0.f;
-  double scale = 0.0, start = 0.0;  // of the row's largest logit
+  Row<T> row(static_cast<const T*>(p.logits), p.V);
+  int lo = 0, hi = 0;       // this warp's granules
+  double rescale = 0.0;     // what makes sh_run this CTA's part of the total
+  double its_sum = 0.0;     // lane r: rank r's part
 
-  // exp((x - by) / temperature), the weight of a logit before any refusal, where x >= floor_of(by), with
-  // scale = scale_of(by), start = -scale by
-  auto weigh = [&](float x, double scale, double start) -> double {
-    const double v = fma(widen<sizeof(T) == 4>(x), scale, start);
-    const double t = v + 6755399441055744.0;  // 1.5 * 2^52: the whole part in the low bits
-    const double r = v - (t - 6755399441055744.0);
-    constexpr double kL = 0.69314718055994531 / kTable;
-    const int n = __double2loint(t);
-    const double e = sh_table[n & (kTable - 1)];
-    return __hiloint2double(__double2hiint(e) + (n << 10), __double2loint(e)) * fma(r, fma(r, kL * kL / 2.0, kL), 1.0);
-  };
-  // what lies below weighs nothing: some 2^-1020 of the largest
-  auto floor_of = [&](float by) -> float { return __double2float_ru(static_cast<double>(by) - 707.0 * static_cast<double>(temp)); };
   // what refusals have left of weight w of token v
   auto left = [&](double w, int v, float qv) -> double {
     if (q) {
@@ -221,74 +315,26 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     }
     return w;
   };
-  auto warp_sum = [&](double s) {
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
-  };
-  // calls f(element index, place in the granule, logit) for the row's elements of granule i, read as `u`
-  auto elements = [&](int i, const uint4& u, auto f) {
-    float x[kVec];
-    unpack_vec<T>(u, x);
-    const int v0 = i * kVec - lead;
-    if (v0 >= 0 && v0 + kVec <= p.V) {
-#pragma unroll
-      for (int y = 0; y < kVec; ++y) f(v0 + y, y, x[y]);
-    } else {
-#pragma unroll
-      for (int y = 0; y < kVec; ++y)
-        if (v0 + y >= 0 && v0 + y < p.V) f(v0 + y, y, x[y]);
-    }
-  };
-  // calls f(granule, its 16 bytes) for the lane's granules, kAhead of them on their way at once
-  auto granules_of = [&](auto f) {
-    for (int i0 = lo + lane; i0 < hi; i0 += 32 * kAhead) {
-      uint4 u[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) u[k] = i0 + 32 * k < hi ? __ldg(frame + i0 + 32 * k) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (i0 + 32 * k < hi) f(i0 + 32 * k, u[k]);
-    }
-  };
-  // q of the elements of granule i
-  auto q_of = [&](int i, float (&f)[kVec]) {
-    const int v0 = i * kVec - lead;
-    const float* src = q + v0;
-    if (v0 >= 0 && v0 + kVec <= p.V && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
-#pragma unroll
-      for (int y = 0; y < kVec; y += 4) {
-        const float4 w = __ldg(reinterpret_cast<const float4*>(src + y));
-        f[y] = w.x;
-        f[y + 1] = w.y;
-        f[y + 2] = w.z;
-        f[y + 3] = w.w;
-      }
-    } else {
-#pragma unroll
-      for (int y = 0; y < kVec; ++y) f[y] = v0 + y >= 0 && v0 + y < p.V ? __ldg(src + y) : 0.f;
-    }
-  };
-  // the weights of granule i, side by side (one after the other, each with its refusals, they took five
-  // times as long)
-  auto weights = [&](int i, const uint4& u, double scale, double start, float low, double (&w)[kVec]) {
-    float x[kVec];
-    unpack_vec<T>(u, x);
-#pragma unroll
-    for (int y = 0; y < kVec; ++y) w[y] = weigh(x[y], scale, start);
-#pragma unroll
-    for (int y = 0; y < kVec; ++y) w[y] = x[y] >= low ? w[y] : 0.0;
-    const int v0 = i * kVec - lead;
-    if (v0 < 0 || v0 + kVec > p.V) {
-#pragma unroll
-      for (int y = 0; y < kVec; ++y)
-        if (v0 + y < 0 || v0 + y >= p.V) w[y] = 0.0;
-    }
-  };
+  // the same of granule i's weights
   auto refuse = [&](int i, double (&w)[kVec]) {
     if (refused == 0) return;
+    const int v0 = row.first(i);
     if (q) {
       float qv[kVec];
-      q_of(i, qv);
+      const float* src = q + v0;
+      if (row.inside(i) && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
+#pragma unroll
+        for (int y = 0; y < kVec; y += 4) {
+          const float4 f = __ldg(reinterpret_cast<const float4*>(src + y));
+          qv[y] = f.x;
+          qv[y + 1] = f.y;
+          qv[y + 2] = f.z;
+          qv[y + 3] = f.w;
+        }
+      } else {
+#pragma unroll
+        for (int y = 0; y < kVec; ++y) qv[y] = v0 + y >= 0 && v0 + y < p.V ? __ldg(src + y) : 0.f;
+      }
       for (int k = 0; k < refused; ++k) {
         const double inv = sh_inv[k];
 #pragma unroll
@@ -299,19 +345,12 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
       }
     } else {
       for (int k = 0; k < refused; ++k) {
-        const int64_t at = sh_gone[k] - (i * kVec - lead);
+        const int64_t at = sh_gone[k] - v0;
 #pragma unroll
         for (int y = 0; y < kVec; ++y)
           if (at == y) w[y] = 0.0;
       }
     }
-  };
-  auto total_of = [](const double (&w)[kVec]) {
-    double s[kVec / 2];
-#pragma unroll
-    for (int y = 0; y < kVec / 2; ++y) s[y] = w[2 * y] + w[2 * y + 1];
-    if constexpr (kVec == 8) return (s[0] + s[1]) + (s[2] + s[3]);
-    return s[0] + s[1];
   };
   // sh_run's sum (and this CTA's largest logit) to all CTAs; on return sh_sums[slot ^ 1] and
   // sh_tops[slot ^ 1] hold the ranks'
@@ -330,33 +369,31 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     cluster_barrier();
     slot ^= 1;
   };
-  // the largest of this CTA's logits, for all its threads
-  auto largest = [&]() -> float {
-    float m = -INFINITY;
-    granules_of([&](int i, const uint4& u) {
-      const int v0 = i * kVec - lead;
-      if (v0 >= 0 && v0 + kVec <= p.V)
-        m = max_nan(m, max_vec<T>(u));
-      else
-        elements(i, u, [&](int, int, float x) { m = max_nan(m, x); });
-    });
-    for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) sh_top[warp] = m;
-    __syncthreads();
-    m = sh_top[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) m = max_nan(m, sh_top[w]);
-    return m;
-  };
-  // the row's first token with logit x, for the whole cluster
-  auto first_of = [&](float x) -> int {
-    int at = 0x7fffffff;
-    granules_of([&](int i, const uint4& u) {
-      elements(i, u, [&](int v, int, float y) {
-        if (y == x && v < at) at = v;
+  auto sum_runs = [&](float mine, const Scale& s) {  // this warp's weights, as refusals have left them
+    double sum = 0.0;
+    if (fabsf(mine) < INFINITY)
+      row.each(lo, hi, [&](int i, const uint4& u) {
+        double w[kVec];
+        row.weights(sh_table, s, i, u, w);
+        refuse(i, w);
+        sum += Row<T>::total_of(w);
       });
-    });
-    at = __reduce_min_sync(0xffffffffu, at);
+    sum = warp_sum(sum);
+    if (lane == 0) sh_run[warp] = sum;
+  };
+  auto sum_up = [&]() {  // by the row's largest logit, which is known
+    __syncthreads();
+    sum_runs(top, by);
+    exchange(false, 0.f);
+    its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] : 0.0;
+    total = warp_sum(its_sum);
+    rescale = 1.0;
+    pared = false;
+  };
+  // the row's first token with its largest logit, by the whole cluster
+  auto find_best = [&]() {
+    const int at = row.first_of(lo, hi, top);
+    __syncthreads();
     if (lane == 0) sh_run[warp] = static_cast<double>(at);
     __syncthreads();
     double low = sh_run[0];
@@ -366,72 +403,42 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     exchange(false, 0.f);
     low = sh_sums[slot ^ 1][0];
     for (uint32_t r = 1; r < ranks; ++r) low = fmin(low, sh_sums[slot ^ 1][r]);
-    return static_cast<int>(low);
-  };
-  // the weight of one logit, by the row's largest
-  auto point = [&](float x) -> double { return x >= floor_x ? weigh(x, scale, start) : 0.0; };
-  auto sum_up = [&]() {  // the weights' sum after another refusal
-    double s = 0.0;
-    granules_of([&](int i, const uint4& u) {
-      double w[kVec];
-      weights(i, u, scale, start, floor_x, w);
-      refuse(i, w);
-      s += total_of(w);
-    });
-    s = warp_sum(s);
-    if (lane == 0) sh_run[warp] = s;
-    exchange(false, 0.f);
-    its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] : 0.0;
-    total = warp_sum(its_sum);
-    rescale = 1.0;
+    best = static_cast<int>(low);
   };
   auto enter = [&]() {  // the row of token cur
     z = static_cast<const T*>(p.logits) + b * p.stride_b + cur * p.stride_t;
     q = p.probs ? p.probs + b * p.probs_stride_b + min(cur, p.T - 2) * p.probs_stride_t : nullptr;
     refused = 0;
-    frame = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(z) & ~static_cast<uintptr_t>(15));
-    lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
-    const int granules = (lead + p.V + kVec - 1) / kVec, warps = static_cast<int>(ranks) * kWarps;
-    const int per = (granules + warps - 1) / warps;
-    lo = min(granules, (static_cast<int>(rank) * kWarps + warp) * per);
-    hi = min(granules, lo + per);
-    // ---- the CTA's largest logit (a NaN counts as the largest)
-    const float mine = largest();
-    // ---- its weights' sum, by that logit
-    const bool sums = !greedy && fabsf(mine) < INFINITY;
-    double s = 0.0;
-    if (sums) {
-      const double by = scale_of(mine), from = -by * static_cast<double>(mine);
-      const float low = floor_of(mine);
-      granules_of([&](int i, const uint4& u) {
-        double w[kVec];
-        weights(i, u, by, from, low, w);
-        s += total_of(w);
-      });
-    }
-    s = warp_sum(s);
-    if (lane == 0) sh_run[warp] = s;
+    pared = false;
+    row = Row<T>(z, p.V);
+    const int warps = static_cast<int>(ranks) * kWarps, per = (row.granules + warps - 1) / warps;
+    lo = min(row.granules, (static_cast<int>(rank) * kWarps + warp) * per);
+    hi = min(row.granules, lo + per);
+    // ---- the CTA's largest logit, its weights' sum by it, and the cluster's
+    float mine = row.largest(lo, hi);
+    if (lane == 0) sh_top[warp] = mine;
+    __syncthreads();
+    mine = sh_top[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) mine = max_nan(mine, sh_top[w]);
+    Scale own{};
+    if (!greedy) own.set(mine, temp);
+    sum_runs(greedy ? INFINITY : mine, own);
     exchange(true, mine);
     top = -INFINITY;
-    bool odd = false;
-    for (uint32_t r = 0; r < ranks; ++r) {
-      const float its = sh_tops[slot ^ 1][r];
-      odd = odd || its != its;
-      top = fmaxf(top, its);
-    }
-    usable = !odd && top != -INFINITY && (greedy || top != INFINITY);
+    for (uint32_t r = 0; r < ranks; ++r) top = max_nan(top, sh_tops[slot ^ 1][r]);
+    usable = top == top && top != -INFINITY && (greedy || top != INFINITY);
     if (!usable) return;
     if (greedy) {
-      best = first_of(top);
+      find_best();
       return;
     }
-    floor_x = floor_of(top);
-    scale = scale_of(top);
-    start = -scale * static_cast<double>(top);
+    by.set(top, temp);
     // the ranks' sums, by the row's largest logit: a lane each
-    its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] * point(sh_tops[slot ^ 1][lane]) : 0.0;
+    its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] * by.point(sh_table, sh_tops[slot ^ 1][lane]) : 0.0;
     total = warp_sum(its_sum);
-    rescale = point(mine);
+    rescale = by.point(sh_table, mine);
+    entered = total;
   };
 
   enter();
@@ -441,12 +448,14 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     const int64_t x = p.tokens[b * p.T + i];
     const bool known = x >= 0 && x < p.V;
     bool take = false;
+    double w = 0.0;
     if (greedy) {
       take = known && x == best;
     } else if (known && total > 0.0) {
       const double u = p.uniforms[b * p.T + i];
       const float qx = q ? q[x] : 1.f;
-      take = u * static_cast<double>(qx) * total < left(point(static_cast<float>(z[x])), static_cast<int>(x), qx);
+      w = left(by.point(sh_table, static_cast<float>(z[x])), static_cast<int>(x), qx);
+      take = u * static_cast<double>(qx) * total < w;
     }
     if (take) {
       cur = i;
@@ -461,14 +470,28 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
       }
       __syncthreads();
       ++refused;
-      sum_up();
+      // Without q a refusal takes one weight away.  As long as a thousandth of the row's weight is left, the
+      // difference has its digits; behind that, and with q, the sum is taken anew.
+      if (q || !(total - w >= entered * 0x1p-10)) {
+        sum_up();
+      } else if (w > 0.0) {
+        total -= w;
+        pared = true;
+        const int warps = static_cast<int>(ranks) * kWarps, per = (row.granules + warps - 1) / warps;
+        const int owner = static_cast<int>((x + row.lead) / kVec) / per;
+        if (lane == owner / kWarps) its_sum -= w;
+        if (static_cast<int>(rank) == owner / kWarps && tid == 0) sh_run[owner % kWarps] -= w / rescale;
+      }
     }
   }
   if (tid == 0 && rank == 0) p.accepted[b] = taken;
   if (!usable || greedy || !(total > 0.0)) {
-    if (usable && !greedy) best = first_of(top);  // refusals have left no weight
+    if (usable && !greedy) find_best();  // refusals have left no weight
     if (tid == 0 && rank == 0) p.next_token[b] = usable ? best : -1;
   } else {
+    // (a difference may have left a part that has no weight some of its last digits: no token to name as last)
+    if (pared && !(static_cast<double>(p.uniforms[b * p.T]) * total < total * (1.0 - 1e-9))) sum_up();
+    __syncthreads();  // sh_run is complete
     // the first token whose cumulated weight exceeds u_0 of the total
     const double goal = static_cast<double>(p.uniforms[b * p.T]) * total;
     double before = 0.0;
@@ -492,9 +515,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
       }
       if (w_at < 0) w_at = w_last;
       // that run again, 32 granules a warp, then the warp in whose granules it lies
-      const int granules = (lead + p.V + kVec - 1) / kVec, warps = static_cast<int>(ranks) * kWarps;
-      const int per = (granules + warps - 1) / warps, first = min(granules, (static_cast<int>(rank) * kWarps + w_at) * per);
-      const int end = min(granules, first + per);
+      const int warps = static_cast<int>(ranks) * kWarps, per = (row.granules + warps - 1) / warps;
+      const int first = min(row.granules, (static_cast<int>(rank) * kWarps + w_at) * per), end = min(row.granules, first + per);
       int found = -1, heavy = -1;
       for (int i0 = first; i0 < end && found < 0; i0 += 32 * kWarps) {
         const int i = i0 + 32 * warp + lane;
@@ -502,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
 #pragma unroll
         for (int y = 0; y < kVec; ++y) w[y] = 0.0;
         if (i < end) {
-          weights(i, __ldg(frame + i), scale, start, floor_x, w);
+          row.weights(sh_table, by, i, __ldg(row.frame + i), w);
           refuse(i, w);
         }
 #pragma unroll
@@ -525,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
         for (int y = 0; y < kVec; ++y) {
           sum += w[y];
           if (w[y] > 0.0) {
-            have = i * kVec - lead + y;
+            have = row.first(i) + y;
             if (hit < 0 && !past && sum > goal) hit = have;
           }
         }
@@ -549,14 +571,11 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
   cluster_barrier();  // no CTA leaves while its words are written
 }
 
-template <typename T>
-int verify_t(const TreeVerifyParams& p, int64_t batch, cudaStream_t st, int num_sms) {
-  // CTAs of a sequence: as many as find room at once, two on an SM, and have a granule for every
-  // lane; sixteen where they fill a third of the card at most (their clusters need whole GPCs).
-  int ctas = 1;
-  while (ctas < 8 && batch * ctas * 2 <= 2ll * num_sms && p.V > kThreads * ctas * 2) ctas *= 2;
-  auto* kernel = tree_verify_kernel<T>;
-  if (ctas == 8 && batch * 48 <= num_sms && p.V > kThreads * 16) {
+template <typename T, int kThreads>
+int verify_t(const TreeVerifyParams& p, int64_t batch, int ctas, cudaStream_t st, int num_sms) {
+  auto* kernel = tree_verify_kernel<T, kThreads>;
+  // sixteen CTAs where they fill a third of the card at most (their clusters need whole GPCs)
+  if (ctas == 8 && batch * 48 <= num_sms && p.V > 8192) {
     static std::mutex mu;
     static bool done[64] = {false};
     int dev = 0;
@@ -590,6 +609,16 @@ int verify_t(const TreeVerifyParams& p, int64_t batch, cudaStream_t st, int num_
   return launch_result();
 }
 
+template <typename T>
+int verify_sized(const TreeVerifyParams& p, int64_t batch, cudaStream_t st, int num_sms) {
+  // CTAs of a sequence: as many as find room at once, two on an SM, and have work for their lanes.
+  // Where eight do, of 256 threads, which have registers for a granule's weights side by side; else of
+  // 512, whose number counts: one chain 22 us instead of 25, 64 chains 106 instead of 99.
+  int ctas = 1;
+  while (ctas < 8 && batch * ctas * 2 <= 2ll * num_sms && p.V > 1024 * ctas) ctas *= 2;
+  return ctas == 8 ? verify_t<T, 256>(p, batch, ctas, st, num_sms) : verify_t<T, 512>(p, batch, ctas, st, num_sms);
+}
+
 }  // namespace
 
 int launch_tree_verify(const void* logits, int dtype, int64_t stride_b, int64_t stride_t, int64_t batch, int tokens,
@@ -600,9 +629,9 @@ int launch_tree_verify(const void* logits, int dtype, int64_t stride_b, int64_t 
   const TreeVerifyParams p{logits, stride_b, stride_t, ids, parents, parents_stride, uniforms, tokens > 1 ? probs : nullptr,
                            probs_stride_b, probs_stride_t, temperatures, temperature, tokens, static_cast<int>(vocab),
                            path, accepted, next_token, status};
-  if (dtype == FITQ_DTYPE_BF16) return verify_t<__nv_bfloat16>(p, batch, st, num_sms);
-  if (dtype == FITQ_DTYPE_F16) return verify_t<__half>(p, batch, st, num_sms);
-  return verify_t<float>(p, batch, st, num_sms);
+  if (dtype == FITQ_DTYPE_BF16) return verify_sized<__nv_bfloat16>(p, batch, st, num_sms);
+  if (dtype == FITQ_DTYPE_F16) return verify_sized<__half>(p, batch, st, num_sms);
+  return verify_sized<float>(p, batch, st, num_sms);
 }
 
 }  // namespace fitq
