@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
   bool usable = true;
   double total = 0.0;       // of the weights as refusals have left them
   double entered = 0.0;     // the total before any refusal
+  uint64_t kids = 0;        // children of token cur
   bool pared = false;       // refusals have been taken out of total, its_sum and sh_run one by one
   float top = 0.f;          // the row's largest logit
   int best = 0;
@@ -414,6 +415,8 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     const int warps = static_cast<int>(ranks) * kWarps, per = (row.granules + warps - 1) / warps;
     lo = min(row.granules, (static_cast<int>(rank) * kWarps + warp) * per);
     hi = min(row.granules, lo + per);
+    kids = __ballot_sync(0xffffffffu, lane < p.T && lane > cur && up[lane] == cur) |
+           static_cast<uint64_t>(__ballot_sync(0xffffffffu, lane + 32 < p.T && lane + 32 > cur && up[lane + 32] == cur)) << 32;
     // ---- the CTA's largest logit, its weights' sum by it, and the cluster's
     float mine = row.largest(lo, hi);
     if (lane == 0) sh_top[warp] = mine;
@@ -421,16 +424,30 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     mine = sh_top[0];
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) mine = max_nan(mine, sh_top[w]);
-    Scale own{};
-    if (!greedy) own.set(mine, temp);
-    sum_runs(greedy ? INFINITY : mine, own);
+    if (greedy) {  // and the first index with it, in the sum's place
+      const int at = row.first_of(lo, hi, mine);
+      if (lane == 0) sh_run[warp] = static_cast<double>(at);
+      __syncthreads();
+      double low = sh_run[0];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) low = fmin(low, sh_run[w]);
+      __syncthreads();
+      if (lane == 0) sh_run[warp] = warp == 0 ? low : 0.0;
+    } else {
+      Scale own{};
+      own.set(mine, temp);
+      sum_runs(mine, own);
+    }
     exchange(true, mine);
     top = -INFINITY;
     for (uint32_t r = 0; r < ranks; ++r) top = max_nan(top, sh_tops[slot ^ 1][r]);
     usable = top == top && top != -INFINITY && (greedy || top != INFINITY);
     if (!usable) return;
     if (greedy) {
-      find_best();
+      double low = 0x7fffffff;
+      for (uint32_t r = 0; r < ranks; ++r)
+        if (sh_tops[slot ^ 1][r] == top) low = fmin(low, sh_sums[slot ^ 1][r]);
+      best = static_cast<int>(low);
       return;
     }
     by.set(top, temp);
@@ -443,8 +460,9 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
 
   enter();
   if (tid == 0 && rank == 0) p.path[b * p.T] = 0;
-  for (int i = 1; i < p.T && usable; ++i) {
-    if (up[i] != cur) continue;
+  while (usable && kids) {
+    const int i = __ffsll(static_cast<long long>(kids)) - 1;
+    kids &= kids - 1;
     const int64_t x = p.tokens[b * p.T + i];
     const bool known = x >= 0 && x < p.V;
     bool take = false;
@@ -613,10 +631,11 @@ template <typename T>
 int verify_sized(const TreeVerifyParams& p, int64_t batch, cudaStream_t st, int num_sms) {
   // CTAs of a sequence: as many as find room at once, two on an SM, and have work for their lanes.
   // Where eight do, of 256 threads, which have registers for a granule's weights side by side; else of
-  // 512, whose number counts: one chain 22 us instead of 25, 64 chains 106 instead of 99.
+  // 384, of which more run at once: one chain 22 us instead of 25, 64 chains 106 instead of 96 (with
+  // 512 of 64 registers 103).
   int ctas = 1;
   while (ctas < 8 && batch * ctas * 2 <= 2ll * num_sms && p.V > 1024 * ctas) ctas *= 2;
-  return ctas == 8 ? verify_t<T, 256>(p, batch, ctas, st, num_sms) : verify_t<T, 512>(p, batch, ctas, st, num_sms);
+  return ctas == 8 ? verify_t<T, 256>(p, batch, ctas, st, num_sms) : verify_t<T, 384>(p, batch, ctas, st, num_sms);
 }
 
 }  // namespace
