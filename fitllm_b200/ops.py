@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -379,77 +380,82 @@ def kv4_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
     return out
 
 
-def _serving_only(what: str, *tensors) -> None:
-    """Refuses tensors whose gradient the call would lose."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError(f"{what}: an input requires a gradient, which this call does not have "
-                                  "(use torch.no_grad())")
+def _serving_only(what: str) -> None:
+    """Refuses a call that would lose its inputs' gradient."""
+    raise NotImplementedError(f"{what}: an input requires a gradient, which this call does not have "
+                              "(use torch.no_grad())")
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_attention_workspace(cap: int, batch: int, t: int, kv_heads: int, d: int, heads: int, device: int) -> int:
+    """fitq_tree_attention_workspace of the sizes, on a device's SMs."""
+    c = _lib.TreeC(1 << 16, 1 << 16, 0, cap, 0, 0, d, batch, t, kv_heads, d, _lib.DTYPE_BF16)
+    return _lib.load().fitq_tree_attention_workspace(c, heads)
 
 
 def _tree_parents(what: str, parents: torch.Tensor, batch: int, t: int, dev) -> int:
     """Entries from sequence to sequence of parents int32 [batch, t], or 0 of [t]."""
-    shape = tuple(parents.shape)
-    if parents.dtype != torch.int32 or shape not in ((batch, t), (t,)) or (t > 1 and parents.stride(-1) != 1):
+    shape, strides = parents.shape, parents.stride()
+    if parents.dtype != torch.int32 or (shape != (batch, t) and shape != (t,)) or (t > 1 and strides[-1] != 1):
         raise ValueError(f"{what}: parents must be int32 [{batch}, {t}] or [{t}] with dense rows (got {parents.dtype} "
-                         f"{shape})")
+                         f"{tuple(shape)})")
     if parents.device != dev:
         raise ValueError(f"{what}: parents is on {parents.device}, not on {dev}")
-    if len(shape) == 1 or batch == 1:
+    if len(strides) == 1 or batch == 1:
         return 0
-    if 0 < parents.stride(0) < t:
+    if 0 < strides[0] < t:
         raise ValueError(f"{what}: rows of parents overlap")
-    return parents.stride(0)
+    return strides[0]
 
 
 def _tree_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix: torch.Tensor, parents: torch.Tensor,
                 t: int) -> _lib.TreeC:
     """The fitq_tree descriptor of a call (its pointers live as long as the tensors)."""
-    dev, shape = k_cache.device, k_cache.shape
-    if k_cache.dtype not in _KV4_DTYPES or len(shape) != 4 or not k_cache.is_cuda:
+    dev, shape, strides, dtype = k_cache.device, k_cache.shape, k_cache.stride(), _KV4_DTYPES.get(k_cache.dtype)
+    if dtype is None or len(shape) != 4 or dev.type != "cuda":
         raise ValueError(f"{what}: caches must be bf16 or fp16 CUDA tensors [batch, kv_heads, capacity, head_dim]")
     if v_cache.shape != shape or v_cache.dtype != k_cache.dtype or v_cache.device != dev:
         raise ValueError(f"{what}: k_cache and v_cache differ in shape, dtype or device")
     batch, kv_heads, cap, d = shape
-    strides = k_cache.stride()
     if v_cache.stride() != strides:
         raise ValueError(f"{what}: k_cache and v_cache differ in strides")
-    sb, sh, sp = (s if n > 1 else 0 for s, n in zip(strides[:3], shape))
-    sp = sp if cap > 1 else d
-    if strides[3] != 1 or sp < d or (sb | sh | sp) % 8 or (sb == 0 and batch > 1) or (sh == 0 and kv_heads > 1) \
-            or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+    sb, sh, sp, one = strides
+    if batch <= 1:
+        sb = 0
+    if kv_heads <= 1:
+        sh = 0
+    if cap <= 1:
+        sp = d
+    if one != 1 or sp < d or (sb | sh | sp) % 8 or (sb == 0 and batch > 1) or (sh == 0 and kv_heads > 1) \
+            or (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
         raise ValueError(f"{what}: caches need dense heads, strides in multiples of 8 elements and 16-byte alignment "
                          f"(got strides {strides})")
     if prefix.dtype != torch.int32 or prefix.shape != (batch,) or not prefix.is_contiguous() or prefix.device != dev:
         raise ValueError(f"{what}: prefix must be contiguous int32 [{batch}] on {dev}")
     ps = _tree_parents(what, parents, batch, t, dev)
-    return _lib.TreeC(parents.data_ptr(), prefix.data_ptr(), ps, cap, sb, sh, sp, batch, t, kv_heads, d,
-                      _KV4_DTYPES[k_cache.dtype])
+    return _lib.TreeC(parents.data_ptr(), prefix.data_ptr(), ps, cap, sb, sh, sp, batch, t, kv_heads, d, dtype)
 
 
-def _tree_tokens(what: str, name: str, x: torch.Tensor, heads: Optional[int], cache: torch.Tensor,
-                 t: int) -> torch.Tensor:
-    """x [batch, t, heads, head_dim] whose tokens follow one another at one stride, heads dense."""
-    shape, d = x.shape, cache.shape[3]
-    if len(shape) != 4 or shape[0] != cache.shape[0] or shape[1] != t or shape[3] != d or shape[2] == 0 \
+def _tree_tokens(what: str, name: str, x: torch.Tensor, heads: Optional[int], c: _lib.TreeC,
+                 cache: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """x [batch, t, heads, head_dim] whose tokens follow one another at one stride, heads dense, and
+    that stride."""
+    shape, d, t = x.shape, c.head_dim, c.tokens
+    if len(shape) != 4 or shape[0] != c.batch or shape[1] != t or shape[3] != d or shape[2] == 0 \
             or (heads is not None and shape[2] != heads):
         raise ValueError(f"{what}: {name} has shape {tuple(shape)}")
     if x.dtype != cache.dtype or x.device != cache.device:
         raise ValueError(f"{what}: {name} must be {cache.dtype} on {cache.device} like the caches (got {x.dtype} on "
                          f"{x.device})")
-    s0, s1, s2, s3 = x.stride()
+    row = shape[2] * d
     if x.is_contiguous() and x.data_ptr() % 16 == 0:
-        return x
+        return x, row
+    s0, s1, s2, s3 = x.stride()
     if t == 1:
-        s1 = s0
-    if s3 != 1 or s2 != d or s1 % 8 or s1 < shape[2] * d or (shape[0] > 1 and s0 != t * s1) or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
-
-
-def _token_stride(x: torch.Tensor) -> int:
-    """Elements from token to token of what _tree_tokens gives."""
-    b, t, h, d = x.shape
-    return x.stride(1) if t > 1 else x.stride(0) if b > 1 else h * d
+        s1 = s0 if shape[0] > 1 else row
+    if s3 != 1 or s2 != d or s1 % 8 or s1 < row or (shape[0] > 1 and s0 != t * s1) or x.data_ptr() % 16:
+        return x.clone(memory_format=torch.contiguous_format), row
+    return x, s1
 
 
 def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -464,24 +470,24 @@ def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     position prefix + depth with row prefix + depth of cos_half, sin_half fp32 [positions,
     D / 2].  Returns the rotated q [B, T, heads, D] (into q_out when given; absent tokens: zeros)."""
     L = _lib.load()
-    _serving_only("tree_append", q, k, v, k_cache, v_cache)
-    t = q.shape[1] if q.dim() == 4 else 0
-    c = _tree_cache("tree_append", k_cache, v_cache, prefix, parents, t)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_cache.requires_grad
+                                    or v_cache.requires_grad):
+        _serving_only("tree_append")
+    c = _tree_cache("tree_append", k_cache, v_cache, prefix, parents, q.shape[1] if q.dim() == 4 else 0)
     dev = k_cache.device
-    q = _tree_tokens("tree_append", "q", q, None, k_cache, t)
-    k = _tree_tokens("tree_append", "k", k, c.kv_heads, k_cache, t)
-    v = _tree_tokens("tree_append", "v", v, c.kv_heads, k_cache, t)
+    q, qs = _tree_tokens("tree_append", "q", q, None, c, k_cache)
+    k, ks = _tree_tokens("tree_append", "k", k, c.kv_heads, c, k_cache)
+    v, vs = _tree_tokens("tree_append", "v", v, c.kv_heads, c, k_cache)
     rows = cos_half.shape
     if len(rows) != 2 or rows[1] * 2 != c.head_dim or sin_half.shape != rows:
         raise ValueError(f"tree_append: cos_half and sin_half must be of one shape [positions, {c.head_dim // 2}]")
     for name, x in (("cos_half", cos_half), ("sin_half", sin_half)):
         if x.dtype != torch.float32 or not x.is_contiguous() or x.device != dev or x.data_ptr() % 16:
             raise ValueError(f"tree_append: {name} must be contiguous, 16-byte aligned fp32 on {dev}")
-    out = _kv4_out("tree_append", "q_out", q_out, q)
+    out = q.new_empty(q.shape) if q_out is None else _kv4_out("tree_append", "q_out", q_out, q)
     with _on(dev):
-        _lib.check(L.fitq_tree_append(c, q.data_ptr(), _token_stride(q), k.data_ptr(), _token_stride(k), v.data_ptr(),
-                                      _token_stride(v), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                      cos_half.data_ptr(), sin_half.data_ptr(), rows[0], q.shape[2],
+        _lib.check(L.fitq_tree_append(c, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
+                                      k_cache.data_ptr(), v_cache.data_ptr(), cos_half.data_ptr(), sin_half.data_ptr(), rows[0], q.shape[2],
                                       _raw_stream(dev.index)), "fitq_tree_append")
     return out
 
@@ -495,18 +501,18 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     positions, its ancestors and itself.  Returns [B, T, heads, D] (into out when given;
     absent tokens: zeros)."""
     L = _lib.load()
-    _serving_only("tree_attention", q, k_cache, v_cache)
-    t = q.shape[1] if q.dim() == 4 else 0
-    c = _tree_cache("tree_attention", k_cache, v_cache, prefix, parents, t)
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        _serving_only("tree_attention")
+    c = _tree_cache("tree_attention", k_cache, v_cache, prefix, parents, q.shape[1] if q.dim() == 4 else 0)
     dev = k_cache.device
-    q = _tree_tokens("tree_attention", "q", q, None, k_cache, t)
-    out = _kv4_out("tree_attention", "out", out, q)
+    q, qs = _tree_tokens("tree_attention", "q", q, None, c, k_cache)
+    out = q.new_empty(q.shape) if out is None else _kv4_out("tree_attention", "out", out, q)
+    heads = q.shape[2]
     with _on(dev):
-        nbytes = L.fitq_tree_attention_workspace(c, q.shape[2])
-        ws = _workspace(nbytes, dev)
-        _lib.check(L.fitq_tree_attention(c, q.data_ptr(), _token_stride(q), k_cache.data_ptr(), v_cache.data_ptr(),
-                                         out.data_ptr(), q.shape[2], ws.data_ptr(), nbytes, _raw_stream(dev.index)),
-                   "fitq_tree_attention")
+        nbytes = _tree_attention_workspace(c.capacity, c.batch, c.tokens, c.kv_heads, c.head_dim, heads, dev.index)
+        ws = prefix.new_empty(nbytes // 4 + 1)
+        _lib.check(L.fitq_tree_attention(c, q.data_ptr(), qs, k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+                                         heads, ws.data_ptr(), nbytes, _raw_stream(dev.index)), "fitq_tree_attention")
     return out
 
 
@@ -528,8 +534,9 @@ def tree_keep(k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor]
             or accepted.device != first.device:
         raise ValueError(f"tree_keep: accepted must be contiguous int64 [{batch}] on the caches' device")
     c = _tree_cache("tree_keep", first, v_caches[0], prefix, path, t)
+    shape, strides, dtype, dev = first.shape, first.stride(), first.dtype, first.device
     for x in (*k_caches, *v_caches):
-        if x.shape != first.shape or x.stride() != first.stride() or x.dtype != first.dtype or x.device != first.device:
+        if x.shape != shape or x.stride() != strides or x.dtype != dtype or x.device != dev:
             raise ValueError("tree_keep: the layers' caches must be of one shape, stride, dtype and device")
     if lengths is None:
         lengths = torch.empty_like(prefix)
@@ -565,7 +572,9 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     each.  Returns [tokens, N] (into out when given, which may be y; rows of no sequence
     are left as they are there)."""
     L = _lib.load()
-    _serving_only("multi_lora", x, lora_a, lora_b, scale, y)
+    if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or lora_a.requires_grad or lora_b.requires_grad
+                                    or scale.requires_grad):
+        _serving_only("multi_lora")
     if x.dim() != 2 or y.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
         raise ValueError("multi_lora: x and y are [tokens, .], lora_a and lora_b [adapters, ., .]")
     tokens, k = x.shape
@@ -592,13 +601,13 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
             raise ValueError(f"multi_lora: q_start must be contiguous int32 [{batch + 1}] on {dev}")
         start = q_start.data_ptr()
     if out is None:
-        out = torch.empty(tokens, n, dtype=x.dtype, device=dev)
+        out = x.new_empty((tokens, n))
     elif out.shape != (tokens, n) or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"multi_lora: out must be a contiguous {x.dtype} tensor {(tokens, n)} on {dev}")
     x, y = _lora_rows(x, k), _lora_rows(y, n)
     with _on(dev):
-        nbytes = L.fitq_multi_lora_workspace(tokens, k, n, r, batch)
-        ws = _workspace(nbytes, dev)
+        ws = scale.new_empty(tokens * r)  # fitq_multi_lora_workspace: x.A^T
+        nbytes = tokens * r * 4
         _lib.check(L.fitq_multi_lora(x.data_ptr(), x.stride(0) if tokens > 1 else k, tokens, k, n, lora_a.data_ptr(),
                                      lora_b.data_ptr(), r, n_ad, scale.data_ptr(), adapter.data_ptr(), start, batch,
                                      y.data_ptr(), y.stride(0) if tokens > 1 else n, out.data_ptr(),

@@ -327,7 +327,6 @@ class TreeVerdict(NamedTuple):
     next_token: torch.Tensor
 
 
-@torch.no_grad()
 def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, uniforms: torch.Tensor,
                 draft_probs: Optional[torch.Tensor] = None, temperature=1.0) -> TreeVerdict:
     """Drafted tokens against the model's probabilities, from given random numbers
@@ -359,7 +358,7 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
         if len(shape) != 3 or shape[0] != b or shape[1] < t - 1 or shape[2] != vocab or draft_probs.device != dev \
                 or not draft_probs.dtype.is_floating_point:
             raise ValueError(f"verify_tree: draft_probs must be [{b}, {t - 1}, {vocab}] on {dev}")
-        q = draft_probs.float()
+        q = draft_probs.detach().float()
         if (vocab > 1 and q.stride(2) != 1) or (shape[1] > 1 and q.stride(1) < vocab):
             q = q.contiguous()
         qb, qt = (q.stride(0) if b > 1 else 0), (q.stride(1) if shape[1] > 1 else vocab)
@@ -370,8 +369,7 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
         temps = temperature.contiguous()
     else:
         temp = float(temperature)
-    r = TreeVerdict(torch.empty(b, t, dtype=torch.int32, device=dev), torch.empty(b, dtype=torch.int64, device=dev),
-                    torch.empty(b, dtype=torch.int64, device=dev))
+    r = TreeVerdict(parents.new_empty((b, t)), tokens.new_empty(b), tokens.new_empty(b))
     with ops._on(dev):
         _lib.check(L.fitq_tree_verify(logits.data_ptr(), _LOGIT_DTYPES[logits.dtype], logits.stride(0) if b > 1 else 0,
                                       logits.stride(1) if t > 1 else vocab, b, t, vocab, tokens.data_ptr(),
