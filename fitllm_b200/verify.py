@@ -404,6 +404,12 @@ class TreeKVCache(KVCache):
     def batch(self) -> int:
         return self.prefix.shape[0]
 
+    def set_lengths(self, lengths: Sequence[int]) -> None:
+        """The sequences' cached positions, e.g. behind a prompt that ``verify_pass`` wrote."""
+        if len(lengths) != self.batch or any(not 0 <= n <= self.capacity for n in lengths):
+            raise ValueError(f"set_lengths: {list(lengths)} for {self.batch} sequences of {self.capacity} positions")
+        self.prefix.copy_(torch.tensor(lengths, dtype=torch.int32))
+
     def keep(self, verdict: TreeVerdict) -> None:
         """The verdict's path stays behind each sequence's length, in all layers."""
         ops.tree_keep(self.k, self.v, self.prefix, verdict.path, verdict.accepted, lengths=self.prefix)

@@ -160,6 +160,13 @@ def test_the_cache_of_trees_refuses_other_layers():
     with pytest.raises(ValueError, match="sequences"):
         tree_pass([layer], h[:1], cache, chain_parents(3, "cpu"))
     assert chain_parents(3, "cpu").tolist() == [-1, 0, 1]
+    cache.set_lengths([3, 16])
+    assert cache.prefix.tolist() == [3, 16]
+    for bad in ([3], [17, 0], [-1, 0]):
+        with pytest.raises(ValueError, match="set_lengths"):
+            cache.set_lengths(bad)
+    cache.release(1)
+    assert cache.prefix.tolist() == [3, 0]
 
 
 def test_adapters_are_loaded_by_name_and_padded():
