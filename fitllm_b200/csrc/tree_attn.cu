@@ -73,7 +73,7 @@ struct TreeAttnParams {
   void* out;
   int4* desc;      // [CTAs] pair that begins in a CTA's run and ends in a later one: sequence, head x rows, parts
   float2* ml_part; // [CTAs][2: the run's first pair, a later one][rows of a pair]
-  float* o_part;   // [..][D]
+  float* o_part;   // [..][rows of a pair][D], of two row tiles [..][D][rows of a pair]
   float* o_sum;    // [CTAs][2 units][128][D], kLong only
   int64_t q_stride;
   int heads, group, row_pairs, pair_rows;  // pair_rows: 128 or 256
@@ -333,12 +333,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) queries[i] = w.has ? source[i] : make_uint4(0, 0, 0, 0);
       }
+      return w;
+    };
+    auto look = [&](const Cursor& c, Row& w) {  // the row's token in the tree
       if (c.b != tree_b) {
         tree = load_tree(tr, c.b, c.pre, lane, warp == 0 && c.kr == 0 && c.t0 == 0, p.status);
         tree_b = c.b;
       }
-      w.here = tree_token(tree, tok, w.seen) && w.has;
-      return w;
+      const int row = c.kr % p.row_pairs * p.pair_rows + (w.has ? (rows_of(c.kr) <= kRows ? lr : r * kRows + lr) : 0);
+      w.here = tree_token(tree, row / p.group, w.seen) && w.has;
     };
     auto put = [&](const Cursor& c, bool has) {  // the queries to shared memory
       const bool par = rows_of(c.kr) <= kRows;
@@ -365,7 +368,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     Row w{};
     if (ok) {
       w = fetch(c);
-      put(c, w.has);
+      // two row tiles load their queries in put: the scores need them first
+      if (kTwo) put(c, w.has);
+      look(c, w);
+      if (!kTwo) put(c, w.has);
     }
     const float cn = p.scale_log2;
     const uint64_t cn2 = pack2(cn, cn);
@@ -483,7 +489,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Row row = w;
       if (!ok) break;
       next_piece(p, c);
-      if (c.left > 0) w = fetch(c);
+      if (c.left > 0) {
+        w = fetch(c);
+        look(c, w);
+      }
       // the last step's products (and those before them), and the cleaned values' notes
       if (ok && steps > 0) ok = wait_all(&b_odone[r][(u + steps - 1) & 1], ((u + steps - 1) >> 1) & 1);
       if (ok) ok = wait_all(&b_fixed, piece & 1);
@@ -520,9 +529,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float ll = (use_a ? ka * ma.y : 0.f) + (use_b ? kb * mb.y : 0.f);
         const bool whole = old.t0 == 0 && old.t1 == old.n;
         const float inv = ll == 0.f ? 0.f : whole ? 1.f / ll : 1.f;
-        const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + (old.t0 > 0 ? 0 : 1)) * p.pair_rows + (par ? lr : r * kRows + lr);
+        const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (old.t0 > 0 ? 0 : 1);
+        const int in_pair = par ? lr : r * kRows + lr;
         const int kvh = old.kr / p.row_pairs;
-        if (!whole && row.has && (!par || r == 0)) p.ml_part[part] = make_float2(mm, ll);
+        if (!whole && row.has && (!par || r == 0)) p.ml_part[slot * p.pair_rows + in_pair] = make_float2(mm, ll);
         const int c0 = par ? r * (D / 2) : 0, c1 = par ? c0 + D / 2 : D;
         const uint32_t o_a = t_o + (par ? 0 : r * 128), o_b = t_o + 128;
         const float4* sum_a = reinterpret_cast<const float4*>(p.o_sum + ((static_cast<int64_t>(blockIdx.x) * 2 + (par ? 0 : r)) * kRows + lr) * D);
@@ -587,9 +597,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 *reinterpret_cast<uint4*>(dst + cc + i) = pack8<T>(g);
               }
             } else {
-              float4* po = reinterpret_cast<float4*>(p.o_part + part * D + cc);
+              // Two row tiles: column by column, a warp's rows side by side (row by row a piece of 160 rows took
+              // 3.7 us).  One: row by row, whose pieces a warp joins with its lanes on them (25 rows of 17
+              // pieces took 18.2 us instead of 13.6 otherwise).
+              float* po = kTwo ? p.o_part + (slot * D + cc) * p.pair_rows + in_pair : p.o_part + (slot * p.pair_rows + in_pair) * D + cc;
+              if (kTwo) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) po[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+                for (int i = 0; i < 32; ++i) po[static_cast<int64_t>(i) * p.pair_rows] = f[i];
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  reinterpret_cast<float4*>(po)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+              }
             }
           }
           __syncwarp();
@@ -856,6 +875,71 @@ __global__ void __launch_bounds__(256) tree_attn_combine_kernel(const TreeAttnPa
     *reinterpret_cast<uint32_t*>(dst) = Half16<T>::pack(f[0] * inv, f[1] * inv);
 }
 
+// The same of two row tiles, whose pieces lie column by column: CTA (c, y) takes 32 rows, a lane per row
+// and D / 8 columns per warp.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) tree_attn_combine_cols_kernel(const TreeAttnParams p) {
+  constexpr int kCols = D / 8, kPitch = 2 * D + 16, kPieces = 4;
+  __shared__ __align__(16) uint8_t tile[32 * kPitch];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  pdl_wait();  // the pieces
+  const int cta = blockIdx.x;
+  const int4 cut = p.desc[cta];
+  if (cut.x < 0) return;
+  const int parts = cut.z, in = static_cast<int>(blockIdx.y) * 32 + lane, row0 = cut.y % p.row_pairs * p.pair_rows;
+  const bool has = in < p.pair_rows && row0 + in < p.tree.tokens * p.group;
+  // piece i: the run's later slot, then the first slots of the runs behind it
+  auto slot = [&](int i) { return static_cast<int64_t>(cta + i) * 2 + (i == 0 ? 1 : 0); };
+  const int at = has ? in : 0;
+  float mx = kFloor;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) {
+    const float2 ml = p.ml_part[slot(i) * p.pair_rows + at];
+    if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
+  }
+  float l = 0.f, f[kCols];
+#pragma unroll
+  for (int x = 0; x < kCols; ++x) f[x] = 0.f;
+  for (int i0 = 0; i0 < parts; i0 += kPieces) {  // several pieces' loads at once
+    float2 ml[kPieces];
+    float v[kPieces][kCols];
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const int64_t from = slot(i0 + k < parts ? i0 + k : 0);
+      ml[k] = p.ml_part[from * p.pair_rows + at];
+      if (i0 + k >= parts) ml[k].y = 0.f;
+#pragma unroll
+      for (int x = 0; x < kCols; ++x) v[k][x] = p.o_part[(from * D + warp * kCols + x) * p.pair_rows + at];
+    }
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+      if (ml[k].y != 0.f) {  // a piece that saw nothing weighs 0, whatever its rows hold
+        const float w = exp2_approx(ml[k].x - mx);
+        l = fmaf(w, ml[k].y, l);
+#pragma unroll
+        for (int x = 0; x < kCols; ++x) f[x] = fmaf(w, v[k][x], f[x]);
+      }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int x = 0; x < kCols; x += 8) {
+    float g[8];
+#pragma unroll
+    for (int y = 0; y < 8; ++y) g[y] = f[x + y] * inv;
+    *reinterpret_cast<uint4*>(tile + lane * kPitch + (warp * kCols + x) * 2) = pack8<T>(g);
+  }
+  __syncthreads();
+  const int kvh = cut.y / p.row_pairs;
+  for (int e = threadIdx.x; e < 32 * (D / 8); e += 256) {
+    const int mine = static_cast<int>(blockIdx.y) * 32 + e / (D / 8), row = row0 + mine;
+    if (mine >= p.pair_rows || row >= p.tree.tokens * p.group) continue;
+    const int64_t token = static_cast<int64_t>(cut.x) * p.tree.tokens + row / p.group;
+    T* dst = static_cast<T*>(p.out) + (token * p.heads + kvh * p.group + row % p.group) * D;
+    reinterpret_cast<uint4*>(dst)[e % (D / 8)] = *reinterpret_cast<const uint4*>(tile + e / (D / 8) * kPitch + e % (D / 8) * 16);
+  }
+}
+
 struct Plan {
   int ctas, row_pairs, pair_rows;
   size_t ml_off, o_off, sum_off, bytes;
@@ -891,7 +975,8 @@ int attn_t(const TreeAttnParams& p, const Plan& a, const CUtensorMap& tk, const 
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   if (a.ctas > 1) {
     const int rows = p.tree.tokens * p.group < a.pair_rows ? p.tree.tokens * p.group : a.pair_rows;
-    e = launch_pdl(tree_attn_combine_kernel<T, D>, dim3(a.ctas, (rows + 7) / 8), dim3(256), 0, st, p);
+    e = kTwo ? launch_pdl(tree_attn_combine_cols_kernel<T, D>, dim3(a.ctas, (rows + 31) / 32), dim3(256), 0, st, p)
+             : launch_pdl(tree_attn_combine_kernel<T, D>, dim3(a.ctas, (rows + 7) / 8), dim3(256), 0, st, p);
     note_launch();
     if (e != cudaSuccess) return FITQ_ERR_CUDA;
   }
