@@ -481,9 +481,10 @@ def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     rows = cos_half.shape
     if len(rows) != 2 or rows[1] * 2 != c.head_dim or sin_half.shape != rows:
         raise ValueError(f"tree_append: cos_half and sin_half must be of one shape [positions, {c.head_dim // 2}]")
-    for name, x in (("cos_half", cos_half), ("sin_half", sin_half)):
-        if x.dtype != torch.float32 or not x.is_contiguous() or x.device != dev or x.data_ptr() % 16:
-            raise ValueError(f"tree_append: {name} must be contiguous, 16-byte aligned fp32 on {dev}")
+    if cos_half.dtype != torch.float32 or sin_half.dtype != torch.float32 or cos_half.device != dev \
+            or sin_half.device != dev or not cos_half.is_contiguous() or not sin_half.is_contiguous() \
+            or (cos_half.data_ptr() | sin_half.data_ptr()) % 16:
+        raise ValueError(f"tree_append: cos_half and sin_half must be contiguous, 16-byte aligned fp32 on {dev}")
     out = q.new_empty(q.shape) if q_out is None else _kv4_out("tree_append", "q_out", q_out, q)
     with _on(dev):
         _lib.check(L.fitq_tree_append(c, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
@@ -552,11 +553,14 @@ def tree_keep(k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor]
     return lengths
 
 
-def _lora_rows(x: torch.Tensor, cols: int) -> torch.Tensor:
-    """x [tokens, cols] with dense, aligned rows (the row stride is free)."""
-    if x.stride(1) != 1 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < cols)) or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+def _lora_rows(x: torch.Tensor, rows: int, cols: int) -> Tuple[torch.Tensor, int]:
+    """x [rows, cols] with dense, aligned rows (the row stride is free), and that stride."""
+    s0, s1 = x.stride()
+    if rows <= 1:
+        s0 = cols
+    if s1 != 1 or s0 % 8 or s0 < cols or x.data_ptr() % 16:
+        return x.clone(memory_format=torch.contiguous_format), cols
+    return x, s0
 
 
 def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scale: torch.Tensor, adapter: torch.Tensor,
@@ -575,26 +579,29 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or lora_a.requires_grad or lora_b.requires_grad
                                     or scale.requires_grad):
         _serving_only("multi_lora")
-    if x.dim() != 2 or y.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
+    xs, ys, sa, sb = x.shape, y.shape, lora_a.shape, lora_b.shape
+    if len(xs) != 2 or len(ys) != 2 or len(sa) != 3 or len(sb) != 3:
         raise ValueError("multi_lora: x and y are [tokens, .], lora_a and lora_b [adapters, ., .]")
-    tokens, k = x.shape
-    n, (n_ad, r) = y.shape[1], lora_a.shape[:2]
-    dev = x.device
-    if lora_a.shape != (n_ad, r, k) or lora_b.shape != (n_ad, n, r) or y.shape[0] != tokens:
-        raise ValueError(f"multi_lora: x {tuple(x.shape)}, y {tuple(y.shape)}, lora_a {tuple(lora_a.shape)} and lora_b "
-                         f"{tuple(lora_b.shape)} do not match")
-    if x.dtype not in _KV4_DTYPES or not x.is_cuda:
+    tokens, k = xs
+    n, dev, dtype = ys[1], x.device, x.dtype
+    n_ad, r, _ = sa
+    if sa[2] != k or sb[0] != n_ad or sb[1] != n or sb[2] != r or ys[0] != tokens:
+        raise ValueError(f"multi_lora: x {tuple(xs)}, y {tuple(ys)}, lora_a {tuple(sa)} and lora_b {tuple(sb)} do not match")
+    code = _KV4_DTYPES.get(dtype)
+    if code is None or dev.type != "cuda":
         raise ValueError("multi_lora: x must be a bf16 or fp16 CUDA tensor")
-    for name, t in (("y", y), ("lora_a", lora_a), ("lora_b", lora_b)):
-        if t.dtype != x.dtype or t.device != dev:
-            raise ValueError(f"multi_lora: {name} must be {x.dtype} on {dev} (got {t.dtype} on {t.device})")
+    if y.dtype != dtype or lora_a.dtype != dtype or lora_b.dtype != dtype or y.device != dev or lora_a.device != dev \
+            or lora_b.device != dev:
+        raise ValueError(f"multi_lora: y, lora_a and lora_b must be {dtype} on {dev} (got {y.dtype}, {lora_a.dtype}, "
+                         f"{lora_b.dtype} on {y.device}, {lora_a.device}, {lora_b.device})")
     if not (lora_a.is_contiguous() and lora_b.is_contiguous()):
         raise ValueError("multi_lora: lora_a and lora_b must be contiguous")
     if scale.dtype != torch.float32 or scale.shape != (n_ad,) or not scale.is_contiguous() or scale.device != dev:
         raise ValueError(f"multi_lora: scale must be contiguous fp32 [{n_ad}] on {dev}")
-    if adapter.dtype != torch.int32 or adapter.dim() != 1 or not adapter.is_contiguous() or adapter.device != dev:
+    ad = adapter.shape
+    if adapter.dtype != torch.int32 or len(ad) != 1 or not adapter.is_contiguous() or adapter.device != dev:
         raise ValueError(f"multi_lora: adapter must be contiguous int32 [batch] on {dev}")
-    batch, start = adapter.shape[0], None
+    batch, start = ad[0], None
     if q_start is not None:
         if q_start.dtype != torch.int32 or q_start.shape != (batch + 1,) or not q_start.is_contiguous() \
                 or q_start.device != dev:
@@ -602,16 +609,15 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
         start = q_start.data_ptr()
     if out is None:
         out = x.new_empty((tokens, n))
-    elif out.shape != (tokens, n) or out.dtype != x.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"multi_lora: out must be a contiguous {x.dtype} tensor {(tokens, n)} on {dev}")
-    x, y = _lora_rows(x, k), _lora_rows(y, n)
+    elif out.shape != (tokens, n) or out.dtype != dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"multi_lora: out must be a contiguous {dtype} tensor {(tokens, n)} on {dev}")
+    x, x_stride = _lora_rows(x, tokens, k)
+    y, y_stride = _lora_rows(y, tokens, n)
     with _on(dev):
         ws = scale.new_empty(tokens * r)  # fitq_multi_lora_workspace: x.A^T
-        nbytes = tokens * r * 4
-        _lib.check(L.fitq_multi_lora(x.data_ptr(), x.stride(0) if tokens > 1 else k, tokens, k, n, lora_a.data_ptr(),
-                                     lora_b.data_ptr(), r, n_ad, scale.data_ptr(), adapter.data_ptr(), start, batch,
-                                     y.data_ptr(), y.stride(0) if tokens > 1 else n, out.data_ptr(),
-                                     _KV4_DTYPES[x.dtype], ws.data_ptr(), nbytes, _raw_stream(dev.index)),
+        _lib.check(L.fitq_multi_lora(x.data_ptr(), x_stride, tokens, k, n, lora_a.data_ptr(), lora_b.data_ptr(), r, n_ad,
+                                     scale.data_ptr(), adapter.data_ptr(), start, batch, y.data_ptr(), y_stride,
+                                     out.data_ptr(), code, ws.data_ptr(), tokens * r * 4, _raw_stream(dev.index)),
                    "fitq_multi_lora")
     return out
 
