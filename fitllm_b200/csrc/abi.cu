@@ -1552,7 +1552,8 @@ static int tree_view(const char* what, const fitq_tree* t, int heads, fitq::Tree
                 t->kv_heads, (long long)t->capacity);
   if (t->parents_stride != 0 && t->parents_stride < t->tokens)
     return fail(FITQ_ERR_SHAPE, "%s: parents_stride=%lld", what, (long long)t->parents_stride);
-  if (t->stride_b < 0 || t->stride_h < 0 || t->stride_p < t->head_dim ||
+  if (t->stride_b < 0 || t->stride_h < 0 || t->stride_p < t->head_dim || (t->stride_b == 0 && t->batch > 1) ||
+      (t->stride_h == 0 && t->kv_heads > 1) ||
       ((t->stride_b | t->stride_h | t->stride_p) & 7) || t->stride_b >= (1ll << 38) || t->stride_h >= (1ll << 38) ||
       t->stride_p >= (1ll << 38))
     return fail(FITQ_ERR_SHAPE, "%s: cache strides must be multiples of 8 that cover a head (got %lld, %lld, %lld)", what,
@@ -1677,6 +1678,9 @@ int fitq_tree_keep(const fitq_tree* tree, void* const* k_caches, void* const* v_
   if ((reinterpret_cast<uintptr_t>(accepted) & 7u) ||
       ((reinterpret_cast<uintptr_t>(path) | reinterpret_cast<uintptr_t>(lengths)) & 3u))
     return fail(FITQ_ERR_ALIGN, "tree_keep: tensors must be aligned to their elements");
+  const uintptr_t from = reinterpret_cast<uintptr_t>(t.prefix), to = reinterpret_cast<uintptr_t>(lengths), size = 4u * t.batch;
+  if (from != to && from < to + size && to < from + size)
+    return fail(FITQ_ERR_ARG, "tree_keep: lengths overlaps prefix, other than being prefix");
   if (!current_sms(&rc)) return rc;
   return launch_status(fitq::launch_tree_keep(t, k_caches, v_caches, layers, tree->head_dim, path, accepted, lengths,
                                               status_ptr(), static_cast<cudaStream_t>(stream)),
@@ -1685,7 +1689,8 @@ int fitq_tree_keep(const fitq_tree* tree, void* const* k_caches, void* const* v_
 
 static bool multi_lora_fits(int64_t tokens, int64_t k, int64_t n, int rank, int batch) {
   return tokens >= 0 && tokens < (1ll << 28) && k >= 8 && k < (1ll << 24) && k % 8 == 0 && n >= 8 && n < (1ll << 24) &&
-         n % 8 == 0 && (rank == 16 || rank == 32 || rank == 48 || rank == 64) && batch >= 1;
+         n % 8 == 0 && (rank == 16 || rank == 32 || rank == 48 || rank == 64) && batch >= 1 && batch <= (1 << 20) &&
+         (tokens / 128 + batch) * (n / 256 + 8) < (1ll << 31);  // CTAs of a launch
 }
 
 size_t fitq_multi_lora_workspace(int64_t tokens, int64_t k, int64_t n, int rank, int batch) {

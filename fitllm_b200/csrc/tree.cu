@@ -109,45 +109,56 @@ struct TreeKeepParams {
   const int32_t* path;      // [batch, tokens]
   const int64_t* accepted;  // [batch]
   int32_t* lengths;         // [batch]
-  int first;                // 1: this launch writes the lengths
   int64_t vec_b, vec_h, vec_p;  // strides in 16-byte pieces
   int per_head;                 // 16-byte pieces of a head
   int* status;
 };
 
+// How many tokens of sequence b stay: the whole CTA asks, thread i holding path[i]; -1 for a path
+// that does not ascend within the tree and the capacity.
+__device__ __forceinline__ int kept_tokens(const TreeKeepParams& p, int b, int64_t pre, int* src) {
+  const TreeView& t = p.tree;
+  const int64_t acc = p.accepted[b];
+  const int count = static_cast<int>(acc < 0 ? 0 : acc + 1 > t.tokens ? t.tokens : acc + 1);
+  bool bad = acc >= t.tokens || acc < -1 || (count > 0 && pre < 0);
+  if (static_cast<int>(threadIdx.x) < count) {
+    const int32_t* path = p.path + static_cast<int64_t>(b) * t.tokens + threadIdx.x;
+    const int before = threadIdx.x ? path[-1] : -1;
+    src[threadIdx.x] = path[0];
+    bad = bad || path[0] <= before || path[0] >= t.tokens || pre + path[0] >= t.capacity;
+  }
+  return __syncthreads_or(bad) ? -1 : count;
+}
+
 // Grid (caches, batch): a CTA moves one sequence's path in one cache.
 __global__ void __launch_bounds__(kKeepThreads) tree_keep_kernel(const TreeKeepParams p) {
-  __shared__ int sh_src[kTreeTokens];
-  __shared__ int sh_count;
+  __shared__ int src[kTreeTokens];
   pdl_launch_dependents();
   pdl_wait();
   const TreeView& t = p.tree;
   const int b = blockIdx.y;
-  const int64_t pre = t.prefix[b], acc = p.accepted[b];
-  if (threadIdx.x == 0) sh_count = static_cast<int>(acc < 0 ? 0 : acc + 1 > t.tokens ? t.tokens : acc + 1);
-  __syncthreads();
-  const int count = sh_count;
-  bool bad = acc >= t.tokens || acc < -1 || (count > 0 && pre < 0);
-  if (threadIdx.x < count) {
-    const int src = p.path[static_cast<int64_t>(b) * t.tokens + threadIdx.x];
-    const int before = threadIdx.x ? p.path[static_cast<int64_t>(b) * t.tokens + threadIdx.x - 1] : -1;
-    sh_src[threadIdx.x] = src;
-    bad = bad || src <= before || src >= t.tokens || pre + src >= t.capacity;
-  }
-  if (__syncthreads_or(bad)) {  // a path that does not ascend within the tree: nothing stays
-    if (threadIdx.x == 0 && blockIdx.x == 0 && p.first) {
-      report_device_error(p.status, FITQ_ERR_ARG);
-      p.lengths[b] = static_cast<int32_t>(pre);
-    }
-    return;
-  }
-  if (threadIdx.x == 0 && blockIdx.x == 0 && p.first) p.lengths[b] = static_cast<int32_t>(pre) + count;
+  const int64_t pre = t.prefix[b];
+  const int count = kept_tokens(p, b, pre, src);
   uint4* base = p.caches[blockIdx.x] + b * p.vec_b + pre * p.vec_p;
   for (int e = threadIdx.x; e < t.kv_heads * p.per_head; e += kKeepThreads) {
     uint4* col = base + (e / p.per_head) * p.vec_h + e % p.per_head;
     for (int i = 0; i < count; ++i)
-      if (sh_src[i] != i) col[i * p.vec_p] = col[sh_src[i] * p.vec_p];
+      if (src[i] != i) col[i * p.vec_p] = col[src[i] * p.vec_p];
   }
+}
+
+// The new lengths, behind all moves: they may be written over the old ones, which every CTA of a
+// move reads.
+__global__ void __launch_bounds__(kTreeTokens) tree_lengths_kernel(const TreeKeepParams p) {
+  __shared__ int src[kTreeTokens];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.x;
+  const int64_t pre = p.tree.prefix[b];
+  const int count = kept_tokens(p, b, pre, src);
+  if (threadIdx.x != 0) return;
+  if (count < 0) report_device_error(p.status, FITQ_ERR_ARG);
+  p.lengths[b] = static_cast<int32_t>(pre) + (count < 0 ? 0 : count);
 }
 
 }  // namespace
@@ -185,11 +196,13 @@ int launch_tree_keep(const TreeView& tree, void* const* k_caches, void* const* v
       p.caches[2 * i] = static_cast<uint4*>(k_caches[at + i]);
       p.caches[2 * i + 1] = static_cast<uint4*>(v_caches[at + i]);
     }
-    p.first = at == 0;
     const cudaError_t e = launch_pdl(tree_keep_kernel, dim3(2 * n, tree.batch), dim3(kKeepThreads), 0, st, p);
     note_launch();
     if (e != cudaSuccess) return FITQ_ERR_CUDA;
   }
+  const cudaError_t e = launch_pdl(tree_lengths_kernel, dim3(tree.batch), dim3(kTreeTokens), 0, st, p);
+  note_launch();
+  if (e != cudaSuccess) return FITQ_ERR_CUDA;
   return launch_result();
 }
 

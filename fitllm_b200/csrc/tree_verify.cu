@@ -592,17 +592,34 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
 template <typename T, int kThreads>
 int verify_t(const TreeVerifyParams& p, int64_t batch, int ctas, cudaStream_t st, int num_sms) {
   auto* kernel = tree_verify_kernel<T, kThreads>;
-  // sixteen CTAs where they fill a third of the card at most (their clusters need whole GPCs)
+  // sixteen CTAs where they fill a third of the card at most, on cards whose GPCs have room for such a cluster
   if (ctas == 8 && batch * 48 <= num_sms && p.V > 8192) {
     static std::mutex mu;
-    static bool done[64] = {false};
+    static int room[64] = {0};  // by device: 0 not asked yet, else clusters + 1
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FITQ_ERR_CUDA;
+    if (!set_smem_limit(kernel, kAlone)) return FITQ_ERR_CUDA;
     std::lock_guard<std::mutex> lk(mu);
-    if (!done[dev] && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-      return FITQ_ERR_CUDA;
-    done[dev] = true;
-    ctas = 16;
+    if (room[dev] == 0) {
+      cudaLaunchConfig_t ask = {};
+      cudaLaunchAttribute shape[1];
+      shape[0].id = cudaLaunchAttributeClusterDimension;
+      shape[0].val.clusterDim.x = 16;
+      shape[0].val.clusterDim.y = shape[0].val.clusterDim.z = 1;
+      ask.gridDim = dim3(16);
+      ask.blockDim = dim3(kThreads);
+      ask.dynamicSmemBytes = kAlone;
+      ask.attrs = shape;
+      ask.numAttrs = 1;
+      int clusters = 0;
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+          cudaOccupancyMaxActiveClusters(&clusters, kernel, &ask) != cudaSuccess) {
+        cudaGetLastError();
+        clusters = 0;
+      }
+      room[dev] = clusters + 1;
+    }
+    if (room[dev] > 1) ctas = 16;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(batch * ctas));

@@ -389,7 +389,7 @@ def _serving_only(what: str) -> None:
 @functools.lru_cache(maxsize=256)
 def _tree_attention_workspace(cap: int, batch: int, t: int, kv_heads: int, d: int, heads: int, device: int) -> int:
     """fitq_tree_attention_workspace of the sizes, on a device's SMs."""
-    c = _lib.TreeC(1 << 16, 1 << 16, 0, cap, 0, 0, d, batch, t, kv_heads, d, _lib.DTYPE_BF16)
+    c = _lib.TreeC(1 << 16, 1 << 16, 0, cap, d, d, d, batch, t, kv_heads, d, _lib.DTYPE_BF16)
     return _lib.load().fitq_tree_attention_workspace(c, heads)
 
 

@@ -464,7 +464,8 @@ FITQ_API int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_st
 /* Attention of the tree's tokens over the cache, their own slots included (appended before).
  * q (q_stride as above), out [batch * tokens, heads, head_dim]; query head h reads KV head
  * h / (heads / kv_heads); scale 1/sqrt(head_dim), fp32 softmax and sums.  An absent token
- * gives zeros.  Slots that no token sees are not read into any sum, whatever they hold.
+ * gives zeros, as does one whose scores are all -inf.  Slots that no token sees are not read into any
+ * sum, whatever they hold.  The weights enter the second product rounded to dtype (their sum does not).
  * Deterministic.  out may be q as above.  The workspace of sizes that no call takes is 0. */
 FITQ_API size_t fitq_tree_attention_workspace(const fitq_tree* tree, int heads);
 FITQ_API int fitq_tree_attention(const fitq_tree* tree, const void* q, int64_t q_stride,

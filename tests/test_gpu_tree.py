@@ -272,6 +272,28 @@ def test_append_and_keep(cuda_dev, dtype, d, shape):
     assert prefix.tolist() == [0, 9, 33, 5] and ops.device_status() == 0
 
 
+def test_lengths_are_written_over_the_old_ones(cuda_dev):
+    """Every cache of every layer moves by the lengths that were, also where the new ones replace them."""
+    from fitllm_b200 import ops
+    b, t, layers, cap = 300, 6, 70, 24
+    g = torch.Generator(device=cuda_dev).manual_seed(9)
+    old = [torch.randn(b, 2, cap, 64, device=cuda_dev, generator=g).half() for _ in range(2 * layers)]
+    new = [x.clone() for x in old]
+    prefix = torch.randint(0, cap - t, (b,), device=cuda_dev, generator=g).int()
+    path = torch.tensor([0, 2, 4, 5, -1, -1], dtype=torch.int32, device=cuda_dev).expand(b, t).contiguous()
+    accepted = torch.full((b,), 3, device=cuda_dev)
+    before = prefix.clone()
+    for _ in range(3):  # three steps in a row, on the lengths that each leaves
+        at = prefix.clone().clamp(max=cap - t)
+        prefix.copy_(at)
+        ops.tree_keep(new[:layers], new[layers:], prefix, path, accepted, lengths=prefix)
+        assert torch.equal(prefix, at + 4)
+        rows = torch.arange(b, device=cuda_dev)[:, None]
+        for x in old:
+            x[rows, :, (at[:, None] + torch.arange(4, device=cuda_dev)).long()] = x[rows, :, (at[:, None] + path[:, :4]).long()]
+    assert not torch.equal(before, prefix) and all(torch.equal(x, y) for x, y in zip(old, new)) and ops.device_status() == 0
+
+
 def test_what_the_device_refuses(cuda_dev):
     """Bad parents, prefixes and paths are recorded, touch nothing and leave the others as they are."""
     from fitllm_b200 import ops

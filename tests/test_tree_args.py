@@ -44,7 +44,7 @@ BAD_TREES = [
     (dict(parents=None), ARG), (dict(prefix=None), ARG), (dict(head_dim=96), UNSUPPORTED), (dict(dtype=2), UNSUPPORTED),
     (dict(tokens=0), UNSUPPORTED), (dict(tokens=65), UNSUPPORTED), (dict(batch=0), SHAPE), (dict(kv_heads=3), SHAPE),
     (dict(capacity=0), SHAPE), (dict(capacity=(1 << 30) + 1), SHAPE), (dict(parents_stride=7), SHAPE),
-    (dict(stride_p=120), SHAPE), (dict(stride_h=12801), SHAPE), (dict(stride_b=-8), SHAPE), (dict(stride_b=1 << 40), SHAPE),
+    (dict(stride_p=120), SHAPE), (dict(stride_b=0), SHAPE), (dict(stride_h=0), SHAPE), (dict(stride_h=12801), SHAPE), (dict(stride_b=-8), SHAPE), (dict(stride_b=1 << 40), SHAPE),
     (dict(parents=P + 2), ALIGN), (dict(prefix=P + 1), ALIGN),
 ]
 
@@ -88,6 +88,7 @@ def test_keep_refusals(L):
     c = _tree()
     assert _keep(L, c, ptr=None) == ARG and _keep(L, c, path=None) == ARG and _keep(L, c, lengths=None) == ARG
     assert _keep(L, c, layers=0) == SHAPE
+    assert _keep(L, c, lengths=P + 4) == ARG  # over the prefix, other than being it
     assert _keep(L, c, ptr=P + 8) == ALIGN and _keep(L, c, acc=P + 4) == ALIGN and _keep(L, c, path=P + 2) == ALIGN
 
 
@@ -116,6 +117,7 @@ def test_multi_lora_refusals(L):
     assert call(x=None) == ARG and call(adapter=None) == ARG and call(ws=None) == ARG and call(out=None) == ARG
     assert call(rank=8) == UNSUPPORTED and call(rank=80) == UNSUPPORTED and call(dtype=2) == UNSUPPORTED
     assert call(k=252, xs=256) == SHAPE and call(n=100, ys=104) == SHAPE and call(tokens=-1) == SHAPE and call(adapters=0) == SHAPE
+    assert call(batch=(1 << 20) + 1, start=P) == SHAPE and call(n=(1 << 24) - 8, ys=1 << 24, tokens=1 << 27, start=P) == SHAPE
     assert call(xs=248) == SHAPE and call(ys=132) == SHAPE and call(tokens=7) == SHAPE and call(batch=0) == SHAPE
     assert call(a=P + 8) == ALIGN and call(scale=P + 2) == ALIGN and call(start=P + 1) == ALIGN
     assert call(out=FAR + 256) == ARG and call(out=FAR, ys=136) == ARG and call(out=P) == ARG  # over y, over x
