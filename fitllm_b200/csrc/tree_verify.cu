@@ -15,14 +15,16 @@
 // what is left here).  An exponential is 2^(n / 1024) from a table times a polynomial of degree
 // two (its Taylor series: 7e-12 of it at |x| <= ln 2 / 2048), summed by the last product:
 // seven fp64 operations and some ten others per element, which the issue of instructions
-// bounds (with twice as many it took 36 us instead of 23 for 64 rows of 152,064).
+// bounds.
 //
-// A cluster of up to eight CTAs walks with a sequence; every warp owns a run of the
+// A cluster of up to sixteen CTAs walks with a sequence; every warp owns a run of the
 // vocabulary, so that the cumulated sum is found by its parts: ranks, warps, lanes.  A CTA sums
 // by its own largest logit, and one exchange over the cluster joins largest logits and
-// sums.  A refused child costs another read of the row (from L1 and L2) with its q.
-// Bound: few sequences, the chain of a row (read, largest, read, exponentials, exchange); many,
-// fp64's rate.
+// sums.  A refused child costs another read of the row (from L1 and L2) with its q, and without a q a
+// subtraction.
+// Bound: the chain of a visited row (largest 1.1, sum 2.8, exchange 0.8, joining 0.8, a child's test 0.7 us
+// on eight CTAs; 5.4 in all on sixteen), and a batch's deepest path.  A chain of 5 rows of 152,064 tokens: 20 us;
+// 64 of them: 97; 16 trees of 32 tokens over 32,001: 18; one row of each of 64 sequences: 21.
 #include <mutex>
 #include <type_traits>
 
@@ -107,8 +109,7 @@ __device__ __forceinline__ float max_vec(const uint4& u) {
   }
 }
 
-// A float as a double by integer operations (the conversion instruction takes two elements per
-// cycle and SM: 36 us for 64 rows, see below).  Zeros and subnormals read as some 2^-127, infinities
+// A float as a double by integer operations (the conversion instruction kept its pipe 64% busy).  Zeros and subnormals read as some 2^-127, infinities
 // as 2^128, none of which a weight shows.  16-bit types leave the low word empty.
 template <bool kLow>
 __device__ __forceinline__ double widen(float x) {
