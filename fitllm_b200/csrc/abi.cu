@@ -1,6 +1,7 @@
 // extern "C" entry points of libfitq (declared in include/fitq.h): argument
 // checks, workspace carving and kernel sequencing.  No entry point allocates
 // device memory; scratch comes from the caller's workspace.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -1585,6 +1586,7 @@ int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_stride, con
   if ((q_out != q && kv4_meets(q_out, n * row * 2, q, n, q_stride, row)) ||
       kv4_meets(q_out, n * row * 2, k, n, k_stride, kv_row) || kv4_meets(q_out, n * row * 2, v, n, v_stride, kv_row))
     return fail(FITQ_ERR_ARG, "tree_append: q_out overlaps q (other than being q), k or v");
+  if (k_cache == v_cache) return fail(FITQ_ERR_ARG, "tree_append: keys and values in one cache");
   if (!current_sms(&rc)) return rc;
   return launch_status(fitq::launch_tree_append(t, q, q_stride, k, k_stride, v, v_stride, q_out, k_cache, v_cache,
                                                 cos_half, sin_half, rope_len, heads, tree->head_dim, tree->dtype,
@@ -1675,6 +1677,11 @@ int fitq_tree_keep(const fitq_tree* tree, void* const* k_caches, void* const* v_
     if (!k_caches[i] || !v_caches[i]) return fail(FITQ_ERR_ARG, "tree_keep: NULL cache of layer %d", i);
     if (!al16(k_caches[i]) || !al16(v_caches[i])) return fail(FITQ_ERR_ALIGN, "tree_keep: 16-byte alignment");
   }
+  std::vector<const void*> all(k_caches, k_caches + layers);  // each moves once
+  all.insert(all.end(), v_caches, v_caches + layers);
+  std::sort(all.begin(), all.end());
+  if (std::adjacent_find(all.begin(), all.end()) != all.end())
+    return fail(FITQ_ERR_ARG, "tree_keep: a cache is given twice");
   if ((reinterpret_cast<uintptr_t>(accepted) & 7u) ||
       ((reinterpret_cast<uintptr_t>(path) | reinterpret_cast<uintptr_t>(lengths)) & 3u))
     return fail(FITQ_ERR_ALIGN, "tree_keep: tensors must be aligned to their elements");

@@ -13,9 +13,8 @@
 // some 1e-14 with the order of a sum and the exponentials' last digits, by 1e-8 in fp32, and a
 // random number falls into that gap once in 10^3 rows of 152,064 tokens (once in 10^6 with
 // what is left here).  An exponential is 2^(n / 1024) from a table times a polynomial of degree
-// two (its Taylor series: 7e-12 of it at |x| <= ln 2 / 2048), summed by the last product:
-// seven fp64 operations and some ten others per element, which the issue of instructions
-// bounds.
+// two (its Taylor series: 7e-12 of it at |x| <= ln 2 / 2048): with its place in the sum eight fp64
+// operations and some ten others per element, which the issue of instructions bounds.
 //
 // A cluster of up to sixteen CTAs walks with a sequence; every warp owns a run of the
 // vocabulary, so that the cumulated sum is found by its parts: ranks, warps, lanes.  A CTA sums
@@ -109,8 +108,9 @@ __device__ __forceinline__ float max_vec(const uint4& u) {
   }
 }
 
-// A float as a double by integer operations (the conversion instruction kept its pipe 64% busy).  Zeros and subnormals read as some 2^-127, infinities
-// as 2^128, none of which a weight shows.  16-bit types leave the low word empty.
+// A float as a double by integer operations (the conversion instruction kept its pipe 64% busy).
+// Zeros and subnormals read as some 2^-127, infinities as 2^128, none of which a weight shows.  16-bit
+// types leave the low word empty.
 template <bool kLow>
 __device__ __forceinline__ double widen(float x) {
   const uint32_t u = __float_as_uint(x);
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
   double total = 0.0;       // of the weights as refusals have left them
   double entered = 0.0;     // the total before any refusal
   uint64_t kids = 0;        // children of token cur
-  bool pared = false;       // refusals have been taken out of total, its_sum and sh_run one by one
+  bool exact = false;       // total, its_sum and sh_run are sums of the weights as they are drawn from
   float top = 0.f;          // the row's largest logit
   int best = 0;
   Scale by{};
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] : 0.0;
     total = warp_sum(its_sum);
     rescale = 1.0;
-    pared = false;
+    exact = true;
   };
   // the row's first token with its largest logit, by the whole cluster
   auto find_best = [&]() {
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     z = static_cast<const T*>(p.logits) + b * p.stride_b + cur * p.stride_t;
     q = p.probs ? p.probs + b * p.probs_stride_b + min(cur, p.T - 2) * p.probs_stride_t : nullptr;
     refused = 0;
-    pared = false;
+    exact = false;
     row = Row<T>(z, p.V);
     const int warps = static_cast<int>(ranks) * kWarps, per = (row.granules + warps - 1) / warps;
     lo = min(row.granules, (static_cast<int>(rank) * kWarps + warp) * per);
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
         sum_up();
       } else if (w > 0.0) {
         total -= w;
-        pared = true;
+        exact = false;
         const int warps = static_cast<int>(ranks) * kWarps, per = (row.granules + warps - 1) / warps;
         const int owner = static_cast<int>((x + row.lead) / kVec) / per;
         if (lane == owner / kWarps) its_sum -= w;
@@ -508,31 +508,61 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     if (usable && !greedy) find_best();  // refusals have left no weight
     if (tid == 0 && rank == 0) p.next_token[b] = usable ? best : -1;
   } else {
-    // (a difference may have left a part that has no weight some of its last digits: no token to name as last)
-    if (pared && !(static_cast<double>(p.uniforms[b * p.T]) * total < total * (1.0 - 1e-9))) sum_up();
-    __syncthreads();  // sh_run is complete
-    // the first token whose cumulated weight exceeds u_0 of the total
-    const double goal = static_cast<double>(p.uniforms[b * p.T]) * total;
-    double before = 0.0;
-    int at = -1, last = 0;
-    for (int r = 0; r < static_cast<int>(ranks); ++r) {
-      const double s = __shfl_sync(0xffffffffu, its_sum, r);
-      if (s > 0.0) last = r;
-      if (at < 0 && before + s > goal) at = r;
-      if (at < 0) before += s;
-    }
-    const bool past = at < 0;  // a random number of one or more: the last token that has weight
-    if (past) at = last;
-    if (static_cast<int>(rank) == at) {
-      int w_at = -1, w_last = 0;
-      double base = past ? 0.0 : before;
-      for (int w = 0; w < kWarps; ++w) {
-        const double s = sh_run[w] * rescale;
-        if (s > 0.0) w_last = w;
-        if (!past && w_at < 0 && base + s > goal) w_at = w;
-        if (w_at < 0 && !past) base += s;
+    // The first token whose cumulated weight exceeds u_0 of the total.  A difference, or a sum by another
+    // largest logit, may leave some last digits to a part in which no weight is left: where the random
+    // number falls next to a border of the parts they are summed anew, and a part then has a sum where
+    // it has a token to name.
+    const double u0 = fmax(static_cast<double>(p.uniforms[b * p.T]), 0.0);
+    double goal, before;
+    int at;
+    bool past;  // a random number of one or more: the last token that has weight
+    for (;;) {
+      __syncthreads();  // sh_run is complete
+      goal = u0 * total;
+      before = 0.0;
+      at = -1;
+      int last = 0;
+      double here = 0.0;
+      for (int r = 0; r < static_cast<int>(ranks); ++r) {
+        const double s = __shfl_sync(0xffffffffu, its_sum, r);
+        if (s > 0.0) last = r;
+        if (at < 0 && before + s > goal) {
+          at = r;
+          here = s;
+        }
+        if (at < 0) before += s;
       }
-      if (w_at < 0) w_at = w_last;
+      past = at < 0;
+      if (past) at = last;
+      if (exact || (!past && goal - before > total * 1e-9 && before + here - goal > total * 1e-9)) break;
+      sum_up();
+    }
+    if (static_cast<int>(rank) == at) {
+      int w_at;
+      double base;
+      for (;;) {
+        int w_last = 0;
+        double here = 0.0;
+        w_at = -1;
+        base = past ? 0.0 : before;
+        for (int w = 0; w < kWarps; ++w) {
+          const double s = sh_run[w] * rescale;
+          if (s > 0.0) w_last = w;
+          if (!past && w_at < 0 && base + s > goal) {
+            w_at = w;
+            here = s;
+          }
+          if (w_at < 0 && !past) base += s;
+        }
+        const bool clear = w_at >= 0 && goal - base > total * 1e-9 && base + here - goal > total * 1e-9;
+        if (w_at < 0) w_at = w_last;
+        if (exact || clear) break;
+        __syncthreads();  // sh_run has been read
+        sum_runs(top, by);
+        rescale = 1.0;
+        exact = true;
+        __syncthreads();
+      }
       // that run again, 32 granules a warp, then the warp in whose granules it lies
       const int warps = static_cast<int>(ranks) * kWarps, per = (row.granules + warps - 1) / warps;
       const int first = min(row.granules, (static_cast<int>(rank) * kWarps + w_at) * per), end = min(row.granules, first + per);

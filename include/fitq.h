@@ -487,7 +487,7 @@ FITQ_API int fitq_tree_attention(const fitq_tree* tree, const void* q, int64_t q
  * path int32 [batch, tokens]: token 0 and the accepted ones, then -1; accepted int64 [batch]:
  * how many drafts; next_token int64 [batch].  A row with a NaN, or without a finite largest logit,
  * ends the walk with next_token -1; a sequence without token 0 gives accepted -1, next_token
- * -1.  Sums are fp64; where refusals leave no weight the largest logit's token is next. */
+ * -1.  Sums are fp64; a weight below exp(-707) of the largest is none; where refusals leave no weight the largest logit's token is next. */
 FITQ_API int fitq_tree_verify(const void* logits, int dtype, int64_t stride_b, int64_t stride_t,
                               int64_t batch, int tokens, int64_t vocab, const int64_t* ids,
                               const int32_t* parents, int64_t parents_stride, const float* uniforms,
@@ -495,7 +495,8 @@ FITQ_API int fitq_tree_verify(const void* logits, int dtype, int64_t stride_b, i
                               const float* temperatures, float temperature, int32_t* path,
                               int64_t* accepted, int64_t* next_token, fitq_stream_t stream);
 /* The accepted path stays: slot prefix + path[i] moves to slot prefix + i for
- * i <= accepted in every layer (k_caches, v_caches: host arrays of `layers` device pointers),
+ * i <= accepted in every layer (k_caches, v_caches: host arrays of `layers` device pointers, no
+ * cache twice),
  * lengths[b] = prefix[b] + accepted[b] + 1 (lengths may be prefix).  path, accepted as
  * fitq_tree_verify writes them; a path that does not ascend within the tree and the capacity
  * records FITQ_ERR_ARG and leaves its sequence as it was. */

@@ -432,6 +432,40 @@ def test_verify_of_refused_children_that_hold_all_the_weight(cuda_dev):
     assert int(verify_tree(z, draft, up, u, draft_probs=q).next_token) in range(v)
 
 
+@pytest.mark.parametrize("v,spread,temp", [(20_000, 2.0, 1.0), (9_000, 0.0, 1.0), (700, 2.0, 0.7), (20_000, 30.0, 0.05)])
+def test_verify_draws_next_to_a_border(cuda_dev, v, spread, temp):
+    """Few tokens allowed, the first of them drafted and refused, and random numbers that fall on a border
+    of the cumulated weights: the next token is always one that has weight."""
+    from fitllm_b200.verify import verify_tree
+    b, t, n = 96, 3, 40
+    g = torch.Generator(device=cuda_dev).manual_seed(v)
+    z = torch.full((b, t, v), float("-inf"), device=cuda_dev)
+    allowed = torch.stack([torch.randperm(min(v, 2500), device=cuda_dev, generator=g)[:n].sort().values for _ in range(b)])
+    some = torch.randn(b, n, device=cuda_dev, generator=g) * spread
+    z[:, 0] = z[:, 0].scatter(1, allowed, some)
+    z = z.bfloat16()
+    # exp(-707), 2^-1020, of the largest weighs nothing (exp(-746) is the last fp64 that is not 0); at the
+    # fourth case's temperature that is 35.35 below the largest, where bf16 logits are multiples of 1/8
+    weighed = z.clone()
+    weighed[z.double() < z.double().amax(-1, keepdim=True) - 707 * temp] = float("-inf")
+    draft = torch.zeros(b, t, dtype=torch.int64, device=cuda_dev)
+    draft[:, 1:] = allowed[:, :2]
+    up = torch.tensor([-1, 0, 0], dtype=torch.int32, device=cuda_dev)
+    for first in (0.0, 1 - 2.0 ** -24, 1.0):
+        u = torch.full((b, t), 1 - 2.0 ** -24, device=cuda_dev)
+        u[:, 0] = first
+        r = verify_tree(z, draft, up, u, temperature=temp)
+        for s in range(b):
+            path, acc, nxt = ref.verify(weighed[s], draft[s].tolist(), [-1, 0, 0], u[s], None, temp)
+            assert (int(r.accepted[s]), int(r.next_token[s])) == (acc, nxt), (first, s)
+    if spread == 0.0:  # equal weights: a random number on each border of the 38 that are left
+        u = torch.full((b, t), 1 - 2.0 ** -24, device=cuda_dev)
+        u[:, 0] = torch.arange(b, device=cuda_dev) % 38 / 38
+        r = verify_tree(z, draft, up, u)
+        at = torch.arange(b, device=cuda_dev)[:, None] % 38 + torch.tensor([1, 2], device=cuda_dev)  # either side of it
+        assert (r.next_token[:, None] == allowed.gather(1, at)).any(1).all() and not (r.next_token[:, None] == draft[:, 1:]).any()
+
+
 def test_verify_is_a_sample_of_the_model(cuda_dev):
     """First accepted-or-next tokens follow p, whatever was drafted: 40,000 sequences of one draft
     of a distribution far from p; chi-square over 8 tokens below its 1 - 1e-6 quantile (40.5 for 7)."""

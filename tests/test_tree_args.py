@@ -27,17 +27,17 @@ def _tree(**kw):
     return _lib.TreeC(**c)
 
 
-def _append(L, c, q=P, k=FAR, v=FAR, out=2 * FAR, kc=P, cos=P, rope=64, heads=8, qs=1024, ks=256):
-    return L.fitq_tree_append(c, q, qs, k, ks, v, ks, out, kc, P, cos, P, rope, heads, None)
+def _append(L, c, q=P, k=FAR, v=FAR, out=2 * FAR, kc=P, vc=3 * FAR, cos=P, rope=64, heads=8, qs=1024, ks=256):
+    return L.fitq_tree_append(c, q, qs, k, ks, v, ks, out, kc, vc, cos, P, rope, heads, None)
 
 
 def _attend(L, c, q=P, qs=1024, kc=P, out=FAR, heads=8, ws=P, size=1 << 40):
     return L.fitq_tree_attention(c, q, qs, kc, P, out, heads, ws, size, None)
 
 
-def _keep(L, c, layers=1, ptr=P, path=P, acc=P, lengths=P):
-    arr = (ctypes.c_void_p * max(layers, 1))(*[ptr] * max(layers, 1))
-    return L.fitq_tree_keep(c, arr, arr, layers, path, acc, lengths, None)
+def _keep(L, c, layers=1, ptr=P, path=P, acc=P, lengths=P, values=FAR):
+    k, v = ((ctypes.c_void_p * max(layers, 1))(*[x and x + i * (1 << 24) for i in range(max(layers, 1))]) for x in (ptr, values))
+    return L.fitq_tree_keep(c, k, v, layers, path, acc, lengths, None)
 
 
 BAD_TREES = [
@@ -67,6 +67,7 @@ def test_append_refusals(L):
     assert _append(L, c, qs=1000) == SHAPE and _append(L, c, qs=1028) == SHAPE and _append(L, c, ks=248) == SHAPE
     assert _append(L, c, q=P + 2) == ALIGN and _append(L, c, kc=P + 8) == ALIGN and _append(L, c, cos=P + 4) == ALIGN
     assert _append(L, c, out=P, qs=2048) == ARG and _append(L, c, out=P + 2048) == ARG and _append(L, c, k=2 * FAR) == ARG
+    assert _append(L, c, vc=P) == ARG  # keys and values in one cache
     if not torch.cuda.is_available():
         assert _append(L, c) == NO_DEVICE and _append(L, c, out=P) == NO_DEVICE
 
@@ -88,6 +89,7 @@ def test_keep_refusals(L):
     c = _tree()
     assert _keep(L, c, ptr=None) == ARG and _keep(L, c, path=None) == ARG and _keep(L, c, lengths=None) == ARG
     assert _keep(L, c, layers=0) == SHAPE
+    assert _keep(L, c, values=P) == ARG and _keep(L, c, layers=3, values=P + (2 << 24)) == ARG  # a cache twice
     assert _keep(L, c, lengths=P + 4) == ARG  # over the prefix, other than being it
     assert _keep(L, c, ptr=P + 8) == ALIGN and _keep(L, c, acc=P + 4) == ALIGN and _keep(L, c, path=P + 2) == ALIGN
 
