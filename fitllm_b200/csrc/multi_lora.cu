@@ -30,6 +30,7 @@
 
 #include "kernels.cuh"
 #include "kv4.cuh"
+#include "umma_warp.cuh"
 
 namespace fitq {
 namespace {
@@ -40,6 +41,7 @@ constexpr int kSlot = 128;       // tokens of a slot: 16 for each warp
 constexpr int kCols = 256;       // columns of a CTA of the second kernel for more than sixteen tokens
 constexpr int kAhead = 4;        // of their groups of 32, those whose y_add is on its way
 constexpr int kMaxParts = 8;     // CTAs of a cluster
+constexpr int kBox = 32;         // tokens of a copy: a slot loads no more than it has, but for the last one
 
 struct MultiLoraParams {
   const void *x, *a, *b, *y_add;
@@ -137,24 +139,24 @@ extern __shared__ float4 g_lora_smem[];
 __device__ __forceinline__ void cp16_zfill(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-
-// Stages of the first kernel's copies: 64 columns of a slot's tokens and of A.
+// Stages of the first kernel's copies: 64 columns of a slot's tokens and of A, as many as leave an SM
+// room for two CTAs.
 template <int R>
 struct ShrinkSmem {
-  static constexpr int kStages = 4;
   static constexpr int kX = kSlot * 128, kA = R * 128, kStage = kX + kA;
-  static constexpr int kRed = kWarps * 16 * R * 4;  // the warps' sums: 16 tokens each
-  static constexpr int kMany = kStages * kStage > kRed ? kStages * kStage : kRed;
+  static constexpr int kStages = R <= 32 ? 5 : 4;
+  static constexpr int kPitch = R + 4;              // floats of a token's sums: 16-byte stores of eight rows meet no bank twice
+  static constexpr int kRed = kWarps * 16 * R * 4;  // up to sixteen tokens: the warps' sums
+  static constexpr int kMany = kStages * kStage + 1024;
+  static constexpr uint32_t kTmem = R <= 32 ? 32 : 64;
+  static_assert(kSlot * kPitch * 4 <= kStages * kStage && kRed <= kMany, "the sums take the stages' place");
 };
 
 // kMany: some slot may have more than sixteen tokens.
 template <typename T, int R, bool kMany>
-__global__ void __launch_bounds__(kThreads, 2) multi_lora_shrink_kernel(const MultiLoraParams p) {
+__global__ void __launch_bounds__(kThreads, 2)
+    multi_lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a,
+                             const MultiLoraParams p) {
   constexpr int NT = R / 8;
   constexpr int kUnroll = R == 16 ? 4 : R == 32 ? 3 : 2;  // what the registers hold beside the sums
   using L = ShrinkSmem<R>;
@@ -203,67 +205,101 @@ __global__ void __launch_bounds__(kThreads, 2) multi_lora_shrink_kernel(const Mu
         }
     }
   } else if constexpr (kMany) {
-    // ---- sixteen tokens per warp, 64 columns at a time through shared memory: rows of 128 bytes,
-    // 16-byte piece c of row r at c ^ (r & 7)
-    const uint32_t base = smem_u32(g_lora_smem);
-    const int steps = (k1 - k0 + 63) / 64;
-    auto load = [&](int s) {
-      if (s < steps) {
-        const uint32_t at = base + s % L::kStages * L::kStage;
-        const int c = threadIdx.x & 7, col = k0 + s * 64 + 8 * c;
-        const uint32_t in = col < k1 ? 16u : 0u;
-#pragma unroll
-        for (int i = 0; i < kSlot / 32; ++i) {
-          const int row = (threadIdx.x >> 3) + 32 * i;
-          const bool ok = row < count && in;
-          cp16_zfill(at + row * 128 + ((c ^ (row & 7)) << 4), ok ? x + row * p.x_stride + col : x, ok ? 16u : 0u);
-        }
-#pragma unroll
-        for (int i = 0; i < (R + 31) / 32; ++i) {
-          const int row = (threadIdx.x >> 3) + 32 * i;
-          if (R % 32 == 0 || row < R)
-            cp16_zfill(at + L::kX + row * 128 + ((c ^ (row & 7)) << 4), in ? a + static_cast<int64_t>(row) * p.k + col : a, in);
-        }
+    // ---- 64 columns at a time: TMA by warp 0, MMAs of 128 tokens x R by warp 1.  Rows of the tile behind the
+    // slot's tokens hold another sequence's or nothing that was written: only their own sums see them.
+    __shared__ uint64_t b_full[L::kStages], b_free[L::kStages], b_done;
+    __shared__ uint32_t sh_tmem;
+    __shared__ int sh_abort;
+    const int steps = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
+    uint8_t* ring = reinterpret_cast<uint8_t*>(g_lora_smem) + ((1024u - (smem_u32(g_lora_smem) & 1023u)) & 1023u);
+    red = reinterpret_cast<float*>(ring);
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < L::kStages; ++i) {
+        mbar_init(&b_full[i], 1);
+        mbar_init(&b_free[i], 1);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    for (int s = 0; s < L::kStages - 1; ++s) load(s);
-    const int mat = lane >> 3, r8 = lane & 7;
-    const int xrow = warp * 16 + (mat & 1) * 8 + r8;  // matrices: rows 0-7 | 8-15 x columns 0-7 | 8-15 of sixteen
-    const int arow = (mat >> 1) * 8 + r8;             // matrices: columns 0-7 | 8-15 x two MMAs' rows
-    for (int s = 0; s < steps; ++s) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 2) : "memory");
-      __syncthreads();  // stage s is there; every warp is done with the one that is loaded next
-      load(s + L::kStages - 1);
-      if (warp * 16 >= count) continue;
-      const uint32_t at = base + s % L::kStages * L::kStage;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t xa[4];
-        ldsm4(at + xrow * 128 + (((2 * kk + (mat >> 1)) ^ (xrow & 7)) << 4), xa);
-#pragma unroll
-        for (int t = 0; t < NT; t += 2) {
-          uint32_t bb[4];
-          const int row = 8 * t + arow;
-          ldsm4(at + L::kX + row * 128 + (((2 * kk + (mat & 1)) ^ (row & 7)) << 4), bb);
-          mma_16816<T>(acc[t], xa[0], xa[1], xa[2], xa[3], bb[0], bb[1]);
-          mma_16816<T>(acc[t + 1], xa[0], xa[1], xa[2], xa[3], bb[2], bb[3]);
-        }
-      }
+      mbar_init(&b_done, 1);
+      fence_mbar_init();
+      sh_abort = 0;
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();  // the stages' place becomes the sums'
-  }
-  float* mine = red + warp * 16 * R;
+    if (warp == 1) {
+      tmem_alloc(&sh_tmem, L::kTmem);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh_tmem;
+    if (warp == 0) {
+      if (lane == 0) {
+        const int boxes = (count + kBox - 1) / kBox;
+        int s = 0;
+        bool ok = true;
+        for (; s < steps; ++s) {
+          const int at = s % L::kStages, col = k0 + 64 * s;
+          if (s >= L::kStages) ok = mbar_wait(&b_free[at], (s / L::kStages & 1) ^ 1, &sh_abort, p.status);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&b_full[at], boxes * (kBox * 128) + L::kA);
+          uint8_t* stage = ring + at * L::kStage;
+          tma_load_2d(stage + L::kX, &tm_a, &b_full[at], col, l * R);
+          for (int i = 0; i < boxes; ++i)
+            tma_load_2d(stage + i * (kBox * 128), &tm_x, &b_full[at], col, static_cast<int>(first) + i * kBox);
+        }
+        if (!ok) {  // the copies in flight land before their place is used again
+          int never = 0;
+          for (int i = s > L::kStages ? s - L::kStages : 0; i < s; ++i)
+            mbar_wait(&b_full[i % L::kStages], i / L::kStages & 1, &never, p.status);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      constexpr uint32_t idesc = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) |
+                                 (static_cast<uint32_t>(R >> 3) << 17) | (static_cast<uint32_t>(kSlot >> 4) << 24);
+      const uint64_t dx = umma_smem_desc_sw128(smem_u32(ring)), da = umma_smem_desc_sw128(smem_u32(ring) + L::kX);
+      for (int s = 0; s < steps; ++s) {
+        const uint32_t at = s % L::kStages;
+        if (!mbar_wait_warp(&b_full[at], s / L::kStages & 1, &sh_abort, p.status)) break;
+        tc_fence_after();
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    *reinterpret_cast<float2*>(mine + g * R + 8 * t + 2 * q) = make_float2(acc[t][0], acc[t][1]);
-    *reinterpret_cast<float2*>(mine + (g + 8) * R + 8 * t + 2 * q) = make_float2(acc[t][2], acc[t][3]);
+        for (int kk = 0; kk < 4; ++kk)
+          umma_f16_ss(tmem, dx + ((at * L::kStage + kk * 32) >> 4), da + ((at * L::kStage + kk * 32) >> 4), idesc,
+                      s > 0 || kk > 0 ? 1u : 0u);
+        commit_warp(&b_free[at]);
+      }
+      commit_warp(&b_done);
+      int never = 0;
+      mbar_wait_warp(&b_done, 0, &never, p.status);
+    }
+    __syncthreads();  // the stages' place becomes the sums'
+    tc_fence_after();
+    const int row = 32 * (warp & 3) + lane;
+    for (int c = 16 * (warp >> 2); c < R; c += 32) {
+      uint32_t v[16];
+      tmem_ld_x16(tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + c, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(red + row * L::kPitch + c + i) =
+            steps > 0 ? make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]))
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem, L::kTmem);
+    }
   }
-  __syncthreads();
   const int cells = count * (R / 4);
   float4* red4 = reinterpret_cast<float4*>(red);
   if (few) {  // the warps' sums in order, into the first warp's place
+    float* mine = red + warp * 16 * R;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      *reinterpret_cast<float2*>(mine + g * R + 8 * t + 2 * q) = make_float2(acc[t][0], acc[t][1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * R + 8 * t + 2 * q) = make_float2(acc[t][2], acc[t][3]);
+    }
+    __syncthreads();
     for (int e = threadIdx.x; e < cells; e += kThreads) {
       float4 s = red4[e];
 #pragma unroll
@@ -278,14 +314,15 @@ __global__ void __launch_bounds__(kThreads, 2) multi_lora_shrink_kernel(const Mu
     }
   }
   float4* out = reinterpret_cast<float4*>(p.t + first * R);
+  auto cell = [&](int e) { return few ? e : e + e / (R / 4) * ((L::kPitch - R) / 4); };
   if (p.parts == 1) {
     __syncthreads();
-    for (int e = threadIdx.x; e < cells; e += kThreads) out[e] = red4[e];
+    for (int e = threadIdx.x; e < cells; e += kThreads) out[e] = red4[cell(e)];
     return;
   }
   cluster_barrier();
   for (int e = threadIdx.x * p.parts + part; e < cells; e += kThreads * p.parts) {
-    const float* at = reinterpret_cast<const float*>(red4 + e);
+    const float* at = reinterpret_cast<const float*>(red4 + cell(e));
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int r = 0; r < p.parts; ++r) {
       const float4 v = remote_float4(at, r);
@@ -493,11 +530,21 @@ int multi_lora_t(MultiLoraParams p, cudaStream_t st, int num_sms) {
   // are counted as a batch of any lengths has them on average (a sequence's last one half full), so
   // that the sums do not depend on how the lengths were passed.
   const int64_t half = p.tokens / kSlot + p.batch / 2, real = half > p.batch ? half : p.batch;
+  const int64_t room = p.tokens > 16ll * p.batch ? num_sms : 2ll * num_sms;
   int parts = 1;
-  while (parts < kMaxParts && real * parts * 2 <= 2ll * num_sms && p.k > 256 * parts) parts *= 2;
+  while (parts < kMaxParts && real * parts * 2 <= room && p.k > 256 * parts) parts *= 2;
   p.parts = parts;
   p.part_cols = ((p.k + parts - 1) / parts + 63) / 64 * 64;
-  const bool many = p.q_start != nullptr || p.t_new > 16;
+  const bool many = p.q_start != nullptr ? p.tokens > 16 : p.t_new > 16;
+  CUtensorMap tx{}, ta{};
+  if (many) {
+    const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if (!encode_tmap_2d(&tx, type, p.x, p.k, p.tokens, p.x_stride * 2, 64, kBox, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
+        !encode_tmap_2d(&ta, type, p.a, p.k, static_cast<uint64_t>(p.adapters) * R, p.k * 2, 64, R, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
+      return FITQ_ERR_CUDA;
+  }
   const int smem = many ? ShrinkSmem<R>::kMany : ShrinkSmem<R>::kRed;
   auto* shrink = many ? multi_lora_shrink_kernel<T, R, true> : multi_lora_shrink_kernel<T, R, false>;
   if (smem > 48 * 1024 && !set_smem_limit(shrink, smem)) return FITQ_ERR_CUDA;
@@ -514,7 +561,7 @@ int multi_lora_t(MultiLoraParams p, cudaStream_t st, int num_sms) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, shrink, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, shrink, tx, ta, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   const int cols = many ? kCols : few_groups<R>() * 32 * kWarps;
