@@ -1,8 +1,8 @@
 // Low-rank adapters of many requests beside a shared projection:
 //   y[n] = y_add[n] + s_l (x[n].A_l^T).B_l^T,   l = adapter of token n's sequence.
 //
-// Both products run on mma.sync m16n8k16: an adapter's R columns or rows give it a few
-// operations per byte, so that the bytes of x, A, B and y are what costs.
+// An adapter's R columns or rows give it a few operations per byte: the bytes of x, A, B and y are
+// what costs.  Few tokens, and the second product, whose contraction is R long, run on mma.sync m16n8k16.
 //
 // Tokens are taken in slots of up to kSlot of one sequence.  Slot numbers need no counting:
 // sequence b, whose tokens begin at q_start[b], owns the numbers from q_start[b] / kSlot + b
@@ -13,8 +13,9 @@
 // K.  Up to sixteen tokens: the eight warps split the part again, and a lane reads 16 bytes of a
 // row of x and of A at a time and feeds them to two MMAs (the contraction index is permuted
 // alike in both), so that a single token is summed by 64 warps with every load in flight at
-// once.  More: sixteen tokens per warp, x and A through four stages of cp.async, 64 columns
-// each.  Parts join in shared memory, then over the cluster, in order (deterministic); T stays
+// once.  More: tcgen05, M = 128 tokens by N = R, x and A through a ring of TMA tiles of 64 columns (a
+// full slot's x is one copy: as four, from one lane, the copies' issue took 172 us where it is 129 now).
+// Parts join in shared memory, then over the cluster, in order (deterministic); T stays
 // in fp32.
 //
 // multi_lora_expand_kernel, y = y_add + s T.B_l^T: T enters as two 16-bit numbers, hi + lo (a
@@ -41,7 +42,7 @@ constexpr int kSlot = 128;       // tokens of a slot: 16 for each warp
 constexpr int kCols = 256;       // columns of a CTA of the second kernel for more than sixteen tokens
 constexpr int kAhead = 4;        // of their groups of 32, those whose y_add is on its way
 constexpr int kMaxParts = 8;     // CTAs of a cluster
-constexpr int kBox = 32;         // tokens of a copy: a slot loads no more than it has, but for the last one
+constexpr int kBox = 32;         // tokens of a copy where a slot is not full: few behind its last one are read
 
 struct MultiLoraParams {
   const void *x, *a, *b, *y_add;
@@ -140,7 +141,8 @@ __device__ __forceinline__ void cp16_zfill(uint32_t dst, const void* src, uint32
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // Stages of the first kernel's copies: 64 columns of a slot's tokens and of A, as many as leave an SM
-// room for two CTAs.
+// room for two CTAs (twice as many for one CTA: no faster where the SMs have equal shares, and slower where
+// clusters then find no place).
 template <int R>
 struct ShrinkSmem {
   static constexpr int kX = kSlot * 128, kA = R * 128, kStage = kX + kA;
@@ -152,11 +154,11 @@ struct ShrinkSmem {
   static_assert(kSlot * kPitch * 4 <= kStages * kStage && kRed <= kMany, "the sums take the stages' place");
 };
 
-// kMany: some slot may have more than sixteen tokens.
+// kMany: some slot may have more than sixteen tokens.  tm_s and tm_x: x in copies of kSlot and kBox tokens.
 template <typename T, int R, bool kMany>
 __global__ void __launch_bounds__(kThreads, 2)
-    multi_lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a,
-                             const MultiLoraParams p) {
+    multi_lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_s, const __grid_constant__ CUtensorMap tm_x,
+                             const __grid_constant__ CUtensorMap tm_a, const MultiLoraParams p) {
   constexpr int NT = R / 8;
   constexpr int kUnroll = R == 16 ? 4 : R == 32 ? 3 : 2;  // what the registers hold beside the sums
   using L = ShrinkSmem<R>;
@@ -231,40 +233,47 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc_fence_after();
     const uint32_t tmem = sh_tmem;
     if (warp == 0) {
-      if (lane == 0) {
-        const int boxes = (count + kBox - 1) / kBox;
-        int s = 0;
-        bool ok = true;
-        for (; s < steps; ++s) {
-          const int at = s % L::kStages, col = k0 + 64 * s;
-          if (s >= L::kStages) ok = mbar_wait(&b_free[at], (s / L::kStages & 1) ^ 1, &sh_abort, p.status);
-          if (!ok) break;
-          mbar_arrive_expect_tx(&b_full[at], boxes * (kBox * 128) + L::kA);
-          uint8_t* stage = ring + at * L::kStage;
-          tma_load_2d(stage + L::kX, &tm_a, &b_full[at], col, l * R);
-          for (int i = 0; i < boxes; ++i)
-            tma_load_2d(stage + i * (kBox * 128), &tm_x, &b_full[at], col, static_cast<int>(first) + i * kBox);
-        }
-        if (!ok) {  // the copies in flight land before their place is used again
-          int never = 0;
-          for (int i = s > L::kStages ? s - L::kStages : 0; i < s; ++i)
-            mbar_wait(&b_full[i % L::kStages], i / L::kStages & 1, &never, p.status);
+      const int rows = count > kSlot - kBox ? kSlot : kBox;
+      const int boxes = (count + rows - 1) / rows;
+      const CUtensorMap* map = lane < boxes ? (rows == kSlot ? &tm_s : &tm_x) : &tm_a;  // a lane per copy
+      const int y = lane < boxes ? static_cast<int>(first) + lane * rows : l * R;
+      uint8_t* dst = ring + (lane < boxes ? lane * (rows * 128) : L::kX);
+      int s = 0, at = 0;
+      uint32_t phase = 1;  // of the stage's release
+      bool ok = true;
+      for (; s < steps; ++s) {
+        if (s >= L::kStages) ok = mbar_wait_warp(&b_free[at], phase, &sh_abort, p.status);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&b_full[at], boxes * (rows * 128) + L::kA);
+        __syncwarp();
+        if (lane <= boxes) tma_load_2d(dst + at * L::kStage, map, &b_full[at], k0 + 64 * s, y);
+        if (++at == L::kStages) {
+          at = 0;
+          phase ^= 1;
         }
       }
-      __syncwarp();
+      if (!ok) {  // the copies in flight land before their place is used again
+        int never = 0;
+        for (int i = s > L::kStages ? s - L::kStages : 0; i < s; ++i)
+          mbar_wait_warp(&b_full[i % L::kStages], i / L::kStages & 1, &never, p.status);
+      }
     } else if (warp == 1) {
       constexpr uint32_t idesc = (1u << 4) | (std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10)) |
                                  (static_cast<uint32_t>(R >> 3) << 17) | (static_cast<uint32_t>(kSlot >> 4) << 24);
       const uint64_t dx = umma_smem_desc_sw128(smem_u32(ring)), da = umma_smem_desc_sw128(smem_u32(ring) + L::kX);
+      uint32_t at = 0, phase = 0;
       for (int s = 0; s < steps; ++s) {
-        const uint32_t at = s % L::kStages;
-        if (!mbar_wait_warp(&b_full[at], s / L::kStages & 1, &sh_abort, p.status)) break;
+        if (!mbar_wait_warp(&b_full[at], phase, &sh_abort, p.status)) break;
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
           umma_f16_ss(tmem, dx + ((at * L::kStage + kk * 32) >> 4), da + ((at * L::kStage + kk * 32) >> 4), idesc,
                       s > 0 || kk > 0 ? 1u : 0u);
         commit_warp(&b_free[at]);
+        if (++at == static_cast<uint32_t>(L::kStages)) {
+          at = 0;
+          phase ^= 1;
+        }
       }
       commit_warp(&b_done);
       int never = 0;
@@ -526,20 +535,28 @@ int64_t slots_of(int64_t tokens, int batch, bool ragged, int size) {
 template <typename T, int R>
 int multi_lora_t(MultiLoraParams p, cudaStream_t st, int num_sms) {
   const int64_t slots = slots_of(p.tokens, p.batch, p.q_start != nullptr, kSlot);
-  // parts of K: as many as find room at once, two CTAs on an SM, of 256 columns at least.  Slots
-  // are counted as a batch of any lengths has them on average (a sequence's last one half full), so
-  // that the sums do not depend on how the lengths were passed.
+  // Parts of K, of 256 columns at least.  Slots are counted as a batch of any lengths has them on average (a
+  // sequence's last one half full), so that the sums do not depend on how the lengths were passed.  Few
+  // tokens: as many parts as find room at once, two CTAs on an SM, a power of two.  Many: a CTA for every SM, or
+  // two parts where that leaves some without (36 slots, K = 27,648, rank 64, 1 to 8 parts: 131, 77, 63, 59,
+  // 57, 59, 76 us; 118 slots: 158, 140, 161, 150; 47 slots, K = 5,120: 32, 24, 25, 25, 27).
   const int64_t half = p.tokens / kSlot + p.batch / 2, real = half > p.batch ? half : p.batch;
-  const int64_t room = p.tokens > 16ll * p.batch ? num_sms : 2ll * num_sms;
+  const bool prompts = p.tokens > 16ll * p.batch;
   int parts = 1;
-  while (parts < kMaxParts && real * parts * 2 <= room && p.k > 256 * parts) parts *= 2;
+  if (prompts) {
+    while (parts < kMaxParts && real * (parts + 1) <= (parts == 1 ? 2ll * num_sms : num_sms) && p.k > 256 * parts) ++parts;
+  } else {
+    while (parts < kMaxParts && real * parts * 2 <= 2ll * num_sms && p.k > 256 * parts) parts *= 2;
+  }
   p.parts = parts;
   p.part_cols = ((p.k + parts - 1) / parts + 63) / 64 * 64;
   const bool many = p.q_start != nullptr ? p.tokens > 16 : p.t_new > 16;
-  CUtensorMap tx{}, ta{};
+  CUtensorMap ts{}, tx{}, ta{};
   if (many) {
     const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    if (!encode_tmap_2d(&tx, type, p.x, p.k, p.tokens, p.x_stride * 2, 64, kBox, CU_TENSOR_MAP_SWIZZLE_128B,
+    if (!encode_tmap_2d(&ts, type, p.x, p.k, p.tokens, p.x_stride * 2, 64, kSlot, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
+        !encode_tmap_2d(&tx, type, p.x, p.k, p.tokens, p.x_stride * 2, 64, kBox, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B) ||
         !encode_tmap_2d(&ta, type, p.a, p.k, static_cast<uint64_t>(p.adapters) * R, p.k * 2, 64, R, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
@@ -547,7 +564,7 @@ int multi_lora_t(MultiLoraParams p, cudaStream_t st, int num_sms) {
   }
   const int smem = many ? ShrinkSmem<R>::kMany : ShrinkSmem<R>::kRed;
   auto* shrink = many ? multi_lora_shrink_kernel<T, R, true> : multi_lora_shrink_kernel<T, R, false>;
-  if (smem > 48 * 1024 && !set_smem_limit(shrink, smem)) return FITQ_ERR_CUDA;
+  if (many && !set_smem_limit(shrink, ShrinkSmem<R>::kMany)) return FITQ_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(slots * parts));
   cfg.blockDim = dim3(kThreads);
@@ -561,7 +578,7 @@ int multi_lora_t(MultiLoraParams p, cudaStream_t st, int num_sms) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, shrink, tx, ta, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, shrink, ts, tx, ta, p);
   note_launch();
   if (e != cudaSuccess) return FITQ_ERR_CUDA;
   const int cols = many ? kCols : few_groups<R>() * 32 * kWarps;
