@@ -24,9 +24,9 @@
 // row: y and y_add move in 16-byte pieces.  One rounding, of y.
 //
 // Bound: one token, two launches (5.3 us at K = N = 5,120, rank 16); 64 tokens of as many adapters on 5,120 x
-// 27,648: 23 us, B at 2.9 TB/s, as a CTA waits for its adapter, T and B in turn; prompts of 4,000 tokens on
-// 27,648 x 5,120 at rank 64: 97 us, 72 of them the first kernel's (x at 3.0 TB/s; mma.sync 41% busy, and its
-// operands' way through shared memory).
+// 27,648: 23 us, B at 2.9 TB/s, as a CTA waits for its adapter, T and B in turn; six prompts of 4,180
+// tokens on 27,648 x 5,120 at rank 64: 88 us, 50 of them the first kernel's (x at 4.3 TB/s, with A 7 TB/s into
+// the SMs), 33 the second's, whose loads and mma.sync (36% busy) wait for each other.
 #include <type_traits>
 
 #include "kernels.cuh"

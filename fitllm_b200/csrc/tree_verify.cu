@@ -23,7 +23,7 @@
 // subtraction.
 // Bound: the chain of a visited row (largest 1.1, sum 2.8, exchange 0.8, joining 0.8, a child's test 0.7 us
 // on eight CTAs; 5.4 in all on sixteen), and a batch's deepest path.  A chain of 5 rows of 152,064 tokens: 20 us;
-// 64 of them: 97; 16 trees of 32 tokens over 32,001: 18; one row of each of 64 sequences: 21.
+// 64 of them: 98; 16 trees of 32 tokens over 32,001: 18; one row of each of 64 sequences: 21.
 #include <mutex>
 #include <type_traits>
 
