@@ -76,6 +76,32 @@ def test_rows_of_no_sequence_stay(cuda_dev):
     assert torch.equal(ops.multi_lora(x, a, b, scale, adapter, y, q_start=start, out=out.clone())[rows], got[rows])
 
 
+@pytest.mark.parametrize("k,r,dtype", [(1032, 64, torch.bfloat16), (8, 16, torch.float16), (2120, 48, torch.float16),
+                                       (264, 32, torch.bfloat16)])
+def test_prompts_beside_one_another(cuda_dev, k, r, dtype):
+    """Slots that are full, nearly so and not, in parts of K some of which are short or empty: rows of other
+    sequences that hold no numbers stand in the same copies and reach nobody."""
+    from fitllm_b200 import ops
+    news = [100, 20, 128, 97, 96, 31, 260, 17, 16, 1]
+    x, y, a, b, scale, adapter, starts = _state(cuda_dev, news, k, 136, r, 3, dtype, seed=k)
+    adapter.copy_(torch.tensor([0, -1, 2, -1, 1, 0, -1, 2, 1, -1]))
+    start = torch.tensor(starts, dtype=torch.int32, device=cuda_dev)
+    clean = ops.multi_lora(x, a, b, scale, adapter, y, q_start=start)
+    _check(x, y, a, b, scale, adapter, starts, clean)
+    for s, l in enumerate(adapter.tolist()):
+        if l < 0:
+            x[starts[s]:starts[s + 1]] = float("nan")
+    assert torch.equal(ops.multi_lora(x, a, b, scale, adapter, y, q_start=start), clean)
+    wide = torch.full((x.shape[0], k + 24), float("inf"), device=cuda_dev).to(dtype)
+    wide[:, 16:16 + k] = x
+    assert torch.equal(ops.multi_lora(wide[:, 16:16 + k], a, b, scale, adapter, y, q_start=start), clean)
+    # equal lengths, told or not
+    even = torch.arange(0, 601, 100, dtype=torch.int32, device=cuda_dev)
+    x, y, adapter = x[:600].nan_to_num(0.5), y[:600], adapter[:6].clamp(min=0)
+    assert torch.equal(ops.multi_lora(x, a, b, scale, adapter, y, q_start=even), ops.multi_lora(x, a, b, scale, adapter, y))
+    assert ops.device_status() == 0
+
+
 def test_in_place_and_strided(cuda_dev):
     from fitllm_b200 import ops
     x, y, a, b, scale, adapter, starts = _state(cuda_dev, [9, 40], 128, 136, 32, 3, torch.float16)
