@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
   double total = 0.0;       // of the weights as refusals have left them
   double entered = 0.0;     // the total before any refusal
   uint64_t kids = 0;        // children of token cur
-  bool exact = false;       // total, its_sum and sh_run are sums of the weights as they are drawn from
+  bool exact = false;       // total, the parts and sh_run are sums of the weights as they are drawn from
   float top = 0.f;          // the row's largest logit
   int best = 0;
   Scale by{};
@@ -306,7 +306,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
   int lo = 0, hi = 0;       // this warp's granules
   double rescale = 0.0;     // what makes sh_run this CTA's part of the total
   double its_sum = 0.0;     // lane r: rank r's part
+  float its_top = 0.f;      // lane r: the logit that it was summed by
 
+  // what makes weights by logit x weights by the row's largest
+  auto part_of = [&](float x) -> double { return x == top ? 1.0 : by.point(sh_table, x); };
   // what refusals have left of weight w of token v
   auto left = [&](double w, int v, float qv) -> double {
     if (q) {
@@ -387,6 +390,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     __syncthreads();
     sum_runs(top, by);
     exchange(false, 0.f);
+    its_top = top;
     its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] : 0.0;
     total = warp_sum(its_sum);
     rescale = 1.0;
@@ -453,9 +457,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     }
     by.set(top, temp);
     // the ranks' sums, by the row's largest logit: a lane each
-    its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] * by.point(sh_table, sh_tops[slot ^ 1][lane]) : 0.0;
+    its_top = lane < static_cast<int>(ranks) ? sh_tops[slot ^ 1][lane] : -INFINITY;
+    its_sum = lane < static_cast<int>(ranks) ? sh_sums[slot ^ 1][lane] * part_of(its_top) : 0.0;
     total = warp_sum(its_sum);
-    rescale = by.point(sh_table, mine);
+    rescale = part_of(mine);
     entered = total;
   };
 
@@ -489,17 +494,22 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
       }
       __syncthreads();
       ++refused;
-      // Without q a refusal takes one weight away.  As long as a thousandth of the row's weight is left, the
-      // difference has its digits; behind that, and with q, the sum is taken anew.
+      // Without q a refusal takes one weight away, by the logit that its part was summed by: what is subtracted
+      // is the number that was added (by another logit it differs by some 1e-11 of itself, which is then all that
+      // is left of a part without tokens).  As long as a thousandth of the row's weight is left, the sums'
+      // roundings, some 100 x 2^-53 of it, are 1e-11 of the difference; behind that, and with q, the sum is taken anew.
       if (q || !(total - w >= entered * 0x1p-10)) {
         sum_up();
       } else if (w > 0.0) {
-        total -= w;
         exact = false;
         const int warps = static_cast<int>(ranks) * kWarps, per = (row.granules + warps - 1) / warps;
         const int owner = static_cast<int>((x + row.lead) / kVec) / per;
-        if (lane == owner / kWarps) its_sum -= w;
-        if (static_cast<int>(rank) == owner / kWarps && tid == 0) sh_run[owner % kWarps] -= w / rescale;
+        Scale own{};
+        own.set(__shfl_sync(0xffffffffu, its_top, owner / kWarps), temp);
+        const double gone = own.point(sh_table, static_cast<float>(z[x]));
+        if (lane == owner / kWarps) its_sum -= gone * part_of(its_top);
+        total = warp_sum(its_sum);
+        if (static_cast<int>(rank) == owner / kWarps && tid == 0) sh_run[owner % kWarps] -= gone;
       }
     }
   }
@@ -508,10 +518,10 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const TreeVeri
     if (usable && !greedy) find_best();  // refusals have left no weight
     if (tid == 0 && rank == 0) p.next_token[b] = usable ? best : -1;
   } else {
-    // The first token whose cumulated weight exceeds u_0 of the total.  A difference, or a sum by another
-    // largest logit, may leave some last digits to a part in which no weight is left: where the random
-    // number falls next to a border of the parts they are summed anew, and a part then has a sum where
-    // it has a token to name.
+    // The first token whose cumulated weight exceeds u_0 of the total.  A difference may leave some last digits
+    // (1e-11 of the total) to a part in which no weight is left, and a sum by another largest logit moves its
+    // borders as far: where the random number falls within 1e-9 of a border the parts are summed anew, and a
+    // part then has a sum where it has a token to name.
     const double u0 = fmax(static_cast<double>(p.uniforms[b * p.T]), 0.0);
     double goal, before;
     int at;
