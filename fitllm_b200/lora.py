@@ -131,7 +131,7 @@ class MultiLoRALinear(nn.Module):
     """An NF4 Linear4bit with ``slots`` adapters of rank up to ``rank``, one per sequence:
     forward(x) = base(x) + scaling[l] (x.A_l^T).B_l^T, l = the sequence's slot in ``route``.
     The adapters are held in bf16 as the kernels read them, A [slots, rank, in] and B [slots,
-    out, rank].  For serving: there is no gradient."""
+    out, rank].  For serving: inputs that require a gradient are refused."""
 
     def __init__(self, base_layer: Linear4bit, slots: int, rank: int, route: AdapterRoute) -> None:
         super().__init__()
@@ -175,6 +175,11 @@ class MultiLoRALinear(nn.Module):
         self.lora_B[slot].zero_()
         self.scaling[slot] = 0.0
 
+    def refuse_gradient(self, *inputs: Optional[torch.Tensor]) -> None:
+        """Raises where an input's gradient would be lost (before the passes' no_grad hides it)."""
+        if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs):
+            ops._serving_only("MultiLoRALinear")
+
     @torch.no_grad()
     def add_adapters(self, x2: torch.Tensor, y2: torch.Tensor) -> torch.Tensor:
         """y2 [tokens, out] (bf16, written over) plus the adapters of x2 [tokens, in]."""
@@ -183,11 +188,12 @@ class MultiLoRALinear(nn.Module):
             return y2
         return ops.multi_lora(x2, self.lora_A, self.lora_B, self.scaling, route.adapter, y2, q_start=route.q_start, out=y2)
 
-    @torch.no_grad()
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        y = self.base_layer(x, residual=residual)
-        y2 = self.add_adapters(ops._bf16_2d(x, self.in_features), ops._bf16_2d(y, self.out_features))
-        return y2.view(y.shape).to(y.dtype)
+        self.refuse_gradient(x, residual)
+        with torch.no_grad():
+            y = self.base_layer(x, residual=residual)
+            y2 = self.add_adapters(ops._bf16_2d(x, self.in_features), ops._bf16_2d(y, self.out_features))
+            return y2.view(y.shape).to(y.dtype)
 
     def extra_repr(self) -> str:
         return f"slots={self.slots}, rank={self.rank}"

@@ -281,17 +281,20 @@ def projection_job(mod: nn.Module, y_add: Optional[torch.Tensor] = None):
     raise TypeError(f"projection_job: not an NF4 projection: {type(mod).__name__}")
 
 
-@torch.no_grad()
 def grouped_forward(mods: Sequence[nn.Module], x: torch.Tensor) -> List[torch.Tensor]:
     """The outputs of up to three projections of the same x in one
     fitq_nf4_gemv_grouped call (no autograd; x.shape[:-1] flattens to M <= 64).
     Same results as calling each module, which the HF layer does one by one
     (fitllm/forward.py:680-686)."""
+    for m in mods:
+        if hasattr(m, "refuse_gradient"):
+            m.refuse_gradient(x)
     lead, k = x.shape[:-1], x.shape[-1]
-    x2 = ops._bf16_2d(x, k)
-    ys = ops.nf4_gemv_grouped(x2, [projection_job(m) for m in mods])
-    ys = [m.add_adapters(x2, y) if hasattr(m, "add_adapters") else y for m, y in zip(mods, ys)]
-    return [y.view(*lead, y.shape[-1]) for y in ys]
+    with torch.no_grad():
+        x2 = ops._bf16_2d(x, k)
+        ys = ops.nf4_gemv_grouped(x2, [projection_job(m) for m in mods])
+        ys = [m.add_adapters(x2, y) if hasattr(m, "add_adapters") else y for m, y in zip(mods, ys)]
+        return [y.view(*lead, y.shape[-1]) for y in ys]
 
 
 @torch.no_grad()

@@ -1,0 +1,54 @@
+"""Wrapped projections with adapters of many requests: what they refuse, with stand-ins for
+the kernels (no GPU needed)."""
+import pytest
+import torch
+
+from fitllm_b200 import ops, qlora
+from fitllm_b200.lora import AdapterRoute, MultiLoRALinear
+from fitllm_b200.qlora import Linear4bit, grouped_forward
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Kernels that return zeros and note the adapters' calls."""
+    seen = []
+
+    def multi_lora(x, a, b, scale, adapter, y, q_start=None, out=None):
+        seen.append((tuple(x.shape), adapter, q_start))
+        return y if out is None else out
+
+    def base(self, x, residual=None):
+        y = x.new_zeros(*x.shape[:-1], self.out_features)
+        return y if residual is None else y + residual
+
+    monkeypatch.setattr(ops, "multi_lora", multi_lora)
+    monkeypatch.setattr(Linear4bit, "forward", base)
+    monkeypatch.setattr(Linear4bit, "wref", lambda self: None)
+    monkeypatch.setattr(ops, "nf4_gemv_grouped", lambda x2, jobs: [x2.new_zeros(x2.shape[0], 64) for _ in jobs])
+    return seen
+
+
+def _wrapped(batch):
+    route = AdapterRoute()
+    route.adapter = None if batch is None else torch.zeros(batch, dtype=torch.int32)
+    return MultiLoRALinear(Linear4bit(64, 64), 2, 16, route)
+
+
+@pytest.mark.parametrize("batch", [None, 3])
+def test_inputs_that_require_a_gradient_are_refused(calls, batch):
+    mod = _wrapped(batch)
+    x, h = torch.zeros(3, 5, 64, dtype=torch.bfloat16), torch.zeros(3, 5, 64, dtype=torch.bfloat16)
+    plain = mod(x, residual=h)
+    assert plain.shape == (3, 5, 64) and len(calls) == (batch is not None)
+    for args in ((x.clone().requires_grad_(), None), (x, h.clone().requires_grad_())):
+        with pytest.raises(NotImplementedError, match="gradient"):
+            mod(args[0], residual=args[1])
+        with torch.no_grad():
+            assert mod(args[0], residual=args[1]).shape == plain.shape
+    live = x.clone().requires_grad_()
+    with pytest.raises(NotImplementedError, match="gradient"):
+        grouped_forward([mod, Linear4bit(64, 64)], live)
+    with torch.no_grad():
+        assert [y.shape for y in grouped_forward([mod, Linear4bit(64, 64)], live)] == [plain.shape] * 2
+    # projections without adapters keep their own rule
+    assert not grouped_forward([Linear4bit(64, 64)], live)[0].requires_grad
