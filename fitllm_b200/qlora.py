@@ -276,8 +276,6 @@ def projection_job(mod: nn.Module, y_add: Optional[torch.Tensor] = None):
                 float(mod.scaling[a]), mod.base_layer.bias, y_add)
     if isinstance(mod, Linear4bit):
         return (mod.wref(), None, None, 1.0, mod.bias, y_add)
-    if hasattr(mod, "add_adapters"):  # the shared projection; grouped_forward adds the requests' adapters
-        return projection_job(mod.base_layer, y_add)
     raise TypeError(f"projection_job: not an NF4 projection: {type(mod).__name__}")
 
 
@@ -292,7 +290,8 @@ def grouped_forward(mods: Sequence[nn.Module], x: torch.Tensor) -> List[torch.Te
     lead, k = x.shape[:-1], x.shape[-1]
     with torch.no_grad():
         x2 = ops._bf16_2d(x, k)
-        ys = ops.nf4_gemv_grouped(x2, [projection_job(m) for m in mods])
+        # of a projection with adapters of many requests the shared part, which they are then added to
+        ys = ops.nf4_gemv_grouped(x2, [projection_job(m.base_layer if hasattr(m, "add_adapters") else m) for m in mods])
         ys = [m.add_adapters(x2, y) if hasattr(m, "add_adapters") else y for m, y in zip(mods, ys)]
         return [y.view(*lead, y.shape[-1]) for y in ys]
 

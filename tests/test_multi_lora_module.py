@@ -52,3 +52,17 @@ def test_inputs_that_require_a_gradient_are_refused(calls, batch):
         assert [y.shape for y in grouped_forward([mod, Linear4bit(64, 64)], live)] == [plain.shape] * 2
     # projections without adapters keep their own rule
     assert not grouped_forward([Linear4bit(64, 64)], live)[0].requires_grad
+
+
+def test_no_call_takes_the_base_for_the_whole(calls, monkeypatch):
+    """A call that does not add the adapters refuses a wrapped projection."""
+    monkeypatch.setattr(ops, "nf4_gemv_swiglu", lambda x2, gate, up: x2.new_zeros(x2.shape[0], 64))
+    mod, plain, x = _wrapped(3), Linear4bit(64, 64), torch.zeros(3, 1, 64, dtype=torch.bfloat16)
+    for pair in ((mod, plain), (plain, mod)):
+        with pytest.raises(TypeError, match="MultiLoRALinear"):
+            qlora.swiglu_forward(*pair, x)
+    with pytest.raises(TypeError, match="MultiLoRALinear"):
+        qlora.projection_job(mod)
+    assert qlora.swiglu_forward(plain, plain, x).shape == (3, 1, 64)
+    grouped_forward([mod, plain, mod], x)
+    assert len(calls) == 2  # the adapters of both wrapped ones
