@@ -18,7 +18,8 @@ batch takes its own (``MultiLoRALinear``, ops.multi_lora).
 from __future__ import annotations
 
 import logging
-from typing import Dict, Iterator, List, Optional, Tuple
+import math
+from typing import Dict, Iterator, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
@@ -119,12 +120,24 @@ class LoRAManager:
 
 class AdapterRoute:
     """Which adapter slot each sequence of the running batch uses: ``adapter`` int32 [batch]
-    (-1: none) and ``q_start`` int32 [batch + 1] of packed tokens, or None where every
-    sequence has as many.  Shared by the layers of a MultiLoRAManager."""
+    (-1: none) and ``q_start`` int32 [batch + 1] of packed tokens (``tokens`` rows of them in a
+    pass), or None where every sequence has as many.  Shared by the layers of a MultiLoRAManager."""
 
     def __init__(self) -> None:
         self.adapter: Optional[torch.Tensor] = None
         self.q_start: Optional[torch.Tensor] = None
+        self.tokens: Optional[int] = None
+
+    def check(self, lead: Sequence[int]) -> None:
+        """Raises where a pass over x [*lead, in] is not of the routed sequences (host values only)."""
+        if self.adapter is None:
+            return
+        if self.q_start is None:
+            if not lead or lead[0] != self.adapter.shape[0]:
+                raise ValueError(f"route: {self.adapter.shape[0]} sequences, the pass has {list(lead)} rows "
+                                 "(the first dimension is the batch; packed tokens need q_start)")
+        elif self.tokens is not None and math.prod(lead) != self.tokens:
+            raise ValueError(f"route: {self.tokens} packed tokens, the pass has {list(lead)} rows")
 
 
 class MultiLoRALinear(nn.Module):
@@ -182,7 +195,8 @@ class MultiLoRALinear(nn.Module):
 
     @torch.no_grad()
     def add_adapters(self, x2: torch.Tensor, y2: torch.Tensor) -> torch.Tensor:
-        """y2 [tokens, out] (bf16, written over) plus the adapters of x2 [tokens, in]."""
+        """y2 [tokens, out] (bf16, written over) plus the adapters of x2 [tokens, in], rows of a
+        pass that ``route.check`` has seen."""
         route = self.route
         if route.adapter is None:
             return y2
@@ -190,6 +204,7 @@ class MultiLoRALinear(nn.Module):
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         self.refuse_gradient(x, residual)
+        self.route.check(x.shape[:-1])
         with torch.no_grad():
             y = self.base_layer(x, residual=residual)
             y2 = self.add_adapters(ops._bf16_2d(x, self.in_features), ops._bf16_2d(y, self.out_features))
@@ -255,8 +270,18 @@ class MultiLoRAManager:
         for layer in self.layers.values():
             layer.unload(slot)
 
-    def route(self, adapter: Optional[torch.Tensor], q_start: Optional[torch.Tensor] = None) -> None:
-        """adapter int32 [batch] slots on the model's device (-1: none), or None: no adapters."""
+    def route(self, adapter: Optional[torch.Tensor], q_start: Optional[torch.Tensor] = None,
+              tokens: Optional[int] = None) -> None:
+        """adapter int32 [batch] slots on the model's device (-1: none), or None: no adapters.  The
+        passes that follow are over [batch, T, hidden] or, with q_start int32 [batch + 1], over
+        ``tokens`` packed rows; others are refused.  tokens None: as many as q_start[batch] says,
+        which is read from the device (but not while a graph is captured: nothing is compared then)."""
         if adapter is not None and (adapter.dtype != torch.int32 or adapter.dim() != 1):
             raise ValueError("route: adapter must be int32 [batch]")
-        self.routing.adapter, self.routing.q_start = adapter, q_start
+        if q_start is not None and (adapter is None or q_start.dtype != torch.int32 or q_start.shape != (adapter.shape[0] + 1,)):
+            raise ValueError("route: q_start must be int32 [batch + 1] beside adapter [batch]")
+        if tokens is not None and (q_start is None or tokens < 0):
+            raise ValueError("route: tokens counts the rows of packed passes (with q_start)")
+        if q_start is not None and tokens is None and not (q_start.is_cuda and torch.cuda.is_current_stream_capturing()):
+            tokens = int(q_start[-1])
+        self.routing.adapter, self.routing.q_start, self.routing.tokens = adapter, q_start, tokens

@@ -285,8 +285,9 @@ def grouped_forward(mods: Sequence[nn.Module], x: torch.Tensor) -> List[torch.Te
     Same results as calling each module, which the HF layer does one by one
     (fitllm/forward.py:680-686)."""
     for m in mods:
-        if hasattr(m, "refuse_gradient"):
+        if hasattr(m, "add_adapters"):
             m.refuse_gradient(x)
+            m.route.check(x.shape[:-1])
     lead, k = x.shape[:-1], x.shape[-1]
     with torch.no_grad():
         x2 = ops._bf16_2d(x, k)

@@ -66,3 +66,45 @@ def test_no_call_takes_the_base_for_the_whole(calls, monkeypatch):
     assert qlora.swiglu_forward(plain, plain, x).shape == (3, 1, 64)
     grouped_forward([mod, plain, mod], x)
     assert len(calls) == 2  # the adapters of both wrapped ones
+
+
+def test_a_pass_of_another_batch_is_refused(calls, monkeypatch):
+    """A route stays until the next one; a pass that is not of its sequences is no call."""
+    from fitllm_b200.lora import MultiLoRAManager
+    model = torch.nn.Module()
+    model.q_proj = Linear4bit(64, 64)
+    m = MultiLoRAManager(4, 16, ("q_proj",))
+    m.apply(model)
+    mod = model.q_proj
+
+    def run(*lead):
+        x = torch.zeros(*lead, 64, dtype=torch.bfloat16)
+        assert mod(x).shape == (*lead, 64)
+        assert grouped_forward([mod, Linear4bit(64, 64)], x)[0].shape == (*lead, 64)
+
+    def refused(*lead):
+        n, x = len(calls), torch.zeros(*lead, 64, dtype=torch.bfloat16)
+        for call in (lambda: mod(x), lambda: grouped_forward([mod, Linear4bit(64, 64)], x)):
+            with pytest.raises(ValueError, match="route"):
+                call()
+        assert len(calls) == n
+
+    run(1, 8)  # no route: any batch
+    m.route(torch.zeros(4, dtype=torch.int32))
+    run(4, 2), run(4, 1), run(4)
+    for lead in ((1, 8), (2, 4), (8, 1), (8,), (1, 4)):
+        refused(*lead)
+    # packed tokens: as many rows as the route's, told or read from its starts
+    starts = torch.tensor([0, 3, 3, 7], dtype=torch.int32)
+    m.route(torch.zeros(3, dtype=torch.int32), q_start=starts)
+    run(1, 7), run(7)
+    refused(1, 8), refused(3, 7), refused(1, 6)
+    m.route(torch.zeros(3, dtype=torch.int32), q_start=starts, tokens=9)  # two rows of padding
+    run(1, 9)
+    refused(1, 7)
+    m.route(None)
+    run(2, 4)
+    for bad in (dict(q_start=starts[:3]), dict(q_start=starts.long()), dict(q_start=starts, tokens=-1), dict(tokens=7)):
+        with pytest.raises(ValueError, match="route"):
+            m.route(torch.zeros(3, dtype=torch.int32), **bad)
+    run(2, 4)  # and changes nothing
