@@ -26,7 +26,7 @@ and attention reads the codes (fitq_kv4_attention) for single tokens, drafts and
 prompts alike.  ``score_drafts`` turns the pass's hidden states into the drafts'
 log probabilities, the model's alternatives and the number of drafts it accepts.
 
-``TreeKVCache`` is the step for trees of drafted tokens: a bf16 or fp16 cache whose lengths
+``TreeKVCache`` is the step for trees of drafted tokens: a bf16 cache whose lengths
 live on the device.  ``tree_pass`` runs the layers over a tree per sequence (ops.tree_append,
 ops.tree_attention), ``verify_tree`` accepts drafts against the model's probabilities by
 given random numbers, and ``TreeKVCache.keep`` leaves the accepted path in the cache.
@@ -385,7 +385,7 @@ def chain_parents(t: int, device) -> torch.Tensor:
 
 
 class TreeKVCache(KVCache):
-    """A KVCache whose sequences have lengths of their own, on the device (``prefix`` int32
+    """A KVCache (bf16) whose sequences have lengths of their own, on the device (``prefix`` int32
     [B]), for passes over trees of drafted tokens: ``tree_pass`` writes a tree's tokens behind
     the lengths without moving them, ``keep`` accepts a path (no copy to the host: a step of
     both can be captured and replayed).  rope_theta: the layers' rotary base (a pass refuses
@@ -395,6 +395,8 @@ class TreeKVCache(KVCache):
                  dtype=torch.bfloat16, rope_theta: float = 1e6):
         if head_dim not in (64, 128):
             raise ValueError(f"TreeKVCache: head_dim must be 64 or 128 (got {head_dim})")
+        if dtype != torch.bfloat16:  # what the layers' projections give, for prompts and trees alike
+            raise ValueError(f"TreeKVCache: the passes write bf16 (got {dtype})")
         super().__init__(num_layers, batch, kv_heads, head_dim, capacity, device, dtype)
         self.rope_theta = rope_theta
         self.prefix = torch.zeros(batch, dtype=torch.int32, device=device)
