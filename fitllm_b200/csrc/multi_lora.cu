@@ -59,54 +59,73 @@ struct MultiLoraParams {
   int* status;
 };
 
-// Tokens [first, first + count) of slot number s (slots of kSize), and their adapter (-1: none).
+__device__ __forceinline__ int start_of(const MultiLoraParams& p, int64_t b) {
+  const int q = p.q_start[b];
+  return q < 0 ? 0 : q > p.tokens ? static_cast<int>(p.tokens) : q;
+}
+// The last sequence b < p.batch for which before(q_start[b], b) holds, or -1: 32 candidates at a time, every lane the
+// same answer.  Starts are clamped to the tokens; `mine` is the lane's.
+template <typename F>
+__device__ __forceinline__ int64_t last_sequence(const MultiLoraParams& p, int lane, int mine, F before) {
+  if (p.batch <= 32) {
+    const uint32_t no = ~__ballot_sync(0xffffffffu, lane < p.batch && before(mine, lane));
+    return no ? __ffs(no) - 2 : 31;
+  }
+  int64_t lo = 0, hi = p.batch;  // answer + 1 in [lo, hi]
+  while (lo < hi) {
+    const int64_t span = hi - lo, step = (span + 31) / 32;
+    const int64_t at = lo + (lane + 1) * step - 1;  // asks whether the answer lies behind
+    bool yes = false;
+    if (at < hi) {
+      yes = before(start_of(p, at), static_cast<int>(at));
+    }
+    const uint32_t all = __ballot_sync(0xffffffffu, yes);
+    const int n = __ffs(~all) ? __ffs(~all) - 1 : 32;  // leading candidates that say so
+    const int64_t up = lo + (n + 1) * step - 1;
+    lo += n * step;
+    if (n < 32 && up < hi) hi = up;
+    if (lo > hi) lo = hi;
+  }
+  return lo - 1;
+}
+
+// Tokens [first, first + count) of slot number s (slots of kSize), and their adapter (-1: none).  Where starts fall
+// sequences may share tokens: each then belongs to the last sequence that begins at or before it, as the search
+// finds it.  That sequence does not fall as the token rises (a candidate's yes stays one), so that a slot whose first
+// and last tokens are its sequence's own meets no other slot; a slot that has others' is left out.
 template <int kSize>
 __device__ __forceinline__ bool slot_of(const MultiLoraParams& p, int64_t s, int lane, int64_t& first, int& count, int& l,
                                         bool report) {
-  int64_t b, begin, end;
+  int64_t b;
+  bool own = true;
   if (p.q_start == nullptr) {
     const int per = (p.t_new + kSize - 1) / kSize;
     b = s / per;
     if (b >= p.batch) return false;
-    begin = b * p.t_new;
-    end = begin + p.t_new;
-    first = begin + (s - b * per) * kSize;
+    first = b * p.t_new + (s - b * per) * kSize;
+    const int64_t left = (b + 1) * p.t_new - first;
+    count = static_cast<int>(left < kSize ? left : kSize);
+    l = p.adapter[b];
   } else {
-    // the last sequence whose numbers begin at or before s: 32 candidates at a time
-    int64_t lo = 0, hi = p.batch;  // answer + 1 in [lo, hi]; every lane holds the same
-    while (lo < hi) {
-      const int64_t span = hi - lo, step = (span + 31) / 32;
-      const int64_t at = lo + (lane + 1) * step - 1;  // asks whether the answer lies behind
-      bool before = false;
-      if (at < hi) {
-        int64_t q = p.q_start[at];
-        q = q < 0 ? 0 : q > p.tokens ? p.tokens : q;
-        before = q / kSize + at <= s;
-      }
-      const uint32_t yes = __ballot_sync(0xffffffffu, before);
-      const int n = __ffs(~yes) ? __ffs(~yes) - 1 : 32;  // leading candidates that say so
-      const int64_t up = lo + (n + 1) * step - 1;
-      lo += n * step;
-      if (n < 32 && up < hi) hi = up;
-      if (lo > hi) lo = hi;
-    }
-    b = lo - 1;
+    const int mine = lane < p.batch ? start_of(p, lane) : 0;
+    b = last_sequence(p, lane, mine, [&](int q, int at) { return q / kSize + at <= s; });
     if (b < 0) return false;
-    begin = p.q_start[b];
-    end = p.q_start[b + 1];
+    int64_t begin = p.q_start[b], end = p.q_start[b + 1];
     begin = begin < 0 ? 0 : begin;
     end = end > p.tokens ? p.tokens : end;
     if (begin > p.tokens) return false;
     first = begin + (s - (begin / kSize + b)) * kSize;
+    if (first < begin || first >= end) return false;
+    count = static_cast<int>(end - first < kSize ? end - first : kSize);
+    l = p.adapter[b];
+    own = last_sequence(p, lane, mine, [&](int q, int) { return q <= first; }) == b &&
+          last_sequence(p, lane, mine, [&](int q, int) { return q < first + count; }) == b;
   }
-  if (first < begin || first >= end) return false;
-  count = static_cast<int>(end - first < kSize ? end - first : kSize);
-  l = p.adapter[b];
   if (l < -1 || l >= p.adapters) {
     if (report && lane == 0) report_device_error(p.status, FITQ_ERR_ARG);
     l = -1;
   }
-  return true;
+  return own;
 }
 
 template <typename T>
@@ -168,8 +187,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int part = blockIdx.x % p.parts;
   int64_t first;
-  int count, l;
-  if (!slot_of<kSlot>(p, blockIdx.x / p.parts, lane, first, count, l, part == 0 && warp == 0) || l < 0) return;  // the whole cluster
+  int count, l, begin = 0, end = 0;
+  // starts that fall or leave the tokens are recorded: there are as many slots as sequences, or more
+  const bool looks = p.q_start != nullptr && part == 0 && threadIdx.x == kThreads - 1 && blockIdx.x / p.parts < p.batch;
+  if (looks) {
+    begin = p.q_start[blockIdx.x / p.parts];
+    end = p.q_start[blockIdx.x / p.parts + 1];
+  }
+  const bool own = slot_of<kSlot>(p, blockIdx.x / p.parts, lane, first, count, l, part == 0 && warp == 0);
+  if (looks && (begin < 0 || end < begin || end > p.tokens)) report_device_error(p.status, FITQ_ERR_ARG);
+  if (!own || l < 0) return;  // the whole cluster
   const int k0 = part * p.part_cols, k1 = min(p.k, k0 + p.part_cols);
   const T* x = static_cast<const T*>(p.x) + first * p.x_stride;
   const T* a = static_cast<const T*>(p.a) + static_cast<int64_t>(l) * R * p.k;

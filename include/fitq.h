@@ -513,9 +513,10 @@ FITQ_API int fitq_tree_keep(const fitq_tree* tree, void* const* k_caches, void* 
  * adapters padded with zeros); k and n multiples of 8; pointers 16-byte aligned.
  * adapter int32 [batch], -1: none, y = y_add; an entry that names no adapter records
  * FITQ_ERR_ARG and counts as -1.  q_start int32 [batch + 1] as in fitq_kv4, or NULL: tokens /
- * batch each; rows of no sequence are left as they are.  fp32 sums, one rounding of y; x.A^T
- * enters the second product as two numbers of dtype.  Deterministic.  The workspace of sizes
- * that no call takes is 0. */
+ * batch each; rows of no sequence are left as they are.  Starts that fall or lie outside [0, tokens]
+ * record FITQ_ERR_ARG: sequences are clamped to the tokens, and a token that several name is one's
+ * of them or left as it is.  fp32 sums, one rounding of y; x.A^T enters the second product as
+ * two numbers of dtype.  Deterministic.  The workspace of sizes that no call takes is 0. */
 FITQ_API size_t fitq_multi_lora_workspace(int64_t tokens, int64_t k, int64_t n, int rank, int batch);
 FITQ_API int fitq_multi_lora(const void* x, int64_t x_stride, int64_t tokens, int64_t k, int64_t n,
                              const void* a, const void* b, int rank, int adapters,
