@@ -1538,6 +1538,50 @@ int fitq_token_logprobs_bwd(const void* logits, int dtype, const int64_t* ids, i
                        "token_logprobs_bwd");
 }
 
+// Two caches of a tree's layout: their distance, and what its dimensions reach, outermost first.
+struct CacheReach {
+  int dims = 0;
+  int64_t stride[3], count[3], inner[4];  // inner[i]: elements from the first to the last of dimensions i on
+};
+static CacheReach cache_reach(const fitq::TreeView& t, int dim) {
+  CacheReach r;
+  const int64_t strides[3] = {t.stride_b, t.stride_h, t.stride_p}, counts[3] = {t.batch, t.kv_heads, t.capacity};
+  for (int i = 0; i < 3; ++i) {
+    if (counts[i] == 1) continue;
+    int at = r.dims++;
+    for (; at > 0 && r.stride[at - 1] < strides[i]; --at) {
+      r.stride[at] = r.stride[at - 1];
+      r.count[at] = r.count[at - 1];
+    }
+    r.stride[at] = strides[i];
+    r.count[at] = counts[i];
+  }
+  r.inner[r.dims] = dim;
+  constexpr int64_t kFar = 1ll << 60;  // behind every address
+  for (int i = r.dims - 1; i >= 0; --i)
+    r.inner[i] = r.count[i] - 1 > kFar / r.stride[i] ? kFar : std::min(kFar, r.inner[i + 1] + (r.count[i] - 1) * r.stride[i]);
+  return r;
+}
+// Whether they share an element, `delta` elements apart: some step along dimension i leaves less than its inner
+// dimensions reach.  Of nested dimensions two steps do at most; where more than 64 do (a cache over itself) the
+// answer is yes.
+static bool caches_meet(const CacheReach& r, int64_t delta, int i = 0) {
+  if (delta < 0) delta = -delta;
+  if (delta >= r.inner[i]) return false;
+  if (i == r.dims) return true;
+  const int64_t s = r.stride[i], reach = r.inner[i + 1] - 1;
+  int64_t lo = delta > reach ? (delta - reach + s - 1) / s : -((reach - delta) / s), hi = (delta + reach) / s;
+  lo = std::max(lo, 1 - r.count[i]);
+  hi = std::min(hi, r.count[i] - 1);
+  if (hi - lo > 64) return true;
+  for (int64_t d = lo; d <= hi; ++d)
+    if (caches_meet(r, delta - d * s, i + 1)) return true;
+  return false;
+}
+static int64_t elements_between(const void* a, const void* b) {
+  return (static_cast<int64_t>(reinterpret_cast<uintptr_t>(b)) - static_cast<int64_t>(reinterpret_cast<uintptr_t>(a))) / 2;
+}
+
 // Shape checks shared by the calls on a tree of drafted tokens; fills the kernels' addressing.
 static int tree_view(const char* what, const fitq_tree* t, int heads, fitq::TreeView* out) {
   if (!t || !t->parents || !t->prefix) return fail(FITQ_ERR_ARG, "%s: NULL tree, parents or prefix", what);
@@ -1586,7 +1630,8 @@ int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_stride, con
   if ((q_out != q && kv4_meets(q_out, n * row * 2, q, n, q_stride, row)) ||
       kv4_meets(q_out, n * row * 2, k, n, k_stride, kv_row) || kv4_meets(q_out, n * row * 2, v, n, v_stride, kv_row))
     return fail(FITQ_ERR_ARG, "tree_append: q_out overlaps q (other than being q), k or v");
-  if (k_cache == v_cache) return fail(FITQ_ERR_ARG, "tree_append: keys and values in one cache");
+  if (caches_meet(cache_reach(t, tree->head_dim), elements_between(k_cache, v_cache)))
+    return fail(FITQ_ERR_ARG, "tree_append: keys and values in one cache, or in caches that overlap");
   if (!current_sms(&rc)) return rc;
   return launch_status(fitq::launch_tree_append(t, q, q_stride, k, k_stride, v, v_stride, q_out, k_cache, v_cache,
                                                 cos_half, sin_half, rope_len, heads, tree->head_dim, tree->dtype,
@@ -1680,8 +1725,11 @@ int fitq_tree_keep(const fitq_tree* tree, void* const* k_caches, void* const* v_
   std::vector<const void*> all(k_caches, k_caches + layers);  // each moves once
   all.insert(all.end(), v_caches, v_caches + layers);
   std::sort(all.begin(), all.end());
-  if (std::adjacent_find(all.begin(), all.end()) != all.end())
-    return fail(FITQ_ERR_ARG, "tree_keep: a cache is given twice");
+  const CacheReach reach = cache_reach(t, tree->head_dim);
+  for (size_t i = 0; i < all.size(); ++i)
+    for (size_t j = i + 1; j < all.size() && elements_between(all[i], all[j]) < reach.inner[0]; ++j)
+      if (caches_meet(reach, elements_between(all[i], all[j])))
+        return fail(FITQ_ERR_ARG, "tree_keep: a cache is given twice, or caches overlap");
   if ((reinterpret_cast<uintptr_t>(accepted) & 7u) ||
       ((reinterpret_cast<uintptr_t>(path) | reinterpret_cast<uintptr_t>(lengths)) & 3u))
     return fail(FITQ_ERR_ALIGN, "tree_keep: tensors must be aligned to their elements");

@@ -456,7 +456,8 @@ typedef struct fitq_tree {
  * [batch * tokens, heads, head_dim], k, v [batch * tokens, kv_heads, head_dim]; *_stride:
  * elements from token to token, a multiple of 8.  Absent tokens' queries are zeros, their
  * slots stay as they are.  q_out may be q when q_stride == heads * head_dim, and overlaps none
- * of the inputs otherwise. */
+ * of the inputs otherwise; k_cache and v_cache may lie between one another's heads, but share
+ * no element. */
 FITQ_API int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_stride, const void* k,
                               int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
                               void* k_cache, void* v_cache, const float* cos_half,
@@ -495,8 +496,8 @@ FITQ_API int fitq_tree_verify(const void* logits, int dtype, int64_t stride_b, i
                               const float* temperatures, float temperature, int32_t* path,
                               int64_t* accepted, int64_t* next_token, fitq_stream_t stream);
 /* The accepted path stays: slot prefix + path[i] moves to slot prefix + i for
- * i <= accepted in every layer (k_caches, v_caches: host arrays of `layers` device pointers, no
- * cache twice),
+ * i <= accepted in every layer (k_caches, v_caches: host arrays of `layers` device pointers, of
+ * caches that share no element),
  * lengths[b] = prefix[b] + accepted[b] + 1 (lengths may be prefix).  path, accepted as
  * fitq_tree_verify writes them; a path that does not ascend within the tree and the capacity
  * records FITQ_ERR_ARG and leaves its sequence as it was. */
