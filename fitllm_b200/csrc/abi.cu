@@ -1578,8 +1578,23 @@ static bool caches_meet(const CacheReach& r, int64_t delta, int i = 0) {
     if (caches_meet(r, delta - d * s, i + 1)) return true;
   return false;
 }
+// Whether elements [lo, hi) from a cache's first on hold one of its own.
+static bool block_meets(const CacheReach& r, int64_t lo, int64_t hi, int i = 0) {
+  if (hi <= 0 || lo >= r.inner[i]) return false;
+  if (i == r.dims) return true;
+  const int64_t s = r.stride[i], behind = lo - r.inner[i + 1] + 1;  // a step whose inner dimensions end before lo is none
+  const int64_t first = behind > 0 ? (behind + s - 1) / s : 0, last = std::min((hi - 1) / s, r.count[i] - 1);
+  if (last - first > 64) return true;
+  for (int64_t d = first; d <= last; ++d)
+    if (block_meets(r, lo - d * s, hi - d * s, i + 1)) return true;
+  return false;
+}
 static int64_t elements_between(const void* a, const void* b) {
   return (static_cast<int64_t>(reinterpret_cast<uintptr_t>(b)) - static_cast<int64_t>(reinterpret_cast<uintptr_t>(a))) / 2;
+}
+static bool result_in_cache(const CacheReach& r, const void* out, int64_t elements, const void* cache) {
+  const int64_t at = elements_between(cache, out);
+  return block_meets(r, at, at + elements);
 }
 
 // Shape checks shared by the calls on a tree of drafted tokens; fills the kernels' addressing.
@@ -1630,7 +1645,10 @@ int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_stride, con
   if ((q_out != q && kv4_meets(q_out, n * row * 2, q, n, q_stride, row)) ||
       kv4_meets(q_out, n * row * 2, k, n, k_stride, kv_row) || kv4_meets(q_out, n * row * 2, v, n, v_stride, kv_row))
     return fail(FITQ_ERR_ARG, "tree_append: q_out overlaps q (other than being q), k or v");
-  if (caches_meet(cache_reach(t, tree->head_dim), elements_between(k_cache, v_cache)))
+  const CacheReach reach = cache_reach(t, tree->head_dim);
+  if (q_out != q && (result_in_cache(reach, q_out, n * row, k_cache) || result_in_cache(reach, q_out, n * row, v_cache)))
+    return fail(FITQ_ERR_ARG, "tree_append: q_out overlaps a cache");
+  if (caches_meet(reach, elements_between(k_cache, v_cache)))
     return fail(FITQ_ERR_ARG, "tree_append: keys and values in one cache, or in caches that overlap");
   if (!current_sms(&rc)) return rc;
   return launch_status(fitq::launch_tree_append(t, q, q_stride, k, k_stride, v, v_stride, q_out, k_cache, v_cache,
@@ -1667,6 +1685,9 @@ int fitq_tree_attention(const fitq_tree* tree, const void* q, int64_t q_stride, 
     return fail(FITQ_ERR_ALIGN, "tree_attention: 16-byte alignment");
   if (!(out == q && q_stride == row) && kv4_meets(out, n * row * 2, q, n, q_stride, row))
     return fail(FITQ_ERR_ARG, "tree_attention: out overlaps q, other than being q of dense tokens");
+  const CacheReach reach = cache_reach(t, tree->head_dim);
+  if (out != q && (result_in_cache(reach, out, n * row, k_cache) || result_in_cache(reach, out, n * row, v_cache)))
+    return fail(FITQ_ERR_ARG, "tree_attention: out overlaps a cache");
   const int sms = current_sms(&rc);
   if (!sms) return rc;
   const size_t need = fitq::tree_attention_workspace(t, heads, tree->head_dim, sms);

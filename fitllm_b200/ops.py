@@ -458,6 +458,36 @@ def _tree_tokens(what: str, name: str, x: torch.Tensor, heads: Optional[int], c:
     return x, s1
 
 
+def _holds(x: torch.Tensor, lo: int, hi: int) -> bool:
+    """Whether bytes [lo, hi) from a tensor's first element on hold one of its own."""
+    size = x.element_size()
+    dims = sorted(((s * size, n) for n, s in zip(x.shape, x.stride()) if n > 1), reverse=True)
+    inner = [size]
+    for s, n in reversed(dims):
+        inner.append(inner[-1] + (n - 1) * s)
+    inner.reverse()
+
+    def meets(lo, hi, i):
+        if hi <= 0 or lo >= inner[i]:
+            return False
+        if i == len(dims):
+            return True
+        s, n = dims[i]
+        first, last = max(0, -(-(lo - inner[i + 1] + 1) // s)), min((hi - 1) // s, n - 1)
+        return last - first > 64 or any(meets(lo - d * s, hi - d * s, i + 1) for d in range(first, last + 1))
+
+    return meets(lo, hi, 0)
+
+
+def _result_beside(what: str, name: str, out: torch.Tensor, *inputs: torch.Tensor) -> None:
+    """Raises where a contiguous result lies over an input that other rows still read."""
+    nbytes = out.numel() * out.element_size()
+    for x in inputs:
+        at = out.data_ptr() - x.data_ptr()
+        if _holds(x, at, at + nbytes):
+            raise ValueError(f"{what}: {name} overlaps an input")
+
+
 def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 prefix: torch.Tensor, parents: torch.Tensor, cos_half: torch.Tensor, sin_half: torch.Tensor,
                 q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -486,6 +516,8 @@ def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
             or (cos_half.data_ptr() | sin_half.data_ptr()) % 16:
         raise ValueError(f"tree_append: cos_half and sin_half must be contiguous, 16-byte aligned fp32 on {dev}")
     out = q.new_empty(q.shape) if q_out is None else _kv4_out("tree_append", "q_out", q_out, q)
+    if q_out is not None:
+        _result_beside("tree_append", "q_out", out, k_cache, v_cache)
     with _on(dev):
         _lib.check(L.fitq_tree_append(c, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
                                       k_cache.data_ptr(), v_cache.data_ptr(), cos_half.data_ptr(), sin_half.data_ptr(), rows[0], q.shape[2],
@@ -507,7 +539,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     c = _tree_cache("tree_attention", k_cache, v_cache, prefix, parents, q.shape[1] if q.dim() == 4 else 0)
     dev = k_cache.device
     q, qs = _tree_tokens("tree_attention", "q", q, None, c, k_cache)
-    out = q.new_empty(q.shape) if out is None else _kv4_out("tree_attention", "out", out, q)
+    if out is None:
+        out = q.new_empty(q.shape)
+    else:
+        _result_beside("tree_attention", "out", _kv4_out("tree_attention", "out", out, q), k_cache, v_cache)
     heads = q.shape[2]
     with _on(dev):
         nbytes = _tree_attention_workspace(c.capacity, c.batch, c.tokens, c.kv_heads, c.head_dim, heads, dev.index)

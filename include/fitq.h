@@ -456,8 +456,8 @@ typedef struct fitq_tree {
  * [batch * tokens, heads, head_dim], k, v [batch * tokens, kv_heads, head_dim]; *_stride:
  * elements from token to token, a multiple of 8.  Absent tokens' queries are zeros, their
  * slots stay as they are.  q_out may be q when q_stride == heads * head_dim, and overlaps none
- * of the inputs otherwise; k_cache and v_cache may lie between one another's heads, but share
- * no element. */
+ * of the inputs and neither cache otherwise; k_cache and v_cache may lie between one another's
+ * heads, but share no element. */
 FITQ_API int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_stride, const void* k,
                               int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
                               void* k_cache, void* v_cache, const float* cos_half,
@@ -467,7 +467,8 @@ FITQ_API int fitq_tree_append(const fitq_tree* tree, const void* q, int64_t q_st
  * h / (heads / kv_heads); scale 1/sqrt(head_dim), fp32 softmax and sums.  An absent token
  * gives zeros, as does one whose scores are all -inf.  Slots that no token sees are not read into any
  * sum, whatever they hold.  The weights enter the second product rounded to dtype (their sum does not).
- * Deterministic.  out may be q as above.  The workspace of sizes that no call takes is 0. */
+ * Deterministic.  out may be q, and overlaps no cache, as above.  The workspace of sizes that
+ * no call takes is 0. */
 FITQ_API size_t fitq_tree_attention_workspace(const fitq_tree* tree, int heads);
 FITQ_API int fitq_tree_attention(const fitq_tree* tree, const void* q, int64_t q_stride,
                                  const void* k_cache, const void* v_cache, void* out, int heads,

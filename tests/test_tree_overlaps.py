@@ -92,3 +92,52 @@ def test_the_largest_strides(L):
     # sequences, heads and slots that lie over one another: such a cache shares elements with any beside it
     c = _tree(batch=65535, heads=2, cap=1 << 30, strides=(big, big, big))
     assert _append(L, c, FAR, FAR + 64 * 2) == ARG
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are nothing's")
+def test_results_over_the_caches(L):
+    c = _tree()  # 3 x 2 x 20 slots of 64 elements: 15,360 bytes; 4 tokens of two heads each: 3,072 bytes
+    caches, row, size, out = (FAR + (1 << 24), FAR + (2 << 24)), 128, 3 * 2 * 20 * 64 * 2, 3 * 4 * 128 * 2
+
+    def attend(at):
+        return L.fitq_tree_attention(c, FAR, row, caches[0], caches[1], at, 2, P, 1 << 40, None)
+
+    for call in (attend, lambda at: _append(L, c, *caches, out=at)):
+        for cache in caches:
+            for at in (cache - out + 16, cache, cache + 4096, cache + size - 16):
+                assert call(at) == ARG
+            assert _good(call(cache - out)) and _good(call(cache + size))
+
+
+def test_results_in_place_over_the_caches(monkeypatch):
+    """The wrappers look at results that are q, too."""
+    from fitllm_b200 import ops
+    from fitllm_b200.ops import _result_beside
+    store = torch.zeros(3, 2, 20, 64, dtype=torch.bfloat16)
+    k, v = store, torch.zeros_like(store)
+    inside, beside = store.view(-1)[:1536].view(3, 4, 2, 64), torch.zeros(3, 4, 2, 64, dtype=torch.bfloat16)
+    for caches in ((k, v), (v, k)):
+        with pytest.raises(ValueError, match="overlaps"):
+            _result_beside("tree_attention", "out", inside, *caches)
+        _result_beside("tree_attention", "out", beside, *caches)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are nothing's")
+@pytest.mark.parametrize("batch,heads,cap,strides", LAYOUTS)
+def test_results_between_the_caches_parts(L, batch, heads, cap, strides):
+    """By counting every element: results that share one with a cache are refused, others are not."""
+    from fitllm_b200.ops import _holds
+    c = _tree(batch, heads, cap, strides, tokens=1)
+    pieces = {sum(i * s for i, s in zip(at, strides)) // 8 + y for at in itertools.product(range(batch), range(heads), range(cap))
+              for y in range(8)}  # of eight elements
+    n, base = batch * heads * 64, FAR + (1 << 24)
+    view = torch.empty(8 * max(pieces) + 8, dtype=torch.bfloat16).as_strided((batch, heads, cap, 64), (*strides, 1))
+    tried = {False: 0, True: 0}
+    for off in range(-n - 16, 8 * max(pieces) + 32, 8):
+        meets = any(off // 8 + i in pieces for i in range(n // 8))
+        for caches in ((base, FAR << 1), (FAR << 1, base)):
+            assert (L.fitq_tree_attention(c, FAR, heads * 64, *caches, base + 2 * off, heads, P, 1 << 40, None) == ARG) == meets, off
+            assert (_append(L, c, *caches, out=base + 2 * off) == ARG) == meets, off
+        assert _holds(view, 2 * off, 2 * (off + n)) == meets, off
+        tried[meets] += 1
+    assert tried[True] and tried[False]
