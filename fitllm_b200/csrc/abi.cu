@@ -1796,6 +1796,10 @@ int fitq_multi_lora(const void* x, int64_t x_stride, int64_t tokens, int64_t k, 
   if (!(y == y_add && y_add_stride == n) && kv4_meets(y, tokens * n * 2, y_add, tokens, y_add_stride, n))
     return fail(FITQ_ERR_ARG, "multi_lora: y overlaps y_add, other than being y_add of dense rows");
   if (kv4_meets(y, tokens * n * 2, x, tokens, x_stride, k)) return fail(FITQ_ERR_ARG, "multi_lora: y overlaps x");
+  auto over = [&](const void* p, int64_t bytes) { return p && kv4_meets(y, tokens * n * 2, p, 1, 0, (bytes + 1) / 2); };
+  if (over(a, 2ll * adapters * rank * k) || over(b, 2ll * adapters * rank * n) || over(scale, 4ll * adapters) ||
+      over(adapter, 4ll * batch) || over(q_start, 4ll * batch + 4) || over(workspace, 4ll * tokens * rank))
+    return fail(FITQ_ERR_ARG, "multi_lora: y overlaps the adapters, their route or the workspace");
   int rc;
   const int sms = current_sms(&rc);
   if (!sms) return rc;

@@ -510,9 +510,10 @@ FITQ_API int fitq_tree_keep(const fitq_tree* tree, void* const* k_caches, void* 
  * PEFT's lora.Linear4bit adds for one adapter, fitllm/qlora.py:74-83):
  *   y[n] = y_add[n] + scale[l] (x[n].A_l^T).B_l^T,  l = adapter[sequence of token n].
  * x [tokens, k], y_add [tokens, n] of dtype (bf16 or fp16), *_stride elements from token to
- * token; y [tokens, n], which may be y_add (y_add_stride == n); a [adapters, rank, k], b
- * [adapters, n, rank] of dtype, scale fp32 [adapters]; rank 16, 32, 48 or 64 (smaller
- * adapters padded with zeros); k and n multiples of 8; pointers 16-byte aligned.
+ * token; y [tokens, n], which may be y_add (y_add_stride == n) and overlaps nothing else;
+ * a [adapters, rank, k], b [adapters, n, rank] of dtype, scale fp32 [adapters]; rank 16, 32,
+ * 48 or 64 (smaller adapters padded with zeros); k and n multiples of 8; pointers 16-byte
+ * aligned.
  * adapter int32 [batch], -1: none, y = y_add; an entry that names no adapter records
  * FITQ_ERR_ARG and counts as -1.  q_start int32 [batch + 1] as in fitq_kv4, or NULL: tokens /
  * batch each; rows of no sequence are left as they are.  Starts that fall or lie outside [0, tokens]

@@ -141,3 +141,26 @@ def test_results_between_the_caches_parts(L, batch, heads, cap, strides):
         assert _holds(view, 2 * off, 2 * (off + n)) == meets, off
         tried[meets] += 1
     assert tried[True] and tried[False]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are nothing's")
+@pytest.mark.parametrize("start", [None, FAR + (6 << 24)])
+def test_results_over_the_adapters(L, start):
+    tokens, k, n, r, adapters, batch = 6, 256, 128, 16, 2, 3
+    at = {name: FAR + (i << 24) for i, name in enumerate(("x", "a", "b", "scale", "adapter", "ws"))}
+    sizes = dict(a=adapters * r * k * 2, b=adapters * n * r * 2, scale=adapters * 4, adapter=batch * 4, ws=tokens * r * 4)
+    if start is not None:
+        at["q_start"], sizes["q_start"] = start, (batch + 1) * 4
+    y = FAR + (8 << 24)
+
+    def call(out, add=y):
+        return L.fitq_multi_lora(at["x"], k, tokens, k, n, at["a"], at["b"], r, adapters, at["scale"], at["adapter"], start, batch,
+                                 add, n, out, 0, at["ws"], sizes["ws"], None)
+
+    size = tokens * n * 2
+    assert _good(call(y)) and _good(call(y + size))
+    for name, nbytes in sizes.items():
+        first, last = at[name] // 16 * 16, (at[name] + nbytes - 1) // 16 * 16
+        for out in (first - size + 16, first, last):
+            assert call(out) == ARG and call(out, add=out) == ARG, name
+        assert _good(call(first - size)) and _good(call(last + 16)), name
