@@ -23,6 +23,7 @@ from typing import Dict, Iterator, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import ops
 from .qlora import Linear4bit, _QLoRAFunction
@@ -189,9 +190,11 @@ class MultiLoRALinear(nn.Module):
         self.scaling[slot] = 0.0
 
     def refuse_gradient(self, *inputs: Optional[torch.Tensor]) -> None:
-        """Raises where an input's gradient would be lost (before the passes' no_grad hides it)."""
+        """Raises where an input's gradient or tangent would be lost (before the passes' no_grad hides it)."""
         if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs):
             ops._serving_only("MultiLoRALinear")
+        if forward_ad._current_level >= 0:
+            ops._refuse_tangents("MultiLoRALinear", *inputs)
 
     @torch.no_grad()
     def add_adapters(self, x2: torch.Tensor, y2: torch.Tensor) -> torch.Tensor:

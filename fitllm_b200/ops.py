@@ -10,6 +10,7 @@ import functools
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .nf4 import Nf4WeightCRef, QuantState
@@ -386,6 +387,12 @@ def _serving_only(what: str) -> None:
                               "(use torch.no_grad())")
 
 
+def _refuse_tangents(what: str, *inputs: Optional[torch.Tensor]) -> None:
+    """Refuses, inside a forward_ad.dual_level, inputs whose tangent a call would lose."""
+    if any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in inputs):
+        raise NotImplementedError(f"{what}: an input carries a tangent (there is no forward-mode derivative)")
+
+
 @functools.lru_cache(maxsize=256)
 def _tree_attention_workspace(cap: int, batch: int, t: int, kv_heads: int, d: int, heads: int, device: int) -> int:
     """fitq_tree_attention_workspace of the sizes, on a device's SMs."""
@@ -503,6 +510,8 @@ def tree_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torc
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_cache.requires_grad
                                     or v_cache.requires_grad):
         _serving_only("tree_append")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("tree_append", q, k, v, k_cache, v_cache)
     c = _tree_cache("tree_append", k_cache, v_cache, prefix, parents, q.shape[1] if q.dim() == 4 else 0)
     dev = k_cache.device
     q, qs = _tree_tokens("tree_append", "q", q, None, c, k_cache)
@@ -536,6 +545,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     L = _lib.load()
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         _serving_only("tree_attention")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("tree_attention", q, k_cache, v_cache)
     c = _tree_cache("tree_attention", k_cache, v_cache, prefix, parents, q.shape[1] if q.dim() == 4 else 0)
     dev = k_cache.device
     q, qs = _tree_tokens("tree_attention", "q", q, None, c, k_cache)
@@ -561,6 +572,10 @@ def tree_keep(k_caches: Sequence[torch.Tensor], v_caches: Sequence[torch.Tensor]
     L = _lib.load()
     if not k_caches or len(k_caches) != len(v_caches):
         raise ValueError(f"tree_keep: {len(k_caches)} key and {len(v_caches)} value caches")
+    if torch.is_grad_enabled() and any(x.requires_grad for x in (*k_caches, *v_caches)):
+        _serving_only("tree_keep")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("tree_keep", *k_caches, *v_caches)
     first = k_caches[0]
     if path.dim() != 2 or path.dtype != torch.int32 or not path.is_contiguous() or path.device != first.device \
             or path.shape[0] != first.shape[0]:
@@ -614,6 +629,8 @@ def multi_lora(x: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, scal
     if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or lora_a.requires_grad or lora_b.requires_grad
                                     or scale.requires_grad):
         _serving_only("multi_lora")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents("multi_lora", x, y, lora_a, lora_b, scale)
     xs, ys, sa, sb = x.shape, y.shape, lora_a.shape, lora_b.shape
     if len(xs) != 2 or len(ys) != 2 or len(sa) != 3 or len(sb) != 3:
         raise ValueError("multi_lora: x and y are [tokens, .], lora_a and lora_b [adapters, ., .]")
