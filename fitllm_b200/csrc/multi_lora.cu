@@ -14,9 +14,9 @@
 // row of x and of A at a time and feeds them to two MMAs (the contraction index is permuted
 // alike in both), so that a single token is summed by 64 warps with every load in flight at
 // once.  More: tcgen05, M = 128 tokens by N = R, x and A through a ring of TMA tiles of 64 columns (a
-// full slot's x is one copy: as four, from one lane, the copies' issue took 172 us where it is 129 now).
-// Parts join in shared memory, then over the cluster, in order (deterministic); T stays
-// in fp32.
+// full slot's x is one copy, as four from one lane are issued too slowly).  Parts join in shared memory, then over
+// the cluster, in order (deterministic); T stays in fp32.  The accumulation in tensor memory rounds towards zero:
+// where one CTA sums all of K = 27,648 the result's error is 1.2% above its own rounding's in fp16, 0.02% in bf16.
 //
 // multi_lora_expand_kernel, y = y_add + s T.B_l^T: T enters as two 16-bit numbers, hi + lo (a
 // relative error of eps^2; one alone would cost the delta half its digits), scaled by a power of
@@ -24,7 +24,8 @@
 // row: y and y_add move in 16-byte pieces.  One rounding, of y.
 //
 // Bound: one token, two launches (5.3 us at K = N = 5,120, rank 16); 64 tokens of as many adapters on 5,120 x
-// 27,648: 23 us, B at 2.9 TB/s, as a CTA waits for its adapter, T and B in turn; six prompts of 4,180
+// 27,648: 23 us, B at 2.9 TB/s, as a CTA waits for its adapter, T and B in turn; one token at K = 27,648, rank 64:
+// 12.4 us, as a slot has eight CTAs at most and they read 3.5 MB of A; six prompts of 4,180
 // tokens on 27,648 x 5,120 at rank 64: 88 us, 50 of them the first kernel's (x at 4.3 TB/s, with A 7 TB/s into
 // the SMs), 33 the second's, whose loads and mma.sync (36% busy) wait for each other.
 #include <type_traits>

@@ -21,7 +21,8 @@
 // over it, and O += P.V takes P from there and V as loaded, position by position (an MN-major
 // operand).  P is rounded to the values' type, which the MMA wants of its operands (relative errors
 // of 2.1e-3 to 2.3e-3 in bf16 where the result's own rounding gives 1.7e-3; 2.9e-4 and 2.1e-4 in fp16);
-// its sum is fp32 of what was not rounded.
+// its sum is fp32 of what was not rounded.  As two numbers of that type, which would leave the result's rounding
+// alone, P would have a second product: 512 more cycles of MMAs in the 2,000 of a tile for two row tiles.
 // With one row tile the units take the tiles in turn, each with sums O, m and l of its own
 // that are joined at the pair's end; with two, a unit is a row tile and both see every tile.
 //
@@ -35,10 +36,11 @@
 // completes on a barrier of warp 10's own, and the slot's is completed by warp 10.
 //
 // Bound: with one row tile the loads (64 sequences of 8 tokens, 40 heads on 8 of 128, over 100 to 8,191
-// positions: 197 us, 5.7 TB/s), and a pair's end, some 3 us that the ring covers in part.  With two the
+// positions: 197 us, 5.7 TB/s, at 1,965 MHz; 232 at the 1,627 MHz that a long run of them is left: its
+// time follows the clock), and a pair's end, some 3 us that the ring covers in part.  With two the
 // chain of a tile: some 2,000 cycles, of which both units' MMAs need 1,280 (48 for one of 32, which waits
 // for Q from shared memory) and the exponentials 1,024 (8 sequences of 32 tokens over 3,500 to 4,099: 50 us;
-// 64 tokens over 131,071 in fp16: 252 us).  Few positions: 14 us for 5 tokens over 1,023.
+// 64 tokens over 131,071 in fp16: 253 us, 298 at 1,605 MHz).  Few positions: 14 us for 5 tokens over 1,023.
 #include <type_traits>
 
 #include "kernels.cuh"

@@ -22,8 +22,10 @@
 // sums.  A refused child costs another read of the row (from L1 and L2) with its q, and without a q a
 // subtraction.
 // Bound: the chain of a visited row (largest 1.1, sum 2.8, exchange 0.8, joining 0.8, a child's test 0.7 us
-// on eight CTAs; 5.4 in all on sixteen), and a batch's deepest path.  A chain of 5 rows of 152,064 tokens: 20 us;
-// 64 of them: 98; 16 trees of 32 tokens over 32,001: 18; one row of each of 64 sequences: 21.
+// on eight CTAs), and a batch's deepest path.  A chain of 5 rows of 152,064 tokens on sixteen CTAs: 28 us where all
+// drafts are accepted, 15 where the first is refused (a row and the row again with its q), 8.9 for a row alone: 4.9 for
+// each further one.  64 such chains: 95 to 99; at temperature 0, which reads a row for its largest logit and again for
+// its index, 56; 16 trees of 32 tokens over 32,001: 19.5; one row of each of 64 sequences: 21.
 #include <mutex>
 #include <type_traits>
 
