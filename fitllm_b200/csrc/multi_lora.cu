@@ -76,12 +76,8 @@ __device__ __forceinline__ int64_t last_sequence(const MultiLoraParams& p, int l
   while (lo < hi) {
     const int64_t span = hi - lo, step = (span + 31) / 32;
     const int64_t at = lo + (lane + 1) * step - 1;  // asks whether the answer lies behind
-    bool yes = false;
-    if (at < hi) {
-      yes = before(start_of(p, at), static_cast<int>(at));
-    }
-    const uint32_t all = __ballot_sync(0xffffffffu, yes);
-    const int n = __ffs(~all) ? __ffs(~all) - 1 : 32;  // leading candidates that say so
+    const uint32_t no = ~__ballot_sync(0xffffffffu, at < hi && before(start_of(p, at), static_cast<int>(at)));
+    const int n = no ? __ffs(no) - 1 : 32;  // leading candidates that say yes
     const int64_t up = lo + (n + 1) * step - 1;
     lo += n * step;
     if (n < 32 && up < hi) hi = up;

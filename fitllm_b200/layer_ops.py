@@ -122,7 +122,8 @@ def rope_kv_append(q, k, v, cos_half, sin_half, k_cache, v_cache, prefix: int, h
     q, k, v = _c(q), _c(k), _c(v)
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("rope_kv_append: caches must be contiguous")
-    if any(x.dtype != torch.bfloat16 for x in (q, k, v, k_cache, v_cache)):  # the kernel reads and writes bf16 bits
+    bf16 = torch.bfloat16  # what the kernel reads and writes
+    if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16 or k_cache.dtype != bf16 or v_cache.dtype != bf16:
         raise ValueError("rope_kv_append: q, k, v and the caches must be bf16")
     out = torch.empty_like(q)
     L = _lib.load()

@@ -96,8 +96,8 @@ def test_the_largest_strides(L):
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are nothing's")
 def test_results_over_the_caches(L):
-    c = _tree()  # 3 x 2 x 20 slots of 64 elements: 15,360 bytes; 4 tokens of two heads each: 3,072 bytes
-    caches, row, size, out = (FAR + (1 << 24), FAR + (2 << 24)), 128, 3 * 2 * 20 * 64 * 2, 3 * 4 * 128 * 2
+    c = _tree(tokens=5)
+    caches, row, size, out = (FAR + (1 << 24), FAR + (2 << 24)), 128, 3 * 2 * 20 * 64 * 2, 3 * 5 * 128 * 2
 
     def attend(at):
         return L.fitq_tree_attention(c, FAR, row, caches[0], caches[1], at, 2, P, 1 << 40, None)
@@ -115,7 +115,7 @@ def test_results_in_place_over_the_caches(monkeypatch):
     from fitllm_b200.ops import _result_beside
     store = torch.zeros(3, 2, 20, 64, dtype=torch.bfloat16)
     k, v = store, torch.zeros_like(store)
-    inside, beside = store.view(-1)[:1536].view(3, 4, 2, 64), torch.zeros(3, 4, 2, 64, dtype=torch.bfloat16)
+    inside, beside = store.view(-1)[:1920].view(3, 5, 2, 64), torch.zeros(3, 5, 2, 64, dtype=torch.bfloat16)
     for caches in ((k, v), (v, k)):
         with pytest.raises(ValueError, match="overlaps"):
             _result_beside("tree_attention", "out", inside, *caches)
